@@ -28,7 +28,7 @@ LIBRARIES = {
     "seq": dict(out=os.path.join(PKG, "libb200seq.so"),
                 sources=["seq_api.cu", "seq_elementwise.cu", "seq_scan.cu", "seq_attention.cu", "seq_latent.cu", "seq_moe.cu", "seq_streams.cu",
                          "seq_depth.cu", "seq_gru.cu", "seq_convrope.cu", "seq_mlstm.cu",
-                         "seq_linear_f32.cu"]),
+                         "seq_linear_f32.cu", "seq_paged.cu", "seq_paged_attn.cu", "seq_paged_tc.cu"]),
 }
 
 

@@ -20,6 +20,7 @@ from .rinirax import Rinirax, RiniraxConfig
 from .lukupel import Lukupel, LukupelConfig
 from .malulorn import Malulorn, MalulornConfig
 from .state import SequenceStatePool, StateSpec
+from .paged import PagedCache, PagedStep, PagePool
 from .engine import Engine
 from .registry import load_model, register
 
@@ -28,5 +29,5 @@ __all__ = [
     "ColBlockQuantizedLinear", "Linear8bitLt", "find_multiple", "llama_model_lookup", "generate", "sample_probs", "sample_token", "patch_reference", "TPLLaMA", "shard_state_dict",
     "Lugovik", "LugovikConfig", "Zenasun", "ZenasunConfig", "Zuvevik", "ZuvevikConfig", "Rinirax", "RiniraxConfig", "Lukupel", "LukupelConfig",
     "Malulorn", "MalulornConfig",
-    "SequenceStatePool", "StateSpec", "Engine", "load_model", "register",
+    "SequenceStatePool", "StateSpec", "PagedCache", "PagedStep", "PagePool", "Engine", "load_model", "register",
 ]

@@ -13,6 +13,7 @@ ACT_GELU_TANH, ACT_SILU, ACT_SIGMOID, ACT_CLAMPED_SWISH, ACT_XIELU, ACT_NONE, AC
 NORM_RMS, NORM_LAYER = 0, 1
 SCORE_SOFTMAX, SCORE_SIGMOID, SCORE_CHOSEN_SOFTMAX = 0, 1, 2
 DECAY_EXP_SOFTPLUS, DECAY_SIGMOID_ROOT = 0, 1
+STORE_ACT, STORE_E4M3, STORE_INT8 = 0, 1, 2
 
 c_void_p, c_int, c_float, c_size_t = C.c_void_p, C.c_int, C.c_float, C.c_size_t
 
@@ -137,6 +138,8 @@ class MlstmArgs(C.Structure):
     ]
 
 
+_PAGED_ROWS = [c_void_p, C.c_longlong, C.c_longlong] * 2 + [c_void_p] * 7 + [c_int] * 11 + [c_void_p]
+
 _SIGS = {
     "b2l_seq_version": (c_int, []),
     "b2l_seq_last_error": (C.c_char_p, []),
@@ -210,6 +213,11 @@ _SIGS = {
     "b2l_seq_mlstm_step": (c_int, [C.POINTER(MlstmArgs), c_void_p]),
     "b2l_seq_mlstm_gates": (c_int, [C.POINTER(MlstmArgs), c_void_p]),
     "b2l_seq_mlstm_readout": (c_int, [C.POINTER(MlstmArgs), c_void_p]),
+    "b2l_seq_paged_write": (c_int, _PAGED_ROWS),
+    "b2l_seq_paged_read": (c_int, _PAGED_ROWS),
+    "b2l_seq_paged_attention": (c_int, [c_void_p, C.c_longlong, C.c_longlong] + [c_void_p] * 7 + [c_int] * 2 + [c_void_p] * 2 + [C.c_longlong] + [c_int] * 10 + [c_float]
+                                + [c_int] * 5 + [c_void_p]),
+    "b2l_seq_paged_attention_work": (C.c_longlong, [c_int] * 15),
 }
 
 EXPORTS = tuple(_SIGS)

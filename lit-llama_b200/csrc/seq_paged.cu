@@ -1,0 +1,227 @@
+// Rows into a paged pool, quantised on the way, and out of it (layout: seq_paged.cuh).
+//
+// A row of size D of one head is quantised by itself: scale s = max(max |x| / c, 2^-126), code = round(x / s) (to nearest, ties to even), c = 448 for e4m3
+// and 127 for int8, so a code is off by at most half a step: 2^-4 of itself (e4m3, normal codes) or s / 2 (int8).  The floor of s keeps x / s finite for
+// rows of zeros and subnormals.  A row with an infinity or NaN gets the scale NaN and codes 0: it reads back as NaN, and its codes stay finite where a mask
+// hides them.  Both divisions are the correctly rounded ones, so the codes are the same wherever the formula is computed in f32.
+//
+// 16 lanes have a row of keys, the other 16 of the warp the row of values of the same token and head, each lane 8 elements at a time: 16-byte loads of bf16.
+// What bounds it: HBM bytes for prompts, the launch and one chain of loads (starts, length, table) for single tokens.
+#include <math_constants.h>
+
+#include "seq_paged.cuh"
+
+namespace b2l {
+namespace paged {
+
+constexpr int HEADS = 4;             // heads of a token that a warp takes: one look for its place, the loads of all in flight together
+
+struct Rows {
+  Step s;
+  const void *k_new, *v_new;         // or, for reading, where the rows go
+  long long ldk, hsk, ldv, hsv;      // elements between tokens and between heads of them
+  void *k, *v;
+  float *ks, *vs;
+  int kv_heads, K, V;
+};
+
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
+  const uint4 u = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 y = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&y);
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <int STORE> __device__ __forceinline__ uint2 codes8(const float (&x)[8], float s) {
+  uint32_t w[2] = {0u, 0u};
+  if (s == s) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a = __fdiv_rn(x[2 * i], s), b = __fdiv_rn(x[2 * i + 1], s);
+      uint32_t c;
+      if (STORE == E4M3) c = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+      else c = (uint32_t)(__float2int_rn(fminf(fmaxf(a, -127.f), 127.f)) & 0xff) | (uint32_t)(__float2int_rn(fminf(fmaxf(b, -127.f), 127.f)) & 0xff) << 8;
+      w[i >> 1] |= c << 16 * (i & 1);
+    }
+  }
+  return make_uint2(w[0], w[1]);
+}
+template <int STORE> __device__ __forceinline__ void values8(uint2 w, float s, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t u = i < 4 ? w.x : w.y;
+    if (STORE == E4M3) {
+      if (i & 1) continue;
+      const float2 f = e4m3_pair(u >> 8 * (i & 2));
+      x[i] = f.x * s;
+      x[i + 1] = f.y * s;
+    } else {
+      x[i] = (float)(int8_t)(u >> 8 * (i & 3)) * s;
+    }
+  }
+}
+
+template <typename act_t, int STORE>
+__global__ void __launch_bounds__(256) paged_write_kernel(const __grid_constant__ Rows a) {
+  const int lane = threadIdx.x & 31, l = lane & 15;
+  const bool value = lane >= 16;
+  const int groups = (a.kv_heads + HEADS - 1) / HEADS;
+  const long long unit = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+  const int row = (int)(unit / groups), h0 = (int)(unit % groups) * HEADS;
+  if (row >= a.s.rows) return;
+  const int D = value ? a.V : a.K;
+  const act_t* src = reinterpret_cast<const act_t*>(value ? a.v_new : a.k_new) + row * (value ? a.ldv : a.ldk) + h0 * (value ? a.hsv : a.hsk);
+  float x[HEADS][2][8];
+#pragma unroll
+  for (int h = 0; h < HEADS; ++h)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (h0 + h < a.kv_heads && 8 * (l + 16 * i) < D) load8(src + h * (value ? a.hsv : a.hsk) + 8 * (l + 16 * i), x[h][i]);
+      else
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[h][i][e] = 0.f;
+  const int b = sequence_of(a.s, row, lane);
+  if (b < 0) return;
+  int start, n, length;
+  sequence(a.s, b, start, n, length);
+  const int p = length - n + row - start;
+  const int page = p >= 0 ? page_of(a.s, b, p) : -1;
+  if (page < 0) return;
+  const int in_page = p & ((1 << a.s.shift) - 1);
+#pragma unroll
+  for (int h = 0; h < HEADS; ++h) {
+    if (h0 + h >= a.kv_heads) break;
+    const size_t at = (((size_t)page * a.kv_heads + h0 + h) << a.s.shift) + in_page;
+    float s = 1.f;
+    if (STORE != ACT) {
+      float top = 0.f;
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          top = fmaxf(top, fabsf(x[h][i][e]));
+          odd |= !(fabsf(x[h][i][e]) < CUDART_INF_F);
+        }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const uint32_t odds = __ballot_sync(0xffffffffu, odd);
+      s = (value ? odds >> 16 : odds & 0xffffu) ? CUDART_NAN_F : fmaxf(__fdiv_rn(top, STORE == E4M3 ? 448.f : 127.f), 1.17549435e-38f);
+      if (l == 0) (value ? a.vs : a.ks)[at] = s;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int c = 8 * (l + 16 * i);
+      if (c >= D) break;
+      if (STORE == ACT) store8(reinterpret_cast<act_t*>(value ? a.v : a.k) + at * D + c, x[h][i]);
+      else *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(value ? a.v : a.k) + at * D + c) = codes8<STORE>(x[h][i], s);
+    }
+  }
+}
+
+template <typename act_t, int STORE>
+__global__ void __launch_bounds__(256) paged_read_kernel(const __grid_constant__ Rows a) {
+  const int lane = threadIdx.x & 31, l = lane & 15;
+  const bool value = lane >= 16;
+  const int groups = (a.kv_heads + HEADS - 1) / HEADS;
+  const long long unit = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+  const int row = (int)(unit / groups), h0 = (int)(unit % groups) * HEADS;
+  if (row >= a.s.rows) return;
+  const int b = sequence_of(a.s, row, lane);
+  if (b < 0) return;
+  int start, n, length;
+  sequence(a.s, b, start, n, length);
+  const int p = length - n + row - start;
+  const int page = p >= 0 ? page_of(a.s, b, p) : -1, in_page = p & ((1 << a.s.shift) - 1);
+  const int D = value ? a.V : a.K;
+  act_t* dst = reinterpret_cast<act_t*>(const_cast<void*>(value ? a.v_new : a.k_new)) + row * (value ? a.ldv : a.ldk) + h0 * (value ? a.hsv : a.hsk);
+  float x[HEADS][2][8], s[HEADS];
+  uint2 w[HEADS][2];
+#pragma unroll
+  for (int h = 0; h < HEADS; ++h) {
+    const size_t at = (((size_t)max(page, 0) * a.kv_heads + h0 + h) << a.s.shift) + in_page;
+    const bool in = page >= 0 && h0 + h < a.kv_heads;
+    s[h] = STORE != ACT && in ? (value ? a.vs : a.ks)[at] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int c = 8 * (l + 16 * i);
+      w[h][i] = make_uint2(0u, 0u);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[h][i][e] = 0.f;
+      if (in && c < D) {
+        if (STORE == ACT) load8(reinterpret_cast<const act_t*>(value ? a.v : a.k) + at * D + c, x[h][i]);
+        else w[h][i] = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(value ? a.v : a.k) + at * D + c);
+      }
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < HEADS; ++h)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int c = 8 * (l + 16 * i);
+      if (h0 + h >= a.kv_heads || c >= D) continue;
+      if (STORE != ACT) values8<STORE>(w[h][i], s[h], x[h][i]);
+      store8(dst + h * (value ? a.hsv : a.hsk) + c, x[h][i]);
+    }
+}
+
+template <bool WRITE>
+static int rows_call(const char* who, const void* k_new, long long ldk, long long hsk, const void* v_new, long long ldv, long long hsv, void* k, void* v, float* ks, float* vs,
+                     const int* starts, const int* lengths, const int* table, int ldt, int width, int rows, int seqs, int pages, int page, int kv_heads, int K, int V, int store,
+                     int act_dtype, b2l_stream_t stream) {
+  B2L_CHECK_ARG(k_new && v_new, "%s: null pointer", who);
+  if (int rc = check_pool(who, k, v, ks, vs, starts, lengths, table, ldt, width, rows, seqs, pages, page, kv_heads, K, V, store, act_dtype)) return rc;
+  const int per = act_dtype == B2L_F32 ? 4 : 8;
+  B2L_CHECK_ARG((((uintptr_t)k_new | (uintptr_t)v_new) & 15) == 0 && ldk % per == 0 && hsk % per == 0 && ldv % per == 0 && hsv % per == 0,
+                "%s: rows must be 16-byte aligned", who);
+  if (rows == 0 || seqs == 0) return 0;
+  Rows a{step_of(starts, lengths, table, ldt, width, rows, seqs, pages, page), k_new, v_new, ldk, hsk, ldv, hsv, k, v, ks, vs, kv_heads, K, V};
+  const long long units = (long long)rows * ((kv_heads + HEADS - 1) / HEADS);
+  // few units go one to a block, so they spread over the SMs
+  const int warps = units >= 8 * 148 ? 8 : 1;
+  const long long blocks = (units + warps - 1) / warps;
+  B2L_CHECK_SUPPORTED(blocks < (1ll << 31), "%s: %d rows of %d heads", who, rows, kv_heads);
+  const cudaStream_t st = (cudaStream_t)stream;
+#define GO(T, ST)                                                                                             \
+  (WRITE ? paged_write_kernel<T, ST><<<(unsigned)blocks, 32 * warps, 0, st>>>(a) : paged_read_kernel<T, ST><<<(unsigned)blocks, 32 * warps, 0, st>>>(a))
+  B2L_SEQ_DISPATCH(act_dtype, if (store == ACT) GO(act_t, ACT); else if (store == E4M3) GO(act_t, E4M3); else GO(act_t, INT8));
+#undef GO
+  B2L_LAUNCH_CHECK("paged rows");
+  return 0;
+}
+
+}  // namespace paged
+}  // namespace b2l
+
+extern "C" int b2l_seq_paged_write(const void* k_new, long long ldk, long long hsk, const void* v_new, long long ldv, long long hsv, void* k, void* v, float* k_scale,
+                                   float* v_scale, const int* starts, const int* lengths, const int* table, int ldt, int width, int rows, int seqs, int pages, int page,
+                                   int kv_heads, int K, int V, int store, int act_dtype, b2l_stream_t stream) {
+  return b2l::paged::rows_call<true>("b2l_seq_paged_write", k_new, ldk, hsk, v_new, ldv, hsv, k, v, k_scale, v_scale, starts, lengths, table, ldt, width, rows, seqs, pages, page,
+                                     kv_heads, K, V, store, act_dtype, stream);
+}
+
+extern "C" int b2l_seq_paged_read(void* k_out, long long ldk, long long hsk, void* v_out, long long ldv, long long hsv, const void* k, const void* v, const float* k_scale,
+                                  const float* v_scale, const int* starts, const int* lengths, const int* table, int ldt, int width, int rows, int seqs, int pages, int page,
+                                  int kv_heads, int K, int V, int store, int act_dtype, b2l_stream_t stream) {
+  return b2l::paged::rows_call<false>("b2l_seq_paged_read", k_out, ldk, hsk, v_out, ldv, hsv, const_cast<void*>(k), const_cast<void*>(v), const_cast<float*>(k_scale),
+                                      const_cast<float*>(v_scale), starts, lengths, table, ldt, width, rows, seqs, pages, page, kv_heads, K, V, store, act_dtype, stream);
+}

@@ -1,0 +1,159 @@
+// Attention over a paged pool: which rows and keys a CTA has, how results are stored, and the slow form for infinities.
+#pragma once
+#include "seq_paged.cuh"
+
+namespace b2l {
+namespace paged {
+
+// 2^x, documented to 2^-22 of the result and without subnormals: as a weight that leaves out what is below 2^-126 of the largest
+__device__ __forceinline__ float exp2_f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// packed rows first .. of sequence b, which has n new tokens from row `start` on and is `length` tokens long with them
+struct Place { int b, start, n, length, first; };
+
+// The keys that some row of a tile sees, [0, early) and [lo, end), in units of a power of two
+struct Keys {
+  int early, lo, end, p_min, p_max, window, first;
+  __device__ __forceinline__ int early_units(int shift) const { return min((early + (1 << shift) - 1) >> shift, lo >> shift); }
+  __device__ __forceinline__ int units(int shift) const { return end <= 0 ? 0 : early_units(shift) + ((end + (1 << shift) - 1) >> shift) - (lo >> shift); }
+  __device__ __forceinline__ int key0(int u, int shift) const {
+    const int e = early_units(shift);
+    return (u < e ? u : u - e + (lo >> shift)) << shift;
+  }
+  // whether every row of the tile sees all of keys j .. j + size - 1
+  __device__ __forceinline__ bool whole(int j, int size) const { return j + size - 1 <= p_min && (window == 0 || j > p_max - window || j + size <= first); }
+};
+
+// partial results of `splits` CTAs per row: maximum and sum [splits][count][2], outputs [splits][count][V]
+struct Parts { float *ml, *o; int splits; long long count; };
+
+struct Attn {
+  Step s;
+  const void *q, *k, *v;
+  const float *ks, *vs;
+  void* out;
+  long long ldq, hsq;
+  int heads, kv_heads, K, V, window, first, few_max;        // few_max: sequences of at most so many packed rows are the few-row kernel's
+  float scale_log2;
+  int f32, store_kind, compact;
+  Parts few, many;                                           // compact in `few` where both kernels run: 16 packed rows per sequence and key/value head
+
+  __device__ __forceinline__ bool sees(int pos, int j) const { return j <= pos && (window == 0 || j > pos - window || j < first); }
+
+  // Tile `slot` of the tiles of R packed rows of all sequences with more than `above` and at most `most` packed rows; a whole warp looks
+  __device__ __forceinline__ bool place(int slot, int R, int above, int most, int lane, Place& pl) const {
+    const int G = heads / kv_heads;
+    int base = 0;
+    for (int b0 = 0; b0 < s.seqs; b0 += 32) {
+      const int b = b0 + lane;
+      int start = 0, n = 0, length = 0, tiles = 0;
+      if (b < s.seqs) {
+        sequence(s, b, start, n, length);
+        const long long packed = (long long)n * G;
+        tiles = packed > above && packed <= most ? (int)((packed + R - 1) / R) : 0;
+      }
+      int upto = tiles;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, slot < base + upto);
+      if (past) {
+        const int at = __ffs(past) - 1;
+        pl.b = b0 + at;
+        pl.start = __shfl_sync(0xffffffffu, start, at);
+        pl.n = __shfl_sync(0xffffffffu, n, at);
+        pl.length = __shfl_sync(0xffffffffu, length, at);
+        pl.first = (slot - base - __shfl_sync(0xffffffffu, upto - tiles, at)) * R;
+        return true;
+      }
+      base += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return false;
+  }
+  __device__ __forceinline__ Keys keys(const Place& pl, int R) const {
+    const int G = heads / kv_heads, last = min(pl.first + R, pl.n * G) - 1;
+    Keys x;
+    x.p_min = pl.length - pl.n + pl.first / G;
+    x.p_max = pl.length - pl.n + last / G;
+    x.end = x.p_max + 1;
+    x.lo = window ? max(x.p_min - window + 1, 0) : 0;
+    x.early = min(first, x.lo);
+    x.window = window;
+    x.first = first;
+    return x;
+  }
+
+  __device__ __forceinline__ void store(size_t at, const float (&x)[4], float inv) const {      // at: of the first of four outputs
+    const float4 y = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+    if (f32) st_act4(reinterpret_cast<float*>(out) + at, y);
+    else st_act4(reinterpret_cast<__nv_bfloat16*>(out) + at, y);
+  }
+
+  __device__ __forceinline__ float element(const void* p, const float* scales, size_t row, int D, int d) const {
+    const size_t at = row * D + d;
+    if (store_kind == ACT) return f32 ? reinterpret_cast<const float*>(p)[at] : bf2f(reinterpret_cast<const __nv_bfloat16*>(p)[at]);
+    const uint8_t c = reinterpret_cast<const uint8_t*>(p)[at];
+    return (store_kind == E4M3 ? e4m3_pair(c).x : (float)(int8_t)c) * scales[row];
+  }
+};
+
+// One row and head again by a warp, key after key over what the row sees and nothing else.  The products above multiply a hidden value by a weight of
+// zero, and an f32 infinity has parts of NaN: a result that is not finite is computed again here, so it is what the formula says.
+static __device__ __noinline__ void mend_row(const Attn& a, int b, int pos, int row, int head, int lane) {
+  const int h = head / (a.heads / a.kv_heads);
+  float q[8], o[8], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int d = lane + 32 * i;
+    const size_t at = (size_t)row * a.ldq + (size_t)head * a.hsq + d;
+    q[i] = d < a.K ? (a.f32 ? reinterpret_cast<const float*>(a.q)[at] : bf2f(reinterpret_cast<const __nv_bfloat16*>(a.q)[at])) : 0.f;
+    o[i] = 0.f;
+  }
+  for (int j = 0; j <= pos; ++j) {
+    if (!a.sees(pos, j)) {
+      j = max(j, pos - a.window);                            // the next key is the window's first
+      continue;
+    }
+    const int page = page_of(a.s, b, j);
+    if (page < 0) continue;
+    const size_t at = (((size_t)page * a.kv_heads + h) << a.s.shift) + (j & ((1 << a.s.shift) - 1));
+    float x = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (lane + 32 * i < a.K) x = fmaf(q[i], a.element(a.k, a.ks, at, a.K, lane + 32 * i), x);
+    x = warp_sum(x) * a.scale_log2;
+    if (x == -INFINITY) continue;
+    const float now = fmaxf(m, x), f = m == now ? 1.f : exp2_f(m - now), w = exp2_f(x - now);
+    m = now;
+    l = l * f + w;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (lane + 32 * i < a.V) o[i] = o[i] * f + w * a.element(a.v, a.vs, at, a.V, lane + 32 * i);
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int d = lane + 32 * i;
+    const size_t at = ((size_t)row * a.heads + head) * a.V + d;
+    if (d < a.V) {
+      if (a.f32) reinterpret_cast<float*>(a.out)[at] = o[i] * inv;
+      else reinterpret_cast<__nv_bfloat16*>(a.out)[at] = f2bf(o[i] * inv);
+    }
+  }
+}
+__device__ __forceinline__ bool finite4(const float (&x)[4], float inv) {
+  return fabsf(x[0] * inv) < INFINITY && fabsf(x[1] * inv) < INFINITY && fabsf(x[2] * inv) < INFINITY && fabsf(x[3] * inv) < INFINITY;
+}
+
+// the tensor-core kernel of longer chunks (seq_paged_tc.cu): heads that it takes, and its launch
+bool many_takes(int K, int V, int store);
+int many_launch(const Attn& a, int tiles, cudaStream_t stream);
+
+}  // namespace paged
+}  // namespace b2l

@@ -99,7 +99,10 @@ struct Entry {
   F(b2l_seq_depth_step) \
   F(b2l_seq_latent_up) \
   F(b2l_seq_head_gate) \
-  F(b2l_seq_linear_few)
+  F(b2l_seq_linear_few) \
+  F(b2l_seq_paged_write) \
+  F(b2l_seq_paged_read) \
+  F(b2l_seq_paged_attention)
 #define ENTRY(name) {#name, Thunk<decltype(&name)>::signature, Thunk<decltype(&name)>::call},
 const Entry entries[] = {ALL(ENTRY)};
 constexpr int N_ENTRIES = (int)(sizeof(entries) / sizeof(entries[0]));

@@ -1,0 +1,269 @@
+"""Paged key/value caches: the keys and values of many sequences in the pages of one pool, for serving sequences whose lengths are not known beforehand.
+
+    PagePool     which sequence has which pages (host side): sequences come, grow and go, a step books what it needs
+    PagedStep    one step's sequences on the device: rows, lengths, page tables.  Made once, used by every layer
+    PagedCache   one layer's pool: `write` (quantising e4m3 or int8 pools as rows come), `read`, and `attend`, causal softmax attention of the step's new
+                 tokens, single ones and chunks together, over all that the pool holds of their sequences; with a window the last `window`
+                 positions and the first `first` ones
+
+        pool = PagePool(n_pages=4096, page=64, device="cuda")
+        caches = [PagedCache.empty(4096, 64, kv_heads=8, dim=128, dtype=torch.bfloat16, store="fp8") for _ in layers]
+        step = pool.step([("a", 512), ("b", 1)])               # 512 new tokens of a, one of b: rows 0..511 and 512
+        caches[i].write(k, v, step)                            # k [513, 8, 128], v [513, 8, 128]
+        out = caches[i].attend(q, step)                        # q [513, 32, 128] -> [513, 32, 128]
+        pool.release("a")
+
+A token's key and value rows are quantised by themselves, per head: scale = max(max |x| / c, 2^-126), code = round(x / scale), c = 448 (fp8, e4m3) or 127
+(int8).  A row that holds an infinity or NaN reads back as NaN.  A row whose weights sum to zero (it sees no key) attends to zeros.  Everything
+is a kernel of libb200seq (include/b2l_seq.h); CUDA only, no CPU fallback, no derivatives."""
+from typing import Dict, Hashable, List, Optional, Sequence, Tuple
+
+import torch
+
+from . import _seqlib as S
+from .state import PoolFull
+
+STORES = {"act": S.STORE_ACT, "fp8": S.STORE_E4M3, "int8": S.STORE_INT8}
+PAGES = (16, 32, 64, 128, 256)
+
+
+class PagedStep:
+    """One step's sequences: sequence b has rows starts[b] .. starts[b + 1] - 1 of the step's tokens, is lengths[b] tokens long with them, and its token j
+    lies in page table[b, j // page].  An entry of the table outside the pool (-1) is a page that is not there: its keys are not seen.
+
+    The tensors (int32, on the device) may be overwritten between replays of a graph that was recorded with them.  `rows` is the number of tokens;
+    max_new, min_new and max_length are what the host knows of the sequences' new tokens and lengths: they pick between equivalent forms (every form is right
+    for every content of the tensors), so they should be about right."""
+
+    def __init__(self, starts: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, *, rows: int, max_new: int = 0, min_new: int = 0,
+                 max_length: int = 0) -> None:
+        for name, t, dims in (("starts", starts, 1), ("lengths", lengths, 1), ("table", table, 2)):
+            if t.dtype != torch.int32 or t.dim() != dims or t.stride(-1) != 1:
+                raise ValueError(f"paged step: {name} must be int32 with {dims} dimension(s), its entries consecutive")
+            if t.device != lengths.device:
+                raise ValueError("paged step: its tensors are on different devices")
+        if starts.numel() != lengths.numel() + 1 or table.shape[0] != lengths.numel() or table.shape[1] < 1:
+            raise ValueError(f"paged step: {lengths.numel()} lengths, {starts.numel()} starts (one more is wanted), a table of {tuple(table.shape)}")
+        if rows < 0:
+            raise ValueError("paged step: a negative number of rows")
+        self.starts, self.lengths, self.table, self.rows, self.seqs = starts, lengths, table, int(rows), lengths.numel()
+        self.device = lengths.device
+        self.max_new, self.max_length = max(int(max_new), 0), max(int(max_length), 0)
+        # all have the same number where that is the most there can be
+        self.min_new = self.max_new if self.seqs and self.max_new * self.seqs == self.rows else max(int(min_new), 0)
+        self._work: Dict[tuple, int] = {}
+
+    @classmethod
+    def of(cls, sequences: Sequence[Tuple[int, int, Sequence[int]]], device, *, width: int = 0) -> "PagedStep":
+        """From the host: (new tokens, length with them, pages) of every sequence; `width`: the table's, at least the longest list of pages."""
+        starts, lengths, rows = [0], [], 0
+        width = max([int(width), 1] + [len(p) for _, _, p in sequences])
+        flat: List[int] = []
+        for new, length, pages in sequences:
+            if new < 0 or length < new:
+                raise ValueError(f"paged step: {new} new tokens of a sequence that is {length} long with them")
+            rows += new
+            starts.append(rows)
+            lengths.append(length)
+            flat += list(pages) + [-1] * (width - len(pages))
+        n = len(lengths)
+        both = torch.tensor(starts + lengths + flat, dtype=torch.int32).to(device)
+        news = [new for new, _, _ in sequences]
+        return cls(both[:n + 1], both[n + 1:2 * n + 1], both[2 * n + 1:].view(n, width), rows=rows, max_new=max(news, default=0),
+                   min_new=min((x for x in news if x), default=0), max_length=max(lengths, default=0))
+
+    def refill(self, other: "PagedStep") -> None:
+        """The other step's sequences in this one's tensors (of the same number of sequences and rows, and at least its width), for a graph that was
+        recorded with this one."""
+        if other.seqs != self.seqs or other.rows != self.rows or other.table.shape[1] > self.table.shape[1]:
+            raise ValueError(f"paged step: {other.seqs} sequences with {other.rows} rows and {other.table.shape[1]} pages do not fit {self.seqs} with {self.rows} and {self.table.shape[1]}")
+        self.starts.copy_(other.starts, non_blocking=True)
+        self.lengths.copy_(other.lengths, non_blocking=True)
+        self.table[:, :other.table.shape[1]].copy_(other.table, non_blocking=True)
+        self.table[:, other.table.shape[1]:].fill_(-1)
+
+
+class PagePool:
+    """Which sequence has which of `n_pages` pages.  With a window, pages that neither the window nor the first `first` positions reach any more
+    are given back as a sequence grows (their place in its table becomes -1): for models whose layers all look back no further."""
+
+    def __init__(self, n_pages: int, page: int, device, *, window: int = 0, first: int = 0) -> None:
+        if n_pages < 1 or page not in PAGES:
+            raise ValueError(f"page pool: {n_pages} pages of {page} tokens: at least one, of {PAGES}")
+        if window < 0 or first < 0:
+            raise ValueError("page pool: a negative window or number of first tokens")
+        self.n_pages, self.page, self.device, self.window, self.first = int(n_pages), int(page), torch.device(device), int(window), int(first)
+        self._free: List[int] = list(range(self.n_pages - 1, -1, -1))       # page 0 first
+        self._pages: Dict[Hashable, List[int]] = {}
+        self._length: Dict[Hashable, int] = {}
+
+    def has(self, request_id: Hashable) -> bool:
+        return request_id in self._pages
+
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def position(self, request_id: Hashable) -> int:
+        """Tokens of the sequence so far."""
+        return self._length[request_id]
+
+    def pages(self, request_id: Hashable) -> List[int]:
+        return list(self._pages[request_id])
+
+    def release(self, request_id: Hashable) -> None:
+        self._free += [p for p in reversed(self._pages.pop(request_id)) if p >= 0]
+        del self._length[request_id]
+
+    def _behind(self, request_id: Hashable) -> List[int]:
+        """Places in the sequence's table that no later token sees."""
+        if not self.window or request_id not in self._pages:
+            return []
+        reach = self._length[request_id] - self.window + 1                  # the first position that the next token's window has
+        return [i for i, p in enumerate(self._pages[request_id]) if p >= 0 and i * self.page >= self.first and (i + 1) * self.page <= reach]
+
+    def step(self, entries: Sequence[Tuple[Hashable, int]], *, width: int = 0) -> PagedStep:
+        """Books `n` more tokens for every (request id, n); ids that are not known begin a sequence.  Raises PoolFull, with nothing booked, where the pages
+        do not suffice."""
+        if len({rid for rid, _ in entries}) < len(entries):
+            raise ValueError("page pool: a request comes twice in one step")
+        if any(n < 0 for _, n in entries):
+            raise ValueError("page pool: a negative number of tokens")
+        behind = {rid: self._behind(rid) for rid, _ in entries}
+        need = sum(max(0, -(-(self._length.get(rid, 0) + n) // self.page) - len(self._pages.get(rid, ()))) for rid, n in entries)
+        if need > len(self._free) + sum(len(b) for b in behind.values()):
+            raise PoolFull(f"{need} pages are needed, {len(self._free)} of {self.n_pages} are free")
+        sequences = []
+        for rid, _ in entries:
+            for i in behind[rid]:
+                self._free.append(self._pages[rid][i])
+                self._pages[rid][i] = -1
+        for rid, n in entries:
+            pages = self._pages.setdefault(rid, [])
+            self._length[rid] = self._length.get(rid, 0) + n
+            while len(pages) * self.page < self._length[rid]:
+                pages.append(self._free.pop())
+            sequences.append((n, self._length[rid], pages))
+        return PagedStep.of(sequences, self.device, width=width)
+
+
+class PagedCache:
+    """One layer's pool: keys [pages, kv_heads, page, dim] and values [pages, kv_heads, page, vdim] in the activation type (bf16 or f32), in e4m3
+    (torch.float8_e4m3fn) or in int8, the 8-bit ones with f32 scales [pages, kv_heads, page].  `dtype`: the activation type of an 8-bit pool."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None, *,
+                 dtype: Optional[torch.dtype] = None) -> None:
+        if k.dtype != v.dtype or k.dim() != 4 or v.dim() != 4 or k.shape[:3] != v.shape[:3] or k.device != v.device:
+            raise ValueError(f"paged cache: keys {tuple(k.shape)} {k.dtype} and values {tuple(v.shape)} {v.dtype} do not belong together")
+        if k.dtype in (torch.float8_e4m3fn, torch.int8):
+            self.store, self.dtype = ("fp8" if k.dtype == torch.float8_e4m3fn else "int8"), dtype or torch.bfloat16
+            for s in (k_scale, v_scale):
+                if s is None or s.dtype != torch.float32 or s.shape != k.shape[:3] or s.device != k.device or not s.is_contiguous():
+                    raise ValueError(f"paged cache: an 8-bit pool needs contiguous f32 scales {tuple(k.shape[:3])}")
+        else:
+            self.store, self.dtype = "act", dtype or k.dtype
+            if k_scale is not None or v_scale is not None:
+                raise ValueError("paged cache: scales belong to an 8-bit pool")
+            if self.dtype != k.dtype:
+                raise ValueError(f"paged cache: a pool in {k.dtype} for activations in {self.dtype}")
+        if not (k.is_contiguous() and v.is_contiguous()):
+            raise ValueError("paged cache: the pool must be contiguous")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.n_pages, self.kv_heads, self.page, self.dim = k.shape
+        self.vdim = v.shape[3]
+        if self.n_pages < 1 or self.kv_heads < 1 or self.page not in PAGES:
+            raise ValueError(f"paged cache: {self.n_pages} pages of {self.kv_heads} heads, {self.page} tokens: at least one, of {PAGES}")
+        if any(d < 16 or d > 256 or d % 16 for d in (self.dim, self.vdim)):
+            raise ValueError(f"paged cache: heads of {self.dim} and {self.vdim} entries: multiples of 16 up to 256")
+        self.device = k.device
+        self._codes = (STORES[self.store], S.act_code(self.dtype))
+
+    @classmethod
+    def empty(cls, n_pages: int, page: int, kv_heads: int, dim: int, vdim: Optional[int] = None, *, dtype: torch.dtype = torch.bfloat16, store: str = "act",
+              device="cuda") -> "PagedCache":
+        """A pool of zeros."""
+        if store not in STORES:
+            raise ValueError(f"paged cache: store {store!r}: one of {sorted(STORES)}")
+        kept = {"act": dtype, "fp8": torch.float8_e4m3fn, "int8": torch.int8}[store]
+        shape = (int(n_pages), int(kv_heads), int(page))
+        k, v = (torch.zeros(shape + (int(d),), dtype=kept, device=device) for d in (dim, vdim or dim))
+        scales = [torch.zeros(shape, dtype=torch.float32, device=device) for _ in range(2)] if store != "act" else [None, None]
+        return cls(k, v, *scales, dtype=dtype)
+
+    def bytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale) if t is not None)
+
+    # ------------------------------------------------------------------ calls
+    def _rows(self, x: torch.Tensor, heads: Optional[int], size: int, step: PagedStep, what: str) -> torch.Tensor:
+        """x [rows, heads, size] as the kernels take it: entries of a head consecutive, rows on 16-byte borders (else a copy)."""
+        if x.dim() != 3 or x.shape[2] != size or (heads is not None and x.shape[1] != heads) or x.dtype != self.dtype or x.device != self.device:
+            raise ValueError(f"paged cache: {what} {tuple(x.shape)} {x.dtype} on {x.device}, [rows, {heads or 'heads'}, {size}] {self.dtype} on {self.device} is wanted")
+        if x.shape[0] < step.rows:
+            raise ValueError(f"paged cache: {what} has {x.shape[0]} rows, the step {step.rows}")
+        per = 4 if self.dtype == torch.float32 else 8
+        s0, s1, s2 = x.stride()
+        if s2 != 1 or s0 % per or s1 % per or x.data_ptr() % 16:
+            x = x.contiguous()
+            if x.data_ptr() % 16:
+                x = x.clone()
+        return x
+
+    def _call(self, name: str, step: PagedStep, *args) -> None:
+        if step.device != self.device:
+            raise ValueError(f"paged cache: a step on {step.device} for a pool on {self.device}")
+        if torch._C._cuda_getDevice() == self.device.index:
+            S.check(getattr(S.lib(), name)(*args, S.stream_ptr()), name)
+        else:
+            with torch.cuda.device(self.device):
+                S.check(getattr(S.lib(), name)(*args, S.stream_ptr()), name)
+
+    def _pool(self) -> tuple:
+        return S.ptr(self.k), S.ptr(self.v), S.ptr(self.k_scale), S.ptr(self.v_scale)
+
+    def _step(self, step: PagedStep) -> tuple:
+        return S.ptr(step.starts), S.ptr(step.lengths), S.ptr(step.table), step.table.stride(0), step.table.shape[1]
+
+    def write(self, k: torch.Tensor, v: torch.Tensor, step: PagedStep) -> None:
+        """The step's keys [rows, kv_heads, dim] and values [rows, kv_heads, vdim] into the pool.  Rows behind the step's last sequence are not looked at.
+        Two rows of one step must not have the same place (a page in two sequences' tables, both writing there)."""
+        k, v = self._rows(k, self.kv_heads, self.dim, step, "keys"), self._rows(v, self.kv_heads, self.vdim, step, "values")
+        self._call("b2l_seq_paged_write", step, S.ptr(k), k.stride(0), k.stride(1), S.ptr(v), v.stride(0), v.stride(1), *self._pool(), *self._step(step),
+                   min(k.shape[0], v.shape[0]), step.seqs, self.n_pages, self.page, self.kv_heads, self.dim, self.vdim, *self._codes)
+
+    def read(self, step: PagedStep) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The rows that `write` with this step puts into the pool, as they lie there: keys [rows, kv_heads, dim] and values in the activation type."""
+        k = torch.empty((step.rows, self.kv_heads, self.dim), dtype=self.dtype, device=self.device)
+        v = torch.empty((step.rows, self.kv_heads, self.vdim), dtype=self.dtype, device=self.device)
+        self._call("b2l_seq_paged_read", step, S.ptr(k), k.stride(0), k.stride(1), S.ptr(v), v.stride(0), v.stride(1), *self._pool(), *self._step(step), step.rows, step.seqs,
+                   self.n_pages, self.page, self.kv_heads, self.dim, self.vdim, *self._codes)
+        return k, v
+
+    def attend(self, q: torch.Tensor, step: PagedStep, *, scale: Optional[float] = None, window: int = 0, first: int = 0,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Causal softmax attention of the step's tokens (already written) over their sequences:
+
+            out[r, h] = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale q[r, h] . k_j), j <= p and (window == 0 or j > p - window or j < first)
+
+        q [rows, heads, dim] with heads a multiple of kv_heads (head h reads key/value head h // (heads / kv_heads)), p the position of row r; scale
+        dim^-1/2 unless given.  Returns [rows, heads, vdim] (`out`, contiguous, where given); rows behind the step's last sequence are zeros, or as they were
+        in `out`."""
+        q = self._rows(q, None, self.dim, step, "queries")
+        rows, heads = q.shape[0], q.shape[1]
+        if heads < 1 or heads % self.kv_heads:
+            raise ValueError(f"paged cache: {heads} query heads over {self.kv_heads} key/value heads")
+        if window < 0 or first < 0:
+            raise ValueError("paged cache: a negative window or number of first tokens")
+        if out is None:
+            out = (torch.empty if rows == step.rows else torch.zeros)((rows, heads, self.vdim), dtype=self.dtype, device=self.device)
+        elif out.shape != (rows, heads, self.vdim) or out.dtype != self.dtype or out.device != self.device or not out.is_contiguous() or out.data_ptr() % 16:
+            raise ValueError(f"paged cache: out must be {(rows, heads, self.vdim)} {self.dtype} on {self.device}, contiguous and 16-byte aligned")
+        sizes = (heads, self.kv_heads, self.dim, self.vdim, window, first)
+        hints = (step.max_new, step.min_new, step.max_length)
+        width = step.table.shape[1]
+        key = (rows, width, self.page, *sizes, *hints, *self._codes)
+        floats = step._work.get(key)
+        if floats is None:
+            floats = step._work[key] = S.lib().b2l_seq_paged_attention_work(rows, step.seqs, width, self.page, *sizes, *hints, *self._codes)
+        work = torch.empty((floats,), dtype=torch.float32, device=self.device) if floats else None
+        self._call("b2l_seq_paged_attention", step, S.ptr(q), q.stride(0), q.stride(1), *self._pool(), *self._step(step), S.ptr(out), S.ptr(work), floats, rows, step.seqs,
+                   self.n_pages, self.page, *sizes, float(self.dim ** -0.5 if scale is None else scale), *hints, *self._codes)
+        return out
