@@ -499,7 +499,7 @@ int b2l_seq_mlstm_readout(const b2l_seq_mlstm_args* a, b2l_stream_t stream);
  * table entry outside the pool is a page that is not there (and so is every negative position's): nothing is written to it, it reads as zeros, and no
  * row sees its keys.  A row of no sequence is left out: nothing is written for it, and its outputs stay as they are.
  *
- *   b2l_seq_paged_write      new rows into the pool; 8-bit: scale = max(max |x| / c, 2^-126), code = round(x / scale) to nearest even, c = 448 (e4m3) or
+ *   b2l_seq_paged_write      new rows into the pool; 8-bit: scale = max(max |x| (1 / c), 2^-126), code = round(x / scale) to nearest even, c = 448 (e4m3) or
  *                            127 (int8), per token and head (of keys and of values); a row with an infinity or NaN gets the scale NaN and codes 0
  *   b2l_seq_paged_read       the step's rows out of the pool: code * scale, rounded to the activation type
  *   b2l_seq_paged_attention  out[r, h] = sum_j w_j v_j / sum_j w_j over the keys j that row r at position p sees, j <= p and (window == 0 or j > p - window

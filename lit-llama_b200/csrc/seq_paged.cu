@@ -1,9 +1,9 @@
 // Rows into a paged pool, quantised on the way, and out of it (layout: seq_paged.cuh).
 //
-// A row of size D of one head is quantised by itself: scale s = max(max |x| / c, 2^-126), code = round(x / s) (to nearest, ties to even), c = 448 for e4m3
+// A row of size D of one head is quantised by itself: scale s = max(max |x| (1 / c), 2^-126), code = round(x / s) (to nearest, ties to even), c = 448 for e4m3
 // and 127 for int8, so a code is off by at most half a step: 2^-4 of itself (e4m3, normal codes) or s / 2 (int8).  The floor of s keeps x / s finite for
 // rows of zeros and subnormals.  A row with an infinity or NaN gets the scale NaN and codes 0: it reads back as NaN, and its codes stay finite where a mask
-// hides them.  Both divisions are the correctly rounded ones, so the codes are the same wherever the formula is computed in f32.
+// hides them.  1 / c is rounded to f32, and the division by s is the correctly rounded one, so the codes are the same wherever the formula is computed in f32.
 //
 // 16 lanes have a row of keys, the other 16 of the warp the row of values of the same token and head, each lane 8 elements at a time: 16-byte loads of bf16.
 // What bounds it: HBM bytes for prompts, the launch and one chain of loads (starts, length, table) for single tokens.
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(256) paged_write_kernel(const __grid_constant_
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       const uint32_t odds = __ballot_sync(0xffffffffu, odd);
-      s = (value ? odds >> 16 : odds & 0xffffu) ? CUDART_NAN_F : fmaxf(__fdiv_rn(top, STORE == E4M3 ? 448.f : 127.f), 1.17549435e-38f);
+      s = (value ? odds >> 16 : odds & 0xffffu) ? CUDART_NAN_F : fmaxf(top * (STORE == E4M3 ? 1.f / 448.f : 1.f / 127.f), 1.17549435e-38f);
       if (l == 0) (value ? a.vs : a.ks)[at] = s;
     }
 #pragma unroll

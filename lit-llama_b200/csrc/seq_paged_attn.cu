@@ -4,31 +4,45 @@
 //
 // The query heads that read one key/value head are packed with the tokens: packed row i G + g is head g of the group at the sequence's new token i.
 // paged_few_kernel takes 16 packed rows (one tile of mma.m16n8k16) against the keys of one head, 16 at a time.  A warp has every W-th such unit of its share
-// all to itself: its own ring of copies (cp.async; a unit is 16 consecutive rows of one page), its own running maximum, sum and outputs in registers, no
+// all to itself: its own ring of tiled copies (16 rows of one page by 128 bytes, swizzled), its own running maximum, sum and outputs in registers, no
 // barrier in the loop.  The warps' results are joined at the end, and those of several CTAs that share a row's keys by paged_merge_kernel.
 //
-// Operands are fed to the tensor cores as bf16: an e4m3 or int8 code is one exactly, its scale goes into the score (keys) and the weight (values); a weight is
-// two bf16 parts (at most 2^-15 of itself is left out); f32 queries, keys, values and weights are three parts each (f32's 24 bits), of whose nine products the six
-// above 2^-24 are taken and added to f32 registers unit by unit, because the tensor core truncates where it adds to its accumulator.
-// The order of a head's entries and of a unit's keys is free as long as both operands have the same: a lane reads four consecutive entries of a key and
-// has them as its share of a k16 step; 8-bit values are transposed as pairs of neighbouring entries.
+// Operands of the tensor cores, all products exact and added in f32:
+//   bf16 pool       as it lies; a weight is two bf16 parts (at most 2^-15 of itself is left out)
+//   8-bit pool      a code is an f16 exactly (two codes an instruction; bf16 took four times as many), and so the queries: a row of them times the power of
+//                   two that brings its largest entry to 2^14 (an entry below 2^-28 of that keeps fewer than 8 bits, off by 2^-39 of it).  The scale of a
+//                   key goes into its score, the scale of a value into the exponent of its weight, w s = 2^(t + log2 s - m), m the largest t + log2 s so
+//                   far: in f16 with a factor of 2^14, off by 2^-11 of itself at most (2^-39 of the largest where it is small), and sum_j w_j adds w s / s
+//   f32             three parts each (f32's 24 bits); of the nine products of two f32 operands the six above 2^-24.  They are added to f32 registers unit by
+//                   unit, because the tensor core truncates where it adds to its accumulator
+// With 8-bit codes a lane has four consecutive entries of a key as its share of a k16 step (queries laid out alike), and values are transposed as pairs
+// of neighbouring entries, so 16-byte rows of ldmatrix do for both.
 //
 // What bounds it: one pass over the keys and values that the rows see, at HBM's rate, for the rows of a token; 16 rows of f32 are bound by their six products.
 #include <algorithm>
 
 #include "seq_paged_attn.cuh"
+#include "tc_common.cuh"
 
 namespace b2l {
 namespace paged {
 
 // ------------------------------------------------------------------------------------------------ pieces
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool in) {      // 16 bytes, or zeros
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+__device__ __forceinline__ void bulk64(uint32_t dst, const void* src, uint32_t bar) {      // 64 bytes, 16-byte aligned
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], 64, [%2];" ::"r"(dst), "l"(src), "r"(bar) : "memory");
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816h(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -53,138 +67,181 @@ template <int PARTS> __device__ __forceinline__ void parts2(float x, float y, ui
   const __nv_bfloat162 r = __floats2bfloat162_rn(x, y);
   p[PARTS - 1] = *reinterpret_cast<const uint32_t*>(&r);
 }
-// four e4m3 or int8 codes as bf16 pairs (0, 1) and (2, 3): exact, so the upper half of the f32
-template <int STORE> __device__ __forceinline__ uint2 codes4(uint32_t w) {
-  if (STORE == E4M3) {
-    const float2 a = e4m3_pair(w), b = e4m3_pair(w >> 16);
-    return make_uint2(pack_hi(a.x, a.y), pack_hi(b.x, b.y));
+// the same in f16, each part rounded
+template <int PARTS> __device__ __forceinline__ void halves2(float x, float y, uint32_t (&p)[PARTS]) {
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i) {
+    const __half2 h = __floats2half2_rn(x, y);
+    p[i] = *reinterpret_cast<const uint32_t*>(&h);
+    if (i + 1 < PARTS) {
+      const float2 f = __half22float2(h);
+      x -= f.x;
+      y -= f.y;
+    }
   }
-  const uint32_t u = w ^ 0x80808080u;                        // 2^23 + 128 + x in the low byte of an f32's mantissa
-  const float x0 = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7650)) - 8388736.f, x1 = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7651)) - 8388736.f;
-  const float x2 = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7652)) - 8388736.f, x3 = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7653)) - 8388736.f;
-  return make_uint2(pack_hi(x0, x1), pack_hi(x2, x3));
+}
+template <bool HALF, int PARTS> __device__ __forceinline__ void operand2(float x, float y, uint32_t (&p)[PARTS]) {
+  if constexpr (HALF) halves2<PARTS>(x, y, p);
+  else parts2<PARTS>(x, y, p);
+}
+// Codes (bytes) A0, A1 and B0, B1 of w as two f16 pairs.  An int8 code x: 1024 + (x + 128) is an f16 with x + 128 in its low byte
+template <int STORE, int A0, int A1, int B0, int B1> __device__ __forceinline__ uint2 codes4(uint32_t w) {
+  uint2 y;
+  if constexpr (STORE == E4M3) {
+    if constexpr (A0 != 0 || A1 != 1 || B0 != 2 || B1 != 3) w = __byte_perm(w, 0u, A0 | A1 << 4 | B0 << 8 | B1 << 12);
+    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3), b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
+    y.x = (uint32_t)a.x | (uint32_t)a.y << 16;
+    y.y = (uint32_t)b.x | (uint32_t)b.y << 16;
+  } else {
+    const uint32_t u = w ^ 0x80808080u, off = 0x64806480u;   // 1152 twice
+    y.x = __byte_perm(u, 0x64646464u, A0 | 0x40 | A1 << 8 | 0x4000);
+    y.y = __byte_perm(u, 0x64646464u, B0 | 0x40 | B1 << 8 | 0x4000);
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(y.x) : "r"(off));
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(y.y) : "r"(off));
+  }
+  return y;
 }
 // of nine products of three parts (index 0 the largest) the six above 2^-24, the smallest first
 __device__ constexpr int PART_A[6] = {2, 1, 0, 1, 0, 0}, PART_B[6] = {0, 1, 2, 0, 1, 0};
 
 // c += sum of the products of a's and b's parts; FRESH: in an accumulator of its own, added to c as f32 additions are rounded
-template <int AP, int BP, int N, bool FRESH>
+template <bool HALF, int AP, int BP, int N, bool FRESH>
 __device__ __forceinline__ void product(float (&c)[4], const uint32_t (&a)[AP][4], const uint32_t* b0, const uint32_t* b1) {
-  if (!FRESH) {
-#pragma unroll
-    for (int x = 0; x < N; ++x) mma16816(c, a[AP - 1 - x], b0[0], b1[0]);
-    return;
-  }
   float z[4] = {0.f, 0.f, 0.f, 0.f};
+  float (&to)[4] = FRESH ? z : c;
 #pragma unroll
-  for (int x = 0; x < N; ++x) mma16816(z, a[BP == 3 ? PART_A[x] : AP - 1 - x], b0[BP == 3 ? PART_B[x] : 0], b1[BP == 3 ? PART_B[x] : 0]);
+  for (int x = 0; x < N; ++x) {
+    const int i = BP == 3 ? PART_A[x] : AP - 1 - x, j = BP == 3 ? PART_B[x] : 0;
+    if constexpr (HALF) mma16816h(to, a[i], b0[j], b1[j]);
+    else mma16816(to, a[i], b0[j], b1[j]);
+  }
+  if (FRESH)
 #pragma unroll
-  for (int e = 0; e < 4; ++e) c[e] += z[e];
+    for (int e = 0; e < 4; ++e) c[e] += z[e];
 }
 
 // ------------------------------------------------------------------------------------------------ 16 rows
-// One unit of keys (16) and values in a ring stage: rows padded so that the loads below meet no bank twice
-template <typename act_t, int STORE> struct Unit {
-  static constexpr int ES = STORE == ACT ? (int)sizeof(act_t) : 1;
-  // words between rows: = 16 (mod 32) for f32, 8 (mod 16) for bf16, 4 (mod 8) for codes, where a lane reads four entries of one of eight keys
-  __host__ __device__ static int k_row(int K) {
-    const int w = K * ES / 4;
-    return 4 * (ES == 4 ? (w % 32 ? w : w + 16) : ES == 2 ? (w % 16 ? w : w + 8) : (w % 8 ? w : w + 4));
-  }
-  // 4 (mod 8) for the transposing loads, and for f32 (4 mod 16), where a lane reads one entry of four keys
-  __host__ __device__ static int v_row(int V) {
-    const int w = V * ES / 4;
-    return 4 * (w % 8 ? w : w + 4);
-  }
-  __host__ __device__ static int bytes(int K, int V) { return 16 * (k_row(K) + v_row(V)) + (STORE == ACT ? 0 : 128); }
-};
+constexpr int ATOM = 2048;           // 16 rows of 128 bytes, as a swizzled tiled copy leaves them: 16-byte piece c of row r at piece c ^ (r & 7)
+constexpr int MOST_STAGES = 8;
+__host__ __device__ inline int atoms_of(int D, int es) { return (D * es + 127) / 128; }
+
+struct FewMaps { CUtensorMap k, v; };
 
 template <typename act_t, int STORE, int NV>      // NV: the most 16-entry parts of a value
-__global__ void __launch_bounds__(128) paged_few_kernel(const __grid_constant__ Attn a, int stages) {
-  using U = Unit<act_t, STORE>;
-  constexpr bool F32 = sizeof(act_t) == 4;
-  constexpr int QP = F32 ? 3 : 1, KP = F32 && STORE == ACT ? 3 : 1, WP = F32 ? 3 : 2, PRODUCTS = KP == 3 ? 6 : QP, V_PRODUCTS = KP == 3 ? 6 : WP;
-  extern __shared__ __align__(128) uint8_t smem[];
+__global__ void __launch_bounds__(128, NV <= 8 ? 3 : 2) paged_few_kernel(const __grid_constant__ Attn a, const __grid_constant__ FewMaps maps, int stages) {
+  constexpr bool F32 = sizeof(act_t) == 4, HALF = STORE != ACT;
+  constexpr int ES = STORE == ACT ? (int)sizeof(act_t) : 1;
+  constexpr int QP = F32 ? 3 : 1, KP = F32 && !HALF ? 3 : 1, WP = F32 ? 3 : HALF ? 1 : 2, PRODUCTS = KP == 3 ? 6 : QP, V_PRODUCTS = KP == 3 ? 6 : WP;
+  constexpr int PER = ES == 1 ? 4 : 2;                       // k16 steps in the 64 bytes of a key that one ldmatrix takes
+  constexpr float LIFT = HALF ? 14.f : 0.f;                  // weights up to 2^14 in f16
+  // Scales below 2^-60 (rows of zeros have 2^-126, places never written 0) go into the exponent as 2^-60, and with one above 2^40 (values beyond 10^14) the row
+  // is computed again: so no weight above 2^-40 of the largest is lost from the sum, at either end of f32
+  constexpr int SMALL = -60;
+  constexpr float SMALLEST = 8.673617379884035e-19f, LARGEST = 1.099511627776e12f;
+  extern __shared__ __align__(1024) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5, g = lane >> 2, t = lane & 3;
-  const int h = blockIdx.y, split = blockIdx.z, G = a.heads / a.kv_heads, steps = a.K / 16;
+  const int h = blockIdx.y, split = blockIdx.z, G = a.heads / a.kv_heads, steps = (a.K / 16 + PER - 1) / PER * PER;
   Place pl;
   if (!a.place(blockIdx.x, 16, 0, a.few_max, lane, pl)) return;
   const Keys ks = a.keys(pl, 16);
   const int all = ks.units(4), per = (all + a.few.splits - 1) / a.few.splits;
   const int u_begin = min(split * per, all), u_end = min(u_begin + per, all);
   __shared__ uint32_t bad;                                   // rows whose result is not finite
+  __shared__ float lifted[2][16];                            // what a row of queries is multiplied with for f16, and a score with to undo it
+  __shared__ __align__(8) uint64_t bars[4 * MOST_STAGES];
+  __shared__ __align__(16) float scales[HALF ? 4 * MOST_STAGES * 32 : 4];
+  const int ka = atoms_of(a.K, ES), va = atoms_of(a.V, ES), unit_bytes = (ka + va) * ATOM;
+  const uint32_t s0 = tc::smem_u32(smem);
+  const uint32_t ring = s0 + (uint32_t)(warp * stages * unit_bytes), sq = s0 + (uint32_t)(W * stages * unit_bytes);
+  const uint32_t bar0 = tc::smem_u32(bars) + warp * MOST_STAGES * 8, sc0 = tc::smem_u32(scales) + warp * MOST_STAGES * 128;
+  uint8_t* queries = smem + W * stages * unit_bytes;
   if (threadIdx.x == 0) bad = 0u;
-  const uint32_t s0 = (uint32_t)__cvta_generic_to_shared(smem), sq = s0;
-  const int kr = U::k_row(a.K), vr = U::v_row(a.V), unit_bytes = U::bytes(a.K, a.V);
-  const uint32_t ring = s0 + (uint32_t)(QP * steps * 512) + (uint32_t)(warp * stages * unit_bytes);
-
-  // the queries as the A operand's registers, part by part: entry 16 s + 4 t + e of rows g and g + 8
-  for (int i = threadIdx.x; i < steps * 32; i += blockDim.x) {
-    const int s = i >> 5, l = i & 31;
-    float x[2][4];
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int r = pl.first + (l >> 2) + 8 * half;
-      if (r < pl.n * G) {
-        const float4 f = ld_act4(reinterpret_cast<const act_t*>(a.q) + (pl.start + r / G) * a.ldq + (h * G + r % G) * a.hsq + 16 * s + 4 * (l & 3));
-        x[half][0] = f.x; x[half][1] = f.y; x[half][2] = f.z; x[half][3] = f.w;
-      } else {
-        x[half][0] = x[half][1] = x[half][2] = x[half][3] = 0.f;
-      }
-    }
-    uint32_t p[4][QP];
-    parts2<QP>(x[0][0], x[0][1], p[0]);
-    parts2<QP>(x[1][0], x[1][1], p[1]);
-    parts2<QP>(x[0][2], x[0][3], p[2]);
-    parts2<QP>(x[1][2], x[1][3], p[3]);
-#pragma unroll
-    for (int q = 0; q < QP; ++q) *reinterpret_cast<uint4*>(smem + (q * steps + s) * 512 + l * 16) = make_uint4(p[0][q], p[1][q], p[2][q], p[3][q]);
+  if (lane == 0) {
+    for (int i = 0; i < stages; ++i) tc::mbar_init(bar0 + 8 * i, 1);
+    tc::mbar_init_fence();
   }
-  __syncthreads();
+  __syncwarp();
 
   const int count = u_begin + warp < u_end ? (u_end - u_begin - warp + W - 1) / W : 0;      // this warp's units: u_begin + warp + W i
   // page of this warp's unit i: 32 at a time, one per lane
   int pages = -1, pages_at = -1;
   auto key0_of = [&](int i) { return ks.key0(u_begin + warp + W * i, 4); };
-  auto page_at = [&](int i) {
+  uint32_t skipped = 0;                                      // ring stages whose page is not there
+  int fill = 0;                                              // stage that is filled next
+  auto load = [&](int i) {
+    if (i >= count) return;
     if (i / 32 != pages_at) {
       pages_at = i / 32;
       const int mine = pages_at * 32 + lane;
       pages = mine < count ? page_of(a.s, pl.b, key0_of(mine)) : -1;
     }
-    return __shfl_sync(0xffffffffu, pages, i & 31);
-  };
-  uint32_t skipped = 0;                                      // ring stages whose page is not there
-  auto load = [&](int i) {
-    const int stage = i % stages;
-    const uint32_t dst = ring + stage * unit_bytes;
-    const int page = i < count ? page_at(i) : -1;
+    const int page = __shfl_sync(0xffffffffu, pages, i & 31);
     if (page >= 0) {
-      skipped &= ~(1u << stage);
-      const int key0 = key0_of(i), valid = min(16, ks.end - key0);      // rows behind the last key that is seen come as zeros
-      const size_t at = (((size_t)page * a.kv_heads + h) << a.s.shift) + (key0 & ((1 << a.s.shift) - 1));
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        const int D = kv ? a.V : a.K, row_chunks = D * U::ES / 16, chunks = 16 * row_chunks, row_bytes = kv ? vr : kr;
-        const uint8_t* src = reinterpret_cast<const uint8_t*>(kv ? a.v : a.k) + at * D * U::ES;
-        const uint32_t base = dst + (kv ? 16 * kr : 0);
-        int r = lane / row_chunks, c = lane - r * row_chunks;
-        const int dr = 32 / row_chunks, dc = 32 - dr * row_chunks;
-        for (int x = lane; x < chunks; x += 32) {
-          cp16(base + r * row_bytes + c * 16, src + (size_t)x * 16, r < valid);
-          r += dr;
-          c += dc;
-          if (c >= row_chunks) { c -= row_chunks; ++r; }
+      skipped &= ~(1u << fill);
+      if (lane == 0) {
+        const int row = ((page * a.kv_heads + h) << a.s.shift) + (key0_of(i) & ((1 << a.s.shift) - 1));
+        const uint32_t dst = ring + fill * unit_bytes, bar = bar0 + 8 * fill;
+        tc::mbar_expect_tx(bar, unit_bytes + (HALF ? 128 : 0));
+        for (int x = 0; x < ka; ++x) tc::tma_load_2d(dst + x * ATOM, &maps.k, x * (128 / ES), row, bar);
+        for (int x = 0; x < va; ++x) tc::tma_load_2d(dst + (ka + x) * ATOM, &maps.v, x * (128 / ES), row, bar);
+        if (HALF) {
+          bulk64(sc0 + 128 * fill, a.ks + row, bar);
+          bulk64(sc0 + 128 * fill + 64, a.vs + row, bar);
         }
       }
-      if (STORE != ACT && lane < 8) cp16(dst + 16 * (kr + vr) + lane * 16, (lane < 4 ? a.ks : a.vs) + at + 4 * (lane & 3), 4 * (lane & 3) < valid);
     } else {
-      skipped |= 1u << stage;
+      skipped |= 1u << fill;
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (++fill == stages) fill = 0;
   };
+  for (int i = 0; i < stages - 1; ++i) load(i);
 
-  float o[2 * NV][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  // the queries as the A operand's registers, part by part: rows g and g + 8 by entries 2 t, + 1 and 8 + 2 t, + 1 of a k16 step, or (codes) 4 t .. 4 t + 3
+  if (HALF) {
+    for (int r = warp; r < 16; r += W) {
+      const int at = pl.first + r;
+      float top = 0.f;
+      if (at < pl.n * G)
+        for (int d = lane; d < a.K; d += 32) top = fmaxf(top, fabsf(ld_act(reinterpret_cast<const act_t*>(a.q), (pl.start + at / G) * a.ldq + (h * G + at % G) * a.hsq + d)));
+      top = warp_max(top);
+      if (lane == 0) {
+        // exponents of 2^14 / top's: within f32's normal range for every top, 0 for a top of 0
+        const int e = (int)(__float_as_uint(top) >> 23) - 127, up = top > 0.f && top < INFINITY ? min(14 - e, 120) : 0;
+        lifted[0][r] = __uint_as_float((uint32_t)(up + 127) << 23);
+        lifted[1][r] = a.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
+      }
+    }
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < steps * 32; i += blockDim.x) {
+    const int s = i >> 5, l = i & 31;
+    uint32_t p[4][QP];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int r = (l >> 2) + 8 * half, at = pl.first + r;
+      const act_t* src = reinterpret_cast<const act_t*>(a.q) + (pl.start + at / G) * a.ldq + (h * G + at % G) * a.hsq + 16 * s;
+      const bool in = at < pl.n * G && 16 * s < a.K;
+      const int d0 = HALF ? 4 * (l & 3) : 2 * (l & 3), d1 = HALF ? d0 + 2 : d0 + 8;
+      float x[4] = {0.f, 0.f, 0.f, 0.f};
+      if (in) {
+        x[0] = ld_act(src, d0);
+        x[1] = ld_act(src, d0 + 1);
+        x[2] = ld_act(src, d1);
+        x[3] = ld_act(src, d1 + 1);
+      }
+      if (HALF)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] *= lifted[0][r];
+      operand2<HALF, QP>(x[0], x[1], p[half]);
+      operand2<HALF, QP>(x[2], x[3], p[2 + half]);
+    }
+#pragma unroll
+    for (int q = 0; q < QP; ++q) *reinterpret_cast<uint4*>(queries + (q * steps + s) * 512 + l * 16) = make_uint4(p[0][q], p[1][q], p[2][q], p[3][q]);
+  }
+  __syncthreads();
+
+  float o[2 * NV][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, cr[2] = {a.scale_log2, a.scale_log2};
+  if (HALF) { cr[0] = lifted[1][g]; cr[1] = lifted[1][g + 8]; }
 #pragma unroll
   for (int i = 0; i < 2 * NV; ++i)
 #pragma unroll
@@ -192,72 +249,112 @@ __global__ void __launch_bounds__(128) paged_few_kernel(const __grid_constant__ 
   int pos[2];                                                // of rows g and g + 8
 #pragma unroll
   for (int r = 0; r < 2; ++r) pos[r] = pl.first + g + 8 * r < pl.n * G ? pl.length - pl.n + (pl.first + g + 8 * r) / G : -1;
+  // where this lane's row of an ldmatrix lies: keys (row lane & 7, piece lane / 8 of four) and values (row lane & 15, piece lane / 16 of two)
+  const uint32_t k_at = (lane & 7) * 128 + (((lane >> 3) ^ (lane & 7)) << 4), v_at = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
 
-  for (int i = 0; i < stages - 1; ++i) load(i);
+  uint32_t dead = (s0 & 1023u) ? 1u : 0u, phase = 0;         // swizzled atoms need 1024-byte alignment
+  int stage = 0;
   for (int i = 0; i < count; ++i) {
     __syncwarp();                                            // every lane has done with the stage that is filled next
     load(i + stages - 1);
-    if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
-    else if (stages == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
-    else if (stages == 4) asm volatile("cp.async.wait_group 3;" ::: "memory");
-    else asm volatile("cp.async.wait_group 5;" ::: "memory");
-    __syncwarp();
-    if (skipped >> (i % stages) & 1u) continue;
-    const uint32_t kb = ring + (i % stages) * unit_bytes, vb = kb + 16 * kr, sb = vb + 16 * vr;
+    const int st = stage;
+    if (++stage == stages) stage = 0;
+    if (skipped >> st & 1u) continue;
+    tc::mbar_wait_warp(bar0 + 8 * st, phase >> st & 1u, dead);
+    phase ^= 1u << st;
+    if (dead) break;
+    const uint32_t kb = ring + st * unit_bytes, vb = kb + ka * ATOM, sb = sc0 + 128 * st;
+    const int key0 = key0_of(i), valid = ks.end - key0;
+    if (valid < 16) {                                        // the last unit: what lies behind the last key that is seen may be anything
+      for (int x = lane; x < (16 - valid) * 8 * va; x += 32) {
+        const int r = valid + x / (8 * va), c = x % (8 * va);
+        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vb + (c >> 3) * ATOM + r * 128 + (c & 7) * 16), "r"(0u) : "memory");
+      }
+      __syncwarp();
+    }
     float s[2][4];
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+    if constexpr (F32 && !HALF) {
 #pragma unroll 2
-    for (int k = 0; k < steps; ++k) {
-      uint32_t q[QP][4];
+      for (int k = 0; k < steps; ++k) {
+        uint32_t q[QP][4];
 #pragma unroll
-      for (int p = 0; p < QP; ++p) {
-        const uint4 u = lds128(sq + (p * steps + k) * 512 + lane * 16);
-        q[p][0] = u.x; q[p][1] = u.y; q[p][2] = u.z; q[p][3] = u.w;
-      }
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const uint32_t at = kb + (8 * n + g) * kr + (16 * k + 4 * t) * U::ES;
-        uint32_t b0[KP], b1[KP];
-        if (STORE != ACT) {
-          const uint2 c = codes4<STORE>(lds32(at));
-          b0[0] = c.x;
-          b1[0] = c.y;
-        } else if (F32) {
-          const uint4 u = lds128(at);
-          parts2<KP>(__uint_as_float(u.x), __uint_as_float(u.y), b0);
-          parts2<KP>(__uint_as_float(u.z), __uint_as_float(u.w), b1);
-        } else {
-          const uint2 u = lds64(at);
-          b0[0] = u.x;
-          b1[0] = u.y;
+        for (int p = 0; p < QP; ++p) {
+          const uint4 u = lds128(sq + (p * steps + k) * 512 + lane * 16);
+          q[p][0] = u.x; q[p][1] = u.y; q[p][2] = u.z; q[p][3] = u.w;
         }
 #pragma unroll
-        for (int x = 0; x < PRODUCTS; ++x) {
-          const int qi = KP == 3 ? PART_A[x] : QP - 1 - x, ki = KP == 3 ? PART_B[x] : 0;
-          mma16816(s[n], q[qi], b0[ki], b1[ki]);
+        for (int n = 0; n < 2; ++n) {
+          const uint32_t row = kb + (k >> 1) * ATOM + (8 * n + g) * 128, c = 4 * (k & 1) + (t >> 1), low = 8 * (t & 1);
+          uint32_t b0[KP], b1[KP];
+          const uint2 u = lds64(row + ((c ^ g) << 4) + low), w = lds64(row + (((c + 2) ^ g) << 4) + low);
+          parts2<KP>(__uint_as_float(u.x), __uint_as_float(u.y), b0);
+          parts2<KP>(__uint_as_float(w.x), __uint_as_float(w.y), b1);
+          product<false, QP, KP, PRODUCTS, false>(s[n], q, b0, b1);
+        }
+      }
+    } else {
+#pragma unroll 2
+      for (int j = 0; j < steps / PER; ++j) {
+        uint32_t r[2][4];
+        const uint32_t at = kb + (j >> 1) * ATOM + (k_at ^ ((j & 1) << 6));
+        ldsm_x4(at, r[0]);
+        ldsm_x4(at + 1024, r[1]);
+#pragma unroll
+        for (int x = 0; x < PER; ++x) {
+          uint32_t q[QP][4];
+#pragma unroll
+          for (int p = 0; p < QP; ++p) {
+            const uint4 u = lds128(sq + (p * steps + PER * j + x) * 512 + lane * 16);
+            q[p][0] = u.x; q[p][1] = u.y; q[p][2] = u.z; q[p][3] = u.w;
+          }
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            if constexpr (HALF) {
+              const uint2 b = codes4<STORE, 0, 1, 2, 3>(r[n][x]);
+              product<true, QP, 1, QP, false>(s[n], q, &b.x, &b.y);
+            } else {
+              product<false, QP, 1, QP, false>(s[n], q, &r[n][2 * x], &r[n][2 * x + 1]);
+            }
+          }
         }
       }
     }
     // scores in powers of two; lane: keys 8 n + 2 t, + 1 of rows g (entries 0, 1) and g + 8 (2, 3)
-    const int key0 = key0_of(i);
-    float top[2] = {-INFINITY, -INFINITY}, vs[2][2] = {{1.f, 1.f}, {1.f, 1.f}};
+    float top[2] = {-INFINITY, -INFINITY}, over[2][2], rest[2][2];      // one over what of the values' scales is in the exponent; what is not
     const bool whole = ks.whole(key0, 16);
+    bool small = false;
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-      float c[2] = {a.scale_log2, a.scale_log2};
-      if (STORE != ACT) {
+      float c[2] = {1.f, 1.f}, add[2] = {0.f, 0.f};
+      if (HALF) {
         const uint2 x = lds64(sb + (8 * n + 2 * t) * 4), y = lds64(sb + 64 + (8 * n + 2 * t) * 4);
-        c[0] *= __uint_as_float(x.x);
-        c[1] *= __uint_as_float(x.y);
-        vs[n][0] = __uint_as_float(y.x);
-        vs[n][1] = __uint_as_float(y.y);
+        c[0] = __uint_as_float(x.x);
+        c[1] = __uint_as_float(x.y);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float v = __uint_as_float(e ? y.y : y.x);
+          if (F32) {                                         // the power of two: exact; NaN, the sign and what is left of a small scale stay in the rest
+            const int exponent = max((int)(__float_as_uint(v) >> 23 & 255u), 127 + SMALL);
+            add[e] = (float)(exponent - 127);
+            over[n][e] = __uint_as_float((uint32_t)(254 - exponent) << 23);
+            rest[n][e] = v * over[n][e];
+          } else {                                           // all of it, to 2^-22 (of log2 s where that is larger than 1), unless it is small
+            const float some = v < SMALLEST ? SMALLEST : v;
+            small |= v < SMALLEST;
+            asm("lg2.approx.f32 %0, %1;" : "=f"(add[e]) : "f"(some));
+            asm("rcp.approx.f32 %0, %1;" : "=f"(over[n][e]) : "f"(some));
+            rest[n][e] = v < SMALLEST ? v * over[n][e] : 1.f;
+          }
+          if (v > LARGEST) over[n][e] = NAN;
+        }
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[n][e] *= c[e & 1];
+        s[n][e] = HALF ? fmaf(s[n][e] * c[e & 1], cr[e >> 1], add[e & 1]) : s[n][e] * cr[0];
         if (!whole && !a.sees(pos[e >> 1], key0 + 8 * n + 2 * t + (e & 1))) s[n][e] = -INFINITY;
         top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
       }
@@ -284,61 +381,70 @@ __global__ void __launch_bounds__(128) paged_few_kernel(const __grid_constant__ 
         o[x][3] *= f[1];
       }
     }
-    uint32_t w[4][WP];                                       // the weights as the A operand of the second product
+    if (HALF && !F32) small = __any_sync(0xffffffffu, small);
+    uint32_t wa[WP][4];                                      // the weights as the A operand of the second product
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         float x[2];
+        uint32_t w[WP];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float z = s[n][2 * r + e];
-          x[e] = z == -INFINITY ? 0.f : exp2_f(z - m[r]);
-          l[r] += x[e];
-          if (STORE != ACT) x[e] = z == -INFINITY ? 0.f : x[e] * vs[n][e];      // a scale that no row may see can be NaN
+          x[e] = exp2_f(F32 ? (z - m[r]) + LIFT : z - (m[r] - LIFT));
+          if (z == -INFINITY) x[e] = 0.f;                    // hidden, or of no weight: whatever its scale is, and while the maximum is -inf
+          else l[r] = HALF ? fmaf(x[e], over[n][e], l[r]) : l[r] + x[e];
+          if (HALF && (F32 || small)) x[e] = z == -INFINITY ? 0.f : x[e] * rest[n][e];
         }
-        parts2<WP>(x[0], x[1], w[2 * n + r]);
+        operand2<HALF, WP>(x[0], x[1], w);
+#pragma unroll
+        for (int p = 0; p < WP; ++p) wa[p][2 * n + r] = w[p];
       }
-    uint32_t wa[WP][4];
+    if constexpr (F32 && !HALF) {
 #pragma unroll
-    for (int p = 0; p < WP; ++p)
+      for (int x = 0; x < 2 * NV; ++x) {
+        if (8 * x >= a.V) break;
+        float v[4];                                          // entry 8 x + g of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
-      for (int e = 0; e < 4; ++e) wa[p][e] = w[e][p];
-    if (STORE != ACT) {
+        for (int e = 0; e < 4; ++e) {
+          const int r = 2 * t + (e & 1) + 8 * (e >> 1), c = 2 * x + (g >> 2);
+          v[e] = __uint_as_float(lds32(vb + (c >> 3) * ATOM + r * 128 + (((c & 7) ^ (r & 7)) << 4) + (g & 3) * 4));
+        }
+        uint32_t b0[KP], b1[KP];
+        parts2<KP>(v[0], v[1], b0);
+        parts2<KP>(v[2], v[3], b1);
+        product<false, WP, KP, V_PRODUCTS, true>(o[x], wa, b0, b1);
+      }
+    } else if constexpr (HALF) {
 #pragma unroll
-      for (int x = 0; x < (NV + 1) / 2; ++x) {
+      for (int x = 0; x < (NV + 1) / 2; ++x) {               // 32 entries at a time; the last 16 may be the copy's zeros
         if (32 * x >= a.V) break;
-        const bool two = 32 * x + 16 < a.V;
         uint32_t r4[4];
-        ldsm_x4_t(vb + (lane & 15) * vr + 32 * x + (two ? lane & 16 : 0), r4);
+        ldsm_x4_t(vb + (x >> 2) * ATOM + (v_at ^ ((x & 3) << 5)), r4);
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-          if (2 * x + y >= NV || (y && !two)) break;
-          const uint2 lo = codes4<STORE>(__byte_perm(r4[2 * y], 0u, 0x3120)), hi = codes4<STORE>(__byte_perm(r4[2 * y + 1], 0u, 0x3120));      // (k0 d0, k1 d0, k0 d1, k1 d1)
-          product<WP, 1, V_PRODUCTS, F32>(o[2 * (2 * x + y)], wa, &lo.x, &hi.x);
-          product<WP, 1, V_PRODUCTS, F32>(o[2 * (2 * x + y) + 1], wa, &lo.y, &hi.y);
+          if (2 * x + y >= NV) break;
+          const uint2 lo = codes4<STORE, 0, 2, 1, 3>(r4[2 * y]), hi = codes4<STORE, 0, 2, 1, 3>(r4[2 * y + 1]);      // entries 2 g and 2 g + 1 of two keys
+          product<true, WP, 1, WP, F32>(o[2 * (2 * x + y)], wa, &lo.x, &hi.x);
+          product<true, WP, 1, WP, F32>(o[2 * (2 * x + y) + 1], wa, &lo.y, &hi.y);
         }
       }
-    } else if (!F32) {
+    } else {
 #pragma unroll
       for (int x = 0; x < NV; ++x) {
         if (16 * x >= a.V) break;
         uint32_t r4[4];
-        ldsm_x4_t(vb + (lane & 15) * vr + 32 * x + (lane & 16), r4);
-        product<WP, 1, V_PRODUCTS, F32>(o[2 * x], wa, &r4[0], &r4[1]);
-        product<WP, 1, V_PRODUCTS, F32>(o[2 * x + 1], wa, &r4[2], &r4[3]);
-      }
-    } else {
-#pragma unroll
-      for (int x = 0; x < 2 * NV; ++x) {
-        if (8 * x >= a.V) break;
-        const uint32_t at = vb + 2 * t * vr + (8 * x + g) * 4;
-        uint32_t b0[KP], b1[KP];
-        parts2<KP>(__uint_as_float(lds32(at)), __uint_as_float(lds32(at + vr)), b0);
-        parts2<KP>(__uint_as_float(lds32(at + 8 * vr)), __uint_as_float(lds32(at + 9 * vr)), b1);
-        product<WP, KP, V_PRODUCTS, F32>(o[x], wa, b0, b1);
+        ldsm_x4_t(vb + (x >> 2) * ATOM + (v_at ^ ((x & 3) << 5)), r4);
+        product<false, WP, 1, WP, false>(o[2 * x], wa, &r4[0], &r4[1]);
+        product<false, WP, 1, WP, false>(o[2 * x + 1], wa, &r4[2], &r4[3]);
       }
     }
+  }
+  if (dead) {                                                // copies under way end before the CTA does; the rows are computed again from memory
+    uint32_t late = 0;
+    for (int i = 0; i < stages; ++i) tc::mbar_wait_warp(bar0 + 8 * i, phase >> i & 1u, late);
+    l[0] = l[1] = NAN;
   }
 
   // the warps' results: reference maximum, sum and outputs of 16 rows each
@@ -347,7 +453,6 @@ __global__ void __launch_bounds__(128) paged_few_kernel(const __grid_constant__ 
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();
   float* sm = reinterpret_cast<float*>(smem);                // [W][16] maxima, [W][16] sums, [W][16][ov] outputs
   const int ov = a.V + 4;
@@ -404,49 +509,72 @@ __global__ void __launch_bounds__(128) paged_few_kernel(const __grid_constant__ 
 }
 
 // ------------------------------------------------------------------------------------------------ joining parts
-// A warp per row and head; rows of sequences whose parts were not split are in place already.
-__global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant__ Attn a) {
-  const int lane = threadIdx.x & 31, G = a.heads / a.kv_heads;
-  const long long unit = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-  const int row = (int)(unit / a.heads), head = (int)(unit % a.heads);
-  if (row >= a.s.rows) return;
-  const int b = sequence_of(a.s, row, lane);
-  if (b < 0) return;
-  int start, n, length;
-  sequence(a.s, b, start, n, length);
+// `per` warps (a power of two) have a row and head, each every per-th part; rows of sequences whose parts were not split are in place already.  Parts are
+// read once, and the loads of a warp's parts do not wait for one another.
+constexpr int MERGE_WARPS = 8;
+__global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const __grid_constant__ Attn a, int per) {
+  __shared__ float4 sx[MERGE_WARPS][64];
+  __shared__ float2 sml[MERGE_WARPS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, G = a.heads / a.kv_heads;
+  const int here = MERGE_WARPS / per, sub = warp / here, own = warp % here;      // part of the unit's warps, unit of the block
+  const long long unit = (long long)blockIdx.x * here + own;
+  const int row = (int)min(unit / a.heads, (long long)a.s.rows), head = (int)(unit % a.heads), h = head / G;
+  const int b = row < a.s.rows ? sequence_of(a.s, row, lane) : -1;
+  int start = 0, n = 0, length = 0;
+  if (b >= 0) sequence(a.s, b, start, n, length);
   const bool few = (long long)n * G <= a.few_max;
   const Parts& p = few ? a.few : a.many;
-  if (p.splits <= 1) return;
-  const int h = head / G;
+  const bool on = b >= 0 && p.splits > 1;
   const long long at = few && a.compact ? (long long)(b * a.kv_heads + h) * 16 + (row - start) * G + head % G : (long long)row * a.heads + head;
   float M = -INFINITY, L = 0.f;
-  for (int i = lane; i < p.splits; i += 32) M = fmaxf(M, p.ml[2 * (i * p.count + at)]);
-  M = warp_max(M);
-  float x[2][4] = {};
-  for (int i = 0; i < p.splits; ++i) {
-    const float2 ml = *reinterpret_cast<const float2*>(p.ml + 2 * (i * p.count + at));
-    if (ml.x == -INFINITY && ml.y == 0.f) continue;          // saw nothing
-    const float f = ml.x == M ? 1.f : exp2_f(ml.x - M);
-    L += f * ml.y;
+  float4 x[2] = {};
+  if (on) {
+#pragma unroll 4
+    for (int i = sub; i < p.splits; i += per) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.ml + 2 * (i * p.count + at));
+      const float4* y = reinterpret_cast<const float4*>(p.o + (i * p.count + at) * a.V) + lane;
+      float4 z[2];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int d = 4 * (lane + 32 * c);
-      if (d >= a.V) break;
-      const float4 y = *reinterpret_cast<const float4*>(p.o + (i * p.count + at) * a.V + d);
-      x[c][0] = fmaf(f, y.x, x[c][0]);
-      x[c][1] = fmaf(f, y.y, x[c][1]);
-      x[c][2] = fmaf(f, y.z, x[c][2]);
-      x[c][3] = fmaf(f, y.w, x[c][3]);
+      for (int c = 0; c < 2; ++c) z[c] = 4 * (lane + 32 * c) < a.V ? y[32 * c] : make_float4(0.f, 0.f, 0.f, 0.f);
+      if (ml.x == -INFINITY && ml.y == 0.f) continue;        // saw nothing
+      const float now = fmaxf(M, ml.x), f = M == now ? 1.f : exp2_f(M - now), w = ml.x == now ? 1.f : exp2_f(ml.x - now);
+      M = now;
+      L = L * f + w * ml.y;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) x[c] = make_float4(x[c].x * f + w * z[c].x, x[c].y * f + w * z[c].y, x[c].z * f + w * z[c].z, x[c].w * f + w * z[c].w);
     }
   }
+  if (per > 1) {
+    if (sub > 0) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) sx[warp][lane + 32 * c] = x[c];
+      if (lane == 0) sml[warp] = make_float2(M, L);
+    }
+    __syncthreads();
+    if (sub > 0) return;
+    for (int w0 = warp + here; w0 < MERGE_WARPS; w0 += here) {
+      const float2 ml = sml[w0];
+      if (ml.x == -INFINITY && ml.y == 0.f) continue;
+      const float now = fmaxf(M, ml.x), f = M == now ? 1.f : exp2_f(M - now), w = ml.x == now ? 1.f : exp2_f(ml.x - now);
+      M = now;
+      L = L * f + w * ml.y;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float4 z = sx[w0][lane + 32 * c];
+        x[c] = make_float4(x[c].x * f + w * z.x, x[c].y * f + w * z.y, x[c].z * f + w * z.z, x[c].w * f + w * z.w);
+      }
+    }
+  }
+  if (!on) return;
   const float inv = L == 0.f ? 0.f : 1.f / L;
   bool fine = true;
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     const int d = 4 * (lane + 32 * c);
     if (d >= a.V) break;
-    a.store(((size_t)row * a.heads + head) * a.V + d, x[c], inv);
-    fine = fine && finite4(x[c], inv);
+    const float y[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+    a.store(((size_t)row * a.heads + head) * a.V + d, y, inv);
+    fine = fine && finite4(y, inv);
   }
   if (!__all_sync(0xffffffffu, fine)) {
     __syncwarp();
@@ -482,7 +610,10 @@ static Plan plan_of(int rows, int seqs, int width, int page, int heads, int kv_h
   p.few_count = p.compact ? (long long)seqs * kv_heads * 16 : (long long)rows * heads;
   p.many_count = (long long)rows * heads;
   if (p.few) {
-    const long long ctas = (long long)kv_heads * std::max(1, p.few_tiles), want = (4ll * sms + ctas - 1) / ctas;
+    // an SM has three or four CTAs at a time.  Few CTAs: as many parts as fill them once.  Many: parts of a quarter of that each, so that sequences of
+    // different lengths share the SMs evenly
+    const long long ctas = (long long)kv_heads * std::max(1, p.few_tiles), slots = 3ll * sms;
+    const long long want = 2 * ctas <= slots ? slots / ctas : (4 * slots + ctas - 1) / ctas;
     p.few_splits = (int)std::max<long long>(1, std::min({want, keys / 256, 128ll, MOST_WORK / (p.few_count * (V + 2) + 1)}));
   }
   auto floats = [&](int splits, long long count) { return splits > 1 ? (2 * splits * count + 3) / 4 * 4 + splits * count * V : 0; };
@@ -491,25 +622,28 @@ static Plan plan_of(int rows, int seqs, int width, int page, int heads, int kv_h
 }
 
 template <typename act_t, int STORE, int NV> static int few_launch(const Attn& a, int tiles, cudaStream_t stream) {
-  using U = Unit<act_t, STORE>;
-  const size_t queries = (size_t)(sizeof(act_t) == 4 ? 3 : 1) * (a.K / 16) * 512, unit = U::bytes(a.K, a.V);
+  constexpr int ES = STORE == ACT ? (int)sizeof(act_t) : 1, PER = ES == 1 ? 4 : 2;
+  const size_t queries = (size_t)(sizeof(act_t) == 4 ? 3 : 1) * ((a.K / 16 + PER - 1) / PER * PER) * 512, unit = (size_t)(atoms_of(a.K, ES) + atoms_of(a.V, ES)) * ATOM;
+  // four warps and as many CTAs on an SM as leave each warp two units in its ring at least; fewer warps where one CTA does not fit
+  constexpr size_t SM = 227 * 1024, OTHER = 6 * 1024;        // static: barriers, scales; the system's 1 KB
   int W = 4, stages = 0;
-  for (size_t room : {(size_t)112 * 1024, (size_t)226 * 1024}) {      // two CTAs per SM, or one
-    for (W = 4; W >= 1 && stages == 0; W /= 2) {
-      if (room > 112 * 1024 || W == 4) {
-        const size_t n = room > queries ? (room - queries) / (W * unit) : 0;
-        stages = n >= 6 ? 6 : n >= 4 ? 4 : n >= 2 ? (int)n : 0;
-        if (stages) break;
-      }
+  for (int ctas = NV <= 8 ? 4 : 2; ctas >= 1 && stages < 2; --ctas)
+    for (W = 4; W >= (ctas == 1 ? 1 : 4); W /= 2) {
+      const size_t room = SM / ctas - OTHER;
+      stages = room > queries ? (int)std::min<size_t>(MOST_STAGES, (room - queries) / (W * unit)) : 0;
+      if (stages >= 2) break;
     }
-    if (stages) break;
-  }
-  B2L_CHECK_SUPPORTED(stages > 0, "b2l_seq_paged_attention: heads of %d and %d entries do not fit", a.K, a.V);
+  B2L_CHECK_SUPPORTED(stages >= 2, "b2l_seq_paged_attention: heads of %d and %d entries do not fit", a.K, a.V);
   const size_t smem = std::max(queries + W * stages * unit, (size_t)W * (32 + 16 * (a.V + 4)) * 4);
+  const CUtensorMapDataType type = ES == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : ES == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  const long long rows = ((long long)a.s.pages * a.kv_heads) << a.s.shift;
+  FewMaps maps;
+  if (int rc = tc::map_sw128(&maps.k, type, ES, a.k, rows, a.K, a.K, 128 / ES, 16)) return rc;
+  if (int rc = tc::map_sw128(&maps.v, type, ES, a.v, rows, a.V, a.V, 128 / ES, 16)) return rc;
   static DynSmemCache cache;
   auto kernel = paged_few_kernel<act_t, STORE, NV>;
   if (int rc = ensure_dyn_smem(kernel, smem, cache)) return rc;
-  kernel<<<dim3((unsigned)tiles, (unsigned)a.kv_heads, (unsigned)a.few.splits), 32 * W, smem, stream>>>(a, stages);
+  kernel<<<dim3((unsigned)tiles, (unsigned)a.kv_heads, (unsigned)a.few.splits), 32 * W, smem, stream>>>(a, maps, stages);
   B2L_LAUNCH_CHECK("paged_few_kernel");
   return 0;
 }
@@ -538,7 +672,8 @@ extern "C" int b2l_seq_paged_attention(const void* q, long long ldq, long long h
   B2L_CHECK_ARG(scale > 0.f && scale < INFINITY, "%s: the scale must be positive and finite", who);
   const int per = act_dtype == B2L_F32 ? 4 : 8;
   B2L_CHECK_ARG((((uintptr_t)q | (uintptr_t)out | (uintptr_t)work) & 15) == 0 && ldq % per == 0 && hsq % per == 0, "%s: rows must be 16-byte aligned", who);
-  B2L_CHECK_SUPPORTED((long long)width * page < (1ll << 30) && kv_heads < 65536 && (long long)rows * heads < (1ll << 31), "%s: sizes beyond the grid's", who);
+  B2L_CHECK_SUPPORTED((long long)width * page < (1ll << 30) && kv_heads < 65536 && (long long)rows * heads < (1ll << 31) && (long long)pages * kv_heads * page < (1ll << 31),
+                      "%s: sizes beyond the grid's or a copy's coordinates", who);
   if (rows == 0 || seqs == 0) return 0;
   const Plan p = plan_of(rows, seqs, width, page, heads, kv_heads, K, V, window, first, max_new, min_new, max_length, store, act_dtype);
   B2L_CHECK_ARG(p.floats == 0 || (work && work_floats >= p.floats), "%s: a work space of %lld floats is needed", who, p.floats);
@@ -572,9 +707,8 @@ extern "C" int b2l_seq_paged_attention(const void* q, long long ldq, long long h
   if (p.many)
     if (int rc = many_launch(a, p.many_tiles, st)) return rc;
   if (a.few.splits > 1 || a.many.splits > 1) {
-    const long long units = (long long)rows * heads;
-    const int warps = units >= 8 * 148 ? 8 : 1;
-    paged_merge_kernel<<<(unsigned)((units + warps - 1) / warps), 32 * warps, 0, st>>>(a);
+    const int most = std::max(a.few.splits, a.many.splits), per = most >= 32 ? 8 : most >= 16 ? 4 : most >= 8 ? 2 : 1, here = MERGE_WARPS / per;
+    paged_merge_kernel<<<(unsigned)(((long long)rows * heads + here - 1) / here), 32 * MERGE_WARPS, 0, st>>>(a, per);
     B2L_LAUNCH_CHECK("paged_merge_kernel");
   }
   return 0;

@@ -13,7 +13,7 @@
         out = caches[i].attend(q, step)                        # q [513, 32, 128] -> [513, 32, 128]
         pool.release("a")
 
-A token's key and value rows are quantised by themselves, per head: scale = max(max |x| / c, 2^-126), code = round(x / scale), c = 448 (fp8, e4m3) or 127
+A token's key and value rows are quantised by themselves, per head: scale = max(max |x| (1 / c), 2^-126), code = round(x / scale), c = 448 (fp8, e4m3) or 127
 (int8).  A row that holds an infinity or NaN reads back as NaN.  A row whose weights sum to zero (it sees no key) attends to zeros.  Everything
 is a kernel of libb200seq (include/b2l_seq.h); CUDA only, no CPU fallback, no derivatives."""
 from typing import Dict, Hashable, List, Optional, Sequence, Tuple

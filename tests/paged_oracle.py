@@ -11,7 +11,7 @@ def quantise(x, store):
     """(codes as the values they stand for without their scale, scales) of rows [..., size], each step rounded as f32 is."""
     x = x.float().cpu()
     c = LARGEST[store]
-    s = torch.maximum(x.abs().amax(-1) / c, torch.tensor(2.0 ** -126))
+    s = torch.maximum(x.abs().amax(-1) * torch.tensor(1.0 / c), torch.tensor(2.0 ** -126))      # 1 / c in f32
     bad = ~torch.isfinite(x).all(-1)
     s = torch.where(bad, torch.tensor(float("nan")), s)
     y = torch.where(bad[..., None], torch.zeros_like(x), x / s[..., None]).clamp(-c, c)
@@ -66,11 +66,13 @@ def attend(q, cache, sequences, scale, window=0, first=0):
     return out, mag, dots
 
 
-def tolerance(out, mag, dots, size, keys, f32):
+def tolerance(out, mag, dots, size, keys, f32, store):
     """How far an output may be off, entry by entry.  A score is a sum of `size` products in f32, each addition off by at most 2^-23 of the sum of absolute
-    values so far (the tensor core truncates): (size + 8) 2^-23 dots, with the scaling's, and as much again in the reference maximum; exp2 is off by 2^-22, a
-    weight's parts (bf16) by 2^-15; sums of weights and products by keys 2^-23 for every key, and the rounding of a bf16 output by 2^-8 of itself.  Second-order terms: a quarter more."""
-    weights = 2 * (size + 8) * 2.0 ** -23 * dots[..., None] + 2.0 ** -22 + (0 if f32 else 2.0 ** -15) + 2 * min(keys, 4096) * 2.0 ** -23
+    values so far (the tensor core truncates): (size + 8) 2^-23 dots, with the scaling's, and as much again in the reference maximum; exp2 is off by 2^-22.  Weights of bf16 activations: two
+    bf16 parts, the first truncated (2^-7 of the weight left), the second rounded (2^-8 of that): 2^-15; with codes one f16, eps / 2 = 2^-11, and the scale's
+    logarithm (2^-22 of at most 8) 2^-19.  Sums of weights and products by keys 2^-23 for every key, and the rounding of a bf16 output by 2^-8 of itself.
+    Second-order terms: a quarter more."""
+    weights = 2 * (size + 8) * 2.0 ** -23 * dots[..., None] + 2.0 ** -22 + (0 if f32 else 2.0 ** -15 if store == "act" else 2.0 ** -11 + 2.0 ** -19) + 2 * min(keys, 4096) * 2.0 ** -23
     return 1.25 * weights * mag + (2.0 ** -22 if f32 else 2.0 ** -8) * out.abs() + 1e-30
 
 

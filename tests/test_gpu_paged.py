@@ -42,7 +42,7 @@ def check(got, q, cache, seqs, scale, window=0, first=0):
     want, mag, dots = O.attend(q, cache, seqs, scale, window, first)
     f32 = q.dtype == torch.float32
     keys = max(m for _, m, _ in seqs)
-    tol = O.tolerance(want, mag, dots, cache.dim, keys, f32)
+    tol = O.tolerance(want, mag, dots, cache.dim, keys, f32, cache.store)
     off = (got.cpu().double() - want).abs()
     assert bool((off <= tol).all()), (float((off / tol).max()), float(off.max()))
     assert O.rel(got, want) < (3e-6 if f32 else 2.0 ** -8), O.rel(got, want)
@@ -247,7 +247,7 @@ def test_what_no_row_may_see(dtype, store, bad):
         want, mag, dots = O.attend(q, cache, seqs, 0.125, window, first)
         assert torch.isfinite(got[rest]).all() and not torch.isfinite(got[last]).any()
         assert torch.equal(got[last].isnan(), want[last].to(dtype).isnan())
-        tol = O.tolerance(want, mag, dots, 64, 5000, dtype == torch.float32)
+        tol = O.tolerance(want, mag, dots, 64, 5000, dtype == torch.float32, store)
         assert bool(((got.double() - want).abs() <= tol)[rest].all())
 
 
@@ -265,7 +265,7 @@ def test_scores_of_any_size(dtype):
     want, mag, dots = O.attend(q, cache, seqs, 0.25)
     assert torch.isfinite(got[:21]).all() and got[21].isnan().all() and want[21].isnan().all()
     dots = torch.full_like(dots, 20.0)                                    # of the keys that count
-    assert bool(((got.double() - want).abs() <= O.tolerance(want, mag, dots, 16, 40, dtype == torch.float32))[:21].all())
+    assert bool(((got.double() - want).abs() <= O.tolerance(want, mag, dots, 16, 40, dtype == torch.float32, "act"))[:21].all())
     for j in range(40):
         cache.k[seqs[0][2][j // 16], 0, j % 16, 0] = -math.inf
     assert (cache.attend(q.to(DEV), step)[0] == 0).all()
@@ -327,6 +327,36 @@ def test_pools_beyond_32_bit_offsets():
         assert torch.equal(got, small.attend(q.to(DEV), PagedStep.of(shifted, DEV)))
         check(got, q, small, shifted, 0.125)
         del cache
+
+
+@pytest.mark.parametrize("dtype,store", [t for t in TYPES if t[1] != "act"], ids=[i for t, i in zip(TYPES, IDS) if t[1] != "act"])
+def test_places_never_written_count_as_zeros(dtype, store):
+    """A pool begins as zeros with scales of zero: a row that sees such places weighs them with its score of zero, in units of their own and beside others."""
+    cache, step, seqs = make(dtype, store, 2, 64, 64, 16, [(1, 64), (20, 100), (1, 40)])
+    for _, length, pages in seqs:
+        for p in pages[:1] + pages[2:3]:
+            for t in (cache.k, cache.v):
+                t.view(torch.uint8)[p, :, 3:] = 0
+            for t in (cache.k_scale, cache.v_scale):
+                t[p, :, 3:] = 0
+    q = torch.randn(step.rows, 4, 64, generator=gen(4)).to(dtype)
+    check(cache.attend(q.to(DEV), step), q, cache, seqs, 0.125)
+
+
+@pytest.mark.parametrize("dtype,store", [t for t in TYPES if t[1] != "act"], ids=[i for t, i in zip(TYPES, IDS) if t[1] != "act"])
+@pytest.mark.parametrize("low,high", [(-126, -120), (-126, 0), (-100, -50), (-95, 90), (-70, 39), (30, 110)])
+def test_scales_of_any_size(dtype, store, low, high):
+    """Values whose scales are powers of two from one end of f32 to the other, small ones beside large ones."""
+    cache, step, seqs = make(dtype, store, 2, 64, 64, 16, [(1, 70), (20, 100), (1, 1)])
+    exponents = torch.randint(low, high + 1, cache.v_scale.shape, generator=gen(3))
+    cache.v_scale.copy_(torch.ldexp(torch.ones_like(exponents, dtype=torch.float64), exponents).float())
+    q = torch.randn(step.rows, 4, 64, generator=gen(4)).to(dtype)
+    got = cache.attend(q.to(DEV), step)
+    want, mag, dots = O.attend(q, cache, seqs, 0.125)
+    tol = O.tolerance(want, mag, dots, 64, 100, dtype == torch.float32, store)
+    # a score with the scale's logarithm is rounded at up to 128 (2^-18), and the logarithm is off by 2^-22 of up to 64
+    tol += 2.0 ** -15 * mag + 2.0 ** -126 + want.abs() * (want.abs() < 2.0 ** -118)      # subnormal results
+    assert bool(((got.cpu().double() - want).abs() <= tol).all())
 
 
 # ----------------------------------------------------------------------------- streams, graphs, runs
