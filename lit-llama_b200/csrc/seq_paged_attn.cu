@@ -12,7 +12,7 @@
 //   8-bit pool      a code is an f16 exactly (two codes an instruction; bf16 took four times as many), and so the queries: a row of them times the power of
 //                   two that brings its largest entry to 2^14 (an entry below 2^-28 of that keeps fewer than 8 bits, off by 2^-39 of it).  The scale of a
 //                   key goes into its score, the scale of a value into the exponent of its weight, w s = 2^(t + log2 s - m), m the largest t + log2 s so
-//                   far: in f16 with a factor of 2^14, off by 2^-11 of itself at most (2^-39 of the largest where it is small), and sum_j w_j adds w s / s
+//                   far (scales between 2^-60 and 2^40; a row that sees others is computed again): in f16 with a factor of 2^14, off by 2^-11 of itself at most (2^-39 of the largest where it is small), and sum_j w_j adds w s / s
 //   f32             three parts each (f32's 24 bits); of the nine products of two f32 operands the six above 2^-24.  They are added to f32 registers unit by
 //                   unit, because the tensor core truncates where it adds to its accumulator
 // With 8-bit codes a lane has four consecutive entries of a key as its share of a k16 step (queries laid out alike), and values are transposed as pairs
@@ -84,23 +84,6 @@ template <bool HALF, int PARTS> __device__ __forceinline__ void operand2(float x
   if constexpr (HALF) halves2<PARTS>(x, y, p);
   else parts2<PARTS>(x, y, p);
 }
-// Codes (bytes) A0, A1 and B0, B1 of w as two f16 pairs.  An int8 code x: 1024 + (x + 128) is an f16 with x + 128 in its low byte
-template <int STORE, int A0, int A1, int B0, int B1> __device__ __forceinline__ uint2 codes4(uint32_t w) {
-  uint2 y;
-  if constexpr (STORE == E4M3) {
-    if constexpr (A0 != 0 || A1 != 1 || B0 != 2 || B1 != 3) w = __byte_perm(w, 0u, A0 | A1 << 4 | B0 << 8 | B1 << 12);
-    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3), b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
-    y.x = (uint32_t)a.x | (uint32_t)a.y << 16;
-    y.y = (uint32_t)b.x | (uint32_t)b.y << 16;
-  } else {
-    const uint32_t u = w ^ 0x80808080u, off = 0x64806480u;   // 1152 twice
-    y.x = __byte_perm(u, 0x64646464u, A0 | 0x40 | A1 << 8 | 0x4000);
-    y.y = __byte_perm(u, 0x64646464u, B0 | 0x40 | B1 << 8 | 0x4000);
-    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(y.x) : "r"(off));
-    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(y.y) : "r"(off));
-  }
-  return y;
-}
 // of nine products of three parts (index 0 the largest) the six above 2^-24, the smallest first
 __device__ constexpr int PART_A[6] = {2, 1, 0, 1, 0, 0}, PART_B[6] = {0, 1, 2, 0, 1, 0};
 
@@ -123,7 +106,6 @@ __device__ __forceinline__ void product(float (&c)[4], const uint32_t (&a)[AP][4
 // ------------------------------------------------------------------------------------------------ 16 rows
 constexpr int ATOM = 2048;           // 16 rows of 128 bytes, as a swizzled tiled copy leaves them: 16-byte piece c of row r at piece c ^ (r & 7)
 constexpr int MOST_STAGES = 8;
-__host__ __device__ inline int atoms_of(int D, int es) { return (D * es + 127) / 128; }
 
 struct FewMaps { CUtensorMap k, v; };
 
@@ -134,10 +116,6 @@ __global__ void __launch_bounds__(128, NV <= 8 ? 3 : 2) paged_few_kernel(const _
   constexpr int QP = F32 ? 3 : 1, KP = F32 && !HALF ? 3 : 1, WP = F32 ? 3 : HALF ? 1 : 2, PRODUCTS = KP == 3 ? 6 : QP, V_PRODUCTS = KP == 3 ? 6 : WP;
   constexpr int PER = ES == 1 ? 4 : 2;                       // k16 steps in the 64 bytes of a key that one ldmatrix takes
   constexpr float LIFT = HALF ? 14.f : 0.f;                  // weights up to 2^14 in f16
-  // Scales below 2^-60 (rows of zeros have 2^-126, places never written 0) go into the exponent as 2^-60, and with one above 2^40 (values beyond 10^14) the row
-  // is computed again: so no weight above 2^-40 of the largest is lost from the sum, at either end of f32
-  constexpr int SMALL = -60;
-  constexpr float SMALLEST = 8.673617379884035e-19f, LARGEST = 1.099511627776e12f;
   extern __shared__ __align__(1024) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5, g = lane >> 2, t = lane & 3;
   const int h = blockIdx.y, split = blockIdx.z, G = a.heads / a.kv_heads, steps = (a.K / 16 + PER - 1) / PER * PER;
@@ -205,10 +183,7 @@ __global__ void __launch_bounds__(128, NV <= 8 ? 3 : 2) paged_few_kernel(const _
         for (int d = lane; d < a.K; d += 32) top = fmaxf(top, fabsf(ld_act(reinterpret_cast<const act_t*>(a.q), (pl.start + at / G) * a.ldq + (h * G + at % G) * a.hsq + d)));
       top = warp_max(top);
       if (lane == 0) {
-        // exponents of 2^14 / top's: within f32's normal range for every top, 0 for a top of 0
-        const int e = (int)(__float_as_uint(top) >> 23) - 127, up = top > 0.f && top < INFINITY ? min(14 - e, 120) : 0;
-        lifted[0][r] = __uint_as_float((uint32_t)(up + 127) << 23);
-        lifted[1][r] = a.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
+        lift_of(top, a.scale_log2, lifted[0][r], lifted[1][r]);
       }
     }
     __syncthreads();
@@ -326,7 +301,7 @@ __global__ void __launch_bounds__(128, NV <= 8 ? 3 : 2) paged_few_kernel(const _
     // scores in powers of two; lane: keys 8 n + 2 t, + 1 of rows g (entries 0, 1) and g + 8 (2, 3)
     float top[2] = {-INFINITY, -INFINITY}, over[2][2], rest[2][2];      // one over what of the values' scales is in the exponent; what is not
     const bool whole = ks.whole(key0, 16);
-    bool small = false;
+    bool zeros = false;                                      // whether a value counts as zeros
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       float c[2] = {1.f, 1.f}, add[2] = {0.f, 0.f};
@@ -337,19 +312,20 @@ __global__ void __launch_bounds__(128, NV <= 8 ? 3 : 2) paged_few_kernel(const _
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float v = __uint_as_float(e ? y.y : y.x);
-          if (F32) {                                         // the power of two: exact; NaN, the sign and what is left of a small scale stay in the rest
-            const int exponent = max((int)(__float_as_uint(v) >> 23 & 255u), 127 + SMALL);
+          const bool zero = v >= 0.f && v <= 1.17549435e-38f;      // 2^-126 (a row of zeros) or 0 (never written): counts as zeros
+          const float some = zero ? SMALLEST_SCALE : v;
+          if (F32) {                                         // the power of two: exact; the rest of it goes with the weight
+            const int exponent = (int)(__float_as_uint(some) >> 23 & 255u);
             add[e] = (float)(exponent - 127);
             over[n][e] = __uint_as_float((uint32_t)(254 - exponent) << 23);
-            rest[n][e] = v * over[n][e];
-          } else {                                           // all of it, to 2^-22 (of log2 s where that is larger than 1), unless it is small
-            const float some = v < SMALLEST ? SMALLEST : v;
-            small |= v < SMALLEST;
+            rest[n][e] = zero ? 0.f : v * over[n][e];
+          } else {                                           // all of it, to 2^-22 (of log2 s where that is larger than 1)
             asm("lg2.approx.f32 %0, %1;" : "=f"(add[e]) : "f"(some));
             asm("rcp.approx.f32 %0, %1;" : "=f"(over[n][e]) : "f"(some));
-            rest[n][e] = v < SMALLEST ? v * over[n][e] : 1.f;
+            rest[n][e] = zero ? 0.f : 1.f;
+            zeros |= zero;
           }
-          if (v > LARGEST) over[n][e] = NAN;
+          if (!(some >= SMALLEST_SCALE && some <= LARGEST_SCALE)) over[n][e] = NAN;
         }
       }
 #pragma unroll
@@ -381,7 +357,7 @@ __global__ void __launch_bounds__(128, NV <= 8 ? 3 : 2) paged_few_kernel(const _
         o[x][3] *= f[1];
       }
     }
-    if (HALF && !F32) small = __any_sync(0xffffffffu, small);
+    if (HALF && !F32) zeros = __any_sync(0xffffffffu, zeros);
     uint32_t wa[WP][4];                                      // the weights as the A operand of the second product
 #pragma unroll
     for (int n = 0; n < 2; ++n)
@@ -395,7 +371,7 @@ __global__ void __launch_bounds__(128, NV <= 8 ? 3 : 2) paged_few_kernel(const _
           x[e] = exp2_f(F32 ? (z - m[r]) + LIFT : z - (m[r] - LIFT));
           if (z == -INFINITY) x[e] = 0.f;                    // hidden, or of no weight: whatever its scale is, and while the maximum is -inf
           else l[r] = HALF ? fmaf(x[e], over[n][e], l[r]) : l[r] + x[e];
-          if (HALF && (F32 || small)) x[e] = z == -INFINITY ? 0.f : x[e] * rest[n][e];
+          if (HALF && (F32 || zeros)) x[e] = z == -INFINITY ? 0.f : x[e] * rest[n][e];
         }
         operand2<HALF, WP>(x[0], x[1], w);
 #pragma unroll
@@ -602,7 +578,7 @@ static Plan plan_of(int rows, int seqs, int width, int page, int heads, int kv_h
   p.compact = p.few && p.many;
   const int most = std::min(seqs, rows);
   p.few_tiles = p.compact ? most : (int)std::min<long long>(packed / 16 + most, INT32_MAX);
-  p.many_tiles = (int)std::min<long long>(packed / 128 + most, INT32_MAX);
+  p.many_tiles = (int)std::min<long long>(packed / 256 + most, INT32_MAX);
   long long keys = (long long)width * page;                  // the most keys that a row sees
   if (max_length > 0) keys = std::min<long long>(keys, max_length);
   if (window > 0) keys = std::min<long long>(keys, (long long)window + first + 16);

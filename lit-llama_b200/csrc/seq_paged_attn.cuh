@@ -12,6 +12,35 @@ __device__ __forceinline__ float exp2_f(float x) {
   return y;
 }
 
+__host__ __device__ inline int atoms_of(int D, int es) { return (D * es + 127) / 128; }      // 128-byte columns of a row
+
+// Scales of values that go into exponents.  A smaller one (of a row of zeros it is 2^-126, of a place never written 0; others are of values below
+// 2^-51) or a larger one (values beyond 10^14) makes the row be computed again: so no weight above 2^-40 of the largest is lost from the sum.
+constexpr float SMALLEST_SCALE = 8.673617379884035e-19f, LARGEST_SCALE = 1.099511627776e12f;      // 2^-60, 2^40
+
+// The power of two that brings a row's largest entry to 2^14 (1 for a row of zeros or with an infinity), and what its scores are multiplied with then
+__device__ __forceinline__ void lift_of(float top, float scale_log2, float& up, float& down) {
+  const int e = (int)(__float_as_uint(top) >> 23) - 127, by = top > 0.f && top < INFINITY ? min(14 - e, 120) : 0;
+  up = __uint_as_float((uint32_t)(by + 127) << 23);
+  down = scale_log2 * __uint_as_float((uint32_t)(127 - by) << 23);
+}
+
+// Codes (bytes) A0, A1 and B0, B1 of w as two f16 pairs.  An int8 code x: 1024 + (x + 128) is an f16 with x + 128 in its low byte
+template <int STORE, int A0, int A1, int B0, int B1> __device__ __forceinline__ uint2 codes4(uint32_t w) {
+  uint2 y;
+  if constexpr (STORE == E4M3) {
+    if constexpr (A0 != 0 || A1 != 1 || B0 != 2 || B1 != 3) w = __byte_perm(w, 0u, A0 | A1 << 4 | B0 << 8 | B1 << 12);
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(y.x), "=r"(y.y) : "r"(w));
+  } else {
+    const uint32_t u = w ^ 0x80808080u, off = 0x64806480u;   // 1152 twice
+    y.x = __byte_perm(u, 0x64646464u, A0 | 0x40 | A1 << 8 | 0x4000);
+    y.y = __byte_perm(u, 0x64646464u, B0 | 0x40 | B1 << 8 | 0x4000);
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(y.x) : "r"(off));
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(y.y) : "r"(off));
+  }
+  return y;
+}
+
 // packed rows first .. of sequence b, which has n new tokens from row `start` on and is `length` tokens long with them
 struct Place { int b, start, n, length, first; };
 
