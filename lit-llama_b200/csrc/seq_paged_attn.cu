@@ -20,6 +20,7 @@
 //
 // What bounds it: one pass over the keys and values that the rows see, at HBM's rate, for the rows of a token; 16 rows of f32 are bound by their six products.
 #include <algorithm>
+#include <cmath>
 
 #include "seq_paged_attn.cuh"
 #include "tc_common.cuh"
@@ -486,18 +487,31 @@ __global__ void __launch_bounds__(128, NV <= 8 ? 3 : 2) paged_few_kernel(const _
 
 // ------------------------------------------------------------------------------------------------ joining parts
 // `per` warps (a power of two) have a row and head, each every per-th part; rows of sequences whose parts were not split are in place already.  Parts are
-// read once, and the loads of a warp's parts do not wait for one another.
+// read once, and the loads of a warp's parts do not wait for one another.  `short_only`: only the few-row kernel's sequences have parts, and a unit is one of
+// the 16 packed rows of each of them and a key/value head.
 constexpr int MERGE_WARPS = 8;
-__global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const __grid_constant__ Attn a, int per) {
+__global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const __grid_constant__ Attn a, int per, int short_only) {
   __shared__ float4 sx[MERGE_WARPS][64];
   __shared__ float2 sml[MERGE_WARPS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, G = a.heads / a.kv_heads;
   const int here = MERGE_WARPS / per, sub = warp / here, own = warp % here;      // part of the unit's warps, unit of the block
   const long long unit = (long long)blockIdx.x * here + own;
-  const int row = (int)min(unit / a.heads, (long long)a.s.rows), head = (int)(unit % a.heads), h = head / G;
-  const int b = row < a.s.rows ? sequence_of(a.s, row, lane) : -1;
-  int start = 0, n = 0, length = 0;
-  if (b >= 0) sequence(a.s, b, start, n, length);
+  int row, head, b = -1, start = 0, n = 0, length = 0;
+  if (short_only) {
+    const int r = (int)(unit % 16), h = (int)(unit / 16 % a.kv_heads), at = (int)(unit / 16 / a.kv_heads);
+    if (at < a.s.seqs) {
+      sequence(a.s, at, start, n, length);
+      if (r < (long long)n * G && (long long)n * G <= a.few_max) b = at;
+    }
+    row = start + r / G;
+    head = h * G + r % G;
+  } else {
+    row = (int)min(unit / a.heads, (long long)a.s.rows);
+    head = (int)(unit % a.heads);
+    if (row < a.s.rows) b = sequence_of(a.s, row, lane);
+    if (b >= 0) sequence(a.s, b, start, n, length);
+  }
+  const int h = head / G;
   const bool few = (long long)n * G <= a.few_max;
   const Parts& p = few ? a.few : a.many;
   const bool on = b >= 0 && p.splits > 1;
@@ -592,6 +606,19 @@ static Plan plan_of(int rows, int seqs, int width, int page, int heads, int kv_h
     const long long want = 2 * ctas <= slots ? slots / ctas : (4 * slots + ctas - 1) / ctas;
     p.few_splits = (int)std::max<long long>(1, std::min({want, keys / 256, 128ll, MOST_WORK / (p.few_count * (V + 2) + 1)}));
   }
+  if (p.many) {
+    // One CTA on an SM at a time, 2.3 us for 128 keys: as many parts as make the rounds shortest, where the last one is seldom full.  A part's results are
+    // written and read at some 4 TB/s, and joining them costs a launch.
+    const double ctas = (double)kv_heads * std::max<long long>(1, (packed + 255) / 256), tiles = (keys + 127) / 128, results = 8.0 * p.many_count * V / 4e6;      // us
+    double least = 0;
+    for (int s = 1; s <= 16 && s <= tiles && (s == 1 || (long long)s * p.many_count * (V + 2) <= MOST_WORK); ++s) {
+      const double us = std::ceil(ctas * s / sms) * std::ceil(tiles / s) * 2.3 + std::ceil(ctas * s / sms) * 6 + (s > 1 ? 4 + s * results : 0);
+      if (s == 1 || us < 0.95 * least) {
+        least = us;
+        p.many_splits = s;
+      }
+    }
+  }
   auto floats = [&](int splits, long long count) { return splits > 1 ? (2 * splits * count + 3) / 4 * 4 + splits * count * V : 0; };
   p.floats = (p.few ? floats(p.few_splits, p.few_count) : 0) + (p.many ? floats(p.many_splits, p.many_count) : 0);
   return p;
@@ -684,7 +711,10 @@ extern "C" int b2l_seq_paged_attention(const void* q, long long ldq, long long h
     if (int rc = many_launch(a, p.many_tiles, st)) return rc;
   if (a.few.splits > 1 || a.many.splits > 1) {
     const int most = std::max(a.few.splits, a.many.splits), per = most >= 32 ? 8 : most >= 16 ? 4 : most >= 8 ? 2 : 1, here = MERGE_WARPS / per;
-    paged_merge_kernel<<<(unsigned)(((long long)rows * heads + here - 1) / here), 32 * MERGE_WARPS, 0, st>>>(a, per);
+    const bool short_only = p.compact && a.many.splits == 1;
+    const long long units = short_only ? 16ll * kv_heads * seqs : (long long)rows * heads;
+    B2L_CHECK_SUPPORTED(units < (1ll << 31), "%s: sizes beyond the grid's", who);
+    paged_merge_kernel<<<(unsigned)((units + here - 1) / here), 32 * MERGE_WARPS, 0, st>>>(a, per, short_only);
     B2L_LAUNCH_CHECK("paged_merge_kernel");
   }
   return 0;

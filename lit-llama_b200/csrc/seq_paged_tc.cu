@@ -125,6 +125,10 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
   __syncthreads();
   fence_after();
   const uint32_t tmem = ct.tmem;
+  // 8-bit pool: 512 threads of 128 registers; a tile's codes, loaded a tile ahead, take 80 of the last warpgroup's, and what the first does not need
+  // (64 x 128 + 128 x 256 + 184 x 128 <= 128 x 512)
+  if (HALF && warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+  if (HALF && warp >= 12) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
 
   if (warp == 0) {
     // ===================== MMA issue =====================
@@ -274,7 +278,8 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
       auto fetch = [&](const void* pool, int D, int pieces, int by, int i) {
         const int x = i * 128 + me, key = x * by >> 16, c = x - key * pieces;
         const long long row = row_of(key);
-        return row >= 0 ? *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(pool) + row * D + c * 16) : make_uint4(0u, 0u, 0u, 0u);
+        const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(pool) + max(row, 0ll) * D + c * 16);
+        return row >= 0 ? w : make_uint4(0u, 0u, 0u, 0u);
       };
       auto put = [&](uint32_t base, int pieces, int by, int i, uint4 w, bool zero) {
         const int x = i * 128 + me, key = x * by >> 16, c = x - key * pieces;
