@@ -4,50 +4,67 @@
 // turn the first one's scores into weights, a thread per row (tensor-memory lane), so no row needs another thread's maximum or sum.
 //
 //   warp 0        issues the MMAs: for a tile of keys t and each row tile, P(t) V, then Q K^T of t + 1 (one commit tells that the scores are there and
-//                 that the output may be touched)
-//   warp 1        bf16 pool: tiled copies of pages, 64 columns each, into 128-byte swizzled rows (keys K-major, values MN-major)
-//   warps 4..11   softmax of row tile 0 (4..7) and 1 (8..11): scores from tensor memory twice, once for the maximum and once for the weights, which go
-//                 back over them in two halves, so the second product begins with the first 64 keys.  A row's reference moves only when it is exceeded
-//                 by more than 8 (weights reach 2^8; nothing is rounded by that), so the output in tensor memory is seldom scaled
-//   warps 12..15  8-bit pool: codes by 16-byte loads a tile ahead, as f16 (exactly) into the same rows, and the tile's scales
+//                 that the output may be touched).  The other row tile's products fill the time of this one's softmax.  (Two issuing warps fell into step:
+//                 both softmaxes at once, then the products, 4300 cycles for a tile; units of 64 keys with two places for their scores took 4160, as an MMA
+//                 of N = 64 takes 75 cycles and one of N = 128 103: its rows of A come out of shared memory for half as many keys.)
+//   warp 1        tiled copies of pages: bf16, 64 columns each, into 128-byte swizzled rows (keys K-major, values MN-major); codes as they lie, with their
+//                 scales, for warps 12..15
+//   warps 4..11   softmax of row tile 0 (4..7) and 1 (8..11): the second half of a row's scores stays in registers from the maximum to the weights, the first is
+//                 read twice; the weights go back over them half by half, and the second product begins with the first half that is there.  A row's reference moves only when it is exceeded by
+//                 more than 8 (weights reach 2^8; nothing is rounded by that), so the output in tensor memory is seldom scaled.  Of four powers of two the
+//                 special function unit computes three; the fourth is a polynomial, or that unit would take as long as the products
+//   warps 12..15  8-bit pool: codes as f16 into the same rows: keys exactly, values times their scale
 //
 // Weights are rounded to one bf16 (by half a step, 2^-8; with 8-bit pools one f16, 2^-11): the first rounding below f32 in the sums, and the price of one
-// product instead of two; outputs in bf16 are off by as much themselves.  8-bit pools: queries as f16 times a power of two per row, the scale of a value in
-// the exponent of its weight, as the few-row kernel has them.
+// product instead of two; outputs in bf16 are off by as much themselves.
+// 8-bit pools: queries as f16 times a power of two per row, the scale of a key goes into its score.  The scale of a value s goes into its codes, code times
+// s 2^e rounded to f16 (2^-11), e such that the largest s of the CTA's first tile comes to 1 .. 2, and the outputs times 2^-e.  A row that sees a scale above
+// 2^7 or below 2^-16 of that, or a scale that is not finite, is computed again.
 //
 // Tensor memory: scores and weights of the row tiles at columns 0 and 128, outputs at 256 and 384.  Shared memory: the queries of both, two stages of keys
-// and values where they fit.  One CTA per SM.
+// and values where they fit (8-bit: of values, and a tile of codes).  One CTA per SM.
 #include <utility>
 
+#include "attn_tc.cuh"
 #include "seq_paged_attn.cuh"
-#include "tc_common.cuh"
 
 namespace b2l {
 namespace paged {
 
 using namespace tc;
+using atc::add2;
+using atc::desc_mn;
+using atc::fma2;
+using atc::mma_ss;
 
 constexpr int KEYS = 128, TILE = 128, ROWS = 2 * TILE, MOST_K = 192, MOST_V = 128;
 constexpr int TC_ATOM = 128 * 128;                           // bytes of 64 columns of 128 rows
 constexpr int INFOS = 4;
 
 struct alignas(16) Info {                                    // of a tile of keys, for the softmax (read by 16 bytes)
-  float ks[KEYS], add[KEYS], over[KEYS];                     // scale of the key, log2 of the value's, one over it (8-bit pools)
-  uint32_t there, zero[KEYS / 32];                           // 16 keys each: whether their page is there; keys whose values count as zeros
+  float ks[KEYS];                                            // scale of the key, NaN where the row is to be computed again (8-bit pools)
+  uint32_t there;                                            // 16 keys each: whether their page is there
 };
 struct Control {
   uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_half[2][2], o_done[2], info_full[INFOS], tail, gave_up;
-  uint32_t tmem;
+  uint64_t ref_full, rk_full, rk_empty, rv_full, rv_empty;   // 8-bit pools: the first tile's largest scale, codes of keys and values
+  uint32_t tmem, ref;                                        // ref: largest scale of the first tile's values, as bits
+};
+struct Codes {                                               // 8-bit pools: what lies beside a tile's codes
+  float ks[KEYS], vs[KEYS];                                  // scales
+  uint2 by[2][KEYS];                                         // what a value's codes are multiplied with (two tiles: one may still be read)
 };
 constexpr size_t CONTROL_BYTES = 1024;
-template <int STORE> constexpr size_t INFO_BYTES = STORE == ACT ? 1024 : (INFOS * sizeof(Info) + 1023) / 1024 * 1024;
+template <int STORE> constexpr size_t INFO_BYTES = STORE == ACT ? 1024 : (INFOS * sizeof(Info) + sizeof(Codes) + 1023) / 1024 * 1024;
 static_assert(sizeof(Control) <= CONTROL_BYTES && sizeof(Info) % 16 == 0);
 
 struct Layout { int ks, vs; size_t smem; };                  // stages of keys and values; none: the sizes do not fit
 template <int STORE> static Layout layout(int K, int V) {
-  const size_t base = CONTROL_BYTES + INFO_BYTES<STORE>, ka = atoms_of(K, 2), va = atoms_of(V, 2), q = 2 * ka * TC_ATOM, room = 227 * 1024;
+  const size_t base = CONTROL_BYTES + INFO_BYTES<STORE> + (STORE == ACT ? 0 : KEYS * (K + V)), ka = atoms_of(K, 2), va = atoms_of(V, 2), q = 2 * ka * TC_ATOM, room = 227 * 1024;
   Layout l{0, 0, 0};
-  for (const auto& [ks, vs] : {std::pair<int, int>{2, 2}, {2, 1}, {1, 1}})
+  // codes: keys become f16 while the tile before is in the softmax, values in a hurry
+  const std::pair<int, int> stages[4] = {{2, 2}, STORE == ACT ? std::pair<int, int>{2, 1} : std::pair<int, int>{1, 2}, {1, 1}, {1, 1}};
+  for (const auto& [ks, vs] : stages)
     if (base + q + (ks * ka + vs * va) * TC_ATOM <= room) {
       l = {ks, vs, base + q + (ks * ka + vs * va) * TC_ATOM};
       break;
@@ -56,28 +73,83 @@ template <int STORE> static Layout layout(int K, int V) {
   return l;
 }
 
-__device__ __forceinline__ void tmem_ld32(uint32_t a, uint32_t (&r)[32]) {
+// 64 consecutive 32-bit columns of this warp's 32 tensor-memory lanes
+__device__ __forceinline__ void tmem_ld64(uint32_t a, uint32_t* r) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
-      "%28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
-        "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]),
+        "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]),
+        "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]),
+        "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
       : "r"(a)
       : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t lead) {
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-               "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
-               : "memory");
+// The largest of three, NaN if one is
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(x), "f"(y), "f"(z));
+  return m;
 }
-// MN-major operand, 128-byte swizzle: rows of 64 consecutive MN entries, one row per k; `lbo` bytes to the next 64 entries
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t lbo) {
-  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+__device__ __forceinline__ void mul2(float& a, float& b, float c, float d) {      // a *= c, b *= d
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}" : "+f"(a), "+f"(b) : "f"(c), "f"(d));
+}
+__device__ __forceinline__ void fma2v(float& a, float& b, float x, float y, float c) {      // a = a x + c, b = b y + c
+  asm("{\n\t.reg .b64 u, v, w;\n\tmov.b64 u, {%0, %1};\n\tmov.b64 v, {%2, %3};\n\tmov.b64 w, {%4, %4};\n\tfma.rn.f32x2 u, u, v, w;\n\tmov.b64 {%0, %1}, u;\n\t}"
+      : "+f"(a), "+f"(b) : "f"(x), "f"(y), "f"(c));
+}
+// Two powers of two on the FMA pipe: 2^n times a polynomial in the rest, |rest| <= 1/2 (fitted to the least largest relative error, 2^-13.3, with p(0) = 1; exact
+// zero from -127 on down, as n = -127 then takes all of 1's exponent).  No NaN, none above 127.
+__device__ __forceinline__ void exp2_poly2(float& x, float& y) {
+  constexpr float MAGIC = 12582912.f;                        // 1.5 2^23: adding it rounds to an integer in the low bits
+  x = fmaxf(x, -127.f);
+  y = fmaxf(y, -127.f);
+  float nx = x, ny = y;
+  add2(nx, ny, MAGIC, MAGIC);
+  float rx = nx, ry = ny;
+  add2(rx, ry, -MAGIC, -MAGIC);
+  atc::sub2(x, y, rx, ry);
+  float px = x, py = y;
+  fma2(px, py, 0.055008940398693085f, 0.2422109991312027f, 0.2422109991312027f);
+  fma2v(px, py, x, y, 0.6932829022407532f);
+  fma2v(px, py, x, y, 1.f);
+  x = __uint_as_float(__float_as_uint(px) + (__float_as_uint(nx) << 23));
+  y = __uint_as_float(__float_as_uint(py) + (__float_as_uint(ny) << 23));
 }
 __device__ __forceinline__ void st128(uint32_t a, uint4 v) { asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory"); }
-__device__ __forceinline__ float4 ldf4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+// A warp that issues waits and commits by its leading lane alone, without a branch: 32 lanes at a barrier that is complete took 150 cycles, a branch around a
+// commit some 100
+__device__ __forceinline__ void wait_lead(uint32_t a, uint32_t parity, uint32_t lead, uint32_t& dead) {
+  if (dead) return;
+  for (uint32_t tries = 0; tries < (1u << 22); ++tries) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %3, 0;\n\tsetp.ne.b32 p, 0, 0;\n\t@q mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(a), "r"(parity), "r"(lead)
+        : "memory");
+    if (__any_sync(0xffffffffu, ok)) return;
+  }
+  dead = 1u;
+}
+__device__ __forceinline__ void commit_by(uint32_t lead, uint32_t mbar) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(mbar), "r"(lead) : "memory");
+}
+// two codes (f16) times a factor of 1 .. 2 in two parts, rounded once, times a power of two
+__device__ __forceinline__ uint32_t scaled(uint32_t u, uint32_t hi, uint32_t lo, uint32_t power) {
+  uint32_t y;
+  asm("{\n\t.reg .b32 x;\n\tmul.rn.f16x2 x, %1, %3;\n\tfma.rn.f16x2 x, %1, %2, x;\n\tmul.rn.f16x2 %0, x, %4;\n\t}" : "=r"(y) : "r"(u), "r"(hi), "r"(lo), "r"(power));
+  return y;
+}
+__device__ __forceinline__ void bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t mbar) {      // multiples of 16 bytes
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(mbar) : "memory");
+}
+// the power of two that brings a largest scale (as bits; 0: none) to 1 .. 2
+__device__ __forceinline__ float value_lift(uint32_t bits) { return bits ? __uint_as_float((254u - (bits >> 23)) << 23) : 1.f; }
 // bits 0 .. n-1 (any n)
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 // place of the 16-byte piece c of row r in tiles of 128 rows
@@ -87,7 +159,7 @@ template <int STORE>
 __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel(const __grid_constant__ Attn a, const __grid_constant__ CUtensorMap map_k,
                                                                                   const __grid_constant__ CUtensorMap map_v, int k_stages, int v_stages) {
   constexpr bool HALF = STORE != ACT;
-  constexpr float LIFT = HALF ? 6.f : 0.f;                   // weights up to 2^8 times this in f16
+  constexpr float LIFT = HALF ? 6.f : 0.f;                   // weights up to 2^14 in f16
   extern __shared__ __align__(1024) uint8_t smem[];
   Control& ct = *reinterpret_cast<Control*>(smem);
   Info* infos = reinterpret_cast<Info*>(smem + CONTROL_BYTES);      // ACT: only `there`, at uint32_t steps
@@ -101,6 +173,8 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
   const int t0 = min(split * per, all), n = min(t0 + per, all) - t0;
   const int ka = atoms_of(a.K, 2), va = atoms_of(a.V, 2);
   const uint32_t sq = smem_u32(smem) + CONTROL_BYTES + INFO_BYTES<STORE>, sk = sq + 2 * ka * TC_ATOM, sv = sk + k_stages * ka * TC_ATOM;
+  const uint32_t raw_k = sv + v_stages * va * TC_ATOM, raw_v = raw_k + KEYS * a.K;      // 8-bit pools
+  Codes& codes = *reinterpret_cast<Codes*>(smem + CONTROL_BYTES + INFOS * sizeof(Info));
   auto bar = [&](const uint64_t& b) { return smem_u32(&b); };
   uint32_t dead = (sq & 1023u) ? 1u : 0u;
   if (tid == 0) {
@@ -115,9 +189,15 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
       mbar_init(bar(ct.p_half[i][1]), 4);
       mbar_init(bar(ct.o_done[i]), 1);
     }
-    for (int i = 0; i < INFOS; ++i) mbar_init(bar(ct.info_full[i]), HALF ? 128 : 1);
-    mbar_init(bar(ct.tail), 1);
     mbar_init(bar(ct.gave_up), 1);
+    for (int i = 0; i < INFOS; ++i) mbar_init(bar(ct.info_full[i]), HALF ? 129 : 1);
+    mbar_init(bar(ct.tail), 1);
+    mbar_init(bar(ct.ref_full), 128);
+    mbar_init(bar(ct.rk_full), 1);
+    mbar_init(bar(ct.rv_full), 1);
+    mbar_init(bar(ct.rk_empty), 128);
+    mbar_init(bar(ct.rv_empty), 128);
+    ct.ref = 0u;
     mbar_init_fence();
   }
   if (warp == 0) tmem_alloc(smem_u32(&ct.tmem), 512);
@@ -125,11 +205,6 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
   __syncthreads();
   fence_after();
   const uint32_t tmem = ct.tmem;
-  // 8-bit pool: 512 threads of 128 registers; a tile's codes, loaded a tile ahead, take 80 of the last warpgroup's, and what the first does not need
-  // (64 x 128 + 128 x 256 + 184 x 128 <= 128 x 512)
-  if (HALF && warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-  if (HALF && warp >= 12) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
-
   if (warp == 0) {
     // ===================== MMA issue =====================
     const uint32_t lead = elect_lane();
@@ -137,72 +212,61 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
     const uint32_t id_s = (1u << 4) | types | ((uint32_t)(KEYS >> 3) << 17) | ((uint32_t)(TILE >> 4) << 24);
     const uint32_t id_o = (1u << 4) | types | (1u << 16) | ((uint32_t)(a.V >> 3) << 17) | ((uint32_t)(TILE >> 4) << 24);
     const int steps = a.K / 16;
-    auto scores = [&](int g, int st) {
-      uint32_t d = tmem + 128 * g;
-#pragma unroll 1
-      for (int x = 0; 4 * x < steps; ++x) {
-        const uint64_t qd = desc_sw128(sq + (g * ka + x) * TC_ATOM), kd = desc_sw128(sk + (st * ka + x) * TC_ATOM);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (4 * x + k < steps) mma_ss(d, qd + 2 * k, kd + 2 * k, id_s, x + k > 0 ? 1u : 0u, lead);
-      }
-    };
-    auto outputs = [&](int g, int half, int st, bool first) {
-      const uint64_t vd = desc_mn(sv + st * va * TC_ATOM + half * (TC_ATOM / 2), TC_ATOM);
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        mma_ts(tmem + 256 + 128 * g, tmem + 128 * g + 32 * half + 8 * k, vd + k * (16 * 128 / 16), id_o, first && half == 0 && k == 0 ? 0u : 1u, lead);
-    };
     int kst = 0, vst = 0;
     uint32_t kph = 0, vph = 0;
-    if (n > 0) {
-      mbar_wait(bar(ct.q_full), 0, dead);
-      mbar_wait_warp(bar(ct.k_full[0]), 0, dead);
-      fence_after();
-      for (int g = 0; g < groups && !dead; ++g) {
-        scores(g, 0);
-        if (lead) commit(bar(ct.s_full[g]));
+    auto scores = [&](int g) {
+#pragma unroll 1
+      for (int x = 0; 4 * x < steps; ++x) {
+        const uint64_t qd = desc_sw128(sq + (g * ka + x) * TC_ATOM), kd = desc_sw128(sk + (kst * ka + x) * TC_ATOM);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (4 * x + k < steps) mma_ss(tmem + 128 * g, qd + 2 * k, kd + 2 * k, id_s, x + k > 0 ? 1u : 0u, lead);
       }
-      if (!dead && lead) commit(bar(ct.k_empty[0]));
-      if (++kst == k_stages) { kst = 0; kph ^= 1u; }
+      commit_by(lead, bar(ct.s_full[g]));
+      if (g == groups - 1) {
+        commit_by(lead, bar(ct.k_empty[kst]));
+        if (++kst == k_stages) { kst = 0; kph ^= 1u; }
+      }
+    };
+    if (n > 0) {
+      wait_lead(bar(ct.q_full), 0, lead, dead);
+      wait_lead(bar(ct.k_full[0]), 0, lead, dead);
+      fence_after();
+      for (int g = 0; g < groups && !dead; ++g) scores(g);
     }
     for (int t = 0; t < n && !dead; ++t) {
-      const bool more = t + 1 < n;
-      mbar_wait_warp(bar(ct.v_full[vst]), vph, dead);
-      for (int g = 0; g < groups && !dead; ++g) {
+      wait_lead(bar(ct.v_full[vst]), vph, lead, dead);
 #pragma unroll 1
-        for (int half = 0; half < 2 && !dead; ++half) {
-          mbar_wait_warp(bar(ct.p_half[g][half]), (uint32_t)t & 1u, dead);
+      for (int g = 0; g < groups; ++g) {
+#pragma unroll
+        for (int half = 1; half >= 0; --half) {
+          wait_lead(bar(ct.p_half[g][half]), (uint32_t)t & 1u, lead, dead);
           if (dead) break;
           fence_after();
-          outputs(g, half, vst, t == 0);
+          const uint64_t vd = desc_mn(sv + vst * va * TC_ATOM + half * (TC_ATOM / 2), TC_ATOM);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mma_ts(tmem + 256 + 128 * g, tmem + 128 * g + 64 * half + 8 * k, vd + k * (16 * 128 / 16), id_o, t == 0 && half == 1 && k == 0 ? 0u : 1u, lead);
         }
         if (dead) break;
-        if (g == groups - 1 && lead) commit(bar(ct.v_empty[vst]));
-        if (more) {
-          if (g == 0) mbar_wait_warp(bar(ct.k_full[kst]), kph, dead);
+        if (g == groups - 1) commit_by(lead, bar(ct.v_empty[vst]));
+        if (t + 1 < n) {
+          if (g == 0) wait_lead(bar(ct.k_full[kst]), kph, lead, dead);
           if (dead) break;
           fence_after();
-          scores(g, kst);
-          if (lead) {
-            commit(bar(ct.s_full[g]));
-            if (g == groups - 1) commit(bar(ct.k_empty[kst]));
-          }
-        } else if (lead) {
-          commit(bar(ct.o_done[g]));
+          scores(g);
+        } else {
+          commit_by(lead, bar(ct.o_done[g]));
         }
-        __syncwarp();
       }
       if (++vst == v_stages) { vst = 0; vph ^= 1u; }
-      if (++kst == k_stages) { kst = 0; kph ^= 1u; }
     }
     if (dead) {                                              // what was issued ends before tensor memory is given back
       uint32_t late = 0;
-      if (lead) commit(bar(ct.gave_up));
+      commit_by(lead, bar(ct.gave_up));
       mbar_wait(bar(ct.gave_up), 0, late);
     }
     __syncwarp();
-  } else if (warp == 1 && !HALF) {
+  } else if (warp == 1) {
     // ===================== tiled copies =====================
     const int box = min(1 << a.s.shift, KEYS), boxes = KEYS / box, gone = (a.s.pages * a.kv_heads) << a.s.shift;      // a row beyond the pool: zeros
     int kst = 0, vst = 0;
@@ -215,138 +279,144 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
       const int row = page >= 0 ? ((page * a.kv_heads + h) << a.s.shift) + ((key0 + lane * box) & ((1 << a.s.shift) - 1)) : gone;
       uint32_t there = 0;                                    // by 16 keys
       for (int i = 0; i < 8; ++i) there |= (seen >> (i * 16 / box) & 1u) << i;
-      mbar_wait_warp(bar(ct.k_empty[kst]), kph, dead);
+      const uint32_t k_to = bar(HALF ? ct.rk_full : ct.k_full[kst]);
+      mbar_wait_warp(bar(HALF ? ct.rk_empty : ct.k_empty[kst]), kph, dead);
       if (dead) break;
       if (lane == 0) {
-        there_of[t % INFOS] = there;
+        if (HALF) infos[t % INFOS].there = there;
+        else there_of[t % INFOS] = there;
         mbar_arrive(bar(ct.info_full[t % INFOS]));
-        mbar_expect_tx(bar(ct.k_full[kst]), ka * TC_ATOM);
+        mbar_expect_tx(k_to, HALF ? KEYS * (a.K + 8) : ka * TC_ATOM);
       }
       for (int i = 0; i < boxes; ++i) {
         const int r = __shfl_sync(0xffffffffu, row, i);
-        if (lane == 0)
-          for (int x = 0; x < ka; ++x) tma_load_2d(sk + (kst * ka + x) * TC_ATOM + i * box * 128, &map_k, 64 * x, r, bar(ct.k_full[kst]));
+        if (lane == 0) {
+          if (HALF) {
+            const int at = r < gone ? r : 0;                 // of a page that is not there: any scales
+            tma_load_2d(raw_k + i * box * a.K, &map_k, 0, r, k_to);
+            bulk(smem_u32(codes.ks + i * box), a.ks + at, 4 * box, k_to);
+            bulk(smem_u32(codes.vs + i * box), a.vs + at, 4 * box, k_to);
+          } else {
+            for (int x = 0; x < ka; ++x) tma_load_2d(sk + (kst * ka + x) * TC_ATOM + i * box * 128, &map_k, 64 * x, r, k_to);
+          }
+        }
       }
-      if (++kst == k_stages) { kst = 0; kph ^= 1u; }
-      mbar_wait_warp(bar(ct.v_empty[vst]), vph, dead);
+      if (HALF || ++kst == k_stages) { kst = 0; kph ^= 1u; }
+      mbar_wait_warp(bar(HALF ? ct.rv_empty : ct.v_empty[vst]), vph, dead);
       if (dead) break;
       const int valid = keys.end - key0;
-      // behind the last key that is seen the page may hold anything, and a weight of zero does not hide an infinity: zeros there
-      const uint32_t to = valid < KEYS ? bar(ct.tail) : bar(ct.v_full[vst]);
-      if (lane == 0) mbar_expect_tx(to, va * TC_ATOM);
+      // bf16: behind the last key that is seen the page may hold anything, and a weight of zero does not hide an infinity: zeros there
+      const bool cut = !HALF && valid < KEYS;
+      const uint32_t v_to = bar(HALF ? ct.rv_full : cut ? ct.tail : ct.v_full[vst]);
+      if (lane == 0) mbar_expect_tx(v_to, HALF ? KEYS * a.V : va * TC_ATOM);
       for (int i = 0; i < boxes; ++i) {
         const int r = __shfl_sync(0xffffffffu, row, i);
-        if (lane == 0)
-          for (int x = 0; x < va; ++x) tma_load_2d(sv + (vst * va + x) * TC_ATOM + i * box * 128, &map_v, 64 * x, r, to);
+        if (lane == 0) {
+          if (HALF) tma_load_2d(raw_v + i * box * a.V, &map_v, 0, r, v_to);
+          else
+            for (int x = 0; x < va; ++x) tma_load_2d(sv + (vst * va + x) * TC_ATOM + i * box * 128, &map_v, 64 * x, r, v_to);
+        }
       }
-      if (valid < KEYS) {
-        mbar_wait_warp(to, tail_waits++ & 1u, dead);
+      if (cut) {
+        mbar_wait_warp(v_to, tail_waits++ & 1u, dead);
         if (dead) break;
         for (int x = lane; x < (KEYS - valid) * 8 * va; x += 32) st128(sv + vst * va * TC_ATOM + piece_at(valid + x / (8 * va), x % (8 * va)), make_uint4(0, 0, 0, 0));
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(ct.v_full[vst]));
       }
-      if (++vst == v_stages) { vst = 0; vph ^= 1u; }
+      if (HALF || ++vst == v_stages) { vst = 0; vph ^= 1u; }
     }
-    // every copy has landed before the CTA ends: the MMAs of all tiles come after them, unless a wait ran out
+    // every copy has landed before the CTA ends: what reads them comes after, unless a wait ran out
     if (dead) {
       uint32_t late = 0;
-      for (int i = 0; i < k_stages; ++i) mbar_wait(bar(ct.k_full[i]), i < kst ? kph ^ 1u : kph, late);
+      for (int i = 0; i < (HALF ? 1 : k_stages); ++i) mbar_wait(bar(HALF ? ct.rk_full : ct.k_full[i]), i < kst ? kph ^ 1u : kph, late);
       late = 0;
-      for (int i = 0; i < v_stages; ++i) mbar_wait(bar(ct.v_full[i]), i < vst ? vph ^ 1u : vph, late);
+      for (int i = 0; i < (HALF ? 1 : v_stages); ++i) mbar_wait(bar(HALF ? ct.rv_full : ct.v_full[i]), i < vst ? vph ^ 1u : vph, late);
     }
     __syncwarp();
   } else if (warp >= 12) {
     // ===================== 8-bit codes to f16 =====================
     if constexpr (HALF) {
-      const int me = tid - 384, kc = a.K / 16, vc = a.V / 16;      // 16-byte pieces of a row
+      const int me = tid - 384, kc = a.K / 16, vc = a.V / 16;      // a thread has a key's scales, and every 128th of the tile's 16-byte pieces
+      const int k_by = 65536 / kc + 1, v_by = 65536 / vc + 1;      // x / pieces = x by >> 16 for x < 128 pieces, pieces <= 12
+      auto raw = [&](uint32_t at) {
+        uint4 v;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+        return v;
+      };
+      auto put = [&](uint32_t base, int key, int c, const uint32_t (&y)[8]) {
+        const int odd = (c >> 2) & 1;                        // neighbours meet different banks
+        const uint4 first = make_uint4(y[0], y[1], y[2], y[3]), second = make_uint4(y[4], y[5], y[6], y[7]);
+        st128(base + piece_at(key, 2 * c + odd), odd ? second : first);
+        st128(base + piece_at(key, 2 * c + 1 - odd), odd ? first : second);
+      };
+      float up = 1.f;                                        // 2^e
       int kst = 0, vst = 0;
       uint32_t kph = 1, vph = 1;
-      int pages = -1, key0 = 0;
-      auto look = [&](int t) {                               // pages of a tile's 16-key parts, in lanes 0..7
-        key0 = keys.key0(t0 + t, 7);
-        const int j = key0 + 16 * (lane & 7);
-        pages = j < keys.end ? page_of(a.s, pl.b, j) : -1;
-      };
-      auto row_of = [&](int key) -> long long {              // of the pool, or -1; a whole warp asks
-        const int page = __shfl_sync(0xffffffffu, pages, key >> 4);
-        const int j = key0 + key;
-        return page >= 0 && j < keys.end ? ((long long)(page * a.kv_heads + h) << a.s.shift) + (j & ((1 << a.s.shift) - 1)) : -1;
-      };
-      const int k_by = 65536 / kc + 1, v_by = 65536 / vc + 1;      // x / pieces = x by >> 16 for x < 128 pieces, pieces <= 12
-      auto fetch = [&](const void* pool, int D, int pieces, int by, int i) {
-        const int x = i * 128 + me, key = x * by >> 16, c = x - key * pieces;
-        const long long row = row_of(key);
-        const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(pool) + max(row, 0ll) * D + c * 16);
-        return row >= 0 ? w : make_uint4(0u, 0u, 0u, 0u);
-      };
-      auto put = [&](uint32_t base, int pieces, int by, int i, uint4 w, bool zero) {
-        const int x = i * 128 + me, key = x * by >> 16, c = x - key * pieces;
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-        uint32_t y[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint2 f = codes4<STORE, 0, 1, 2, 3>(u[e]);
-          y[2 * e] = zero ? 0u : f.x;
-          y[2 * e + 1] = zero ? 0u : f.y;
-        }
-        const int odd = (c >> 2) & 1;                        // neighbours meet different banks
-        const uint4 lo = make_uint4(y[0], y[1], y[2], y[3]), hi = make_uint4(y[4], y[5], y[6], y[7]);
-        st128(base + piece_at(key, 2 * c + odd), odd ? hi : lo);
-        st128(base + piece_at(key, 2 * c + 1 - odd), odd ? lo : hi);
-      };
-      uint4 kw[MOST_K / 16], vw[MOST_V / 16];
-      float ks = 0.f, vs = 0.f;
-      auto fetch_keys = [&](int t) {
-        look(t);
-#pragma unroll
-        for (int i = 0; i < MOST_K / 16; ++i)
-          if (i < kc) kw[i] = fetch(a.k, a.K, kc, k_by, i);
-        const long long row = row_of(me);
-        ks = row >= 0 ? a.ks[row] : 0.f;
-        vs = row >= 0 ? a.vs[row] : 1.f;
-      };
-      if (n > 0) fetch_keys(0);
       for (int t = 0; t < n; ++t) {
         Info& info = infos[t % INFOS];
-        const bool zero_row = vs <= 1.17549435e-38f && vs >= 0.f;      // 2^-126 (a row of zeros) or 0 (never written): counts as zeros
-        const uint32_t there = __ballot_sync(0xffffffffu, pages >= 0) & 0xffu, zeros = __ballot_sync(0xffffffffu, zero_row);
-        float add = 0.f, over = 1.f;
-        const float some = zero_row ? SMALLEST_SCALE : vs;
-        asm("lg2.approx.f32 %0, %1;" : "=f"(add) : "f"(some));
-        asm("rcp.approx.f32 %0, %1;" : "=f"(over) : "f"(some));
-        if (!(some >= SMALLEST_SCALE && some <= LARGEST_SCALE)) over = NAN;
-#pragma unroll
-        for (int i = 0; i < MOST_V / 16; ++i)
-          if (i < vc) vw[i] = fetch(a.v, a.V, vc, v_by, i);
+        const int valid = keys.end - keys.key0(t0 + t, 7);
+        mbar_wait_warp(bar(ct.rk_full), (uint32_t)t & 1u, dead);
+        if (dead) break;
+        const float ks = codes.ks[me], vs = me < valid ? codes.vs[me] : 0.f;
+        if (t == 0) {
+          if (vs >= SMALLEST_SCALE && vs <= 1.f / SMALLEST_SCALE) atomicMax(&ct.ref, __float_as_uint(vs));
+          mbar_arrive(bar(ct.ref_full));
+          mbar_wait_warp(bar(ct.ref_full), 0, dead);
+          if (dead) break;
+          up = value_lift(ct.ref);
+        }
+        // what a value's codes are multiplied with: the part of the scale in 1 .. 2 in two f16 (22 bits), and its power of two; 0 hides whatever they are
+        const float s = vs * up;
+        const bool fits = s >= 1.52587890625e-05f && s <= 128.f, zero = vs >= 0.f && vs <= 1.17549435e-38f;      // 2^-126 (a row of zeros) or 0 (never written)
+        const float one = __uint_as_float((__float_as_uint(s) & 0x007fffffu) | 0x3f800000u);
+        const __half hi = __float2half_rn(one), lo = __float2half_rn(one - __half2float(hi)), power = __float2half_rn(__uint_as_float(__float_as_uint(s) & 0x7f800000u));
+        codes.by[t & 1][me] = fits ? make_uint2((uint32_t)__half_as_ushort(hi) | (uint32_t)__half_as_ushort(lo) << 16, __half_as_ushort(power) * 0x10001u) : make_uint2(0u, 0u);
         mbar_wait_warp(bar(ct.k_empty[kst]), kph, dead);
         if (dead) break;
-        info.ks[me] = ks;
-        info.add[me] = add;
-        info.over[me] = over;
-        if (lane == 0) info.zero[warp - 12] = zeros;
-        if (me == 0) info.there = there;
+        info.ks[me] = fits || zero ? ks : NAN;
         mbar_arrive(bar(ct.info_full[t % INFOS]));
+#pragma unroll 2
+        for (int i = 0; i < kc; ++i) {
+          const int x = i * 128 + me, key = x * k_by >> 16;
+          const uint4 w = raw(raw_k + 16 * x);
+          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+          uint32_t y[8];
 #pragma unroll
-        for (int i = 0; i < MOST_K / 16; ++i)
-          if (i < kc) put(sk + kst * ka * TC_ATOM, kc, k_by, i, kw[i], false);
+          for (int e = 0; e < 4; ++e) {
+            const uint2 f = codes4<STORE, 0, 1, 2, 3>(u[e]);
+            y[2 * e] = f.x;
+            y[2 * e + 1] = f.y;
+          }
+          put(sk + kst * ka * TC_ATOM, key, x - key * kc, y);
+        }
         fence_proxy_async();
         mbar_arrive(bar(ct.k_full[kst]));
+        mbar_arrive(bar(ct.rk_empty));
         if (++kst == k_stages) { kst = 0; kph ^= 1u; }
-        if (t + 1 < n) fetch_keys(t + 1);
+        mbar_wait_warp(bar(ct.rv_full), (uint32_t)t & 1u, dead);
+        mbar_wait_warp(bar(ct.info_full[t % INFOS]), (uint32_t)(t / INFOS) & 1u, dead);      // all keys' factors
         mbar_wait_warp(bar(ct.v_empty[vst]), vph, dead);
         if (dead) break;
-        mbar_wait_warp(bar(ct.info_full[t % INFOS]), (uint32_t)(t / INFOS) & 1u, dead);      // all four warps' zero rows are known
-        if (dead) break;
+#pragma unroll 2
+        for (int i = 0; i < vc; ++i) {
+          const int x = i * 128 + me, key = x * v_by >> 16;
+          const uint4 w = raw(raw_v + 16 * x);
+          const uint2 by = codes.by[t & 1][key];
+          const uint32_t u[4] = {w.x, w.y, w.z, w.w}, h2 = __byte_perm(by.x, 0u, 0x1010), l2 = __byte_perm(by.x, 0u, 0x3232);
+          uint32_t y[8];
 #pragma unroll
-        for (int i = 0; i < MOST_V / 16; ++i)
-          if (i < vc) {
-            const int key = (i * 128 + me) * v_by >> 16;
-            put(sv + vst * va * TC_ATOM, vc, v_by, i, vw[i], info.zero[key >> 5] >> (key & 31) & 1u);
+          for (int e = 0; e < 4; ++e) {
+            const uint2 f = codes4<STORE, 0, 1, 2, 3>(u[e]);
+            y[2 * e] = by.y ? scaled(f.x, h2, l2, by.y) : 0u;
+            y[2 * e + 1] = by.y ? scaled(f.y, h2, l2, by.y) : 0u;
           }
+          put(sv + vst * va * TC_ATOM, key, x - key * vc, y);
+        }
         fence_proxy_async();
         mbar_arrive(bar(ct.v_full[vst]));
+        mbar_arrive(bar(ct.rv_empty));
         if (++vst == v_stages) { vst = 0; vph ^= 1u; }
       }
     }
@@ -385,6 +455,7 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
       mbar_arrive(bar(ct.q_full));
     }
     float m = -INFINITY, l = 0.f;
+    bool odd = false;
     // positions of this group's rows: where all of them see a tile no mask is needed
     const int p_min = pl.length - pl.n + (pl.first + TILE * g) / G, p_max = pl.length - pl.n + (pl.first + min(TILE * (g + 1), rows) - 1) / G;
     if (g < groups) {
@@ -404,32 +475,39 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
           if (a.window) x &= ~low_bits(pos - a.window + 1 - j) | low_bits(a.first - j);
           return x & (((there >> 2 * c & 1u) ? 0xffffu : 0u) | ((there >> (2 * c + 1) & 1u) ? 0xffff0000u : 0u));
         };
-        float top = -INFINITY;
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t u[32];
-          tmem_ld32(S + 32 * c, u);
-          float x[4] = {top, -INFINITY, -INFINITY, -INFINITY};
+        // scores of keys 64 half .. + 63, by the keys' scales, hidden ones -inf
+        auto load = [&](int half, uint32_t (&u)[64]) {
+          tmem_ld64(S + 64 * half, u);
           if (HALF) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const float4 k4 = ldf4(info.ks + 32 * c + i), a4 = ldf4(info.add + 32 * c + i);
-              u[i] = __float_as_uint(fmaf(__uint_as_float(u[i]) * k4.x, cr, a4.x));
-              u[i + 1] = __float_as_uint(fmaf(__uint_as_float(u[i + 1]) * k4.y, cr, a4.y));
-              u[i + 2] = __float_as_uint(fmaf(__uint_as_float(u[i + 2]) * k4.z, cr, a4.z));
-              u[i + 3] = __float_as_uint(fmaf(__uint_as_float(u[i + 3]) * k4.w, cr, a4.w));
+            for (int i = 0; i < 64; i += 4) {
+              const float4 k4 = *reinterpret_cast<const float4*>(info.ks + 64 * half + i);
+              float x[4] = {__uint_as_float(u[i]), __uint_as_float(u[i + 1]), __uint_as_float(u[i + 2]), __uint_as_float(u[i + 3])};
+              mul2(x[0], x[1], k4.x, k4.y);
+              mul2(x[2], x[3], k4.z, k4.w);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) u[i + e] = __float_as_uint(x[e]);
             }
           }
           if (!whole) {
-            const uint32_t mask = seen(c);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) u[i] = mask >> i & 1u ? u[i] : 0xff800000u;
+            for (int c = 0; c < 2; ++c) {
+              const uint32_t mask = seen(2 * half + c);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) u[32 * c + i] = mask >> i & 1u ? u[32 * c + i] : 0xff800000u;
+            }
           }
+        };
+        uint32_t u[64];
+        float x4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int i = 0; i < 32; ++i) x[i & 3] = fmaxf(x[i & 3], __uint_as_float(u[i]));
-          top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        for (int half = 0; half < 2; ++half) {               // the second half's stay in registers
+          load(half, u);
+#pragma unroll
+          for (int i = 0; i < 64; i += 2) x4[i / 2 & 3] = max3(x4[i / 2 & 3], __uint_as_float(u[i]), __uint_as_float(u[i + 1]));
         }
-        if (!HALF) top *= cr;
+        const float top = max3(max3(x4[0], x4[1], x4[2]), x4[3], -INFINITY) * cr;
+        if (!(top < INFINITY)) odd = true;                   // NaN or an infinity: the row is computed again
         const bool grows = top > m + 8.f || (m == -INFINITY && top > m);
         if (__any_sync(0xffffffffu, grows)) {
           const float f = grows ? exp2_f(m - top) : 1.f;     // 0 where nothing was added yet
@@ -448,56 +526,44 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
         }
         const float ref = m == -INFINITY ? 0.f : m - LIFT;
         float sum[2] = {0.f, 0.f};
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t u[32], w[16];
-          tmem_ld32(S + 32 * c, u);
-          if (!whole) {
-            const uint32_t mask = seen(c);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) u[i] = mask >> i & 1u ? u[i] : 0xff800000u;
-          }
-          if (HALF) {
+        for (int half = 1; half >= 0; --half) {              // the second half first, over its own scores; then the first, read again
+          if (half == 0) load(0, u);
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const float4 k4 = ldf4(info.ks + 32 * c + i), a4 = ldf4(info.add + 32 * c + i), o4 = ldf4(info.over + 32 * c + i);
-              float x[4] = {fmaf(__uint_as_float(u[i]) * k4.x, cr, a4.x), fmaf(__uint_as_float(u[i + 1]) * k4.y, cr, a4.y),
-                            fmaf(__uint_as_float(u[i + 2]) * k4.z, cr, a4.z), fmaf(__uint_as_float(u[i + 3]) * k4.w, cr, a4.w)};
-              const float ov[4] = {o4.x, o4.y, o4.z, o4.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const bool none = u[i + e] == 0xff800000u;   // hidden: whatever its scales are
-                x[e] = none ? 0.f : exp2_f(x[e] - ref);
-                sum[e & 1] = fmaf(x[e], none ? 0.f : ov[e], sum[e & 1]);
-              }
-              const __half2 lo = __floats2half2_rn(x[0], x[1]), hi = __floats2half2_rn(x[2], x[3]);
-              w[i / 2] = *reinterpret_cast<const uint32_t*>(&lo);
-              w[i / 2 + 1] = *reinterpret_cast<const uint32_t*>(&hi);
-            }
-          } else {
+          for (int c = 0; c < 2; ++c) {
+            uint32_t w[16];
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
-              const float x = exp2_f(fmaf(__uint_as_float(u[i]), cr, -ref)), y = exp2_f(fmaf(__uint_as_float(u[i + 1]), cr, -ref));
-              sum[0] += x;
-              sum[1] += y;
-              const __nv_bfloat162 z = __floats2bfloat162_rn(x, y);
-              w[i / 2] = *reinterpret_cast<const uint32_t*>(&z);
+              float x = __uint_as_float(u[32 * c + i]), y = __uint_as_float(u[32 * c + i + 1]);
+              fma2(x, y, cr, -ref, -ref);
+              if (i % 8 == 6) {
+                exp2_poly2(x, y);
+              } else {
+                x = exp2_f(x);
+                y = exp2_f(y);
+              }
+              add2(sum[0], sum[1], x, y);
+              if (HALF) {
+                const __half2 z = __floats2half2_rn(x, y);
+                w[i / 2] = *reinterpret_cast<const uint32_t*>(&z);
+              } else {
+                const __nv_bfloat162 z = __floats2bfloat162_rn(x, y);
+                w[i / 2] = *reinterpret_cast<const uint32_t*>(&z);
+              }
             }
+            tmem_st16(S + 64 * half + 16 * c, w);
           }
-          tmem_st16(S + 16 * c, w);
-          if (c & 1) {                                       // half of the weights
-            tmem_wait_st();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(ct.p_half[g][c >> 1]));
-          }
+          tmem_wait_st();
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(ct.p_half[g][half]));
         }
         l += sum[0] + sum[1];
       }
       if (n > 0) mbar_wait_warp(bar(ct.o_done[g]), 0, dead);
       fence_after();
-      if (dead) l = NAN;
-      const float inv = a.many.splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+      if (dead || odd) l = NAN;
+      const float down = HALF && n > 0 ? 1.f / value_lift(ct.ref) : 1.f, inv = a.many.splits > 1 ? down : l == 0.f ? 0.f : down / l;
       bool fine = true;
       const long long to = ((long long)split * a.many.count + (long long)row * a.heads + head);
 #pragma unroll 1
@@ -510,7 +576,7 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[e] = dead ? NAN : n > 0 ? __uint_as_float(o[i + e]) : 0.f;
           if (!live) continue;
-          if (a.many.splits > 1) *reinterpret_cast<float4*>(a.many.o + to * a.V + 16 * c + i) = make_float4(x[0], x[1], x[2], x[3]);
+          if (a.many.splits > 1) *reinterpret_cast<float4*>(a.many.o + to * a.V + 16 * c + i) = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
           else a.store(((size_t)row * a.heads + head) * a.V + 16 * c + i, x, inv);
           fine = fine && finite4(x, inv);
         }
@@ -535,14 +601,35 @@ bool many_takes(int K, int V, int store) {
   return (store == ACT ? layout<ACT>(K, V) : layout<INT8>(K, V)).ks > 0;
 }
 
+// Rows of `cols` bytes (a multiple of 16, up to 256), whole ones, as they lie
+static int map_rows(CUtensorMap* m, const void* base, long long rows, int cols, int box_rows) {
+  EncodeFn fn = encoder();
+  if (fn == nullptr) {
+    set_error("cuTensorMapEncodeTiled is not available from this driver");
+    return B2L_E_STATE;
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)cols};
+  const cuuint32_t box[2] = {(cuuint32_t)cols, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+  const CUresult cr = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (cr != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed (%d) for %lld x %d", (int)cr, rows, cols);
+    return B2L_E_ARG;
+  }
+  return 0;
+}
+
 template <int STORE> static int go(const Attn& a, int tiles, cudaStream_t stream) {
   const Layout l = layout<STORE>(a.K, a.V);
-  CUtensorMap mk{}, mv{};
+  CUtensorMap mk, mv;
+  const long long rows = ((long long)a.s.pages * a.kv_heads) << a.s.shift;
+  const int box = 1 << a.s.shift < KEYS ? 1 << a.s.shift : KEYS;
   if (STORE == ACT) {
-    const long long rows = ((long long)a.s.pages * a.kv_heads) << a.s.shift;
-    const int box = 1 << a.s.shift < KEYS ? 1 << a.s.shift : KEYS;
     if (int rc = map_sw128(&mk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.k, rows, a.K, a.K, 64, box)) return rc;
     if (int rc = map_sw128(&mv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.v, rows, a.V, a.V, 64, box)) return rc;
+  } else {
+    if (int rc = map_rows(&mk, a.k, rows, a.K, box)) return rc;
+    if (int rc = map_rows(&mv, a.v, rows, a.V, box)) return rc;
   }
   static DynSmemCache cache;
   if (int rc = ensure_dyn_smem(paged_many_kernel<STORE>, l.smem, cache)) return rc;
