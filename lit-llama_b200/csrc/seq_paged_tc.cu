@@ -9,10 +9,10 @@
 //                 of N = 64 takes 75 cycles and one of N = 128 103: its rows of A come out of shared memory for half as many keys.)
 //   warp 1        tiled copies of pages: bf16, 64 columns each, into 128-byte swizzled rows (keys K-major, values MN-major); codes as they lie, with their
 //                 scales, for warps 12..15
-//   warps 4..11   softmax of row tile 0 (4..7) and 1 (8..11): the second half of a row's scores stays in registers from the maximum to the weights, the first is
-//                 read twice; the weights go back over them half by half, and the second product begins with the first half that is there.  A row's reference moves only when it is exceeded by
-//                 more than 8 (weights reach 2^8; nothing is rounded by that), so the output in tensor memory is seldom scaled.  Of four powers of two the
-//                 special function unit computes three; the fourth is a polynomial, or that unit would take as long as the products
+//   warps 4..11   softmax of row tile 0 (4..7) and 1 (8..11): a row's scores into registers, its weights back over them in two halves, so the second product
+//                 begins with the half that is there.  A row's reference moves only when it is exceeded by more than 8 (weights reach 2^8; nothing is
+//                 rounded by that), so the output in tensor memory is seldom scaled.  bf16: of four powers of two the special function unit computes
+//                 three and a polynomial the fourth: 2048 tokens over 16384 of 32 / 8 heads take 454 us so, 484 without, 461 with three of eight, 475 with half
 //   warps 12..15  8-bit pool: codes as f16 into the same rows: keys exactly, values times their scale
 //
 // Weights are rounded to one bf16 (by half a step, 2^-8; with 8-bit pools one f16, 2^-11): the first rounding below f32 in the sums, and the price of one
@@ -73,13 +73,14 @@ template <int STORE> static Layout layout(int K, int V) {
   return l;
 }
 
-// 64 consecutive 32-bit columns of this warp's 32 tensor-memory lanes
+// 64 consecutive 32-bit columns of this warp's 32 tensor-memory lanes, on their way: the registers hold them after tmem_wait_ld64, which takes them as operands
+// so that nothing uses them before it
 __device__ __forceinline__ void tmem_ld64(uint32_t a, uint32_t* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
       "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
       "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
-      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
         "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
         "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]),
@@ -88,6 +89,13 @@ __device__ __forceinline__ void tmem_ld64(uint32_t a, uint32_t* r) {
         "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
       : "r"(a)
       : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld64(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 64; i += 16)
+    asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]), "+r"(r[i + 8]), "+r"(r[i + 9]),
+                 "+r"(r[i + 10]), "+r"(r[i + 11]), "+r"(r[i + 12]), "+r"(r[i + 13]), "+r"(r[i + 14]), "+r"(r[i + 15]) : : "memory");
 }
 // The largest of three, NaN if one is
 __device__ __forceinline__ float max3(float x, float y, float z) {
@@ -205,7 +213,10 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
   __syncthreads();
   fence_after();
   const uint32_t tmem = ct.tmem;
-  if (warp == 0) {
+  if (warp < 4) {
+   // 8-bit pool: a row's 128 scores in registers, which the softmax takes from the other warps (56 x 128 + 184 x 256 + 88 x 128 = 128 x 512)
+   if constexpr (HALF) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+   if (warp == 0) {
     // ===================== MMA issue =====================
     const uint32_t lead = elect_lane();
     const uint32_t types = HALF ? 0u : (1u << 7) | (1u << 10);      // f16 or bf16, both operands
@@ -266,7 +277,7 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
       mbar_wait(bar(ct.gave_up), 0, late);
     }
     __syncwarp();
-  } else if (warp == 1) {
+   } else if (warp == 1) {
     // ===================== tiled copies =====================
     const int box = min(1 << a.s.shift, KEYS), boxes = KEYS / box, gone = (a.s.pages * a.kv_heads) << a.s.shift;      // a row beyond the pool: zeros
     int kst = 0, vst = 0;
@@ -335,9 +346,11 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
       for (int i = 0; i < (HALF ? 1 : v_stages); ++i) mbar_wait(bar(HALF ? ct.rv_full : ct.v_full[i]), i < vst ? vph ^ 1u : vph, late);
     }
     __syncwarp();
+   }
   } else if (warp >= 12) {
     // ===================== 8-bit codes to f16 =====================
     if constexpr (HALF) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
       const int me = tid - 384, kc = a.K / 16, vc = a.V / 16;      // a thread has a key's scales, and every 128th of the tile's 16-byte pieces
       const int k_by = 65536 / kc + 1, v_by = 65536 / vc + 1;      // x / pieces = x by >> 16 for x < 128 pieces, pieces <= 12
       auto raw = [&](uint32_t at) {
@@ -420,7 +433,8 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
         if (++vst == v_stages) { vst = 0; vph ^= 1u; }
       }
     }
-  } else if (warp >= 4) {
+  } else {
+    if constexpr (HALF) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     // ===================== queries, softmax, outputs =====================
     const int g = (warp - 4) >> 2, r = (warp & 3) * 32 + lane, at = pl.first + TILE * g + r;
     const bool live = TILE * g + r < rows;
@@ -476,8 +490,7 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
           return x & (((there >> 2 * c & 1u) ? 0xffffu : 0u) | ((there >> (2 * c + 1) & 1u) ? 0xffff0000u : 0u));
         };
         // scores of keys 64 half .. + 63, by the keys' scales, hidden ones -inf
-        auto load = [&](int half, uint32_t (&u)[64]) {
-          tmem_ld64(S + 64 * half, u);
+        auto finish = [&](int half, uint32_t* u) {
           if (HALF) {
 #pragma unroll
             for (int i = 0; i < 64; i += 4) {
@@ -498,13 +511,26 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
             }
           }
         };
-        uint32_t u[64];
+        // bf16: the second half's stay in registers from the maximum to the weights, the first is read twice.  All 128 in registers took 3% longer (and with
+        // 8-bit codes 10% less, as there the instructions count)
+        uint32_t u[HALF ? KEYS : KEYS / 2];
         float x4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (HALF) {
+          tmem_ld64(S, u);
+          tmem_ld64(S + 64, u + (HALF ? 64 : 0));
+          tmem_wait_ld64(u);
+          tmem_wait_ld64(u + (HALF ? 64 : 0));
+        }
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {               // the second half's stay in registers
-          load(half, u);
+        for (int half = 0; half < 2; ++half) {
+          uint32_t* x = u + (HALF ? 64 * half : 0);
+          if (!HALF) {
+            tmem_ld64(S + 64 * half, x);
+            tmem_wait_ld64(x);
+          }
+          finish(half, x);
 #pragma unroll
-          for (int i = 0; i < 64; i += 2) x4[i / 2 & 3] = max3(x4[i / 2 & 3], __uint_as_float(u[i]), __uint_as_float(u[i + 1]));
+          for (int i = 0; i < 64; i += 2) x4[i / 2 & 3] = max3(x4[i / 2 & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
         }
         const float top = max3(max3(x4[0], x4[1], x4[2]), x4[3], -INFINITY) * cr;
         if (!(top < INFINITY)) odd = true;                   // NaN or an infinity: the row is computed again
@@ -527,16 +553,21 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
         const float ref = m == -INFINITY ? 0.f : m - LIFT;
         float sum[2] = {0.f, 0.f};
 #pragma unroll
-        for (int half = 1; half >= 0; --half) {              // the second half first, over its own scores; then the first, read again
-          if (half == 0) load(0, u);
+        for (int half = 1; half >= 0; --half) {              // the second half first, over its own scores
+          uint32_t* z = u + (HALF ? 64 * half : 0);
+          if (!HALF && half == 0) {
+            tmem_ld64(S, z);
+            tmem_wait_ld64(z);
+            finish(0, z);
+          }
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             uint32_t w[16];
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
-              float x = __uint_as_float(u[32 * c + i]), y = __uint_as_float(u[32 * c + i + 1]);
+              float x = __uint_as_float(z[32 * c + i]), y = __uint_as_float(z[32 * c + i + 1]);
               fma2(x, y, cr, -ref, -ref);
-              if (i % 8 == 6) {
+              if (!HALF && i % 8 == 6) {
                 exp2_poly2(x, y);
               } else {
                 x = exp2_f(x);
@@ -544,11 +575,11 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
               }
               add2(sum[0], sum[1], x, y);
               if (HALF) {
-                const __half2 z = __floats2half2_rn(x, y);
-                w[i / 2] = *reinterpret_cast<const uint32_t*>(&z);
+                const __half2 p = __floats2half2_rn(x, y);
+                w[i / 2] = *reinterpret_cast<const uint32_t*>(&p);
               } else {
-                const __nv_bfloat162 z = __floats2bfloat162_rn(x, y);
-                w[i / 2] = *reinterpret_cast<const uint32_t*>(&z);
+                const __nv_bfloat162 p = __floats2bfloat162_rn(x, y);
+                w[i / 2] = *reinterpret_cast<const uint32_t*>(&p);
               }
             }
             tmem_st16(S + 64 * half + 16 * c, w);
