@@ -128,6 +128,11 @@ __device__ __forceinline__ void exp2_poly2(float& x, float& y) {
   x = __uint_as_float(__float_as_uint(px) + (__float_as_uint(nx) << 23));
   y = __uint_as_float(__float_as_uint(py) + (__float_as_uint(ny) << 23));
 }
+__device__ __forceinline__ uint4 ld128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
 __device__ __forceinline__ void st128(uint32_t a, uint4 v) { asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory"); }
 // A warp that issues waits and commits by its leading lane alone, without a branch: 32 lanes at a barrier that is complete took 150 cycles, a branch around a
 // commit some 100
@@ -353,11 +358,6 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
       asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
       const int me = tid - 384, kc = a.K / 16, vc = a.V / 16;      // a thread has a key's scales, and every 128th of the tile's 16-byte pieces
       const int k_by = 65536 / kc + 1, v_by = 65536 / vc + 1;      // x / pieces = x by >> 16 for x < 128 pieces, pieces <= 12
-      auto raw = [&](uint32_t at) {
-        uint4 v;
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
-        return v;
-      };
       auto put = [&](uint32_t base, int key, int c, const uint32_t (&y)[8]) {
         const int odd = (c >> 2) & 1;                        // neighbours meet different banks
         const uint4 first = make_uint4(y[0], y[1], y[2], y[3]), second = make_uint4(y[4], y[5], y[6], y[7]);
@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
 #pragma unroll 2
         for (int i = 0; i < kc; ++i) {
           const int x = i * 128 + me, key = x * k_by >> 16;
-          const uint4 w = raw(raw_k + 16 * x);
+          const uint4 w = ld128(raw_k + 16 * x);
           const uint32_t u[4] = {w.x, w.y, w.z, w.w};
           uint32_t y[8];
 #pragma unroll
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
 #pragma unroll 2
         for (int i = 0; i < vc; ++i) {
           const int x = i * 128 + me, key = x * v_by >> 16;
-          const uint4 w = raw(raw_v + 16 * x);
+          const uint4 w = ld128(raw_v + 16 * x);
           const uint2 by = codes.by[t & 1][key];
           const uint32_t u[4] = {w.x, w.y, w.z, w.w}, h2 = __byte_perm(by.x, 0u, 0x1010), l2 = __byte_perm(by.x, 0u, 0x3232);
           uint32_t y[8];
@@ -442,28 +442,37 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), S = lanes + 128 * g, O = lanes + 256 + 128 * g;
     float cr = a.scale_log2;
     {
-      const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)row * a.ldq + (size_t)head * a.hsq;
-      float up = 1.f;
-      if (HALF) {
-        float top = 0.f;
-        for (int c = 0; c < a.K / 8 && live; ++c) {
-          const float4 x = ld_act4(src + 8 * c), y = ld_act4(src + 8 * c + 4);
-          top = fmaxf(fmaxf(fmaxf(fmaxf(top, fabsf(x.x)), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))), fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
-        }
-        lift_of(top, a.scale_log2, up, cr);
+      // The warp's 32 rows, neighbouring lanes along a row: with a row per lane the load unit was busy with 32 lines for every instruction, 5400 cycles.  A
+      // small loop, as code that runs once is fetched at some 12 cycles an instruction; a row's lane knows where it is
+      const int pieces = a.K / 8, by = 65536 / pieces + 1;   // x / pieces = x by >> 16 for x < 32 pieces, pieces <= 24
+      const uint32_t mine = sq + g * ka * TC_ATOM;
+      const unsigned long long from = reinterpret_cast<unsigned long long>(reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)row * a.ldq + (size_t)head * a.hsq);
+#pragma unroll 2
+      for (int x = lane; x < 32 * pieces; x += 32) {
+        const int k = x * by >> 16, c = x - k * pieces;
+        const unsigned long long src = __shfl_sync(0xffffffffu, from, k);
+        atc::cp16(mine + piece_at((warp & 3) * 32 + k, c), reinterpret_cast<const void*>(src + 16 * c), TILE * g + (warp & 3) * 32 + k < rows);
       }
-      for (int c = 0; c < a.K / 8; ++c) {
-        uint4 w = live ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
-        if (HALF) {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      if (HALF) {                                            // then a lane has a row: its largest entry, and the row as f16
+        __syncwarp();
+        uint32_t top2 = 0u;                                  // of two entries' absolute values, as bits: as large as their values are
+        for (int c = 0; c < pieces; ++c) {
+          const uint4 w = ld128(mine + piece_at(r, c));
+          top2 = __vmaxu2(__vmaxu2(__vmaxu2(top2, w.x & 0x7fff7fffu), __vmaxu2(w.y & 0x7fff7fffu, w.z & 0x7fff7fffu)), w.w & 0x7fff7fffu);
+        }
+        float up;
+        lift_of(fmaxf(__uint_as_float(top2 << 16), __uint_as_float(top2 & 0xffff0000u)), a.scale_log2, up, cr);
+        for (int c = 0; c < pieces; ++c) {
+          const uint4 w = ld128(mine + piece_at(r, c));
           uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const __half2 f = __floats2half2_rn(__uint_as_float(u[e] << 16) * up, __uint_as_float(u[e] & 0xffff0000u) * up);
             u[e] = *reinterpret_cast<const uint32_t*>(&f);
           }
-          w = make_uint4(u[0], u[1], u[2], u[3]);
+          st128(mine + piece_at(r, c), make_uint4(u[0], u[1], u[2], u[3]));
         }
-        st128(sq + g * ka * TC_ATOM + piece_at(r, c), w);
       }
       fence_proxy_async();
       mbar_arrive(bar(ct.q_full));
@@ -596,21 +605,52 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
       if (dead || odd) l = NAN;
       const float down = HALF && n > 0 ? 1.f / value_lift(ct.ref) : 1.f, inv = a.many.splits > 1 ? down : l == 0.f ? 0.f : down / l;
       bool fine = true;
+      const bool part = a.many.splits > 1;
+      const int place = live ? row * a.heads + head : -1;    // of the row's outputs
       const long long to = ((long long)split * a.many.count + (long long)row * a.heads + head);
+      // Outputs through the warp's rows of the queries (every score of this row tile is done), 128 bytes of each row at a time; then eight lanes along a row (a
+      // row per lane took 9500 cycles)
+      const int per = part ? 32 : 64;                        // columns
 #pragma unroll 1
-      for (int c = 0; 16 * c < a.V; ++c) {
-        uint32_t o[16];
-        if (n > 0 && !dead) tmem_ld16(O + 16 * c, o);
-        float x[4];
+      for (int c0 = 0; c0 < a.V; c0 += per) {
+#pragma unroll 1
+        for (int c = c0; c < min(c0 + per, a.V); c += 16) {
+          uint32_t o[16];
+          if (n > 0 && !dead) tmem_ld16(O + c, o);
+          float x[16];
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
+          for (int i = 0; i < 16; ++i) x[i] = dead ? NAN : n > 0 ? __uint_as_float(o[i]) * inv : 0.f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = dead ? NAN : n > 0 ? __uint_as_float(o[i + e]) : 0.f;
-          if (!live) continue;
-          if (a.many.splits > 1) *reinterpret_cast<float4*>(a.many.o + to * a.V + 16 * c + i) = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-          else a.store(((size_t)row * a.heads + head) * a.V + 16 * c + i, x, inv);
-          fine = fine && finite4(x, inv);
+          for (int i = 0; i < 16; ++i) fine = fine && fabsf(x[i]) < INFINITY;
+          if (part) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+              st128(sq + g * ka * TC_ATOM + piece_at(r, (c - c0 + i) / 4), make_uint4(__float_as_uint(x[i]), __float_as_uint(x[i + 1]), __float_as_uint(x[i + 2]), __float_as_uint(x[i + 3])));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; i += 8) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const __nv_bfloat162 y = __floats2bfloat162_rn(x[i + 2 * e], x[i + 2 * e + 1]);
+                w[e] = *reinterpret_cast<const uint32_t*>(&y);
+              }
+              st128(sq + g * ka * TC_ATOM + piece_at(r, (c - c0 + i) / 8), make_uint4(w[0], w[1], w[2], w[3]));
+            }
+          }
         }
+        __syncwarp();
+        const int c = lane & 7, column = c0 + c * (per / 8); // this lane's 16 bytes
+#pragma unroll 2
+        for (int k = lane >> 3; k < 32; k += 4) {
+          const int there = __shfl_sync(0xffffffffu, place, k);
+          if (there >= 0 && column < a.V) {
+            const uint4 w = ld128(sq + g * ka * TC_ATOM + piece_at((warp & 3) * 32 + k, c));
+            if (part) *reinterpret_cast<uint4*>(a.many.o + ((size_t)split * a.many.count + there) * a.V + column) = w;
+            else *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)there * a.V + column) = w;
+          }
+        }
+        __syncwarp();
       }
       if (live && a.many.splits > 1) *reinterpret_cast<float2*>(a.many.ml + 2 * to) = make_float2(m, l);
       if (a.many.splits == 1) {
