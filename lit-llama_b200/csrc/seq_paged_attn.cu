@@ -3,7 +3,9 @@
 //   out[r, h] = sum_j w_j v_j / sum_j w_j,   w_j = 2^(c q . k_j - m),   c = scale log2(e),   j the keys that row r sees
 //
 // The query heads that read one key/value head are packed with the tokens: packed row i G + g is head g of the group at the sequence's new token i.
-// paged_few_kernel takes 16 packed rows (one tile of mma.m16n8k16) against the keys of one head, 16 at a time.  A warp has every W-th such unit of its share
+// paged_few_kernel takes 8 or 16 packed rows against the keys of one head, 16 at a time, as mma.m16n8k16 with the keys (and then the entries of a value) for
+// its 16 rows and the queries for its 8 columns: a token of a group of up to 8 heads fills the product that it needs, where queries as rows left three
+// quarters of the scores and their softmax unused (600 instructions for 16 keys of 128 8-bit entries, now 300).  A warp has every W-th such unit of its share
 // all to itself: its own ring of tiled copies (16 rows of one page by 128 bytes, swizzled), its own running maximum, sum and outputs in registers, no
 // barrier in the loop.  The warps' results are joined at the end, and those of several CTAs that share a row's keys by paged_merge_kernel.
 //
@@ -16,7 +18,7 @@
 //   f32             three parts each (f32's 24 bits); of the nine products of two f32 operands the six above 2^-24.  They are added to f32 registers unit by
 //                   unit, because the tensor core truncates where it adds to its accumulator
 // With 8-bit codes a lane has four consecutive entries of a key as its share of a k16 step (queries laid out alike), and values are transposed as pairs
-// of neighbouring entries, so 16-byte rows of ldmatrix do for both.
+// of neighbouring entries, so 16-byte rows of ldmatrix do for both.  Weights turn from keys by rows into the second product's operand by movmatrix.
 //
 // What bounds it: one pass over the keys and values that the rows see, at HBM's rate, for the rows of a token; 16 rows of f32 are bound by their six products.
 #include <algorithm>
@@ -47,6 +49,11 @@ __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
 }
 __device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {      // of an 8 x 8 matrix of 16-bit entries, two per lane
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 __device__ __forceinline__ uint32_t lds32(uint32_t a) { uint32_t v; asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory"); return v; }
 __device__ __forceinline__ uint2 lds64(uint32_t a) { uint2 v; asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory"); return v; }
@@ -88,16 +95,16 @@ template <bool HALF, int PARTS> __device__ __forceinline__ void operand2(float x
 // of nine products of three parts (index 0 the largest) the six above 2^-24, the smallest first
 __device__ constexpr int PART_A[6] = {2, 1, 0, 1, 0, 0}, PART_B[6] = {0, 1, 2, 0, 1, 0};
 
-// c += sum of the products of a's and b's parts; FRESH: in an accumulator of its own, added to c as f32 additions are rounded
+// c += sum of the products of a's and b's parts (one of a, or three of each); FRESH: in an accumulator of its own, added to c as f32 additions are rounded
 template <bool HALF, int AP, int BP, int N, bool FRESH>
-__device__ __forceinline__ void product(float (&c)[4], const uint32_t (&a)[AP][4], const uint32_t* b0, const uint32_t* b1) {
+__device__ __forceinline__ void product(float (&c)[4], const uint32_t (&a)[AP][4], const uint32_t (&b)[BP][2]) {
   float z[4] = {0.f, 0.f, 0.f, 0.f};
   float (&to)[4] = FRESH ? z : c;
 #pragma unroll
   for (int x = 0; x < N; ++x) {
-    const int i = BP == 3 ? PART_A[x] : AP - 1 - x, j = BP == 3 ? PART_B[x] : 0;
-    if constexpr (HALF) mma16816h(to, a[i], b0[j], b1[j]);
-    else mma16816(to, a[i], b0[j], b1[j]);
+    const int i = AP == 3 ? PART_A[x] : 0, j = AP == 3 ? PART_B[x] : BP - 1 - x;
+    if constexpr (HALF) mma16816h(to, a[i], b[j][0], b[j][1]);
+    else mma16816(to, a[i], b[j][0], b[j][1]);
   }
   if (FRESH)
 #pragma unroll
@@ -110,19 +117,21 @@ constexpr int MOST_STAGES = 8;
 
 struct FewMaps { CUtensorMap k, v; };
 
-template <typename act_t, int STORE, int NV>      // NV: the most 16-entry parts of a value
-__global__ void __launch_bounds__(128, NV <= 8 ? 3 : 2) paged_few_kernel(const __grid_constant__ Attn a, const __grid_constant__ FewMaps maps, int stages) {
+// NV: the most 16-entry parts of a value (and, up to 8, of a key); NR: columns of 8 rows
+template <typename act_t, int STORE, int NV, int NR>
+__global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 3) : 2) paged_few_kernel(const __grid_constant__ Attn a, const __grid_constant__ FewMaps maps, int stages) {
   constexpr bool F32 = sizeof(act_t) == 4, HALF = STORE != ACT;
-  constexpr int ES = STORE == ACT ? (int)sizeof(act_t) : 1;
+  constexpr int ES = STORE == ACT ? (int)sizeof(act_t) : 1, R = 8 * NR;
   constexpr int QP = F32 ? 3 : 1, KP = F32 && !HALF ? 3 : 1, WP = F32 ? 3 : HALF ? 1 : 2, PRODUCTS = KP == 3 ? 6 : QP, V_PRODUCTS = KP == 3 ? 6 : WP;
-  constexpr int PER = ES == 1 ? 4 : 2;                       // k16 steps in the 64 bytes of a key that one ldmatrix takes
+  constexpr int PER = ES == 4 ? 1 : ES == 2 ? 1 : 2;         // k16 steps in the two 16-byte pieces that one ldmatrix takes
+  constexpr bool HELD = !F32 && NV <= 8;                     // queries in registers
   constexpr float LIFT = HALF ? 14.f : 0.f;                  // weights up to 2^14 in f16
   extern __shared__ __align__(1024) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5, g = lane >> 2, t = lane & 3;
   const int h = blockIdx.y, split = blockIdx.z, G = a.heads / a.kv_heads, steps = (a.K / 16 + PER - 1) / PER * PER;
   Place pl;
-  if (!a.place(blockIdx.x, 16, 0, a.few_max, lane, pl)) return;
-  const Keys ks = a.keys(pl, 16);
+  if (!a.place(blockIdx.x, R, 0, a.few_max, lane, pl)) return;
+  const Keys ks = a.keys(pl, R);
   const int all = ks.units(4), per = (all + a.few.splits - 1) / a.few.splits;
   const int u_begin = min(split * per, all), u_end = min(u_begin + per, all);
   __shared__ uint32_t bad;                                   // rows whose result is not finite
@@ -142,23 +151,22 @@ __global__ void __launch_bounds__(128, NV <= 8 ? 3 : 2) paged_few_kernel(const _
   __syncwarp();
 
   const int count = u_begin + warp < u_end ? (u_end - u_begin - warp + W - 1) / W : 0;      // this warp's units: u_begin + warp + W i
-  // page of this warp's unit i: 32 at a time, one per lane
-  int pages = -1, pages_at = -1;
   auto key0_of = [&](int i) { return ks.key0(u_begin + warp + W * i, 4); };
+  int row_of = -1;                                           // where this warp's unit i begins in the pool, or -1: 32 at a time, one per lane
   uint32_t skipped = 0;                                      // ring stages whose page is not there
-  int fill = 0;                                              // stage that is filled next
-  auto load = [&](int i) {
-    if (i >= count) return;
-    if (i / 32 != pages_at) {
-      pages_at = i / 32;
-      const int mine = pages_at * 32 + lane;
-      pages = mine < count ? page_of(a.s, pl.b, key0_of(mine)) : -1;
+  int fill = 0, next = 0;                                    // stage that is filled next, and unit
+  auto load = [&]() {
+    if (next >= count) return;
+    if ((next & 31) == 0) {
+      const int mine = next + lane, key0 = mine < count ? key0_of(mine) : 0;
+      const int page = mine < count ? page_of(a.s, pl.b, key0) : -1;
+      row_of = page >= 0 ? ((page * a.kv_heads + h) << a.s.shift) + (key0 & ((1 << a.s.shift) - 1)) : -1;
     }
-    const int page = __shfl_sync(0xffffffffu, pages, i & 31);
-    if (page >= 0) {
+    const int row = __shfl_sync(0xffffffffu, row_of, next & 31);
+    ++next;
+    if (row >= 0) {
       skipped &= ~(1u << fill);
       if (lane == 0) {
-        const int row = ((page * a.kv_heads + h) << a.s.shift) + (key0_of(i) & ((1 << a.s.shift) - 1));
         const uint32_t dst = ring + fill * unit_bytes, bar = bar0 + 8 * fill;
         tc::mbar_expect_tx(bar, unit_bytes + (HALF ? 128 : 0));
         for (int x = 0; x < ka; ++x) tc::tma_load_2d(dst + x * ATOM, &maps.k, x * (128 / ES), row, bar);
@@ -173,66 +181,77 @@ __global__ void __launch_bounds__(128, NV <= 8 ? 3 : 2) paged_few_kernel(const _
     }
     if (++fill == stages) fill = 0;
   };
-  for (int i = 0; i < stages - 1; ++i) load(i);
+  for (int i = 0; i < stages - 1; ++i) load();
 
-  // the queries as the A operand's registers, part by part: rows g and g + 8 by entries 2 t, + 1 and 8 + 2 t, + 1 of a k16 step, or (codes) 4 t .. 4 t + 3
+  // the queries as the B operand's registers, part by part: row g of a column by entries 2 t, + 1 and 8 + 2 t, + 1 of a k16 step, or (codes) 4 t .. 4 t + 3
   if (HALF) {
-    for (int r = warp; r < 16; r += W) {
+    for (int r = warp; r < R; r += W) {
       const int at = pl.first + r;
       float top = 0.f;
       if (at < pl.n * G)
         for (int d = lane; d < a.K; d += 32) top = fmaxf(top, fabsf(ld_act(reinterpret_cast<const act_t*>(a.q), (pl.start + at / G) * a.ldq + (h * G + at % G) * a.hsq + d)));
       top = warp_max(top);
-      if (lane == 0) {
-        lift_of(top, a.scale_log2, lifted[0][r], lifted[1][r]);
-      }
+      if (lane == 0) lift_of(top, a.scale_log2, lifted[0][r], lifted[1][r]);
     }
     __syncthreads();
   }
-  for (int i = threadIdx.x; i < steps * 32; i += blockDim.x) {
-    const int s = i >> 5, l = i & 31;
-    uint32_t p[4][QP];
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int r = (l >> 2) + 8 * half, at = pl.first + r;
-      const act_t* src = reinterpret_cast<const act_t*>(a.q) + (pl.start + at / G) * a.ldq + (h * G + at % G) * a.hsq + 16 * s;
-      const bool in = at < pl.n * G && 16 * s < a.K;
-      const int d0 = HALF ? 4 * (l & 3) : 2 * (l & 3), d1 = HALF ? d0 + 2 : d0 + 8;
-      float x[4] = {0.f, 0.f, 0.f, 0.f};
-      if (in) {
-        x[0] = ld_act(src, d0);
-        x[1] = ld_act(src, d0 + 1);
-        x[2] = ld_act(src, d1);
-        x[3] = ld_act(src, d1 + 1);
-      }
-      if (HALF)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] *= lifted[0][r];
-      operand2<HALF, QP>(x[0], x[1], p[half]);
-      operand2<HALF, QP>(x[2], x[3], p[2 + half]);
+  for (int i = threadIdx.x; i < steps * NR * 32; i += blockDim.x) {
+    const int s = i / (32 * NR), l = i & 31, r = 8 * ((i >> 5) % NR) + (l >> 2), at = pl.first + r;
+    const act_t* src = reinterpret_cast<const act_t*>(a.q) + (pl.start + at / G) * a.ldq + (h * G + at % G) * a.hsq + 16 * s;
+    const int d0 = HALF ? 4 * (l & 3) : 2 * (l & 3), d1 = HALF ? d0 + 2 : d0 + 8;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    if (at < pl.n * G && 16 * s < a.K) {
+      x[0] = ld_act(src, d0);
+      x[1] = ld_act(src, d0 + 1);
+      x[2] = ld_act(src, d1);
+      x[3] = ld_act(src, d1 + 1);
     }
+    if (HALF)
 #pragma unroll
-    for (int q = 0; q < QP; ++q) *reinterpret_cast<uint4*>(queries + (q * steps + s) * 512 + l * 16) = make_uint4(p[0][q], p[1][q], p[2][q], p[3][q]);
+      for (int e = 0; e < 4; ++e) x[e] *= lifted[0][r];
+    uint32_t p[2][QP];
+    operand2<HALF, QP>(x[0], x[1], p[0]);
+    operand2<HALF, QP>(x[2], x[3], p[1]);
+#pragma unroll
+    for (int q = 0; q < QP; ++q) *reinterpret_cast<uint2*>(queries + q * steps * NR * 256 + i * 8) = make_uint2(p[0][q], p[1][q]);
   }
   __syncthreads();
+  uint32_t held[HELD ? NV : 1][NR][1][2];
+  if (HELD)
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        const uint2 u = k < steps ? lds64(sq + (k * NR + r) * 256 + lane * 8) : make_uint2(0u, 0u);
+        held[k][r][0][0] = u.x;
+        held[k][r][0][1] = u.y;
+      }
 
-  float o[2 * NV][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, cr[2] = {a.scale_log2, a.scale_log2};
-  if (HALF) { cr[0] = lifted[1][g]; cr[1] = lifted[1][g + 8]; }
+  float o[NR][NV][4], m[NR][2], l[NR][2], cr[NR][2];         // rows 8 r + 2 t, + 1; outputs: entries by rows
+  int pos[NR][2];
 #pragma unroll
-  for (int i = 0; i < 2 * NV; ++i)
+  for (int r = 0; r < NR; ++r) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-  int pos[2];                                                // of rows g and g + 8
+    for (int e = 0; e < 2; ++e) {
+      const int at = 8 * r + 2 * t + e;
+      m[r][e] = -INFINITY;
+      l[r][e] = 0.f;
+      cr[r][e] = HALF ? lifted[1][at] : a.scale_log2;
+      pos[r][e] = pl.first + at < pl.n * G ? pl.length - pl.n + (pl.first + at) / G : -1;
+    }
 #pragma unroll
-  for (int r = 0; r < 2; ++r) pos[r] = pl.first + g + 8 * r < pl.n * G ? pl.length - pl.n + (pl.first + g + 8 * r) / G : -1;
-  // where this lane's row of an ldmatrix lies: keys (row lane & 7, piece lane / 8 of four) and values (row lane & 15, piece lane / 16 of two)
-  const uint32_t k_at = (lane & 7) * 128 + (((lane >> 3) ^ (lane & 7)) << 4), v_at = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
+    for (int x = 0; x < NV; ++x)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[r][x][e] = 0.f;
+  }
+  // where this lane's row of an ldmatrix lies: row lane & 15, piece lane / 16 of two; or (bf16 values) row (lane & 7) + 8 (lane / 16), piece lane / 8 % 2
+  const uint32_t at_16 = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) << 4), at_8 = ((lane & 7) + (lane >> 4) * 8) * 128 + (((lane >> 3 & 1) ^ (lane & 7)) << 4);
 
   uint32_t dead = (s0 & 1023u) ? 1u : 0u, phase = 0;         // swizzled atoms need 1024-byte alignment
   int stage = 0;
   for (int i = 0; i < count; ++i) {
     __syncwarp();                                            // every lane has done with the stage that is filled next
-    load(i + stages - 1);
+    load();
     const int st = stage;
     if (++stage == stages) stage = 0;
     if (skipped >> st & 1u) continue;
@@ -248,222 +267,247 @@ __global__ void __launch_bounds__(128, NV <= 8 ? 3 : 2) paged_few_kernel(const _
       }
       __syncwarp();
     }
-    float s[2][4];
+    float s[NR][4];
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int r = 0; r < NR; ++r)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+      for (int e = 0; e < 4; ++e) s[r][e] = 0.f;
+    auto score = [&](int k, const uint32_t (&key)[KP][4]) {
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        if constexpr (HELD) {
+          product<HALF, KP, QP, PRODUCTS, false>(s[r], key, held[k][r]);
+        } else {
+          uint32_t q[QP][2];
+#pragma unroll
+          for (int p = 0; p < QP; ++p) {
+            const uint2 u = lds64(sq + ((p * steps + k) * NR + r) * 256 + lane * 8);
+            q[p][0] = u.x;
+            q[p][1] = u.y;
+          }
+          product<HALF, KP, QP, PRODUCTS, false>(s[r], key, q);
+        }
+      }
+    };
+    auto key_pieces = [&](int j) {                           // pieces 2 j, 2 j + 1 of the keys: PER steps
+      uint32_t r4[4];
+      ldsm_x4(kb + (j >> 2) * ATOM + (at_16 ^ ((j & 3) << 5)), r4);
+#pragma unroll
+      for (int x = 0; x < PER; ++x) {
+        uint32_t key[KP][4];
+        if constexpr (HALF) {
+          const uint2 u = codes4<STORE, 0, 1, 2, 3>(r4[2 * x]), v = codes4<STORE, 0, 1, 2, 3>(r4[2 * x + 1]);
+          key[0][0] = u.x; key[0][1] = v.x; key[0][2] = u.y; key[0][3] = v.y;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) key[0][e] = r4[e];
+        }
+        score(PER * j + x, key);
+      }
+    };
     if constexpr (F32 && !HALF) {
 #pragma unroll 2
       for (int k = 0; k < steps; ++k) {
-        uint32_t q[QP][4];
+        uint32_t key[KP][4];
 #pragma unroll
-        for (int p = 0; p < QP; ++p) {
-          const uint4 u = lds128(sq + (p * steps + k) * 512 + lane * 16);
-          q[p][0] = u.x; q[p][1] = u.y; q[p][2] = u.z; q[p][3] = u.w;
-        }
+        for (int e = 0; e < 4; ++e) {                        // rows g, g + 8 by entries 2 t and 8 + 2 t
+          const uint32_t c = 4 * (k & 1) + (t >> 1) + (e & 2);
+          const uint2 u = lds64(kb + (k >> 1) * ATOM + (g + 8 * (e & 1)) * 128 + ((c ^ g) << 4) + 8 * (t & 1));
+          uint32_t p[KP];
+          parts2<KP>(__uint_as_float(u.x), __uint_as_float(u.y), p);
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const uint32_t row = kb + (k >> 1) * ATOM + (8 * n + g) * 128, c = 4 * (k & 1) + (t >> 1), low = 8 * (t & 1);
-          uint32_t b0[KP], b1[KP];
-          const uint2 u = lds64(row + ((c ^ g) << 4) + low), w = lds64(row + (((c + 2) ^ g) << 4) + low);
-          parts2<KP>(__uint_as_float(u.x), __uint_as_float(u.y), b0);
-          parts2<KP>(__uint_as_float(w.x), __uint_as_float(w.y), b1);
-          product<false, QP, KP, PRODUCTS, false>(s[n], q, b0, b1);
+          for (int x = 0; x < KP; ++x) key[x][e] = p[x];
         }
+        score(k, key);
+      }
+    } else if constexpr (HELD) {
+#pragma unroll
+      for (int j = 0; j < NV / PER; ++j) {
+        if (PER * j >= steps) break;
+        key_pieces(j);
       }
     } else {
 #pragma unroll 2
-      for (int j = 0; j < steps / PER; ++j) {
-        uint32_t r[2][4];
-        const uint32_t at = kb + (j >> 1) * ATOM + (k_at ^ ((j & 1) << 6));
-        ldsm_x4(at, r[0]);
-        ldsm_x4(at + 1024, r[1]);
-#pragma unroll
-        for (int x = 0; x < PER; ++x) {
-          uint32_t q[QP][4];
-#pragma unroll
-          for (int p = 0; p < QP; ++p) {
-            const uint4 u = lds128(sq + (p * steps + PER * j + x) * 512 + lane * 16);
-            q[p][0] = u.x; q[p][1] = u.y; q[p][2] = u.z; q[p][3] = u.w;
-          }
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            if constexpr (HALF) {
-              const uint2 b = codes4<STORE, 0, 1, 2, 3>(r[n][x]);
-              product<true, QP, 1, QP, false>(s[n], q, &b.x, &b.y);
-            } else {
-              product<false, QP, 1, QP, false>(s[n], q, &r[n][2 * x], &r[n][2 * x + 1]);
-            }
-          }
-        }
-      }
+      for (int j = 0; j < steps / PER; ++j) key_pieces(j);
     }
-    // scores in powers of two; lane: keys 8 n + 2 t, + 1 of rows g (entries 0, 1) and g + 8 (2, 3)
-    float top[2] = {-INFINITY, -INFINITY}, over[2][2], rest[2][2];      // one over what of the values' scales is in the exponent; what is not
-    const bool whole = ks.whole(key0, 16);
+    // scores in powers of two; lane: keys g (entries 0, 1) and g + 8 (2, 3) of rows 2 t and 2 t + 1
+    float c[2] = {1.f, 1.f}, add[2] = {0.f, 0.f}, over[2], rest[2];      // one over what of the values' scales is in the exponent; what is not
     bool zeros = false;                                      // whether a value counts as zeros
+    if (HALF) {
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      float c[2] = {1.f, 1.f}, add[2] = {0.f, 0.f};
-      if (HALF) {
-        const uint2 x = lds64(sb + (8 * n + 2 * t) * 4), y = lds64(sb + 64 + (8 * n + 2 * t) * 4);
-        c[0] = __uint_as_float(x.x);
-        c[1] = __uint_as_float(x.y);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float v = __uint_as_float(e ? y.y : y.x);
-          const bool zero = v >= 0.f && v <= 1.17549435e-38f;      // 2^-126 (a row of zeros) or 0 (never written): counts as zeros
-          const float some = zero ? SMALLEST_SCALE : v;
-          if (F32) {                                         // the power of two: exact; the rest of it goes with the weight
-            const int exponent = (int)(__float_as_uint(some) >> 23 & 255u);
-            add[e] = (float)(exponent - 127);
-            over[n][e] = __uint_as_float((uint32_t)(254 - exponent) << 23);
-            rest[n][e] = zero ? 0.f : v * over[n][e];
-          } else {                                           // all of it, to 2^-22 (of log2 s where that is larger than 1)
-            asm("lg2.approx.f32 %0, %1;" : "=f"(add[e]) : "f"(some));
-            asm("rcp.approx.f32 %0, %1;" : "=f"(over[n][e]) : "f"(some));
-            rest[n][e] = zero ? 0.f : 1.f;
-            zeros |= zero;
-          }
-          if (!(some >= SMALLEST_SCALE && some <= LARGEST_SCALE)) over[n][e] = NAN;
+      for (int e = 0; e < 2; ++e) {
+        c[e] = __uint_as_float(lds32(sb + (g + 8 * e) * 4));
+        const float v = __uint_as_float(lds32(sb + 64 + (g + 8 * e) * 4));
+        const bool zero = v >= 0.f && v <= 1.17549435e-38f;  // 2^-126 (a row of zeros) or 0 (never written): counts as zeros
+        const float some = zero ? SMALLEST_SCALE : v;
+        if (F32) {                                           // the power of two: exact; the rest of it goes with the weight
+          const int exponent = (int)(__float_as_uint(some) >> 23 & 255u);
+          add[e] = (float)(exponent - 127);
+          over[e] = __uint_as_float((uint32_t)(254 - exponent) << 23);
+          rest[e] = zero ? 0.f : v * over[e];
+        } else {                                             // all of it, to 2^-22 (of log2 s where that is larger than 1)
+          asm("lg2.approx.f32 %0, %1;" : "=f"(add[e]) : "f"(some));
+          asm("rcp.approx.f32 %0, %1;" : "=f"(over[e]) : "f"(some));
+          rest[e] = zero ? 0.f : 1.f;
+          zeros |= zero;
         }
+        if (!(some >= SMALLEST_SCALE && some <= LARGEST_SCALE)) over[e] = NAN;
       }
+      if (!F32) zeros = __any_sync(0xffffffffu, zeros);
+    }
+    const bool whole = ks.whole(key0, 16);
+    bool grows = false;
+    float top[NR][2];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[n][e] = HALF ? fmaf(s[n][e] * c[e & 1], cr[e >> 1], add[e & 1]) : s[n][e] * cr[0];
-        if (!whole && !a.sees(pos[e >> 1], key0 + 8 * n + 2 * t + (e & 1))) s[n][e] = -INFINITY;
-        top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-    }
-    if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
-      float f[2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float now = fmaxf(m[r], top[r]);
-        f[r] = m[r] == now ? 1.f : exp2_f(m[r] - now);
-        m[r] = now;
-        l[r] *= f[r];
+        s[r][e] = HALF ? fmaf(s[r][e] * c[e >> 1], cr[r][e & 1], add[e >> 1]) : s[r][e] * a.scale_log2;
+        if (!whole && !a.sees(pos[r][e & 1], key0 + g + 8 * (e >> 1))) s[r][e] = -INFINITY;
       }
 #pragma unroll
-      for (int x = 0; x < 2 * NV; ++x) {
-        o[x][0] *= f[0];
-        o[x][1] *= f[0];
-        o[x][2] *= f[1];
-        o[x][3] *= f[1];
+      for (int e = 0; e < 2; ++e) {
+        top[r][e] = fmaxf(s[r][e], s[r][2 + e]);
+        top[r][e] = fmaxf(top[r][e], __shfl_xor_sync(0xffffffffu, top[r][e], 4));
+        top[r][e] = fmaxf(top[r][e], __shfl_xor_sync(0xffffffffu, top[r][e], 8));
+        top[r][e] = fmaxf(top[r][e], __shfl_xor_sync(0xffffffffu, top[r][e], 16));
+        grows |= top[r][e] > m[r][e];
       }
     }
-    if (HALF && !F32) zeros = __any_sync(0xffffffffu, zeros);
-    uint32_t wa[WP][4];                                      // the weights as the A operand of the second product
+    if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+      for (int r = 0; r < NR; ++r) {
+        float f[2];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
+        for (int e = 0; e < 2; ++e) {
+          const float now = fmaxf(m[r][e], top[r][e]);
+          f[e] = m[r][e] == now ? 1.f : exp2_f(m[r][e] - now);
+          m[r][e] = now;
+          l[r][e] *= f[e];
+        }
+#pragma unroll
+        for (int x = 0; x < NV; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[r][x][e] *= f[e & 1];
+      }
+    }
+    uint32_t wb[NR][WP][2];                                  // the weights as the B operand of the second product
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {                          // key g or g + 8
         float x[2];
         uint32_t w[WP];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float z = s[n][2 * r + e];
-          x[e] = exp2_f(F32 ? (z - m[r]) + LIFT : z - (m[r] - LIFT));
+          const float z = s[r][2 * k + e];
+          x[e] = exp2_f(F32 ? (z - m[r][e]) + LIFT : z - (m[r][e] - LIFT));
           if (z == -INFINITY) x[e] = 0.f;                    // hidden, or of no weight: whatever its scale is, and while the maximum is -inf
-          else l[r] = HALF ? fmaf(x[e], over[n][e], l[r]) : l[r] + x[e];
-          if (HALF && (F32 || zeros)) x[e] = z == -INFINITY ? 0.f : x[e] * rest[n][e];
+          else l[r][e] = HALF ? fmaf(x[e], over[k], l[r][e]) : l[r][e] + x[e];
+          if (HALF && (F32 || zeros)) x[e] = z == -INFINITY ? 0.f : x[e] * rest[k];
         }
         operand2<HALF, WP>(x[0], x[1], w);
 #pragma unroll
-        for (int p = 0; p < WP; ++p) wa[p][2 * n + r] = w[p];
+        for (int p = 0; p < WP; ++p) wb[r][p][k] = transposed(w[p]);
       }
+    auto value = [&](int x, const uint32_t (&v)[KP][4]) {    // 16 entries of the values
+#pragma unroll
+      for (int r = 0; r < NR; ++r) product<HALF, KP, WP, V_PRODUCTS, F32>(o[r][x], v, wb[r]);
+    };
     if constexpr (F32 && !HALF) {
 #pragma unroll
-      for (int x = 0; x < 2 * NV; ++x) {
-        if (8 * x >= a.V) break;
-        float v[4];                                          // entry 8 x + g of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+      for (int x = 0; x < NV; ++x) {
+        if (16 * x >= a.V) break;
+        uint32_t v[KP][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 2 * t + (e & 1) + 8 * (e >> 1), c = 2 * x + (g >> 2);
-          v[e] = __uint_as_float(lds32(vb + (c >> 3) * ATOM + r * 128 + (((c & 7) ^ (r & 7)) << 4) + (g & 3) * 4));
+        for (int e = 0; e < 4; ++e) {                        // entries 16 x + g, + 8 of keys 2 t, 2 t + 1 and 8 more
+          float y[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int r = 2 * t + k + 8 * (e >> 1), c = 4 * x + (g >> 2) + 2 * (e & 1);
+            y[k] = __uint_as_float(lds32(vb + (c >> 3) * ATOM + r * 128 + (((c & 7) ^ (r & 7)) << 4) + (g & 3) * 4));
+          }
+          uint32_t p[KP];
+          parts2<KP>(y[0], y[1], p);
+#pragma unroll
+          for (int k = 0; k < KP; ++k) v[k][e] = p[k];
         }
-        uint32_t b0[KP], b1[KP];
-        parts2<KP>(v[0], v[1], b0);
-        parts2<KP>(v[2], v[3], b1);
-        product<false, WP, KP, V_PRODUCTS, true>(o[x], wa, b0, b1);
+        value(x, v);
       }
     } else if constexpr (HALF) {
 #pragma unroll
       for (int x = 0; x < (NV + 1) / 2; ++x) {               // 32 entries at a time; the last 16 may be the copy's zeros
         if (32 * x >= a.V) break;
         uint32_t r4[4];
-        ldsm_x4_t(vb + (x >> 2) * ATOM + (v_at ^ ((x & 3) << 5)), r4);
+        ldsm_x4_t(vb + (x >> 2) * ATOM + (at_16 ^ ((x & 3) << 5)), r4);
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
           if (2 * x + y >= NV) break;
           const uint2 lo = codes4<STORE, 0, 2, 1, 3>(r4[2 * y]), hi = codes4<STORE, 0, 2, 1, 3>(r4[2 * y + 1]);      // entries 2 g and 2 g + 1 of two keys
-          product<true, WP, 1, WP, F32>(o[2 * (2 * x + y)], wa, &lo.x, &hi.x);
-          product<true, WP, 1, WP, F32>(o[2 * (2 * x + y) + 1], wa, &lo.y, &hi.y);
+          const uint32_t v[1][4] = {{lo.x, lo.y, hi.x, hi.y}};
+          value(2 * x + y, v);
         }
       }
     } else {
 #pragma unroll
       for (int x = 0; x < NV; ++x) {
         if (16 * x >= a.V) break;
-        uint32_t r4[4];
-        ldsm_x4_t(vb + (x >> 2) * ATOM + (v_at ^ ((x & 3) << 5)), r4);
-        product<false, WP, 1, WP, false>(o[2 * x], wa, &r4[0], &r4[1]);
-        product<false, WP, 1, WP, false>(o[2 * x + 1], wa, &r4[2], &r4[3]);
+        uint32_t v[1][4];
+        ldsm_x4_t(vb + (x >> 2) * ATOM + (at_8 ^ ((x & 3) << 5)), v[0]);
+        value(x, v);
       }
     }
   }
   if (dead) {                                                // copies under way end before the CTA does; the rows are computed again from memory
     uint32_t late = 0;
     for (int i = 0; i < stages; ++i) tc::mbar_wait_warp(bar0 + 8 * i, phase >> i & 1u, late);
-    l[0] = l[1] = NAN;
+#pragma unroll
+    for (int r = 0; r < NR; ++r) l[r][0] = l[r][1] = NAN;
   }
 
-  // the warps' results: reference maximum, sum and outputs of 16 rows each
+  // the warps' results: reference maximum, sum and outputs of R rows each
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-  }
+  for (int r = 0; r < NR; ++r)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int k = 4; k < 32; k <<= 1) l[r][e] += __shfl_xor_sync(0xffffffffu, l[r][e], k);
   __syncthreads();
-  float* sm = reinterpret_cast<float*>(smem);                // [W][16] maxima, [W][16] sums, [W][16][ov] outputs
+  float* sm = reinterpret_cast<float*>(smem);                // [W][R] maxima, [W][R] sums, [W][R][ov] outputs
   const int ov = a.V + 4;
-  float* so = sm + 32 * W;
-  if (t == 0) {
+  float* so = sm + 2 * R * W;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      sm[16 * warp + g + 8 * r] = m[r];
-      sm[16 * W + 16 * warp + g + 8 * r] = l[r];
-    }
-  }
+  for (int r = 0; r < NR; ++r) {
+    if (g == 0)
 #pragma unroll
-  for (int x = 0; x < 2 * NV; ++x) {
-    if (16 * (x / 2) >= a.V) break;
+      for (int e = 0; e < 2; ++e) {
+        sm[R * warp + 8 * r + 2 * t + e] = m[r][e];
+        sm[R * (W + warp) + 8 * r + 2 * t + e] = l[r][e];
+      }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int d = STORE != ACT ? 16 * (x / 2) + 4 * t + 2 * (e & 1) + (x & 1) : 8 * x + 2 * t + (e & 1);
-      so[(16 * warp + g + 8 * (e >> 1)) * ov + d] = o[x][e];
+    for (int x = 0; x < NV; ++x) {
+      if (16 * x >= a.V) break;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) so[(R * warp + 8 * r + 2 * t + (e & 1)) * ov + 16 * x + (HALF ? 2 * g + (e >> 1) : g + 8 * (e >> 1))] = o[r][x][e];
     }
   }
   __syncthreads();
   const int quads = a.V / 4;
-  for (int i = threadIdx.x; i < 16 * quads; i += blockDim.x) {
+  for (int i = threadIdx.x; i < R * quads; i += blockDim.x) {
     const int r = i / quads, d = 4 * (i - r * quads), at = pl.first + r;
     if (at >= pl.n * G) break;
     float M = -INFINITY, L = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int w = 0; w < W; ++w) M = fmaxf(M, sm[16 * w + r]);
+    for (int w = 0; w < W; ++w) M = fmaxf(M, sm[R * w + r]);
     for (int w = 0; w < W; ++w) {
-      const float mw = sm[16 * w + r];
-      if (mw == -INFINITY && sm[16 * W + 16 * w + r] == 0.f) continue;
+      const float mw = sm[R * w + r];
+      if (mw == -INFINITY && sm[R * (W + w) + r] == 0.f) continue;
       const float f = mw == M ? 1.f : exp2_f(mw - M);
-      L += f * sm[16 * W + 16 * w + r];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = fmaf(f, so[(16 * w + r) * ov + d + e], x[e]);
+      L += f * sm[R * (W + w) + r];
+      const float4 y = *reinterpret_cast<const float4*>(so + (R * w + r) * ov + d);
+      x[0] = fmaf(f, y.x, x[0]);
+      x[1] = fmaf(f, y.y, x[1]);
+      x[2] = fmaf(f, y.z, x[2]);
+      x[3] = fmaf(f, y.w, x[3]);
     }
     const int row = pl.start + at / G, head = h * G + at % G;
     if (a.few.splits > 1) {
@@ -575,7 +619,7 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const __g
 // ------------------------------------------------------------------------------------------------ host
 struct Plan {
   bool few, many;
-  int few_max, few_tiles, many_tiles, few_splits, many_splits, compact;
+  int few_max, few_rows, few_tiles, many_tiles, few_splits, many_splits, compact;
   long long few_count, many_count, floats;
 };
 constexpr long long MOST_WORK = 1ll << 27;                   // floats of partial results
@@ -591,7 +635,9 @@ static Plan plan_of(int rows, int seqs, int width, int page, int heads, int kv_h
   p.few_max = !p.many ? INT32_MAX : p.few ? 16 : 0;
   p.compact = p.few && p.many;
   const int most = std::min(seqs, rows);
-  p.few_tiles = p.compact ? most : (int)std::min<long long>(packed / 16 + most, INT32_MAX);
+  // rows of a tile: 8 where a token's heads, or all that the longest of the sequences has, fit
+  p.few_rows = (max_new > 0 ? (long long)max_new * G <= 8 : G <= 8 && packed <= 8ll * most) && !p.compact ? 8 : 16;
+  p.few_tiles = p.compact ? most : (int)std::min<long long>(packed / p.few_rows + most, INT32_MAX);
   p.many_tiles = (int)std::min<long long>(packed / 256 + most, INT32_MAX);
   long long keys = (long long)width * page;                  // the most keys that a row sees
   if (max_length > 0) keys = std::min<long long>(keys, max_length);
@@ -624,27 +670,27 @@ static Plan plan_of(int rows, int seqs, int width, int page, int heads, int kv_h
   return p;
 }
 
-template <typename act_t, int STORE, int NV> static int few_launch(const Attn& a, int tiles, cudaStream_t stream) {
-  constexpr int ES = STORE == ACT ? (int)sizeof(act_t) : 1, PER = ES == 1 ? 4 : 2;
-  const size_t queries = (size_t)(sizeof(act_t) == 4 ? 3 : 1) * ((a.K / 16 + PER - 1) / PER * PER) * 512, unit = (size_t)(atoms_of(a.K, ES) + atoms_of(a.V, ES)) * ATOM;
+template <typename act_t, int STORE, int NV, int NR> static int few_launch(const Attn& a, int tiles, cudaStream_t stream) {
+  constexpr int ES = STORE == ACT ? (int)sizeof(act_t) : 1, PER = ES == 1 ? 2 : 1;
+  const size_t queries = (size_t)(sizeof(act_t) == 4 ? 3 : 1) * ((a.K / 16 + PER - 1) / PER * PER) * NR * 256, unit = (size_t)(atoms_of(a.K, ES) + atoms_of(a.V, ES)) * ATOM;
   // four warps and as many CTAs on an SM as leave each warp two units in its ring at least; fewer warps where one CTA does not fit
   constexpr size_t SM = 227 * 1024, OTHER = 6 * 1024;        // static: barriers, scales; the system's 1 KB
   int W = 4, stages = 0;
-  for (int ctas = NV <= 8 ? 4 : 2; ctas >= 1 && stages < 2; --ctas)
+  for (int ctas = NV <= 8 ? (NR == 1 && ES == 1 ? 4 : 3) : 2; ctas >= 1 && stages < 2; --ctas)
     for (W = 4; W >= (ctas == 1 ? 1 : 4); W /= 2) {
       const size_t room = SM / ctas - OTHER;
       stages = room > queries ? (int)std::min<size_t>(MOST_STAGES, (room - queries) / (W * unit)) : 0;
       if (stages >= 2) break;
     }
   B2L_CHECK_SUPPORTED(stages >= 2, "b2l_seq_paged_attention: heads of %d and %d entries do not fit", a.K, a.V);
-  const size_t smem = std::max(queries + W * stages * unit, (size_t)W * (32 + 16 * (a.V + 4)) * 4);
+  const size_t smem = std::max(queries + W * stages * unit, (size_t)W * 8 * NR * (a.V + 6) * 4);
   const CUtensorMapDataType type = ES == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : ES == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   const long long rows = ((long long)a.s.pages * a.kv_heads) << a.s.shift;
   FewMaps maps;
   if (int rc = tc::map_sw128(&maps.k, type, ES, a.k, rows, a.K, a.K, 128 / ES, 16)) return rc;
   if (int rc = tc::map_sw128(&maps.v, type, ES, a.v, rows, a.V, a.V, 128 / ES, 16)) return rc;
   static DynSmemCache cache;
-  auto kernel = paged_few_kernel<act_t, STORE, NV>;
+  auto kernel = paged_few_kernel<act_t, STORE, NV, NR>;
   if (int rc = ensure_dyn_smem(kernel, smem, cache)) return rc;
   kernel<<<dim3((unsigned)tiles, (unsigned)a.kv_heads, (unsigned)a.few.splits), 32 * W, smem, stream>>>(a, maps, stages);
   B2L_LAUNCH_CHECK("paged_few_kernel");
@@ -702,7 +748,10 @@ extern "C" int b2l_seq_paged_attention(const void* q, long long ldq, long long h
   const cudaStream_t st = (cudaStream_t)stream;
   if (p.few) {
     int rc = 0;
-#define GO(ST) (V <= 128 ? few_launch<act_t, ST, 8>(a, p.few_tiles, st) : few_launch<act_t, ST, 16>(a, p.few_tiles, st))
+    const bool small = V <= 128 && K <= 128;
+#define GO(ST)                                                                                                                              \
+  (p.few_rows == 8 ? (small ? few_launch<act_t, ST, 8, 1>(a, p.few_tiles, st) : few_launch<act_t, ST, 16, 1>(a, p.few_tiles, st))            \
+                   : (small ? few_launch<act_t, ST, 8, 2>(a, p.few_tiles, st) : few_launch<act_t, ST, 16, 2>(a, p.few_tiles, st)))
     B2L_SEQ_DISPATCH(act_dtype, rc = store == ACT ? GO(ACT) : store == E4M3 ? GO(E4M3) : GO(INT8));
 #undef GO
     if (rc) return rc;
