@@ -3,7 +3,7 @@
 //   out[r, h] = sum_j w_j v_j / sum_j w_j,   w_j = 2^(c q . k_j - m),   c = scale log2(e),   j the keys that row r sees
 //
 // The query heads that read one key/value head are packed with the tokens: packed row i G + g is head g of the group at the sequence's new token i.
-// paged_few_kernel takes 8 or 16 packed rows against the keys of one head, 16 at a time, as mma.m16n8k16 with the keys (and then the entries of a value) for
+// paged_few_kernel takes 8 or 16 packed rows against the keys of one head, 16 (8-bit: 32) at a time, as mma.m16n8k16 with the keys (and then the entries of a value) for
 // its 16 rows and the queries for its 8 columns: a token of a group of up to 8 heads fills the product that it needs, where queries as rows left three
 // quarters of the scores and their softmax unused (600 instructions for 16 keys of 128 8-bit entries, now 300).  A warp has every W-th such unit of its share
 // all to itself: its own ring of tiled copies (16 rows of one page by 128 bytes, swizzled), its own running maximum, sum and outputs in registers, no
@@ -112,8 +112,9 @@ __device__ __forceinline__ void product(float (&c)[4], const uint32_t (&a)[AP][4
 }
 
 // ------------------------------------------------------------------------------------------------ 16 rows
-constexpr int ATOM = 2048;           // 16 rows of 128 bytes, as a swizzled tiled copy leaves them: 16-byte piece c of row r at piece c ^ (r & 7)
-constexpr int MOST_STAGES = 8;
+constexpr int ATOM = 2048;           // 16 rows of 128 bytes, as a swizzled tiled copy leaves them: 16-byte piece c of row r at piece c ^ (r & 7); the next 16 follow
+
+__host__ __device__ constexpr int most_stages(int store) { return store == ACT ? 8 : 4; }
 
 struct FewMaps { CUtensorMap k, v; };
 
@@ -125,6 +126,8 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
   constexpr int QP = F32 ? 3 : 1, KP = F32 && !HALF ? 3 : 1, WP = F32 ? 3 : HALF ? 1 : 2, PRODUCTS = KP == 3 ? 6 : QP, V_PRODUCTS = KP == 3 ? 6 : WP;
   constexpr int PER = ES == 4 ? 1 : ES == 2 ? 1 : 2;         // k16 steps in the two 16-byte pieces that one ldmatrix takes
   constexpr bool HELD = !F32 && NV <= 8;                     // queries in registers
+  constexpr int STAGES = most_stages(STORE);
+  constexpr int NK = HALF ? 2 : 1, SHIFT = HALF ? 5 : 4;     // 16-key parts of a unit: half as many copies, waits and maxima for codes' half as many bytes
   constexpr float LIFT = HALF ? 14.f : 0.f;                  // weights up to 2^14 in f16
   extern __shared__ __align__(1024) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5, g = lane >> 2, t = lane & 3;
@@ -132,16 +135,16 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
   Place pl;
   if (!a.place(blockIdx.x, R, 0, a.few_max, lane, pl)) return;
   const Keys ks = a.keys(pl, R);
-  const int all = ks.units(4), per = (all + a.few.splits - 1) / a.few.splits;
+  const int all = ks.units(SHIFT), per = (all + a.few.splits - 1) / a.few.splits;
   const int u_begin = min(split * per, all), u_end = min(u_begin + per, all);
   __shared__ uint32_t bad;                                   // rows whose result is not finite
   __shared__ float lifted[2][16];                            // what a row of queries is multiplied with for f16, and a score with to undo it
-  __shared__ __align__(8) uint64_t bars[4 * MOST_STAGES];
-  __shared__ __align__(16) float scales[HALF ? 4 * MOST_STAGES * 32 : 4];
-  const int ka = atoms_of(a.K, ES), va = atoms_of(a.V, ES), unit_bytes = (ka + va) * ATOM;
+  __shared__ __align__(8) uint64_t bars[4 * STAGES];
+  __shared__ __align__(16) float scales[HALF ? 4 * STAGES * 64 : 4];
+  const int ka = atoms_of(a.K, ES), va = atoms_of(a.V, ES), unit_bytes = NK * (ka + va) * ATOM;
   const uint32_t s0 = tc::smem_u32(smem);
   const uint32_t ring = s0 + (uint32_t)(warp * stages * unit_bytes), sq = s0 + (uint32_t)(W * stages * unit_bytes);
-  const uint32_t bar0 = tc::smem_u32(bars) + warp * MOST_STAGES * 8, sc0 = tc::smem_u32(scales) + warp * MOST_STAGES * 128;
+  const uint32_t bar0 = tc::smem_u32(bars) + warp * STAGES * 8, sc0 = tc::smem_u32(scales) + warp * STAGES * 256;
   uint8_t* queries = smem + W * stages * unit_bytes;
   if (threadIdx.x == 0) bad = 0u;
   if (lane == 0) {
@@ -151,33 +154,43 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
   __syncwarp();
 
   const int count = u_begin + warp < u_end ? (u_end - u_begin - warp + W - 1) / W : 0;      // this warp's units: u_begin + warp + W i
-  auto key0_of = [&](int i) { return ks.key0(u_begin + warp + W * i, 4); };
-  int row_of = -1;                                           // where this warp's unit i begins in the pool, or -1: 32 at a time, one per lane
-  uint32_t skipped = 0;                                      // ring stages whose page is not there
+  auto key0_of = [&](int i) { return ks.key0(u_begin + warp + W * i, SHIFT); };
+  // where 16-key parts of this warp's units begin in the pool: 32 at a time, one per lane; of a page that is not there a row beyond the pool, which reads as
+  // zeros
+  const int beyond = (a.s.pages * a.kv_heads) << a.s.shift;
+  const bool wide = NK == 2 && a.s.shift >= 5;               // a unit is in one page: one copy
+  int row_of = beyond;
+  uint32_t gone = 0;                                         // 16-key parts of the ring's stages whose page is not there
   int fill = 0, next = 0;                                    // stage that is filled next, and unit
   auto load = [&]() {
     if (next >= count) return;
-    if ((next & 31) == 0) {
-      const int mine = next + lane, key0 = mine < count ? key0_of(mine) : 0;
-      const int page = mine < count ? page_of(a.s, pl.b, key0) : -1;
-      row_of = page >= 0 ? ((page * a.kv_heads + h) << a.s.shift) + (key0 & ((1 << a.s.shift) - 1)) : -1;
+    if ((next & (32 / NK - 1)) == 0) {
+      const int mine = next + lane / NK, key0 = key0_of(mine) + 16 * (lane % NK);
+      const int page = mine < count && key0 < ks.end ? page_of(a.s, pl.b, key0) : -1;
+      row_of = page >= 0 ? ((page * a.kv_heads + h) << a.s.shift) + (key0 & ((1 << a.s.shift) - 1)) : beyond;
     }
-    const int row = __shfl_sync(0xffffffffu, row_of, next & 31);
+    const int at = NK * (next & (32 / NK - 1)), r0 = __shfl_sync(0xffffffffu, row_of, at), r1 = NK == 2 ? __shfl_sync(0xffffffffu, row_of, at + 1) : beyond;
     ++next;
-    if (row >= 0) {
-      skipped &= ~(1u << fill);
+    gone = (gone & ~(3u << 2 * fill)) | ((r0 == beyond ? 1u : 0u) | (r1 == beyond ? 2u : 0u)) << 2 * fill;
+    if (r0 != beyond || r1 != beyond) {
       if (lane == 0) {
-        const uint32_t dst = ring + fill * unit_bytes, bar = bar0 + 8 * fill;
-        tc::mbar_expect_tx(bar, unit_bytes + (HALF ? 128 : 0));
-        for (int x = 0; x < ka; ++x) tc::tma_load_2d(dst + x * ATOM, &maps.k, x * (128 / ES), row, bar);
-        for (int x = 0; x < va; ++x) tc::tma_load_2d(dst + (ka + x) * ATOM, &maps.v, x * (128 / ES), row, bar);
-        if (HALF) {
-          bulk64(sc0 + 128 * fill, a.ks + row, bar);
-          bulk64(sc0 + 128 * fill + 64, a.vs + row, bar);
+        const uint32_t dst = ring + fill * unit_bytes, bar = bar0 + 8 * fill, sc = sc0 + 256 * fill;
+        tc::mbar_expect_tx(bar, unit_bytes + (HALF ? 256 : 0));
+        const int from = wide ? r0 & ~31 : r0;               // (a unit's second half may lie behind the last key: its page is not looked for)
+        for (int x = 0; x < ka; ++x) tc::tma_load_2d(dst + x * NK * ATOM, &maps.k, x * (128 / ES), from, bar);
+        for (int x = 0; x < va; ++x) tc::tma_load_2d(dst + (ka + x) * NK * ATOM, &maps.v, x * (128 / ES), from, bar);
+        if (NK == 2 && !wide) {
+          for (int x = 0; x < ka; ++x) tc::tma_load_2d(dst + x * NK * ATOM + ATOM, &maps.k, x * (128 / ES), r1, bar);
+          for (int x = 0; x < va; ++x) tc::tma_load_2d(dst + (ka + x) * NK * ATOM + ATOM, &maps.v, x * (128 / ES), r1, bar);
+        }
+        if (HALF) {                                          // of a page that is not there: any scales
+          const int s1 = wide ? from + 16 : r1 == beyond ? 0 : r1, z = wide ? from : r0 == beyond ? 0 : r0;
+          bulk64(sc, a.ks + z, bar);
+          bulk64(sc + 64, a.ks + s1, bar);
+          bulk64(sc + 128, a.vs + z, bar);
+          bulk64(sc + 192, a.vs + s1, bar);
         }
       }
-    } else {
-      skipped |= 1u << fill;
     }
     if (++fill == stages) fill = 0;
   };
@@ -254,29 +267,32 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
     load();
     const int st = stage;
     if (++stage == stages) stage = 0;
-    if (skipped >> st & 1u) continue;
+    const uint32_t lost = gone >> 2 * st & 3u;
+    if (lost == 3u) continue;
     tc::mbar_wait_warp(bar0 + 8 * st, phase >> st & 1u, dead);
     phase ^= 1u << st;
     if (dead) break;
-    const uint32_t kb = ring + st * unit_bytes, vb = kb + ka * ATOM, sb = sc0 + 128 * st;
+    const uint32_t kb = ring + st * unit_bytes, vb = kb + NK * ka * ATOM, sb = sc0 + 256 * st;
     const int key0 = key0_of(i), valid = ks.end - key0;
-    if (valid < 16) {                                        // the last unit: what lies behind the last key that is seen may be anything
-      for (int x = lane; x < (16 - valid) * 8 * va; x += 32) {
+    if (valid < 16 * NK) {                                   // the last unit: what lies behind the last key that is seen may be anything
+      for (int x = lane; x < (16 * NK - valid) * 8 * va; x += 32) {
         const int r = valid + x / (8 * va), c = x % (8 * va);
-        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vb + (c >> 3) * ATOM + r * 128 + (c & 7) * 16), "r"(0u) : "memory");
+        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vb + (c >> 3) * NK * ATOM + r * 128 + (c & 7) * 16), "r"(0u) : "memory");
       }
       __syncwarp();
     }
-    float s[NR][4];
+    float s[NK][NR][4];
 #pragma unroll
-    for (int r = 0; r < NR; ++r)
+    for (int n = 0; n < NK; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[r][e] = 0.f;
-    auto score = [&](int k, const uint32_t (&key)[KP][4]) {
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][r][e] = 0.f;
+    auto score = [&](int n, int k, const uint32_t (&key)[KP][4]) {
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
         if constexpr (HELD) {
-          product<HALF, KP, QP, PRODUCTS, false>(s[r], key, held[k][r]);
+          product<HALF, KP, QP, PRODUCTS, false>(s[n][r], key, held[k][r]);
         } else {
           uint32_t q[QP][2];
 #pragma unroll
@@ -285,24 +301,27 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
             q[p][0] = u.x;
             q[p][1] = u.y;
           }
-          product<HALF, KP, QP, PRODUCTS, false>(s[r], key, q);
+          product<HALF, KP, QP, PRODUCTS, false>(s[n][r], key, q);
         }
       }
     };
     auto key_pieces = [&](int j) {                           // pieces 2 j, 2 j + 1 of the keys: PER steps
-      uint32_t r4[4];
-      ldsm_x4(kb + (j >> 2) * ATOM + (at_16 ^ ((j & 3) << 5)), r4);
 #pragma unroll
-      for (int x = 0; x < PER; ++x) {
-        uint32_t key[KP][4];
-        if constexpr (HALF) {
-          const uint2 u = codes4<STORE, 0, 1, 2, 3>(r4[2 * x]), v = codes4<STORE, 0, 1, 2, 3>(r4[2 * x + 1]);
-          key[0][0] = u.x; key[0][1] = v.x; key[0][2] = u.y; key[0][3] = v.y;
-        } else {
+      for (int n = 0; n < NK; ++n) {
+        uint32_t r4[4];
+        ldsm_x4(kb + ((j >> 2) * NK + n) * ATOM + (at_16 ^ ((j & 3) << 5)), r4);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) key[0][e] = r4[e];
+        for (int x = 0; x < PER; ++x) {
+          uint32_t key[KP][4];
+          if constexpr (HALF) {
+            const uint2 u = codes4<STORE, 0, 1, 2, 3>(r4[2 * x]), v = codes4<STORE, 0, 1, 2, 3>(r4[2 * x + 1]);
+            key[0][0] = u.x; key[0][1] = v.x; key[0][2] = u.y; key[0][3] = v.y;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) key[0][e] = r4[e];
+          }
+          score(n, PER * j + x, key);
         }
-        score(PER * j + x, key);
       }
     };
     if constexpr (F32 && !HALF) {
@@ -318,7 +337,7 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
 #pragma unroll
           for (int x = 0; x < KP; ++x) key[x][e] = p[x];
         }
-        score(k, key);
+        score(0, k, key);
       }
     } else if constexpr (HELD) {
 #pragma unroll
@@ -330,44 +349,58 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
 #pragma unroll 2
       for (int j = 0; j < steps / PER; ++j) key_pieces(j);
     }
-    // scores in powers of two; lane: keys g (entries 0, 1) and g + 8 (2, 3) of rows 2 t and 2 t + 1
-    float c[2] = {1.f, 1.f}, add[2] = {0.f, 0.f}, over[2], rest[2];      // one over what of the values' scales is in the exponent; what is not
+    // Scores in powers of two; lane: keys 16 n + g (entries 0, 1) and 16 n + g + 8 (2, 3) of rows 2 t and 2 t + 1.  Codes: a lane prepares one key's scales
+    float c[NK][2], add[NK][2], over[NK][2], rest[NK][2];    // one over what of the values' scales is in the exponent; what is not
     bool zeros = false;                                      // whether a value counts as zeros
-    if (HALF) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        c[e] = __uint_as_float(lds32(sb + (g + 8 * e) * 4));
-        const float v = __uint_as_float(lds32(sb + 64 + (g + 8 * e) * 4));
-        const bool zero = v >= 0.f && v <= 1.17549435e-38f;  // 2^-126 (a row of zeros) or 0 (never written): counts as zeros
-        const float some = zero ? SMALLEST_SCALE : v;
-        if (F32) {                                           // the power of two: exact; the rest of it goes with the weight
-          const int exponent = (int)(__float_as_uint(some) >> 23 & 255u);
-          add[e] = (float)(exponent - 127);
-          over[e] = __uint_as_float((uint32_t)(254 - exponent) << 23);
-          rest[e] = zero ? 0.f : v * over[e];
-        } else {                                             // all of it, to 2^-22 (of log2 s where that is larger than 1)
-          asm("lg2.approx.f32 %0, %1;" : "=f"(add[e]) : "f"(some));
-          asm("rcp.approx.f32 %0, %1;" : "=f"(over[e]) : "f"(some));
-          rest[e] = zero ? 0.f : 1.f;
-          zeros |= zero;
-        }
-        if (!(some >= SMALLEST_SCALE && some <= LARGEST_SCALE)) over[e] = NAN;
+    if constexpr (HALF) {
+      const float k1 = __uint_as_float(lds32(sb + lane * 4)), v = __uint_as_float(lds32(sb + 128 + lane * 4));
+      const bool zero = v >= 0.f && v <= 1.17549435e-38f;    // 2^-126 (a row of zeros) or 0 (never written): counts as zeros
+      const float some = zero ? SMALLEST_SCALE : v;
+      float a1, o1, r1;
+      if (F32) {                                             // the power of two: exact; the rest of it goes with the weight
+        const int exponent = (int)(__float_as_uint(some) >> 23 & 255u);
+        a1 = (float)(exponent - 127);
+        o1 = __uint_as_float((uint32_t)(254 - exponent) << 23);
+        r1 = zero ? 0.f : v * o1;
+      } else {                                               // all of it, to 2^-22 (of log2 s where that is larger than 1)
+        asm("lg2.approx.f32 %0, %1;" : "=f"(a1) : "f"(some));
+        asm("rcp.approx.f32 %0, %1;" : "=f"(o1) : "f"(some));
+        r1 = zero ? 0.f : 1.f;
+        zeros = __any_sync(0xffffffffu, zero);
       }
-      if (!F32) zeros = __any_sync(0xffffffffu, zeros);
+      if (!(some >= SMALLEST_SCALE && some <= LARGEST_SCALE)) o1 = NAN;
+#pragma unroll
+      for (int n = 0; n < NK; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int from = 16 * n + 8 * e + g;
+          c[n][e] = __shfl_sync(0xffffffffu, k1, from);
+          add[n][e] = __shfl_sync(0xffffffffu, a1, from);
+          over[n][e] = __shfl_sync(0xffffffffu, o1, from);
+          if (F32) rest[n][e] = __shfl_sync(0xffffffffu, r1, from);
+        }
+      if (!F32 && zeros)
+#pragma unroll
+        for (int n = 0; n < NK; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) rest[n][e] = __shfl_sync(0xffffffffu, r1, 16 * n + 8 * e + g);
     }
-    const bool whole = ks.whole(key0, 16);
+    const bool whole = lost == (NK == 2 ? 0u : 2u) && ks.whole(key0, 16 * NK);
     bool grows = false;
     float top[NR][2];
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[r][e] = HALF ? fmaf(s[r][e] * c[e >> 1], cr[r][e & 1], add[e >> 1]) : s[r][e] * a.scale_log2;
-        if (!whole && !a.sees(pos[r][e & 1], key0 + g + 8 * (e >> 1))) s[r][e] = -INFINITY;
-      }
+      for (int n = 0; n < NK; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[n][r][e] = HALF ? fmaf(s[n][r][e] * c[n][e >> 1], cr[r][e & 1], add[n][e >> 1]) : s[n][r][e] * a.scale_log2;
+          if (!whole && (lost >> n & 1u || !a.sees(pos[r][e & 1], key0 + 16 * n + g + 8 * (e >> 1)))) s[n][r][e] = -INFINITY;
+        }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        top[r][e] = fmaxf(s[r][e], s[r][2 + e]);
+        top[r][e] = fmaxf(s[0][r][e], s[0][r][2 + e]);
+        if (NK == 2) top[r][e] = fmaxf(top[r][e], fmaxf(s[NK - 1][r][e], s[NK - 1][r][2 + e]));
         top[r][e] = fmaxf(top[r][e], __shfl_xor_sync(0xffffffffu, top[r][e], 4));
         top[r][e] = fmaxf(top[r][e], __shfl_xor_sync(0xffffffffu, top[r][e], 8));
         top[r][e] = fmaxf(top[r][e], __shfl_xor_sync(0xffffffffu, top[r][e], 16));
@@ -391,28 +424,30 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
           for (int e = 0; e < 4; ++e) o[r][x][e] *= f[e & 1];
       }
     }
-    uint32_t wb[NR][WP][2];                                  // the weights as the B operand of the second product
+    uint32_t wb[NK][NR][WP][2];                              // the weights as the B operand of the second product
 #pragma unroll
-    for (int r = 0; r < NR; ++r)
+    for (int n = 0; n < NK; ++n)
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {                          // key g or g + 8
-        float x[2];
-        uint32_t w[WP];
+      for (int r = 0; r < NR; ++r)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float z = s[r][2 * k + e];
-          x[e] = exp2_f(F32 ? (z - m[r][e]) + LIFT : z - (m[r][e] - LIFT));
-          if (z == -INFINITY) x[e] = 0.f;                    // hidden, or of no weight: whatever its scale is, and while the maximum is -inf
-          else l[r][e] = HALF ? fmaf(x[e], over[k], l[r][e]) : l[r][e] + x[e];
-          if (HALF && (F32 || zeros)) x[e] = z == -INFINITY ? 0.f : x[e] * rest[k];
+        for (int k = 0; k < 2; ++k) {                        // key g or g + 8
+          float x[2];
+          uint32_t w[WP];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float z = s[n][r][2 * k + e];
+            x[e] = exp2_f(F32 ? (z - m[r][e]) + LIFT : z - (m[r][e] - LIFT));
+            if (z == -INFINITY) x[e] = 0.f;                  // hidden, or of no weight: whatever its scale is, and while the maximum is -inf
+            else l[r][e] = HALF ? fmaf(x[e], over[n][k], l[r][e]) : l[r][e] + x[e];
+            if (HALF && (F32 || zeros)) x[e] = z == -INFINITY ? 0.f : x[e] * rest[n][k];
+          }
+          operand2<HALF, WP>(x[0], x[1], w);
+#pragma unroll
+          for (int p = 0; p < WP; ++p) wb[n][r][p][k] = transposed(w[p]);
         }
-        operand2<HALF, WP>(x[0], x[1], w);
+    auto value = [&](int n, int x, const uint32_t (&v)[KP][4]) {      // 16 entries of the values
 #pragma unroll
-        for (int p = 0; p < WP; ++p) wb[r][p][k] = transposed(w[p]);
-      }
-    auto value = [&](int x, const uint32_t (&v)[KP][4]) {    // 16 entries of the values
-#pragma unroll
-      for (int r = 0; r < NR; ++r) product<HALF, KP, WP, V_PRODUCTS, F32>(o[r][x], v, wb[r]);
+      for (int r = 0; r < NR; ++r) product<HALF, KP, WP, V_PRODUCTS, F32>(o[r][x], v, wb[n][r]);
     };
     if constexpr (F32 && !HALF) {
 #pragma unroll
@@ -432,20 +467,23 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
 #pragma unroll
           for (int k = 0; k < KP; ++k) v[k][e] = p[k];
         }
-        value(x, v);
+        value(0, x, v);
       }
     } else if constexpr (HALF) {
 #pragma unroll
       for (int x = 0; x < (NV + 1) / 2; ++x) {               // 32 entries at a time; the last 16 may be the copy's zeros
         if (32 * x >= a.V) break;
-        uint32_t r4[4];
-        ldsm_x4_t(vb + (x >> 2) * ATOM + (at_16 ^ ((x & 3) << 5)), r4);
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          if (2 * x + y >= NV) break;
-          const uint2 lo = codes4<STORE, 0, 2, 1, 3>(r4[2 * y]), hi = codes4<STORE, 0, 2, 1, 3>(r4[2 * y + 1]);      // entries 2 g and 2 g + 1 of two keys
-          const uint32_t v[1][4] = {{lo.x, lo.y, hi.x, hi.y}};
-          value(2 * x + y, v);
+        for (int n = 0; n < NK; ++n) {
+          uint32_t r4[4];
+          ldsm_x4_t(vb + ((x >> 2) * NK + n) * ATOM + (at_16 ^ ((x & 3) << 5)), r4);
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            if (2 * x + y >= NV) break;
+            const uint2 lo = codes4<STORE, 0, 2, 1, 3>(r4[2 * y]), hi = codes4<STORE, 0, 2, 1, 3>(r4[2 * y + 1]);      // entries 2 g and 2 g + 1 of two keys
+            const uint32_t v[1][4] = {{lo.x, lo.y, hi.x, hi.y}};
+            value(n, 2 * x + y, v);
+          }
         }
       }
     } else {
@@ -454,7 +492,7 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
         if (16 * x >= a.V) break;
         uint32_t v[1][4];
         ldsm_x4_t(vb + (x >> 2) * ATOM + (at_8 ^ ((x & 3) << 5)), v[0]);
-        value(x, v);
+        value(0, x, v);
       }
     }
   }
@@ -672,14 +710,14 @@ static Plan plan_of(int rows, int seqs, int width, int page, int heads, int kv_h
 
 template <typename act_t, int STORE, int NV, int NR> static int few_launch(const Attn& a, int tiles, cudaStream_t stream) {
   constexpr int ES = STORE == ACT ? (int)sizeof(act_t) : 1, PER = ES == 1 ? 2 : 1;
-  const size_t queries = (size_t)(sizeof(act_t) == 4 ? 3 : 1) * ((a.K / 16 + PER - 1) / PER * PER) * NR * 256, unit = (size_t)(atoms_of(a.K, ES) + atoms_of(a.V, ES)) * ATOM;
+  const size_t queries = (size_t)(sizeof(act_t) == 4 ? 3 : 1) * ((a.K / 16 + PER - 1) / PER * PER) * NR * 256, unit = (size_t)(atoms_of(a.K, ES) + atoms_of(a.V, ES)) * ATOM * (ES == 1 ? 2 : 1);
   // four warps and as many CTAs on an SM as leave each warp two units in its ring at least; fewer warps where one CTA does not fit
-  constexpr size_t SM = 227 * 1024, OTHER = 6 * 1024;        // static: barriers, scales; the system's 1 KB
+  constexpr size_t SM = 227 * 1024, OTHER = ES == 1 ? 6 * 1024 : 2 * 1024;      // static: barriers, scales; the system's 1 KB
   int W = 4, stages = 0;
   for (int ctas = NV <= 8 ? (NR == 1 && ES == 1 ? 4 : 3) : 2; ctas >= 1 && stages < 2; --ctas)
     for (W = 4; W >= (ctas == 1 ? 1 : 4); W /= 2) {
       const size_t room = SM / ctas - OTHER;
-      stages = room > queries ? (int)std::min<size_t>(MOST_STAGES, (room - queries) / (W * unit)) : 0;
+      stages = room > queries ? (int)std::min<size_t>(most_stages(STORE), (room - queries) / (W * unit)) : 0;
       if (stages >= 2) break;
     }
   B2L_CHECK_SUPPORTED(stages >= 2, "b2l_seq_paged_attention: heads of %d and %d entries do not fit", a.K, a.V);
@@ -687,8 +725,9 @@ template <typename act_t, int STORE, int NV, int NR> static int few_launch(const
   const CUtensorMapDataType type = ES == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : ES == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   const long long rows = ((long long)a.s.pages * a.kv_heads) << a.s.shift;
   FewMaps maps;
-  if (int rc = tc::map_sw128(&maps.k, type, ES, a.k, rows, a.K, a.K, 128 / ES, 16)) return rc;
-  if (int rc = tc::map_sw128(&maps.v, type, ES, a.v, rows, a.V, a.V, 128 / ES, 16)) return rc;
+  const int box = ES == 1 && a.s.shift >= 5 ? 32 : 16;
+  if (int rc = tc::map_sw128(&maps.k, type, ES, a.k, rows, a.K, a.K, 128 / ES, box)) return rc;
+  if (int rc = tc::map_sw128(&maps.v, type, ES, a.v, rows, a.V, a.V, 128 / ES, box)) return rc;
   static DynSmemCache cache;
   auto kernel = paged_few_kernel<act_t, STORE, NV, NR>;
   if (int rc = ensure_dyn_smem(kernel, smem, cache)) return rc;

@@ -195,7 +195,7 @@ def units_of(p_min, p_max, window, first, shift):
     return [(u if u < e else u - e + (lo >> shift)) << shift for u in range(n)]
 
 
-@pytest.mark.parametrize("shift", [4, 7])
+@pytest.mark.parametrize("shift", [4, 5, 7])
 def test_units_cover_what_is_seen_once_and_splits_cover_the_units(shift):
     size = 1 << shift
     for p_min, rows in ((-3, 2), (0, 1), (0, 5), (15, 1), (16, 1), (300, 40), (1000, 128), (517, 3)):
