@@ -132,13 +132,18 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
   extern __shared__ __align__(1024) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5, g = lane >> 2, t = lane & 3;
   const int h = blockIdx.y, split = blockIdx.z, G = a.heads / a.kv_heads, steps = (a.K / 16 + PER - 1) / PER * PER;
+  // The first tile of every sequence, found without looking through the others, and then the rest of those that have more
   Place pl;
-  if (!a.place(blockIdx.x, R, 0, a.few_max, lane, pl)) return;
-  const Keys ks = a.keys(pl, R);
-  const int all = ks.units(SHIFT), per = (all + a.few.splits - 1) / a.few.splits;
-  const int u_begin = min(split * per, all), u_end = min(u_begin + per, all);
+  if ((int)blockIdx.x < a.s.seqs) {
+    pl.b = blockIdx.x;
+    sequence(a.s, pl.b, pl.start, pl.n, pl.length);
+    pl.first = 0;
+    if (pl.n == 0 || (long long)pl.n * G > a.few_max) return;
+  } else if (!a.place(blockIdx.x - a.s.seqs, R, 0, a.few_max, 1, lane, pl)) {
+    return;
+  }
   __shared__ uint32_t bad;                                   // rows whose result is not finite
-  __shared__ float lifted[2][16];                            // what a row of queries is multiplied with for f16, and a score with to undo it
+  __shared__ uint32_t largest[16];                           // entry of a row of queries, as bits
   __shared__ __align__(8) uint64_t bars[4 * STAGES];
   __shared__ __align__(16) float scales[HALF ? 4 * STAGES * 64 : 4];
   const int ka = atoms_of(a.K, ES), va = atoms_of(a.V, ES), unit_bytes = NK * (ka + va) * ATOM;
@@ -146,12 +151,45 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
   const uint32_t ring = s0 + (uint32_t)(warp * stages * unit_bytes), sq = s0 + (uint32_t)(W * stages * unit_bytes);
   const uint32_t bar0 = tc::smem_u32(bars) + warp * STAGES * 8, sc0 = tc::smem_u32(scales) + warp * STAGES * 256;
   uint8_t* queries = smem + W * stages * unit_bytes;
-  if (threadIdx.x == 0) bad = 0u;
   if (lane == 0) {
     for (int i = 0; i < stages; ++i) tc::mbar_init(bar0 + 8 * i, 1);
     tc::mbar_init_fence();
   }
   __syncwarp();
+  uint32_t dead = (s0 & 1023u) ? 1u : 0u, phase = 0;         // swizzled atoms need 1024-byte alignment
+  int fill = 0, stage = 0;                                   // stage that is filled next, and read next
+  const Keys ks = a.keys(pl, R);
+  const int all = ks.units(SHIFT), per = (all + a.few.splits - 1) / a.few.splits;
+  const int u_begin = min(split * per, all), u_end = min(u_begin + per, all);
+  // Queries on their way while the first pages are looked up: entries d0, + 1 and d1, + 1 of a row, as the B operand has them: row g of a column by entries 2 t, + 1 and
+  // 8 + 2 t, + 1 of a k16 step, or (codes) 4 t .. 4 t + 3
+  auto place_of = [&](int i, int& k, int& r, int& l) {
+    const int x = threadIdx.x + i * blockDim.x;
+    k = x / (32 * NR);
+    l = x & 31;
+    r = 8 * ((x >> 5) % NR) + (l >> 2);
+    return k < steps;
+  };
+  auto query = [&](int k, int r, int l, float (&x)[4]) {
+    const int at = pl.first + r, d0 = HALF ? 4 * (l & 3) : 2 * (l & 3), d1 = HALF ? d0 + 2 : d0 + 8;
+    x[0] = x[1] = x[2] = x[3] = 0.f;
+    if (at < pl.n * G && 16 * k < a.K) {
+      const act_t* src = reinterpret_cast<const act_t*>(a.q) + (pl.start + at / G) * a.ldq + (h * G + at % G) * a.hsq + 16 * k;
+      x[0] = ld_act(src, d0);
+      x[1] = ld_act(src, d0 + 1);
+      x[2] = ld_act(src, d1);
+      x[3] = ld_act(src, d1 + 1);
+    }
+  };
+  constexpr int AHEAD = 4;                                   // places of a thread that are loaded ahead: all of them for up to 128 entries and 16 rows
+  float early[AHEAD][4];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) {
+    int k, r, l;
+    if (place_of(i, k, r, l)) query(k, r, l, early[i]);
+  }
+  if (threadIdx.x == 0) bad = 0u;
+  if (threadIdx.x < 16) largest[threadIdx.x] = 0u;
 
   const int count = u_begin + warp < u_end ? (u_end - u_begin - warp + W - 1) / W : 0;      // this warp's units: u_begin + warp + W i
   auto key0_of = [&](int i) { return ks.key0(u_begin + warp + W * i, SHIFT); };
@@ -161,7 +199,7 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
   const bool wide = NK == 2 && a.s.shift >= 5;               // a unit is in one page: one copy
   int row_of = beyond;
   uint32_t gone = 0;                                         // 16-key parts of the ring's stages whose page is not there
-  int fill = 0, next = 0;                                    // stage that is filled next, and unit
+  int next = 0;                                              // unit that is loaded next
   auto load = [&]() {
     if (next >= count) return;
     if ((next & (32 / NK - 1)) == 0) {
@@ -196,38 +234,38 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
   };
   for (int i = 0; i < stages - 1; ++i) load();
 
-  // the queries as the B operand's registers, part by part: row g of a column by entries 2 t, + 1 and 8 + 2 t, + 1 of a k16 step, or (codes) 4 t .. 4 t + 3
-  if (HALF) {
-    for (int r = warp; r < R; r += W) {
-      const int at = pl.first + r;
-      float top = 0.f;
-      if (at < pl.n * G)
-        for (int d = lane; d < a.K; d += 32) top = fmaxf(top, fabsf(ld_act(reinterpret_cast<const act_t*>(a.q), (pl.start + at / G) * a.ldq + (h * G + at % G) * a.hsq + d)));
-      top = warp_max(top);
-      if (lane == 0) lift_of(top, a.scale_log2, lifted[0][r], lifted[1][r]);
+  __syncthreads();
+  auto each_place = [&](auto&& take) {                       // take(place, step, row, lane, entries)
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      int k, r, l;
+      if (place_of(i, k, r, l)) take(i, k, r, l, early[i]);
     }
+    int k, r, l;
+    for (int i = AHEAD; place_of(i, k, r, l); ++i) {
+      float x[4];
+      query(k, r, l, x);
+      take(i, k, r, l, x);
+    }
+  };
+  if (HALF) {                                                // the largest entry of every row
+    each_place([&](int, int, int r, int l, const float (&x)[4]) {
+      float top = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      if ((l & 3) == 0) atomicMax(&largest[r], __float_as_uint(top));
+    });
     __syncthreads();
   }
-  for (int i = threadIdx.x; i < steps * NR * 32; i += blockDim.x) {
-    const int s = i / (32 * NR), l = i & 31, r = 8 * ((i >> 5) % NR) + (l >> 2), at = pl.first + r;
-    const act_t* src = reinterpret_cast<const act_t*>(a.q) + (pl.start + at / G) * a.ldq + (h * G + at % G) * a.hsq + 16 * s;
-    const int d0 = HALF ? 4 * (l & 3) : 2 * (l & 3), d1 = HALF ? d0 + 2 : d0 + 8;
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    if (at < pl.n * G && 16 * s < a.K) {
-      x[0] = ld_act(src, d0);
-      x[1] = ld_act(src, d0 + 1);
-      x[2] = ld_act(src, d1);
-      x[3] = ld_act(src, d1 + 1);
-    }
-    if (HALF)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] *= lifted[0][r];
+  each_place([&](int i, int, int r, int, const float (&x)[4]) {
+    float up = 1.f, down;
+    if (HALF) lift_of(__uint_as_float(largest[r]), a.scale_log2, up, down);
     uint32_t p[2][QP];
-    operand2<HALF, QP>(x[0], x[1], p[0]);
-    operand2<HALF, QP>(x[2], x[3], p[1]);
+    operand2<HALF, QP>(x[0] * up, x[1] * up, p[0]);
+    operand2<HALF, QP>(x[2] * up, x[3] * up, p[1]);
 #pragma unroll
-    for (int q = 0; q < QP; ++q) *reinterpret_cast<uint2*>(queries + q * steps * NR * 256 + i * 8) = make_uint2(p[0][q], p[1][q]);
-  }
+    for (int q = 0; q < QP; ++q) *reinterpret_cast<uint2*>(queries + q * steps * NR * 256 + (threadIdx.x + i * blockDim.x) * 8) = make_uint2(p[0][q], p[1][q]);
+  });
   __syncthreads();
   uint32_t held[HELD ? NV : 1][NR][1][2];
   if (HELD)
@@ -249,7 +287,11 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
       const int at = 8 * r + 2 * t + e;
       m[r][e] = -INFINITY;
       l[r][e] = 0.f;
-      cr[r][e] = HALF ? lifted[1][at] : a.scale_log2;
+      cr[r][e] = a.scale_log2;
+      if (HALF) {
+        float up;
+        lift_of(__uint_as_float(largest[at]), a.scale_log2, up, cr[r][e]);
+      }
       pos[r][e] = pl.first + at < pl.n * G ? pl.length - pl.n + (pl.first + at) / G : -1;
     }
 #pragma unroll
@@ -260,8 +302,6 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
   // where this lane's row of an ldmatrix lies: row lane & 15, piece lane / 16 of two; or (bf16 values) row (lane & 7) + 8 (lane / 16), piece lane / 8 % 2
   const uint32_t at_16 = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) << 4), at_8 = ((lane & 7) + (lane >> 4) * 8) * 128 + (((lane >> 3 & 1) ^ (lane & 7)) << 4);
 
-  uint32_t dead = (s0 & 1023u) ? 1u : 0u, phase = 0;         // swizzled atoms need 1024-byte alignment
-  int stage = 0;
   for (int i = 0; i < count; ++i) {
     __syncwarp();                                            // every lane has done with the stage that is filled next
     load();
@@ -600,6 +640,7 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const __g
   const long long at = few && a.compact ? (long long)(b * a.kv_heads + h) * 16 + (row - start) * G + head % G : (long long)row * a.heads + head;
   float M = -INFINITY, L = 0.f;
   float4 x[2] = {};
+  pdl_wait();                                                // launched while the parts are computed
   if (on) {
 #pragma unroll 4
     for (int i = sub; i < p.splits; i += per) {
@@ -675,7 +716,7 @@ static Plan plan_of(int rows, int seqs, int width, int page, int heads, int kv_h
   const int most = std::min(seqs, rows);
   // rows of a tile: 8 where a token's heads, or all that the longest of the sequences has, fit
   p.few_rows = (max_new > 0 ? (long long)max_new * G <= 8 : G <= 8 && packed <= 8ll * most) && !p.compact ? 8 : 16;
-  p.few_tiles = p.compact ? most : (int)std::min<long long>(packed / p.few_rows + most, INT32_MAX);
+  p.few_tiles = seqs + (p.compact ? 0 : (int)std::min<long long>(packed / p.few_rows, INT32_MAX - seqs));
   p.many_tiles = (int)std::min<long long>(packed / 256 + most, INT32_MAX);
   long long keys = (long long)width * page;                  // the most keys that a row sees
   if (max_length > 0) keys = std::min<long long>(keys, max_length);
@@ -686,9 +727,9 @@ static Plan plan_of(int rows, int seqs, int width, int page, int heads, int kv_h
   if (p.few) {
     // an SM has three or four CTAs at a time.  Few CTAs: as many parts as fill them once.  Many: parts of a quarter of that each, so that sequences of
     // different lengths share the SMs evenly
-    const long long ctas = (long long)kv_heads * std::max(1, p.few_tiles), slots = 3ll * sms;
+    const long long ctas = (long long)kv_heads * std::max<long long>(seqs, p.compact ? 0 : packed / p.few_rows), slots = 3ll * sms;
     const long long want = 2 * ctas <= slots ? slots / ctas : (4 * slots + ctas - 1) / ctas;
-    p.few_splits = (int)std::max<long long>(1, std::min({want, keys / 256, 128ll, MOST_WORK / (p.few_count * (V + 2) + 1)}));
+    p.few_splits = (int)std::max<long long>(1, std::min({want, keys / 128, 128ll, MOST_WORK / (p.few_count * (V + 2) + 1)}));
   }
   if (p.many) {
     // One CTA on an SM at a time, 2.3 us for 128 keys: as many parts as make the rounds shortest, where the last one is seldom full.  A part's results are
@@ -802,7 +843,8 @@ extern "C" int b2l_seq_paged_attention(const void* q, long long ldq, long long h
     const bool short_only = p.compact && a.many.splits == 1;
     const long long units = short_only ? 16ll * kv_heads * seqs : (long long)rows * heads;
     B2L_CHECK_SUPPORTED(units < (1ll << 31), "%s: sizes beyond the grid's", who);
-    paged_merge_kernel<<<(unsigned)((units + here - 1) / here), 32 * MERGE_WARPS, 0, st>>>(a, per, short_only);
+    LaunchCfg launch(dim3((unsigned)((units + here - 1) / here)), dim3(32 * MERGE_WARPS), 0, st, true);
+    B2L_CUDA(cudaLaunchKernelEx(&launch.cfg, paged_merge_kernel, a, per, (int)short_only));
     B2L_LAUNCH_CHECK("paged_merge_kernel");
   }
   return 0;

@@ -73,8 +73,9 @@ struct Attn {
 
   __device__ __forceinline__ bool sees(int pos, int j) const { return j <= pos && (window == 0 || j > pos - window || j < first); }
 
-  // Tile `slot` of the tiles of R packed rows of all sequences with more than `above` and at most `most` packed rows; a whole warp looks
-  __device__ __forceinline__ bool place(int slot, int R, int above, int most, int lane, Place& pl) const {
+  // Tile `slot` of the tiles of R packed rows, without the first `skip` of each, of all sequences with more than `above` and at most `most` packed rows; a
+  // whole warp looks
+  __device__ __forceinline__ bool place(int slot, int R, int above, int most, int skip, int lane, Place& pl) const {
     const int G = heads / kv_heads;
     int base = 0;
     for (int b0 = 0; b0 < s.seqs; b0 += 32) {
@@ -83,7 +84,7 @@ struct Attn {
       if (b < s.seqs) {
         sequence(s, b, start, n, length);
         const long long packed = (long long)n * G;
-        tiles = packed > above && packed <= most ? (int)((packed + R - 1) / R) : 0;
+        tiles = packed > above && packed <= most ? max((int)((packed + R - 1) / R) - skip, 0) : 0;
       }
       int upto = tiles;
 #pragma unroll
@@ -98,7 +99,7 @@ struct Attn {
         pl.start = __shfl_sync(0xffffffffu, start, at);
         pl.n = __shfl_sync(0xffffffffu, n, at);
         pl.length = __shfl_sync(0xffffffffu, length, at);
-        pl.first = (slot - base - __shfl_sync(0xffffffffu, upto - tiles, at)) * R;
+        pl.first = (slot - base - __shfl_sync(0xffffffffu, upto - tiles, at) + skip) * R;
         return true;
       }
       base += __shfl_sync(0xffffffffu, upto, 31);

@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
   uint32_t* there_of = reinterpret_cast<uint32_t*>(smem + CONTROL_BYTES);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.heads / a.kv_heads, h = blockIdx.y, split = blockIdx.z;
   Place pl;
-  if (!a.place(gridDim.x - 1 - blockIdx.x, ROWS, a.few_max, INT32_MAX, lane, pl)) return;      // later rows, with more keys, first
+  if (!a.place(gridDim.x - 1 - blockIdx.x, ROWS, a.few_max, INT32_MAX, 0, lane, pl)) return;      // later rows, with more keys, first
   const int rows = min(ROWS, pl.n * G - pl.first), groups = rows > TILE ? 2 : 1;
   const Keys keys = a.keys(pl, ROWS);
   const int all = keys.units(7), per = (all + a.many.splits - 1) / a.many.splits;
