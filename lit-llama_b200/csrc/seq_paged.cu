@@ -51,16 +51,59 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8]) {
   }
   *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
-template <int STORE> __device__ __forceinline__ uint2 codes8(const float (&x)[8], float s) {
-  uint32_t w[2] = {0u, 0u};
-  if (s == s) {
+// Eight entries as they lie: the largest absolute value as f32 bits (an infinity's or more where one is not finite), and the entries
+struct Raw8f { float4 a, b; };
+__device__ __forceinline__ Raw8f raw8(const float* p) { return {*reinterpret_cast<const float4*>(p), *reinterpret_cast<const float4*>(p + 4)}; }
+__device__ __forceinline__ uint4 raw8(const __nv_bfloat16* p) { return *reinterpret_cast<const uint4*>(p); }
+__device__ __forceinline__ void clear(Raw8f& w) { w.a = w.b = make_float4(0.f, 0.f, 0.f, 0.f); }
+__device__ __forceinline__ void clear(uint4& w) { w = make_uint4(0u, 0u, 0u, 0u); }
+__device__ __forceinline__ uint32_t largest8(const Raw8f& w) {
+  auto bits = [](float x) { return __float_as_uint(x) & 0x7fffffffu; };
+  return max(max(max(bits(w.a.x), bits(w.a.y)), max(bits(w.a.z), bits(w.a.w))), max(max(bits(w.b.x), bits(w.b.y)), max(bits(w.b.z), bits(w.b.w))));
+}
+__device__ __forceinline__ uint32_t largest8(const uint4& w) {      // two entries at a time
+  const uint32_t m = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+  return max(m << 16, m & 0xffff0000u);
+}
+__device__ __forceinline__ void entries8(const Raw8f& w, float (&x)[8]) {
+  x[0] = w.a.x; x[1] = w.a.y; x[2] = w.a.z; x[3] = w.a.w; x[4] = w.b.x; x[5] = w.b.y; x[6] = w.b.z; x[7] = w.b.w;
+}
+__device__ __forceinline__ void entries8(const uint4& w, float (&x)[8]) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float a = __fdiv_rn(x[2 * i], s), b = __fdiv_rn(x[2 * i + 1], s);
-      uint32_t c;
-      if (STORE == E4M3) c = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-      else c = (uint32_t)(__float2int_rn(fminf(fmaxf(a, -127.f), 127.f)) & 0xff) | (uint32_t)(__float2int_rn(fminf(fmaxf(b, -127.f), 127.f)) & 0xff) << 8;
-      w[i >> 1] |= c << 16 * (i & 1);
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(u[i] << 16);
+    x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+  }
+}
+// x / s correctly rounded, two at a time: the quotient by the correctly rounded reciprocal, corrected by its own remainder (Markstein).  The remainder is exact
+// while it is a normal number, so for s above 2^-90 or so; below the division operator (a third of the instructions of a row otherwise)
+__device__ __forceinline__ void over2(float& x, float& y, float s, float r) {
+  asm("{\n\t.reg .b64 a, q, d, r, s;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 r, {%2, %2};\n\tmov.b64 s, {%3, %3};\n\tmul.rn.f32x2 q, a, r;\n\tfma.rn.f32x2 d, q, s, a;\n\t"
+      "fma.rn.f32x2 q, d, r, q;\n\tmov.b64 {%0, %1}, q;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(r), "f"(-s));
+}
+template <int STORE> __device__ __forceinline__ uint2 codes8(float (&x)[8], float s, float r) {      // s: not NaN
+  if (s > 8.077935669463161e-28f) {                          // 2^-90
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) over2(x[i], x[i + 1], s, r);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __fdiv_rn(x[i], s);
+  }
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (STORE == E4M3) {
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i], x[4 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i + 2], x[4 * i + 3]), __NV_SATFINITE, __NV_E4M3);
+      w[i] = lo | hi << 16;
+    } else {                                                 // 1.5 2^23 more: the nearest integer in the low byte; |x / s| is at most 127 (1 + 2^-22)
+      uint32_t b[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) b[e] = __float_as_uint(x[4 * i + e] + 12582912.f);
+      w[i] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
     }
   }
   return make_uint2(w[0], w[1]);
@@ -80,7 +123,7 @@ template <int STORE> __device__ __forceinline__ void values8(uint2 w, float s, f
   }
 }
 
-template <typename act_t, int STORE>
+template <typename act_t, int STORE, int NI>      // NI: 128-entry parts of the longest row
 __global__ void __launch_bounds__(256) paged_write_kernel(const __grid_constant__ Rows a) {
   const int lane = threadIdx.x & 31, l = lane & 15;
   const bool value = lane >= 16;
@@ -89,16 +132,15 @@ __global__ void __launch_bounds__(256) paged_write_kernel(const __grid_constant_
   const int row = (int)(unit / groups), h0 = (int)(unit % groups) * HEADS;
   if (row >= a.s.rows) return;
   const int D = value ? a.V : a.K;
-  const act_t* src = reinterpret_cast<const act_t*>(value ? a.v_new : a.k_new) + row * (value ? a.ldv : a.ldk) + h0 * (value ? a.hsv : a.hsk);
-  float x[HEADS][2][8];
+  const long long hs = value ? a.hsv : a.hsk;
+  const act_t* src = reinterpret_cast<const act_t*>(value ? a.v_new : a.k_new) + row * (value ? a.ldv : a.ldk) + h0 * hs + 8 * l;
+  decltype(raw8(src)) raw[HEADS][NI];
 #pragma unroll
   for (int h = 0; h < HEADS; ++h)
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (h0 + h < a.kv_heads && 8 * (l + 16 * i) < D) load8(src + h * (value ? a.hsv : a.hsk) + 8 * (l + 16 * i), x[h][i]);
-      else
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[h][i][e] = 0.f;
+    for (int i = 0; i < NI; ++i)
+      if (h0 + h < a.kv_heads && 8 * (l + 16 * i) < D) raw[h][i] = raw8(src + h * hs + 128 * i);
+      else clear(raw[h][i]);
   const int b = sequence_of(a.s, row, lane);
   if (b < 0) return;
   int start, n, length;
@@ -106,34 +148,32 @@ __global__ void __launch_bounds__(256) paged_write_kernel(const __grid_constant_
   const int p = length - n + row - start;
   const int page = p >= 0 ? page_of(a.s, b, p) : -1;
   if (page < 0) return;
-  const int in_page = p & ((1 << a.s.shift) - 1);
+  size_t at = (((size_t)page * a.kv_heads + h0) << a.s.shift) + (p & ((1 << a.s.shift) - 1));
 #pragma unroll
-  for (int h = 0; h < HEADS; ++h) {
+  for (int h = 0; h < HEADS; ++h, at += (size_t)1 << a.s.shift) {
     if (h0 + h >= a.kv_heads) break;
-    const size_t at = (((size_t)page * a.kv_heads + h0 + h) << a.s.shift) + in_page;
-    float s = 1.f;
-    if (STORE != ACT) {
-      float top = 0.f;
-      bool odd = false;
+    if (STORE == ACT) {
+      act_t* dst = reinterpret_cast<act_t*>(value ? a.v : a.k) + at * D + 8 * l;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          top = fmaxf(top, fabsf(x[h][i][e]));
-          odd |= !(fabsf(x[h][i][e]) < CUDART_INF_F);
-        }
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const uint32_t odds = __ballot_sync(0xffffffffu, odd);
-      s = (value ? odds >> 16 : odds & 0xffffu) ? CUDART_NAN_F : fmaxf(top * (STORE == E4M3 ? 1.f / 448.f : 1.f / 127.f), 1.17549435e-38f);
-      if (l == 0) (value ? a.vs : a.ks)[at] = s;
+      for (int i = 0; i < NI; ++i)
+        if (8 * (l + 16 * i) < D) *reinterpret_cast<decltype(raw8(src))*>(dst + 128 * i) = raw[h][i];
+      continue;
     }
+    uint32_t top = 0u;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int c = 8 * (l + 16 * i);
-      if (c >= D) break;
-      if (STORE == ACT) store8(reinterpret_cast<act_t*>(value ? a.v : a.k) + at * D + c, x[h][i]);
-      else *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(value ? a.v : a.k) + at * D + c) = codes8<STORE>(x[h][i], s);
+    for (int i = 0; i < NI; ++i) top = max(top, largest8(raw[h][i]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const bool odd = top >= 0x7f800000u;                     // an infinity or NaN
+    const float s = odd ? CUDART_NAN_F : fmaxf(__uint_as_float(top) * (STORE == E4M3 ? 1.f / 448.f : 1.f / 127.f), 1.17549435e-38f), r = __frcp_rn(s);
+    if (l == 0) (value ? a.vs : a.ks)[at] = s;
+    uint8_t* dst = reinterpret_cast<uint8_t*>(value ? a.v : a.k) + at * D + 8 * l;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      if (8 * (l + 16 * i) >= D) break;
+      float x[8];
+      entries8(raw[h][i], x);
+      *reinterpret_cast<uint2*>(dst + 128 * i) = odd ? make_uint2(0u, 0u) : codes8<STORE>(x, s, r);
     }
   }
 }
@@ -201,8 +241,10 @@ static int rows_call(const char* who, const void* k_new, long long ldk, long lon
   const long long blocks = (units + warps - 1) / warps;
   B2L_CHECK_SUPPORTED(blocks < (1ll << 31), "%s: %d rows of %d heads", who, rows, kv_heads);
   const cudaStream_t st = (cudaStream_t)stream;
-#define GO(T, ST)                                                                                             \
-  (WRITE ? paged_write_kernel<T, ST><<<(unsigned)blocks, 32 * warps, 0, st>>>(a) : paged_read_kernel<T, ST><<<(unsigned)blocks, 32 * warps, 0, st>>>(a))
+#define GO(T, ST)                                                                                                      \
+  (!WRITE ? paged_read_kernel<T, ST><<<(unsigned)blocks, 32 * warps, 0, st>>>(a)                                        \
+   : K <= 128 && V <= 128 ? paged_write_kernel<T, ST, 1><<<(unsigned)blocks, 32 * warps, 0, st>>>(a)                    \
+                          : paged_write_kernel<T, ST, 2><<<(unsigned)blocks, 32 * warps, 0, st>>>(a))
   B2L_SEQ_DISPATCH(act_dtype, if (store == ACT) GO(act_t, ACT); else if (store == E4M3) GO(act_t, E4M3); else GO(act_t, INT8));
 #undef GO
   B2L_LAUNCH_CHECK("paged rows");

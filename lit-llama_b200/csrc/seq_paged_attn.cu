@@ -725,11 +725,13 @@ static Plan plan_of(int rows, int seqs, int width, int page, int heads, int kv_h
   p.few_count = p.compact ? (long long)seqs * kv_heads * 16 : (long long)rows * heads;
   p.many_count = (long long)rows * heads;
   if (p.few) {
-    // an SM has three or four CTAs at a time.  Few CTAs: as many parts as fill them once.  Many: parts of a quarter of that each, so that sequences of
-    // different lengths share the SMs evenly
+    // An SM has three CTAs at a time.  Few CTAs: as many parts as fill them once, of 128 keys at least (one token over 1031 keys of 32 heads: 15.1 us in 4 parts,
+    // 13.0 in 8).  Many: parts of a quarter of that each, of 512 keys at least, so that sequences of different lengths share the SMs evenly (48 over up to 8192
+    // keys of an e4m3 pool: 143 us whole, 128 in 4 parts, 140 in 8)
     const long long ctas = (long long)kv_heads * std::max<long long>(seqs, p.compact ? 0 : packed / p.few_rows), slots = 3ll * sms;
-    const long long want = 2 * ctas <= slots ? slots / ctas : (4 * slots + ctas - 1) / ctas;
-    p.few_splits = (int)std::max<long long>(1, std::min({want, keys / 128, 128ll, MOST_WORK / (p.few_count * (V + 2) + 1)}));
+    const bool room = 2 * ctas <= slots;
+    const long long want = room ? slots / ctas : (4 * slots + ctas - 1) / ctas;
+    p.few_splits = (int)std::max<long long>(1, std::min({want, keys / (room ? 128 : 512), 128ll, MOST_WORK / (p.few_count * (V + 2) + 1)}));
   }
   if (p.many) {
     // One CTA on an SM at a time, 2.3 us for 128 keys: as many parts as make the rounds shortest, where the last one is seldom full.  A part's results are
