@@ -46,12 +46,18 @@ class PagedStep:
             raise ValueError(f"paged step: {lengths.numel()} lengths, {starts.numel()} starts (one more is wanted), a table of {tuple(table.shape)}")
         if rows < 0:
             raise ValueError("paged step: a negative number of rows")
-        self.starts, self.lengths, self.table, self.rows, self.seqs = starts, lengths, table, int(rows), lengths.numel()
+        self._tensors, self.rows, self.seqs = (starts, lengths, table), int(rows), lengths.numel()
         self.device = lengths.device
         self.max_new, self.max_length = max(int(max_new), 0), max(int(max_length), 0)
         # all have the same number where that is the most there can be
         self.min_new = self.max_new if self.seqs and self.max_new * self.seqs == self.rows else max(int(min_new), 0)
-        self._work: Dict[tuple, int] = {}
+        self._at = (S.ptr(starts), S.ptr(lengths), S.ptr(table), table.stride(0), table.shape[1]) if lengths.is_cuda else None
+        self._plans: Dict[tuple, tuple] = {}                                # of attend: what does not change from layer to layer
+
+    # the kernels have the tensors' addresses: their contents may change, they stay
+    starts = property(lambda self: self._tensors[0])
+    lengths = property(lambda self: self._tensors[1])
+    table = property(lambda self: self._tensors[2])
 
     @classmethod
     def of(cls, sequences: Sequence[Tuple[int, int, Sequence[int]]], device, *, width: int = 0) -> "PagedStep":
@@ -167,15 +173,23 @@ class PagedCache:
                 raise ValueError(f"paged cache: a pool in {k.dtype} for activations in {self.dtype}")
         if not (k.is_contiguous() and v.is_contiguous()):
             raise ValueError("paged cache: the pool must be contiguous")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.n_pages, self.kv_heads, self.page, self.dim = k.shape
-        self.vdim = v.shape[3]
+        self._pool = (k, v, k_scale, v_scale)
+        (self.n_pages, self.kv_heads, self.page, self.dim), self.vdim = k.shape, v.shape[3]
         if self.n_pages < 1 or self.kv_heads < 1 or self.page not in PAGES:
             raise ValueError(f"paged cache: {self.n_pages} pages of {self.kv_heads} heads, {self.page} tokens: at least one, of {PAGES}")
         if any(d < 16 or d > 256 or d % 16 for d in (self.dim, self.vdim)):
             raise ValueError(f"paged cache: heads of {self.dim} and {self.vdim} entries: multiples of 16 up to 256")
         self.device = k.device
         self._codes = (STORES[self.store], S.act_code(self.dtype))
+        self._sizes = (self.n_pages, self.page, self.kv_heads, self.dim, self.vdim) + self._codes
+        self._per = 4 if self.dtype == torch.float32 else 8                 # entries in 16 bytes
+        self._at = tuple(S.ptr(t) for t in (k, v, k_scale, v_scale)) if k.is_cuda else None
+
+    # the kernels have the tensors' addresses: their contents may change, they stay
+    k = property(lambda self: self._pool[0])
+    v = property(lambda self: self._pool[1])
+    k_scale = property(lambda self: self._pool[2])
+    v_scale = property(lambda self: self._pool[3])
 
     @classmethod
     def empty(cls, n_pages: int, page: int, kv_heads: int, dim: int, vdim: Optional[int] = None, *, dtype: torch.dtype = torch.bfloat16, store: str = "act",
@@ -190,18 +204,18 @@ class PagedCache:
         return cls(k, v, *scales, dtype=dtype)
 
     def bytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale) if t is not None)
+        return sum(t.numel() * t.element_size() for t in self._pool if t is not None)
 
-    # ------------------------------------------------------------------ calls
-    def _rows(self, x: torch.Tensor, heads: Optional[int], size: int, step: PagedStep, what: str) -> torch.Tensor:
+    # ------------------------------------------------------------------ calls (of every layer and step: some 5 us each beside the launches)
+    def _rows(self, x: torch.Tensor, heads: int, size: int, step: PagedStep, what: str) -> torch.Tensor:
         """x [rows, heads, size] as the kernels take it: entries of a head consecutive, rows on 16-byte borders (else a copy)."""
-        if x.dim() != 3 or x.shape[2] != size or (heads is not None and x.shape[1] != heads) or x.dtype != self.dtype or x.device != self.device:
-            raise ValueError(f"paged cache: {what} {tuple(x.shape)} {x.dtype} on {x.device}, [rows, {heads or 'heads'}, {size}] {self.dtype} on {self.device} is wanted")
-        if x.shape[0] < step.rows:
-            raise ValueError(f"paged cache: {what} has {x.shape[0]} rows, the step {step.rows}")
-        per = 4 if self.dtype == torch.float32 else 8
+        shape = x.shape
+        if len(shape) != 3 or shape[2] != size or (heads and shape[1] != heads) or x.dtype is not self.dtype or x.device != self.device:
+            raise ValueError(f"paged cache: {what} {tuple(shape)} {x.dtype} on {x.device}, [rows, {heads or 'heads'}, {size}] {self.dtype} on {self.device} is wanted")
+        if shape[0] < step.rows:
+            raise ValueError(f"paged cache: {what} has {shape[0]} rows, the step {step.rows}")
         s0, s1, s2 = x.stride()
-        if s2 != 1 or s0 % per or s1 % per or x.data_ptr() % 16:
+        if s2 != 1 or s0 % self._per or s1 % self._per or x.data_ptr() % 16:
             x = x.contiguous()
             if x.data_ptr() % 16:
                 x = x.clone()
@@ -210,31 +224,31 @@ class PagedCache:
     def _call(self, name: str, step: PagedStep, *args) -> None:
         if step.device != self.device:
             raise ValueError(f"paged cache: a step on {step.device} for a pool on {self.device}")
+        if self._at is None:
+            raise RuntimeError(f"pool on {self.device}: the sequence kernels run on CUDA only (no CPU fallback)")
+        function = getattr(S.lib(), name)
         if torch._C._cuda_getDevice() == self.device.index:
-            S.check(getattr(S.lib(), name)(*args, S.stream_ptr()), name)
+            rc = function(*args, S.stream_ptr())
         else:
             with torch.cuda.device(self.device):
-                S.check(getattr(S.lib(), name)(*args, S.stream_ptr()), name)
-
-    def _pool(self) -> tuple:
-        return S.ptr(self.k), S.ptr(self.v), S.ptr(self.k_scale), S.ptr(self.v_scale)
-
-    def _step(self, step: PagedStep) -> tuple:
-        return S.ptr(step.starts), S.ptr(step.lengths), S.ptr(step.table), step.table.stride(0), step.table.shape[1]
+                rc = function(*args, S.stream_ptr())
+        if rc:
+            S.check(rc, name)
 
     def write(self, k: torch.Tensor, v: torch.Tensor, step: PagedStep) -> None:
         """The step's keys [rows, kv_heads, dim] and values [rows, kv_heads, vdim] into the pool.  Rows behind the step's last sequence are not looked at.
         Two rows of one step must not have the same place (a page in two sequences' tables, both writing there)."""
         k, v = self._rows(k, self.kv_heads, self.dim, step, "keys"), self._rows(v, self.kv_heads, self.vdim, step, "values")
-        self._call("b2l_seq_paged_write", step, S.ptr(k), k.stride(0), k.stride(1), S.ptr(v), v.stride(0), v.stride(1), *self._pool(), *self._step(step),
-                   min(k.shape[0], v.shape[0]), step.seqs, self.n_pages, self.page, self.kv_heads, self.dim, self.vdim, *self._codes)
+        k0, k1, _ = k.stride()
+        v0, v1, _ = v.stride()
+        self._call("b2l_seq_paged_write", step, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, *(self._at or ()), *(step._at or ()), min(k.shape[0], v.shape[0]), step.seqs, *self._sizes)
 
     def read(self, step: PagedStep) -> Tuple[torch.Tensor, torch.Tensor]:
         """The rows that `write` with this step puts into the pool, as they lie there: keys [rows, kv_heads, dim] and values in the activation type."""
-        k = torch.empty((step.rows, self.kv_heads, self.dim), dtype=self.dtype, device=self.device)
-        v = torch.empty((step.rows, self.kv_heads, self.vdim), dtype=self.dtype, device=self.device)
-        self._call("b2l_seq_paged_read", step, S.ptr(k), k.stride(0), k.stride(1), S.ptr(v), v.stride(0), v.stride(1), *self._pool(), *self._step(step), step.rows, step.seqs,
-                   self.n_pages, self.page, self.kv_heads, self.dim, self.vdim, *self._codes)
+        G, K, V = self.kv_heads, self.dim, self.vdim
+        k = torch.empty((step.rows, G, K), dtype=self.dtype, device=self.device)
+        v = torch.empty((step.rows, G, V), dtype=self.dtype, device=self.device)
+        self._call("b2l_seq_paged_read", step, k.data_ptr(), G * K, K, v.data_ptr(), G * V, V, *(self._at or ()), *(step._at or ()), step.rows, step.seqs, *self._sizes)
         return k, v
 
     def attend(self, q: torch.Tensor, step: PagedStep, *, scale: Optional[float] = None, window: int = 0, first: int = 0,
@@ -246,24 +260,30 @@ class PagedCache:
         q [rows, heads, dim] with heads a multiple of kv_heads (head h reads key/value head h // (heads / kv_heads)), p the position of row r; scale
         dim^-1/2 unless given.  Returns [rows, heads, vdim] (`out`, contiguous, where given); rows behind the step's last sequence are zeros, or as they were
         in `out`."""
-        q = self._rows(q, None, self.dim, step, "queries")
-        rows, heads = q.shape[0], q.shape[1]
+        q = self._rows(q, 0, self.dim, step, "queries")
+        rows, heads, _ = q.shape
+        plan = step._plans.get((rows, heads, scale, window, first, self._sizes))
+        if plan is None:
+            plan = self._plan(rows, heads, scale, window, first, step)
+        floats, sizes = plan
+        if out is None:
+            out = (q.new_empty if rows == step.rows else q.new_zeros)((rows, heads, self.vdim))
+        elif out.shape != (rows, heads, self.vdim) or out.dtype != self.dtype or out.device != self.device or not out.is_contiguous() or out.data_ptr() % 16:
+            raise ValueError(f"paged cache: out must be {(rows, heads, self.vdim)} {self.dtype} on {self.device}, contiguous and 16-byte aligned")
+        work = step._tensors[1].new_empty((floats,)) if floats else None          # four bytes an entry
+        s0, s1, _ = q.stride()
+        self._call("b2l_seq_paged_attention", step, q.data_ptr(), s0, s1, *(self._at or ()), *(step._at or ()), out.data_ptr(), work.data_ptr() if floats else None, floats, *sizes)
+        return out
+
+    def _plan(self, rows: int, heads: int, scale: Optional[float], window: int, first: int, step: PagedStep) -> tuple:
+        """(floats of work space, arguments that are the same in every layer of the step); kept with the step."""
         if heads < 1 or heads % self.kv_heads:
             raise ValueError(f"paged cache: {heads} query heads over {self.kv_heads} key/value heads")
         if window < 0 or first < 0:
             raise ValueError("paged cache: a negative window or number of first tokens")
-        if out is None:
-            out = (torch.empty if rows == step.rows else torch.zeros)((rows, heads, self.vdim), dtype=self.dtype, device=self.device)
-        elif out.shape != (rows, heads, self.vdim) or out.dtype != self.dtype or out.device != self.device or not out.is_contiguous() or out.data_ptr() % 16:
-            raise ValueError(f"paged cache: out must be {(rows, heads, self.vdim)} {self.dtype} on {self.device}, contiguous and 16-byte aligned")
         sizes = (heads, self.kv_heads, self.dim, self.vdim, window, first)
-        hints = (step.max_new, step.min_new, step.max_length)
-        width = step.table.shape[1]
-        key = (rows, width, self.page, *sizes, *hints, *self._codes)
-        floats = step._work.get(key)
-        if floats is None:
-            floats = step._work[key] = S.lib().b2l_seq_paged_attention_work(rows, step.seqs, width, self.page, *sizes, *hints, *self._codes)
-        work = torch.empty((floats,), dtype=torch.float32, device=self.device) if floats else None
-        self._call("b2l_seq_paged_attention", step, S.ptr(q), q.stride(0), q.stride(1), *self._pool(), *self._step(step), S.ptr(out), S.ptr(work), floats, rows, step.seqs,
-                   self.n_pages, self.page, *sizes, float(self.dim ** -0.5 if scale is None else scale), *hints, *self._codes)
-        return out
+        hints = (step.max_new, step.min_new, step.max_length) + self._codes
+        floats = S.lib().b2l_seq_paged_attention_work(rows, step.seqs, step.table.shape[1], self.page, *sizes, *hints)
+        plan = (floats, (rows, step.seqs, self.n_pages, self.page) + sizes + (float(self.dim ** -0.5 if scale is None else scale),) + hints)
+        step._plans[(rows, heads, scale, window, first, self._sizes)] = plan
+        return plan
