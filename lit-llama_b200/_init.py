@@ -22,12 +22,12 @@ from .malulorn import Malulorn, MalulornConfig
 from .state import SequenceStatePool, StateSpec
 from .paged import PagedCache, PagedStep, PagePool
 from .engine import Engine
-from .registry import load_model, register
+from .registry import PagedLLaMAModel, load_model, register
 
 __all__ = [
     "LLaMA", "LLaMAConfig", "Block", "CausalSelfAttention", "MLP", "RMSNorm", "build_rope_cache", "apply_rope",
     "ColBlockQuantizedLinear", "Linear8bitLt", "find_multiple", "llama_model_lookup", "generate", "sample_probs", "sample_token", "patch_reference", "TPLLaMA", "shard_state_dict",
     "Lugovik", "LugovikConfig", "Zenasun", "ZenasunConfig", "Zuvevik", "ZuvevikConfig", "Rinirax", "RiniraxConfig", "Lukupel", "LukupelConfig",
     "Malulorn", "MalulornConfig",
-    "SequenceStatePool", "StateSpec", "PagedCache", "PagedStep", "PagePool", "Engine", "load_model", "register",
+    "SequenceStatePool", "StateSpec", "PagedCache", "PagedStep", "PagePool", "PagedLLaMAModel", "Engine", "load_model", "register",
 ]

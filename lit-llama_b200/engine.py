@@ -2,7 +2,8 @@
 
 A model plugs in through three members: `state_specs()` (what a sequence carries between steps), `vocab`, and
 `forward_portion(tokens, ctx, want)` (run the next tokens of one sequence from the state earlier steps left,
-return f32 logits at the wanted places).  The engine owns the `SequenceStatePool`, maps request ids to slots,
+return f32 logits at the wanted places); one that books memory of its own for a slot (pages of a cache) is told by
+`release_slot(slot)` when its request is gone.  The engine owns the `SequenceStatePool`, maps request ids to slots,
 and offers two ways in:
 
   * `step(entries, end)`: the caller decides which tokens each request gets in this step (a replayed trace,
@@ -50,7 +51,7 @@ class Engine:
     def __init__(self, model, *, n_slots: int = 4, max_tokens: int = 0, prefill_chunk: int = 512, device: Optional[torch.device] = None) -> None:
         self.model = model
         self.device = torch.device(device) if device is not None else model.device
-        self.pool = SequenceStatePool(model.state_specs(), n_slots, self.device, max_tokens=max_tokens)
+        self.pool = SequenceStatePool(model.state_specs(), n_slots, self.device, max_tokens=max_tokens, on_release=getattr(model, "release_slot", None))
         self.prefill_chunk = int(prefill_chunk)
         self.waiting: deque = deque()
         self.live: "OrderedDict[Hashable, Request]" = OrderedDict()

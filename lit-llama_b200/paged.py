@@ -182,6 +182,7 @@ class PagedCache:
         self.device = k.device
         self._codes = (STORES[self.store], S.act_code(self.dtype))
         self._sizes = (self.n_pages, self.page, self.kv_heads, self.dim, self.vdim) + self._codes
+        self._like = torch.empty(0, dtype=self.dtype, device=k.device)
         self._per = 4 if self.dtype == torch.float32 else 8                 # entries in 16 bytes
         self._at = tuple(S.ptr(t) for t in (k, v, k_scale, v_scale)) if k.is_cuda else None
 
@@ -246,8 +247,7 @@ class PagedCache:
     def read(self, step: PagedStep) -> Tuple[torch.Tensor, torch.Tensor]:
         """The rows that `write` with this step puts into the pool, as they lie there: keys [rows, kv_heads, dim] and values in the activation type."""
         G, K, V = self.kv_heads, self.dim, self.vdim
-        k = torch.empty((step.rows, G, K), dtype=self.dtype, device=self.device)
-        v = torch.empty((step.rows, G, V), dtype=self.dtype, device=self.device)
+        k, v = self._like.new_empty((step.rows, G, K)), self._like.new_empty((step.rows, G, V))
         self._call("b2l_seq_paged_read", step, k.data_ptr(), G * K, K, v.data_ptr(), G * V, V, *(self._at or ()), *(step._at or ()), step.rows, step.seqs, *self._sizes)
         return k, v
 

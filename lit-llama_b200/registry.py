@@ -65,7 +65,8 @@ def _load_malulorn(model_dir: str, dtype: torch.dtype, device: torch.device, max
 
 @register("LLaMA")
 def _load_llama(model_dir: str, dtype: torch.dtype, device: torch.device, max_positions: int, config: dict):
-    """config.json: {"architecture": "LLaMA", "name": "7B" | sizes..., "quantize": null | "gptq.int4" | ..., "checkpoint": file}."""
+    """config.json: {"architecture": "LLaMA", "name": "7B" | sizes..., "quantize": null | "gptq.int4" | ..., "checkpoint": file,
+    "kv_cache": {"pages", "page", "store", "window", "first"}}: with "kv_cache" the arguments of `PagedLLaMAModel`, without it `LLaMASequenceModel`."""
     from .model import LLaMA, LLaMAConfig
     from .utils import EmptyInitOnDevice, lazy_load
 
@@ -77,6 +78,8 @@ def _load_llama(model_dir: str, dtype: torch.dtype, device: torch.device, max_po
         model = LLaMA(cfg)
     with lazy_load(os.path.join(model_dir, config.get("checkpoint", "lit-llama.pth"))) as sd:
         model.load_state_dict(sd)
+    if "kv_cache" in config:
+        return PagedLLaMAModel(model.eval(), max_positions=max_positions, **config["kv_cache"])
     return LLaMASequenceModel(model.eval(), max_positions or cfg.block_size)
 
 
@@ -104,6 +107,75 @@ class LLaMASequenceModel:
         input_pos = torch.arange(pos0, pos0 + T, device=tokens.device)
         logits = self.model(tokens.view(1, -1).to(torch.int64), self.max_seq_length, input_pos)[0]
         return (logits if want is None else logits.index_select(0, want.to(torch.int64))).float()
+
+
+class PagedLLaMAModel:
+    """The package's LLaMA behind the Engine's model interface with its keys and values in pages (paged.py), in bf16, e4m3 or int8: as many sequences at a
+    time as there are slots, each with the pages that its length needs.  A model of MHA layers: every head has keys and values of its own.
+
+    `pages` of `page` tokens are shared by the sequences (as many again for every layer); a portion that finds none left raises PoolFull.  With `window` a
+    token sees the last `window` positions and the first `first` ones, and a sequence keeps no pages for the others, so it may grow without end; else
+    it may have `max_positions` (default: the model's block size)."""
+    graph_safe = False     # pages are booked on the host
+
+    def __init__(self, model, *, pages: int, page: int = 64, store: str = "act", window: int = 0, first: int = 0, max_positions: int = 0) -> None:
+        from .paged import PagedCache, PagePool
+
+        cfg = model.config
+        self.model, self.vocab, self.dtype = model, cfg.padded_vocab_size, torch.bfloat16
+        self.device = next(model.parameters()).device
+        self.heads, self.size = cfg.n_head, cfg.n_embd // cfg.n_head
+        self.window, self.first = int(window), int(first)
+        self.max_positions = int(max_positions) or (0 if window else cfg.block_size)
+        self.pages = PagePool(pages, page, self.device, window=self.window, first=self.first)
+        self.caches = [PagedCache.empty(pages, page, self.heads, self.size, dtype=self.dtype, store=store, device=self.device) for _ in range(cfg.n_layer)]
+        self.freq = (1.0 / 10000 ** (torch.arange(0, self.size, 2, dtype=torch.float32) / self.size)).to(self.device)
+
+    def state_specs(self):
+        return {}
+
+    def release_slot(self, slot: int) -> None:
+        """The engine's slot is free: so are its sequence's pages."""
+        if self.pages.has(slot):
+            self.pages.release(slot)
+
+    def _rotated(self, x: torch.Tensor, ctx) -> torch.Tensor:
+        """Every head of x [T, heads * size] (rows of a wider product) turned by position, pairs of neighbouring entries (lit_llama/model.py:306-323)."""
+        from . import _seqlib as S
+
+        T, n = x.shape
+        out = torch.empty((T, self.heads, self.size), dtype=x.dtype, device=x.device)
+        S.check(S.lib().b2l_seq_rope(S.ptr(x), x.stride(0), 0, S.ptr(self.freq), self.size, 1, 0, 1.0, 1.0, S.ptr(ctx.meta), S.ptr(out), n, 0, T, self.heads, self.size, self.size,
+                                     self.size, ctx.act, ctx.stream), "b2l_seq_rope")
+        return out
+
+    @torch.no_grad()
+    def forward_portion(self, tokens: torch.Tensor, ctx, want: Optional[torch.Tensor] = None) -> torch.Tensor:
+        from . import _lib as L
+        from .model import _add
+
+        slot, pos0 = (ctx.slot_hint, ctx.pos_hint) if ctx.slot_hint is not None else ctx.meta.tolist()
+        if pos0 == 0:
+            self.release_slot(slot)
+        elif not self.pages.has(slot) or self.pages.position(slot) != pos0:
+            raise RuntimeError(f"paged LLaMA: slot {slot} is not at position {pos0}")
+        T, C = tokens.numel(), self.heads * self.size
+        step = self.pages.step([(slot, T)])
+        tokens = tokens.to(torch.int64).contiguous()
+        wte = self.model.transformer.wte.weight
+        x = torch.empty((1, T, C), dtype=self.dtype, device=self.device)
+        L.check(L.lib().b2l_embedding(tokens.data_ptr(), 1, wte.data_ptr(), x.data_ptr(), T, C, wte.shape[0], L.stream_ptr()), "b2l_embedding")
+        for block, cache in zip(self.model.transformer.h, self.caches):
+            qkv = block.attn.c_attn(block.rms_1(x))[0]
+            cache.write(self._rotated(qkv[:, C:2 * C], ctx), qkv[:, 2 * C:].unflatten(1, (self.heads, self.size)), step)
+            att = cache.attend(self._rotated(qkv[:, :C], ctx), step, window=self.window, first=self.first)
+            x = _add(x, block.attn.c_proj(att.view(1, T, C)))
+            x = _add(x, block.mlp(block.rms_2(x)))
+        if want is not None:
+            x = x.index_select(1, want.to(torch.int64))
+        if x.shape[1] == 0:
+            return torch.empty((0, self.vocab), dtype=torch.float32, device=self.device)
+        return self.model.lm_head(self.model.transformer.ln_f(x))[0].float()
 
 
 def read_config(model_dir: str) -> dict:

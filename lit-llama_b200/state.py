@@ -8,7 +8,7 @@ sequence.  Kernels address a slot through the device int32 pair {slot, position}
 replays for any slot."""
 import ctypes as C
 from dataclasses import dataclass
-from typing import Dict, Hashable, List, Tuple
+from typing import Callable, Dict, Hashable, List, Optional, Tuple
 
 import torch
 
@@ -27,7 +27,8 @@ class PoolFull(RuntimeError):
 
 
 class SequenceStatePool:
-    def __init__(self, specs: Dict[str, StateSpec], n_slots: int, device: torch.device, max_tokens: int = 0) -> None:
+    def __init__(self, specs: Dict[str, StateSpec], n_slots: int, device: torch.device, max_tokens: int = 0,
+                 on_release: Optional[Callable[[int], None]] = None) -> None:
         if n_slots < 1:
             raise ValueError("n_slots must be at least 1")
         self.specs = dict(specs)
@@ -42,6 +43,7 @@ class SequenceStatePool:
         self.acquired = 0                            # lifetime counters (tests and diagnostics)
         self.reused = 0
         self._used_before = set()
+        self.on_release = on_release                 # told of every slot that becomes free
 
     # ------------------------------------------------------------------ slots
     def has(self, request_id: Hashable) -> bool:
@@ -82,6 +84,8 @@ class SequenceStatePool:
         slot = self._slot_of.pop(request_id)
         del self._pos[slot]
         self._free.append(slot)
+        if self.on_release is not None:
+            self.on_release(slot)
 
     def slot(self, request_id: Hashable) -> int:
         return self._slot_of[request_id]
