@@ -609,17 +609,18 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
 
 // ------------------------------------------------------------------------------------------------ joining parts
 // `per` warps (a power of two) have a row and head, each every per-th part; rows of sequences whose parts were not split are in place already.  Parts are
-// read once, and the loads of a warp's parts do not wait for one another.  `short_only`: only the few-row kernel's sequences have parts, and a unit is one of
-// the 16 packed rows of each of them and a key/value head.
+// read once, and the loads of a warp's parts do not wait for one another.  The first `short_units` units are the 16 packed rows of each of the few-row kernel's
+// sequences and a key/value head where both kernels run, the others the rows and heads from the first on.
 constexpr int MERGE_WARPS = 8;
-__global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const __grid_constant__ Attn a, int per, int short_only) {
+__global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const __grid_constant__ Attn a, int per, int short_units) {
   __shared__ float4 sx[MERGE_WARPS][64];
   __shared__ float2 sml[MERGE_WARPS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, G = a.heads / a.kv_heads;
   const int here = MERGE_WARPS / per, sub = warp / here, own = warp % here;      // part of the unit's warps, unit of the block
-  const long long unit = (long long)blockIdx.x * here + own;
+  long long unit = (long long)blockIdx.x * here + own;
+  const bool is_short = unit < short_units;
   int row, head, b = -1, start = 0, n = 0, length = 0;
-  if (short_only) {
+  if (is_short) {
     const int r = (int)(unit % 16), h = (int)(unit / 16 % a.kv_heads), at = (int)(unit / 16 / a.kv_heads);
     if (at < a.s.seqs) {
       sequence(a.s, at, start, n, length);
@@ -628,6 +629,7 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const __g
     row = start + r / G;
     head = h * G + r % G;
   } else {
+    unit -= short_units;
     row = (int)min(unit / a.heads, (long long)a.s.rows);
     head = (int)(unit % a.heads);
     if (row < a.s.rows) b = sequence_of(a.s, row, lane);
@@ -636,7 +638,7 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const __g
   const int h = head / G;
   const bool few = (long long)n * G <= a.few_max;
   const Parts& p = few ? a.few : a.many;
-  const bool on = b >= 0 && p.splits > 1;
+  bool on = b >= 0 && p.splits > 1 && (!a.compact || few == is_short);
   const long long at = few && a.compact ? (long long)(b * a.kv_heads + h) * 16 + (row - start) * G + head % G : (long long)row * a.heads + head;
   float M = -INFINITY, L = 0.f;
   float4 x[2] = {};
@@ -650,6 +652,10 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const __g
 #pragma unroll
       for (int c = 0; c < 2; ++c) z[c] = 4 * (lane + 32 * c) < a.V ? y[32 * c] : make_float4(0.f, 0.f, 0.f, 0.f);
       if (ml.x == -INFINITY && ml.y == 0.f) continue;        // saw nothing
+      if (ml.x == INFINITY && ml.y == 0.f) {                 // was not shared: its result is in place
+        on = false;
+        break;
+      }
       const float now = fmaxf(M, ml.x), f = M == now ? 1.f : exp2_f(M - now), w = ml.x == now ? 1.f : exp2_f(ml.x - now);
       M = now;
       L = L * f + w * ml.y;
@@ -698,8 +704,8 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const __g
 // ------------------------------------------------------------------------------------------------ host
 struct Plan {
   bool few, many;
-  int few_max, few_rows, few_tiles, many_tiles, few_splits, many_splits, compact;
-  long long few_count, many_count, floats;
+  int few_max, few_rows, few_tiles, many_tiles, many_whole, part_rows, few_splits, many_splits, compact;
+  long long many_ctas, few_count, many_count, floats;
 };
 constexpr long long MOST_WORK = 1ll << 27;                   // floats of partial results
 
@@ -734,17 +740,25 @@ static Plan plan_of(int rows, int seqs, int width, int page, int heads, int kv_h
     p.few_splits = (int)std::max<long long>(1, std::min({want, keys / (room ? 128 : 512), 128ll, MOST_WORK / (p.few_count * (V + 2) + 1)}));
   }
   if (p.many) {
-    // One CTA on an SM at a time, 2.3 us for 128 keys: as many parts as make the rounds shortest, where the last one is seldom full.  A part's results are
-    // written and read at some 4 TB/s, and joining them costs a launch.
-    const double ctas = (double)kv_heads * std::max<long long>(1, (packed + 255) / 256), tiles = (keys + 127) / 128, results = 8.0 * p.many_count * V / 4e6;      // us
+    // One CTA on an SM at a time, some 1.8 us (8-bit: 2.8) for 128 keys of 128 + 128 entries and 15 beside.  Row tiles that fill rounds of all SMs run whole; the
+    // rest in as many parts as make what is left shortest, a launch of 8 us and 4 TB/s for the parts' results included: 256 tokens over 16384 of 32 / 8 heads,
+    // 32 row tiles, take 234 us whole, 131 in 2 parts, 80 in 4 and 120 in 5, a second round
+    const long long rest = (packed + 255) / 256 + (min_new == max_new && seqs == 1 ? 0 : seqs / 2);
+    const long long items = (long long)kv_heads * std::max<long long>(1, std::min<long long>(rest, p.many_tiles)), whole = items / sms * sms, left = items - whole;
+    const double tiles = (keys + 127) / 128, tile = (store == ACT ? 1.8 : 2.8) * (K + V) / 256;
     double least = 0;
-    for (int s = 1; s <= 16 && s <= tiles && (s == 1 || (long long)s * p.many_count * (V + 2) <= MOST_WORK); ++s) {
-      const double us = std::ceil(ctas * s / sms) * std::ceil(tiles / s) * 2.3 + std::ceil(ctas * s / sms) * 6 + (s > 1 ? 4 + s * results : 0);
+    p.many_splits = 1;
+    for (int s = 1; left > 0 && s <= 16 && s <= tiles && (s == 1 || (long long)s * p.many_count * (V + 2) <= MOST_WORK); ++s) {
+      const double us = std::ceil((double)left * s / sms) * (std::ceil(tiles / s) * tile + 15) + (s > 1 ? 8 + s * left * 256.0 * V * 4 / 4e6 : 0);
       if (s == 1 || us < 0.95 * least) {
         least = us;
         p.many_splits = s;
       }
     }
+    p.many_whole = (int)std::min<long long>(p.many_splits > 1 ? whole : 0, INT32_MAX);
+    p.many_ctas = p.many_whole + std::max<long long>(0, (long long)p.many_tiles * kv_heads - p.many_whole) * p.many_splits;
+    // the rows that may have parts: the last row tiles to be begun are the first ones, and between them lie short sequences
+    p.part_rows = p.many_splits == 1 ? 0 : (int)std::min<long long>(rows, whole == 0 ? rows : ((long long)p.many_tiles - whole / kv_heads + 1) * (256 / std::min(G, 256) + 1) + 16ll * seqs);
   }
   auto floats = [&](int splits, long long count) { return splits > 1 ? (2 * splits * count + 3) / 4 * 4 + splits * count * V : 0; };
   p.floats = (p.few ? floats(p.few_splits, p.few_count) : 0) + (p.many ? floats(p.many_splits, p.many_count) : 0);
@@ -838,15 +852,18 @@ extern "C" int b2l_seq_paged_attention(const void* q, long long ldq, long long h
 #undef GO
     if (rc) return rc;
   }
-  if (p.many)
-    if (int rc = many_launch(a, p.many_tiles, st)) return rc;
+  if (p.many) {
+    B2L_CHECK_SUPPORTED(p.many_ctas < (1ll << 31), "%s: sizes beyond the grid's", who);
+    a.many_whole = p.many_whole;
+    if (int rc = many_launch(a, (int)p.many_ctas, st)) return rc;
+  }
   if (a.few.splits > 1 || a.many.splits > 1) {
     const int most = std::max(a.few.splits, a.many.splits), per = most >= 32 ? 8 : most >= 16 ? 4 : most >= 8 ? 2 : 1, here = MERGE_WARPS / per;
-    const bool short_only = p.compact && a.many.splits == 1;
-    const long long units = short_only ? 16ll * kv_heads * seqs : (long long)rows * heads;
+    const long long short_units = p.compact && a.few.splits > 1 ? 16ll * kv_heads * seqs : 0, at_rows = p.compact || a.few.splits == 1 ? p.part_rows : rows;
+    const long long units = short_units + at_rows * heads;
     B2L_CHECK_SUPPORTED(units < (1ll << 31), "%s: sizes beyond the grid's", who);
     LaunchCfg launch(dim3((unsigned)((units + here - 1) / here)), dim3(32 * MERGE_WARPS), 0, st, true);
-    B2L_CUDA(cudaLaunchKernelEx(&launch.cfg, paged_merge_kernel, a, per, (int)short_only));
+    B2L_CUDA(cudaLaunchKernelEx(&launch.cfg, paged_merge_kernel, a, per, (int)short_units));
     B2L_LAUNCH_CHECK("paged_merge_kernel");
   }
   return 0;

@@ -69,6 +69,7 @@ struct Attn {
   int heads, kv_heads, K, V, window, first, few_max;        // few_max: sequences of at most so many packed rows are the few-row kernel's
   float scale_log2;
   int f32, store_kind, compact;
+  int many_whole;                                            // row tiles and heads, in the order they are begun, that are not shared among CTAs
   Parts few, many;                                           // compact in `few` where both kernels run: 16 packed rows per sequence and key/value head
 
   __device__ __forceinline__ bool sees(int pos, int j) const { return j <= pos && (window == 0 || j > pos - window || j < first); }
@@ -105,6 +106,18 @@ struct Attn {
       base += __shfl_sync(0xffffffffu, upto, 31);
     }
     return false;
+  }
+  // The same counted from the last one
+  __device__ __forceinline__ bool place_back(int slot, int R, int above, int most, int lane, Place& pl) const {
+    const int G = heads / kv_heads;
+    int total = 0;
+    for (int b0 = 0; b0 < s.seqs; b0 += 32) {
+      int start, n = 0, length;
+      if (b0 + lane < s.seqs) sequence(s, b0 + lane, start, n, length);
+      const long long packed = (long long)n * G;
+      total += __reduce_add_sync(0xffffffffu, packed > above && packed <= most ? (int)((packed + R - 1) / R) : 0);
+    }
+    return slot < total && place(total - 1 - slot, R, above, most, 0, lane, pl);
   }
   __device__ __forceinline__ Keys keys(const Place& pl, int R) const {
     const int G = heads / kv_heads, last = min(pl.first + R, pl.n * G) - 1;
@@ -183,7 +196,7 @@ __device__ __forceinline__ bool finite4(const float (&x)[4], float inv) {
 
 // the tensor-core kernel of longer chunks (seq_paged_tc.cu): heads that it takes, and its launch
 bool many_takes(int K, int V, int store);
-int many_launch(const Attn& a, int tiles, cudaStream_t stream);
+int many_launch(const Attn& a, int ctas, cudaStream_t stream);
 
 }  // namespace paged
 }  // namespace b2l

@@ -177,12 +177,15 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
   Control& ct = *reinterpret_cast<Control*>(smem);
   Info* infos = reinterpret_cast<Info*>(smem + CONTROL_BYTES);      // ACT: only `there`, at uint32_t steps
   uint32_t* there_of = reinterpret_cast<uint32_t*>(smem + CONTROL_BYTES);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.heads / a.kv_heads, h = blockIdx.y, split = blockIdx.z;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.heads / a.kv_heads;
+  // Later rows, which mostly have more keys, first; the first ones whole, what would be a last round that is not full in parts
+  const int over = (int)blockIdx.x - a.many_whole, splits = over < 0 ? 1 : a.many.splits, split = over < 0 ? 0 : over % splits;
+  const int item = over < 0 ? (int)blockIdx.x : a.many_whole + over / splits, h = item % a.kv_heads;
   Place pl;
-  if (!a.place(gridDim.x - 1 - blockIdx.x, ROWS, a.few_max, INT32_MAX, 0, lane, pl)) return;      // later rows, with more keys, first
+  if (!a.place_back(item / a.kv_heads, ROWS, a.few_max, INT32_MAX, lane, pl)) return;
   const int rows = min(ROWS, pl.n * G - pl.first), groups = rows > TILE ? 2 : 1;
   const Keys keys = a.keys(pl, ROWS);
-  const int all = keys.units(7), per = (all + a.many.splits - 1) / a.many.splits;
+  const int all = keys.units(7), per = (all + splits - 1) / splits;
   const int t0 = min(split * per, all), n = min(t0 + per, all) - t0;
   const int ka = atoms_of(a.K, 2), va = atoms_of(a.V, 2);
   const uint32_t sq = smem_u32(smem) + CONTROL_BYTES + INFO_BYTES<STORE>, sk = sq + 2 * ka * TC_ATOM, sv = sk + k_stages * ka * TC_ATOM;
@@ -304,19 +307,19 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
         mbar_arrive(bar(ct.info_full[t % INFOS]));
         mbar_expect_tx(k_to, HALF ? KEYS * (a.K + 8) : ka * TC_ATOM);
       }
-      for (int i = 0; i < boxes; ++i) {
-        const int r = __shfl_sync(0xffffffffu, row, i);
-        if (lane == 0) {
-          if (HALF) {
-            const int at = r < gone ? r : 0;                 // of a page that is not there: any scales
-            tma_load_2d(raw_k + i * box * a.K, &map_k, 0, r, k_to);
-            bulk(smem_u32(codes.ks + i * box), a.ks + at, 4 * box, k_to);
-            bulk(smem_u32(codes.vs + i * box), a.vs + at, 4 * box, k_to);
-          } else {
-            for (int x = 0; x < ka; ++x) tma_load_2d(sk + (kst * ka + x) * TC_ATOM + i * box * 128, &map_k, 64 * x, r, k_to);
-          }
+      __syncwarp();                                          // the bytes are expected before they come
+      // a lane per box: one lane after the other took 100 ns for each, with pages of 16 tokens 3.1 us for a tile
+      const int b = lane & (boxes - 1), x = lane / boxes, r = __shfl_sync(0xffffffffu, row, b);      // 24 boxes at most
+      if (x < (HALF ? 3 : ka)) {
+        if (HALF) {
+          const int at = r < gone ? r : 0;                   // of a page that is not there: any scales
+          if (x == 0) tma_load_2d(raw_k + b * box * a.K, &map_k, 0, r, k_to);
+          else bulk(smem_u32((x == 1 ? codes.ks : codes.vs) + b * box), (x == 1 ? a.ks : a.vs) + at, 4 * box, k_to);
+        } else {
+          tma_load_2d(sk + (kst * ka + x) * TC_ATOM + b * box * 128, &map_k, 64 * x, r, k_to);
         }
       }
+      __syncwarp();
       if (HALF || ++kst == k_stages) { kst = 0; kph ^= 1u; }
       mbar_wait_warp(bar(HALF ? ct.rv_empty : ct.v_empty[vst]), vph, dead);
       if (dead) break;
@@ -325,14 +328,12 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
       const bool cut = !HALF && valid < KEYS;
       const uint32_t v_to = bar(HALF ? ct.rv_full : cut ? ct.tail : ct.v_full[vst]);
       if (lane == 0) mbar_expect_tx(v_to, HALF ? KEYS * a.V : va * TC_ATOM);
-      for (int i = 0; i < boxes; ++i) {
-        const int r = __shfl_sync(0xffffffffu, row, i);
-        if (lane == 0) {
-          if (HALF) tma_load_2d(raw_v + i * box * a.V, &map_v, 0, r, v_to);
-          else
-            for (int x = 0; x < va; ++x) tma_load_2d(sv + (vst * va + x) * TC_ATOM + i * box * 128, &map_v, 64 * x, r, v_to);
-        }
+      __syncwarp();
+      if (x < (HALF ? 1 : va)) {
+        if (HALF) tma_load_2d(raw_v + b * box * a.V, &map_v, 0, r, v_to);
+        else tma_load_2d(sv + (vst * va + x) * TC_ATOM + b * box * 128, &map_v, 64 * x, r, v_to);
       }
+      __syncwarp();
       if (cut) {
         mbar_wait_warp(v_to, tail_waits++ & 1u, dead);
         if (dead) break;
@@ -603,9 +604,9 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
       if (n > 0) mbar_wait_warp(bar(ct.o_done[g]), 0, dead);
       fence_after();
       if (dead || odd) l = NAN;
-      const float down = HALF && n > 0 ? 1.f / value_lift(ct.ref) : 1.f, inv = a.many.splits > 1 ? down : l == 0.f ? 0.f : down / l;
+      const float down = HALF && n > 0 ? 1.f / value_lift(ct.ref) : 1.f, inv = splits > 1 ? down : l == 0.f ? 0.f : down / l;
       bool fine = true;
-      const bool part = a.many.splits > 1;
+      const bool part = splits > 1;
       const int place = live ? row * a.heads + head : -1;    // of the row's outputs
       const long long to = ((long long)split * a.many.count + (long long)row * a.heads + head);
       // Outputs through the warp's rows of the queries (every score of this row tile is done), 128 bytes of each row at a time; then eight lanes along a row (a
@@ -652,8 +653,8 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
         }
         __syncwarp();
       }
-      if (live && a.many.splits > 1) *reinterpret_cast<float2*>(a.many.ml + 2 * to) = make_float2(m, l);
-      if (a.many.splits == 1) {
+      if (live && a.many.splits > 1) *reinterpret_cast<float2*>(a.many.ml + 2 * to) = part ? make_float2(m, l) : make_float2(INFINITY, 0.f);      // (whole: nothing to join)
+      if (!part) {
         __syncwarp();
         for (uint32_t left = __ballot_sync(0xffffffffu, live && !(fine && fabsf(l) < INFINITY)); left; left &= left - 1) {
           const int i = __ffs(left) - 1;
@@ -690,7 +691,7 @@ static int map_rows(CUtensorMap* m, const void* base, long long rows, int cols, 
   return 0;
 }
 
-template <int STORE> static int go(const Attn& a, int tiles, cudaStream_t stream) {
+template <int STORE> static int go(const Attn& a, int ctas, cudaStream_t stream) {
   const Layout l = layout<STORE>(a.K, a.V);
   CUtensorMap mk, mv;
   const long long rows = ((long long)a.s.pages * a.kv_heads) << a.s.shift;
@@ -704,12 +705,12 @@ template <int STORE> static int go(const Attn& a, int tiles, cudaStream_t stream
   }
   static DynSmemCache cache;
   if (int rc = ensure_dyn_smem(paged_many_kernel<STORE>, l.smem, cache)) return rc;
-  paged_many_kernel<STORE><<<dim3((unsigned)tiles, (unsigned)a.kv_heads, (unsigned)a.many.splits), STORE == ACT ? 384 : 512, l.smem, stream>>>(a, mk, mv, l.ks, l.vs);
+  paged_many_kernel<STORE><<<(unsigned)ctas, STORE == ACT ? 384 : 512, l.smem, stream>>>(a, mk, mv, l.ks, l.vs);
   B2L_LAUNCH_CHECK("paged_many_kernel");
   return 0;
 }
-int many_launch(const Attn& a, int tiles, cudaStream_t stream) {
-  return a.store_kind == ACT ? go<ACT>(a, tiles, stream) : a.store_kind == E4M3 ? go<E4M3>(a, tiles, stream) : go<INT8>(a, tiles, stream);
+int many_launch(const Attn& a, int ctas, cudaStream_t stream) {
+  return a.store_kind == ACT ? go<ACT>(a, ctas, stream) : a.store_kind == E4M3 ? go<E4M3>(a, ctas, stream) : go<INT8>(a, ctas, stream);
 }
 
 }  // namespace paged
