@@ -197,6 +197,7 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
   // zeros
   const int beyond = (a.s.pages * a.kv_heads) << a.s.shift;
   const bool wide = NK == 2 && a.s.shift >= 5;               // a unit is in one page: one copy
+  const int copies = ka + va;                                // of a page: up to 16, and 8-bit 4
   int row_of = beyond;
   uint32_t gone = 0;                                         // 16-key parts of the ring's stages whose page is not there
   int next = 0;                                              // unit that is loaded next
@@ -211,24 +212,21 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
     ++next;
     gone = (gone & ~(3u << 2 * fill)) | ((r0 == beyond ? 1u : 0u) | (r1 == beyond ? 2u : 0u)) << 2 * fill;
     if (r0 != beyond || r1 != beyond) {
-      if (lane == 0) {
-        const uint32_t dst = ring + fill * unit_bytes, bar = bar0 + 8 * fill, sc = sc0 + 256 * fill;
-        tc::mbar_expect_tx(bar, unit_bytes + (HALF ? 256 : 0));
-        const int from = wide ? r0 & ~31 : r0;               // (a unit's second half may lie behind the last key: its page is not looked for)
-        for (int x = 0; x < ka; ++x) tc::tma_load_2d(dst + x * NK * ATOM, &maps.k, x * (128 / ES), from, bar);
-        for (int x = 0; x < va; ++x) tc::tma_load_2d(dst + (ka + x) * NK * ATOM, &maps.v, x * (128 / ES), from, bar);
-        if (NK == 2 && !wide) {
-          for (int x = 0; x < ka; ++x) tc::tma_load_2d(dst + x * NK * ATOM + ATOM, &maps.k, x * (128 / ES), r1, bar);
-          for (int x = 0; x < va; ++x) tc::tma_load_2d(dst + (ka + x) * NK * ATOM + ATOM, &maps.v, x * (128 / ES), r1, bar);
-        }
-        if (HALF) {                                          // of a page that is not there: any scales
-          const int s1 = wide ? from + 16 : r1 == beyond ? 0 : r1, z = wide ? from : r0 == beyond ? 0 : r0;
-          bulk64(sc, a.ks + z, bar);
-          bulk64(sc + 64, a.ks + s1, bar);
-          bulk64(sc + 128, a.vs + z, bar);
-          bulk64(sc + 192, a.vs + s1, bar);
-        }
+      const uint32_t dst = ring + fill * unit_bytes, bar = bar0 + 8 * fill;
+      if (lane == 0) tc::mbar_expect_tx(bar, unit_bytes + (HALF ? 256 : 0));
+      __syncwarp();                                          // the bytes are expected before they come
+      // a lane per copy: one lane after the other took some 100 ns for each
+      const int half = lane >= copies ? 1 : 0, x = lane - half * copies;
+      const int from = wide ? r0 & ~31 : half ? r1 : r0;     // (a unit's second half may lie behind the last key: its page is not looked for)
+      if (lane < (NK == 2 && !wide ? 2 : 1) * copies) {
+        if (x < ka) tc::tma_load_2d(dst + x * NK * ATOM + half * ATOM, &maps.k, x * (128 / ES), from, bar);
+        else tc::tma_load_2d(dst + x * NK * ATOM + half * ATOM, &maps.v, (x - ka) * (128 / ES), from, bar);
       }
+      if (HALF && lane >= 28) {                              // the scales; of a page that is not there any
+        const int second = lane & 1, at = wide ? from + 16 * second : second ? r1 : r0;
+        bulk64(sc0 + 256 * fill + 64 * (lane - 28), (lane & 2 ? a.vs : a.ks) + (at == beyond ? 0 : at), bar);
+      }
+      __syncwarp();
     }
     if (++fill == stages) fill = 0;
   };
