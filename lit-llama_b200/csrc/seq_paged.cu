@@ -14,8 +14,6 @@
 namespace b2l {
 namespace paged {
 
-constexpr int HEADS = 4;             // heads of a token that a warp takes: one look for its place, the loads of all in flight together
-
 struct Rows {
   Step s;
   const void *k_new, *v_new;         // or, for reading, where the rows go
@@ -25,19 +23,6 @@ struct Rows {
   int kv_heads, K, V;
 };
 
-__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = __uint_as_float(w[i] << 16);
-    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
-}
 __device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
   *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
   *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
@@ -110,20 +95,25 @@ template <int STORE> __device__ __forceinline__ uint2 codes8(float (&x)[8], floa
 }
 template <int STORE> __device__ __forceinline__ void values8(uint2 w, float s, float (&x)[8]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t u = i < 4 ? w.x : w.y;
+  for (int i = 0; i < 8; i += 4) {
+    const uint32_t u = i ? w.y : w.x;
     if (STORE == E4M3) {
-      if (i & 1) continue;
-      const float2 f = e4m3_pair(u >> 8 * (i & 2));
-      x[i] = f.x * s;
-      x[i + 1] = f.y * s;
-    } else {
-      x[i] = (float)(int8_t)(u >> 8 * (i & 3)) * s;
+      const float2 f = e4m3_pair(u), g = e4m3_pair(u >> 16);
+      x[i] = f.x; x[i + 1] = f.y; x[i + 2] = g.x; x[i + 3] = g.y;
+    } else {                                                 // 2^23 + 128 + code, less 2^23 + 128 (a conversion is a fourth as fast)
+      const uint32_t v = u ^ 0x80808080u;
+      x[i] = __uint_as_float(__byte_perm(v, 0x4b000000u, 0x7650)) - 8388736.f;
+      x[i + 1] = __uint_as_float(__byte_perm(v, 0x4b000000u, 0x7651)) - 8388736.f;
+      x[i + 2] = __uint_as_float(__byte_perm(v, 0x4b000000u, 0x7652)) - 8388736.f;
+      x[i + 3] = __uint_as_float(__byte_perm(v, 0x4b000000u, 0x7653)) - 8388736.f;
     }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[i + e] *= s;
   }
 }
 
-template <typename act_t, int STORE, int NI>      // NI: 128-entry parts of the longest row
+// NI: 128-entry parts of the longest row; HEADS: of a token that a warp takes: one look for its place, the loads of all in flight together
+template <typename act_t, int STORE, int NI, int HEADS>
 __global__ void __launch_bounds__(256) paged_write_kernel(const __grid_constant__ Rows a) {
   const int lane = threadIdx.x & 31, l = lane & 15;
   const bool value = lane >= 16;
@@ -178,7 +168,7 @@ __global__ void __launch_bounds__(256) paged_write_kernel(const __grid_constant_
   }
 }
 
-template <typename act_t, int STORE>
+template <typename act_t, int STORE, int NI, int HEADS>
 __global__ void __launch_bounds__(256) paged_read_kernel(const __grid_constant__ Rows a) {
   const int lane = threadIdx.x & 31, l = lane & 15;
   const bool value = lane >= 16;
@@ -191,36 +181,46 @@ __global__ void __launch_bounds__(256) paged_read_kernel(const __grid_constant__
   int start, n, length;
   sequence(a.s, b, start, n, length);
   const int p = length - n + row - start;
-  const int page = p >= 0 ? page_of(a.s, b, p) : -1, in_page = p & ((1 << a.s.shift) - 1);
+  const int page = p >= 0 ? page_of(a.s, b, p) : -1;
   const int D = value ? a.V : a.K;
-  act_t* dst = reinterpret_cast<act_t*>(const_cast<void*>(value ? a.v_new : a.k_new)) + row * (value ? a.ldv : a.ldk) + h0 * (value ? a.hsv : a.hsk);
-  float x[HEADS][2][8], s[HEADS];
-  uint2 w[HEADS][2];
+  const size_t at = (((size_t)max(page, 0) * a.kv_heads + h0) << a.s.shift) + (p & ((1 << a.s.shift) - 1)), to_next = (size_t)1 << a.s.shift;
+  const long long hs = value ? a.hsv : a.hsk;
+  act_t* dst = reinterpret_cast<act_t*>(const_cast<void*>(value ? a.v_new : a.k_new)) + row * (value ? a.ldv : a.ldk) + h0 * hs + 8 * l;
+  if (STORE == ACT) {
+    const act_t* src = reinterpret_cast<const act_t*>(value ? a.v : a.k) + at * D + 8 * l;
+    decltype(raw8(src)) raw[HEADS][NI];
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h)
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        if (page >= 0 && h0 + h < a.kv_heads && 8 * (l + 16 * i) < D) raw[h][i] = raw8(src + h * to_next * D + 128 * i);
+        else clear(raw[h][i]);
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h)
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        if (h0 + h < a.kv_heads && 8 * (l + 16 * i) < D) *reinterpret_cast<decltype(raw8(src))*>(dst + h * hs + 128 * i) = raw[h][i];
+    return;
+  }
+  const uint8_t* src = reinterpret_cast<const uint8_t*>(value ? a.v : a.k) + at * D + 8 * l;
+  const float* scale = (value ? a.vs : a.ks) + at;
+  uint2 w[HEADS][NI];
+  float s[HEADS];
 #pragma unroll
   for (int h = 0; h < HEADS; ++h) {
-    const size_t at = (((size_t)max(page, 0) * a.kv_heads + h0 + h) << a.s.shift) + in_page;
     const bool in = page >= 0 && h0 + h < a.kv_heads;
-    s[h] = STORE != ACT && in ? (value ? a.vs : a.ks)[at] : 0.f;
+    s[h] = in ? scale[h * to_next] : 0.f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int c = 8 * (l + 16 * i);
-      w[h][i] = make_uint2(0u, 0u);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[h][i][e] = 0.f;
-      if (in && c < D) {
-        if (STORE == ACT) load8(reinterpret_cast<const act_t*>(value ? a.v : a.k) + at * D + c, x[h][i]);
-        else w[h][i] = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(value ? a.v : a.k) + at * D + c);
-      }
-    }
+    for (int i = 0; i < NI; ++i) w[h][i] = in && 8 * (l + 16 * i) < D ? *reinterpret_cast<const uint2*>(src + h * to_next * D + 128 * i) : make_uint2(0u, 0u);
   }
 #pragma unroll
   for (int h = 0; h < HEADS; ++h)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int c = 8 * (l + 16 * i);
-      if (h0 + h >= a.kv_heads || c >= D) continue;
-      if (STORE != ACT) values8<STORE>(w[h][i], s[h], x[h][i]);
-      store8(dst + h * (value ? a.hsv : a.hsk) + c, x[h][i]);
+    for (int i = 0; i < NI; ++i) {
+      if (h0 + h >= a.kv_heads || 8 * (l + 16 * i) >= D) continue;
+      float x[8];
+      values8<STORE>(w[h][i], s[h], x);
+      store8(dst + h * hs + 128 * i, x);
     }
 }
 
@@ -235,18 +235,22 @@ static int rows_call(const char* who, const void* k_new, long long ldk, long lon
                 "%s: rows must be 16-byte aligned", who);
   if (rows == 0 || seqs == 0) return 0;
   Rows a{step_of(starts, lengths, table, ldt, width, rows, seqs, pages, page), k_new, v_new, ldk, hsk, ldv, hsv, k, v, ks, vs, kv_heads, K, V};
-  const long long units = (long long)rows * ((kv_heads + HEADS - 1) / HEADS);
-  // few units go one to a block, so they spread over the SMs
-  const int warps = units >= 8 * 148 ? 8 : 1;
+  // Few rows: two heads to a warp and a warp to a block, so they spread over the SMs; many: more heads, as a warp's look for its place is a third of its work then
+  constexpr int HEADS = WRITE ? 8 : 4;
+  const bool many = (long long)rows * kv_heads >= 64 * 148;
+  const int per_warp = many ? HEADS : 2, warps = many ? 8 : 1;
+  const long long units = (long long)rows * ((kv_heads + per_warp - 1) / per_warp);
   const long long blocks = (units + warps - 1) / warps;
   B2L_CHECK_SUPPORTED(blocks < (1ll << 31), "%s: %d rows of %d heads", who, rows, kv_heads);
   const cudaStream_t st = (cudaStream_t)stream;
-#define GO(T, ST)                                                                                                      \
-  (!WRITE ? paged_read_kernel<T, ST><<<(unsigned)blocks, 32 * warps, 0, st>>>(a)                                        \
-   : K <= 128 && V <= 128 ? paged_write_kernel<T, ST, 1><<<(unsigned)blocks, 32 * warps, 0, st>>>(a)                    \
-                          : paged_write_kernel<T, ST, 2><<<(unsigned)blocks, 32 * warps, 0, st>>>(a))
+#define LAUNCH(T, ST, NI, H)                                                                       \
+  (WRITE ? paged_write_kernel<T, ST, NI, H><<<(unsigned)blocks, 32 * warps, 0, st>>>(a)            \
+         : paged_read_kernel<T, ST, NI, H><<<(unsigned)blocks, 32 * warps, 0, st>>>(a))
+#define GO(T, ST) \
+  (K <= 128 && V <= 128 ? (many ? LAUNCH(T, ST, 1, HEADS) : LAUNCH(T, ST, 1, 2)) : (many ? LAUNCH(T, ST, 2, HEADS) : LAUNCH(T, ST, 2, 2)))
   B2L_SEQ_DISPATCH(act_dtype, if (store == ACT) GO(act_t, ACT); else if (store == E4M3) GO(act_t, E4M3); else GO(act_t, INT8));
 #undef GO
+#undef LAUNCH
   B2L_LAUNCH_CHECK("paged rows");
   return 0;
 }
