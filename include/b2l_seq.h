@@ -505,7 +505,8 @@ int b2l_seq_mlstm_readout(const b2l_seq_mlstm_args* a, b2l_stream_t stream);
  *   b2l_seq_paged_attention  out[r, h] = sum_j w_j v_j / sum_j w_j over the keys j that row r at position p sees, j <= p and (window == 0 or j > p - window
  *                            or j < first); w_j = exp(scale q . k_j - max); query head h reads key / value head h / (heads / kv_heads).  A row whose
  *                            weights sum to 0 (it sees no key) gives zeros.  scale > 0.  q and out act [rows, heads, K or V].
- *                            max_new, min_new, max_length: what the host knows of the step's sequences (0 or less: nothing); they pick between equivalent forms.
+ *                            max_new, max_length: the most new tokens and the longest of the step's sequences, where the host knows (0 or less: it does not); they pick
+ *                            between equivalent forms.
  *                            `work` has b2l_seq_paged_attention_work floats (may be null when that is 0).
  * ldX and hsX: elements between tokens and between heads (rows 16-byte aligned, the entries of a head consecutive). */
 enum { B2L_SEQ_STORE_ACT = 0, B2L_SEQ_STORE_E4M3 = 1, B2L_SEQ_STORE_INT8 = 2 };
@@ -517,9 +518,9 @@ int b2l_seq_paged_read(void* k_out, long long ldk, long long hsk, void* v_out, l
                        int K, int V, int store, int act_dtype, b2l_stream_t stream);
 int b2l_seq_paged_attention(const void* q, long long ldq, long long hsq, const void* k, const void* v, const float* k_scale, const float* v_scale, const int* starts,
                             const int* lengths, const int* table, int ldt, int width, void* out, float* work, long long work_floats, int rows, int seqs, int pages, int page,
-                            int heads, int kv_heads, int K, int V, int window, int first, float scale, int max_new, int min_new, int max_length, int store, int act_dtype,
+                            int heads, int kv_heads, int K, int V, int window, int first, float scale, int max_new, int max_length, int store, int act_dtype,
                             b2l_stream_t stream);
-long long b2l_seq_paged_attention_work(int rows, int seqs, int width, int page, int heads, int kv_heads, int K, int V, int window, int first, int max_new, int min_new,
+long long b2l_seq_paged_attention_work(int rows, int seqs, int width, int page, int heads, int kv_heads, int K, int V, int window, int first, int max_new,
                                        int max_length, int store, int act_dtype);
 
 #ifdef __cplusplus

@@ -216,8 +216,8 @@ _SIGS = {
     "b2l_seq_paged_write": (c_int, _PAGED_ROWS),
     "b2l_seq_paged_read": (c_int, _PAGED_ROWS),
     "b2l_seq_paged_attention": (c_int, [c_void_p, C.c_longlong, C.c_longlong] + [c_void_p] * 7 + [c_int] * 2 + [c_void_p] * 2 + [C.c_longlong] + [c_int] * 10 + [c_float]
-                                + [c_int] * 5 + [c_void_p]),
-    "b2l_seq_paged_attention_work": (C.c_longlong, [c_int] * 15),
+                                + [c_int] * 4 + [c_void_p]),
+    "b2l_seq_paged_attention_work": (C.c_longlong, [c_int] * 14),
 }
 
 EXPORTS = tuple(_SIGS)

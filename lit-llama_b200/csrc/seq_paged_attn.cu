@@ -138,8 +138,8 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
     pl.b = blockIdx.x;
     sequence(a.s, pl.b, pl.start, pl.n, pl.length);
     pl.first = 0;
-    if (pl.n == 0 || (long long)pl.n * G > a.few_max) return;
-  } else if (!a.place(blockIdx.x - a.s.seqs, R, 0, a.few_max, 1, lane, pl)) {
+    if (pl.n == 0) return;
+  } else if (!a.place(blockIdx.x - a.s.seqs, R, lane, pl)) {
     return;
   }
   __shared__ uint32_t bad;                                   // rows whose result is not finite
@@ -587,7 +587,7 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
     }
     const int row = pl.start + at / G, head = h * G + at % G;
     if (a.few.splits > 1) {
-      const long long to = (long long)split * a.few.count + (a.compact ? (long long)(pl.b * a.kv_heads + h) * 16 + at : (long long)row * a.heads + head);
+      const long long to = (long long)split * a.few.count + (long long)row * a.heads + head;
       if (d == 0) *reinterpret_cast<float2*>(a.few.ml + 2 * to) = make_float2(M, L);
       *reinterpret_cast<float4*>(a.few.o + to * a.V + d) = make_float4(x[0], x[1], x[2], x[3]);
     } else {
@@ -606,38 +606,17 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
 }
 
 // ------------------------------------------------------------------------------------------------ joining parts
-// `per` warps (a power of two) have a row and head, each every per-th part; rows of sequences whose parts were not split are in place already.  Parts are
-// read once, and the loads of a warp's parts do not wait for one another.  The first `short_units` units are the 16 packed rows of each of the few-row kernel's
-// sequences and a key/value head where both kernels run, the others the rows and heads from the first on.
+// `per` warps (a power of two) have a row and head, each every per-th part.  Parts are read once, and the loads of a warp's parts do not wait for one another.
 constexpr int MERGE_WARPS = 8;
-__global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const __grid_constant__ Attn a, int per, int short_units) {
+__global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const __grid_constant__ Attn a, int per) {
   __shared__ float4 sx[MERGE_WARPS][64];
   __shared__ float2 sml[MERGE_WARPS];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, G = a.heads / a.kv_heads;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
   const int here = MERGE_WARPS / per, sub = warp / here, own = warp % here;      // part of the unit's warps, unit of the block
-  long long unit = (long long)blockIdx.x * here + own;
-  const bool is_short = unit < short_units;
-  int row, head, b = -1, start = 0, n = 0, length = 0;
-  if (is_short) {
-    const int r = (int)(unit % 16), h = (int)(unit / 16 % a.kv_heads), at = (int)(unit / 16 / a.kv_heads);
-    if (at < a.s.seqs) {
-      sequence(a.s, at, start, n, length);
-      if (r < (long long)n * G && (long long)n * G <= a.few_max) b = at;
-    }
-    row = start + r / G;
-    head = h * G + r % G;
-  } else {
-    unit -= short_units;
-    row = (int)min(unit / a.heads, (long long)a.s.rows);
-    head = (int)(unit % a.heads);
-    if (row < a.s.rows) b = sequence_of(a.s, row, lane);
-    if (b >= 0) sequence(a.s, b, start, n, length);
-  }
-  const int h = head / G;
-  const bool few = (long long)n * G <= a.few_max;
-  const Parts& p = few ? a.few : a.many;
-  bool on = b >= 0 && p.splits > 1 && (!a.compact || few == is_short);
-  const long long at = few && a.compact ? (long long)(b * a.kv_heads + h) * 16 + (row - start) * G + head % G : (long long)row * a.heads + head;
+  const long long at = (long long)blockIdx.x * here + own;
+  const int row = (int)min(at / a.heads, (long long)a.s.rows), head = (int)(at % a.heads), b = row < a.s.rows ? sequence_of(a.s, row, lane) : -1;
+  const Parts& p = a.few;
+  const bool on = b >= 0;
   float M = -INFINITY, L = 0.f;
   float4 x[2] = {};
   pdl_wait();                                                // launched while the parts are computed
@@ -650,10 +629,6 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const __g
 #pragma unroll
       for (int c = 0; c < 2; ++c) z[c] = 4 * (lane + 32 * c) < a.V ? y[32 * c] : make_float4(0.f, 0.f, 0.f, 0.f);
       if (ml.x == -INFINITY && ml.y == 0.f) continue;        // saw nothing
-      if (ml.x == INFINITY && ml.y == 0.f) {                 // was not shared: its result is in place
-        on = false;
-        break;
-      }
       const float now = fmaxf(M, ml.x), f = M == now ? 1.f : exp2_f(M - now), w = ml.x == now ? 1.f : exp2_f(ml.x - now);
       M = now;
       L = L * f + w * ml.y;
@@ -695,71 +670,45 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const __g
   }
   if (!__all_sync(0xffffffffu, fine)) {
     __syncwarp();
+    int start, n, length;
+    sequence(a.s, b, start, n, length);
     mend_row(a, b, length - n + row - start, row, head, lane);
   }
 }
 
 // ------------------------------------------------------------------------------------------------ host
 struct Plan {
-  bool few, many;
-  int few_max, few_rows, few_tiles, many_tiles, many_whole, part_rows, few_splits, many_splits, compact;
-  long long many_ctas, few_count, many_count, floats;
+  int few_rows, few_tiles, few_splits, many_ctas;            // many_ctas: of the chunk kernel, 0 where the few-row kernel takes the step
+  long long floats;
 };
 constexpr long long MOST_WORK = 1ll << 27;                   // floats of partial results
 
-static Plan plan_of(int rows, int seqs, int width, int page, int heads, int kv_heads, int K, int V, int window, int first, int max_new, int min_new, int max_length, int store,
-                    int act_dtype) {
+static long long few_floats(int splits, long long count, int V) { return splits > 1 ? (2 * splits * count + 3) / 4 * 4 + splits * count * V : 0; }
+
+static Plan plan_of(int rows, int seqs, int width, int page, int heads, int kv_heads, int K, int V, int window, int first, int max_new, int max_length, int store, int act_dtype) {
   Plan p{};
-  const int G = heads / kv_heads, sms = sm_count();
-  const bool tensor = act_dtype == B2L_BF16 && many_takes(K, V, store);
-  const long long packed = (long long)rows * G;
-  p.few = !tensor || !(min_new > 0 && (long long)min_new * G > 16);
-  p.many = tensor && !(max_new > 0 && (long long)max_new * G <= 16);
-  p.few_max = !p.many ? INT32_MAX : p.few ? 16 : 0;
-  p.compact = p.few && p.many;
-  const int most = std::min(seqs, rows);
-  // rows of a tile: 8 where a token's heads, or all that the longest of the sequences has, fit
-  p.few_rows = (max_new > 0 ? (long long)max_new * G <= 8 : G <= 8 && packed <= 8ll * most) && !p.compact ? 8 : 16;
-  p.few_tiles = seqs + (p.compact ? 0 : (int)std::min<long long>(packed / p.few_rows, INT32_MAX - seqs));
-  p.many_tiles = (int)std::min<long long>(packed / 256 + most, INT32_MAX);
+  const int G = heads / kv_heads, sms = sm_count(), most = std::min(seqs, rows);
+  const long long packed = (long long)rows * G, longest = (long long)(max_new > 0 ? std::min(max_new, rows) : rows) * G;      // packed rows of one sequence
   long long keys = (long long)width * page;                  // the most keys that a row sees
   if (max_length > 0) keys = std::min<long long>(keys, max_length);
   if (window > 0) keys = std::min<long long>(keys, (long long)window + first + 16);
-  p.few_splits = p.many_splits = 1;
-  p.few_count = p.compact ? (long long)seqs * kv_heads * 16 : (long long)rows * heads;
-  p.many_count = (long long)rows * heads;
-  if (p.few) {
-    // An SM has three CTAs at a time.  Few CTAs: as many parts as fill them once, of 128 keys at least (one token over 1031 keys of 32 heads: 15.1 us in 4 parts,
-    // 13.0 in 8).  Many: parts of a quarter of that each, of 512 keys at least, so that sequences of different lengths share the SMs evenly (48 over up to 8192
-    // keys of an e4m3 pool: 143 us whole, 128 in 4 parts, 140 in 8)
-    const long long ctas = (long long)kv_heads * std::max<long long>(seqs, p.compact ? 0 : packed / p.few_rows), slots = 3ll * sms;
-    const bool room = 2 * ctas <= slots;
-    const long long want = room ? slots / ctas : (4 * slots + ctas - 1) / ctas;
-    p.few_splits = (int)std::max<long long>(1, std::min({want, keys / (room ? 128 : 512), 128ll, MOST_WORK / (p.few_count * (V + 2) + 1)}));
+  // The chunk kernel takes steps with a sequence of more than 16 packed rows, single tokens among them too
+  if (act_dtype == B2L_BF16 && longest > 16 && many_takes(K, V, store)) {
+    p.many_ctas = many_ctas((packed / 256 + most) * kv_heads, keys + (window > 0 ? 256 / G : 0), sms);
+    p.floats = many_floats(p.many_ctas, V);
+    return p;
   }
-  if (p.many) {
-    // One CTA on an SM at a time, some 1.8 us (8-bit: 2.8) for 128 keys of 128 + 128 entries and 15 beside.  Row tiles that fill rounds of all SMs run whole; the
-    // rest in as many parts as make what is left shortest, a launch of 8 us and 4 TB/s for the parts' results included: 256 tokens over 16384 of 32 / 8 heads,
-    // 32 row tiles, take 234 us whole, 131 in 2 parts, 80 in 4 and 120 in 5, a second round
-    const long long rest = (packed + 255) / 256 + (min_new == max_new && seqs == 1 ? 0 : seqs / 2);
-    const long long items = (long long)kv_heads * std::max<long long>(1, std::min<long long>(rest, p.many_tiles)), whole = items / sms * sms, left = items - whole;
-    const double tiles = (keys + 127) / 128, tile = (store == ACT ? 1.8 : 2.8) * (K + V) / 256;
-    double least = 0;
-    p.many_splits = 1;
-    for (int s = 1; left > 0 && s <= 16 && s <= tiles && (s == 1 || (long long)s * p.many_count * (V + 2) <= MOST_WORK); ++s) {
-      const double us = std::ceil((double)left * s / sms) * (std::ceil(tiles / s) * tile + 15) + (s > 1 ? 8 + s * left * 256.0 * V * 4 / 4e6 : 0);
-      if (s == 1 || us < 0.95 * least) {
-        least = us;
-        p.many_splits = s;
-      }
-    }
-    p.many_whole = (int)std::min<long long>(p.many_splits > 1 ? whole : 0, INT32_MAX);
-    p.many_ctas = p.many_whole + std::max<long long>(0, (long long)p.many_tiles * kv_heads - p.many_whole) * p.many_splits;
-    // the rows that may have parts: the last row tiles to be begun are the first ones, and between them lie short sequences
-    p.part_rows = p.many_splits == 1 ? 0 : (int)std::min<long long>(rows, whole == 0 ? rows : ((long long)p.many_tiles - whole / kv_heads + 1) * (256 / std::min(G, 256) + 1) + 16ll * seqs);
-  }
-  auto floats = [&](int splits, long long count) { return splits > 1 ? (2 * splits * count + 3) / 4 * 4 + splits * count * V : 0; };
-  p.floats = (p.few ? floats(p.few_splits, p.few_count) : 0) + (p.many ? floats(p.many_splits, p.many_count) : 0);
+  // rows of a tile: 8 where a token's heads, or all that the longest of the sequences has, fit
+  p.few_rows = (max_new > 0 ? (long long)max_new * G <= 8 : G <= 8 && packed <= 8ll * most) ? 8 : 16;
+  p.few_tiles = seqs + (int)std::min<long long>(packed / p.few_rows, INT32_MAX - seqs);
+  // An SM has three CTAs at a time.  Few CTAs: as many parts as fill them once, of 128 keys at least (one token over 1031 keys of 32 heads: 15.1 us in 4 parts,
+  // 13.0 in 8).  Many: parts of a quarter of that each, of 512 keys at least, so that sequences of different lengths share the SMs evenly (48 over up to 8192
+  // keys of an e4m3 pool: 143 us whole, 128 in 4 parts, 140 in 8)
+  const long long ctas = (long long)kv_heads * std::max<long long>(seqs, packed / p.few_rows), slots = 3ll * sms, count = (long long)rows * heads;
+  const bool room = 2 * ctas <= slots;
+  const long long want = room ? slots / ctas : (4 * slots + ctas - 1) / ctas;
+  p.few_splits = (int)std::max<long long>(1, std::min({want, keys / (room ? 128 : 512), 128ll, MOST_WORK / (count * (V + 2) + 1)}));
+  p.floats = few_floats(p.few_splits, count, V);
   return p;
 }
 
@@ -796,15 +745,15 @@ template <typename act_t, int STORE, int NV, int NR> static int few_launch(const
 
 using namespace b2l;
 
-extern "C" long long b2l_seq_paged_attention_work(int rows, int seqs, int width, int page, int heads, int kv_heads, int K, int V, int window, int first, int max_new, int min_new,
+extern "C" long long b2l_seq_paged_attention_work(int rows, int seqs, int width, int page, int heads, int kv_heads, int K, int V, int window, int first, int max_new,
                                                   int max_length, int store, int act_dtype) {
   if (rows <= 0 || seqs <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0) return 0;
-  return paged::plan_of(rows, seqs, width, page, heads, kv_heads, K, V, window, first, max_new, min_new, max_length, store, act_dtype).floats;
+  return paged::plan_of(rows, seqs, width, page, heads, kv_heads, K, V, window, first, max_new, max_length, store, act_dtype).floats;
 }
 
 extern "C" int b2l_seq_paged_attention(const void* q, long long ldq, long long hsq, const void* k, const void* v, const float* k_scale, const float* v_scale, const int* starts,
                                        const int* lengths, const int* table, int ldt, int width, void* out, float* work, long long work_floats, int rows, int seqs, int pages,
-                                       int page, int heads, int kv_heads, int K, int V, int window, int first, float scale, int max_new, int min_new, int max_length, int store,
+                                       int page, int heads, int kv_heads, int K, int V, int window, int first, float scale, int max_new, int max_length, int store,
                                        int act_dtype, b2l_stream_t stream) {
   using namespace paged;
   const char* who = "b2l_seq_paged_attention";
@@ -818,7 +767,7 @@ extern "C" int b2l_seq_paged_attention(const void* q, long long ldq, long long h
   B2L_CHECK_SUPPORTED((long long)width * page < (1ll << 30) && kv_heads < 65536 && (long long)rows * heads < (1ll << 31) && (long long)pages * kv_heads * page < (1ll << 31),
                       "%s: sizes beyond the grid's or a copy's coordinates", who);
   if (rows == 0 || seqs == 0) return 0;
-  const Plan p = plan_of(rows, seqs, width, page, heads, kv_heads, K, V, window, first, max_new, min_new, max_length, store, act_dtype);
+  const Plan p = plan_of(rows, seqs, width, page, heads, kv_heads, K, V, window, first, max_new, max_length, store, act_dtype);
   B2L_CHECK_ARG(p.floats == 0 || (work && work_floats >= p.floats), "%s: a work space of %lld floats is needed", who, p.floats);
   Attn a{};
   a.s = step_of(starts, lengths, table, ldt, width, rows, seqs, pages, page);
@@ -826,43 +775,25 @@ extern "C" int b2l_seq_paged_attention(const void* q, long long ldq, long long h
   a.ldq = ldq; a.hsq = hsq;
   a.heads = heads; a.kv_heads = kv_heads; a.K = K; a.V = V;
   a.window = window; a.first = window ? first : 0;
-  a.few_max = p.few_max;
   a.scale_log2 = scale * 1.44269502162933349609375f;         // log2(e)
-  a.f32 = act_dtype == B2L_F32; a.store_kind = store; a.compact = p.compact;
-  auto take = [&](Parts& x, int splits, long long count) {
-    x.splits = splits;
-    x.count = count;
-    if (splits <= 1) return;
-    x.ml = work;
-    x.o = work + (2 * splits * count + 3) / 4 * 4;
-    work = x.o + splits * count * V;
-  };
-  take(a.few, p.few ? p.few_splits : 1, p.few_count);
-  take(a.many, p.many ? p.many_splits : 1, p.many_count);
+  a.f32 = act_dtype == B2L_F32; a.store_kind = store;
   const cudaStream_t st = (cudaStream_t)stream;
-  if (p.few) {
-    int rc = 0;
-    const bool small = V <= 128 && K <= 128;
+  if (p.many_ctas) return many_launch(a, p.many_ctas, work, st);
+  a.few.splits = p.few_splits;
+  a.few.count = (long long)rows * heads;
+  a.few.ml = work;
+  a.few.o = work + (2 * p.few_splits * a.few.count + 3) / 4 * 4;
+  int rc = 0;
+  const bool small = V <= 128 && K <= 128;
 #define GO(ST)                                                                                                                              \
   (p.few_rows == 8 ? (small ? few_launch<act_t, ST, 8, 1>(a, p.few_tiles, st) : few_launch<act_t, ST, 16, 1>(a, p.few_tiles, st))            \
                    : (small ? few_launch<act_t, ST, 8, 2>(a, p.few_tiles, st) : few_launch<act_t, ST, 16, 2>(a, p.few_tiles, st)))
-    B2L_SEQ_DISPATCH(act_dtype, rc = store == ACT ? GO(ACT) : store == E4M3 ? GO(E4M3) : GO(INT8));
+  B2L_SEQ_DISPATCH(act_dtype, rc = store == ACT ? GO(ACT) : store == E4M3 ? GO(E4M3) : GO(INT8));
 #undef GO
-    if (rc) return rc;
-  }
-  if (p.many) {
-    B2L_CHECK_SUPPORTED(p.many_ctas < (1ll << 31), "%s: sizes beyond the grid's", who);
-    a.many_whole = p.many_whole;
-    if (int rc = many_launch(a, (int)p.many_ctas, st)) return rc;
-  }
-  if (a.few.splits > 1 || a.many.splits > 1) {
-    const int most = std::max(a.few.splits, a.many.splits), per = most >= 32 ? 8 : most >= 16 ? 4 : most >= 8 ? 2 : 1, here = MERGE_WARPS / per;
-    const long long short_units = p.compact && a.few.splits > 1 ? 16ll * kv_heads * seqs : 0, at_rows = p.compact || a.few.splits == 1 ? p.part_rows : rows;
-    const long long units = short_units + at_rows * heads;
-    B2L_CHECK_SUPPORTED(units < (1ll << 31), "%s: sizes beyond the grid's", who);
-    LaunchCfg launch(dim3((unsigned)((units + here - 1) / here)), dim3(32 * MERGE_WARPS), 0, st, true);
-    B2L_CUDA(cudaLaunchKernelEx(&launch.cfg, paged_merge_kernel, a, per, (int)short_units));
-    B2L_LAUNCH_CHECK("paged_merge_kernel");
-  }
+  if (rc || p.few_splits == 1) return rc;
+  const int warps = p.few_splits >= 32 ? 8 : p.few_splits >= 16 ? 4 : p.few_splits >= 8 ? 2 : 1, here = MERGE_WARPS / warps;
+  LaunchCfg launch(dim3((unsigned)((a.few.count + here - 1) / here)), dim3(32 * MERGE_WARPS), 0, st, true);
+  B2L_CUDA(cudaLaunchKernelEx(&launch.cfg, paged_merge_kernel, a, warps));
+  B2L_LAUNCH_CHECK("paged_merge_kernel");
   return 0;
 }

@@ -60,23 +60,26 @@ struct Keys {
 // partial results of `splits` CTAs per row: maximum and sum [splits][count][2], outputs [splits][count][V]
 struct Parts { float *ml, *o; int splits; long long count; };
 
+// What the CTAs of the chunk kernel leave for one another: of each the last row tile if it goes on in the next CTA (sequence, first packed row, head, number of
+// CTAs that have a part; none: 0), and two places for partial results of 256 rows (the first row tile's, the last one's) [2 ctas][256][2] and [2 ctas][256][V]
+struct Shared { int4* last; float *ml, *o; int ctas; };
+
 struct Attn {
   Step s;
   const void *q, *k, *v;
   const float *ks, *vs;
   void* out;
   long long ldq, hsq;
-  int heads, kv_heads, K, V, window, first, few_max;        // few_max: sequences of at most so many packed rows are the few-row kernel's
+  int heads, kv_heads, K, V, window, first;
   float scale_log2;
-  int f32, store_kind, compact;
-  int many_whole;                                            // row tiles and heads, in the order they are begun, that are not shared among CTAs
-  Parts few, many;                                           // compact in `few` where both kernels run: 16 packed rows per sequence and key/value head
+  int f32, store_kind;
+  Parts few;
+  Shared many;
 
   __device__ __forceinline__ bool sees(int pos, int j) const { return j <= pos && (window == 0 || j > pos - window || j < first); }
 
-  // Tile `slot` of the tiles of R packed rows, without the first `skip` of each, of all sequences with more than `above` and at most `most` packed rows; a
-  // whole warp looks
-  __device__ __forceinline__ bool place(int slot, int R, int above, int most, int skip, int lane, Place& pl) const {
+  // Tile `slot` of the tiles of R packed rows of all sequences, without the first of each; a whole warp looks
+  __device__ __forceinline__ bool place(int slot, int R, int lane, Place& pl) const {
     const int G = heads / kv_heads;
     int base = 0;
     for (int b0 = 0; b0 < s.seqs; b0 += 32) {
@@ -85,7 +88,7 @@ struct Attn {
       if (b < s.seqs) {
         sequence(s, b, start, n, length);
         const long long packed = (long long)n * G;
-        tiles = packed > above && packed <= most ? max((int)((packed + R - 1) / R) - skip, 0) : 0;
+        tiles = max((int)((packed + R - 1) / R) - 1, 0);
       }
       int upto = tiles;
 #pragma unroll
@@ -100,24 +103,12 @@ struct Attn {
         pl.start = __shfl_sync(0xffffffffu, start, at);
         pl.n = __shfl_sync(0xffffffffu, n, at);
         pl.length = __shfl_sync(0xffffffffu, length, at);
-        pl.first = (slot - base - __shfl_sync(0xffffffffu, upto - tiles, at) + skip) * R;
+        pl.first = (slot - base - __shfl_sync(0xffffffffu, upto - tiles, at) + 1) * R;
         return true;
       }
       base += __shfl_sync(0xffffffffu, upto, 31);
     }
     return false;
-  }
-  // The same counted from the last one
-  __device__ __forceinline__ bool place_back(int slot, int R, int above, int most, int lane, Place& pl) const {
-    const int G = heads / kv_heads;
-    int total = 0;
-    for (int b0 = 0; b0 < s.seqs; b0 += 32) {
-      int start, n = 0, length;
-      if (b0 + lane < s.seqs) sequence(s, b0 + lane, start, n, length);
-      const long long packed = (long long)n * G;
-      total += __reduce_add_sync(0xffffffffu, packed > above && packed <= most ? (int)((packed + R - 1) / R) : 0);
-    }
-    return slot < total && place(total - 1 - slot, R, above, most, 0, lane, pl);
   }
   __device__ __forceinline__ Keys keys(const Place& pl, int R) const {
     const int G = heads / kv_heads, last = min(pl.first + R, pl.n * G) - 1;
@@ -194,9 +185,11 @@ __device__ __forceinline__ bool finite4(const float (&x)[4], float inv) {
   return fabsf(x[0] * inv) < INFINITY && fabsf(x[1] * inv) < INFINITY && fabsf(x[2] * inv) < INFINITY && fabsf(x[3] * inv) < INFINITY;
 }
 
-// the tensor-core kernel of longer chunks (seq_paged_tc.cu): heads that it takes, and its launch
+// the tensor-core kernel of longer chunks (seq_paged_tc.cu): heads that it takes, the CTAs for at most so many row tiles and keys, its work space, its launch
 bool many_takes(int K, int V, int store);
-int many_launch(const Attn& a, int ctas, cudaStream_t stream);
+int many_ctas(long long row_tiles, long long keys, int sms);
+long long many_floats(int ctas, int V);
+int many_launch(Attn& a, int ctas, float* work, cudaStream_t stream);
 
 }  // namespace paged
 }  // namespace b2l

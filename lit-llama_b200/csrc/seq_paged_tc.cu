@@ -23,6 +23,7 @@
 //
 // Tensor memory: scores and weights of the row tiles at columns 0 and 128, outputs at 256 and 384.  Shared memory: the queries of both, two stages of keys
 // and values where they fit (8-bit: of values, and a tile of codes).  One CTA per SM.
+#include <algorithm>
 #include <utility>
 
 #include "attn_tc.cuh"
@@ -44,11 +45,21 @@ constexpr int INFOS = 4;
 struct alignas(16) Info {                                    // of a tile of keys, for the softmax (read by 16 bytes)
   float ks[KEYS];                                            // scale of the key, NaN where the row is to be computed again (8-bit pools)
   uint32_t there;                                            // 16 keys each: whether their page is there
+  float up;                                                  // 8-bit pools: what the values' scales are multiplied with
+};
+// A row tile: 256 packed rows of a head, the tiles of its sequence's rows one after the other, then the next head's, then the next sequence's
+struct Walk {
+  Place pl;
+  int h;
+  long long at;                                              // cost of all before it
 };
 struct Control {
   uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_half[2][2], o_done[2], info_full[INFOS], tail, gave_up;
   uint64_t ref_full, rk_full, rk_empty, rv_full, rv_empty;   // 8-bit pools: the first tile's largest scale, codes of keys and values
-  uint32_t tmem, ref;                                        // ref: largest scale of the first tile's values, as bits
+  uint32_t tmem, ref[3];                                     // ref: largest scale of the first tile's values, as bits, of a row tile, the next and the one before
+  long long x0, x1;                                          // the CTA's part
+  Walk at[16];                                               // each warp's row tile
+  long long costs[16];                                       // of the sequences that a warp counts
 };
 struct Codes {                                               // 8-bit pools: what lies beside a tile's codes
   float ks[KEYS], vs[KEYS];                                  // scales
@@ -168,6 +179,93 @@ __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xfffffff
 // place of the 16-byte piece c of row r in tiles of 128 rows
 __device__ __forceinline__ uint32_t piece_at(int r, int c) { return (uint32_t)((c >> 3) * TC_ATOM + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
 
+// ---- which CTA computes what: an equal part of the cost of everything, in the order of `Walk`, so a CTA has whole row tiles and begins and ends inside one.
+// Every CTA counts the cost itself.  A tile of keys costs 4 (3 where the row tile has one half only), a row tile 16 beside.
+constexpr int EXTRA = 16, LEAST = 2, SMALLEST_SHARE = 48;      // LEAST: tiles of keys that a cut leaves on either side
+
+struct Cost {
+  int all, units, each;                                      // tiles of keys, the same but one at least, cost of each
+  __device__ __forceinline__ int total() const { return EXTRA + units * each; }
+  __device__ __forceinline__ int cut(long long d) const {      // tiles of keys before a cut at d
+    if (d <= 0) return 0;
+    if (d >= total()) return units;
+    const int y = max((int)d - EXTRA, 0) / each;
+    return y < LEAST ? 0 : units - y < LEAST ? units : y;
+  }
+};
+__device__ __forceinline__ Cost cost_of(const Attn& a, const Place& pl) {
+  Cost c;
+  c.all = a.keys(pl, ROWS).units(7);
+  c.units = max(c.all, 1);
+  c.each = pl.n * (a.heads / a.kv_heads) - pl.first > TILE ? 4 : 3;
+  return c;
+}
+// of one head of a sequence, by a whole warp
+__device__ __forceinline__ long long sequence_cost(const Attn& a, Place pl, int lane) {
+  long long sum = 0;
+  for (pl.first = lane * ROWS; pl.first < pl.n * (a.heads / a.kv_heads); pl.first += 32 * ROWS) sum += cost_of(a, pl).total();
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum;
+}
+// each sequence lo .. hi - 1 with rows, until f says true
+template <typename F> __device__ __forceinline__ void each_sequence(const Attn& a, int lo, int hi, int lane, F f) {
+  for (int b0 = lo; b0 < hi; b0 += 32) {
+    int start = 0, n = 0, length = 0;
+    if (b0 + lane < hi) sequence(a.s, b0 + lane, start, n, length);
+    for (uint32_t left = __ballot_sync(0xffffffffu, n > 0); left; left &= left - 1) {
+      const int i = __ffs(left) - 1;
+      if (f(Place{b0 + i, __shfl_sync(0xffffffffu, start, i), __shfl_sync(0xffffffffu, n, i), __shfl_sync(0xffffffffu, length, i), 0})) return;
+    }
+  }
+}
+// the row tile after this one; pl.n is 0 behind the last
+__device__ __forceinline__ void advance(const Attn& a, Walk& w, const Cost& c, int lane) {
+  w.at += c.total();
+  if (w.pl.n * (a.heads / a.kv_heads) - w.pl.first > ROWS) {
+    w.pl.first += ROWS;
+    return;
+  }
+  w.pl.first = 0;
+  if (++w.h < a.kv_heads) return;
+  w.h = 0;
+  w.pl.n = 0;
+  each_sequence(a, w.pl.b + 1, a.s.seqs, lane, [&](const Place& pl) {
+    w.pl = pl;
+    return true;
+  });
+}
+// Every warp goes through the CTA's row tiles by itself: this one (tiles of keys t0 .. t1 - 1), and what follows it in shared memory, as registers are few
+struct Item {
+  Place pl;
+  int h, t0, t1, n;                                          // n: tiles of keys that its rows see
+  bool whole;
+};
+__device__ __forceinline__ bool next(const Attn& a, Control& ct, int warp, int lane, Item& x) {
+  Walk w = ct.at[warp];
+  const long long x0 = ct.x0, x1 = ct.x1;
+  bool found = false;
+  while (!found && w.pl.n > 0 && w.at < x1) {
+    const Cost c = cost_of(a, w.pl);
+    x.t0 = c.cut(x0 - w.at);
+    x.t1 = c.cut(x1 - w.at);
+    if ((found = x.t0 < x.t1)) {
+      x.pl = w.pl;
+      x.h = w.h;
+      x.whole = x.t0 == 0 && x.t1 == c.units;
+      x.t1 = min(x.t1, c.all);
+      x.n = max(x.t1 - x.t0, 0);
+    }
+    advance(a, w, c, lane);
+  }
+  __syncwarp();
+  if (lane == 0) ct.at[warp] = w;
+  __syncwarp();
+  return found;
+}
+
+__device__ __forceinline__ int pl_groups(const Place& pl, int G) { return pl.n * G - pl.first > TILE ? 2 : 1; }
+
 template <int STORE>
 __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel(const __grid_constant__ Attn a, const __grid_constant__ CUtensorMap map_k,
                                                                                   const __grid_constant__ CUtensorMap map_v, int k_stages, int v_stages) {
@@ -178,15 +276,58 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
   Info* infos = reinterpret_cast<Info*>(smem + CONTROL_BYTES);      // ACT: only `there`, at uint32_t steps
   uint32_t* there_of = reinterpret_cast<uint32_t*>(smem + CONTROL_BYTES);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.heads / a.kv_heads;
-  // Later rows, which mostly have more keys, first; the first ones whole, what would be a last round that is not full in parts
-  const int over = (int)blockIdx.x - a.many_whole, splits = over < 0 ? 1 : a.many.splits, split = over < 0 ? 0 : over % splits;
-  const int item = over < 0 ? (int)blockIdx.x : a.many_whole + over / splits, h = item % a.kv_heads;
-  Place pl;
-  if (!a.place_back(item / a.kv_heads, ROWS, a.few_max, INT32_MAX, lane, pl)) return;
-  const int rows = min(ROWS, pl.n * G - pl.first), groups = rows > TILE ? 2 : 1;
-  const Keys keys = a.keys(pl, ROWS);
-  const int all = keys.units(7), per = (all + splits - 1) / splits;
-  const int t0 = min(split * per, all), n = min(t0 + per, all) - t0;
+  // this CTA's part, x0 .. x1
+  {
+    const int warps = blockDim.x / 32, by = (a.s.seqs + warps - 1) / warps, lo = min(warp * by, a.s.seqs), hi = min(lo + by, a.s.seqs);
+    long long mine = 0, before = 0, all = 0;
+    each_sequence(a, lo, hi, lane, [&](const Place& pl) {
+      mine += sequence_cost(a, pl, lane) * a.kv_heads;
+      return false;
+    });
+    if (lane == 0) ct.costs[warp] = mine;
+    __syncthreads();
+    for (int i = 0; i < warps; ++i) {
+      if (i == warp) before = all;
+      all += ct.costs[i];
+    }
+    const long long share = max((all + gridDim.x - 1) / gridDim.x, (long long)SMALLEST_SHARE);
+    const long long x0 = blockIdx.x * share;
+    if (x0 >= all) {                                         // nothing is left
+      if (tid == 0) a.many.last[blockIdx.x] = make_int4(0, 0, 0, 0);
+      return;
+    }
+    if (tid == 0) {
+      ct.x0 = x0;
+      ct.x1 = min(x0 + share, all);
+    }
+    if (before <= x0 && x0 < before + mine)
+      each_sequence(a, lo, hi, lane, [&](Place pl) {
+        const long long one = sequence_cost(a, pl, lane);
+        if (x0 >= before + one * a.kv_heads) {
+          before += one * a.kv_heads;
+          return false;
+        }
+        const int h = (int)((x0 - before) / one);
+        before += h * one;
+        for (int f0 = 0;; f0 += 32 * ROWS) {                 // the row tile of the head's
+          pl.first = f0 + lane * ROWS;
+          long long upto = pl.first < pl.n * G ? cost_of(a, pl).total() : 0;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+          }
+          const uint32_t past = __ballot_sync(0xffffffffu, x0 < before + upto);
+          if (past) {
+            const int k = __ffs(past) - 1, first = __shfl_sync(0xffffffffu, pl.first, k);
+            const long long at = __shfl_sync(0xffffffffu, before + upto - cost_of(a, pl).total(), k);
+            if (lane < warps) ct.at[lane] = Walk{Place{pl.b, pl.start, pl.n, pl.length, first}, h, at};
+            return true;
+          }
+          before += __shfl_sync(0xffffffffu, upto, 31);
+        }
+      });
+  }
   const int ka = atoms_of(a.K, 2), va = atoms_of(a.V, 2);
   const uint32_t sq = smem_u32(smem) + CONTROL_BYTES + INFO_BYTES<STORE>, sk = sq + 2 * ka * TC_ATOM, sv = sk + k_stages * ka * TC_ATOM;
   const uint32_t raw_k = sv + v_stages * va * TC_ATOM, raw_v = raw_k + KEYS * a.K;      // 8-bit pools
@@ -213,7 +354,7 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
     mbar_init(bar(ct.rv_full), 1);
     mbar_init(bar(ct.rk_empty), 128);
     mbar_init(bar(ct.rv_empty), 128);
-    ct.ref = 0u;
+    for (int i = 0; i < 3; ++i) ct.ref[i] = 0u;
     mbar_init_fence();
   }
   if (warp == 0) tmem_alloc(smem_u32(&ct.tmem), 512);
@@ -221,6 +362,7 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
   __syncthreads();
   fence_after();
   const uint32_t tmem = ct.tmem;
+  Item x;
   if (warp < 4) {
    // 8-bit pool: a row's 128 scores in registers, which the softmax takes from the other warps (56 x 128 + 184 x 256 + 88 x 128 = 128 x 512)
    if constexpr (HALF) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -231,8 +373,8 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
     const uint32_t id_s = (1u << 4) | types | ((uint32_t)(KEYS >> 3) << 17) | ((uint32_t)(TILE >> 4) << 24);
     const uint32_t id_o = (1u << 4) | types | (1u << 16) | ((uint32_t)(a.V >> 3) << 17) | ((uint32_t)(TILE >> 4) << 24);
     const int steps = a.K / 16;
-    int kst = 0, vst = 0;
-    uint32_t kph = 0, vph = 0;
+    int kst = 0, vst = 0, groups = 0;
+    uint32_t kph = 0, vph = 0, item = 0, done[2] = {0, 0};      // row tiles; tiles of keys of each half
     auto scores = [&](int g) {
 #pragma unroll 1
       for (int x = 0; 4 * x < steps; ++x) {
@@ -247,19 +389,21 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
         if (++kst == k_stages) { kst = 0; kph ^= 1u; }
       }
     };
-    if (n > 0) {
-      wait_lead(bar(ct.q_full), 0, lead, dead);
-      wait_lead(bar(ct.k_full[0]), 0, lead, dead);
-      fence_after();
-      for (int g = 0; g < groups && !dead; ++g) scores(g);
-    }
-    for (int t = 0; t < n && !dead; ++t) {
+    while (!dead && next(a, ct, warp, lane, x)) {
+     const int n = x.n;
+     if (n == 0) continue;                                   // rows that see nothing
+     groups = pl_groups(x.pl, G);
+     wait_lead(bar(ct.q_full), item++ & 1u, lead, dead);
+     wait_lead(bar(ct.k_full[kst]), kph, lead, dead);
+     fence_after();
+     for (int g = 0; g < groups && !dead; ++g) scores(g);
+     for (int t = 0; t < n && !dead; ++t) {
       wait_lead(bar(ct.v_full[vst]), vph, lead, dead);
 #pragma unroll 1
       for (int g = 0; g < groups; ++g) {
 #pragma unroll
         for (int half = 1; half >= 0; --half) {
-          wait_lead(bar(ct.p_half[g][half]), (uint32_t)t & 1u, lead, dead);
+          wait_lead(bar(ct.p_half[g][half]), (done[g] + t) & 1u, lead, dead);
           if (dead) break;
           fence_after();
           const uint64_t vd = desc_mn(sv + vst * va * TC_ATOM + half * (TC_ATOM / 2), TC_ATOM);
@@ -278,6 +422,9 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
         }
       }
       if (++vst == v_stages) { vst = 0; vph ^= 1u; }
+     }
+     done[0] += n;
+     if (groups > 1) done[1] += n;
     }
     if (dead) {                                              // what was issued ends before tensor memory is given back
       uint32_t late = 0;
@@ -289,11 +436,14 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
     // ===================== tiled copies =====================
     const int box = min(1 << a.s.shift, KEYS), boxes = KEYS / box, gone = (a.s.pages * a.kv_heads) << a.s.shift;      // a row beyond the pool: zeros
     int kst = 0, vst = 0;
-    uint32_t kph = 1, vph = 1, tail_waits = 0;               // a stage is free at first
-    for (int t = 0; t < n; ++t) {
-      const int key0 = keys.key0(t0 + t, 7);
+    uint32_t kph = 1, vph = 1, tail_waits = 0, tile = 0;     // a stage is free at first
+    while (!dead && next(a, ct, warp, lane, x)) {
+     const Keys keys = a.keys(x.pl, ROWS);
+     const int h = x.h, sequence = x.pl.b;
+     for (int t = x.t0; t < x.t1; ++t, ++tile) {
+      const int key0 = keys.key0(t, 7);
       int page = -1;
-      if (lane < boxes && key0 + lane * box < keys.end) page = page_of(a.s, pl.b, key0 + lane * box);
+      if (lane < boxes && key0 + lane * box < keys.end) page = page_of(a.s, sequence, key0 + lane * box);
       const uint32_t seen = __ballot_sync(0xffffffffu, page >= 0);
       const int row = page >= 0 ? ((page * a.kv_heads + h) << a.s.shift) + ((key0 + lane * box) & ((1 << a.s.shift) - 1)) : gone;
       uint32_t there = 0;                                    // by 16 keys
@@ -302,9 +452,9 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
       mbar_wait_warp(bar(HALF ? ct.rk_empty : ct.k_empty[kst]), kph, dead);
       if (dead) break;
       if (lane == 0) {
-        if (HALF) infos[t % INFOS].there = there;
-        else there_of[t % INFOS] = there;
-        mbar_arrive(bar(ct.info_full[t % INFOS]));
+        if (HALF) infos[tile % INFOS].there = there;
+        else there_of[tile % INFOS] = there;
+        mbar_arrive(bar(ct.info_full[tile % INFOS]));
         mbar_expect_tx(k_to, HALF ? KEYS * (a.K + 8) : ka * TC_ATOM);
       }
       __syncwarp();                                          // the bytes are expected before they come
@@ -343,6 +493,7 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
         if (lane == 0) mbar_arrive(bar(ct.v_full[vst]));
       }
       if (HALF || ++vst == v_stages) { vst = 0; vph ^= 1u; }
+     }
     }
     // every copy has landed before the CTA ends: what reads them comes after, unless a wait ran out
     if (dead) {
@@ -352,6 +503,21 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
       for (int i = 0; i < (HALF ? 1 : v_stages); ++i) mbar_wait(bar(HALF ? ct.rv_full : ct.v_full[i]), i < vst ? vph ^ 1u : vph, late);
     }
     __syncwarp();
+   } else if (warp == 2) {
+    // ===================== the row tile that goes on in the next CTAs =====================
+    int4 last = make_int4(0, 0, 0, 0);
+    Walk w = ct.at[warp];
+    const long long x0 = ct.x0, x1 = ct.x1;
+    while (w.pl.n > 0 && w.at < x1) {
+      const Cost c = cost_of(a, w.pl);
+      if (c.cut(x0 - w.at) == 0 && c.cut(x1 - w.at) > 0 && c.cut(x1 - w.at) < c.units) {
+        int parts = 1;
+        while (c.cut((blockIdx.x + parts) * (x1 - x0) - w.at) < c.units) ++parts;      // x1 - x0 is a whole share: this CTA is not the last one
+        last = make_int4(w.pl.b, w.pl.first, w.h, parts);
+      }
+      advance(a, w, c, lane);
+    }
+    if (lane == 0) a.many.last[blockIdx.x] = last;
    }
   } else if (warp >= 12) {
     // ===================== 8-bit codes to f16 =====================
@@ -366,31 +532,36 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
         st128(base + piece_at(key, 2 * c + 1 - odd), odd ? first : second);
       };
       float up = 1.f;                                        // 2^e
-      int kst = 0, vst = 0;
-      uint32_t kph = 1, vph = 1;
-      for (int t = 0; t < n; ++t) {
-        Info& info = infos[t % INFOS];
-        const int valid = keys.end - keys.key0(t0 + t, 7);
-        mbar_wait_warp(bar(ct.rk_full), (uint32_t)t & 1u, dead);
+      int kst = 0, vst = 0, ref = 0;
+      uint32_t kph = 1, vph = 1, tile = 0, item = 0;
+      while (!dead && next(a, ct, warp, lane, x)) {
+       const Keys keys = a.keys(x.pl, ROWS);
+       for (int t = x.t0; t < x.t1; ++t, ++tile) {
+        Info& info = infos[tile % INFOS];
+        const int valid = keys.end - keys.key0(t, 7);
+        mbar_wait_warp(bar(ct.rk_full), tile & 1u, dead);
         if (dead) break;
         const float ks = codes.ks[me], vs = me < valid ? codes.vs[me] : 0.f;
-        if (t == 0) {
-          if (vs >= SMALLEST_SCALE && vs <= 1.f / SMALLEST_SCALE) atomicMax(&ct.ref, __float_as_uint(vs));
+        if (t == x.t0) {
+          if (vs >= SMALLEST_SCALE && vs <= 1.f / SMALLEST_SCALE) atomicMax(&ct.ref[ref], __float_as_uint(vs));
           mbar_arrive(bar(ct.ref_full));
-          mbar_wait_warp(bar(ct.ref_full), 0, dead);
+          mbar_wait_warp(bar(ct.ref_full), item++ & 1u, dead);
           if (dead) break;
-          up = value_lift(ct.ref);
+          up = value_lift(*reinterpret_cast<volatile uint32_t*>(&ct.ref[ref]));
+          if (me == 0) ct.ref[ref == 0 ? 2 : ref - 1] = 0u;  // the one before's, which all have read: for the one after the next
+          ref = ref == 2 ? 0 : ref + 1;
         }
         // what a value's codes are multiplied with: the part of the scale in 1 .. 2 in two f16 (22 bits), and its power of two; 0 hides whatever they are
         const float s = vs * up;
         const bool fits = s >= 1.52587890625e-05f && s <= 128.f, zero = vs >= 0.f && vs <= 1.17549435e-38f;      // 2^-126 (a row of zeros) or 0 (never written)
         const float one = __uint_as_float((__float_as_uint(s) & 0x007fffffu) | 0x3f800000u);
         const __half hi = __float2half_rn(one), lo = __float2half_rn(one - __half2float(hi)), power = __float2half_rn(__uint_as_float(__float_as_uint(s) & 0x7f800000u));
-        codes.by[t & 1][me] = fits ? make_uint2((uint32_t)__half_as_ushort(hi) | (uint32_t)__half_as_ushort(lo) << 16, __half_as_ushort(power) * 0x10001u) : make_uint2(0u, 0u);
+        codes.by[tile & 1][me] = fits ? make_uint2((uint32_t)__half_as_ushort(hi) | (uint32_t)__half_as_ushort(lo) << 16, __half_as_ushort(power) * 0x10001u) : make_uint2(0u, 0u);
         mbar_wait_warp(bar(ct.k_empty[kst]), kph, dead);
         if (dead) break;
         info.ks[me] = fits || zero ? ks : NAN;
-        mbar_arrive(bar(ct.info_full[t % INFOS]));
+        if (me == 0) info.up = up;
+        mbar_arrive(bar(ct.info_full[tile % INFOS]));
 #pragma unroll 2
         for (int i = 0; i < kc; ++i) {
           const int x = i * 128 + me, key = x * k_by >> 16;
@@ -409,15 +580,15 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
         mbar_arrive(bar(ct.k_full[kst]));
         mbar_arrive(bar(ct.rk_empty));
         if (++kst == k_stages) { kst = 0; kph ^= 1u; }
-        mbar_wait_warp(bar(ct.rv_full), (uint32_t)t & 1u, dead);
-        mbar_wait_warp(bar(ct.info_full[t % INFOS]), (uint32_t)(t / INFOS) & 1u, dead);      // all keys' factors
+        mbar_wait_warp(bar(ct.rv_full), tile & 1u, dead);
+        mbar_wait_warp(bar(ct.info_full[tile % INFOS]), tile / INFOS & 1u, dead);      // all keys' factors
         mbar_wait_warp(bar(ct.v_empty[vst]), vph, dead);
         if (dead) break;
 #pragma unroll 2
         for (int i = 0; i < vc; ++i) {
           const int x = i * 128 + me, key = x * v_by >> 16;
           const uint4 w = ld128(raw_v + 16 * x);
-          const uint2 by = codes.by[t & 1][key];
+          const uint2 by = codes.by[tile & 1][key];
           const uint32_t u[4] = {w.x, w.y, w.z, w.w}, h2 = __byte_perm(by.x, 0u, 0x1010), l2 = __byte_perm(by.x, 0u, 0x3232);
           uint32_t y[8];
 #pragma unroll
@@ -432,65 +603,79 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
         mbar_arrive(bar(ct.v_full[vst]));
         mbar_arrive(bar(ct.rv_empty));
         if (++vst == v_stages) { vst = 0; vph ^= 1u; }
+       }
       }
     }
   } else {
     if constexpr (HALF) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     // ===================== queries, softmax, outputs =====================
-    const int g = (warp - 4) >> 2, r = (warp & 3) * 32 + lane, at = pl.first + TILE * g + r;
-    const bool live = TILE * g + r < rows;
-    const int token = live ? at / G : 0, head = h * G + (live ? at % G : 0), row = pl.start + token, pos = live ? pl.length - pl.n + token : -1;
+    const int g = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), S = lanes + 128 * g, O = lanes + 256 + 128 * g;
+    uint32_t tile = 0, mine = 0, item = 0, own_items = 0;    // tiles of keys, those of this half; row tiles with keys, those of this half
+    while (next(a, ct, warp, lane, x)) {
+    const Place pl = x.pl;
+    const int n = x.n, t0 = x.t0, rows = min(ROWS, pl.n * G - pl.first), groups = pl_groups(pl, G), at = pl.first + TILE * g + r;
+    const bool part = !x.whole, live = TILE * g + r < rows;
+    const int token = live ? at / G : 0, head = x.h * G + (live ? at % G : 0), row = pl.start + token, pos = live ? pl.length - pl.n + token : -1;
+    const Keys keys = a.keys(pl, ROWS);
     float cr = a.scale_log2;
-    {
+    if (n > 0) {
+     if (g < groups) {
       // The warp's 32 rows, neighbouring lanes along a row: with a row per lane the load unit was busy with 32 lines for every instruction, 5400 cycles.  A
       // small loop, as code that runs once is fetched at some 12 cycles an instruction; a row's lane knows where it is
       const int pieces = a.K / 8, by = 65536 / pieces + 1;   // x / pieces = x by >> 16 for x < 32 pieces, pieces <= 24
-      const uint32_t mine = sq + g * ka * TC_ATOM;
+      const uint32_t own = sq + g * ka * TC_ATOM;
       const unsigned long long from = reinterpret_cast<unsigned long long>(reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)row * a.ldq + (size_t)head * a.hsq);
 #pragma unroll 2
       for (int x = lane; x < 32 * pieces; x += 32) {
         const int k = x * by >> 16, c = x - k * pieces;
         const unsigned long long src = __shfl_sync(0xffffffffu, from, k);
-        atc::cp16(mine + piece_at((warp & 3) * 32 + k, c), reinterpret_cast<const void*>(src + 16 * c), TILE * g + (warp & 3) * 32 + k < rows);
+        atc::cp16(own + piece_at((warp & 3) * 32 + k, c), reinterpret_cast<const void*>(src + 16 * c), TILE * g + (warp & 3) * 32 + k < rows);
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
       if (HALF) {                                            // then a lane has a row: its largest entry, and the row as f16
         __syncwarp();
         uint32_t top2 = 0u;                                  // of two entries' absolute values, as bits: as large as their values are
         for (int c = 0; c < pieces; ++c) {
-          const uint4 w = ld128(mine + piece_at(r, c));
+          const uint4 w = ld128(own + piece_at(r, c));
           top2 = __vmaxu2(__vmaxu2(__vmaxu2(top2, w.x & 0x7fff7fffu), __vmaxu2(w.y & 0x7fff7fffu, w.z & 0x7fff7fffu)), w.w & 0x7fff7fffu);
         }
         float up;
         lift_of(fmaxf(__uint_as_float(top2 << 16), __uint_as_float(top2 & 0xffff0000u)), a.scale_log2, up, cr);
         for (int c = 0; c < pieces; ++c) {
-          const uint4 w = ld128(mine + piece_at(r, c));
+          const uint4 w = ld128(own + piece_at(r, c));
           uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const __half2 f = __floats2half2_rn(__uint_as_float(u[e] << 16) * up, __uint_as_float(u[e] & 0xffff0000u) * up);
             u[e] = *reinterpret_cast<const uint32_t*>(&f);
           }
-          st128(mine + piece_at(r, c), make_uint4(u[0], u[1], u[2], u[3]));
+          st128(own + piece_at(r, c), make_uint4(u[0], u[1], u[2], u[3]));
         }
       }
       fence_proxy_async();
-      mbar_arrive(bar(ct.q_full));
+     }
+     mbar_arrive(bar(ct.q_full));
     }
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f, down = 1.f;
     bool odd = false;
     // positions of this group's rows: where all of them see a tile no mask is needed
     const int p_min = pl.length - pl.n + (pl.first + TILE * g) / G, p_max = pl.length - pl.n + (pl.first + min(TILE * (g + 1), rows) - 1) / G;
     if (g < groups) {
+      const bool idle = !__any_sync(0xffffffffu, live);
       for (int t = 0; t < n; ++t) {
         const int key0 = keys.key0(t0 + t, 7);
-        mbar_wait(bar(ct.info_full[t % INFOS]), (uint32_t)(t / INFOS) & 1u, dead);
-        mbar_wait_warp(bar(ct.s_full[g]), (uint32_t)t & 1u, dead);
+        mbar_wait(bar(ct.info_full[(tile + t) % INFOS]), (tile + t) / INFOS & 1u, dead);
+        mbar_wait_warp(bar(ct.s_full[g]), (mine + t) & 1u, dead);
         if (dead) break;
+        if (idle) {                                          // no row: whatever the weights are
+          if (lane < 2) mbar_arrive(bar(ct.p_half[g][lane]));
+          continue;
+        }
         fence_after();
-        const Info& info = infos[t % INFOS];
-        const uint32_t there = HALF ? info.there : there_of[t % INFOS];
+        const Info& info = infos[(tile + t) % INFOS];
+        const uint32_t there = HALF ? info.there : there_of[(tile + t) % INFOS];
+        if (HALF && t == n - 1) down = 1.f / info.up;
         const bool whole = there == 0xffu && key0 + KEYS - 1 <= p_min && (a.window == 0 || key0 > p_max - a.window || key0 + KEYS <= a.first);
         // keys that the row sees, as bits of 32
         auto seen = [&](int c) {
@@ -601,14 +786,12 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
         }
         l += sum[0] + sum[1];
       }
-      if (n > 0) mbar_wait_warp(bar(ct.o_done[g]), 0, dead);
+      if (n > 0) mbar_wait_warp(bar(ct.o_done[g]), own_items & 1u, dead);
       fence_after();
       if (dead || odd) l = NAN;
-      const float down = HALF && n > 0 ? 1.f / value_lift(ct.ref) : 1.f, inv = splits > 1 ? down : l == 0.f ? 0.f : down / l;
+      const float inv = part ? down : l == 0.f ? 0.f : down / l;
       bool fine = true;
-      const bool part = splits > 1;
-      const int place = live ? row * a.heads + head : -1;    // of the row's outputs
-      const long long to = ((long long)split * a.many.count + (long long)row * a.heads + head);
+      const int slot = 2 * (int)blockIdx.x + (t0 == 0 ? 1 : 0), place = !live ? -1 : part ? slot * ROWS + TILE * g + r : row * a.heads + head;      // of the row's outputs
       // Outputs through the warp's rows of the queries (every score of this row tile is done), 128 bytes of each row at a time; then eight lanes along a row (a
       // row per lane took 9500 cycles)
       const int per = part ? 32 : 64;                        // columns
@@ -646,14 +829,14 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
         for (int k = lane >> 3; k < 32; k += 4) {
           const int there = __shfl_sync(0xffffffffu, place, k);
           if (there >= 0 && column < a.V) {
-            const uint4 w = ld128(sq + g * ka * TC_ATOM + piece_at((warp & 3) * 32 + k, c));
-            if (part) *reinterpret_cast<uint4*>(a.many.o + ((size_t)split * a.many.count + there) * a.V + column) = w;
-            else *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)there * a.V + column) = w;
+            const uint4 y = ld128(sq + g * ka * TC_ATOM + piece_at((warp & 3) * 32 + k, c));
+            if (part) *reinterpret_cast<uint4*>(a.many.o + (size_t)there * a.V + column) = y;
+            else *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)there * a.V + column) = y;
           }
         }
         __syncwarp();
       }
-      if (live && a.many.splits > 1) *reinterpret_cast<float2*>(a.many.ml + 2 * to) = part ? make_float2(m, l) : make_float2(INFINITY, 0.f);      // (whole: nothing to join)
+      if (part) *reinterpret_cast<float2*>(a.many.ml + 2 * (slot * ROWS + TILE * g + r)) = make_float2(m, l);
       if (!part) {
         __syncwarp();
         for (uint32_t left = __ballot_sync(0xffffffffu, live && !(fine && fabsf(l) < INFINITY)); left; left &= left - 1) {
@@ -662,11 +845,81 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
         }
       }
     }
+    if (n > 0) {
+      // both halves keep to the same row tile: its products are over before the next one's queries are said to be there
+      if (g > 0) mbar_wait_warp(bar(ct.o_done[0]), item & 1u, dead);
+      ++item;
+      tile += n;
+      if (g < groups) {
+        mine += n;
+        ++own_items;
+      }
+    }
+    }
   }
   fence_before();
   __syncthreads();
   if (warp == 0) tmem_dealloc(tmem, 512);
 }
+
+// The row tiles that go on from CTA blockIdx.x to others; a warp has four rows, a lane four columns of each
+__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ Attn a) {
+  const int lane = threadIdx.x & 31, G = a.heads / a.kv_heads, r0 = blockIdx.y * 32 + threadIdx.x / 32 * 4;
+  pdl_wait();                                                // launched while the parts are computed
+  const int4 last = a.many.last[blockIdx.x];
+  if (last.w < 2) return;
+  int start, n, length;
+  sequence(a.s, last.x, start, n, length);
+  const int rows = min(ROWS, n * G - last.y);
+  if (r0 >= rows) return;
+  float M[4], L[4];
+  float4 x[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    M[k] = -INFINITY;
+    L[k] = 0.f;
+    x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  for (int i = 0; i < last.w; ++i) {
+    const int at = (i == 0 ? 2 * (int)blockIdx.x + 1 : 2 * ((int)blockIdx.x + i)) * ROWS + r0;
+    float2 ml[4];
+    float4 z[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      ml[k] = make_float2(-INFINITY, 0.f);
+      z[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r0 + k < rows) {
+        ml[k] = *reinterpret_cast<const float2*>(a.many.ml + 2 * (at + k));
+        if (4 * lane < a.V) z[k] = *reinterpret_cast<const float4*>(a.many.o + (size_t)(at + k) * a.V + 4 * lane);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (ml[k].x == -INFINITY && ml[k].y == 0.f) continue;  // saw nothing
+      const float now = fmaxf(M[k], ml[k].x), f = M[k] == now ? 1.f : exp2_f(M[k] - now), w = ml[k].x == now ? 1.f : exp2_f(ml[k].x - now);
+      M[k] = now;
+      L[k] = L[k] * f + w * ml[k].y;
+      x[k] = make_float4(x[k].x * f + w * z[k].x, x[k].y * f + w * z[k].y, x[k].z * f + w * z[k].z, x[k].w * f + w * z[k].w);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (r0 + k >= rows) break;
+    const int at = last.y + r0 + k, row = start + at / G, head = last.z * G + at % G;
+    const float inv = L[k] == 0.f ? 0.f : 1.f / L[k], y[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+    if (4 * lane < a.V) a.store(((size_t)row * a.heads + head) * a.V + 4 * lane, y, inv);
+    if (!__all_sync(0xffffffffu, finite4(y, inv) && fabsf(L[k]) < INFINITY)) {
+      __syncwarp();
+      mend_row(a, last.x, length - n + at / G, row, head, lane);
+    }
+  }
+}
+
+int many_ctas(long long row_tiles, long long keys, int sms) {
+  const long long cost = row_tiles * (EXTRA + 4 * ((keys + KEYS - 1) / KEYS + 2));
+  return (int)std::max<long long>(1, std::min<long long>(sms, cost / SMALLEST_SHARE));
+}
+long long many_floats(int ctas, int V) { return 4ll * ctas + 2ll * ctas * ROWS * (2 + V); }
 
 bool many_takes(int K, int V, int store) {
   if (K > MOST_K || V > MOST_V) return false;
@@ -709,8 +962,17 @@ template <int STORE> static int go(const Attn& a, int ctas, cudaStream_t stream)
   B2L_LAUNCH_CHECK("paged_many_kernel");
   return 0;
 }
-int many_launch(const Attn& a, int ctas, cudaStream_t stream) {
-  return a.store_kind == ACT ? go<ACT>(a, ctas, stream) : a.store_kind == E4M3 ? go<E4M3>(a, ctas, stream) : go<INT8>(a, ctas, stream);
+int many_launch(Attn& a, int ctas, float* work, cudaStream_t stream) {
+  a.many.ctas = ctas;
+  a.many.last = reinterpret_cast<int4*>(work);
+  a.many.ml = work + 4 * ctas;
+  a.many.o = a.many.ml + 4ll * ctas * ROWS;
+  const int rc = a.store_kind == ACT ? go<ACT>(a, ctas, stream) : a.store_kind == E4M3 ? go<E4M3>(a, ctas, stream) : go<INT8>(a, ctas, stream);
+  if (rc || ctas == 1) return rc;
+  LaunchCfg launch(dim3((unsigned)ctas, ROWS / 32), dim3(256), 0, stream, true);
+  B2L_CUDA(cudaLaunchKernelEx(&launch.cfg, paged_join_kernel, a));
+  B2L_LAUNCH_CHECK("paged_join_kernel");
+  return 0;
 }
 
 }  // namespace paged

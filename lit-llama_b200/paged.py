@@ -32,11 +32,10 @@ class PagedStep:
     lies in page table[b, j // page].  An entry of the table outside the pool (-1) is a page that is not there: its keys are not seen.
 
     The tensors (int32, on the device) may be overwritten between replays of a graph that was recorded with them.  `rows` is the number of tokens;
-    max_new, min_new and max_length are what the host knows of the sequences' new tokens and lengths: they pick between equivalent forms (every form is right
-    for every content of the tensors), so they should be about right."""
+    max_new and max_length are what the host knows of the sequences' most new tokens and lengths: they pick between equivalent forms (every form is right for
+    every content of the tensors), so they should be about right."""
 
-    def __init__(self, starts: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, *, rows: int, max_new: int = 0, min_new: int = 0,
-                 max_length: int = 0) -> None:
+    def __init__(self, starts: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, *, rows: int, max_new: int = 0, max_length: int = 0) -> None:
         for name, t, dims in (("starts", starts, 1), ("lengths", lengths, 1), ("table", table, 2)):
             if t.dtype != torch.int32 or t.dim() != dims or t.stride(-1) != 1:
                 raise ValueError(f"paged step: {name} must be int32 with {dims} dimension(s), its entries consecutive")
@@ -49,8 +48,6 @@ class PagedStep:
         self._tensors, self.rows, self.seqs = (starts, lengths, table), int(rows), lengths.numel()
         self.device = lengths.device
         self.max_new, self.max_length = max(int(max_new), 0), max(int(max_length), 0)
-        # all have the same number where that is the most there can be
-        self.min_new = self.max_new if self.seqs and self.max_new * self.seqs == self.rows else max(int(min_new), 0)
         self._at = (S.ptr(starts), S.ptr(lengths), S.ptr(table), table.stride(0), table.shape[1]) if lengths.is_cuda else None
         self._plans: Dict[tuple, tuple] = {}                                # of attend: what does not change from layer to layer
 
@@ -74,9 +71,8 @@ class PagedStep:
             flat += list(pages) + [-1] * (width - len(pages))
         n = len(lengths)
         both = torch.tensor(starts + lengths + flat, dtype=torch.int32).to(device)
-        news = [new for new, _, _ in sequences]
-        return cls(both[:n + 1], both[n + 1:2 * n + 1], both[2 * n + 1:].view(n, width), rows=rows, max_new=max(news, default=0),
-                   min_new=min((x for x in news if x), default=0), max_length=max(lengths, default=0))
+        return cls(both[:n + 1], both[n + 1:2 * n + 1], both[2 * n + 1:].view(n, width), rows=rows,
+                   max_new=max((new for new, _, _ in sequences), default=0), max_length=max(lengths, default=0))
 
     def refill(self, other: "PagedStep") -> None:
         """The other step's sequences in this one's tensors (of the same number of sequences and rows, and at least its width), for a graph that was
@@ -282,7 +278,7 @@ class PagedCache:
         if window < 0 or first < 0:
             raise ValueError("paged cache: a negative window or number of first tokens")
         sizes = (heads, self.kv_heads, self.dim, self.vdim, window, first)
-        hints = (step.max_new, step.min_new, step.max_length) + self._codes
+        hints = (step.max_new, step.max_length) + self._codes
         floats = S.lib().b2l_seq_paged_attention_work(rows, step.seqs, step.table.shape[1], self.page, *sizes, *hints)
         plan = (floats, (rows, step.seqs, self.n_pages, self.page) + sizes + (float(self.dim ** -0.5 if scale is None else scale),) + hints)
         step._plans[(rows, heads, scale, window, first, self._sizes)] = plan

@@ -287,12 +287,12 @@ def test_queries_of_any_stride_and_rows_behind_the_last_sequence(dtype, store):
 
 @pytest.mark.parametrize("dtype,store", TYPES, ids=IDS)
 def test_what_the_host_says_of_a_step_changes_no_result(dtype, store):
-    """Wrong numbers for the most and fewest new tokens and the longest sequence: other forms, the same sequences."""
+    """Wrong numbers for the most new tokens and the longest sequence: other forms, the same sequences."""
     from lit_llama_b200 import PagedStep
 
     cache, step, seqs = make(dtype, store, 2, 64, 64, 32, [(1, 700), (130, 400), (3, 3), (40, 900)])
     q = torch.randn(step.rows, 8, 64, generator=gen(3)).to(dtype)
-    for hints in (dict(), dict(max_new=1, min_new=1, max_length=16), dict(max_new=100000, min_new=1000, max_length=10 ** 6), dict(max_new=1, max_length=900), dict(min_new=130)):
+    for hints in (dict(), dict(max_new=1, max_length=16), dict(max_new=100000, max_length=10 ** 6), dict(max_new=1, max_length=900), dict(max_new=130)):
         s = PagedStep(step.starts, step.lengths, step.table, rows=step.rows, **hints)
         check(cache.attend(q.to(DEV), s), q, cache, seqs, 0.125)
 

@@ -21,7 +21,7 @@ def test_pages_are_booked_as_sequences_grow_and_given_back():
     p = pool()
     s = p.step([("a", 17), ("b", 1)])
     assert s.rows == 18 and s.starts.tolist() == [0, 17, 18] and s.lengths.tolist() == [17, 1] and s.table.tolist() == [[0, 1], [2, -1]]
-    assert (s.max_new, s.min_new, s.max_length) == (17, 1, 17)
+    assert (s.max_new, s.max_length) == (17, 17)
     s = p.step([("b", 15), ("a", 1)])
     assert s.lengths.tolist() == [16, 18] and s.table.tolist() == [[2, -1], [0, 1]] and p.position("a") == 18 and p.free_pages() == 5
     p.step([("b", 1)])
@@ -162,7 +162,7 @@ def call(name, **kw):
     if name == "attention":
         return lib.b2l_seq_paged_attention(a["x"], a["ld"], a["hs"], a["k"], a["v"], a["ks"], a["vs"], a["starts"], a["lengths"], a["table"], a["ldt"], a["width"], a["y"], a["work"],
                                            a["floats"], a["rows"], a["seqs"], a["pages"], a["page"], a["heads"], a["kv_heads"], a["K"], a["V"], a["window"], a["first"], a["scale"],
-                                           0, 0, 0, a["store"], a["act"], None)
+                                           0, 0, a["store"], a["act"], None)
     f = lib.b2l_seq_paged_write if name == "write" else lib.b2l_seq_paged_read
     return f(a["x"], a["ld"], a["hs"], a["y"], a["ld"], a["hs"], a["k"], a["v"], a["ks"], a["vs"], a["starts"], a["lengths"], a["table"], a["ldt"], a["width"], a["rows"], a["seqs"],
              a["pages"], a["page"], a["kv_heads"], a["K"], a["V"], a["store"], a["act"], None)
@@ -178,7 +178,7 @@ def test_the_c_entries_refuse_before_they_launch(name):
         bad += [dict(heads=3), dict(heads=0), dict(window=-1), dict(first=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")), dict(scale=float("nan")), dict(y=72),
                 dict(rows=1, seqs=1, width=1 << 26, ldt=1 << 26)]
         big = dict(rows=1, seqs=1, width=4096, ldt=4096)                       # long enough to be split, without the space
-        assert S.lib().b2l_seq_paged_attention_work(1, 1, 4096, 16, 4, 2, 32, 32, 0, 0, 0, 0, 0, 0, 0) > 0
+        assert S.lib().b2l_seq_paged_attention_work(1, 1, 4096, 16, 4, 2, 32, 32, 0, 0, 0, 0, 0, 0) > 0
         bad += [big, dict(big, work=64, floats=10), dict(work=72)]
     for kw in bad:
         rc = call(name, **dict(dict(rows=3), **kw))
