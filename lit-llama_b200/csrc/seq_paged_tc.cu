@@ -13,13 +13,14 @@
 //                 begins with the half that is there.  A row's reference moves only when it is exceeded by more than 8 (weights reach 2^8; nothing is
 //                 rounded by that), so the output in tensor memory is seldom scaled.  bf16: of four powers of two the special function unit computes
 //                 three and a polynomial the fourth: 2048 tokens over 16384 of 32 / 8 heads take 454 us so, 484 without, 461 with three of eight, 475 with half
-//   warps 12..15  8-bit pool: codes as f16 into the same rows: keys exactly, values times their scale
+//   warps 12..19  8-bit pool: codes times their scale as f16 into the same rows, keys (12..15) and values
 //
 // Weights are rounded to one bf16 (by half a step, 2^-8; with 8-bit pools one f16, 2^-11): the first rounding below f32 in the sums, and the price of one
 // product instead of two; outputs in bf16 are off by as much themselves.
-// 8-bit pools: queries as f16 times a power of two per row, the scale of a key goes into its score.  The scale of a value s goes into its codes, code times
-// s 2^e rounded to f16 (2^-11), e such that the largest s of the CTA's first tile comes to 1 .. 2, and the outputs times 2^-e.  A row that sees a scale above
-// 2^7 or below 2^-16 of that, or a scale that is not finite, is computed again.
+// 8-bit pools: queries as f16 times a power of two per row.  The scale s of a key or value goes into its codes: code times s 2^e rounded to f16 (2^-11), e such
+// that the largest s of the row tile's first keys comes to 1 .. 2; the scores and the outputs times 2^-e.  (A key's scale times its scores instead, without that
+// rounding: every thread needs all of them, 128 KB of reads from shared memory for a tile; 2048 tokens over 16384 keys took 750 us.)  A row that sees a scale
+// above 2^7 or below 2^-12 of that, or one that is not finite, is computed again.
 //
 // Tensor memory: scores and weights of the row tiles at columns 0 and 128, outputs at 256 and 384.  Shared memory: the queries of both, two stages of keys
 // and values where they fit (8-bit: of values, and a tile of codes).  One CTA per SM.
@@ -42,10 +43,10 @@ constexpr int KEYS = 128, TILE = 128, ROWS = 2 * TILE, MOST_K = 192, MOST_V = 12
 constexpr int TC_ATOM = 128 * 128;                           // bytes of 64 columns of 128 rows
 constexpr int INFOS = 4;
 
-struct alignas(16) Info {                                    // of a tile of keys, for the softmax (read by 16 bytes)
-  float ks[KEYS];                                            // scale of the key, NaN where the row is to be computed again (8-bit pools)
+struct alignas(16) Info {                                    // of a tile of keys
+  uint2 k_by[KEYS], v_by[KEYS];                              // 8-bit pools: what a key's and a value's codes are multiplied with
   uint32_t there;                                            // 16 keys each: whether their page is there
-  float up;                                                  // 8-bit pools: what the values' scales are multiplied with
+  float k_up, v_up;                                          // 8-bit pools: powers of two that the scales were multiplied with
 };
 // A row tile: 256 packed rows of a head, the tiles of its sequence's rows one after the other, then the next head's, then the next sequence's
 struct Walk {
@@ -55,26 +56,22 @@ struct Walk {
 };
 struct Control {
   uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_half[2][2], o_done[2], info_full[INFOS], tail, gave_up;
-  uint64_t ref_full, rk_full, rk_empty, rv_full, rv_empty;   // 8-bit pools: the first tile's largest scale, codes of keys and values
-  uint32_t tmem, ref[3];                                     // ref: largest scale of the first tile's values, as bits, of a row tile, the next and the one before
+  uint64_t ref_full, rk_full, rk_empty, rv_full, rv_empty;   // 8-bit pools: the first tile's largest scales, codes of keys and values
+  uint32_t tmem, k_ref[3], v_ref[3];                         // largest scales of the first tile's keys and values, as bits, of a row tile, the next and the one before
   long long x0, x1;                                          // the CTA's part
-  Walk at[16];                                               // each warp's row tile
-  long long costs[16];                                       // of the sequences that a warp counts
+  Walk at[20];                                               // each warp's row tile
 };
-struct Codes {                                               // 8-bit pools: what lies beside a tile's codes
-  float ks[KEYS], vs[KEYS];                                  // scales
-  uint2 by[2][KEYS];                                         // what a value's codes are multiplied with (two tiles: one may still be read)
-};
+struct Scales { float k[KEYS], v[KEYS]; };                   // 8-bit pools: what lies beside a tile's codes
 constexpr size_t CONTROL_BYTES = 1024;
-template <int STORE> constexpr size_t INFO_BYTES = STORE == ACT ? 1024 : (INFOS * sizeof(Info) + sizeof(Codes) + 1023) / 1024 * 1024;
+template <int STORE> constexpr size_t INFO_BYTES = STORE == ACT ? 1024 : (INFOS * sizeof(Info) + sizeof(Scales) + 1023) / 1024 * 1024;
 static_assert(sizeof(Control) <= CONTROL_BYTES && sizeof(Info) % 16 == 0);
+template <int STORE> constexpr int THREADS = STORE == ACT ? 384 : 640;
 
 struct Layout { int ks, vs; size_t smem; };                  // stages of keys and values; none: the sizes do not fit
 template <int STORE> static Layout layout(int K, int V) {
   const size_t base = CONTROL_BYTES + INFO_BYTES<STORE> + (STORE == ACT ? 0 : KEYS * (K + V)), ka = atoms_of(K, 2), va = atoms_of(V, 2), q = 2 * ka * TC_ATOM, room = 227 * 1024;
   Layout l{0, 0, 0};
-  // codes: keys become f16 while the tile before is in the softmax, values in a hurry
-  const std::pair<int, int> stages[4] = {{2, 2}, STORE == ACT ? std::pair<int, int>{2, 1} : std::pair<int, int>{1, 2}, {1, 1}, {1, 1}};
+  const std::pair<int, int> stages[3] = {{2, 2}, {2, 1}, {1, 1}};
   for (const auto& [ks, vs] : stages)
     if (base + q + (ks * ka + vs * va) * TC_ATOM <= room) {
       l = {ks, vs, base + q + (ks * ka + vs * va) * TC_ATOM};
@@ -163,10 +160,10 @@ __device__ __forceinline__ void wait_lead(uint32_t a, uint32_t parity, uint32_t 
 __device__ __forceinline__ void commit_by(uint32_t lead, uint32_t mbar) {
   asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(mbar), "r"(lead) : "memory");
 }
-// two codes (f16) times a factor of 1 .. 2 in two parts, rounded once, times a power of two
-__device__ __forceinline__ uint32_t scaled(uint32_t u, uint32_t hi, uint32_t lo, uint32_t power) {
+// two codes (f16) times a factor in two parts, rounded once
+__device__ __forceinline__ uint32_t scaled(uint32_t u, uint32_t hi, uint32_t lo) {
   uint32_t y;
-  asm("{\n\t.reg .b32 x;\n\tmul.rn.f16x2 x, %1, %3;\n\tfma.rn.f16x2 x, %1, %2, x;\n\tmul.rn.f16x2 %0, x, %4;\n\t}" : "=r"(y) : "r"(u), "r"(hi), "r"(lo), "r"(power));
+  asm("{\n\t.reg .b32 x;\n\tmul.rn.f16x2 x, %1, %3;\n\tfma.rn.f16x2 %0, %1, %2, x;\n\t}" : "=r"(y) : "r"(u), "r"(hi), "r"(lo));
   return y;
 }
 __device__ __forceinline__ void bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t mbar) {      // multiples of 16 bytes
@@ -178,6 +175,42 @@ __device__ __forceinline__ float value_lift(uint32_t bits) { return bits ? __uin
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 // place of the 16-byte piece c of row r in tiles of 128 rows
 __device__ __forceinline__ uint32_t piece_at(int r, int c) { return (uint32_t)((c >> 3) * TC_ATOM + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
+
+// This thread's 16-byte pieces of a tile's codes (rows of D bytes) as f16 into its rows, code times its row's factor (in two parts) rounded once: every `threads`-th
+// piece.  HIDE: a factor of 0 hides whatever the codes are
+template <int STORE, bool HIDE> __device__ __forceinline__ void codes_to_f16(uint32_t raw, int D, const uint2* factors, uint32_t base, int me, int threads) {
+  const int pieces = D / 16;
+  auto one = [&](uint32_t from, uint2 f, uint32_t first, uint32_t second, bool odd) {
+    uint4 w = ld128(from);
+    if (HIDE && f.x == 0u) w = make_uint4(0u, 0u, 0u, 0u);
+    const uint32_t u[4] = {odd ? w.z : w.x, odd ? w.w : w.y, odd ? w.x : w.z, odd ? w.y : w.w};      // neighbours store their halves in turn: they meet different banks
+    uint32_t y[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint2 p = codes4<STORE, 0, 1, 2, 3>(u[e]);
+      y[2 * e] = scaled(p.x, f.x, f.y);
+      y[2 * e + 1] = scaled(p.y, f.x, f.y);
+    }
+    st128(first, make_uint4(y[0], y[1], y[2], y[3]));
+    st128(second, make_uint4(y[4], y[5], y[6], y[7]));
+  };
+  if ((pieces & (pieces - 1)) == 0) {                        // a thread's pieces lie at the same place of every 128th, 64th .. key
+    const int c = me & (pieces - 1), key = me / pieces, step = threads / pieces;
+    const bool odd = (c >> 2) & 1;
+    uint32_t from = raw + 16 * me, first = base + piece_at(key, 2 * c + odd), second = base + piece_at(key, 2 * c + 1 - odd);
+#pragma unroll 2
+    for (int k = key; k < KEYS; k += step, from += 16 * threads, first += 128 * step, second += 128 * step) one(from, factors[k], first, second, odd);
+  } else {
+    const int by = 65536 / pieces + 1;                       // x / pieces = x by >> 16 for x < 128 pieces, pieces <= 12
+#pragma unroll 1
+    for (int x = me; x < KEYS * pieces; x += threads) {
+      const int key = x * by >> 16, c = x - key * pieces;
+      const bool odd = (c >> 2) & 1;
+      one(raw + 16 * x, factors[key], base + piece_at(key, 2 * c + odd), base + piece_at(key, 2 * c + 1 - odd), odd);
+    }
+  }
+  fence_proxy_async();
+}
 
 // ---- which CTA computes what: an equal part of the cost of everything, in the order of `Walk`, so a CTA has whole row tiles and begins and ends inside one.
 // Every CTA counts the cost itself.  A tile of keys costs 4 (3 where the row tile has one half only), a row tile 16 beside.
@@ -267,7 +300,7 @@ __device__ __forceinline__ bool next(const Attn& a, Control& ct, int warp, int l
 __device__ __forceinline__ int pl_groups(const Place& pl, int G) { return pl.n * G - pl.first > TILE ? 2 : 1; }
 
 template <int STORE>
-__global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel(const __grid_constant__ Attn a, const __grid_constant__ CUtensorMap map_k,
+__global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __grid_constant__ Attn a, const __grid_constant__ CUtensorMap map_k,
                                                                                   const __grid_constant__ CUtensorMap map_v, int k_stages, int v_stages) {
   constexpr bool HALF = STORE != ACT;
   constexpr float LIFT = HALF ? 6.f : 0.f;                   // weights up to 2^14 in f16
@@ -284,11 +317,12 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
       mine += sequence_cost(a, pl, lane) * a.kv_heads;
       return false;
     });
-    if (lane == 0) ct.costs[warp] = mine;
+    long long* costs = reinterpret_cast<long long*>(smem + CONTROL_BYTES);      // where the tiles' notes come later
+    if (lane == 0) costs[warp] = mine;
     __syncthreads();
     for (int i = 0; i < warps; ++i) {
       if (i == warp) before = all;
-      all += ct.costs[i];
+      all += costs[i];
     }
     const long long share = max((all + gridDim.x - 1) / gridDim.x, (long long)SMALLEST_SHARE);
     const long long x0 = blockIdx.x * share;
@@ -331,7 +365,7 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
   const int ka = atoms_of(a.K, 2), va = atoms_of(a.V, 2);
   const uint32_t sq = smem_u32(smem) + CONTROL_BYTES + INFO_BYTES<STORE>, sk = sq + 2 * ka * TC_ATOM, sv = sk + k_stages * ka * TC_ATOM;
   const uint32_t raw_k = sv + v_stages * va * TC_ATOM, raw_v = raw_k + KEYS * a.K;      // 8-bit pools
-  Codes& codes = *reinterpret_cast<Codes*>(smem + CONTROL_BYTES + INFOS * sizeof(Info));
+  Scales& scales = *reinterpret_cast<Scales*>(smem + CONTROL_BYTES + INFOS * sizeof(Info));
   auto bar = [&](const uint64_t& b) { return smem_u32(&b); };
   uint32_t dead = (sq & 1023u) ? 1u : 0u;
   if (tid == 0) {
@@ -354,7 +388,7 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
     mbar_init(bar(ct.rv_full), 1);
     mbar_init(bar(ct.rk_empty), 128);
     mbar_init(bar(ct.rv_empty), 128);
-    for (int i = 0; i < 3; ++i) ct.ref[i] = 0u;
+    for (int i = 0; i < 3; ++i) ct.k_ref[i] = ct.v_ref[i] = 0u;
     mbar_init_fence();
   }
   if (warp == 0) tmem_alloc(smem_u32(&ct.tmem), 512);
@@ -364,8 +398,8 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
   const uint32_t tmem = ct.tmem;
   Item x;
   if (warp < 4) {
-   // 8-bit pool: a row's 128 scores in registers, which the softmax takes from the other warps (56 x 128 + 184 x 256 + 88 x 128 = 128 x 512)
-   if constexpr (HALF) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+   // 8-bit pool: 48 x 128 + 144 x 256 + 72 x 256 = 96 x 640 registers
+   if constexpr (HALF) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
    if (warp == 0) {
     // ===================== MMA issue =====================
     const uint32_t lead = elect_lane();
@@ -464,7 +498,7 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
         if (HALF) {
           const int at = r < gone ? r : 0;                   // of a page that is not there: any scales
           if (x == 0) tma_load_2d(raw_k + b * box * a.K, &map_k, 0, r, k_to);
-          else bulk(smem_u32((x == 1 ? codes.ks : codes.vs) + b * box), (x == 1 ? a.ks : a.vs) + at, 4 * box, k_to);
+          else bulk(smem_u32((x == 1 ? scales.k : scales.v) + b * box), (x == 1 ? a.ks : a.vs) + at, 4 * box, k_to);
         } else {
           tma_load_2d(sk + (kst * ka + x) * TC_ATOM + b * box * 128, &map_k, 64 * x, r, k_to);
         }
@@ -522,92 +556,72 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
   } else if (warp >= 12) {
     // ===================== 8-bit codes to f16 =====================
     if constexpr (HALF) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-      const int me = tid - 384, kc = a.K / 16, vc = a.V / 16;      // a thread has a key's scales, and every 128th of the tile's 16-byte pieces
-      const int k_by = 65536 / kc + 1, v_by = 65536 / vc + 1;      // x / pieces = x by >> 16 for x < 128 pieces, pieces <= 12
-      auto put = [&](uint32_t base, int key, int c, const uint32_t (&y)[8]) {
-        const int odd = (c >> 2) & 1;                        // neighbours meet different banks
-        const uint4 first = make_uint4(y[0], y[1], y[2], y[3]), second = make_uint4(y[4], y[5], y[6], y[7]);
-        st128(base + piece_at(key, 2 * c + odd), odd ? second : first);
-        st128(base + piece_at(key, 2 * c + 1 - odd), odd ? first : second);
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+      const bool keys_too = warp < 16;                       // warps 12 .. 15: the factors of keys and values, and the keys; 16 .. 19: the values
+      const int me = tid & 127;
+      int st = 0, ref = 0;
+      uint32_t ph = 1, tile = 0, item = 0;
+      float k_up = 1.f, v_up = 1.f;
+      // the factor in two f16, twice each: as precise as 22 bits, or steps of 2^-25 (2^-13 of the smallest); NaN where the scale is out of range; 0 for a row of
+      // zeros (2^-126) or one never written (0)
+      constexpr uint32_t NO = 0x7e007e00u;
+      auto factor = [](float scale, float up) {
+        const float s = scale * up;
+        if (scale >= 0.f && scale <= 1.17549435e-38f) return make_uint2(0u, 0u);
+        if (!(s >= 2.44140625e-4f && s <= 128.f)) return make_uint2(NO, NO);
+        const __half hi = __float2half_rn(s), lo = __float2half_rn(s - __half2float(hi));
+        return make_uint2(__half_as_ushort(hi) * 0x10001u, __half_as_ushort(lo) * 0x10001u);
       };
-      float up = 1.f;                                        // 2^e
-      int kst = 0, vst = 0, ref = 0;
-      uint32_t kph = 1, vph = 1, tile = 0, item = 0;
       while (!dead && next(a, ct, warp, lane, x)) {
        const Keys keys = a.keys(x.pl, ROWS);
        for (int t = x.t0; t < x.t1; ++t, ++tile) {
         Info& info = infos[tile % INFOS];
-        const int valid = keys.end - keys.key0(t, 7);
-        mbar_wait_warp(bar(ct.rk_full), tile & 1u, dead);
-        if (dead) break;
-        const float ks = codes.ks[me], vs = me < valid ? codes.vs[me] : 0.f;
-        if (t == x.t0) {
-          if (vs >= SMALLEST_SCALE && vs <= 1.f / SMALLEST_SCALE) atomicMax(&ct.ref[ref], __float_as_uint(vs));
-          mbar_arrive(bar(ct.ref_full));
-          mbar_wait_warp(bar(ct.ref_full), item++ & 1u, dead);
+        if (keys_too) {
+          mbar_wait_warp(bar(ct.rk_full), tile & 1u, dead);
           if (dead) break;
-          up = value_lift(*reinterpret_cast<volatile uint32_t*>(&ct.ref[ref]));
-          if (me == 0) ct.ref[ref == 0 ? 2 : ref - 1] = 0u;  // the one before's, which all have read: for the one after the next
-          ref = ref == 2 ? 0 : ref + 1;
-        }
-        // what a value's codes are multiplied with: the part of the scale in 1 .. 2 in two f16 (22 bits), and its power of two; 0 hides whatever they are
-        const float s = vs * up;
-        const bool fits = s >= 1.52587890625e-05f && s <= 128.f, zero = vs >= 0.f && vs <= 1.17549435e-38f;      // 2^-126 (a row of zeros) or 0 (never written)
-        const float one = __uint_as_float((__float_as_uint(s) & 0x007fffffu) | 0x3f800000u);
-        const __half hi = __float2half_rn(one), lo = __float2half_rn(one - __half2float(hi)), power = __float2half_rn(__uint_as_float(__float_as_uint(s) & 0x7f800000u));
-        codes.by[tile & 1][me] = fits ? make_uint2((uint32_t)__half_as_ushort(hi) | (uint32_t)__half_as_ushort(lo) << 16, __half_as_ushort(power) * 0x10001u) : make_uint2(0u, 0u);
-        mbar_wait_warp(bar(ct.k_empty[kst]), kph, dead);
-        if (dead) break;
-        info.ks[me] = fits || zero ? ks : NAN;
-        if (me == 0) info.up = up;
-        mbar_arrive(bar(ct.info_full[tile % INFOS]));
-#pragma unroll 2
-        for (int i = 0; i < kc; ++i) {
-          const int x = i * 128 + me, key = x * k_by >> 16;
-          const uint4 w = ld128(raw_k + 16 * x);
-          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-          uint32_t y[8];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint2 f = codes4<STORE, 0, 1, 2, 3>(u[e]);
-            y[2 * e] = f.x;
-            y[2 * e + 1] = f.y;
+          const float ks = scales.k[me], vs = scales.v[me];
+          const bool valid = me < keys.end - keys.key0(t, 7);      // behind the last key that is seen there may be anything
+          if (t == x.t0) {
+            if (valid && ks >= SMALLEST_SCALE && ks <= 1.f / SMALLEST_SCALE) atomicMax(&ct.k_ref[ref], __float_as_uint(ks));
+            if (valid && vs >= SMALLEST_SCALE && vs <= 1.f / SMALLEST_SCALE) atomicMax(&ct.v_ref[ref], __float_as_uint(vs));
+            mbar_arrive(bar(ct.ref_full));
+            mbar_wait_warp(bar(ct.ref_full), item++ & 1u, dead);
+            if (dead) break;
+            k_up = value_lift(*reinterpret_cast<volatile uint32_t*>(&ct.k_ref[ref]));
+            v_up = value_lift(*reinterpret_cast<volatile uint32_t*>(&ct.v_ref[ref]));
+            if (me == 0) ct.k_ref[ref == 0 ? 2 : ref - 1] = ct.v_ref[ref == 0 ? 2 : ref - 1] = 0u;      // the ones before, which all have read: for the ones after the next
+            ref = ref == 2 ? 0 : ref + 1;
           }
-          put(sk + kst * ka * TC_ATOM, key, x - key * kc, y);
+          uint2 k_by = factor(ks, k_up), v_by = valid ? factor(vs, v_up) : make_uint2(0u, 0u);
+          if (v_by.x == NO) {                                // a row that sees this key is computed again: its scores say so
+            k_by = v_by;
+            v_by = make_uint2(0u, 0u);
+          }
+          mbar_wait_warp(bar(ct.k_empty[st]), ph, dead);
+          if (dead) break;
+          info.k_by[me] = k_by;
+          info.v_by[me] = v_by;
+          if (me == 0) {
+            info.k_up = k_up;
+            info.v_up = v_up;
+          }
+          mbar_arrive(bar(ct.info_full[tile % INFOS]));
+        } else {
+          mbar_wait_warp(bar(ct.rv_full), tile & 1u, dead);
+          mbar_wait_warp(bar(ct.v_empty[st]), ph, dead);
         }
-        fence_proxy_async();
-        mbar_arrive(bar(ct.k_full[kst]));
-        mbar_arrive(bar(ct.rk_empty));
-        if (++kst == k_stages) { kst = 0; kph ^= 1u; }
-        mbar_wait_warp(bar(ct.rv_full), tile & 1u, dead);
         mbar_wait_warp(bar(ct.info_full[tile % INFOS]), tile / INFOS & 1u, dead);      // all keys' factors
-        mbar_wait_warp(bar(ct.v_empty[vst]), vph, dead);
         if (dead) break;
-#pragma unroll 2
-        for (int i = 0; i < vc; ++i) {
-          const int x = i * 128 + me, key = x * v_by >> 16;
-          const uint4 w = ld128(raw_v + 16 * x);
-          const uint2 by = codes.by[tile & 1][key];
-          const uint32_t u[4] = {w.x, w.y, w.z, w.w}, h2 = __byte_perm(by.x, 0u, 0x1010), l2 = __byte_perm(by.x, 0u, 0x3232);
-          uint32_t y[8];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint2 f = codes4<STORE, 0, 1, 2, 3>(u[e]);
-            y[2 * e] = by.y ? scaled(f.x, h2, l2, by.y) : 0u;
-            y[2 * e + 1] = by.y ? scaled(f.y, h2, l2, by.y) : 0u;
-          }
-          put(sv + vst * va * TC_ATOM, key, x - key * vc, y);
-        }
-        fence_proxy_async();
-        mbar_arrive(bar(ct.v_full[vst]));
-        mbar_arrive(bar(ct.rv_empty));
-        if (++vst == v_stages) { vst = 0; vph ^= 1u; }
+        if (keys_too) codes_to_f16<STORE, false>(raw_k, a.K, info.k_by, sk + st * ka * TC_ATOM, me, 128);
+        else codes_to_f16<STORE, true>(raw_v, a.V, info.v_by, sv + st * va * TC_ATOM, me, 128);
+        mbar_arrive(bar(keys_too ? ct.k_full[st] : ct.v_full[st]));
+        mbar_arrive(bar(keys_too ? ct.rk_empty : ct.rv_empty));
+        if (++st == (keys_too ? k_stages : v_stages)) { st = 0; ph ^= 1u; }
        }
       }
     }
   } else {
-    if constexpr (HALF) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    if constexpr (HALF) asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     // ===================== queries, softmax, outputs =====================
     const int g = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), S = lanes + 128 * g, O = lanes + 256 + 128 * g;
@@ -675,7 +689,10 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
         fence_after();
         const Info& info = infos[(tile + t) % INFOS];
         const uint32_t there = HALF ? info.there : there_of[(tile + t) % INFOS];
-        if (HALF && t == n - 1) down = 1.f / info.up;
+        if (HALF && t == 0) {
+          cr *= 1.f / info.k_up;
+          down = 1.f / info.v_up;
+        }
         const bool whole = there == 0xffu && key0 + KEYS - 1 <= p_min && (a.window == 0 || key0 > p_max - a.window || key0 + KEYS <= a.first);
         // keys that the row sees, as bits of 32
         auto seen = [&](int c) {
@@ -684,19 +701,8 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
           if (a.window) x &= ~low_bits(pos - a.window + 1 - j) | low_bits(a.first - j);
           return x & (((there >> 2 * c & 1u) ? 0xffffu : 0u) | ((there >> (2 * c + 1) & 1u) ? 0xffff0000u : 0u));
         };
-        // scores of keys 64 half .. + 63, by the keys' scales, hidden ones -inf
+        // scores of keys 64 half .. + 63: hidden ones -inf
         auto finish = [&](int half, uint32_t* u) {
-          if (HALF) {
-#pragma unroll
-            for (int i = 0; i < 64; i += 4) {
-              const float4 k4 = *reinterpret_cast<const float4*>(info.ks + 64 * half + i);
-              float x[4] = {__uint_as_float(u[i]), __uint_as_float(u[i + 1]), __uint_as_float(u[i + 2]), __uint_as_float(u[i + 3])};
-              mul2(x[0], x[1], k4.x, k4.y);
-              mul2(x[2], x[3], k4.z, k4.w);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) u[i + e] = __float_as_uint(x[e]);
-            }
-          }
           if (!whole) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -708,18 +714,12 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
         };
         // bf16: the second half's stay in registers from the maximum to the weights, the first is read twice.  All 128 in registers took 3% longer (and with
         // 8-bit codes 10% less, as there the instructions count)
-        uint32_t u[HALF ? KEYS : KEYS / 2];
+        uint32_t u[KEYS / 2];
         float x4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        if (HALF) {
-          tmem_ld64(S, u);
-          tmem_ld64(S + 64, u + (HALF ? 64 : 0));
-          tmem_wait_ld64(u);
-          tmem_wait_ld64(u + (HALF ? 64 : 0));
-        }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          uint32_t* x = u + (HALF ? 64 * half : 0);
-          if (!HALF) {
+          uint32_t* x = u;
+          {
             tmem_ld64(S + 64 * half, x);
             tmem_wait_ld64(x);
           }
@@ -749,8 +749,8 @@ __global__ void __launch_bounds__(STORE == ACT ? 384 : 512, 1) paged_many_kernel
         float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int half = 1; half >= 0; --half) {              // the second half first, over its own scores
-          uint32_t* z = u + (HALF ? 64 * half : 0);
-          if (!HALF && half == 0) {
+          uint32_t* z = u;
+          if (half == 0) {
             tmem_ld64(S, z);
             tmem_wait_ld64(z);
             finish(0, z);
@@ -958,7 +958,7 @@ template <int STORE> static int go(const Attn& a, int ctas, cudaStream_t stream)
   }
   static DynSmemCache cache;
   if (int rc = ensure_dyn_smem(paged_many_kernel<STORE>, l.smem, cache)) return rc;
-  paged_many_kernel<STORE><<<(unsigned)ctas, STORE == ACT ? 384 : 512, l.smem, stream>>>(a, mk, mv, l.ks, l.vs);
+  paged_many_kernel<STORE><<<(unsigned)ctas, THREADS<STORE>, l.smem, stream>>>(a, mk, mv, l.ks, l.vs);
   B2L_LAUNCH_CHECK("paged_many_kernel");
   return 0;
 }
