@@ -5,7 +5,7 @@
 // The query heads that read one key/value head are packed with the tokens: packed row i G + g is head g of the group at the sequence's new token i.
 // paged_few_kernel takes 8 or 16 packed rows against the keys of one head, 16 (8-bit: 32) at a time, as mma.m16n8k16 with the keys (and then the entries of a value) for
 // its 16 rows and the queries for its 8 columns: a token of a group of up to 8 heads fills the product that it needs, where queries as rows left three
-// quarters of the scores and their softmax unused (600 instructions for 16 keys of 128 8-bit entries, now 300).  A warp has every W-th such unit of its share
+// quarters of the scores and their softmax unused (537 instructions for 16 keys of 128 8-bit entries, now 440 with all beside).  A warp has every W-th such unit of its share
 // all to itself: its own ring of tiled copies (16 rows of one page by 128 bytes, swizzled), its own running maximum, sum and outputs in registers, no
 // barrier in the loop.  The warps' results are joined at the end, and those of several CTAs that share a row's keys by paged_merge_kernel.
 //
@@ -20,7 +20,10 @@
 // With 8-bit codes a lane has four consecutive entries of a key as its share of a k16 step (queries laid out alike), and values are transposed as pairs
 // of neighbouring entries, so 16-byte rows of ldmatrix do for both.  Weights turn from keys by rows into the second product's operand by movmatrix.
 //
-// What bounds it: one pass over the keys and values that the rows see, at HBM's rate, for the rows of a token; 16 rows of f32 are bound by their six products.
+// What bounds it: one pass over the keys and values that the rows see.  One token over 131072 keys of 4 heads of 128, bf16: 55.5 us, 4.8 TB/s.  Tokens of 48
+// sequences over up to 8192 keys of 8 heads, e4m3: 123 us, 4.3 TB/s, where the issue of instructions is busy for half of the cycles and their latency is the
+// other half (12 warps on an SM, as many as the copies in flight leave room for).  One token over 1031 keys: 12 us, two launches of a chain of loads each.
+// 16 rows of f32 are bound by their six products: 461 tokens over a window of 512, 8 / 2 heads of 128, 73 us.
 #include <algorithm>
 #include <cmath>
 

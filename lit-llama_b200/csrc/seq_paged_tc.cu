@@ -8,22 +8,28 @@
 //                 both softmaxes at once, then the products, 4300 cycles for a tile; units of 64 keys with two places for their scores took 4160, as an MMA
 //                 of N = 64 takes 75 cycles and one of N = 128 103: its rows of A come out of shared memory for half as many keys.)
 //   warp 1        tiled copies of pages: bf16, 64 columns each, into 128-byte swizzled rows (keys K-major, values MN-major); codes as they lie, with their
-//                 scales, for warps 12..15
+//                 scales, for warps 12..19
 //   warps 4..11   softmax of row tile 0 (4..7) and 1 (8..11): a row's scores into registers, its weights back over them in two halves, so the second product
 //                 begins with the half that is there.  A row's reference moves only when it is exceeded by more than 8 (weights reach 2^8; nothing is
 //                 rounded by that), so the output in tensor memory is seldom scaled.  bf16: of four powers of two the special function unit computes
-//                 three and a polynomial the fourth: 2048 tokens over 16384 of 32 / 8 heads take 454 us so, 484 without, 461 with three of eight, 475 with half
+//                 three and a polynomial the fourth: 2048 tokens over 16384 of 32 / 8 heads take 430 us so, 441 without, 439 with three of eight, 447 with half
 //   warps 12..19  8-bit pool: codes times their scale as f16 into the same rows, keys (12..15) and values
 //
 // Weights are rounded to one bf16 (by half a step, 2^-8; with 8-bit pools one f16, 2^-11): the first rounding below f32 in the sums, and the price of one
 // product instead of two; outputs in bf16 are off by as much themselves.
 // 8-bit pools: queries as f16 times a power of two per row.  The scale s of a key or value goes into its codes: code times s 2^e rounded to f16 (2^-11), e such
-// that the largest s of the row tile's first keys comes to 1 .. 2; the scores and the outputs times 2^-e.  (A key's scale times its scores instead, without that
+// that the largest s of the CTA's first 128 keys of a row tile comes to 1 .. 2; the scores and the outputs times 2^-e.  (A key's scale times its scores instead, without that
 // rounding: every thread needs all of them, 128 KB of reads from shared memory for a tile; 2048 tokens over 16384 keys took 750 us.)  A row that sees a scale
 // above 2^7 or below 2^-12 of that, or one that is not finite, is computed again.
 //
 // Tensor memory: scores and weights of the row tiles at columns 0 and 128, outputs at 256 and 384.  Shared memory: the queries of both, two stages of keys
-// and values where they fit (8-bit: of values, and a tile of codes).  One CTA per SM.
+// and values where they fit (8-bit: of keys, and a tile of codes).  One CTA per SM, which goes through row tiles: the next one's first keys are fetched while the
+// outputs of the last are stored.
+//
+// What bounds it, 2048 tokens over 16384 keys, 32 / 8 heads of 128: bf16 430 us, 1198 TFLOP/s, the tensor core 60% busy; the rest is each row tile's softmax,
+// which its next product waits for.  8-bit 646 us: a row tile waits for its values' codes as well (f16 twice in shared memory do not fit), and queries, keys,
+// values and codes keep shared memory's 128 bytes a cycle busy for some 2700 of a tile's 5600 cycles.  (8 warps for keys and values together: 731; with keys a
+// tile ahead 787.)
 #include <algorithm>
 #include <utility>
 
@@ -213,8 +219,10 @@ template <int STORE, bool HIDE> __device__ __forceinline__ void codes_to_f16(uin
 }
 
 // ---- which CTA computes what: an equal part of the cost of everything, in the order of `Walk`, so a CTA has whole row tiles and begins and ends inside one.
-// Every CTA counts the cost itself.  A tile of keys costs 4 (3 where the row tile has one half only), a row tile 16 beside.
-constexpr int EXTRA = 16, LEAST = 2, SMALLEST_SHARE = 48;      // LEAST: tiles of keys that a cut leaves on either side
+// Every CTA counts the cost itself.  A tile of keys costs 4 (3 where the row tile has one half only), a row tile 16 beside: 6 chunks of up to 512 tokens over
+// 6000 keys of an e4m3 pool take 209 us so, 217 with 12 or 8, 224 with 24 (and 250 in row tiles that were all cut into as many parts).  No share is below 16: 64
+// tokens over 4096 keys, 41 us, take 55 in shares of 48.
+constexpr int EXTRA = 16, LEAST = 2, SMALLEST_SHARE = 16;      // LEAST: tiles of keys that a cut leaves on either side
 
 struct Cost {
   int all, units, each;                                      // tiles of keys, the same but one at least, cost of each
@@ -712,20 +720,16 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
             }
           }
         };
-        // bf16: the second half's stay in registers from the maximum to the weights, the first is read twice.  All 128 in registers took 3% longer (and with
-        // 8-bit codes 10% less, as there the instructions count)
+        // the second half's stay in registers from the maximum to the weights, the first is read twice: all 128 in registers took 3% longer
         uint32_t u[KEYS / 2];
         float x4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          uint32_t* x = u;
-          {
-            tmem_ld64(S + 64 * half, x);
-            tmem_wait_ld64(x);
-          }
-          finish(half, x);
+          tmem_ld64(S + 64 * half, u);
+          tmem_wait_ld64(u);
+          finish(half, u);
 #pragma unroll
-          for (int i = 0; i < 64; i += 2) x4[i / 2 & 3] = max3(x4[i / 2 & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+          for (int i = 0; i < 64; i += 2) x4[i / 2 & 3] = max3(x4[i / 2 & 3], __uint_as_float(u[i]), __uint_as_float(u[i + 1]));
         }
         const float top = max3(max3(x4[0], x4[1], x4[2]), x4[3], -INFINITY) * cr;
         if (!(top < INFINITY)) odd = true;                   // NaN or an infinity: the row is computed again
@@ -749,18 +753,17 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
         float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int half = 1; half >= 0; --half) {              // the second half first, over its own scores
-          uint32_t* z = u;
           if (half == 0) {
-            tmem_ld64(S, z);
-            tmem_wait_ld64(z);
-            finish(0, z);
+            tmem_ld64(S, u);
+            tmem_wait_ld64(u);
+            finish(0, u);
           }
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             uint32_t w[16];
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
-              float x = __uint_as_float(z[32 * c + i]), y = __uint_as_float(z[32 * c + i + 1]);
+              float x = __uint_as_float(u[32 * c + i]), y = __uint_as_float(u[32 * c + i + 1]);
               fma2(x, y, cr, -ref, -ref);
               if (!HALF && i % 8 == 6) {
                 exp2_poly2(x, y);

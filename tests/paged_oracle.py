@@ -70,9 +70,11 @@ def tolerance(out, mag, dots, size, keys, f32, store):
     """How far an output may be off, entry by entry.  A score is a sum of `size` products in f32, each addition off by at most 2^-23 of the sum of absolute
     values so far (the tensor core truncates): (size + 8) 2^-23 dots, with the scaling's, and as much again in the reference maximum; exp2 is off by 2^-22.  Weights of bf16 activations: one
     bf16, eps / 2 = 2^-8 (single tokens: two parts, 2^-15); with codes one f16, 2^-11, and either the scale's logarithm (2^-22 of at most 8), 2^-19, or
-    a value times its scale in f16, 2^-11.  Sums of weights and products by keys 2^-23 for every key, and the rounding of a bf16 output by 2^-8 of itself.
+    a key and a value times their scales in f16, 2^-11 each: a score is then off by 2^-11 of the sum of its products' absolute values, 2^-11 dots, and the
+    reference maximum by as much.  Sums of weights and products by keys 2^-23 for every key, and the rounding of a bf16 output by 2^-8 of itself.
     Second-order terms: a quarter more."""
-    weights = 2 * (size + 8) * 2.0 ** -23 * dots[..., None] + 2.0 ** -22 + (0 if f32 else 2.0 ** -8 if store == "act" else 2.0 ** -10) + 2 * min(keys, 4096) * 2.0 ** -23
+    keys_f16 = 0 if f32 or store == "act" else 2.0 ** -11
+    weights = 2 * ((size + 8) * 2.0 ** -23 + keys_f16) * dots[..., None] + 2.0 ** -22 + (0 if f32 else 2.0 ** -8 if store == "act" else 2.0 ** -10) + 2 * min(keys, 4096) * 2.0 ** -23
     return 1.25 * weights * mag + (2.0 ** -22 if f32 else 2.0 ** -8) * out.abs() + 1e-30
 
 

@@ -344,6 +344,17 @@ def test_places_never_written_count_as_zeros(dtype, store):
 
 
 @pytest.mark.parametrize("dtype,store", [t for t in TYPES if t[1] != "act"], ids=[i for t, i in zip(TYPES, IDS) if t[1] != "act"])
+@pytest.mark.parametrize("low,high", [(-126, -100), (-24, -8), (-10, -7)])
+def test_scales_of_keys_of_any_size(dtype, store, low, high):
+    """Keys whose scales are powers of two, within what their codes in f16 take and far outside of it."""
+    cache, step, seqs = make(dtype, store, 2, 64, 64, 16, [(1, 70), (20, 300), (1, 1), (90, 90)])
+    exponents = torch.randint(low, high + 1, cache.k_scale.shape, generator=gen(3))
+    cache.k_scale.copy_(torch.ldexp(torch.ones_like(exponents, dtype=torch.float64), exponents).float())
+    q = torch.randn(step.rows, 4, 64, generator=gen(4)).to(dtype)
+    check(cache.attend(q.to(DEV), step), q, cache, seqs, 0.125)
+
+
+@pytest.mark.parametrize("dtype,store", [t for t in TYPES if t[1] != "act"], ids=[i for t, i in zip(TYPES, IDS) if t[1] != "act"])
 @pytest.mark.parametrize("low,high", [(-126, -120), (-126, 0), (-100, -50), (-95, 90), (-70, 39), (30, 110)])
 def test_scales_of_any_size(dtype, store, low, high):
     """Values whose scales are powers of two from one end of f32 to the other, small ones beside large ones."""
