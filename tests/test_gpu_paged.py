@@ -188,6 +188,37 @@ def test_a_chunk_over_a_long_sequence(dtype, store):
     check(cache.attend(q.to(DEV), step), q, cache, seqs, 128 ** -0.5)
 
 
+SHARES = [                                          # heads, kv heads, K, V, page, window, first, sequences: row tiles of 256 rows cut among the SMs
+    (4, 1, 64, 64, 64, 0, 0, [(700, 20000)]),                              # each over many SMs
+    (8, 2, 64, 64, 32, 0, 0, [(1, 9000), (300, 300), (1, 1), (0, 50), (513, 4000), (1, 5000), (65, 65)]),      # single tokens among chunks
+    (8, 8, 32, 32, 16, 0, 0, [(5 + i % 30, 5 + 7 * i) for i in range(150)]),      # more row tiles than SMs, short ones
+    (64, 1, 128, 64, 16, 0, 0, [(9, 700), (130, 500)]),                    # a group of 64 heads
+    (4, 2, 192, 128, 128, 200, 3, [(400, 6000), (1, 6000), (600, 600)]),   # windows: few keys for each
+]
+
+
+@pytest.mark.parametrize("dtype,store", TYPES[:3], ids=IDS[:3])
+@pytest.mark.parametrize("shape", SHARES, ids=[str(i) for i in range(len(SHARES))])
+def test_row_tiles_shared_among_sms(dtype, store, shape):
+    heads, kv_heads, dim, vdim, page, window, first, sequences = shape
+    cache, step, seqs = make(dtype, store, kv_heads, dim, vdim, page, sequences)
+    q = torch.randn(step.rows, heads, dim, generator=gen(3)).to(dtype)
+    check(cache.attend(q.to(DEV), step, window=window, first=first), q, cache, seqs, dim ** -0.5, window, first)
+
+
+@pytest.mark.parametrize("dtype,store", TYPES, ids=IDS)
+def test_sequences_shorter_than_their_new_tokens(dtype, store):
+    """Lengths that were changed on the device: rows at negative positions see nothing, the others what there is."""
+    cache, step, seqs = make(dtype, store, 2, 64, 64, 16, [(40, 40), (300, 300), (1, 1), (200, 900)])
+    lengths = [7, 10, 0, 100]
+    step.lengths.copy_(torch.tensor(lengths, dtype=torch.int32))
+    seqs = [(n, m, pages) for (n, _, pages), m in zip(seqs, lengths)]
+    q = torch.randn(step.rows, 8, 64, generator=gen(3)).to(dtype)
+    got = cache.attend(q.to(DEV), step)
+    check(got, q, cache, seqs, 0.125)
+    assert not got[:33].any() and not got[40:330].any() and not got[340].any() and not got[341:441].any()
+
+
 @pytest.mark.parametrize("dtype,store", TYPES, ids=IDS)
 def test_pages_that_are_not_there(dtype, store):
     """Keys on them are not seen, whatever is in the pool; a row that sees nothing attends to zeros."""

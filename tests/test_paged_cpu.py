@@ -1,5 +1,8 @@
 """CPU: paged caches without a device: what is refused, which pages a sequence has, and the arithmetic of units and splits that the kernels index by."""
 import ctypes as C
+import os
+import random
+import re
 
 import pytest
 import torch
@@ -7,6 +10,7 @@ import torch
 import paged_oracle as O
 from lit_llama_b200 import PagedCache, PagedStep, PagePool
 from lit_llama_b200 import _seqlib as S
+from lit_llama_b200 import paged
 from lit_llama_b200.state import PoolFull
 
 CPU = torch.device("cpu")
@@ -212,23 +216,39 @@ def test_units_cover_what_is_seen_once_and_splits_cover_the_units(shift):
                 assert got == list(range(len(starts)))
 
 
-def test_padded_rows_meet_no_bank_twice():
-    """The row strides of csrc/seq_paged_attn.cu: what the eight or sixteen lanes of one phase of a load read lies in different banks."""
-    for D in range(16, 257, 16):
-        for es in (1, 2, 4):
-            w = D * es // 4
-            k = {4: w if w % 32 else w + 16, 2: w if w % 16 else w + 8, 1: w if w % 8 else w + 4}[es]
-            v = w if w % 8 else w + 4
-            assert k >= w and v >= w and k * 4 % 16 == 0 and v * 4 % 16 == 0
-            lanes = {1: 32, 2: 16, 4: 8}[es]                            # a phase: 128 bytes
-            banks = [(g * k + es * t + i) % 32 for g in range(lanes // 4) for t in range(4) for i in range(es)]
-            assert len(set(banks)) == len(banks), (D, es)
-            if es < 4:
-                banks = [(r * v + i) % 32 for r in range(8) for i in range(4)]
-                assert len(set(banks)) == 32, (D, es)
-            else:
-                banks = [(2 * t * v + g) % 32 for t in range(4) for g in range(8)]
-                assert len(set(banks)) == 32, (D, es)
+def test_shares_of_row_tiles_cover_all_keys_once():
+    """csrc/seq_paged_tc.cu: cuts at equal costs give every tile of keys of every row tile to one SM, the parts of a row tile to consecutive ones, and no SM
+    more than one part that goes on and one that came from before."""
+    source = open(os.path.join(os.path.dirname(paged.__file__), "csrc", "seq_paged_tc.cu")).read()
+    extra, least, smallest = (int(x) for x in re.search(r"EXTRA = (\d+), LEAST = (\d+), SMALLEST_SHARE = (\d+);", source).groups())
+
+    def cut(units, each, d):
+        if d <= 0 or d >= extra + units * each:
+            return 0 if d <= 0 else units
+        y = max(d - extra, 0) // each
+        return 0 if y < least else units if units - y < least else y
+
+    rng = random.Random(1)
+    for _ in range(300):
+        tiles = [(max(rng.choice([0, 1, 2, 3, 4, 5, rng.randint(0, 40), rng.randint(0, 1000)]), 1), rng.choice([3, 4])) for _ in range(rng.choice([1, 2, 7, 60, 300]))]
+        at = [0]
+        for units, each in tiles:
+            at.append(at[-1] + extra + units * each)
+        ctas = rng.choice([1, 2, 5, 148])
+        share = max(-(-at[-1] // ctas), smallest)
+        parts, goes_on, came = [[] for _ in tiles], set(), set()
+        for c in range(ctas):
+            for i, (units, each) in enumerate(tiles):
+                t0, t1 = (cut(units, each, min(x * share, at[-1]) - at[i]) for x in (c, c + 1))
+                if t0 < t1:
+                    parts[i].append((c, t0, t1))
+                    if t1 - t0 < units:
+                        side = goes_on if t0 == 0 else came
+                        assert c not in side
+                        side.add(c)
+        for (units, _), mine in zip(tiles, parts):
+            assert [t0 for _, t0, _ in mine] == [0] + [t1 for _, _, t1 in mine[:-1]] and mine[-1][2] == units
+            assert [c for c, _, _ in mine] == list(range(mine[0][0], mine[0][0] + len(mine)))
 
 
 def test_the_oracle_sees_what_the_formula_says():
