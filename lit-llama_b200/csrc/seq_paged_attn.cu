@@ -767,7 +767,7 @@ extern "C" int b2l_seq_paged_attention(const void* q, long long ldq, long long h
   B2L_CHECK_ARG(scale > 0.f && scale < INFINITY, "%s: the scale must be positive and finite", who);
   const int per = act_dtype == B2L_F32 ? 4 : 8;
   B2L_CHECK_ARG((((uintptr_t)q | (uintptr_t)out | (uintptr_t)work) & 15) == 0 && ldq % per == 0 && hsq % per == 0, "%s: rows must be 16-byte aligned", who);
-  B2L_CHECK_SUPPORTED((long long)width * page < (1ll << 30) && kv_heads < 65536 && (long long)rows * heads < (1ll << 31) && (long long)pages * kv_heads * page < (1ll << 31),
+  B2L_CHECK_SUPPORTED((long long)width * page < (1ll << 30) && kv_heads < 65536 && (long long)rows * heads < (1ll << 31) - 65536 && (long long)pages * kv_heads * page < (1ll << 31),
                       "%s: sizes beyond the grid's or a copy's coordinates", who);
   if (rows == 0 || seqs == 0) return 0;
   const Plan p = plan_of(rows, seqs, width, page, heads, kv_heads, K, V, window, first, max_new, max_length, store, act_dtype);
