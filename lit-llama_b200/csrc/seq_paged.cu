@@ -119,8 +119,8 @@ template <typename act_t, int STORE, int NI, int HEADS>
 __global__ void __launch_bounds__(256) paged_write_kernel(const __grid_constant__ Rows a) {
   const int lane = threadIdx.x & 31, l = lane & 15;
   const bool value = lane >= 16;
-  const int groups = (a.kv_heads + HEADS - 1) / HEADS;
-  const long long unit = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+  const uint32_t groups = (uint32_t)(a.kv_heads + HEADS - 1) / HEADS;
+  const uint32_t unit = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
   const int row = (int)(unit / groups), h0 = (int)(unit % groups) * HEADS;
   if (row >= a.s.rows) return;
   const int D = value ? a.V : a.K;
@@ -174,8 +174,8 @@ template <typename act_t, int STORE, int NI, int HEADS>
 __global__ void __launch_bounds__(256) paged_read_kernel(const __grid_constant__ Rows a) {
   const int lane = threadIdx.x & 31, l = lane & 15;
   const bool value = lane >= 16;
-  const int groups = (a.kv_heads + HEADS - 1) / HEADS;
-  const long long unit = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+  const uint32_t groups = (uint32_t)(a.kv_heads + HEADS - 1) / HEADS;
+  const uint32_t unit = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
   const int row = (int)(unit / groups), h0 = (int)(unit % groups) * HEADS;
   if (row >= a.s.rows) return;
   const int b = sequence_of(a.s, row, lane);
@@ -244,7 +244,7 @@ static int rows_call(const char* who, const void* k_new, long long ldk, long lon
   const int per_warp = many ? HEADS : 2, warps = many ? 8 : 1;
   const long long units = (long long)rows * ((kv_heads + per_warp - 1) / per_warp);
   const long long blocks = (units + warps - 1) / warps;
-  B2L_CHECK_SUPPORTED(blocks < (1ll << 31), "%s: %d rows of %d heads", who, rows, kv_heads);
+  B2L_CHECK_SUPPORTED(units < (1ll << 31), "%s: %d rows of %d heads", who, rows, kv_heads);
   const cudaStream_t st = (cudaStream_t)stream;
 #define LAUNCH(T, ST, NI, H)                                                                       \
   (WRITE ? paged_write_kernel<T, ST, NI, H><<<(unsigned)blocks, 32 * warps, 0, st>>>(a)            \
