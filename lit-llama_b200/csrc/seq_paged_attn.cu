@@ -691,7 +691,8 @@ static long long few_floats(int splits, long long count, int V) { return splits 
 static Plan plan_of(int rows, int seqs, int width, int page, int heads, int kv_heads, int K, int V, int window, int first, int max_new, int max_length, int store, int act_dtype) {
   Plan p{};
   const int G = heads / kv_heads, sms = sm_count(), most = std::min(seqs, rows);
-  const long long packed = (long long)rows * G, longest = (long long)(max_new > 0 ? std::min(max_new, rows) : rows) * G;      // packed rows of one sequence
+  // packed rows of the longest of the sequences; where the host says nothing, a token each if there are no more rows than sequences
+  const long long packed = (long long)rows * G, longest = (long long)(max_new > 0 ? std::min(max_new, rows) : rows <= seqs ? 1 : rows) * G;
   long long keys = (long long)width * page;                  // the most keys that a row sees
   if (max_length > 0) keys = std::min<long long>(keys, max_length);
   if (window > 0) keys = std::min<long long>(keys, (long long)window + first + 16);

@@ -62,7 +62,7 @@ struct Parts { float *ml, *o; int splits; long long count; };
 
 // What the CTAs of the chunk kernel leave for one another: of each the last row tile if it goes on in the next CTA (sequence, first packed row, head, number of
 // CTAs that have a part; none: 0), and two places for partial results of 256 rows (the first row tile's, the last one's) [2 ctas][256][2] and [2 ctas][256][V]
-struct Shared { int4* last; float *ml, *o; int ctas; };
+struct Shared { int4* last; float *ml, *o; };
 
 struct Attn {
   Step s;

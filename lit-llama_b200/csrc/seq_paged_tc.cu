@@ -966,7 +966,6 @@ template <int STORE> static int go(const Attn& a, int ctas, cudaStream_t stream)
   return 0;
 }
 int many_launch(Attn& a, int ctas, float* work, cudaStream_t stream) {
-  a.many.ctas = ctas;
   a.many.last = reinterpret_cast<int4*>(work);
   a.many.ml = work + 4 * ctas;
   a.many.o = a.many.ml + 4ll * ctas * ROWS;

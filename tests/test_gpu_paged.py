@@ -326,6 +326,11 @@ def test_what_the_host_says_of_a_step_changes_no_result(dtype, store):
     for hints in (dict(), dict(max_new=1, max_length=16), dict(max_new=100000, max_length=10 ** 6), dict(max_new=1, max_length=900), dict(max_new=130)):
         s = PagedStep(step.starts, step.lengths, step.table, rows=step.rows, **hints)
         check(cache.attend(q.to(DEV), s), q, cache, seqs, 0.125)
+    # no more rows than sequences, all of one of them
+    cache, step, seqs = make(dtype, store, 2, 64, 64, 32, [(0, 5)] * 20 + [(40, 300)] + [(0, 0)] * 20)
+    q = torch.randn(step.rows, 8, 64, generator=gen(3)).to(dtype)
+    for hints in (dict(), dict(max_new=40)):
+        check(cache.attend(q.to(DEV), PagedStep(step.starts, step.lengths, step.table, rows=step.rows, **hints)), q, cache, seqs, 0.125)
 
 
 def test_the_same_call_gives_the_same_bits():
