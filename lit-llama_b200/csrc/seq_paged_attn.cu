@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
     pl.b = blockIdx.x;
     sequence(a.s, pl.b, pl.start, pl.n, pl.length);
     pl.first = 0;
-    if (pl.n == 0) return;
+    if (pl.n == 0 || (long long)pl.n * G > a.few_max) return;
   } else if (!a.place(blockIdx.x - a.s.seqs, R, lane, pl)) {
     return;
   }
@@ -590,7 +590,7 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
     }
     const int row = pl.start + at / G, head = h * G + at % G;
     if (a.few.splits > 1) {
-      const long long to = (long long)split * a.few.count + (long long)row * a.heads + head;
+      const long long to = (long long)split * a.few.count + (a.both ? (long long)(pl.b * a.kv_heads + h) * a.few_max + at : (long long)row * a.heads + head);
       if (d == 0) *reinterpret_cast<float2*>(a.few.ml + 2 * to) = make_float2(M, L);
       *reinterpret_cast<float4*>(a.few.o + to * a.V + d) = make_float4(x[0], x[1], x[2], x[3]);
     } else {
@@ -617,7 +617,20 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const __g
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
   const int here = MERGE_WARPS / per, sub = warp / here, own = warp % here;      // part of the unit's warps, unit of the block
   const long long at = (long long)blockIdx.x * here + own;
-  const int row = (int)min(at / a.heads, (long long)a.s.rows), head = (int)(at % a.heads), b = row < a.s.rows ? sequence_of(a.s, row, lane) : -1;
+  int row, head, b = -1;
+  if (a.both) {                                              // the packed rows of every sequence and key/value head
+    const int G = a.heads / a.kv_heads, r = (int)(at % a.few_max), h = (int)(at / a.few_max % a.kv_heads);
+    const long long of = at / a.few_max / a.kv_heads;
+    int start = 0, n = 0, length;
+    if (of < a.s.seqs) sequence(a.s, (int)of, start, n, length);
+    if ((long long)n * G <= a.few_max && r < n * G) b = (int)of;
+    row = start + r / G;
+    head = h * G + r % G;
+  } else {
+    row = (int)min(at / a.heads, (long long)a.s.rows);
+    head = (int)(at % a.heads);
+    if (row < a.s.rows) b = sequence_of(a.s, row, lane);
+  }
   const Parts& p = a.few;
   const bool on = b >= 0;
   float M = -INFINITY, L = 0.f;
@@ -681,8 +694,8 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const __g
 
 // ------------------------------------------------------------------------------------------------ host
 struct Plan {
-  int few_rows, few_tiles, few_splits, many_ctas;            // many_ctas: of the chunk kernel, 0 where the few-row kernel takes the step
-  long long floats;
+  int few_max, few_rows, few_tiles, few_splits, many_ctas;   // few_tiles: of the few-row kernel, 0 where the chunk kernel takes the step; many_ctas: the other way round
+  long long few_count, floats;
 };
 constexpr long long MOST_WORK = 1ll << 27;                   // floats of partial results
 
@@ -696,23 +709,38 @@ static Plan plan_of(int rows, int seqs, int width, int page, int heads, int kv_h
   long long keys = (long long)width * page;                  // the most keys that a row sees
   if (max_length > 0) keys = std::min<long long>(keys, max_length);
   if (window > 0) keys = std::min<long long>(keys, (long long)window + first + 16);
-  // The chunk kernel takes steps with a sequence of more than 16 packed rows, single tokens among them too
+  // The chunk kernel takes steps with a sequence of more than 16 packed rows.  Single tokens among them too, at up to 3.5 times the few-row kernel's time from
+  // 8-bit pools and 1.3 times from bf16 ones, until what that adds is more than the 12 us of two more launches: a chunk of 512 with 8, 48 or 192 tokens of others
+  // over 4096 keys of 8 heads takes 107, 184 or 381 us in both kernels from e4m3, 121, 332 or 1084 in the one; from bf16 with 48 or 192 215 and 573, or 210
+  // and 670.  There are at most `singles` of them.
+  long long singles = seqs;
+  p.few_max = INT32_MAX;
   if (act_dtype == B2L_BF16 && longest > 16 && many_takes(K, V, store)) {
     p.many_ctas = many_ctas((packed / 256 + most) * kv_heads, keys + (window > 0 ? 256 / G : 0), sms);
     p.floats = many_floats(p.many_ctas, V);
-    return p;
+    const long long more = longest / G - 1;                  // rows of the longest beside its first
+    singles -= (std::max(rows - seqs, 0) + more - 1) / std::max(more, 1ll);
+    const bool both = G <= 16 && singles > 0 && singles * kv_heads * 0.5 * keys * (store == ACT ? 0.015e-3 : 0.119e-3) > 12;
+    p.few_max = both ? (G <= 8 ? 8 : 16) : 0;
+    if (!both) return p;
+    p.few_rows = p.few_max;
+    p.few_tiles = seqs;
+    p.few_count = (long long)seqs * kv_heads * p.few_max;
+  } else {
+    // rows of a tile: 8 where a token's heads, or all that the longest of the sequences has, fit
+    p.few_rows = (max_new > 0 ? (long long)max_new * G <= 8 : G <= 8 && packed <= 8ll * most) ? 8 : 16;
+    p.few_tiles = seqs + (int)std::min<long long>(packed / p.few_rows, INT32_MAX - seqs);
+    p.few_count = (long long)rows * heads;
+    singles = std::max<long long>(seqs, packed / p.few_rows);
   }
-  // rows of a tile: 8 where a token's heads, or all that the longest of the sequences has, fit
-  p.few_rows = (max_new > 0 ? (long long)max_new * G <= 8 : G <= 8 && packed <= 8ll * most) ? 8 : 16;
-  p.few_tiles = seqs + (int)std::min<long long>(packed / p.few_rows, INT32_MAX - seqs);
   // An SM has three CTAs at a time.  Few CTAs: as many parts as fill them once, of 128 keys at least (one token over 1031 keys of 32 heads: 15.1 us in 4 parts,
   // 13.0 in 8).  Many: parts of a quarter of that each, of 512 keys at least, so that sequences of different lengths share the SMs evenly (48 over up to 8192
   // keys of an e4m3 pool: 143 us whole, 128 in 4 parts, 140 in 8)
-  const long long ctas = (long long)kv_heads * std::max<long long>(seqs, packed / p.few_rows), slots = 3ll * sms, count = (long long)rows * heads;
+  const long long ctas = (long long)kv_heads * singles, slots = 3ll * sms;
   const bool room = 2 * ctas <= slots;
   const long long want = room ? slots / ctas : (4 * slots + ctas - 1) / ctas;
-  p.few_splits = (int)std::max<long long>(1, std::min({want, keys / (room ? 128 : 512), 128ll, MOST_WORK / (count * (V + 2) + 1)}));
-  p.floats = few_floats(p.few_splits, count, V);
+  p.few_splits = (int)std::max<long long>(1, std::min({want, keys / (room ? 128 : 512), 128ll, MOST_WORK / (p.few_count * (V + 2) + 1)}));
+  p.floats += few_floats(p.few_splits, p.few_count, V);
   return p;
 }
 
@@ -782,9 +810,15 @@ extern "C" int b2l_seq_paged_attention(const void* q, long long ldq, long long h
   a.scale_log2 = scale * 1.44269502162933349609375f;         // log2(e)
   a.f32 = act_dtype == B2L_F32; a.store_kind = store;
   const cudaStream_t st = (cudaStream_t)stream;
-  if (p.many_ctas) return many_launch(a, p.many_ctas, work, st);
+  a.few_max = p.few_max;
+  a.both = p.few_tiles > 0 && p.many_ctas > 0;
+  if (p.many_ctas) {
+    const int rc = many_launch(a, p.many_ctas, work, st);
+    if (rc || !a.both) return rc;
+    work += many_floats(p.many_ctas, V);
+  }
   a.few.splits = p.few_splits;
-  a.few.count = (long long)rows * heads;
+  a.few.count = p.few_count;
   a.few.ml = work;
   a.few.o = work + (2 * p.few_splits * a.few.count + 3) / 4 * 4;
   int rc = 0;

@@ -71,8 +71,9 @@ struct Attn {
   void* out;
   long long ldq, hsq;
   int heads, kv_heads, K, V, window, first;
+  int few_max;                                               // sequences of at most so many packed rows are the few-row kernel's, the others the chunk kernel's
   float scale_log2;
-  int f32, store_kind;
+  int f32, store_kind, both;                                 // both: the two kernels share the step, few_max packed rows of every sequence and head in `few`
   Parts few;
   Shared many;
 

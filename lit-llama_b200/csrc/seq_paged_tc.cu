@@ -249,12 +249,12 @@ __device__ __forceinline__ long long sequence_cost(const Attn& a, Place pl, int 
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   return sum;
 }
-// each sequence lo .. hi - 1 with rows, until f says true
+// each sequence lo .. hi - 1 that is this kernel's, until f says true
 template <typename F> __device__ __forceinline__ void each_sequence(const Attn& a, int lo, int hi, int lane, F f) {
   for (int b0 = lo; b0 < hi; b0 += 32) {
     int start = 0, n = 0, length = 0;
     if (b0 + lane < hi) sequence(a.s, b0 + lane, start, n, length);
-    for (uint32_t left = __ballot_sync(0xffffffffu, n > 0); left; left &= left - 1) {
+    for (uint32_t left = __ballot_sync(0xffffffffu, (long long)n * (a.heads / a.kv_heads) > a.few_max); left; left &= left - 1) {
       const int i = __ffs(left) - 1;
       if (f(Place{b0 + i, __shfl_sync(0xffffffffu, start, i), __shfl_sync(0xffffffffu, n, i), __shfl_sync(0xffffffffu, length, i), 0})) return;
     }

@@ -194,6 +194,8 @@ SHARES = [                                          # heads, kv heads, K, V, pag
     (8, 8, 32, 32, 16, 0, 0, [(5 + i % 30, 5 + 7 * i) for i in range(150)]),      # more row tiles than SMs, short ones
     (64, 1, 128, 64, 16, 0, 0, [(9, 700), (130, 500)]),                    # a group of 64 heads
     (4, 2, 192, 128, 128, 200, 3, [(400, 6000), (1, 6000), (600, 600)]),   # windows: few keys for each
+    (12, 4, 64, 64, 64, 0, 0, [(1 + i % 4, 9000 - 100 * i) for i in range(60)] + [(200, 300), (0, 7), (9, 9), (1, 1)]),      # both kernels: 8 packed rows and more
+    (16, 1, 64, 64, 64, 0, 0, [(1, 9000 - 60 * i) for i in range(100)] + [(64, 3000), (2, 70)]),      # and 16
 ]
 
 
