@@ -497,17 +497,18 @@ int b2l_seq_mlstm_readout(const b2l_seq_mlstm_args* a, b2l_stream_t stream);
  * tokens long with them (device int32 [seqs]), and its token j lies in page table[b*ldt + j/page], place j%page (device int32, `width` entries per
  * sequence).  The row starts[b]+i is at position lengths[b] - (rows of b) + i.  These are read on the device and clipped to rows, width and pages; a
  * table entry outside the pool is a page that is not there (and so is every negative position's): nothing is written to it, it reads as zeros, and no
- * row sees its keys.  A row of no sequence is left out: nothing is written for it, and its outputs stay as they are.
+ * row sees its keys.  A row of no sequence is left out: nothing is written for it, and its outputs stay as they are (where not said otherwise).
  *
  *   b2l_seq_paged_write      new rows into the pool; 8-bit: scale = max(max |x| (1 / c), 2^-126), code = round(x / scale) to nearest even, c = 448 (e4m3) or
  *                            127 (int8), per token and head (of keys and of values); a row with an infinity or NaN gets the scale NaN and codes 0
- *   b2l_seq_paged_read       the step's rows out of the pool: code * scale, rounded to the activation type
+ *   b2l_seq_paged_read       the step's rows out of the pool: code * scale, rounded to the activation type; a row of no sequence: zeros
  *   b2l_seq_paged_attention  out[r, h] = sum_j w_j v_j / sum_j w_j over the keys j that row r at position p sees, j <= p and (window == 0 or j > p - window
  *                            or j < first); w_j = exp(scale q . k_j - max); query head h reads key / value head h / (heads / kv_heads).  A row whose
  *                            weights sum to 0 (it sees no key) gives zeros.  scale > 0.  q and out act [rows, heads, K or V].
  *                            max_new, max_length: the most new tokens and the longest of the step's sequences, where the host knows (0 or less: it does not); they pick
  *                            between equivalent forms.
  *                            `work` has b2l_seq_paged_attention_work floats (may be null when that is 0).
+ *   b2l_seq_paged_attention_all  the same, and zeros in the outputs of rows of no sequence
  * ldX and hsX: elements between tokens and between heads (rows 16-byte aligned, the entries of a head consecutive). */
 enum { B2L_SEQ_STORE_ACT = 0, B2L_SEQ_STORE_E4M3 = 1, B2L_SEQ_STORE_INT8 = 2 };
 int b2l_seq_paged_write(const void* k_new, long long ldk, long long hsk, const void* v_new, long long ldv, long long hsv, void* k, void* v, float* k_scale, float* v_scale,
@@ -520,6 +521,10 @@ int b2l_seq_paged_attention(const void* q, long long ldq, long long hsq, const v
                             const int* lengths, const int* table, int ldt, int width, void* out, float* work, long long work_floats, int rows, int seqs, int pages, int page,
                             int heads, int kv_heads, int K, int V, int window, int first, float scale, int max_new, int max_length, int store, int act_dtype,
                             b2l_stream_t stream);
+int b2l_seq_paged_attention_all(const void* q, long long ldq, long long hsq, const void* k, const void* v, const float* k_scale, const float* v_scale, const int* starts,
+                                const int* lengths, const int* table, int ldt, int width, void* out, float* work, long long work_floats, int rows, int seqs, int pages, int page,
+                                int heads, int kv_heads, int K, int V, int window, int first, float scale, int max_new, int max_length, int store, int act_dtype,
+                                b2l_stream_t stream);
 long long b2l_seq_paged_attention_work(int rows, int seqs, int width, int page, int heads, int kv_heads, int K, int V, int window, int first, int max_new,
                                        int max_length, int store, int act_dtype);
 

@@ -138,6 +138,8 @@ class MlstmArgs(C.Structure):
     ]
 
 
+_PAGED_ATTENTION = ([c_void_p, C.c_longlong, C.c_longlong] + [c_void_p] * 7 + [c_int] * 2 + [c_void_p] * 2 + [C.c_longlong] + [c_int] * 10 + [c_float] + [c_int] * 4
+                    + [c_void_p])
 _PAGED_ROWS = [c_void_p, C.c_longlong, C.c_longlong] * 2 + [c_void_p] * 7 + [c_int] * 11 + [c_void_p]
 
 _SIGS = {
@@ -215,8 +217,8 @@ _SIGS = {
     "b2l_seq_mlstm_readout": (c_int, [C.POINTER(MlstmArgs), c_void_p]),
     "b2l_seq_paged_write": (c_int, _PAGED_ROWS),
     "b2l_seq_paged_read": (c_int, _PAGED_ROWS),
-    "b2l_seq_paged_attention": (c_int, [c_void_p, C.c_longlong, C.c_longlong] + [c_void_p] * 7 + [c_int] * 2 + [c_void_p] * 2 + [C.c_longlong] + [c_int] * 10 + [c_float]
-                                + [c_int] * 4 + [c_void_p]),
+    "b2l_seq_paged_attention": (c_int, _PAGED_ATTENTION),
+    "b2l_seq_paged_attention_all": (c_int, _PAGED_ATTENTION),
     "b2l_seq_paged_attention_work": (C.c_longlong, [c_int] * 14),
 }
 

@@ -179,10 +179,9 @@ __global__ void __launch_bounds__(256) paged_read_kernel(const __grid_constant__
   const int row = (int)(unit / groups), h0 = (int)(unit % groups) * HEADS;
   if (row >= a.s.rows) return;
   const int b = sequence_of(a.s, row, lane);
-  if (b < 0) return;
-  int start, n, length;
-  sequence(a.s, b, start, n, length);
-  const int p = length - n + row - start;
+  int start = 0, n = 0, length = 0;
+  if (b >= 0) sequence(a.s, b, start, n, length);
+  const int p = b >= 0 ? length - n + row - start : -1;      // a row of no sequence reads as one whose page is not there
   const int page = p >= 0 ? page_of(a.s, b, p) : -1;
   const int D = value ? a.V : a.K;
   const size_t at = (((size_t)max(page, 0) * a.kv_heads + h0) << a.s.shift) + (p & ((1 << a.s.shift) - 1)), to_next = (size_t)1 << a.s.shift;

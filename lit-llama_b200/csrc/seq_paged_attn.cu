@@ -141,6 +141,10 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
     pl.b = blockIdx.x;
     sequence(a.s, pl.b, pl.start, pl.n, pl.length);
     pl.first = 0;
+    if (a.zeros && split == 0) {                             // sequences' rows follow one another: the rest lies before the first and behind the last
+      if (pl.b == 0 && pl.start > 0) clear_rows(a, 0, pl.start, h * G, G, threadIdx.x, blockDim.x);
+      if (pl.b == a.s.seqs - 1 && pl.start + pl.n < a.s.rows) clear_rows(a, pl.start + pl.n, a.s.rows, h * G, G, threadIdx.x, blockDim.x);
+    }
     if (pl.n == 0 || (long long)pl.n * G > a.few_max) return;
   } else if (!a.place(blockIdx.x - a.s.seqs, R, lane, pl)) {
     return;
@@ -783,12 +787,11 @@ extern "C" long long b2l_seq_paged_attention_work(int rows, int seqs, int width,
   return paged::plan_of(rows, seqs, width, page, heads, kv_heads, K, V, window, first, max_new, max_length, store, act_dtype).floats;
 }
 
-extern "C" int b2l_seq_paged_attention(const void* q, long long ldq, long long hsq, const void* k, const void* v, const float* k_scale, const float* v_scale, const int* starts,
-                                       const int* lengths, const int* table, int ldt, int width, void* out, float* work, long long work_floats, int rows, int seqs, int pages,
-                                       int page, int heads, int kv_heads, int K, int V, int window, int first, float scale, int max_new, int max_length, int store,
-                                       int act_dtype, b2l_stream_t stream) {
+static int attention(const char* who, bool zeros, const void* q, long long ldq, long long hsq, const void* k, const void* v, const float* k_scale, const float* v_scale,
+                     const int* starts, const int* lengths, const int* table, int ldt, int width, void* out, float* work, long long work_floats, int rows, int seqs, int pages,
+                     int page, int heads, int kv_heads, int K, int V, int window, int first, float scale, int max_new, int max_length, int store, int act_dtype,
+                     b2l_stream_t stream) {
   using namespace paged;
-  const char* who = "b2l_seq_paged_attention";
   B2L_CHECK_ARG(q && out, "%s: null pointer", who);
   if (int rc = check_pool(who, k, v, k_scale, v_scale, starts, lengths, table, ldt, width, rows, seqs, pages, page, kv_heads, K, V, store, act_dtype)) return rc;
   B2L_CHECK_ARG(heads > 0 && heads % kv_heads == 0, "%s: %d heads over %d key/value heads", who, heads, kv_heads);
@@ -811,10 +814,12 @@ extern "C" int b2l_seq_paged_attention(const void* q, long long ldq, long long h
   a.f32 = act_dtype == B2L_F32; a.store_kind = store;
   const cudaStream_t st = (cudaStream_t)stream;
   a.few_max = p.few_max;
+  a.zeros = zeros;
   a.both = p.few_tiles > 0 && p.many_ctas > 0;
   if (p.many_ctas) {
     const int rc = many_launch(a, p.many_ctas, work, st);
     if (rc || !a.both) return rc;
+    a.zeros = 0;                                             // they are there
     work += many_floats(p.many_ctas, V);
   }
   a.few.splits = p.few_splits;
@@ -834,4 +839,20 @@ extern "C" int b2l_seq_paged_attention(const void* q, long long ldq, long long h
   B2L_CUDA(cudaLaunchKernelEx(&launch.cfg, paged_merge_kernel, a, warps));
   B2L_LAUNCH_CHECK("paged_merge_kernel");
   return 0;
+}
+
+extern "C" int b2l_seq_paged_attention(const void* q, long long ldq, long long hsq, const void* k, const void* v, const float* k_scale, const float* v_scale, const int* starts,
+                                       const int* lengths, const int* table, int ldt, int width, void* out, float* work, long long work_floats, int rows, int seqs, int pages,
+                                       int page, int heads, int kv_heads, int K, int V, int window, int first, float scale, int max_new, int max_length, int store,
+                                       int act_dtype, b2l_stream_t stream) {
+  return attention("b2l_seq_paged_attention", false, q, ldq, hsq, k, v, k_scale, v_scale, starts, lengths, table, ldt, width, out, work, work_floats, rows, seqs, pages, page, heads,
+                   kv_heads, K, V, window, first, scale, max_new, max_length, store, act_dtype, stream);
+}
+
+extern "C" int b2l_seq_paged_attention_all(const void* q, long long ldq, long long hsq, const void* k, const void* v, const float* k_scale, const float* v_scale, const int* starts,
+                                           const int* lengths, const int* table, int ldt, int width, void* out, float* work, long long work_floats, int rows, int seqs, int pages,
+                                           int page, int heads, int kv_heads, int K, int V, int window, int first, float scale, int max_new, int max_length, int store,
+                                           int act_dtype, b2l_stream_t stream) {
+  return attention("b2l_seq_paged_attention_all", true, q, ldq, hsq, k, v, k_scale, v_scale, starts, lengths, table, ldt, width, out, work, work_floats, rows, seqs, pages, page,
+                   heads, kv_heads, K, V, window, first, scale, max_new, max_length, store, act_dtype, stream);
 }

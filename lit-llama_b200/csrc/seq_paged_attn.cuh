@@ -73,6 +73,7 @@ struct Attn {
   int heads, kv_heads, K, V, window, first;
   int few_max;                                               // sequences of at most so many packed rows are the few-row kernel's, the others the chunk kernel's
   float scale_log2;
+  int zeros;                                                 // whether rows of no sequence become zeros (else they stay as they are)
   int f32, store_kind, both;                                 // both: the two kernels share the step, few_max packed rows of every sequence and head in `few`
   Parts few;
   Shared many;
@@ -137,6 +138,13 @@ struct Attn {
     return (store_kind == E4M3 ? e4m3_pair(c).x : (float)(int8_t)c) * scales[row];
   }
 };
+
+// Zeros in the outputs of rows r0 .. r1 - 1, n heads from `head` on
+static __device__ __noinline__ void clear_rows(const Attn& a, int r0, int r1, int head, int n, int me, int threads) {
+  const int es = a.f32 ? 4 : 2, pieces = n * a.V * es / 16;
+  for (long long i = me; i < (long long)(r1 - r0) * pieces; i += threads)
+    *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(a.out) + ((size_t)(r0 + i / pieces) * a.heads + head) * a.V * es + i % pieces * 16) = make_uint4(0u, 0u, 0u, 0u);
+}
 
 // One row and head again by a warp, key after key over what the row sees and nothing else.  The products above multiply a hidden value by a weight of
 // zero, and an f32 infinity has parts of NaN: a result that is not finite is computed again here, so it is what the formula says.

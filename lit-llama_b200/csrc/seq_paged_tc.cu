@@ -321,6 +321,11 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
   {
     const int warps = blockDim.x / 32, by = (a.s.seqs + warps - 1) / warps, lo = min(warp * by, a.s.seqs), hi = min(lo + by, a.s.seqs);
     long long mine = 0, before = 0, all = 0;
+    int r0 = 0, r1 = a.s.rows;                               // rows of no sequence: before r0 and from r1 on; warp 3 has nothing else to do
+    if (a.zeros && warp == 3) {
+      r0 = min(max(a.s.starts[0], 0), a.s.rows);
+      r1 = max(min(a.s.starts[a.s.seqs], a.s.rows), r0);
+    }
     each_sequence(a, lo, hi, lane, [&](const Place& pl) {
       mine += sequence_cost(a, pl, lane) * a.kv_heads;
       return false;
@@ -331,6 +336,10 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
     for (int i = 0; i < warps; ++i) {
       if (i == warp) before = all;
       all += costs[i];
+    }
+    if (a.zeros && warp == 3) {                              // every CTA's part of them
+      if (r0 > 0) clear_rows(a, 0, r0, 0, a.heads, blockIdx.x * 32 + lane, gridDim.x * 32);
+      if (r1 < a.s.rows) clear_rows(a, r1, a.s.rows, 0, a.heads, blockIdx.x * 32 + lane, gridDim.x * 32);
     }
     const long long share = max((all + gridDim.x - 1) / gridDim.x, (long long)SMALLEST_SHARE);
     const long long x0 = blockIdx.x * share;

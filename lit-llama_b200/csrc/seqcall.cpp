@@ -102,7 +102,8 @@ struct Entry {
   F(b2l_seq_linear_few) \
   F(b2l_seq_paged_write) \
   F(b2l_seq_paged_read) \
-  F(b2l_seq_paged_attention)
+  F(b2l_seq_paged_attention) \
+  F(b2l_seq_paged_attention_all)
 #define ENTRY(name) {#name, Thunk<decltype(&name)>::signature, Thunk<decltype(&name)>::call},
 const Entry entries[] = {ALL(ENTRY)};
 constexpr int N_ENTRIES = (int)(sizeof(entries) / sizeof(entries[0]));

@@ -241,7 +241,8 @@ class PagedCache:
         self._call("b2l_seq_paged_write", step, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, *(self._at or ()), *(step._at or ()), min(k.shape[0], v.shape[0]), step.seqs, *self._sizes)
 
     def read(self, step: PagedStep) -> Tuple[torch.Tensor, torch.Tensor]:
-        """The rows that `write` with this step puts into the pool, as they lie there: keys [rows, kv_heads, dim] and values in the activation type."""
+        """The rows that `write` with this step puts into the pool, as they lie there: keys [rows, kv_heads, dim] and values in the activation type; zeros where the
+        step's tensors have no sequence for a row."""
         G, K, V = self.kv_heads, self.dim, self.vdim
         k, v = self._like.new_empty((step.rows, G, K)), self._like.new_empty((step.rows, G, V))
         self._call("b2l_seq_paged_read", step, k.data_ptr(), G * K, K, v.data_ptr(), G * V, V, *(self._at or ()), *(step._at or ()), step.rows, step.seqs, *self._sizes)
@@ -254,21 +255,22 @@ class PagedCache:
             out[r, h] = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale q[r, h] . k_j), j <= p and (window == 0 or j > p - window or j < first)
 
         q [rows, heads, dim] with heads a multiple of kv_heads (head h reads key/value head h // (heads / kv_heads)), p the position of row r; scale
-        dim^-1/2 unless given.  Returns [rows, heads, vdim] (`out`, contiguous, where given); rows behind the step's last sequence are zeros, or as they were
-        in `out`."""
+        dim^-1/2 unless given.  Returns [rows, heads, vdim] (`out`, contiguous, where given); rows of no sequence, behind the step's last one or before its first,
+        are zeros, or as they were in `out`."""
         q = self._rows(q, 0, self.dim, step, "queries")
         rows, heads, _ = q.shape
         plan = step._plans.get((rows, heads, scale, window, first, self._sizes))
         if plan is None:
             plan = self._plan(rows, heads, scale, window, first, step)
         floats, sizes = plan
+        name = "b2l_seq_paged_attention"
         if out is None:
-            out = (q.new_empty if rows == step.rows else q.new_zeros)((rows, heads, self.vdim))
+            out, name = q.new_empty((rows, heads, self.vdim)), "b2l_seq_paged_attention_all"      # which rows have a sequence is known on the device only
         elif out.shape != (rows, heads, self.vdim) or out.dtype != self.dtype or out.device != self.device or not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError(f"paged cache: out must be {(rows, heads, self.vdim)} {self.dtype} on {self.device}, contiguous and 16-byte aligned")
         work = step._tensors[1].new_empty((floats,)) if floats else None          # four bytes an entry
         s0, s1, _ = q.stride()
-        self._call("b2l_seq_paged_attention", step, q.data_ptr(), s0, s1, *(self._at or ()), *(step._at or ()), out.data_ptr(), work.data_ptr() if floats else None, floats, *sizes)
+        self._call(name, step, q.data_ptr(), s0, s1, *(self._at or ()), *(step._at or ()), out.data_ptr(), work.data_ptr() if floats else None, floats, *sizes)
         return out
 
     def _plan(self, rows: int, heads: int, scale: Optional[float], window: int, first: int, step: PagedStep) -> tuple:
