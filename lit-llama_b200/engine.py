@@ -214,9 +214,9 @@ class Engine:
     def _turn(self, r: Request) -> None:
         if r.fed < len(r.prompt):
             part = r.prompt[r.fed: r.fed + self.prefill_chunk]
-            r.fed += len(part)
-            last = r.fed == len(r.prompt)
+            last = r.fed + len(part) == len(r.prompt)
             out = self._run(r.request_id, part, [len(part) - 1] if last else [])
+            r.fed += len(part)                               # not before: a portion that could not run (PoolFull) is the next one again
             if not last:
                 return
         else:
