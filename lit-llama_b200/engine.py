@@ -3,13 +3,14 @@
 A model plugs in through three members: `state_specs()` (what a sequence carries between steps), `vocab`, and
 `forward_portion(tokens, ctx, want)` (run the next tokens of one sequence from the state earlier steps left,
 return f32 logits at the wanted places); one that books memory of its own for a slot (pages of a cache) is told by
-`release_slot(slot)` when its request is gone.  The engine owns the `SequenceStatePool`, maps request ids to slots,
+`release_slot(slot)` when its request is gone, and may be asked `has_room(live, tokens, portion)` (slot -> the tokens that its sequence grows to)
+before a request of `tokens` tokens is let in beside the live ones.  The engine owns the `SequenceStatePool`, maps request ids to slots,
 and offers two ways in:
 
   * `step(entries, end)`: the caller decides which tokens each request gets in this step (a replayed trace,
     an external scheduler);
   * `add_request()` + `run()` / `generate()`: the engine's own scheduler: waiting requests are admitted while
-    slots and the token budget allow, prompts are fed in portions of at most `prefill_chunk` tokens, live
+    slots, the token budget and the model's memory allow, prompts are fed in portions of at most `prefill_chunk` tokens, live
     requests take turns (one portion or one decoded token per turn), finished ones give their slot back.
 
 Single-token steps are replayed as a CUDA graph once warm (slot and position are read on the device), and so are portions of a length that
@@ -23,7 +24,7 @@ import torch
 
 from . import replay
 from .mixers import StepContext
-from .state import PoolFull, SequenceStatePool
+from .state import PagesFull, PoolFull, SequenceStatePool
 
 
 @dataclass
@@ -200,9 +201,22 @@ class Engine:
                     if not self.live:
                         raise PoolFull(f"request {r.request_id!r} needs {need} tokens, the budget is {self.pool.max_tokens}")
                     break
+            if self.live and not self._room(r):              # (alone it is let in: it may end before its last token)
+                break
             self.waiting.popleft()
             self.pool.acquire(r.request_id)
             self.live[r.request_id] = r
+
+    def _room(self, r: Request) -> bool:
+        """Whether the model has memory for all of r beside all of the live requests."""
+        ask = getattr(self.model, "has_room", None)
+        if ask is None:
+            return True
+
+        def tokens(q: Request) -> int:                       # that are fed: not the last one that comes out
+            return len(q.prompt) + max(q.max_new_tokens - 1, 0)
+
+        return ask({self.pool.slot(rid): tokens(q) for rid, q in self.live.items()}, tokens(r), self.prefill_chunk)
 
     def _sample(self, logits: torch.Tensor, r: Request) -> int:
         if r.temperature <= 0.0:
@@ -230,16 +244,25 @@ class Engine:
             r.done = True
 
     def run(self) -> Dict[Hashable, List[int]]:
-        """Serve until every request is finished; request id -> generated tokens (the EOS token included)."""
+        """Serve until every request is finished; request id -> generated tokens (the EOS token included).  An exception leaves the requests where they are:
+        what was finished is kept for the run that ends."""
         while self.waiting or self.live:
             self._admit()
+            ran, full = False, None
             for rid in list(self.live):
                 r = self.live[rid]
-                self._turn(r)
+                try:
+                    self._turn(r)
+                except PagesFull as e:                       # its turn comes again, as long as others' give pages back
+                    full = e
+                    continue
+                ran = True
                 if r.done:
                     del self.live[rid]
                     self.pool.release(rid)
                     self.finished[rid] = r
+            if full is not None and not ran:
+                raise full
         out = {rid: r.output for rid, r in self.finished.items()}
         self.finished = {}
         return out

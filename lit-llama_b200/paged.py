@@ -16,12 +16,12 @@
 A token's key and value rows are quantised by themselves, per head: scale = max(max |x| (1 / c), 2^-126), code = round(x / scale), c = 448 (fp8, e4m3) or 127
 (int8).  A row that holds an infinity or NaN reads back as NaN.  A row whose weights sum to zero (it sees no key) attends to zeros.  Everything
 is a kernel of libb200seq (include/b2l_seq.h); CUDA only, no CPU fallback, no derivatives."""
-from typing import Dict, Hashable, List, Optional, Sequence, Tuple
+from typing import Dict, Hashable, List, Mapping, Optional, Sequence, Tuple
 
 import torch
 
 from . import _seqlib as S
-from .state import PoolFull
+from .state import PagesFull
 
 STORES = {"act": S.STORE_ACT, "fp8": S.STORE_E4M3, "int8": S.STORE_INT8}
 PAGES = (16, 32, 64, 128, 256)
@@ -112,6 +112,20 @@ class PagePool:
     def pages(self, request_id: Hashable) -> List[int]:
         return list(self._pages[request_id])
 
+    def most_pages(self, tokens: int, portion: int = 0) -> int:
+        """The most pages at a time of a sequence that grows to `tokens` tokens, at most `portion` of them in a step (0: any number)."""
+        whole = -(-tokens // self.page)
+        if not self.window:
+            return whole
+        reach = self.window - 1 + (min(portion, tokens) if portion else tokens)      # positions that a step's tokens see or are
+        return min(whole, -(-self.first // self.page) + (reach + 2 * self.page - 2) // self.page)
+
+    def has_room(self, live: Mapping[Hashable, int], tokens: int, portion: int = 0) -> bool:
+        """Whether one more sequence, of `tokens` tokens, finds its pages whatever the sequences of `live` (request id -> the tokens that it grows to) still
+        take.  Other sequences are counted with the pages that they have."""
+        held = sum(sum(p >= 0 for p in self._pages.get(rid, ())) for rid in live)
+        return len(self._free) + held >= sum(self.most_pages(n, portion) for n in live.values()) + self.most_pages(tokens, portion)
+
     def release(self, request_id: Hashable) -> None:
         self._free += [p for p in reversed(self._pages.pop(request_id)) if p >= 0]
         del self._length[request_id]
@@ -124,8 +138,8 @@ class PagePool:
         return [i for i, p in enumerate(self._pages[request_id]) if p >= 0 and i * self.page >= self.first and (i + 1) * self.page <= reach]
 
     def step(self, entries: Sequence[Tuple[Hashable, int]], *, width: int = 0) -> PagedStep:
-        """Books `n` more tokens for every (request id, n); ids that are not known begin a sequence.  Raises PoolFull, with nothing booked, where the pages
-        do not suffice."""
+        """Books `n` more tokens for every (request id, n); ids that are not known begin a sequence.  Raises PagesFull, with nothing booked, where the
+        pages do not suffice."""
         if len({rid for rid, _ in entries}) < len(entries):
             raise ValueError("page pool: a request comes twice in one step")
         if any(n < 0 for _, n in entries):
@@ -133,7 +147,7 @@ class PagePool:
         behind = {rid: self._behind(rid) for rid, _ in entries}
         need = sum(max(0, -(-(self._length.get(rid, 0) + n) // self.page) - len(self._pages.get(rid, ()))) for rid, n in entries)
         if need > len(self._free) + sum(len(b) for b in behind.values()):
-            raise PoolFull(f"{need} pages are needed, {len(self._free)} of {self.n_pages} are free")
+            raise PagesFull(f"{need} pages are needed, {len(self._free)} of {self.n_pages} are free")
         sequences = []
         for rid, _ in entries:
             for i in behind[rid]:

@@ -113,7 +113,8 @@ class PagedLLaMAModel:
     """The package's LLaMA behind the Engine's model interface with its keys and values in pages (paged.py), in bf16, e4m3 or int8: as many sequences at a
     time as there are slots, each with the pages that its length needs.  A model of MHA layers: every head has keys and values of its own.
 
-    `pages` of `page` tokens are shared by the sequences (as many again for every layer); a portion that finds none left raises PoolFull.  With `window` a
+    `pages` of `page` tokens are shared by the sequences (as many again for every layer).  The engine's scheduler lets a request wait until there are pages
+    for all of it; a portion that finds none left raises PagesFull (a PoolFull), and the sequence stands where it stood.  With `window` a
     token sees the last `window` positions and the first `first` ones, and a sequence keeps no pages for the others, so it may grow without end; else
     it may have `max_positions` (default: the model's block size)."""
     graph_safe = False     # pages are booked on the host
@@ -138,6 +139,14 @@ class PagedLLaMAModel:
         """The engine's slot is free: so are its sequence's pages."""
         if self.pages.has(slot):
             self.pages.release(slot)
+
+    def has_room(self, live, tokens: int, portion: int) -> bool:
+        """Whether one more sequence, of `tokens` tokens, finds pages beside those of `live` (slot -> the tokens that its sequence grows to), fed at most
+        `portion` tokens at a time."""
+        def most(n: int) -> int:
+            return min(n, self.max_positions) if self.max_positions else n
+
+        return self.pages.has_room({slot: most(n) for slot, n in live.items()}, most(tokens), portion)
 
     def _rotated(self, x: torch.Tensor, ctx) -> torch.Tensor:
         """Every head of x [T, heads * size] (rows of a wider product) turned by position, pairs of neighbouring entries (lit_llama/model.py:306-323)."""

@@ -26,6 +26,10 @@ class PoolFull(RuntimeError):
     """No free slot, or the token budget of the pool is used up."""
 
 
+class PagesFull(PoolFull):
+    """No page is free at the moment: sequences that end, or whose windows move on, give some back."""
+
+
 class SequenceStatePool:
     def __init__(self, specs: Dict[str, StateSpec], n_slots: int, device: torch.device, max_tokens: int = 0,
                  on_release: Optional[Callable[[int], None]] = None) -> None:

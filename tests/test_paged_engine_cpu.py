@@ -57,3 +57,93 @@ def requests(*sizes):
 def test_a_portion_that_could_not_run_is_run_again(fails):
     asked = requests((40, 5), (33, 7), (16, 3))
     assert serve(Told(fails), asked, tries=len(fails) + 1) == serve(Told(), asked)
+
+
+class Paged(Told):
+    """The same with pages that all slots share."""
+
+    def __init__(self, n_pages, window=0, first=0):
+        super().__init__()
+        self.pages = PagePool(n_pages, 16, torch.device("cpu"), window=window, first=first)
+
+    def release_slot(self, slot):
+        if self.pages.has(slot):
+            self.pages.release(slot)
+
+    def has_room(self, live, tokens, portion):
+        return self.pages.has_room(live, tokens, portion)
+
+    def book(self, slot, pos0, n):
+        if pos0 == 0:
+            self.release_slot(slot)
+        assert pos0 == 0 or self.pages.position(slot) == pos0
+        self.pages.step([(slot, n)])
+
+
+@pytest.mark.parametrize("n_pages,window,first,sizes", [
+    (5, 0, 0, [(20, 40), (80, 1)]),                         # the second needs every page
+    (5, 0, 0, [(1, 80), (80, 1), (5, 3)]),
+    (6, 0, 0, [(16, 17), (17, 16), (40, 50), (90, 7), (1, 1)]),
+    (12, 0, 0, [(60, 60), (60, 60), (3, 100), (100, 3)]),
+    (6, 24, 2, [(23, 150), (70, 40), (5, 5)]),              # a window: pages for what it reaches
+    (11, 24, 2, [(23, 150), (70, 40), (5, 5), (33, 60)]),
+])
+def test_requests_wait_for_pages(n_pages, window, first, sizes):
+    """More slots than pages suffice for: everything is served, each request as it is alone, and all pages come back."""
+    asked = requests(*sizes)
+    model = Paged(n_pages, window, first)
+    assert serve(model, asked, n_slots=4) == serve(Told(), asked)
+    assert model.pages.free_pages() == n_pages
+
+
+def test_a_request_that_is_larger_than_all_pages():
+    """It runs by itself until the pages are used up and is then refused, as often as it is asked for; what was served before is not lost."""
+    model = Paged(5)
+    engine = P.Engine(model, n_slots=3, prefill_chunk=16)
+    for rid, (prompt, n) in requests((20, 4), (30, 100)).items():
+        engine.add_request(rid, prompt, n)
+    for _ in range(2):
+        with pytest.raises(PoolFull, match="pages"):
+            engine.run()
+    assert engine.finished[0].output == serve(Told(), requests((20, 4)))[0] and model.seen[0] and engine.live[1].fed == 30
+    assert not engine.live[1].done and len(engine.live[1].output) == 5 * 16 - 30 + 1
+
+
+@pytest.mark.parametrize("taken,enough", [(64, True), (80, False)])
+def test_pages_that_another_user_of_the_pool_has_for_a_while(taken, enough):
+    """A request that finds no page waits while others run; where nothing runs the shortage is reported, and nothing of any request is lost."""
+    asked = requests((31, 20), (18, 14))                    # 4 and 2 pages: the first is at its third long before the second ends
+    model = Paged(8)
+    engine = P.Engine(model, n_slots=2, prefill_chunk=16)
+    for rid, (prompt, n) in asked.items():
+        engine.add_request(rid, prompt, n)
+    engine._admit()
+    model.pages.step([("elsewhere", taken)])                # booked after both were let in
+    if not enough:
+        with pytest.raises(PoolFull, match="pages"):
+            engine.run()
+        model.pages.release("elsewhere")
+    assert engine.run() == serve(Told(), asked)
+
+
+@pytest.mark.parametrize("window,first", [(0, 0), (1, 0), (16, 0), (17, 3), (40, 16), (33, 17), (100, 130)])
+@pytest.mark.parametrize("portion", [1, 7, 16, 33])
+def test_the_most_pages_of_a_sequence(window, first, portion):
+    for total in (1, 15, 16, 17, 64, 100, 333):
+        p = PagePool(64, 16, torch.device("cpu"), window=window, first=first)
+        most, at = 0, 0
+        while at < total:
+            n = min(portion, total - at)
+            p.step([("a", n)])
+            at += n
+            most = max(most, 64 - p.free_pages())
+        assert most <= p.most_pages(total, portion) <= most + (1 + (first % 16 > 0) if window else 0)
+        assert p.most_pages(total, portion) <= p.most_pages(total)
+
+
+def test_room_beside_others():
+    p = PagePool(8, 16, torch.device("cpu"))
+    assert p.has_room({}, 128) and not p.has_room({}, 129)
+    p.step([("a", 20), ("other", 1)])                       # a has 2 pages and will have 4; other has 1
+    assert p.has_room({"a": 64}, 48) and not p.has_room({"a": 64}, 49)
+    assert p.has_room({"a": 64, "new": 16}, 32) and not p.has_room({"a": 64, "new": 17}, 32)
