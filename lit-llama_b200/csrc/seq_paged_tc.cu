@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
       const int b = lane & (boxes - 1), x = lane / boxes, r = __shfl_sync(0xffffffffu, row, b);      // 24 boxes at most
       if (x < (HALF ? 3 : ka)) {
         if (HALF) {
-          const int at = r < gone ? r : 0;                   // of a page that is not there: any scales
+          const int at = r < gone ? r : 0;                   // of a page that is not there: any scales, which nobody takes
           if (x == 0) tma_load_2d(raw_k + b * box * a.K, &map_k, 0, r, k_to);
           else bulk(smem_u32((x == 1 ? scales.k : scales.v) + b * box), (x == 1 ? a.ks : a.vs) + at, 4 * box, k_to);
         } else {
@@ -597,7 +597,10 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
           mbar_wait_warp(bar(ct.rk_full), tile & 1u, dead);
           if (dead) break;
           const float ks = scales.k[me], vs = scales.v[me];
-          const bool valid = me < keys.end - keys.key0(t, 7);      // behind the last key that is seen there may be anything
+          // A key that some row sees: behind the last one and before the windows there may be anything, and of a page that is not there the scales are those of
+          // another place (`there` was written before the copies were asked for)
+          const int j = keys.key0(t, 7) + me;
+          const bool valid = j < keys.end && (j >= keys.lo || j < keys.early) && (*reinterpret_cast<volatile uint32_t*>(&info.there) >> (me / 16) & 1u);
           if (t == x.t0) {
             if (valid && ks >= SMALLEST_SCALE && ks <= 1.f / SMALLEST_SCALE) atomicMax(&ct.k_ref[ref], __float_as_uint(ks));
             if (valid && vs >= SMALLEST_SCALE && vs <= 1.f / SMALLEST_SCALE) atomicMax(&ct.v_ref[ref], __float_as_uint(vs));
@@ -609,7 +612,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
             if (me == 0) ct.k_ref[ref == 0 ? 2 : ref - 1] = ct.v_ref[ref == 0 ? 2 : ref - 1] = 0u;      // the ones before, which all have read: for the ones after the next
             ref = ref == 2 ? 0 : ref + 1;
           }
-          uint2 k_by = factor(ks, k_up), v_by = valid ? factor(vs, v_up) : make_uint2(0u, 0u);
+          uint2 k_by = valid ? factor(ks, k_up) : make_uint2(0u, 0u), v_by = valid ? factor(vs, v_up) : make_uint2(0u, 0u);
           if (v_by.x == NO) {                                // a row that sees this key is computed again: its scores say so
             k_by = v_by;
             v_by = make_uint2(0u, 0u);
