@@ -218,19 +218,25 @@ class PagedCache:
         return sum(t.numel() * t.element_size() for t in self._pool if t is not None)
 
     # ------------------------------------------------------------------ calls (of every layer and step: some 5 us each beside the launches)
-    def _rows(self, x: torch.Tensor, heads: int, size: int, step: PagedStep, what: str) -> torch.Tensor:
-        """x [rows, heads, size] as the kernels take it: entries of a head consecutive, rows on 16-byte borders (else a copy)."""
+    def _rows(self, x: torch.Tensor, heads: int, size: int, step: PagedStep, what: str) -> Tuple[torch.Tensor, int, int]:
+        """x [rows, heads, size] as the kernels take it, entries of a head consecutive and rows on 16-byte borders (else a copy), with the entries between its
+        rows and between its heads."""
         shape = x.shape
         if len(shape) != 3 or shape[2] != size or (heads and shape[1] != heads) or x.dtype is not self.dtype or x.device != self.device:
             raise ValueError(f"paged cache: {what} {tuple(shape)} {x.dtype} on {x.device}, [rows, {heads or 'heads'}, {size}] {self.dtype} on {self.device} is wanted")
         if shape[0] < step.rows:
             raise ValueError(f"paged cache: {what} has {shape[0]} rows, the step {step.rows}")
         s0, s1, s2 = x.stride()
+        if shape[1] == 1:                                                   # of one head or row: whatever torch says
+            s1 = size
+        if shape[0] == 1:
+            s0 = shape[1] * size
         if s2 != 1 or s0 % self._per or s1 % self._per or x.data_ptr() % 16:
             x = x.contiguous()
             if x.data_ptr() % 16:
-                x = x.clone()
-        return x
+                x = x.clone(memory_format=torch.contiguous_format)
+            s0, s1 = shape[1] * size, size
+        return x, s0, s1
 
     def _call(self, name: str, step: PagedStep, *args) -> None:
         if step.device != self.device:
@@ -249,9 +255,8 @@ class PagedCache:
     def write(self, k: torch.Tensor, v: torch.Tensor, step: PagedStep) -> None:
         """The step's keys [rows, kv_heads, dim] and values [rows, kv_heads, vdim] into the pool.  Rows behind the step's last sequence are not looked at.
         Two rows of one step must not have the same place (a page in two sequences' tables, both writing there)."""
-        k, v = self._rows(k, self.kv_heads, self.dim, step, "keys"), self._rows(v, self.kv_heads, self.vdim, step, "values")
-        k0, k1, _ = k.stride()
-        v0, v1, _ = v.stride()
+        k, k0, k1 = self._rows(k, self.kv_heads, self.dim, step, "keys")
+        v, v0, v1 = self._rows(v, self.kv_heads, self.vdim, step, "values")
         self._call("b2l_seq_paged_write", step, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, *(self._at or ()), *(step._at or ()), min(k.shape[0], v.shape[0]), step.seqs, *self._sizes)
 
     def read(self, step: PagedStep) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -271,7 +276,7 @@ class PagedCache:
         q [rows, heads, dim] with heads a multiple of kv_heads (head h reads key/value head h // (heads / kv_heads)), p the position of row r; scale
         dim^-1/2 unless given.  Returns [rows, heads, vdim] (`out`, contiguous, where given); rows of no sequence, behind the step's last one or before its first,
         are zeros, or as they were in `out`."""
-        q = self._rows(q, 0, self.dim, step, "queries")
+        q, s0, s1 = self._rows(q, 0, self.dim, step, "queries")
         rows, heads, _ = q.shape
         plan = step._plans.get((rows, heads, scale, window, first, self._sizes))
         if plan is None:
@@ -283,7 +288,6 @@ class PagedCache:
         elif out.shape != (rows, heads, self.vdim) or out.dtype != self.dtype or out.device != self.device or not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError(f"paged cache: out must be {(rows, heads, self.vdim)} {self.dtype} on {self.device}, contiguous and 16-byte aligned")
         work = step._tensors[1].new_empty((floats,)) if floats else None          # four bytes an entry
-        s0, s1, _ = q.stride()
         self._call(name, step, q.data_ptr(), s0, s1, *(self._at or ()), *(step._at or ()), out.data_ptr(), work.data_ptr() if floats else None, floats, *sizes)
         return out
 

@@ -264,3 +264,18 @@ def test_the_oracle_sees_what_the_formula_says():
         for h in range(2):
             w = torch.exp(0.3 * k @ q[i, h].double())
             torch.testing.assert_close(got[i, h], (w[:, None] * v).sum(0) / w.sum(), rtol=1e-12, atol=1e-12)
+
+
+@pytest.mark.parametrize("rows,heads", [(1, 4), (1, 1), (5, 1), (5, 4)])
+def test_rows_as_the_kernels_take_them(rows, heads):
+    """Whatever the strides: entries of a head consecutive, tokens and heads at multiples of 16 bytes, and the values are the same."""
+    c, s = cache(), PagedStep.of([(rows, rows, [0])], CPU)
+    wide = torch.randn(rows + 1, heads * 32 + 11).to(torch.bfloat16)
+    flat = torch.randn(rows * heads * 33 + 1).to(torch.bfloat16)
+    for x in (wide[:rows, :heads * 32].unflatten(1, (heads, 32)), wide[1:, 1:1 + heads * 32].unflatten(1, (heads, 32)), flat[1:1 + rows * heads * 32].view(rows, heads, 32),
+              flat[:-1].view(rows, heads, 33)[..., :32], flat[:-1].view(rows, heads, 33)[..., 1:], flat[:rows * heads * 32].view(heads, rows, 32).transpose(0, 1),
+              flat[:rows * heads * 32].view(rows, 32, heads).transpose(1, 2), flat[:32].expand(rows, heads, 32), flat[1:33].expand(rows, heads, 32)):
+        y, s0, s1 = c._rows(x, heads, 32, s, "rows")
+        assert s0 % 8 == 0 and s1 % 8 == 0 and y.data_ptr() % 16 == 0
+        at = y.storage_offset()
+        assert torch.equal(torch.as_strided(y, (rows, heads, 32), (s0, s1, 1), at), x)
