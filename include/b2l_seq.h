@@ -497,7 +497,8 @@ int b2l_seq_mlstm_readout(const b2l_seq_mlstm_args* a, b2l_stream_t stream);
  * tokens long with them (device int32 [seqs]), and its token j lies in page table[b*ldt + j/page], place j%page (device int32, `width` entries per
  * sequence).  The row starts[b]+i is at position lengths[b] - (rows of b) + i.  These are read on the device and clipped to rows, width and pages; a
  * table entry outside the pool is a page that is not there (and so is every negative position's): nothing is written to it, it reads as zeros, and no
- * row sees its keys.  A row of no sequence is left out: nothing is written for it, and its outputs stay as they are (where not said otherwise).
+ * row sees its keys.  A row of no sequence is left out: nothing is written for it, and its outputs stay as they are (where not said otherwise).  A call
+ * without rows or without sequences does nothing; what has no entries may be null then.
  *
  *   b2l_seq_paged_write      new rows into the pool; 8-bit: scale = max(max |x| (1 / c), 2^-126), code = round(x / scale) to nearest even, c = 448 (e4m3) or
  *                            127 (int8), per token and head (of keys and of values); a row with an infinity or NaN gets the scale NaN and codes 0

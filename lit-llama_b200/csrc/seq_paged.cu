@@ -229,7 +229,7 @@ template <bool WRITE>
 static int rows_call(const char* who, const void* k_new, long long ldk, long long hsk, const void* v_new, long long ldv, long long hsv, void* k, void* v, float* ks, float* vs,
                      const int* starts, const int* lengths, const int* table, int ldt, int width, int rows, int seqs, int pages, int page, int kv_heads, int K, int V, int store,
                      int act_dtype, b2l_stream_t stream) {
-  B2L_CHECK_ARG(k_new && v_new, "%s: null pointer", who);
+  B2L_CHECK_ARG(rows == 0 || (k_new && v_new), "%s: null pointer", who);
   if (int rc = check_pool(who, k, v, ks, vs, starts, lengths, table, ldt, width, rows, seqs, pages, page, kv_heads, K, V, store, act_dtype)) return rc;
   const int per = act_dtype == B2L_F32 ? 4 : 8;
   B2L_CHECK_ARG((((uintptr_t)k_new | (uintptr_t)v_new) & 15) == 0 && ldk % per == 0 && hsk % per == 0 && ldv % per == 0 && hsv % per == 0,

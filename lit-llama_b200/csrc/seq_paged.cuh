@@ -56,7 +56,7 @@ __device__ __forceinline__ float2 e4m3_pair(uint32_t w) {
 // ---- host
 inline int check_pool(const char* who, const void* k, const void* v, const void* ks, const void* vs, const int* starts, const int* lengths, const int* table, int ldt, int width,
                       int rows, int seqs, int pages, int page, int kv_heads, int K, int V, int store, int act_dtype) {
-  B2L_CHECK_ARG(k && v && starts && lengths && table, "%s: null pointer", who);
+  B2L_CHECK_ARG(k && v && (rows == 0 || seqs == 0 || (starts && lengths && table)), "%s: null pointer", who);      // empty tensors have no address
   B2L_CHECK_SUPPORTED(act_dtype == B2L_BF16 || act_dtype == B2L_F32, "%s: act_dtype %d unsupported", who, act_dtype);
   B2L_CHECK_SUPPORTED(store == ACT || store == E4M3 || store == INT8, "%s: store %d unsupported", who, store);
   B2L_CHECK_ARG(store == ACT || (ks && vs), "%s: an 8-bit pool needs its scales", who);

@@ -792,7 +792,7 @@ static int attention(const char* who, bool zeros, const void* q, long long ldq, 
                      int page, int heads, int kv_heads, int K, int V, int window, int first, float scale, int max_new, int max_length, int store, int act_dtype,
                      b2l_stream_t stream) {
   using namespace paged;
-  B2L_CHECK_ARG(q && out, "%s: null pointer", who);
+  B2L_CHECK_ARG(rows == 0 || (q && out), "%s: null pointer", who);
   if (int rc = check_pool(who, k, v, k_scale, v_scale, starts, lengths, table, ldt, width, rows, seqs, pages, page, kv_heads, K, V, store, act_dtype)) return rc;
   B2L_CHECK_ARG(heads > 0 && heads % kv_heads == 0, "%s: %d heads over %d key/value heads", who, heads, kv_heads);
   B2L_CHECK_ARG(window >= 0 && first >= 0, "%s: a negative window or number of first tokens", who);

@@ -263,7 +263,8 @@ class PagedCache:
         """The rows that `write` with this step puts into the pool, as they lie there: keys [rows, kv_heads, dim] and values in the activation type; zeros where the
         step's tensors have no sequence for a row."""
         G, K, V = self.kv_heads, self.dim, self.vdim
-        k, v = self._like.new_empty((step.rows, G, K)), self._like.new_empty((step.rows, G, V))
+        make = self._like.new_empty if step.seqs else self._like.new_zeros
+        k, v = make((step.rows, G, K)), make((step.rows, G, V))
         self._call("b2l_seq_paged_read", step, k.data_ptr(), G * K, K, v.data_ptr(), G * V, V, *(self._at or ()), *(step._at or ()), step.rows, step.seqs, *self._sizes)
         return k, v
 
@@ -284,7 +285,7 @@ class PagedCache:
         floats, sizes = plan
         name = "b2l_seq_paged_attention"
         if out is None:
-            out, name = q.new_empty((rows, heads, self.vdim)), "b2l_seq_paged_attention_all"      # which rows have a sequence is known on the device only
+            out, name = (q.new_empty if step.seqs else q.new_zeros)((rows, heads, self.vdim)), "b2l_seq_paged_attention_all"      # which rows have a sequence is known on the device only
         elif out.shape != (rows, heads, self.vdim) or out.dtype != self.dtype or out.device != self.device or not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError(f"paged cache: out must be {(rows, heads, self.vdim)} {self.dtype} on {self.device}, contiguous and 16-byte aligned")
         work = step._tensors[1].new_empty((floats,)) if floats else None          # four bytes an entry

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from test_gpu_paged import DEV, IDS, TYPES, check, gen, make
+from test_gpu_paged_rows import poison, step_of
 
 pytestmark = pytest.mark.gpu
 
@@ -66,3 +67,36 @@ def test_one_row_of_many_as_a_slice():
     cache.write(x, x, step)
     assert all(torch.equal(y, x) for y in cache.read(step))
     check(cache.attend(x, step), x.cpu(), cache, seqs, 32 ** -0.5)
+
+
+@pytest.mark.parametrize("dtype,store", [TYPES[0], TYPES[1], TYPES[3]], ids=[IDS[0], IDS[1], IDS[3]])
+def test_steps_without_rows(dtype, store):
+    """No sequences, or sequences without new tokens: nothing is written, and the results are empty."""
+    from lit_llama_b200 import PagePool
+
+    cache, _, _ = make(dtype, store, 2, 64, 32, 16, [(1, 40)])
+    before = [x.clone() for x in cache._pool if x is not None]
+    pool = PagePool(8, 16, DEV)
+    k, v, q = (torch.empty(0, h, d, dtype=dtype, device=DEV) for h, d in ((2, 64), (2, 32), (4, 64)))
+    for entries in ([], [("a", 0)], [("a", 0), ("b", 0)]):
+        step = pool.step(entries)
+        cache.write(k, v, step)
+        assert [tuple(x.shape) for x in cache.read(step)] == [(0, 2, 64), (0, 2, 32)]
+        assert cache.attend(q, step).shape == (0, 4, 32)
+        out = torch.empty(0, 4, 32, dtype=dtype, device=DEV)
+        assert cache.attend(q, step, out=out) is out
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(before, (x for x in cache._pool if x is not None)))
+    # rows behind a step without any
+    some = torch.ones(3, 4, 64, dtype=dtype, device=DEV)
+    cache.write(some[:, :2], some[:, :2, :32].contiguous(), step)
+    poison((3, 4, 32), dtype=dtype)
+    assert cache.attend(some, step).shape == (3, 4, 32) and not cache.attend(some, step).any()
+
+
+@pytest.mark.parametrize("dtype,store", [TYPES[0], TYPES[1], TYPES[3]], ids=[IDS[0], IDS[1], IDS[3]])
+def test_a_step_without_sequences_is_zeros(dtype, store):
+    cache, _, _ = make(dtype, store, 2, 64, 32, 16, [(1, 40)])
+    step = step_of([0], [], 6)
+    poison((6, 4, 32), (6, 2, 64), (6, 2, 32), dtype=dtype)
+    assert not cache.attend(torch.ones(6, 4, 64, dtype=dtype, device=DEV), step).any()
+    assert not any(x.any() for x in cache.read(step))

@@ -279,3 +279,12 @@ def test_rows_as_the_kernels_take_them(rows, heads):
         assert s0 % 8 == 0 and s1 % 8 == 0 and y.data_ptr() % 16 == 0
         at = y.storage_offset()
         assert torch.equal(torch.as_strided(y, (rows, heads, 32), (s0, s1, 1), at), x)
+
+
+@pytest.mark.parametrize("name", ["write", "read", "attention"])
+def test_the_c_entries_have_nothing_to_do_without_rows_or_sequences(name):
+    """Empty tensors have no address; sizes are looked at all the same."""
+    none = dict(x=None, y=None, starts=None, lengths=None, table=None)
+    assert call(name, **none) == 0 and call(name, rows=3, seqs=0, starts=None, lengths=None, table=None) == 0
+    for kw in (dict(page=24), dict(K=24), dict(seqs=-1), dict(kv_heads=0), dict(act=2)):
+        assert call(name, **dict(none, **kw)) < 0, kw
