@@ -689,7 +689,9 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
       }
       fence_proxy_async();
      }
-     mbar_arrive(bar(ct.q_full));
+     // A warp whose wait ran out (rows that others compute again, key by key, can take longer) says nothing any more: it no longer keeps pace, and arrivals of
+     // its later row tiles would stand for those of a warp that still has to come, whose queries were then multiplied before they are there
+     if (!dead) mbar_arrive(bar(ct.q_full));
     }
     float m = -INFINITY, l = 0.f, down = 1.f;
     bool odd = false;

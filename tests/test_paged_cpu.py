@@ -288,3 +288,34 @@ def test_the_c_entries_have_nothing_to_do_without_rows_or_sequences(name):
     assert call(name, **none) == 0 and call(name, rows=3, seqs=0, starts=None, lengths=None, table=None) == 0
     for kw in (dict(page=24), dict(K=24), dict(seqs=-1), dict(kv_heads=0), dict(act=2)):
         assert call(name, **dict(none, **kw)) < 0, kw
+
+
+@pytest.mark.parametrize("seed", range(20))
+def test_queries_are_multiplied_only_when_all_warps_have_them_there(seed):
+    """csrc/seq_paged_tc.cu: eight softmax warps arrive at one barrier for every row tile.  One of them takes long over a row tile's outputs (rows computed again),
+    others' waits may run out meanwhile: they go on without waiting, and what they do must not complete a row tile's phase before the slow one has come."""
+    source = open(os.path.join(os.path.dirname(paged.__file__), "csrc", "seq_paged_tc.cu")).read()
+    arrivals = re.findall(r"(if \(!dead\) )?mbar_arrive\(bar\(ct\.q_full\)\)", source)
+    assert len(arrivals) == 1
+    guarded, rng, warps, tiles = bool(arrivals[0]), random.Random(seed), 8, 4
+    slow, slow_at = rng.randrange(warps), rng.randrange(tiles - 1)
+    gave_up, came, phase, count = [False] * warps, [0] * warps, 0, 0          # came: row tiles whose queries the warp has put there
+    released = False
+    for _ in range(2000):
+        w = rng.randrange(warps)
+        if came[w] == tiles:
+            continue
+        if came[w] > phase and not gave_up[w]:                                 # waits for the products of its row tile
+            if rng.random() < 0.1 and not released and came[slow] == slow_at + 1:
+                gave_up[w] = w != slow
+            continue
+        if w == slow and came[w] == slow_at + 1 and not released:              # still at the outputs of the row tile before
+            released = rng.random() < 0.02
+            continue
+        came[w] += 1
+        if guarded and gave_up[w]:
+            continue
+        count += 1
+        if count == warps:
+            assert min(came) > phase, (came, phase)
+            phase, count = phase + 1, 0
