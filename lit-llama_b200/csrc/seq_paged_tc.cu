@@ -20,7 +20,9 @@
 // 8-bit pools: queries as f16 times a power of two per row.  The scale s of a key or value goes into its codes: code times s 2^e rounded to f16 (2^-11), e such
 // that the largest s of the CTA's first 128 keys of a row tile comes to 1 .. 2; the scores and the outputs times 2^-e.  (A key's scale times its scores instead, without that
 // rounding: every thread needs all of them, 128 KB of reads from shared memory for a tile; 2048 tokens over 16384 keys took 750 us.)  A row that sees a scale
-// above 2^7 or below 2^-12 of that, or one that is not finite, is computed again.
+// above 2^7 of that, or one that is not finite, is computed again.  A scale below 2^-12 of that is off by up to 2^-25 (c 2^-25 for its key or value, c the largest
+// code), which beside others of the size is nothing.  Where a CTA met one, a row is computed again if it is not nothing: a score's error K 2^15 c 2^-25 cr may
+// be above 2^-10, or the row's largest output is so small that c 2^-25 is above 2^-12 of it.
 //
 // Tensor memory: scores and weights of the row tiles at columns 0 and 128, outputs at 256 and 384.  Shared memory: the queries of both, two stages of keys
 // and values where they fit (8-bit: of keys, and a tile of codes).  One CTA per SM, which goes through row tiles: the next one's first keys are fetched while the
@@ -63,6 +65,7 @@ struct Walk {
 struct Control {
   uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_half[2][2], o_done[2], info_full[INFOS], tail, gave_up;
   uint64_t ref_full, rk_full, rk_empty, rv_full, rv_empty;   // 8-bit pools: the first tile's largest scales, codes of keys and values
+  uint32_t small;                                            // 8-bit pools: whether the CTA met a scale of a key (1), a value (2) below 2^-12 of the largest
   uint32_t tmem, k_ref[3], v_ref[3];                         // largest scales of the first tile's keys and values, as bits, of a row tile, the next and the one before
   long long x0, x1;                                          // the CTA's part
   Walk at[20];                                               // each warp's row tile
@@ -406,6 +409,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
     mbar_init(bar(ct.rk_empty), 128);
     mbar_init(bar(ct.rv_empty), 128);
     for (int i = 0; i < 3; ++i) ct.k_ref[i] = ct.v_ref[i] = 0u;
+    ct.small = 0u;
     mbar_init_fence();
   }
   if (warp == 0) tmem_alloc(smem_u32(&ct.tmem), 512);
@@ -579,13 +583,16 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
       int st = 0, ref = 0;
       uint32_t ph = 1, tile = 0, item = 0;
       float k_up = 1.f, v_up = 1.f;
-      // the factor in two f16, twice each: as precise as 22 bits, or steps of 2^-25 (2^-13 of the smallest); NaN where the scale is out of range; 0 for a row of
+      // the factor in two f16, twice each: as precise as 22 bits, or steps of 2^-25 (2^-13 of a factor of 2^-12); NaN where the scale is out of range; 0 for a row of
       // zeros (2^-126) or one never written (0)
       constexpr uint32_t NO = 0x7e007e00u;
-      auto factor = [](float scale, float up) {
+      auto factor = [&](float scale, float up, uint32_t which) {
         const float s = scale * up;
         if (scale >= 0.f && scale <= 1.17549435e-38f) return make_uint2(0u, 0u);
-        if (!(s >= 2.44140625e-4f && s <= 128.f)) return make_uint2(NO, NO);
+        if (!(s >= 2.44140625e-4f && s <= 128.f)) {
+          if (!(s >= 0.f && s <= 128.f)) return make_uint2(NO, NO);
+          atomicOr(&ct.small, which);
+        }
         const __half hi = __float2half_rn(s), lo = __float2half_rn(s - __half2float(hi));
         return make_uint2(__half_as_ushort(hi) * 0x10001u, __half_as_ushort(lo) * 0x10001u);
       };
@@ -612,7 +619,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
             if (me == 0) ct.k_ref[ref == 0 ? 2 : ref - 1] = ct.v_ref[ref == 0 ? 2 : ref - 1] = 0u;      // the ones before, which all have read: for the ones after the next
             ref = ref == 2 ? 0 : ref + 1;
           }
-          uint2 k_by = valid ? factor(ks, k_up) : make_uint2(0u, 0u), v_by = valid ? factor(vs, v_up) : make_uint2(0u, 0u);
+          uint2 k_by = valid ? factor(ks, k_up, 1u) : make_uint2(0u, 0u), v_by = valid ? factor(vs, v_up, 2u) : make_uint2(0u, 0u);
           if (v_by.x == NO) {                                // a row that sees this key is computed again: its scores say so
             k_by = v_by;
             v_by = make_uint2(0u, 0u);
@@ -807,7 +814,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
       fence_after();
       if (dead || odd) l = NAN;
       const float inv = part ? down : l == 0.f ? 0.f : down / l;
-      bool fine = true;
+      float peak = 0.f;                                      // the row's largest output, NaN if one is
       const int slot = 2 * (int)blockIdx.x + (t0 == 0 ? 1 : 0), place = !live ? -1 : part ? slot * ROWS + TILE * g + r : row * a.heads + head;      // of the row's outputs
       // Outputs through the warp's rows of the queries (every score of this row tile is done), 128 bytes of each row at a time; then eight lanes along a row (a
       // row per lane took 9500 cycles)
@@ -822,7 +829,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
 #pragma unroll
           for (int i = 0; i < 16; ++i) x[i] = dead ? NAN : n > 0 ? __uint_as_float(o[i]) * inv : 0.f;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) fine = fine && fabsf(x[i]) < INFINITY;
+          for (int i = 0; i < 16; i += 2) peak = max3(peak, fabsf(x[i]), fabsf(x[i + 1]));
           if (part) {
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
@@ -853,10 +860,15 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
         }
         __syncwarp();
       }
+      if constexpr (HALF) {
+        constexpr float LARGEST = STORE == E4M3 ? 448.f : 127.f;
+        const uint32_t small = n > 0 ? *reinterpret_cast<volatile uint32_t*>(&ct.small) : 0u;
+        if (small && l > 0.f && (((small & 1u) && cr * (float)a.K * LARGEST > 1.f) || ((small & 2u) && !(peak >= LARGEST * 1.220703125e-4f * down * (part ? l : 1.f))))) l = NAN;
+      }
       if (part) *reinterpret_cast<float2*>(a.many.ml + 2 * (slot * ROWS + TILE * g + r)) = make_float2(m, l);
       if (!part) {
         __syncwarp();
-        for (uint32_t left = __ballot_sync(0xffffffffu, live && !(fine && fabsf(l) < INFINITY)); left; left &= left - 1) {
+        for (uint32_t left = __ballot_sync(0xffffffffu, live && !(peak < INFINITY && fabsf(l) < INFINITY)); left; left &= left - 1) {
           const int i = __ffs(left) - 1;
           mend_row(a, pl.b, __shfl_sync(0xffffffffu, pos, i), __shfl_sync(0xffffffffu, row, i), __shfl_sync(0xffffffffu, head, i), lane);
         }

@@ -4,6 +4,7 @@ import math
 import pytest
 import torch
 
+import paged_oracle as O
 from test_gpu_paged import DEV, IDS, TYPES, check, gen, make
 
 pytestmark = pytest.mark.gpu
@@ -53,3 +54,45 @@ def test_keys_before_every_window_bring_no_scales(dtype, store, sequences, windo
         results.append(cache.attend(q.to(DEV), step, window=window, first=first))
     check(results[0], q, cache, seqs, 0.125, window, first)
     assert all(torch.equal(r, results[0]) for r in results[1:])
+
+
+@pytest.mark.parametrize("store", ["fp8", "int8"])
+@pytest.mark.parametrize("sequences", [[(90, 700)], [(120, 500), (1, 300), (40, 40)]])
+@pytest.mark.parametrize("where,exponent", [("early", -20), ("early", -14), ("early", 9), ("early", 15), ("early", 30), ("late", 9), ("late", 30), ("late", 70), ("rising", 1), ("falling", 1),
+                                            ("most", -13), ("most", -30), ("none", 0)])
+def test_scales_far_from_the_others(store, sequences, where, exponent):
+    """Values, keys and both whose scales are far from the others' at one place, at most places, or rise and fall along the sequence."""
+    for which in ("k", "v", "kv"):
+        cache, step, seqs = make(torch.bfloat16, store, 2, 64, 32, 16, sequences)
+        for name in which:
+            t = cache.k_scale if name == "k" else cache.v_scale
+            by = 2.0 ** (exponent / 4 if name == "k" and exponent > 0 and where in ("early", "late") else exponent)      # (a key's makes its scores large)
+            for new, length, pages in seqs:
+                for j in range(length):
+                    at = (pages[j // 16], slice(None), j % 16)
+                    if where == "early" and j == 3 or where == "late" and j == length - new // 2 - 1 or where == "most" and j >= 5:
+                        t[at] *= by
+                    elif where in ("rising", "falling"):
+                        t[at] *= 2.0 ** ((j if where == "rising" else length - j) * (4 if name == "k" else 40) / length - (4 if name == "k" else 20))
+                    elif where == "none" and j < 140:
+                        t[at] = 0.0
+        q = torch.randn(step.rows, 8, 64, generator=gen(4)).to(torch.bfloat16)
+        got = cache.attend(q.to(DEV), step)
+        want, mag, dots = O.attend(q, cache, seqs, 0.125)
+        # Beside the roundings relative to each entry (weights, codes times scales, outputs):
+        #   a small scale's factor is off by 2^-25 where the largest of the sequence, which a row need not see, is 1 .. 2: c 2^-25 for an entry (c the largest code) and
+        #   2^-24 for two roundings of a product below f16's normal numbers; a row whose largest output is so small that this is more than 2^-12 of it is computed in f32
+        #   the same of keys changes a score by up to 2^-10, and so does its reference; else the row is computed in f32
+        #   weights are in f16, the largest at least 2^6, so each is off by half the least step, 2^-25, whatever its size: 2^-31 of the sum of the values' absolute values
+        c = O.LARGEST[store]
+
+        def seen(x):                                                             # [pages, heads, page, ..] of each row's keys, one after the other
+            return [torch.cat(list(x.cpu()[torch.tensor(pages)].transpose(1, 2)))[:length].double() for _, length, pages in seqs]
+
+        largest = torch.cat([x.amax(0).expand(new, 2) for x, (new, _, _) in zip(seen(cache.v_scale), seqs)]).repeat_interleave(4, 1)[..., None]
+        total = torch.cat([x.abs().cumsum(0)[length - new:] for x, (new, length, _) in zip(seen(O.values(cache, "v")), seqs)]).repeat_interleave(4, 1)
+        peak = want.abs().amax(-1, keepdim=True)
+        tol = O.tolerance(want, mag, dots, 64, 700, False, store) + torch.minimum((c * 2.0 ** -25 + 2.0 ** -24) * largest, 2.0 ** -12 * peak) + 2.0 ** -31 * total
+        tol = tol + ("k" in which) * 2 * 2.0 ** -10 * mag + 2.0 ** -133        # (and bf16's least step)
+        off = (got.cpu().double() - want).abs()
+        assert bool((off <= tol).all()), (which, float((off / tol).max()))
