@@ -605,10 +605,8 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
   }
   if (a.few.splits == 1) {
     __syncthreads();
-    for (uint32_t left = bad; left; left &= left - 1) {
-      const int r = __ffs(left) - 1, at = pl.first + r;
-      if (r % W == warp) mend_row(a, pl.b, pl.length - pl.n + at / G, pl.start + at / G, h * G + at % G, lane);
-    }
+    const uint32_t own = (W == 4 ? 0x11111111u : W == 2 ? 0x55555555u : 0xffffffffu) << warp;      // every W-th row
+    if (bad & own) mend_rows<4>(a, pl.b, pl.start, pl.length - pl.n, h, pl.first, bad & own, lane);
   }
 }
 
@@ -692,7 +690,8 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const __g
     __syncwarp();
     int start, n, length;
     sequence(a.s, b, start, n, length);
-    mend_row(a, b, length - n + row - start, row, head, lane);
+    const int G = a.heads / a.kv_heads;
+    mend_rows<4>(a, b, start, length - n, head / G, (row - start) * G + head % G, 1u, lane);
   }
 }
 

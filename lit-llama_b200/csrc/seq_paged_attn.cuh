@@ -131,11 +131,29 @@ struct Attn {
     else st_act4(reinterpret_cast<__nv_bfloat16*>(out) + at, y);
   }
 
-  __device__ __forceinline__ float element(const void* p, const float* scales, size_t row, int D, int d) const {
-    const size_t at = row * D + d;
-    if (store_kind == ACT) return f32 ? reinterpret_cast<const float*>(p)[at] : bf2f(reinterpret_cast<const __nv_bfloat16*>(p)[at]);
-    const uint8_t c = reinterpret_cast<const uint8_t*>(p)[at];
-    return (store_kind == E4M3 ? e4m3_pair(c).x : (float)(int8_t)c) * scales[row];
+  // eight entries from `at` on, of the activation type (scale: none) or codes
+  __device__ __forceinline__ void eight(const void* p, size_t at, const float* scale, float (&x)[8]) const {
+    if (scale == nullptr) {
+      float4 u, v;
+      if (f32) {
+        u = ld_act4(reinterpret_cast<const float*>(p) + at);
+        v = ld_act4(reinterpret_cast<const float*>(p) + at + 4);
+      } else {
+        u = ld_act4(reinterpret_cast<const __nv_bfloat16*>(p) + at);
+        v = ld_act4(reinterpret_cast<const __nv_bfloat16*>(p) + at + 4);
+      }
+      x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+      return;
+    }
+    const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(p) + at);
+    const float s = *scale;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const uint32_t u = (i < 4 ? w.x : w.y) >> 8 * (i & 2);
+      const float2 y = store_kind == E4M3 ? e4m3_pair(u) : make_float2((float)(int8_t)u, (float)(int8_t)(u >> 8));
+      x[i] = y.x * s;
+      x[i + 1] = y.y * s;
+    }
   }
 };
 
@@ -146,48 +164,118 @@ static __device__ __noinline__ void clear_rows(const Attn& a, int r0, int r1, in
     *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(a.out) + ((size_t)(r0 + i / pieces) * a.heads + head) * a.V * es + i % pieces * 16) = make_uint4(0u, 0u, 0u, 0u);
 }
 
-// One row and head again by a warp, key after key over what the row sees and nothing else.  The products above multiply a hidden value by a weight of
-// zero, and an f32 infinity has parts of NaN: a result that is not finite is computed again here, so it is what the formula says.
-static __device__ __noinline__ void mend_row(const Attn& a, int b, int pos, int row, int head, int lane) {
-  const int h = head / (a.heads / a.kv_heads);
-  float q[8], o[8], m = -INFINITY, l = 0.f;
+// Rows and heads of one sequence and key/value head, again by a warp, over what each sees and nothing else, in f32.  The products above multiply a hidden value by
+// a weight of zero, and an f32 infinity has parts of NaN: a result that is not finite is computed again here, so it is what the formula says.
+// 32 keys at a time, of which a lane has one for the scores, and then 8 entries of every value, for MENDED rows together: four, and two in the chunk kernel, which
+// with more spills registers in its loops.  All of 512 tokens' rows again, 32 / 8 heads of 128 over 4096 keys of an int8 pool: 11.3 ms (78 with a row at a time, key
+// after key); one token's over 16384 keys 9.6 ms (37).  Where all of a row is NaN it stays so, and the rest is left out: 1.7 and 0.4 ms with a NaN among the first.
+template <int MENDED> struct Again { int n, pos[MENDED], row[MENDED], head[MENDED]; };
+template <int MENDED> __device__ __forceinline__ void mend_few(const Attn& a, int b, int h, const Again<MENDED>& x, int lane) {
+  float m[MENDED], l[MENDED], o[MENDED][8];
+  int p_min = x.pos[0], p_max = x.pos[0];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int d = lane + 32 * i;
-    const size_t at = (size_t)row * a.ldq + (size_t)head * a.hsq + d;
-    q[i] = d < a.K ? (a.f32 ? reinterpret_cast<const float*>(a.q)[at] : bf2f(reinterpret_cast<const __nv_bfloat16*>(a.q)[at])) : 0.f;
-    o[i] = 0.f;
+  for (int r = 0; r < MENDED; ++r) {
+    if (r < x.n) {
+      p_min = min(p_min, x.pos[r]);
+      p_max = max(p_max, x.pos[r]);
+    }
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[r][e] = 0.f;
   }
-  for (int j = 0; j <= pos; ++j) {
-    if (!a.sees(pos, j)) {
-      j = max(j, pos - a.window);                            // the next key is the window's first
+  for (int j0 = 0; j0 <= p_max; j0 += 32) {
+    if (a.window && j0 >= a.first && j0 + 31 <= p_min - a.window) {      // on to the first window
+      j0 = ((p_min - a.window + 1) & ~31) - 32;
       continue;
     }
-    const int page = page_of(a.s, b, j);
-    if (page < 0) continue;
-    const size_t at = (((size_t)page * a.kv_heads + h) << a.s.shift) + (j & ((1 << a.s.shift) - 1));
-    float x = 0.f;
+    const int j = j0 + lane;
+    bool any = false;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < a.K) x = fmaf(q[i], a.element(a.k, a.ks, at, a.K, lane + 32 * i), x);
-    x = warp_sum(x) * a.scale_log2;
-    if (x == -INFINITY) continue;
-    const float now = fmaxf(m, x), f = m == now ? 1.f : exp2_f(m - now), w = exp2_f(x - now);
-    m = now;
-    l = l * f + w;
+    for (int r = 0; r < MENDED; ++r) any |= r < x.n && a.sees(x.pos[r], j);
+    const int page = any ? page_of(a.s, b, j) : -1;
+    const size_t at = (((size_t)max(page, 0) * a.kv_heads + h) << a.s.shift) + (j & ((1 << a.s.shift) - 1));
+    float w[MENDED] = {};
+    if (page >= 0)
+      for (int d = 0; d < a.K; d += 8) {
+        float k[8];
+        a.eight(a.k, at * a.K + d, a.store_kind == ACT ? nullptr : a.ks + at, k);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < a.V) o[i] = o[i] * f + w * a.element(a.v, a.vs, at, a.V, lane + 32 * i);
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+        for (int r = 0; r < MENDED; ++r) {
+          if (r >= x.n) break;
+          float q[8];
+          a.eight(a.q, (size_t)x.row[r] * a.ldq + (size_t)x.head[r] * a.hsq + d, nullptr, q);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int d = lane + 32 * i;
-    const size_t at = ((size_t)row * a.heads + head) * a.V + d;
-    if (d < a.V) {
-      if (a.f32) reinterpret_cast<float*>(a.out)[at] = o[i] * inv;
-      else reinterpret_cast<__nv_bfloat16*>(a.out)[at] = f2bf(o[i] * inv);
+          for (int e = 0; e < 8; ++e) w[r] = fmaf(q[e], k[e], w[r]);
+        }
+      }
+    bool has = false;                                        // whether the key has a weight in some row; a weight of -1: it is not seen
+#pragma unroll
+    for (int r = 0; r < MENDED; ++r) {
+      if (r >= x.n) break;
+      const float s = page >= 0 && a.sees(x.pos[r], j) ? w[r] * a.scale_log2 : -INFINITY;
+      float now = s;
+#pragma unroll
+      for (int y = 16; y > 0; y >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, y));
+      now = fmaxf(now, m[r]);
+      const float f = m[r] == now ? 1.f : exp2_f(m[r] - now);
+      m[r] = now;
+      w[r] = s == -INFINITY ? -1.f : exp2_f(s - now);
+      has |= s != -INFINITY;
+      l[r] = l[r] * f + warp_sum(s == -INFINITY ? 0.f : w[r]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[r][e] *= f;
     }
+    const uint32_t mine = __ballot_sync(0xffffffffu, has);
+#pragma unroll 2
+    for (int i = 0; i < 32; ++i) {
+      if (!(mine >> i & 1u)) continue;
+      const size_t of = __shfl_sync(0xffffffffu, (unsigned long long)at, i);
+      float v[8] = {};
+      if (8 * lane < a.V) a.eight(a.v, of * a.V + 8 * lane, a.store_kind == ACT ? nullptr : a.vs + of, v);
+#pragma unroll
+      for (int r = 0; r < MENDED; ++r) {
+        const float y = __shfl_sync(0xffffffffu, w[r], i);
+        if (r < x.n && !(y < 0.f))
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[r][e] = fmaf(y, v[e], o[r][e]);
+      }
+    }
+    bool over = true;                                        // all of every row is NaN
+#pragma unroll
+    for (int r = 0; r < MENDED; ++r) {
+      bool nan = true;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) nan = nan && o[r][e] != o[r][e];
+      over = over && (r >= x.n || l[r] != l[r] || 8 * lane >= a.V || nan);
+    }
+    if (__all_sync(0xffffffffu, over)) break;
+  }
+#pragma unroll
+  for (int r = 0; r < MENDED; ++r) {
+    if (r >= x.n || 8 * lane >= a.V) break;
+    const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+    const size_t at = ((size_t)x.row[r] * a.heads + x.head[r]) * a.V + 8 * lane;
+    const float lo[4] = {o[r][0], o[r][1], o[r][2], o[r][3]}, hi[4] = {o[r][4], o[r][5], o[r][6], o[r][7]};
+    a.store(at, lo, inv);
+    a.store(at + 4, hi, inv);
+  }
+}
+// Packed rows at + i of sequence b and key/value head h, for the bits i of `left`; its rows begin at `start`, its new tokens at position `pos`
+template <int MENDED> static __device__ __noinline__ void mend_rows(const Attn& a, int b, int start, int pos, int h, int at, uint32_t left, int lane) {
+  const int G = a.heads / a.kv_heads;
+  while (left) {
+    Again<MENDED> x;
+    x.n = min(__popc(left), MENDED);
+#pragma unroll
+    for (int r = 0; r < MENDED; ++r) {
+      const int i = at + (left ? __ffs(left) - 1 : 0);       // (one too many is not looked at)
+      left &= left - 1;
+      x.pos[r] = pos + i / G;
+      x.row[r] = start + i / G;
+      x.head[r] = h * G + i % G;
+    }
+    mend_few<MENDED>(a, b, h, x, lane);
   }
 }
 __device__ __forceinline__ bool finite4(const float (&x)[4], float inv) {

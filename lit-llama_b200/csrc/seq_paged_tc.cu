@@ -868,10 +868,8 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
       if (part) *reinterpret_cast<float2*>(a.many.ml + 2 * (slot * ROWS + TILE * g + r)) = make_float2(m, l);
       if (!part) {
         __syncwarp();
-        for (uint32_t left = __ballot_sync(0xffffffffu, live && !(peak < INFINITY && fabsf(l) < INFINITY)); left; left &= left - 1) {
-          const int i = __ffs(left) - 1;
-          mend_row(a, pl.b, __shfl_sync(0xffffffffu, pos, i), __shfl_sync(0xffffffffu, row, i), __shfl_sync(0xffffffffu, head, i), lane);
-        }
+        const uint32_t bad = __ballot_sync(0xffffffffu, live && !(peak < INFINITY && fabsf(l) < INFINITY));
+        if (bad) mend_rows<2>(a, pl.b, pl.start, pl.length - pl.n, x.h, pl.first + TILE * g + (warp & 3) * 32, bad, lane);
       }
     }
     if (n > 0) {
@@ -931,17 +929,17 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
       x[k] = make_float4(x[k].x * f + w * z[k].x, x[k].y * f + w * z[k].y, x[k].z * f + w * z[k].z, x[k].w * f + w * z[k].w);
     }
   }
+  uint32_t bad = 0u;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     if (r0 + k >= rows) break;
     const int at = last.y + r0 + k, row = start + at / G, head = last.z * G + at % G;
     const float inv = L[k] == 0.f ? 0.f : 1.f / L[k], y[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
     if (4 * lane < a.V) a.store(((size_t)row * a.heads + head) * a.V + 4 * lane, y, inv);
-    if (!__all_sync(0xffffffffu, finite4(y, inv) && fabsf(L[k]) < INFINITY)) {
-      __syncwarp();
-      mend_row(a, last.x, length - n + at / G, row, head, lane);
-    }
+    if (!__all_sync(0xffffffffu, finite4(y, inv) && fabsf(L[k]) < INFINITY)) bad |= 1u << k;
   }
+  __syncwarp();
+  if (bad) mend_rows<2>(a, last.x, start, length - n, last.z, last.y + r0, bad, lane);
 }
 
 int many_ctas(long long row_tiles, long long keys, int sms) {
