@@ -4,7 +4,8 @@ A model plugs in through three members: `state_specs()` (what a sequence carries
 `forward_portion(tokens, ctx, want)` (run the next tokens of one sequence from the state earlier steps left,
 return f32 logits at the wanted places); one that books memory of its own for a slot (pages of a cache) is told by
 `release_slot(slot)` when its request is gone, and may be asked `has_room(live, tokens, portion)` (slot -> the tokens that its sequence grows to)
-before a request of `tokens` tokens is let in beside the live ones.  The engine owns the `SequenceStatePool`, maps request ids to slots,
+before a request of `tokens` tokens is let in beside the live ones; where several engines may have it, `for_engine()` gives each the object that it calls, with
+slots of its own.  The engine owns the `SequenceStatePool`, maps request ids to slots,
 and offers two ways in:
 
   * `step(entries, end)`: the caller decides which tokens each request gets in this step (a replayed trace,
@@ -50,7 +51,7 @@ class Engine:
     portion_graphs: int = 4
 
     def __init__(self, model, *, n_slots: int = 4, max_tokens: int = 0, prefill_chunk: int = 512, device: Optional[torch.device] = None) -> None:
-        self.model = model
+        self.model = model = model.for_engine() if hasattr(model, "for_engine") else model
         self.device = torch.device(device) if device is not None else model.device
         self.pool = SequenceStatePool(model.state_specs(), n_slots, self.device, max_tokens=max_tokens, on_release=getattr(model, "release_slot", None))
         self.prefill_chunk = int(prefill_chunk)

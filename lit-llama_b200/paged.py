@@ -102,6 +102,9 @@ class PagePool:
     def has(self, request_id: Hashable) -> bool:
         return request_id in self._pages
 
+    def requests(self) -> List[Hashable]:
+        return list(self._pages)
+
     def free_pages(self) -> int:
         return len(self._free)
 

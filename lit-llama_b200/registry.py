@@ -1,8 +1,10 @@
 """Model registry: config.json's "architecture" picks the loader, as `llama_model_lookup` picks a LLaMA size from
 a checkpoint.  A loader returns an object the Engine can serve (state_specs / vocab / dtype / device /
 forward_portion)."""
+import copy
 import json
 import os
+import weakref
 from typing import Callable, Dict, Optional
 
 import torch
@@ -109,6 +111,11 @@ class LLaMASequenceModel:
         return (logits if want is None else logits.index_select(0, want.to(torch.int64))).float()
 
 
+def _release_all(pages, owner) -> None:
+    for request_id in [r for r in pages.requests() if isinstance(r, tuple) and r and r[0] is owner]:
+        pages.release(request_id)
+
+
 class PagedLLaMAModel:
     """The package's LLaMA behind the Engine's model interface with its keys and values in pages (paged.py), in bf16, e4m3 or int8: as many sequences at a
     time as there are slots, each with the pages that its length needs.  A model of MHA layers: every head has keys and values of its own.
@@ -131,14 +138,31 @@ class PagedLLaMAModel:
         self.pages = PagePool(pages, page, self.device, window=self.window, first=self.first)
         self.caches = [PagedCache.empty(pages, page, self.heads, self.size, dtype=self.dtype, store=store, device=self.device) for _ in range(cfg.n_layer)]
         self.freq = (1.0 / 10000 ** (torch.arange(0, self.size, 2, dtype=torch.float32) / self.size)).to(self.device)
+        self._owner = object()                              # whose slots these are: the model's own, or an engine's
+
+    def for_engine(self) -> "PagedLLaMAModel":
+        """The same weights and pages with slots of its own, which an engine has: engines that share a model number their slots alike.  Pages of an engine that is
+        gone are free.  Pages that one gives back another takes, so engines that share a model run on one stream."""
+        view = copy.copy(self)
+        view._owner = object()
+        weakref.finalize(view, _release_all, self.pages, view._owner).atexit = False
+        return view
 
     def state_specs(self):
         return {}
 
     def release_slot(self, slot: int) -> None:
         """The engine's slot is free: so are its sequence's pages."""
-        if self.pages.has(slot):
-            self.pages.release(slot)
+        if self.pages.has((self._owner, slot)):
+            self.pages.release((self._owner, slot))
+
+    def book(self, slot: int, pos0: int, n: int):
+        """The step of a slot's next n tokens, at position pos0 of its sequence; a slot at position 0 begins a new one."""
+        if pos0 == 0:
+            self.release_slot(slot)
+        elif not self.pages.has((self._owner, slot)) or self.pages.position((self._owner, slot)) != pos0:
+            raise RuntimeError(f"paged LLaMA: slot {slot} is not at position {pos0}")
+        return self.pages.step([((self._owner, slot), n)])
 
     def has_room(self, live, tokens: int, portion: int) -> bool:
         """Whether one more sequence, of `tokens` tokens, finds pages beside those of `live` (slot -> the tokens that its sequence grows to), fed at most
@@ -146,7 +170,7 @@ class PagedLLaMAModel:
         def most(n: int) -> int:
             return min(n, self.max_positions) if self.max_positions else n
 
-        return self.pages.has_room({slot: most(n) for slot, n in live.items()}, most(tokens), portion)
+        return self.pages.has_room({(self._owner, slot): most(n) for slot, n in live.items()}, most(tokens), portion)
 
     def _rotated(self, x: torch.Tensor, ctx) -> torch.Tensor:
         """Every head of x [T, heads * size] (rows of a wider product) turned by position, pairs of neighbouring entries (lit_llama/model.py:306-323)."""
@@ -164,12 +188,8 @@ class PagedLLaMAModel:
         from .model import _add
 
         slot, pos0 = (ctx.slot_hint, ctx.pos_hint) if ctx.slot_hint is not None else ctx.meta.tolist()
-        if pos0 == 0:
-            self.release_slot(slot)
-        elif not self.pages.has(slot) or self.pages.position(slot) != pos0:
-            raise RuntimeError(f"paged LLaMA: slot {slot} is not at position {pos0}")
         T, C = tokens.numel(), self.heads * self.size
-        step = self.pages.step([(slot, T)])
+        step = self.book(slot, pos0, T)
         tokens = tokens.to(torch.int64).contiguous()
         wte = self.model.transformer.wte.weight
         x = torch.empty((1, T, C), dtype=self.dtype, device=self.device)

@@ -1,4 +1,4 @@
-"""GPU: the LLaMA with its pages behind engines that share them: requests that wait for pages."""
+"""GPU: the LLaMA with its pages behind engines that share them: requests that wait for pages, engines side by side."""
 import pytest
 
 import lit_llama_b200 as P
@@ -28,3 +28,25 @@ def test_requests_wait_for_pages(kw, pages):
         engine.add_request(r, p, 20)
     assert engine.run() == alone(model, 20, **kw)
     assert paged.pages.free_pages() == pages
+
+
+def test_two_engines_side_by_side():
+    """Both have their request in slot 0, at the same positions, and take turns."""
+    import torch
+
+    model = llama()
+    prompts = [PROMPT, PROMPT[::-1]]
+    want = []
+    for p in prompts:
+        engine = P.Engine(P.PagedLLaMAModel(model, pages=12, page=16), n_slots=1)
+        want.append(torch.cat([engine.step([dict(id=0, tokens=part, want=list(range(len(part))))])[0] for part in (p[:9], p[9:17], p[17:18], p[18:])]))
+    paged = P.PagedLLaMAModel(model, pages=12, page=16)
+    engines, got = [P.Engine(paged, n_slots=1) for _ in prompts], [[], []]
+    for i, j in ((0, 9), (9, 17), (17, 18), (18, 23)):
+        for engine, p, out in zip(engines, prompts, got):
+            out += engine.step([dict(id=0, tokens=p[i:j], want=list(range(j - i)))])
+    for a, b in zip(got, want):
+        assert torch.equal(torch.cat(a), b)
+    assert paged.pages.free_pages() == 8
+    del engine, engines
+    assert paged.pages.free_pages() == 12

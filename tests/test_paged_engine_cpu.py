@@ -147,3 +147,51 @@ def test_room_beside_others():
     p.step([("a", 20), ("other", 1)])                       # a has 2 pages and will have 4; other has 1
     assert p.has_room({"a": 64}, 48) and not p.has_room({"a": 64}, 49)
     assert p.has_room({"a": 64, "new": 16}, 32) and not p.has_room({"a": 64, "new": 17}, 32)
+
+
+def paged_llama(**kw):
+    """A PagedLLaMAModel whose pages can be looked at without a device."""
+    from types import SimpleNamespace as N
+
+    config = N(padded_vocab_size=96, n_head=2, n_embd=32, n_layer=1, block_size=64)
+    wte = torch.nn.Embedding(96, 32, dtype=torch.bfloat16)
+    return P.PagedLLaMAModel(N(config=config, transformer=N(wte=wte), parameters=wte.parameters), **dict(dict(pages=8, page=16), **kw))
+
+
+def test_engines_that_share_a_model_have_slots_of_their_own():
+    model = paged_llama()
+    a, b = P.Engine(model, n_slots=2), P.Engine(model, n_slots=2)
+    for engine in (a, b):
+        engine.pool.acquire("r")
+        engine.model.book(0, 0, 20)                        # both in slot 0
+    assert model.pages.free_pages() == 4
+    assert not a.model.has_room({0: 64}, 48, 16) and a.model.has_room({0: 48}, 48, 16)      # the other engine's two pages are not free
+    b.model.book(0, 20, 20)
+    with pytest.raises(RuntimeError, match="position"):
+        a.model.book(0, 40, 1)
+    a.model.book(0, 20, 5)
+    a.pool.release("r")
+    assert model.pages.free_pages() == 5 and b.model.book(0, 40, 1).lengths.tolist() == [41]
+    b.pool.release("r")
+    assert model.pages.free_pages() == 8
+
+
+def test_an_engine_that_goes_gives_its_pages_back():
+    import gc
+
+    model = paged_llama()
+    a, b = P.Engine(model, n_slots=2), P.Engine(model, n_slots=2)
+    a.pool.acquire("r")
+    a.model.book(0, 0, 40)
+    b.pool.acquire("r")
+    b.model.book(0, 0, 20)
+    model.book(0, 0, 5)                                    # a caller's own, without an engine
+    assert model.pages.free_pages() == 2
+    del a
+    gc.collect()
+    assert model.pages.free_pages() == 5
+    del b
+    gc.collect()
+    assert model.pages.free_pages() == 7
+    model.release_slot(0)
+    assert model.pages.free_pages() == 8
