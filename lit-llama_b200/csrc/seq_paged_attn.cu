@@ -704,8 +704,12 @@ constexpr long long MOST_WORK = 1ll << 27;                   // floats of partia
 
 static long long few_floats(int splits, long long count, int V) { return splits > 1 ? (2 * splits * count + 3) / 4 * 4 + splits * count * V : 0; }
 
+// A window, or a number of first tokens, as long as all that a table holds.  (A position below zero less a longer window need not fit 32 bits.)
+static bool hides_nothing(int window, int first, int width, int page) { return std::max(window, first) >= (long long)width * page; }
+
 static Plan plan_of(int rows, int seqs, int width, int page, int heads, int kv_heads, int K, int V, int window, int first, int max_new, int max_length, int store, int act_dtype) {
   Plan p{};
+  if (hides_nothing(window, first, width, page)) window = first = 0;
   const int G = heads / kv_heads, sms = sm_count(), most = std::min(seqs, rows);
   // packed rows of the longest of the sequences; where the host says nothing, a token each if there are no more rows than sequences
   const long long packed = (long long)rows * G, longest = (long long)(max_new > 0 ? std::min(max_new, rows) : rows <= seqs ? 1 : rows) * G;
@@ -801,6 +805,7 @@ static int attention(const char* who, bool zeros, const void* q, long long ldq, 
   B2L_CHECK_SUPPORTED((long long)width * page < (1ll << 30) && kv_heads < 65536 && (long long)rows * heads < (1ll << 31) - 65536 && (long long)pages * kv_heads * page < (1ll << 31),
                       "%s: sizes beyond the grid's or a copy's coordinates", who);
   if (rows == 0 || seqs == 0) return 0;
+  if (paged::hides_nothing(window, first, width, page)) window = first = 0;
   const Plan p = plan_of(rows, seqs, width, page, heads, kv_heads, K, V, window, first, max_new, max_length, store, act_dtype);
   B2L_CHECK_ARG(p.floats == 0 || (work && work_floats >= p.floats), "%s: a work space of %lld floats is needed", who, p.floats);
   Attn a{};

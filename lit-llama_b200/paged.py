@@ -301,6 +301,11 @@ class PagedCache:
             raise ValueError(f"paged cache: {heads} query heads over {self.kv_heads} key/value heads")
         if window < 0 or first < 0:
             raise ValueError("paged cache: a negative window or number of first tokens")
+        places = step.table.shape[1] * self.page                            # positions below it
+        if window >= places or first >= places:
+            window = 0                                                      # nothing is hidden
+        if not window:
+            first = 0
         sizes = (heads, self.kv_heads, self.dim, self.vdim, window, first)
         hints = (step.max_new, step.max_length) + self._codes
         floats = S.lib().b2l_seq_paged_attention_work(rows, step.seqs, step.table.shape[1], self.page, *sizes, *hints)

@@ -91,3 +91,25 @@ def test_a_recorded_step_that_covers_fewer_rows_later(dtype, store, new, heads):
     torch.cuda.synchronize()
     check(out[:2 * new], q[:2 * new], cache, seqs[:2], 0.125)
     assert not any(x[2 * new:].any() for x in (out, *back))
+
+
+@pytest.mark.parametrize("dtype,store", TYPES, ids=IDS)
+def test_windows_beyond_every_position(dtype, store):
+    """At positions below zero as well, where window and position together leave 32 bits; through the C entry itself, too."""
+    cache, step, seqs = make(dtype, store, 2, 64, 64, 16, [(40, 40), (300, 300), (1, 1), (200, 900)])
+    step.lengths.copy_(torch.tensor([7, 10, 0, 100], dtype=torch.int32))
+    q = torch.randn(step.rows, 8, 64, generator=gen(3)).to(dtype).to(DEV)
+    whole = cache.attend(q, step)
+    assert whole.any()
+    for window, first in ((16 * step.table.shape[1], 0), (2 ** 31 - 1, 0), (2 ** 31 - 1, 9), (2 ** 31, 0), (2 ** 32 + 5, 0), (3, 2 ** 31 - 1), (3, 2 ** 35)):
+        assert torch.equal(cache.attend(q, step, window=window, first=first), whole)
+    from lit_llama_b200 import _seqlib as S
+
+    for window, first in ((2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1), (3, 2 ** 31 - 1)):
+        sizes = (8, 2, 64, 64, window, first)
+        codes = (step.max_new, step.max_length) + cache._codes
+        floats = S.lib().b2l_seq_paged_attention_work(step.rows, step.seqs, step.table.shape[1], 16, *sizes, *codes)
+        work, out = torch.empty(max(floats, 1), device=DEV), torch.zeros_like(whole)
+        S.check(S.lib().b2l_seq_paged_attention(q.data_ptr(), 512, 64, *cache._at, *step._at, out.data_ptr(), work.data_ptr(), floats, step.rows, step.seqs, cache.n_pages, 16, *sizes,
+                                                0.125, *codes, S.stream_ptr()), "b2l_seq_paged_attention")
+        assert torch.equal(out, whole)

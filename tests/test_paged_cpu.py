@@ -319,3 +319,12 @@ def test_queries_are_multiplied_only_when_all_warps_have_them_there(seed):
         if count == warps:
             assert min(came) > phase, (came, phase)
             phase, count = phase + 1, 0
+
+
+def test_windows_and_first_tokens_beyond_every_position_are_none():
+    """A table of 4 pages of 16 has positions 0 .. 63: what is longer hides nothing, and what does not fit the C entry's int never reaches it."""
+    c, s = cache(), PagedStep.of([(2, 2, [0])], CPU, width=4)
+    whole = c._plan(2, 4, None, 0, 0, s)
+    assert c._plan(2, 4, None, 63, 3, s)[1][8:10] == (63, 3) and whole[1][8:10] == (0, 0)
+    for window, first in ((64, 0), (64, 3), (2 ** 31 - 1, 0), (2 ** 31, 7), (2 ** 32 + 5, 2 ** 40), (5, 64), (5, 2 ** 32 + 1)):
+        assert c._plan(2, 4, None, window, first, s) == whole
