@@ -130,6 +130,8 @@ class PagedLLaMAModel:
         from .paged import PagedCache, PagePool
 
         cfg = model.config
+        if model.transformer.wte.weight.dtype != torch.bfloat16:
+            raise RuntimeError(f"wte dtype {model.transformer.wte.weight.dtype} unsupported; the model must be bf16 (model.to(torch.bfloat16))")
         self.model, self.vocab, self.dtype = model, cfg.padded_vocab_size, torch.bfloat16
         self.device = next(model.parameters()).device
         self.heads, self.size = cfg.n_head, cfg.n_embd // cfg.n_head

@@ -195,3 +195,13 @@ def test_an_engine_that_goes_gives_its_pages_back():
     assert model.pages.free_pages() == 7
     model.release_slot(0)
     assert model.pages.free_pages() == 8
+
+
+def test_a_model_that_is_not_in_bf16_is_refused():
+    """Its embedding's bytes would be read as bf16."""
+    from types import SimpleNamespace as N
+
+    model = paged_llama().model
+    wte = torch.nn.Embedding(96, 32)
+    with pytest.raises(RuntimeError, match="float32"):
+        P.PagedLLaMAModel(N(config=model.config, transformer=N(wte=wte), parameters=wte.parameters), pages=8, page=16)
