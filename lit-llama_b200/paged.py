@@ -133,6 +133,15 @@ class PagePool:
         self._free += [p for p in reversed(self._pages.pop(request_id)) if p >= 0]
         del self._length[request_id]
 
+    def take_back(self, request_id: Hashable, n: int) -> None:
+        """The last n tokens that were booked for a sequence did not come: it is as long as it was, and pages of theirs alone are free again."""
+        if not 0 <= n <= self._length[request_id]:
+            raise ValueError(f"page pool: {n} tokens of {self._length[request_id]}")
+        self._length[request_id] -= n
+        pages, keep = self._pages[request_id], -(-self._length[request_id] // self.page)
+        self._free += [p for p in reversed(pages[keep:]) if p >= 0]
+        del pages[keep:]
+
     def _behind(self, request_id: Hashable) -> List[int]:
         """Places in the sequence's table that no later token sees."""
         if not self.window or request_id not in self._pages:
@@ -147,7 +156,7 @@ class PagePool:
             raise ValueError("page pool: a request comes twice in one step")
         if any(n < 0 for _, n in entries):
             raise ValueError("page pool: a negative number of tokens")
-        behind = {rid: self._behind(rid) for rid, _ in entries}
+        behind, new = {rid: self._behind(rid) for rid, _ in entries}, {rid for rid, _ in entries if rid not in self._pages}
         need = sum(max(0, -(-(self._length.get(rid, 0) + n) // self.page) - len(self._pages.get(rid, ()))) for rid, n in entries)
         if need > len(self._free) + sum(len(b) for b in behind.values()):
             raise PagesFull(f"{need} pages are needed, {len(self._free)} of {self.n_pages} are free")
@@ -162,7 +171,14 @@ class PagePool:
             while len(pages) * self.page < self._length[rid]:
                 pages.append(self._free.pop())
             sequences.append((n, self._length[rid], pages))
-        return PagedStep.of(sequences, self.device, width=width)
+        try:
+            return PagedStep.of(sequences, self.device, width=width)
+        except BaseException:                                               # no memory on the device
+            for rid, n in entries:
+                self.take_back(rid, n)
+                if rid in new:
+                    self.release(rid)
+            raise
 
 
 class PagedCache:

@@ -1,6 +1,7 @@
 """Model registry: config.json's "architecture" picks the loader, as `llama_model_lookup` picks a LLaMA size from
 a checkpoint.  A loader returns an object the Engine can serve (state_specs / vocab / dtype / device /
 forward_portion)."""
+import contextlib
 import copy
 import json
 import os
@@ -166,6 +167,16 @@ class PagedLLaMAModel:
             raise RuntimeError(f"paged LLaMA: slot {slot} is not at position {pos0}")
         return self.pages.step([((self._owner, slot), n)])
 
+    @contextlib.contextmanager
+    def booked(self, slot: int, pos0: int, n: int):
+        """The same for what runs inside: if it raises, the slot's sequence stands where it stood."""
+        step = self.book(slot, pos0, n)
+        try:
+            yield step
+        except BaseException:
+            self.pages.take_back((self._owner, slot), n)
+            raise
+
     def has_room(self, live, tokens: int, portion: int) -> bool:
         """Whether one more sequence, of `tokens` tokens, finds pages beside those of `live` (slot -> the tokens that its sequence grows to), fed at most
         `portion` tokens at a time."""
@@ -186,12 +197,15 @@ class PagedLLaMAModel:
 
     @torch.no_grad()
     def forward_portion(self, tokens: torch.Tensor, ctx, want: Optional[torch.Tensor] = None) -> torch.Tensor:
+        slot, pos0 = (ctx.slot_hint, ctx.pos_hint) if ctx.slot_hint is not None else ctx.meta.tolist()
+        with self.booked(slot, pos0, tokens.numel()) as step:
+            return self._portion(tokens, ctx, want, step)
+
+    def _portion(self, tokens: torch.Tensor, ctx, want: Optional[torch.Tensor], step) -> torch.Tensor:
         from . import _lib as L
         from .model import _add
 
-        slot, pos0 = (ctx.slot_hint, ctx.pos_hint) if ctx.slot_hint is not None else ctx.meta.tolist()
         T, C = tokens.numel(), self.heads * self.size
-        step = self.book(slot, pos0, T)
         tokens = tokens.to(torch.int64).contiguous()
         wte = self.model.transformer.wte.weight
         x = torch.empty((1, T, C), dtype=self.dtype, device=self.device)

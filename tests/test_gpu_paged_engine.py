@@ -50,3 +50,25 @@ def test_two_engines_side_by_side():
     assert paged.pages.free_pages() == 8
     del engine, engines
     assert paged.pages.free_pages() == 12
+
+
+def test_a_portion_that_fails_midway_can_be_run_again():
+    import torch
+
+    model = llama()
+    want = P.Engine(P.PagedLLaMAModel(model, pages=12, page=16), n_slots=1).step([dict(id=0, tokens=PROMPT, want=[22])])[0]
+    paged = P.PagedLLaMAModel(model, pages=12, page=16)
+    engine = P.Engine(paged, n_slots=1)
+    engine.step([dict(id=0, tokens=PROMPT[:9])])
+    last, attend = paged.caches[-1], paged.caches[-1].attend
+
+    def no_memory(*args, **kw):
+        raise torch.cuda.OutOfMemoryError("none left")
+    last.attend = no_memory
+    with pytest.raises(torch.cuda.OutOfMemoryError):
+        engine.step([dict(id=0, tokens=PROMPT[9:], want=[13])])
+    last.attend = attend
+    got = engine.step([dict(id=0, tokens=PROMPT[9:], want=[13])])[0]
+    assert float((got.double() - want.double()).norm() / want.double().norm()) < 0.012
+    engine.pool.release(0)
+    assert paged.pages.free_pages() == 12

@@ -205,3 +205,53 @@ def test_a_model_that_is_not_in_bf16_is_refused():
     wte = torch.nn.Embedding(96, 32)
     with pytest.raises(RuntimeError, match="float32"):
         P.PagedLLaMAModel(N(config=model.config, transformer=N(wte=wte), parameters=wte.parameters), pages=8, page=16)
+
+
+def test_a_portion_that_fails_after_its_pages_were_booked_can_be_run_again():
+    for window in (0, 24):
+        model = paged_llama(window=window)
+        for slot, lengths in ((0, [5]), (1, [20, 16, 7, 16])):
+            at = 0
+            for n in lengths:
+                model.book(slot, at, n)
+                at += n
+            free, pages = model.pages.free_pages(), model.pages.pages((model._owner, slot))
+            with pytest.raises(MemoryError):
+                with model.booked(slot, at, 30):
+                    raise MemoryError
+            kept = model.pages.pages((model._owner, slot))
+            assert model.pages.position((model._owner, slot)) == at and model.pages.free_pages() >= free
+            assert kept == [-1 if k < 0 else p for k, p in zip(kept, pages)]      # the same ones, but for those behind the window
+            with model.booked(slot, at, 30) as step:
+                assert step.lengths.tolist() == [at + 30]
+            model.release_slot(slot)
+        assert model.pages.free_pages() == 8
+
+
+def test_a_step_that_could_not_be_made_books_nothing(monkeypatch):
+    from lit_llama_b200 import PagedStep
+
+    p = PagePool(8, 16, torch.device("cpu"))
+    p.step([("a", 20)])
+    before = p.pages("a")
+
+    def none_left(*args, **kw):
+        raise MemoryError
+    with monkeypatch.context() as m:
+        m.setattr(PagedStep, "of", none_left)
+        with pytest.raises(MemoryError):
+            p.step([("a", 30), ("b", 17), ("c", 0)])
+    assert p.pages("a") == before and p.position("a") == 20 and p.requests() == ["a"] and p.free_pages() == 6
+    assert p.step([("a", 30), ("b", 17)]).lengths.tolist() == [50, 17]
+
+
+def test_tokens_that_did_not_come():
+    p = PagePool(8, 16, torch.device("cpu"))
+    p.step([("a", 20)])
+    p.step([("a", 40)])
+    with pytest.raises(ValueError):
+        p.take_back("a", 61)
+    p.take_back("a", 40)
+    assert p.position("a") == 20 and p.free_pages() == 6
+    p.take_back("a", 20)
+    assert p.position("a") == 0 and p.pages("a") == [] and p.free_pages() == 8
