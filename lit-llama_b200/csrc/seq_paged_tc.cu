@@ -21,8 +21,8 @@
 // that the largest s of the CTA's first 128 keys of a row tile comes to 1 .. 2; the scores and the outputs times 2^-e.  (A key's scale times its scores instead, without that
 // rounding: every thread needs all of them, 128 KB of reads from shared memory for a tile; 2048 tokens over 16384 keys took 750 us.)  A row that sees a scale
 // above 2^7 of that, or one that is not finite, is computed again.  A scale below 2^-12 of that is off by up to 2^-25 (c 2^-25 for its key or value, c the largest
-// code), which beside others of the size is nothing.  Where a CTA met one, a row is computed again if it is not nothing: a score's error K 2^15 c 2^-25 cr may
-// be above 2^-10, or the row's largest output is so small that c 2^-25 is above 2^-12 of it.
+// code), which beside others of the size is nothing.  Where a tile of a row's had one, the row is computed again if it is not nothing: a score's error K 2^15 c 2^-25
+// cr may be above 2^-10, or the row's largest output is so small that c 2^-25 is above 2^-12 of it.
 //
 // Tensor memory: scores and weights of the row tiles at columns 0 and 128, outputs at 256 and 384.  Shared memory: the queries of both, two stages of keys
 // and values where they fit (8-bit: of keys, and a tile of codes).  One CTA per SM, which goes through row tiles: the next one's first keys are fetched while the
@@ -53,7 +53,7 @@ constexpr int INFOS = 4;
 
 struct alignas(16) Info {                                    // of a tile of keys
   uint2 k_by[KEYS], v_by[KEYS];                              // 8-bit pools: what a key's and a value's codes are multiplied with
-  uint32_t there;                                            // 16 keys each: whether their page is there
+  uint32_t there;                                            // 16 keys each: whether their page is there; bits 8 and 9: whether a scale of a key, a value is below 2^-12 of the largest
   float k_up, v_up;                                          // 8-bit pools: powers of two that the scales were multiplied with
 };
 // A row tile: 256 packed rows of a head, the tiles of its sequence's rows one after the other, then the next head's, then the next sequence's
@@ -65,7 +65,6 @@ struct Walk {
 struct Control {
   uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_half[2][2], o_done[2], info_full[INFOS], tail, gave_up;
   uint64_t ref_full, rk_full, rk_empty, rv_full, rv_empty;   // 8-bit pools: the first tile's largest scales, codes of keys and values
-  uint32_t small;                                            // 8-bit pools: whether the CTA met a scale of a key (1), a value (2) below 2^-12 of the largest
   uint32_t tmem, k_ref[3], v_ref[3];                         // largest scales of the first tile's keys and values, as bits, of a row tile, the next and the one before
   long long x0, x1;                                          // the CTA's part
   Walk at[20];                                               // each warp's row tile
@@ -409,7 +408,6 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
     mbar_init(bar(ct.rk_empty), 128);
     mbar_init(bar(ct.rv_empty), 128);
     for (int i = 0; i < 3; ++i) ct.k_ref[i] = ct.v_ref[i] = 0u;
-    ct.small = 0u;
     mbar_init_fence();
   }
   if (warp == 0) tmem_alloc(smem_u32(&ct.tmem), 512);
@@ -586,12 +584,12 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
       // the factor in two f16, twice each: as precise as 22 bits, or steps of 2^-25 (2^-13 of a factor of 2^-12); NaN where the scale is out of range; 0 for a row of
       // zeros (2^-126) or one never written (0)
       constexpr uint32_t NO = 0x7e007e00u;
-      auto factor = [&](float scale, float up, uint32_t which) {
+      auto factor = [](float scale, float up, uint32_t which, uint32_t* notes) {
         const float s = scale * up;
         if (scale >= 0.f && scale <= 1.17549435e-38f) return make_uint2(0u, 0u);
         if (!(s >= 2.44140625e-4f && s <= 128.f)) {
           if (!(s >= 0.f && s <= 128.f)) return make_uint2(NO, NO);
-          atomicOr(&ct.small, which);
+          atomicOr(notes, which);
         }
         const __half hi = __float2half_rn(s), lo = __float2half_rn(s - __half2float(hi));
         return make_uint2(__half_as_ushort(hi) * 0x10001u, __half_as_ushort(lo) * 0x10001u);
@@ -619,7 +617,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
             if (me == 0) ct.k_ref[ref == 0 ? 2 : ref - 1] = ct.v_ref[ref == 0 ? 2 : ref - 1] = 0u;      // the ones before, which all have read: for the ones after the next
             ref = ref == 2 ? 0 : ref + 1;
           }
-          uint2 k_by = valid ? factor(ks, k_up, 1u) : make_uint2(0u, 0u), v_by = valid ? factor(vs, v_up, 2u) : make_uint2(0u, 0u);
+          uint2 k_by = valid ? factor(ks, k_up, 256u, &info.there) : make_uint2(0u, 0u), v_by = valid ? factor(vs, v_up, 512u, &info.there) : make_uint2(0u, 0u);
           if (v_by.x == NO) {                                // a row that sees this key is computed again: its scores say so
             k_by = v_by;
             v_by = make_uint2(0u, 0u);
@@ -701,7 +699,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
      if (!dead) mbar_arrive(bar(ct.q_full));
     }
     float m = -INFINITY, l = 0.f, down = 1.f;
-    bool odd = false;
+    uint32_t notes = 0;                                      // those of its tiles; bit 31: a score that is NaN or an infinity
     // positions of this group's rows: where all of them see a tile no mask is needed
     const int p_min = pl.length - pl.n + (pl.first + TILE * g) / G, p_max = pl.length - pl.n + (pl.first + min(TILE * (g + 1), rows) - 1) / G;
     if (g < groups) {
@@ -722,7 +720,8 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
           cr *= 1.f / info.k_up;
           down = 1.f / info.v_up;
         }
-        const bool whole = there == 0xffu && key0 + KEYS - 1 <= p_min && (a.window == 0 || key0 > p_max - a.window || key0 + KEYS <= a.first);
+        if (HALF) notes |= there;
+        const bool whole = (there & 0xffu) == 0xffu && key0 + KEYS - 1 <= p_min && (a.window == 0 || key0 > p_max - a.window || key0 + KEYS <= a.first);
         // keys that the row sees, as bits of 32
         auto seen = [&](int c) {
           const int j = key0 + 32 * c;
@@ -753,7 +752,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
           for (int i = 0; i < 64; i += 2) x4[i / 2 & 3] = max3(x4[i / 2 & 3], __uint_as_float(u[i]), __uint_as_float(u[i + 1]));
         }
         const float top = max3(max3(x4[0], x4[1], x4[2]), x4[3], -INFINITY) * cr;
-        if (!(top < INFINITY)) odd = true;                   // NaN or an infinity: the row is computed again
+        if (!(top < INFINITY)) notes |= 1u << 31;            // the row is computed again
         const bool grows = top > m + 8.f || (m == -INFINITY && top > m);
         if (__any_sync(0xffffffffu, grows)) {
           const float f = grows ? exp2_f(m - top) : 1.f;     // 0 where nothing was added yet
@@ -812,7 +811,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
       }
       if (n > 0) mbar_wait_warp(bar(ct.o_done[g]), own_items & 1u, dead);
       fence_after();
-      if (dead || odd) l = NAN;
+      if (dead || notes >> 31) l = NAN;
       const float inv = part ? down : l == 0.f ? 0.f : down / l;
       float peak = 0.f;                                      // the row's largest output, NaN if one is
       const int slot = 2 * (int)blockIdx.x + (t0 == 0 ? 1 : 0), place = !live ? -1 : part ? slot * ROWS + TILE * g + r : row * a.heads + head;      // of the row's outputs
@@ -862,8 +861,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
       }
       if constexpr (HALF) {
         constexpr float LARGEST = STORE == E4M3 ? 448.f : 127.f;
-        const uint32_t small = n > 0 ? *reinterpret_cast<volatile uint32_t*>(&ct.small) : 0u;
-        if (small && l > 0.f && (((small & 1u) && cr * (float)a.K * LARGEST > 1.f) || ((small & 2u) && !(peak >= LARGEST * 1.220703125e-4f * down * (part ? l : 1.f))))) l = NAN;
+        if (notes > 255u && l > 0.f && (((notes & 256u) && cr * (float)a.K * LARGEST > 1.f) || ((notes & 512u) && !(peak >= LARGEST * 1.220703125e-4f * down * (part ? l : 1.f))))) l = NAN;
       }
       if (part) *reinterpret_cast<float2*>(a.many.ml + 2 * (slot * ROWS + TILE * g + r)) = make_float2(m, l);
       if (!part) {

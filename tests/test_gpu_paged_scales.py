@@ -96,3 +96,21 @@ def test_scales_far_from_the_others(store, sequences, where, exponent):
         tol = tol + ("k" in which) * 2 * 2.0 ** -10 * mag + 2.0 ** -133        # (and bf16's least step)
         off = (got.cpu().double() - want).abs()
         assert bool((off <= tol).all()), (which, float((off / tol).max()))
+
+
+@pytest.mark.parametrize("store", ["fp8", "int8"])
+def test_far_scales_of_one_sequence_reach_no_other(store):
+    """Some hundred short sequences, several row tiles for every SM; every third has scales far below its others, and scores so large that this matters.  The same
+    bits every time, and those of the others whether or not it has."""
+    sequences = [(5 + i % 30, 40 + 7 * (i % 50)) for i in range(300)]
+    cache, step, seqs = make(torch.bfloat16, store, 8, 32, 32, 16, sequences)
+    q = (torch.randn(step.rows, 8, 32, generator=gen(4)) * 200).to(torch.bfloat16).to(DEV)
+    others = torch.cat([torch.full((n,), i % 3 != 1) for i, (n, _, _) in enumerate(seqs)])
+    usual = cache.attend(q, step)
+    for i in range(1, 300, 3):
+        for t in (cache.k_scale, cache.v_scale):
+            t[seqs[i][2][1]] *= 2.0 ** -14
+    first = cache.attend(q, step)
+    assert torch.equal(first.cpu()[others], usual.cpu()[others]) and not torch.equal(first, usual)
+    for _ in range(10):
+        assert torch.equal(cache.attend(q, step), first)
