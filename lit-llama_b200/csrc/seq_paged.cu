@@ -6,7 +6,7 @@
 // hides them.  1 / c is rounded to f32, and the division by s is the correctly rounded one, so the codes are the same wherever the formula is computed in f32.
 //
 // 16 lanes have a row of keys, the other 16 of the warp the row of values of the same token and head, each lane 8 elements at a time: 16-byte loads of bf16.
-// What bounds it: the write of prompts, 10367 tokens of 32 + 32 heads of 128 into int8 in 58 us or 4.4 TB/s, by its instructions (the issue is 77% busy:
+// What bounds it: the write of prompts, 10367 tokens of 32 + 32 heads of 128 into int8 in 58 us or 4.4 TB/s, by its instructions (the issue is 72% busy:
 // largest entry, quotients and codes); their read, 44056 tokens of 8 + 8 heads in 52 us, 5.3 TB/s, by HBM.  Single tokens: the launch and one chain of loads
 // (starts, length, table), 2.2 us for one, 3.2 us for 96.
 #include <math_constants.h>

@@ -637,7 +637,7 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const __g
   const bool on = b >= 0;
   float M = -INFINITY, L = 0.f;
   float4 x[2] = {};
-  pdl_wait();                                                // launched while the parts are computed
+  pdl_wait();                                                // launched as the last CTAs that compute parts end: they let nothing in earlier
   if (on) {
 #pragma unroll 4
     for (int i = sub; i < p.splits; i += per) {
@@ -719,7 +719,7 @@ static Plan plan_of(int rows, int seqs, int width, int page, int heads, int kv_h
   // The chunk kernel takes steps with a sequence of more than 16 packed rows.  Single tokens among them too, at up to 3.5 times the few-row kernel's time from
   // 8-bit pools and 1.3 times from bf16 ones, until what that adds is more than the 12 us of two more launches: a chunk of 512 with 8, 48 or 192 tokens of others
   // over 4096 keys of 8 heads takes 107, 184 or 381 us in both kernels from e4m3, 121, 332 or 1084 in the one; from bf16 with 48 or 192 215 and 573, or 210
-  // and 670.  There are at most `singles` of them.
+  // and 670.  There are at most `singles` of them.  (Heads of 128 in groups of four; other sizes were not measured.)
   long long singles = seqs;
   p.few_max = INT32_MAX;
   if (act_dtype == B2L_BF16 && longest > 16 && many_takes(K, V, store)) {
@@ -740,7 +740,8 @@ static Plan plan_of(int rows, int seqs, int width, int page, int heads, int kv_h
     p.few_count = (long long)rows * heads;
     singles = std::max<long long>(seqs, packed / p.few_rows);
   }
-  // An SM has three CTAs at a time.  Few CTAs: as many parts as fill them once, of 128 keys at least (one token over 1031 keys of 32 heads: 15.1 us in 4 parts,
+  // An SM has three CTAs at a time (with f32 rows, or heads beyond 128, two or one: then this takes up to three times the parts that fill it, or finds room for parts
+  // where there is none; chosen and measured for three).  Few CTAs: as many parts as fill them once, of 128 keys at least (one token over 1031 keys of 32 heads: 15.1 us in 4 parts,
   // 13.0 in 8).  Many: parts of a quarter of that each, of 512 keys at least, so that sequences of different lengths share the SMs evenly (48 over up to 8192
   // keys of an e4m3 pool: 143 us whole, 128 in 4 parts, 140 in 8)
   const long long ctas = (long long)kv_heads * singles, slots = 3ll * sms;

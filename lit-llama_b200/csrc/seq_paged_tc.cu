@@ -29,7 +29,7 @@
 // outputs of the last are stored.
 //
 // What bounds it, 2048 tokens over 16384 keys, 32 / 8 heads of 128: bf16 430 us, 1198 TFLOP/s, the tensor core 60% busy; the rest is each row tile's softmax,
-// which its next product waits for.  8-bit 646 us: a row tile waits for its values' codes as well (f16 twice in shared memory do not fit), and queries, keys,
+// which its next product waits for.  8-bit 650 us (e4m3; int8 695): a row tile waits for its values' codes as well (f16 twice in shared memory do not fit), and queries, keys,
 // values and codes keep shared memory's 128 bytes a cycle busy for some 2700 of a tile's 5600 cycles.  (8 warps for keys and values together: 731; with keys a
 // tile ahead 787.)
 #include <algorithm>
@@ -890,7 +890,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
 // The row tiles that go on from CTA blockIdx.x to others; a warp has four rows, a lane four columns of each
 __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ Attn a) {
   const int lane = threadIdx.x & 31, G = a.heads / a.kv_heads, r0 = blockIdx.y * 32 + threadIdx.x / 32 * 4;
-  pdl_wait();                                                // launched while the parts are computed
+  pdl_wait();                                                // launched as the last CTAs that compute parts end: they let nothing in earlier
   const int4 last = a.many.last[blockIdx.x];
   if (last.w < 2) return;
   int start, n, length;
