@@ -29,7 +29,7 @@
 // outputs of the last are stored.
 //
 // What bounds it, 2048 tokens over 16384 keys, 32 / 8 heads of 128: bf16 430 us, 1198 TFLOP/s, the tensor core 60% busy; the rest is each row tile's softmax,
-// which its next product waits for.  8-bit 650 us (e4m3; int8 695): a row tile waits for its values' codes as well (f16 twice in shared memory do not fit), and queries, keys,
+// which its next product waits for.  8-bit 645 us (e4m3; int8 690): a row tile waits for its values' codes as well (f16 twice in shared memory do not fit), and queries, keys,
 // values and codes keep shared memory's 128 bytes a cycle busy for some 2700 of a tile's 5600 cycles.  (8 warps for keys and values together: 731; with keys a
 // tile ahead 787.)
 #include <algorithm>
@@ -150,11 +150,30 @@ __device__ __forceinline__ uint4 ld128(uint32_t a) {
   return v;
 }
 __device__ __forceinline__ void st128(uint32_t a, uint4 v) { asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory"); }
+// Waits are bounded by time, some ten seconds: others may be computing rows again all the while (32 rows over 16384 keys take 0.1 s).  Counted in tries, one of them
+// lasts 40 ns or 4 us: a warp gave up after 0.15 s, and those that waited for it after 17 s.
+constexpr long long PATIENCE = 20'000'000'000;               // cycles
+__device__ __forceinline__ void wait_for(uint32_t a, uint32_t parity, uint32_t& dead) {
+  if (dead) return;
+  for (long long begin = 0;;) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(a), "r"(parity) : "memory");
+    if (ok) return;
+    const long long now = clock64();
+    if (begin == 0) begin = now;
+    if (now - begin > PATIENCE) break;
+  }
+  dead = 1u;
+}
+__device__ __forceinline__ void wait_warp(uint32_t a, uint32_t parity, uint32_t& dead) {      // a warp that acts on the outcome together
+  wait_for(a, parity, dead);
+  dead = __any_sync(0xffffffffu, dead) ? 1u : 0u;
+}
 // A warp that issues waits and commits by its leading lane alone, without a branch: 32 lanes at a barrier that is complete took 150 cycles, a branch around a
 // commit some 100
 __device__ __forceinline__ void wait_lead(uint32_t a, uint32_t parity, uint32_t lead, uint32_t& dead) {
   if (dead) return;
-  for (uint32_t tries = 0; tries < (1u << 22); ++tries) {
+  for (long long begin = 0;;) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %3, 0;\n\tsetp.ne.b32 p, 0, 0;\n\t@q mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
@@ -162,6 +181,9 @@ __device__ __forceinline__ void wait_lead(uint32_t a, uint32_t parity, uint32_t 
         : "r"(a), "r"(parity), "r"(lead)
         : "memory");
     if (__any_sync(0xffffffffu, ok)) return;
+    const long long now = clock64();
+    if (begin == 0) begin = now;
+    if (__any_sync(0xffffffffu, now - begin > PATIENCE)) break;
   }
   dead = 1u;
 }
@@ -482,7 +504,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
     if (dead) {                                              // what was issued ends before tensor memory is given back
       uint32_t late = 0;
       commit_by(lead, bar(ct.gave_up));
-      mbar_wait(bar(ct.gave_up), 0, late);
+      wait_for(bar(ct.gave_up), 0, late);
     }
     __syncwarp();
    } else if (warp == 1) {
@@ -502,7 +524,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
       uint32_t there = 0;                                    // by 16 keys
       for (int i = 0; i < 8; ++i) there |= (seen >> (i * 16 / box) & 1u) << i;
       const uint32_t k_to = bar(HALF ? ct.rk_full : ct.k_full[kst]);
-      mbar_wait_warp(bar(HALF ? ct.rk_empty : ct.k_empty[kst]), kph, dead);
+      wait_warp(bar(HALF ? ct.rk_empty : ct.k_empty[kst]), kph, dead);
       if (dead) break;
       if (lane == 0) {
         if (HALF) infos[tile % INFOS].there = there;
@@ -524,7 +546,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
       }
       __syncwarp();
       if (HALF || ++kst == k_stages) { kst = 0; kph ^= 1u; }
-      mbar_wait_warp(bar(HALF ? ct.rv_empty : ct.v_empty[vst]), vph, dead);
+      wait_warp(bar(HALF ? ct.rv_empty : ct.v_empty[vst]), vph, dead);
       if (dead) break;
       const int valid = keys.end - key0;
       // bf16: behind the last key that is seen the page may hold anything, and a weight of zero does not hide an infinity: zeros there
@@ -538,7 +560,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
       }
       __syncwarp();
       if (cut) {
-        mbar_wait_warp(v_to, tail_waits++ & 1u, dead);
+        wait_warp(v_to, tail_waits++ & 1u, dead);
         if (dead) break;
         for (int x = lane; x < (KEYS - valid) * 8 * va; x += 32) st128(sv + vst * va * TC_ATOM + piece_at(valid + x / (8 * va), x % (8 * va)), make_uint4(0, 0, 0, 0));
         fence_proxy_async();
@@ -551,9 +573,9 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
     // every copy has landed before the CTA ends: what reads them comes after, unless a wait ran out
     if (dead) {
       uint32_t late = 0;
-      for (int i = 0; i < (HALF ? 1 : k_stages); ++i) mbar_wait(bar(HALF ? ct.rk_full : ct.k_full[i]), i < kst ? kph ^ 1u : kph, late);
+      for (int i = 0; i < (HALF ? 1 : k_stages); ++i) wait_for(bar(HALF ? ct.rk_full : ct.k_full[i]), i < kst ? kph ^ 1u : kph, late);
       late = 0;
-      for (int i = 0; i < (HALF ? 1 : v_stages); ++i) mbar_wait(bar(HALF ? ct.rv_full : ct.v_full[i]), i < vst ? vph ^ 1u : vph, late);
+      for (int i = 0; i < (HALF ? 1 : v_stages); ++i) wait_for(bar(HALF ? ct.rv_full : ct.v_full[i]), i < vst ? vph ^ 1u : vph, late);
     }
     __syncwarp();
    } else if (warp == 2) {
@@ -599,7 +621,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
        for (int t = x.t0; t < x.t1; ++t, ++tile) {
         Info& info = infos[tile % INFOS];
         if (keys_too) {
-          mbar_wait_warp(bar(ct.rk_full), tile & 1u, dead);
+          wait_warp(bar(ct.rk_full), tile & 1u, dead);
           if (dead) break;
           const float ks = scales.k[me], vs = scales.v[me];
           // A key that some row sees: behind the last one and before the windows there may be anything, and of a page that is not there the scales are those of
@@ -610,7 +632,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
             if (valid && ks >= SMALLEST_SCALE && ks <= 1.f / SMALLEST_SCALE) atomicMax(&ct.k_ref[ref], __float_as_uint(ks));
             if (valid && vs >= SMALLEST_SCALE && vs <= 1.f / SMALLEST_SCALE) atomicMax(&ct.v_ref[ref], __float_as_uint(vs));
             mbar_arrive(bar(ct.ref_full));
-            mbar_wait_warp(bar(ct.ref_full), item++ & 1u, dead);
+            wait_warp(bar(ct.ref_full), item++ & 1u, dead);
             if (dead) break;
             k_up = value_lift(*reinterpret_cast<volatile uint32_t*>(&ct.k_ref[ref]));
             v_up = value_lift(*reinterpret_cast<volatile uint32_t*>(&ct.v_ref[ref]));
@@ -622,7 +644,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
             k_by = v_by;
             v_by = make_uint2(0u, 0u);
           }
-          mbar_wait_warp(bar(ct.k_empty[st]), ph, dead);
+          wait_warp(bar(ct.k_empty[st]), ph, dead);
           if (dead) break;
           info.k_by[me] = k_by;
           info.v_by[me] = v_by;
@@ -632,10 +654,10 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
           }
           mbar_arrive(bar(ct.info_full[tile % INFOS]));
         } else {
-          mbar_wait_warp(bar(ct.rv_full), tile & 1u, dead);
-          mbar_wait_warp(bar(ct.v_empty[st]), ph, dead);
+          wait_warp(bar(ct.rv_full), tile & 1u, dead);
+          wait_warp(bar(ct.v_empty[st]), ph, dead);
         }
-        mbar_wait_warp(bar(ct.info_full[tile % INFOS]), tile / INFOS & 1u, dead);      // all keys' factors
+        wait_warp(bar(ct.info_full[tile % INFOS]), tile / INFOS & 1u, dead);      // all keys' factors
         if (dead) break;
         if (keys_too) codes_to_f16<STORE, false>(raw_k, a.K, info.k_by, sk + st * ka * TC_ATOM, me, 128);
         else codes_to_f16<STORE, true>(raw_v, a.V, info.v_by, sv + st * va * TC_ATOM, me, 128);
@@ -706,8 +728,8 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
       const bool idle = !__any_sync(0xffffffffu, live);
       for (int t = 0; t < n; ++t) {
         const int key0 = keys.key0(t0 + t, 7);
-        mbar_wait(bar(ct.info_full[(tile + t) % INFOS]), (tile + t) / INFOS & 1u, dead);
-        mbar_wait_warp(bar(ct.s_full[g]), (mine + t) & 1u, dead);
+        wait_for(bar(ct.info_full[(tile + t) % INFOS]), (tile + t) / INFOS & 1u, dead);
+        wait_warp(bar(ct.s_full[g]), (mine + t) & 1u, dead);
         if (dead) break;
         if (idle) {                                          // no row: whatever the weights are
           if (lane < 2) mbar_arrive(bar(ct.p_half[g][lane]));
@@ -809,7 +831,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
         }
         l += sum[0] + sum[1];
       }
-      if (n > 0) mbar_wait_warp(bar(ct.o_done[g]), own_items & 1u, dead);
+      if (n > 0) wait_warp(bar(ct.o_done[g]), own_items & 1u, dead);
       fence_after();
       if (dead || notes >> 31) l = NAN;
       const float inv = part ? down : l == 0.f ? 0.f : down / l;
@@ -872,7 +894,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
     }
     if (n > 0) {
       // both halves keep to the same row tile: its products are over before the next one's queries are said to be there
-      if (g > 0) mbar_wait_warp(bar(ct.o_done[0]), item & 1u, dead);
+      if (g > 0) wait_warp(bar(ct.o_done[0]), item & 1u, dead);
       ++item;
       tile += n;
       if (g < groups) {

@@ -73,3 +73,31 @@ def test_scales_that_are_not_finite_or_out_of_range(dtype, store, form):
         cache.k_scale[pages[j // page], 0, j % page] = math.nan
     fine = expect(cache.attend(q.to(DEV), step, window=window, first=first), q, cache, seqs, K ** -0.5, window, first)
     assert not fine.all()
+
+
+def test_rows_that_take_long_hold_nobody_up():
+    """Three row tiles of 256 rows for every SM, each over 24576 keys; the last 32 rows of each see a value whose scale is out of range.  One warp computes them again
+    for longer than a wait lasted once; the others wait for it and go on as ever: their rows have the bits that they have without that scale."""
+    from lit_llama_b200 import PagedCache, PagedStep
+
+    heads, length, new, page = 3 * torch.cuda.get_device_properties(0).multi_processor_count, 24576, 256, 256
+    n_pages = length // page
+    g = torch.Generator(DEV).manual_seed(1)
+    cache = PagedCache.empty(n_pages, page, heads, 16, 16, store="int8", device=DEV)
+    for pool, scale in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+        pool.copy_((torch.randn(pool.shape, generator=g, device=DEV) * 60).round().clamp(-127, 127).to(torch.int8))
+        scale.fill_(2.0 ** -6)
+    step = PagedStep.of([(new, length, list(range(n_pages)))], DEV)
+    q = torch.randn(new, heads, 16, generator=g, device=DEV).to(torch.bfloat16)
+    usual = cache.attend(q, step)
+    at = length - 32
+    cache.v_scale[at // page, :, at % page] = 2.0 ** 70
+    got = cache.attend(q, step)
+    assert torch.equal(got[:224], usual[:224])
+    for h in range(0, heads, 37):                           # and the others the formula's value: some heads, in 64 bits
+        k, v = (x[:, h].double().reshape(length, 16) * s[:, h].double().reshape(length, 1) for x, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+        s = (q[224:, h].double() @ k.T * 0.25).masked_fill(torch.arange(length, device=DEV)[None] > torch.arange(at, length, device=DEV)[:, None], -math.inf)
+        w = torch.softmax(s, -1)
+        dots = (q[224:, h].double().abs() @ k.abs().T).amax(-1) * 0.25
+        tol = O.tolerance(w @ v, w @ v.abs(), dots, 16, length, False, "int8")
+        assert bool(((got[224:, h].double() - w @ v).abs() <= tol).all())
