@@ -137,8 +137,11 @@ class PagePool:
         """The last n tokens that were booked for a sequence did not come: it is as long as it was, and pages of theirs alone are free again."""
         if not 0 <= n <= self._length[request_id]:
             raise ValueError(f"page pool: {n} tokens of {self._length[request_id]}")
-        self._length[request_id] -= n
-        pages, keep = self._pages[request_id], -(-self._length[request_id] // self.page)
+        length = self._length[request_id] - n
+        pages, keep, reach = self._pages[request_id], -(-length // self.page), length - self.window + 1
+        if any(p < 0 and (i * self.page < self.first or (i + 1) * self.page > reach) for i, p in enumerate(pages[:keep])):
+            raise ValueError(f"page pool: pages that the window at {length} reaches were given back")
+        self._length[request_id] = length
         self._free += [p for p in reversed(pages[keep:]) if p >= 0]
         del pages[keep:]
 

@@ -255,3 +255,17 @@ def test_tokens_that_did_not_come():
     assert p.position("a") == 20 and p.free_pages() == 6
     p.take_back("a", 20)
     assert p.position("a") == 0 and p.pages("a") == [] and p.free_pages() == 8
+
+
+def test_tokens_whose_window_is_gone_are_not_taken_back():
+    """Pages that the window has left are other sequences' by now."""
+    p = PagePool(12, 16, torch.device("cpu"), window=24, first=2)
+    for n in (60, 40, 5):
+        p.step([("a", n)])
+    assert -1 in p.pages("a")
+    free, pages = p.free_pages(), p.pages("a")
+    with pytest.raises(ValueError, match="window"):
+        p.take_back("a", 50)
+    assert p.position("a") == 105 and p.free_pages() == free and p.pages("a") == pages
+    p.take_back("a", 5)
+    assert p.position("a") == 100
