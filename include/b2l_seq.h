@@ -254,6 +254,9 @@ int b2l_seq_softcap(float* z, size_t n, float cap, b2l_stream_t stream);
 int b2l_seq_rope(const void* x, int ldx, int in_f32, const float* freq, int rot_dims, int interleaved, int rot_off, float mult,
                  float rot_mult, const int* meta, void* out, int ldo, int out_f32, int T, int heads, int size, int hsx, int hso, int act_dtype,
                  b2l_stream_t stream);
+/* The same by the angle positions[t] * freq[i] (device int32 [T]): tokens of several sequences, or of a tree. */
+int b2l_seq_rope_at(const void* x, int ldx, int in_f32, const float* freq, int rot_dims, int interleaved, int rot_off, float mult, float rot_mult, const int* positions,
+                    void* out, int ldo, int out_f32, int T, int heads, int size, int hsx, int hso, int act_dtype, b2l_stream_t stream);
 
 /* ---- latent attention ----
  * Keys and values of all heads are linear images of one latent vector per position; beside it one rotated key part
@@ -528,6 +531,52 @@ int b2l_seq_paged_attention_all(const void* q, long long ldq, long long hsq, con
                                 b2l_stream_t stream);
 long long b2l_seq_paged_attention_work(int rows, int seqs, int width, int page, int heads, int kv_heads, int K, int V, int window, int first, int max_new,
                                        int max_length, int store, int act_dtype);
+
+/* ---- several continuations of a sequence: trees of drafted tokens, beams ----
+ * The new tokens of a step's sequences (starts, lengths and table as above) are trees: token i of a sequence has the parent parents[starts[b] + i], a place among
+ * the sequence's new tokens before i, or none (-1, or whatever else is not before i).  Its depth is the number of its ancestors, its position
+ * lengths[b] - (rows of b) + depth; keys and values lie in the order of the tokens all the same.
+ *
+ *   b2l_seq_tree_build            masks [rows][words] (uint32, bit i of a row: whether it sees token i of its sequence's new ones), depths and positions (int32
+ *                                 [rows]): each token sees its ancestors and itself, with a window those whose position is above its own less the window, or below
+ *                                 `first`.  Tokens from 32 words on have no bit.  A row of no sequence: zeros.
+ *   b2l_seq_paged_attention_tree  b2l_seq_paged_attention over the context (keys before the new tokens; the window counts from the row's position, depths
+ *                                 clipped to 0 .. rows of b - 1) and, of the new tokens, those of the row's mask (any mask).  zeros: whether the outputs of rows of no
+ *                                 sequence become zeros (else they stay).  Its work space is b2l_seq_paged_attention_work's.
+ *   b2l_seq_tree_accept           target[r] = argmax_v x[r, v], or with noise (f32 [rows, ldn]) argmax_v x[r, v] / temperature - log noise[r, v], which draws v with
+ *                                 probability softmax(x / temperature)[v] where the noise is Exp(1); ties to the lowest v, a NaN is nowhere the largest, 0 where
+ *                                 nothing is above -inf.  x act [rows, ld].  Then from each sequence's first new token on: its first child (of the lowest place)
+ *                                 whose token (int32, or int64 with tokens64) is its target, and so on.  kept[starts[b] + k]: the place of the k-th of these tokens
+ *                                 among the sequence's new ones (the first has place 0), -1 behind the last and for rows of no sequence; counts[b]: how many;
+ *                                 next[b]: the target of the last one (-1 for a sequence without new tokens).  `work` has b2l_seq_tree_accept_work bytes.
+ *   b2l_seq_paged_keep            in the pools of all layers the row of token kept[starts[b] + k] goes to the place of token k, k < counts[b].  kept ascends, so kept[..+ k] >=
+ *                                 k; what is not a place among the sequence's new tokens, or has no page, is left out.
+ *   b2l_seq_paged_copy            in the pools of all layers page pairs[2 i] is copied to page pairs[2 i + 1], i < n; pairs with a page outside the pool are left out.  No
+ *                                 page comes twice as a target, and none as a source and a target.
+ * pools: host array of 4 addresses for each of `layers` layers: k, v, k_scale, v_scale (these null where there are none).
+ *
+ *   b2l_seq_beam_select           for each of `groups` groups of `beams` rows of logits x (act, `ld` entries between rows, group after group) the `count` (at most 64)
+ *                                 largest of scores[g, w] + x[w, v] - log sum_u exp x[w, u], falling, ties to the lowest w vocab + v: values (f32), from (the beam w)
+ *                                 and tokens (v), [groups, count] each.  The order is that before values are rounded to f32.  A beam is out (all its values
+ *                                 are -inf) where its score is no finite number, a logit is NaN or +inf, or none is above -inf.  `work` has
+ *                                 b2l_seq_beam_work bytes.  At most 64 beams. */
+int b2l_seq_tree_build(const int* parents, const int* starts, const int* lengths, unsigned* masks, int words, int* depths, int* positions, int rows, int seqs, int window,
+                       int first, b2l_stream_t stream);
+int b2l_seq_paged_attention_tree(const void* q, long long ldq, long long hsq, const void* k, const void* v, const float* k_scale, const float* v_scale, const int* starts,
+                                 const int* lengths, const int* table, int ldt, int width, const unsigned* masks, int words, const int* depths, int zeros, void* out,
+                                 float* work, long long work_floats, int rows, int seqs, int pages, int page, int heads, int kv_heads, int K, int V, int window, int first,
+                                 float scale, int max_new, int max_length, int store, int act_dtype, b2l_stream_t stream);
+int b2l_seq_tree_accept(const void* logits, long long ld, const float* noise, long long ldn, float temperature, const int* parents, const int* starts, const void* tokens,
+                        int tokens64, int* kept, int* counts, int* next, void* work, long long work_bytes, int rows, int seqs, int vocab, int act_dtype,
+                        b2l_stream_t stream);
+long long b2l_seq_tree_accept_work(int rows, int vocab);
+int b2l_seq_paged_keep(const void* const* pools, int layers, const int* starts, const int* lengths, const int* table, int ldt, int width, const int* kept, const int* counts,
+                       int rows, int seqs, int pages, int page, int kv_heads, int K, int V, int store, int act_dtype, b2l_stream_t stream);
+int b2l_seq_paged_copy(const void* const* pools, int layers, const int* pairs, int n, int pages, int page, int kv_heads, int K, int V, int store, int act_dtype,
+                       b2l_stream_t stream);
+int b2l_seq_beam_select(const void* logits, long long ld, const float* scores, float* values, int* from, int* tokens, void* work, long long work_bytes, int groups, int beams,
+                        int vocab, int count, int act_dtype, b2l_stream_t stream);
+long long b2l_seq_beam_work(int groups, int beams, int vocab, int count);
 
 #ifdef __cplusplus
 }

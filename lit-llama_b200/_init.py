@@ -20,7 +20,8 @@ from .rinirax import Rinirax, RiniraxConfig
 from .lukupel import Lukupel, LukupelConfig
 from .malulorn import Malulorn, MalulornConfig
 from .state import SequenceStatePool, StateSpec
-from .paged import PagedCache, PagedStep, PagePool
+from .paged import PagedCache, PagedLayers, PagedStep, PagedTree, PagePool
+from .search import beam_select
 from .engine import Engine
 from .registry import PagedLLaMAModel, load_model, register
 
@@ -29,5 +30,5 @@ __all__ = [
     "ColBlockQuantizedLinear", "Linear8bitLt", "find_multiple", "llama_model_lookup", "generate", "sample_probs", "sample_token", "patch_reference", "TPLLaMA", "shard_state_dict",
     "Lugovik", "LugovikConfig", "Zenasun", "ZenasunConfig", "Zuvevik", "ZuvevikConfig", "Rinirax", "RiniraxConfig", "Lukupel", "LukupelConfig",
     "Malulorn", "MalulornConfig",
-    "SequenceStatePool", "StateSpec", "PagedCache", "PagedStep", "PagePool", "PagedLLaMAModel", "Engine", "load_model", "register",
+    "SequenceStatePool", "StateSpec", "PagedCache", "PagedLayers", "PagedStep", "PagedTree", "PagePool", "beam_select", "PagedLLaMAModel", "Engine", "load_model", "register",
 ]

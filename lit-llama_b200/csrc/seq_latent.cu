@@ -23,14 +23,14 @@ namespace b2l {
 // `mult` afterwards.  Heads start every hsx (input) / hso (output) elements.  One warp per (token, head).
 template <typename in_t, typename out_t>
 __global__ void seq_rope_kernel(const in_t* __restrict__ x, int ldx, const float* __restrict__ freq, int rot_dims, int interleaved,
-                                int off, float mult, float rot_mult, const int* __restrict__ meta, out_t* __restrict__ out, int ldo, int n_rows, int heads,
-                                int size, int hsx, int hso) {
+                                int off, float mult, float rot_mult, const int* __restrict__ meta, const int* __restrict__ positions, out_t* __restrict__ out, int ldo,
+                                int n_rows, int heads, int size, int hsx, int hso) {
   const int id = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (id >= n_rows * heads) return;
   const int t = id / heads, hd = id % heads;
   const in_t* p = x + (size_t)t * ldx + (size_t)hd * hsx;
   out_t* q = out + (size_t)t * ldo + (size_t)hd * hso;
-  const float pos = (float)(meta[1] + t);
+  const float pos = (float)(positions ? positions[t] : meta[1] + t);
   const int half = rot_dims / 2;
   for (int i = lane; i < off; i += 32) st_act(q, i, ld_act(p, i) * mult);
   for (int i = lane; i < half; i += 32) {
@@ -52,8 +52,8 @@ __global__ void seq_rope_kernel(const in_t* __restrict__ x, int ldx, const float
 // token 1.7 / 2.0, 300 2.6 / 2.7, 777 4.2 / 3.3; 8 heads, 300 tokens 2.2 / 2.5, 777 2.9 / 2.7), hence the launch's line of 40 heads an SM.
 template <typename in_t, typename out_t, int P>
 __global__ void __launch_bounds__(128) seq_rope_heads_kernel(const in_t* x, int ldx, const float* __restrict__ freq, int rot_dims, int interleaved, int off, float mult,
-                                                             float rot_mult, const int* __restrict__ meta, out_t* out, int ldo, int n_rows, int heads, int size,
-                                                             int hsx, int hso) {
+                                                             float rot_mult, const int* __restrict__ meta, const int* __restrict__ positions, out_t* out, int ldo, int n_rows,
+                                                             int heads, int size, int hsx, int hso) {
   const int groups = (heads + 3) / 4, id = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, t = id / groups, h0 = (id - t * groups) * 4;
   if (t >= n_rows) return;
   const int half = rot_dims / 2, n = min(4, heads - h0), plain = (size - rot_dims) / 4;
@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(128) seq_rope_heads_kernel(const in_t* x, int 
     for (int h = 0; h < 4; ++h)
       if (h < n) st_act4(q + (size_t)h * hso + e, make_float4(y[h].x * mult, y[h].y * mult, y[h].z * mult, y[h].w * mult));
   }
-  const float pos = (float)(meta[1] + t);
+  const float pos = (float)(positions ? positions[t] : meta[1] + t);
 #pragma unroll
   for (int j = 0; j < P; ++j) {
     const int i = lane + 32 * j;
@@ -786,14 +786,14 @@ static int launch_latent(const b2l_seq_latent_attn_args& a, int row_warps, size_
 
 using namespace b2l;
 
-extern "C" int b2l_seq_rope(const void* x, int ldx, int in_f32, const float* freq, int rot_dims, int interleaved, int rot_off,
-                            float mult, float rot_mult, const int* meta, void* out, int ldo, int out_f32, int T, int heads, int size,
-                            int hsx, int hso, int act_dtype, b2l_stream_t stream) {
-  B2L_CHECK_ARG(x && meta && out, "b2l_seq_rope: null pointer");
+// positions: of every token, else meta's and on
+static int rope(const char* who, const void* x, int ldx, int in_f32, const float* freq, int rot_dims, int interleaved, int rot_off, float mult, float rot_mult, const int* meta,
+                const int* positions, void* out, int ldo, int out_f32, int T, int heads, int size, int hsx, int hso, int act_dtype, b2l_stream_t stream) {
+  B2L_CHECK_ARG(x && (meta || positions) && out, "%s: null pointer", who);
   B2L_CHECK_ARG(T >= 0 && heads > 0 && size > 0 && hsx >= size && hso >= size && ldx >= (heads - 1) * hsx + size && ldo >= (heads - 1) * hso + size,
-                "b2l_seq_rope: bad size");
+                "%s: bad size", who);
   B2L_CHECK_ARG(rot_dims >= 0 && rot_off >= 0 && rot_off + rot_dims <= size && rot_dims % 2 == 0 && (rot_dims == 0 || freq),
-                "b2l_seq_rope: bad rotation");
+                "%s: bad rotation", who);
   if (T == 0) return 0;
   const int ids = T * heads, grid = (ids + 3) / 4;
   cudaStream_t st = (cudaStream_t)stream;
@@ -801,7 +801,7 @@ extern "C" int b2l_seq_rope(const void* x, int ldx, int in_f32, const float* fre
   const bool by_heads = (long long)T * heads >= 40LL * sm_count() && rot_dims >= 2 && rot_dims <= 128 && rot_dims % 4 == 0 && rot_off % 4 == 0 && size % 4 == 0 && hsx % 4 == 0 && hso % 4 == 0 && ldx % 4 == 0 &&
                         ldo % 4 == 0 && al4(x, isz) && al4(out, osz) && (size_t)T * ((heads + 3) / 4) < (1ull << 31);
   const int warps = (int)(by_heads ? (size_t)T * ((heads + 3) / 4) : 0);
-#define B2L_ROPE_ARGS(IN, OUT) (const IN*)x, ldx, freq, rot_dims, interleaved, rot_off, mult, rot_mult, meta, (OUT*)out, ldo, T, heads, size, hsx, hso
+#define B2L_ROPE_ARGS(IN, OUT) (const IN*)x, ldx, freq, rot_dims, interleaved, rot_off, mult, rot_mult, meta, positions, (OUT*)out, ldo, T, heads, size, hsx, hso
 #define B2L_ROPE_GO(IN, OUT) \
   if (by_heads && rot_dims <= 64) seq_rope_heads_kernel<IN, OUT, 1><<<(warps + 3) / 4, 128, 0, st>>>(B2L_ROPE_ARGS(IN, OUT)); \
   else if (by_heads) seq_rope_heads_kernel<IN, OUT, 2><<<(warps + 3) / 4, 128, 0, st>>>(B2L_ROPE_ARGS(IN, OUT)); \
@@ -816,6 +816,17 @@ extern "C" int b2l_seq_rope(const void* x, int ldx, int in_f32, const float* fre
 #undef B2L_ROPE_ARGS
   B2L_LAUNCH_CHECK("seq_rope_kernel");
   return 0;
+}
+
+extern "C" int b2l_seq_rope(const void* x, int ldx, int in_f32, const float* freq, int rot_dims, int interleaved, int rot_off,
+                            float mult, float rot_mult, const int* meta, void* out, int ldo, int out_f32, int T, int heads, int size,
+                            int hsx, int hso, int act_dtype, b2l_stream_t stream) {
+  return rope("b2l_seq_rope", x, ldx, in_f32, freq, rot_dims, interleaved, rot_off, mult, rot_mult, meta, nullptr, out, ldo, out_f32, T, heads, size, hsx, hso, act_dtype, stream);
+}
+
+extern "C" int b2l_seq_rope_at(const void* x, int ldx, int in_f32, const float* freq, int rot_dims, int interleaved, int rot_off, float mult, float rot_mult, const int* positions,
+                               void* out, int ldo, int out_f32, int T, int heads, int size, int hsx, int hso, int act_dtype, b2l_stream_t stream) {
+  return rope("b2l_seq_rope_at", x, ldx, in_f32, freq, rot_dims, interleaved, rot_off, mult, rot_mult, nullptr, positions, out, ldo, out_f32, T, heads, size, hsx, hso, act_dtype, stream);
 }
 
 extern "C" int b2l_seq_latent_prep(const float* proj, int ld, int q_off, int q_rank, const void* w_q, void* cq, int kv_off,

@@ -122,8 +122,8 @@ __host__ __device__ constexpr int most_stages(int store) { return store == ACT ?
 struct FewMaps { CUtensorMap k, v; };
 
 // NV: the most 16-entry parts of a value (and, up to 8, of a key); NR: columns of 8 rows
-template <typename act_t, int STORE, int NV, int NR>
-__global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 3) : 2) paged_few_kernel(const __grid_constant__ Attn a, const __grid_constant__ FewMaps maps, int stages) {
+template <typename act_t, int STORE, int NV, int NR, bool TREE>
+__global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 3) : 2) paged_few_kernel(const __grid_constant__ Attn<TREE> a, const __grid_constant__ FewMaps maps, int stages) {
   constexpr bool F32 = sizeof(act_t) == 4, HALF = STORE != ACT;
   constexpr int ES = STORE == ACT ? (int)sizeof(act_t) : 1, R = 8 * NR;
   constexpr int QP = F32 ? 3 : 1, KP = F32 && !HALF ? 3 : 1, WP = F32 ? 3 : HALF ? 1 : 2, PRODUCTS = KP == 3 ? 6 : QP, V_PRODUCTS = KP == 3 ? 6 : WP;
@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
         float up;
         lift_of(__uint_as_float(largest[at]), a.scale_log2, up, cr[r][e]);
       }
-      pos[r][e] = pl.first + at < pl.n * G ? pl.length - pl.n + (pl.first + at) / G : -1;
+      pos[r][e] = pl.first + at < pl.n * G ? a.position(pl.start, pl.length - pl.n, pl.n, (pl.first + at) / G) : -1;
     }
 #pragma unroll
     for (int x = 0; x < NV; ++x)
@@ -435,12 +435,23 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
     float top[NR][2];
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
+      uint32_t seen[2];                                      // TREE: keys key0 .. that rows 2 t and 2 t + 1 see
+      if (TREE && !whole)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int at = pl.first + 8 * r + 2 * t + e;
+          seen[e] = at < pl.n * G ? a.seen32(pos[r][e], pl.start + at / G, pl.length - pl.n, pl.n, key0) : 0u;
+        }
 #pragma unroll
       for (int n = 0; n < NK; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           s[n][r][e] = HALF ? fmaf(s[n][r][e] * c[n][e >> 1], cr[r][e & 1], add[n][e >> 1]) : s[n][r][e] * a.scale_log2;
-          if (!whole && (lost >> n & 1u || !a.sees(pos[r][e & 1], key0 + 16 * n + g + 8 * (e >> 1)))) s[n][r][e] = -INFINITY;
+          if constexpr (TREE) {
+            if (!whole && (lost >> n & 1u || !(seen[e & 1] >> (16 * n + g + 8 * (e >> 1)) & 1u))) s[n][r][e] = -INFINITY;
+          } else {
+            if (!whole && (lost >> n & 1u || !a.sees(pos[r][e & 1], 0, 0, 0, key0 + 16 * n + g + 8 * (e >> 1)))) s[n][r][e] = -INFINITY;
+          }
         }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -613,7 +624,7 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
 // ------------------------------------------------------------------------------------------------ joining parts
 // `per` warps (a power of two) have a row and head, each every per-th part.  Parts are read once, and the loads of a warp's parts do not wait for one another.
 constexpr int MERGE_WARPS = 8;
-__global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const __grid_constant__ Attn a, int per) {
+template <bool TREE> __global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const __grid_constant__ Attn<TREE> a, int per) {
   __shared__ float4 sx[MERGE_WARPS][64];
   __shared__ float2 sml[MERGE_WARPS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
@@ -752,7 +763,7 @@ static Plan plan_of(int rows, int seqs, int width, int page, int heads, int kv_h
   return p;
 }
 
-template <typename act_t, int STORE, int NV, int NR> static int few_launch(const Attn& a, int tiles, cudaStream_t stream) {
+template <typename act_t, int STORE, int NV, int NR, bool TREE> static int few_launch(const Attn<TREE>& a, int tiles, cudaStream_t stream) {
   constexpr int ES = STORE == ACT ? (int)sizeof(act_t) : 1, PER = ES == 1 ? 2 : 1;
   const size_t queries = (size_t)(sizeof(act_t) == 4 ? 3 : 1) * ((a.K / 16 + PER - 1) / PER * PER) * NR * 256, unit = (size_t)(atoms_of(a.K, ES) + atoms_of(a.V, ES)) * ATOM * (ES == 1 ? 2 : 1);
   // four warps and as many CTAs on an SM as leave each warp two units in its ring at least; fewer warps where one CTA does not fit
@@ -773,7 +784,7 @@ template <typename act_t, int STORE, int NV, int NR> static int few_launch(const
   if (int rc = tc::map_sw128(&maps.k, type, ES, a.k, rows, a.K, a.K, 128 / ES, box)) return rc;
   if (int rc = tc::map_sw128(&maps.v, type, ES, a.v, rows, a.V, a.V, 128 / ES, box)) return rc;
   static DynSmemCache cache;
-  auto kernel = paged_few_kernel<act_t, STORE, NV, NR>;
+  auto kernel = paged_few_kernel<act_t, STORE, NV, NR, TREE>;
   if (int rc = ensure_dyn_smem(kernel, smem, cache)) return rc;
   kernel<<<dim3((unsigned)tiles, (unsigned)a.kv_heads, (unsigned)a.few.splits), 32 * W, smem, stream>>>(a, maps, stages);
   B2L_LAUNCH_CHECK("paged_few_kernel");
@@ -791,7 +802,7 @@ extern "C" long long b2l_seq_paged_attention_work(int rows, int seqs, int width,
   return paged::plan_of(rows, seqs, width, page, heads, kv_heads, K, V, window, first, max_new, max_length, store, act_dtype).floats;
 }
 
-static int attention(const char* who, bool zeros, const void* q, long long ldq, long long hsq, const void* k, const void* v, const float* k_scale, const float* v_scale,
+template <bool TREE> static int attention(const char* who, bool zeros, const paged::Tree& nodes, const void* q, long long ldq, long long hsq, const void* k, const void* v, const float* k_scale, const float* v_scale,
                      const int* starts, const int* lengths, const int* table, int ldt, int width, void* out, float* work, long long work_floats, int rows, int seqs, int pages,
                      int page, int heads, int kv_heads, int K, int V, int window, int first, float scale, int max_new, int max_length, int store, int act_dtype,
                      b2l_stream_t stream) {
@@ -809,7 +820,7 @@ static int attention(const char* who, bool zeros, const void* q, long long ldq, 
   if (paged::hides_nothing(window, first, width, page)) window = first = 0;
   const Plan p = plan_of(rows, seqs, width, page, heads, kv_heads, K, V, window, first, max_new, max_length, store, act_dtype);
   B2L_CHECK_ARG(p.floats == 0 || (work && work_floats >= p.floats), "%s: a work space of %lld floats is needed", who, p.floats);
-  Attn a{};
+  Attn<TREE> a{};
   a.s = step_of(starts, lengths, table, ldt, width, rows, seqs, pages, page);
   a.q = q; a.k = k; a.v = v; a.ks = k_scale; a.vs = v_scale; a.out = out;
   a.ldq = ldq; a.hsq = hsq;
@@ -820,6 +831,7 @@ static int attention(const char* who, bool zeros, const void* q, long long ldq, 
   const cudaStream_t st = (cudaStream_t)stream;
   a.few_max = p.few_max;
   a.zeros = zeros;
+  a.nodes = nodes;
   a.both = p.few_tiles > 0 && p.many_ctas > 0;
   if (p.many_ctas) {
     const int rc = many_launch(a, p.many_ctas, work, st);
@@ -834,14 +846,14 @@ static int attention(const char* who, bool zeros, const void* q, long long ldq, 
   int rc = 0;
   const bool small = V <= 128 && K <= 128;
 #define GO(ST)                                                                                                                              \
-  (p.few_rows == 8 ? (small ? few_launch<act_t, ST, 8, 1>(a, p.few_tiles, st) : few_launch<act_t, ST, 16, 1>(a, p.few_tiles, st))            \
-                   : (small ? few_launch<act_t, ST, 8, 2>(a, p.few_tiles, st) : few_launch<act_t, ST, 16, 2>(a, p.few_tiles, st)))
+  (p.few_rows == 8 ? (small ? few_launch<act_t, ST, 8, 1, TREE>(a, p.few_tiles, st) : few_launch<act_t, ST, 16, 1, TREE>(a, p.few_tiles, st))            \
+                   : (small ? few_launch<act_t, ST, 8, 2, TREE>(a, p.few_tiles, st) : few_launch<act_t, ST, 16, 2, TREE>(a, p.few_tiles, st)))
   B2L_SEQ_DISPATCH(act_dtype, rc = store == ACT ? GO(ACT) : store == E4M3 ? GO(E4M3) : GO(INT8));
 #undef GO
   if (rc || p.few_splits == 1) return rc;
   const int warps = p.few_splits >= 32 ? 8 : p.few_splits >= 16 ? 4 : p.few_splits >= 8 ? 2 : 1, here = MERGE_WARPS / warps;
   LaunchCfg launch(dim3((unsigned)((a.few.count + here - 1) / here)), dim3(32 * MERGE_WARPS), 0, st, true);
-  B2L_CUDA(cudaLaunchKernelEx(&launch.cfg, paged_merge_kernel, a, warps));
+  B2L_CUDA(cudaLaunchKernelEx(&launch.cfg, paged_merge_kernel<TREE>, a, warps));
   B2L_LAUNCH_CHECK("paged_merge_kernel");
   return 0;
 }
@@ -850,7 +862,7 @@ extern "C" int b2l_seq_paged_attention(const void* q, long long ldq, long long h
                                        const int* lengths, const int* table, int ldt, int width, void* out, float* work, long long work_floats, int rows, int seqs, int pages,
                                        int page, int heads, int kv_heads, int K, int V, int window, int first, float scale, int max_new, int max_length, int store,
                                        int act_dtype, b2l_stream_t stream) {
-  return attention("b2l_seq_paged_attention", false, q, ldq, hsq, k, v, k_scale, v_scale, starts, lengths, table, ldt, width, out, work, work_floats, rows, seqs, pages, page, heads,
+  return attention<false>("b2l_seq_paged_attention", false, {}, q, ldq, hsq, k, v, k_scale, v_scale, starts, lengths, table, ldt, width, out, work, work_floats, rows, seqs, pages, page, heads,
                    kv_heads, K, V, window, first, scale, max_new, max_length, store, act_dtype, stream);
 }
 
@@ -858,6 +870,16 @@ extern "C" int b2l_seq_paged_attention_all(const void* q, long long ldq, long lo
                                            const int* lengths, const int* table, int ldt, int width, void* out, float* work, long long work_floats, int rows, int seqs, int pages,
                                            int page, int heads, int kv_heads, int K, int V, int window, int first, float scale, int max_new, int max_length, int store,
                                            int act_dtype, b2l_stream_t stream) {
-  return attention("b2l_seq_paged_attention_all", true, q, ldq, hsq, k, v, k_scale, v_scale, starts, lengths, table, ldt, width, out, work, work_floats, rows, seqs, pages, page,
+  return attention<false>("b2l_seq_paged_attention_all", true, {}, q, ldq, hsq, k, v, k_scale, v_scale, starts, lengths, table, ldt, width, out, work, work_floats, rows, seqs, pages, page,
                    heads, kv_heads, K, V, window, first, scale, max_new, max_length, store, act_dtype, stream);
+}
+
+extern "C" int b2l_seq_paged_attention_tree(const void* q, long long ldq, long long hsq, const void* k, const void* v, const float* k_scale, const float* v_scale, const int* starts,
+                                            const int* lengths, const int* table, int ldt, int width, const unsigned* masks, int words, const int* depths, int zeros, void* out,
+                                            float* work, long long work_floats, int rows, int seqs, int pages, int page, int heads, int kv_heads, int K, int V, int window, int first,
+                                            float scale, int max_new, int max_length, int store, int act_dtype, b2l_stream_t stream) {
+  B2L_CHECK_ARG(rows == 0 || seqs == 0 || (masks && depths), "b2l_seq_paged_attention_tree: null pointer");
+  B2L_CHECK_ARG(words > 0, "b2l_seq_paged_attention_tree: masks of %d words", words);
+  return attention<true>("b2l_seq_paged_attention_tree", zeros != 0, {masks, depths, words}, q, ldq, hsq, k, v, k_scale, v_scale, starts, lengths, table, ldt, width, out, work, work_floats,
+                         rows, seqs, pages, page, heads, kv_heads, K, V, window, first, scale, max_new, max_length, store, act_dtype, stream);
 }

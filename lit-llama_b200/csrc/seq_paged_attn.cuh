@@ -64,7 +64,14 @@ struct Parts { float *ml, *o; int splits; long long count; };
 // CTAs that have a part; none: 0), and two places for partial results of 256 rows (the first row tile's, the last one's) [2 ctas][256][2] and [2 ctas][256][V]
 struct Shared { int4* last; float *ml, *o; };
 
-struct Attn {
+// What the new tokens of a step see of one another: token i of a sequence those before it and itself, or (TREE) those whose bits its mask has, [rows][words] words of
+// 32; then its position is the sequence's first new token's plus its depth
+struct Tree { const uint32_t* masks; const int* depths; int words; };
+
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }      // bits 0 .. n-1 (any n)
+
+template <bool TREE> struct Attn {
+  static constexpr bool tree = TREE;
   Step s;
   const void *q, *k, *v;
   const float *ks, *vs;
@@ -77,8 +84,34 @@ struct Attn {
   int f32, store_kind, both;                                 // both: the two kernels share the step, few_max packed rows of every sequence and head in `few`
   Parts few;
   Shared many;
+  Tree nodes;
 
-  __device__ __forceinline__ bool sees(int pos, int j) const { return j <= pos && (window == 0 || j > pos - window || j < first); }
+  // position of new token i of a sequence whose n new ones begin at position `base` and row `start`
+  __device__ __forceinline__ int position(int start, int base, int n, int i) const {
+    if constexpr (TREE) return base + min(max(nodes.depths[start + i], 0), n - 1);
+    else return base + i;
+  }
+  __device__ __forceinline__ bool in_window(int pos, int j) const { return window == 0 || j > pos - window || j < first; }
+  // Bits i0 .. i0 + 31 of the mask of a row, of a sequence with n new tokens
+  __device__ __forceinline__ uint32_t tree_bits(int row, int n, int i0) const {
+    if (i0 >= n || i0 <= -32) return 0u;
+    const uint32_t* m = nodes.masks + (size_t)row * nodes.words;
+    const int w = i0 >> 5;                                   // -1 where the context ends inside
+    const uint32_t lo = w >= 0 && w < nodes.words ? m[w] : 0u, hi = w + 1 < nodes.words ? m[w + 1] : 0u;
+    return __funnelshift_r(lo, hi, i0 & 31) & low_bits(n - i0);
+  }
+  // whether a row at position `pos` sees key j; its sequence's n new tokens begin at `base`
+  __device__ __forceinline__ bool sees(int pos, int row, int base, int n, int j) const {
+    if constexpr (TREE) return j < base ? in_window(pos, j) : (tree_bits(row, n, j - base) & 1u) != 0u;
+    else return j <= pos && in_window(pos, j);
+  }
+  // the same of keys j .. j + 31, as bits
+  __device__ __forceinline__ uint32_t seen32(int pos, int row, int base, int n, int j) const {
+    uint32_t x = low_bits((TREE ? base : pos + 1) - j);
+    if (window) x &= ~low_bits(pos - window + 1 - j) | low_bits(first - j);
+    if constexpr (TREE) x |= tree_bits(row, n, j - base);
+    return x;
+  }
 
   // Tile `slot` of the tiles of R packed rows of all sequences, without the first of each; a whole warp looks
   __device__ __forceinline__ bool place(int slot, int R, int lane, Place& pl) const {
@@ -115,10 +148,17 @@ struct Attn {
   __device__ __forceinline__ Keys keys(const Place& pl, int R) const {
     const int G = heads / kv_heads, last = min(pl.first + R, pl.n * G) - 1;
     Keys x;
-    x.p_min = pl.length - pl.n + pl.first / G;
-    x.p_max = pl.length - pl.n + last / G;
-    x.end = x.p_max + 1;
+    if constexpr (TREE) {                                    // rows of any depth
+      x.p_min = pl.length - pl.n;
+      x.p_max = pl.length - 1;
+      x.end = pl.length;
+    } else {
+      x.p_min = pl.length - pl.n + pl.first / G;
+      x.p_max = pl.length - pl.n + last / G;
+      x.end = x.p_max + 1;
+    }
     x.lo = window ? max(x.p_min - window + 1, 0) : 0;
+    if constexpr (TREE) --x.p_min;                           // the last key that all of them may see
     x.early = min(first, x.lo);
     x.window = window;
     x.first = first;
@@ -158,7 +198,7 @@ struct Attn {
 };
 
 // Zeros in the outputs of rows r0 .. r1 - 1, n heads from `head` on
-static __device__ __noinline__ void clear_rows(const Attn& a, int r0, int r1, int head, int n, int me, int threads) {
+template <bool TREE> static __device__ __noinline__ void clear_rows(const Attn<TREE>& a, int r0, int r1, int head, int n, int me, int threads) {
   const int es = a.f32 ? 4 : 2, pieces = n * a.V * es / 16;
   for (long long i = me; i < (long long)(r1 - r0) * pieces; i += threads)
     *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(a.out) + ((size_t)(r0 + i / pieces) * a.heads + head) * a.V * es + i % pieces * 16) = make_uint4(0u, 0u, 0u, 0u);
@@ -170,7 +210,7 @@ static __device__ __noinline__ void clear_rows(const Attn& a, int r0, int r1, in
 // with more spills registers in its loops.  All of 512 tokens' rows again, 32 / 8 heads of 128 over 4096 keys of an int8 pool: 11.3 ms (78 with a row at a time, key
 // after key); one token's over 16384 keys 9.6 ms (37).  Where all of a row is NaN it stays so, and the rest is left out: 1.7 and 0.4 ms with a NaN among the first.
 template <int MENDED> struct Again { int n, pos[MENDED], row[MENDED], head[MENDED]; };
-template <int MENDED> __device__ __forceinline__ void mend_few(const Attn& a, int b, int h, const Again<MENDED>& x, int lane) {
+template <int MENDED, bool TREE> __device__ __forceinline__ void mend_few(const Attn<TREE>& a, int b, int h, const Again<MENDED>& x, int base, int n_new, int lane) {
   float m[MENDED], l[MENDED], o[MENDED][8];
   int p_min = x.pos[0], p_max = x.pos[0];
 #pragma unroll
@@ -184,6 +224,7 @@ template <int MENDED> __device__ __forceinline__ void mend_few(const Attn& a, in
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[r][e] = 0.f;
   }
+  if constexpr (TREE) p_max = base + n_new - 1;
   for (int j0 = 0; j0 <= p_max; j0 += 32) {
     if (a.window && j0 >= a.first && j0 + 31 <= p_min - a.window) {      // on to the first window
       j0 = ((p_min - a.window + 1) & ~31) - 32;
@@ -192,7 +233,7 @@ template <int MENDED> __device__ __forceinline__ void mend_few(const Attn& a, in
     const int j = j0 + lane;
     bool any = false;
 #pragma unroll
-    for (int r = 0; r < MENDED; ++r) any |= r < x.n && a.sees(x.pos[r], j);
+    for (int r = 0; r < MENDED; ++r) any |= r < x.n && a.sees(x.pos[r], x.row[r], base, n_new, j);
     const int page = any ? page_of(a.s, b, j) : -1;
     const size_t at = (((size_t)max(page, 0) * a.kv_heads + h) << a.s.shift) + (j & ((1 << a.s.shift) - 1));
     float w[MENDED] = {};
@@ -213,7 +254,7 @@ template <int MENDED> __device__ __forceinline__ void mend_few(const Attn& a, in
 #pragma unroll
     for (int r = 0; r < MENDED; ++r) {
       if (r >= x.n) break;
-      const float s = page >= 0 && a.sees(x.pos[r], j) ? w[r] * a.scale_log2 : -INFINITY;
+      const float s = page >= 0 && a.sees(x.pos[r], x.row[r], base, n_new, j) ? w[r] * a.scale_log2 : -INFINITY;
       float now = s;
 #pragma unroll
       for (int y = 16; y > 0; y >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, y));
@@ -262,8 +303,13 @@ template <int MENDED> __device__ __forceinline__ void mend_few(const Attn& a, in
   }
 }
 // Packed rows at + i of sequence b and key/value head h, for the bits i of `left`; its rows begin at `start`, its new tokens at position `pos`
-template <int MENDED> static __device__ __noinline__ void mend_rows(const Attn& a, int b, int start, int pos, int h, int at, uint32_t left, int lane) {
+template <int MENDED, bool TREE> static __device__ __noinline__ void mend_rows(const Attn<TREE>& a, int b, int start, int pos, int h, int at, uint32_t left, int lane) {
   const int G = a.heads / a.kv_heads;
+  int n = 0;
+  if constexpr (TREE) {
+    int first_row, length;
+    sequence(a.s, b, first_row, n, length);
+  }
   while (left) {
     Again<MENDED> x;
     x.n = min(__popc(left), MENDED);
@@ -271,11 +317,11 @@ template <int MENDED> static __device__ __noinline__ void mend_rows(const Attn& 
     for (int r = 0; r < MENDED; ++r) {
       const int i = at + (left ? __ffs(left) - 1 : 0);       // (one too many is not looked at)
       left &= left - 1;
-      x.pos[r] = pos + i / G;
+      x.pos[r] = a.position(start, pos, n, min(i / G, TREE ? n - 1 : i / G));
       x.row[r] = start + i / G;
       x.head[r] = h * G + i % G;
     }
-    mend_few<MENDED>(a, b, h, x, lane);
+    mend_few<MENDED>(a, b, h, x, pos, n, lane);
   }
 }
 __device__ __forceinline__ bool finite4(const float (&x)[4], float inv) {
@@ -286,7 +332,7 @@ __device__ __forceinline__ bool finite4(const float (&x)[4], float inv) {
 bool many_takes(int K, int V, int store);
 int many_ctas(long long row_tiles, long long keys, int sms);
 long long many_floats(int ctas, int V);
-int many_launch(Attn& a, int ctas, float* work, cudaStream_t stream);
+template <bool TREE> int many_launch(Attn<TREE>& a, int ctas, float* work, cudaStream_t stream);
 
 }  // namespace paged
 }  // namespace b2l

@@ -201,8 +201,6 @@ __device__ __forceinline__ void bulk(uint32_t dst, const void* src, uint32_t byt
 }
 // the power of two that brings a largest scale (as bits; 0: none) to 1 .. 2
 __device__ __forceinline__ float value_lift(uint32_t bits) { return bits ? __uint_as_float((254u - (bits >> 23)) << 23) : 1.f; }
-// bits 0 .. n-1 (any n)
-__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 // place of the 16-byte piece c of row r in tiles of 128 rows
 __device__ __forceinline__ uint32_t piece_at(int r, int c) { return (uint32_t)((c >> 3) * TC_ATOM + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
 
@@ -258,7 +256,7 @@ struct Cost {
     return y < LEAST ? 0 : units - y < LEAST ? units : y;
   }
 };
-__device__ __forceinline__ Cost cost_of(const Attn& a, const Place& pl) {
+template <bool TREE> __device__ __forceinline__ Cost cost_of(const Attn<TREE>& a, const Place& pl) {
   Cost c;
   c.all = a.keys(pl, ROWS).units(7);
   c.units = max(c.all, 1);
@@ -266,7 +264,7 @@ __device__ __forceinline__ Cost cost_of(const Attn& a, const Place& pl) {
   return c;
 }
 // of one head of a sequence, by a whole warp
-__device__ __forceinline__ long long sequence_cost(const Attn& a, Place pl, int lane) {
+template <bool TREE> __device__ __forceinline__ long long sequence_cost(const Attn<TREE>& a, Place pl, int lane) {
   long long sum = 0;
   for (pl.first = lane * ROWS; pl.first < pl.n * (a.heads / a.kv_heads); pl.first += 32 * ROWS) sum += cost_of(a, pl).total();
 #pragma unroll
@@ -274,7 +272,7 @@ __device__ __forceinline__ long long sequence_cost(const Attn& a, Place pl, int 
   return sum;
 }
 // each sequence lo .. hi - 1 that is this kernel's, until f says true
-template <typename F> __device__ __forceinline__ void each_sequence(const Attn& a, int lo, int hi, int lane, F f) {
+template <bool TREE, typename F> __device__ __forceinline__ void each_sequence(const Attn<TREE>& a, int lo, int hi, int lane, F f) {
   for (int b0 = lo; b0 < hi; b0 += 32) {
     int start = 0, n = 0, length = 0;
     if (b0 + lane < hi) sequence(a.s, b0 + lane, start, n, length);
@@ -285,7 +283,7 @@ template <typename F> __device__ __forceinline__ void each_sequence(const Attn& 
   }
 }
 // the row tile after this one; pl.n is 0 behind the last
-__device__ __forceinline__ void advance(const Attn& a, Walk& w, const Cost& c, int lane) {
+template <bool TREE> __device__ __forceinline__ void advance(const Attn<TREE>& a, Walk& w, const Cost& c, int lane) {
   w.at += c.total();
   if (w.pl.n * (a.heads / a.kv_heads) - w.pl.first > ROWS) {
     w.pl.first += ROWS;
@@ -306,7 +304,7 @@ struct Item {
   int h, t0, t1, n;                                          // n: tiles of keys that its rows see
   bool whole;
 };
-__device__ __forceinline__ bool next(const Attn& a, Control& ct, int warp, int lane, Item& x) {
+template <bool TREE> __device__ __forceinline__ bool next(const Attn<TREE>& a, Control& ct, int warp, int lane, Item& x) {
   Walk w = ct.at[warp];
   const long long x0 = ct.x0, x1 = ct.x1;
   bool found = false;
@@ -331,8 +329,8 @@ __device__ __forceinline__ bool next(const Attn& a, Control& ct, int warp, int l
 
 __device__ __forceinline__ int pl_groups(const Place& pl, int G) { return pl.n * G - pl.first > TILE ? 2 : 1; }
 
-template <int STORE>
-__global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __grid_constant__ Attn a, const __grid_constant__ CUtensorMap map_k,
+template <int STORE, bool TREE>
+__global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __grid_constant__ Attn<TREE> a, const __grid_constant__ CUtensorMap map_k,
                                                                                   const __grid_constant__ CUtensorMap map_v, int k_stages, int v_stages) {
   constexpr bool HALF = STORE != ACT;
   constexpr float LIFT = HALF ? 6.f : 0.f;                   // weights up to 2^14 in f16
@@ -677,7 +675,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
     const Place pl = x.pl;
     const int n = x.n, t0 = x.t0, rows = min(ROWS, pl.n * G - pl.first), groups = pl_groups(pl, G), at = pl.first + TILE * g + r;
     const bool part = !x.whole, live = TILE * g + r < rows;
-    const int token = live ? at / G : 0, head = x.h * G + (live ? at % G : 0), row = pl.start + token, pos = live ? pl.length - pl.n + token : -1;
+    const int token = live ? at / G : 0, head = x.h * G + (live ? at % G : 0), row = pl.start + token, base = pl.length - pl.n, pos = live ? a.position(pl.start, base, pl.n, token) : -1;
     const Keys keys = a.keys(pl, ROWS);
     float cr = a.scale_log2;
     if (n > 0) {
@@ -723,7 +721,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
     float m = -INFINITY, l = 0.f, down = 1.f;
     uint32_t notes = 0;                                      // those of its tiles; bit 31: a score that is NaN or an infinity
     // positions of this group's rows: where all of them see a tile no mask is needed
-    const int p_min = pl.length - pl.n + (pl.first + TILE * g) / G, p_max = pl.length - pl.n + (pl.first + min(TILE * (g + 1), rows) - 1) / G;
+    const int p_min = TREE ? keys.p_min : pl.length - pl.n + (pl.first + TILE * g) / G, p_max = TREE ? keys.p_max : pl.length - pl.n + (pl.first + min(TILE * (g + 1), rows) - 1) / G;
     if (g < groups) {
       const bool idle = !__any_sync(0xffffffffu, live);
       for (int t = 0; t < n; ++t) {
@@ -747,8 +745,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
         // keys that the row sees, as bits of 32
         auto seen = [&](int c) {
           const int j = key0 + 32 * c;
-          uint32_t x = low_bits(pos + 1 - j);
-          if (a.window) x &= ~low_bits(pos - a.window + 1 - j) | low_bits(a.first - j);
+          const uint32_t x = live || !TREE ? a.seen32(pos, row, base, pl.n, j) : 0u;
           return x & (((there >> 2 * c & 1u) ? 0xffffu : 0u) | ((there >> (2 * c + 1) & 1u) ? 0xffff0000u : 0u));
         };
         // scores of keys 64 half .. + 63: hidden ones -inf
@@ -910,7 +907,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
 }
 
 // The row tiles that go on from CTA blockIdx.x to others; a warp has four rows, a lane four columns of each
-__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ Attn a) {
+template <bool TREE> __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ Attn<TREE> a) {
   const int lane = threadIdx.x & 31, G = a.heads / a.kv_heads, r0 = blockIdx.y * 32 + threadIdx.x / 32 * 4;
   pdl_wait();                                                // launched as the last CTAs that compute parts end: they let nothing in earlier
   const int4 last = a.many.last[blockIdx.x];
@@ -991,7 +988,7 @@ static int map_rows(CUtensorMap* m, const void* base, long long rows, int cols, 
   return 0;
 }
 
-template <int STORE> static int go(const Attn& a, int ctas, cudaStream_t stream) {
+template <int STORE, bool TREE> static int go(const Attn<TREE>& a, int ctas, cudaStream_t stream) {
   const Layout l = layout<STORE>(a.K, a.V);
   CUtensorMap mk, mv;
   const long long rows = ((long long)a.s.pages * a.kv_heads) << a.s.shift;
@@ -1004,22 +1001,24 @@ template <int STORE> static int go(const Attn& a, int ctas, cudaStream_t stream)
     if (int rc = map_rows(&mv, a.v, rows, a.V, box)) return rc;
   }
   static DynSmemCache cache;
-  if (int rc = ensure_dyn_smem(paged_many_kernel<STORE>, l.smem, cache)) return rc;
-  paged_many_kernel<STORE><<<(unsigned)ctas, THREADS<STORE>, l.smem, stream>>>(a, mk, mv, l.ks, l.vs);
+  if (int rc = ensure_dyn_smem(paged_many_kernel<STORE, TREE>, l.smem, cache)) return rc;
+  paged_many_kernel<STORE, TREE><<<(unsigned)ctas, THREADS<STORE>, l.smem, stream>>>(a, mk, mv, l.ks, l.vs);
   B2L_LAUNCH_CHECK("paged_many_kernel");
   return 0;
 }
-int many_launch(Attn& a, int ctas, float* work, cudaStream_t stream) {
+template <bool TREE> int many_launch(Attn<TREE>& a, int ctas, float* work, cudaStream_t stream) {
   a.many.last = reinterpret_cast<int4*>(work);
   a.many.ml = work + 4 * ctas;
   a.many.o = a.many.ml + 4ll * ctas * ROWS;
   const int rc = a.store_kind == ACT ? go<ACT>(a, ctas, stream) : a.store_kind == E4M3 ? go<E4M3>(a, ctas, stream) : go<INT8>(a, ctas, stream);
   if (rc || ctas == 1) return rc;
   LaunchCfg launch(dim3((unsigned)ctas, ROWS / 32), dim3(256), 0, stream, true);
-  B2L_CUDA(cudaLaunchKernelEx(&launch.cfg, paged_join_kernel, a));
+  B2L_CUDA(cudaLaunchKernelEx(&launch.cfg, paged_join_kernel<TREE>, a));
   B2L_LAUNCH_CHECK("paged_join_kernel");
   return 0;
 }
+template int many_launch<false>(Attn<false>&, int, float*, cudaStream_t);
+template int many_launch<true>(Attn<true>&, int, float*, cudaStream_t);
 
 }  // namespace paged
 }  // namespace b2l

@@ -1,0 +1,241 @@
+// Trees of drafted tokens: what each token sees, and which of them are accepted.
+//
+// Token i of a sequence's new ones has a parent among those before it (or none: -1), so its ancestors are found by going up.  Its depth is the number of them.
+//   target[r] = argmax_v x[r, v]                    or, drawn, argmax_v x[r, v] / T - log q[r, v], q ~ Exp(1): v with probability softmax(x / T)[v]
+//   path: the first new token; then, as long as there is one, the first child whose token is its parent's target
+// The second launch joins the parts of the rows and goes down the trees, a block for each sequence.
+//
+// What bounds acceptance: logits (and noise) read once.  Values are compared in 64 bits, as two logits may be neighbours: a block finds its largest in f32 and
+// computes those close to it (a margin of 16 times what f32 loses) again.
+#include "seq_paged.cuh"
+#include "seq_rows.cuh"
+
+namespace b2l {
+namespace tree {
+
+// ------------------------------------------------------------------------------------------------ ancestors
+struct Build {
+  const int *parents, *starts, *lengths;
+  uint32_t* masks;
+  int *depths, *positions;
+  int words, rows, seqs, window, first;
+};
+__global__ void __launch_bounds__(128) tree_build_kernel(const __grid_constant__ Build a) {
+  const int row = blockIdx.x * blockDim.x + threadIdx.x;
+  if (row >= a.rows) return;
+  int lo = 0, hi = a.seqs;                                   // starts[lo] <= row < starts[hi], if any
+  const bool in = row >= a.starts[0] && row < a.starts[a.seqs];
+  while (in && hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (a.starts[mid] <= row) lo = mid;
+    else hi = mid;
+  }
+  uint32_t* mask = a.masks + (size_t)row * a.words;
+  if (!in) {
+    for (int w = 0; w < a.words; ++w) mask[w] = 0u;
+    a.depths[row] = 0;
+    a.positions[row] = 0;
+    return;
+  }
+  const int start = max(a.starts[lo], 0), n = min(a.starts[lo + 1], a.rows) - start, base = max(a.lengths[lo], 0) - n;
+  auto parent = [&](int i) {                                 // before its child, or none
+    const int p = a.parents[start + i];
+    return p >= 0 && p < i ? p : -1;
+  };
+  int depth = 0;
+  for (int i = parent(row - start); i >= 0; i = parent(i)) ++depth;
+  int at = a.words - 1, steps = 0;
+  uint32_t bits = 0u;
+  for (int i = row - start; i >= 0; i = parent(i), ++steps) {      // falling, so the words are written from the last on
+    if (i >= 32 * a.words) continue;
+    while (i >> 5 < at) {
+      mask[at--] = bits;
+      bits = 0u;
+    }
+    if (a.window == 0 || steps < a.window || base + depth - steps < a.first) bits |= 1u << (i & 31);
+  }
+  for (; at >= 0; --at, bits = 0u) mask[at] = bits;
+  a.depths[row] = depth;
+  a.positions[row] = base + depth;
+}
+
+// ------------------------------------------------------------------------------------------------ targets
+struct Best { double value; int at; };
+__device__ __forceinline__ bool better(const Best& x, const Best& y) { return x.value > y.value || (x.value == y.value && x.at < y.at); }
+struct Targets {
+  const void* logits;
+  const float* noise;
+  long long ld, ldn;
+  float temperature;
+  int rows, vocab, splits;
+  Best* parts;                                               // [rows][splits]
+};
+constexpr int THREADS = 256, ENTRIES = 16, CHUNK = THREADS * ENTRIES;
+
+template <typename act_t, bool DRAWN>
+__global__ void __launch_bounds__(THREADS) tree_targets_kernel(const __grid_constant__ Targets a) {
+  __shared__ float tops[THREADS / 32];
+  __shared__ Best bests[THREADS / 32];
+  const int row = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const act_t* logits = reinterpret_cast<const act_t*>(a.logits) + row * a.ld;
+  constexpr int VECS = ENTRIES / rows::PER<act_t>;
+  const int at = rows::border(logits) + blockIdx.x * CHUNK;
+  float x[ENTRIES];
+  rows::load<act_t, VECS>(logits, at, a.vocab, -INFINITY, x);
+  auto index = [&](int i) { return at + (i / rows::PER<act_t> * THREADS + (int)threadIdx.x) * rows::PER<act_t> + i % rows::PER<act_t>; };
+  Best best{-INFINITY, INT32_MAX};
+  if constexpr (!DRAWN) {
+#pragma unroll
+    for (int i = 0; i < ENTRIES; ++i)
+      if (x[i] > best.value) best = {x[i], index(i)};        // no NaN; a thread's entries ascend
+  } else {
+    const float* noise = a.noise + row * a.ldn;
+    const float over = 1.f / a.temperature;
+    float y[ENTRIES], top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < ENTRIES; ++i) {
+      const int v = index(i);
+      y[i] = v >= 0 && v < a.vocab ? __ldcs(noise + v) : 1.f;
+    }
+#pragma unroll
+    for (int i = 0; i < ENTRIES; ++i) {
+      // off by less than 2^-20 of its two terms; NaN nowhere (then -inf)
+      const float z = x[i] * over - __logf(y[i]);
+      top = fmaxf(top, z);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) tops[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) top = fmaxf(top, tops[w]);
+#pragma unroll
+    for (int i = 0; i < ENTRIES; ++i) {
+      const float u = x[i] * over, l = __logf(y[i]), z = u - l;
+      if (z == top || z >= top - 1.52587890625e-5f * (1.f + fabsf(u) + fabsf(l) + fabsf(top))) {      // 2^-16
+        const double value = (double)x[i] / (double)a.temperature - log((double)y[i]);
+        const Best here{value, index(i)};
+        if (value > -INFINITY && better(here, best)) best = here;
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const Best other{__shfl_xor_sync(0xffffffffu, best.value, o), __shfl_xor_sync(0xffffffffu, best.at, o)};
+    if (better(other, best)) best = other;
+  }
+  if (lane == 0) bests[warp] = best;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 1; w < THREADS / 32; ++w)
+      if (better(bests[w], best)) best = bests[w];
+    a.parts[(size_t)row * a.splits + blockIdx.x] = best;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ the way down
+struct Walk {
+  const Best* parts;
+  int splits;
+  int* targets;                                              // [rows]
+  const int *parents, *starts;
+  const void* tokens;
+  int wide;                                                  // tokens of 64 bits
+  int rows, seqs;
+  int *kept, *counts, *next;
+};
+__global__ void __launch_bounds__(128) tree_walk_kernel(const __grid_constant__ Walk a) {
+  const int b = blockIdx.x, lane = threadIdx.x & 31;
+  const int start = min(max(a.starts[b], 0), a.rows), n = max(min(a.starts[b + 1], a.rows) - start, 0);
+  if (b == 0)
+    for (int r = threadIdx.x; r < start; r += blockDim.x) a.kept[r] = -1;
+  if (b == a.seqs - 1)
+    for (int r = start + n + threadIdx.x; r < a.rows; r += blockDim.x) a.kept[r] = -1;
+  pdl_wait();
+  for (int r = start + threadIdx.x; r < start + n; r += blockDim.x) {
+    Best best{-INFINITY, INT32_MAX};
+    for (int s = 0; s < a.splits; ++s) {
+      const Best other = a.parts[(size_t)r * a.splits + s];
+      if (better(other, best)) best = other;
+    }
+    a.targets[r] = best.at == INT32_MAX ? 0 : best.at;       // no logit above -inf: the first token
+  }
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
+  int at = 0, count = 0, target = -1;
+  while (at < n) {
+    if (lane == 0) a.kept[start + count] = at;
+    ++count;
+    target = a.targets[start + at];
+    int child = n;
+    for (int j0 = at + 1; j0 < n && child == n; j0 += 32) {
+      const int j = j0 + lane;
+      bool fits = false;
+      if (j < n && a.parents[start + j] == at)
+        fits = a.wide ? reinterpret_cast<const long long*>(a.tokens)[start + j] == target : reinterpret_cast<const int*>(a.tokens)[start + j] == target;
+      const uint32_t mine = __ballot_sync(0xffffffffu, fits);
+      if (mine) child = j0 + __ffs(mine) - 1;
+    }
+    at = child;
+  }
+  for (int i = count + lane; i < n; i += 32) a.kept[start + i] = -1;
+  if (lane == 0) {
+    a.counts[b] = count;
+    a.next[b] = target;
+  }
+}
+
+}  // namespace tree
+}  // namespace b2l
+
+using namespace b2l;
+
+extern "C" int b2l_seq_tree_build(const int* parents, const int* starts, const int* lengths, unsigned* masks, int words, int* depths, int* positions, int rows, int seqs, int window,
+                                  int first, b2l_stream_t stream) {
+  const char* who = "b2l_seq_tree_build";
+  B2L_CHECK_ARG(rows >= 0 && seqs >= 0 && words > 0 && window >= 0 && first >= 0, "%s: bad sizes", who);
+  B2L_CHECK_ARG(rows == 0 || seqs == 0 || (parents && starts && lengths && masks && depths && positions), "%s: null pointer", who);
+  B2L_CHECK_SUPPORTED(rows < (1 << 30), "%s: %d rows", who, rows);
+  if (rows == 0 || seqs == 0) return 0;
+  tree::tree_build_kernel<<<(rows + 127) / 128, 128, 0, (cudaStream_t)stream>>>({parents, starts, lengths, masks, depths, positions, words, rows, seqs, window, first});
+  B2L_LAUNCH_CHECK("tree_build_kernel");
+  return 0;
+}
+
+static int accept_splits(int vocab) { return (vocab + 7 + tree::CHUNK - 1) / tree::CHUNK; }      // 7: a row that does not begin on a border
+
+extern "C" long long b2l_seq_tree_accept_work(int rows, int vocab) {
+  return rows <= 0 || vocab <= 0 ? 0 : (long long)rows * accept_splits(vocab) * (long long)sizeof(tree::Best) + 4ll * rows;
+}
+
+extern "C" int b2l_seq_tree_accept(const void* logits, long long ld, const float* noise, long long ldn, float temperature, const int* parents, const int* starts, const void* tokens,
+                                   int tokens64, int* kept, int* counts, int* next, void* work, long long work_bytes, int rows, int seqs, int vocab, int act_dtype,
+                                   b2l_stream_t stream) {
+  using namespace tree;
+  const char* who = "b2l_seq_tree_accept";
+  B2L_CHECK_ARG(rows >= 0 && seqs >= 0 && vocab > 0, "%s: bad sizes", who);
+  B2L_CHECK_ARG(seqs == 0 || (starts && counts && next), "%s: null pointer", who);
+  B2L_CHECK_ARG(rows == 0 || seqs == 0 || (logits && parents && tokens && kept), "%s: null pointer", who);
+  B2L_CHECK_ARG(ld >= vocab && (!noise || (ldn >= vocab && temperature > 0.f && temperature < INFINITY)), "%s: rows shorter than the vocabulary, or a temperature that is not positive", who);
+  B2L_CHECK_SUPPORTED(rows < 65536 && vocab < (1 << 30), "%s: %d rows over %d tokens", who, rows, vocab);
+  if (seqs == 0) return 0;
+  const long long need = b2l_seq_tree_accept_work(rows, vocab);
+  B2L_CHECK_ARG(need == 0 || (work && work_bytes >= need && ((uintptr_t)work & 15) == 0), "%s: a work space of %lld bytes is needed", who, need);
+  const cudaStream_t st = (cudaStream_t)stream;
+  const int splits = accept_splits(vocab);
+  Best* parts = (Best*)work;
+  if (rows > 0) {
+    const Targets t{logits, noise, ld, ldn, temperature, rows, vocab, splits, parts};
+    B2L_SEQ_DISPATCH(act_dtype, {
+      if (noise) tree_targets_kernel<act_t, true><<<dim3(splits, rows), THREADS, 0, st>>>(t);
+      else tree_targets_kernel<act_t, false><<<dim3(splits, rows), THREADS, 0, st>>>(t);
+    });
+    B2L_LAUNCH_CHECK("tree_targets_kernel");
+  }
+  const Walk w{parts, splits, rows > 0 ? (int*)(parts + (size_t)rows * splits) : nullptr, parents, starts, tokens, tokens64, rows, seqs, kept, counts, next};
+  LaunchCfg launch(dim3((unsigned)seqs), dim3(128), 0, st, rows > 0);
+  B2L_CUDA(cudaLaunchKernelEx(&launch.cfg, tree_walk_kernel, w));
+  B2L_LAUNCH_CHECK("tree_walk_kernel");
+  return 0;
+}

@@ -103,7 +103,14 @@ struct Entry {
   F(b2l_seq_paged_write) \
   F(b2l_seq_paged_read) \
   F(b2l_seq_paged_attention) \
-  F(b2l_seq_paged_attention_all)
+  F(b2l_seq_paged_attention_all) \
+  F(b2l_seq_rope_at) \
+  F(b2l_seq_tree_build) \
+  F(b2l_seq_paged_attention_tree) \
+  F(b2l_seq_tree_accept) \
+  F(b2l_seq_paged_keep) \
+  F(b2l_seq_paged_copy) \
+  F(b2l_seq_beam_select)
 #define ENTRY(name) {#name, Thunk<decltype(&name)>::signature, Thunk<decltype(&name)>::call},
 const Entry entries[] = {ALL(ENTRY)};
 constexpr int N_ENTRIES = (int)(sizeof(entries) / sizeof(entries[0]));

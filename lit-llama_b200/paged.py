@@ -13,10 +13,25 @@
         out = caches[i].attend(q, step)                        # q [513, 32, 128] -> [513, 32, 128]
         pool.release("a")
 
+Several continuations of a sequence, drafted tokens that form a tree or beams:
+
+    PagedTree    the parents of a step's tokens: what each of them sees (for `attend`), and which are accepted
+    PagedLayers  the pools of all layers: pages copied, accepted rows moved together
+    PagePool     `fork`, `reorder`, `own`, `compact`: pages that sequences share are counted, and say which pages have to be copied
+
+        step = pool.step([("b", 4)])                           # the last token and three drafts: two that follow it, one that follows the first of these
+        tree = PagedTree(step, torch.tensor([-1, 0, 0, 1], dtype=torch.int32, device="cuda"))
+        out = caches[i].attend(q, step, tree=tree)
+        kept, counts, following = tree.accept(logits, tokens)
+        layers.keep(step, kept, counts)
+        pool.take_back("b", 4 - int(counts[0]))
+        layers.copy(pool.fork("b", "c"))                       # c goes on from where b stands
+
 A token's key and value rows are quantised by themselves, per head: scale = max(max |x| (1 / c), 2^-126), code = round(x / scale), c = 448 (fp8, e4m3) or 127
 (int8).  A row that holds an infinity or NaN reads back as NaN.  A row whose weights sum to zero (it sees no key) attends to zeros.  Everything
 is a kernel of libb200seq (include/b2l_seq.h); CUDA only, no CPU fallback, no derivatives."""
-from typing import Dict, Hashable, List, Mapping, Optional, Sequence, Tuple
+import ctypes as C
+from typing import Dict, Hashable, List, Mapping, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -98,6 +113,7 @@ class PagePool:
         self._free: List[int] = list(range(self.n_pages - 1, -1, -1))       # page 0 first
         self._pages: Dict[Hashable, List[int]] = {}
         self._length: Dict[Hashable, int] = {}
+        self._shared: Dict[int, int] = {}                                   # pages that more than one sequence has -> how many
 
     def has(self, request_id: Hashable) -> bool:
         return request_id in self._pages
@@ -126,11 +142,23 @@ class PagePool:
     def has_room(self, live: Mapping[Hashable, int], tokens: int, portion: int = 0) -> bool:
         """Whether one more sequence, of `tokens` tokens, finds its pages whatever the sequences of `live` (request id -> the tokens that it grows to) still
         take.  Other sequences are counted with the pages that they have."""
-        held = sum(sum(p >= 0 for p in self._pages.get(rid, ())) for rid in live)
+        held = len({p for rid in live for p in self._pages.get(rid, ()) if p >= 0})
         return len(self._free) + held >= sum(self.most_pages(n, portion) for n in live.values()) + self.most_pages(tokens, portion)
 
+    def _give(self, page: int) -> None:
+        """One sequence no longer has the page: it is free where no other has it."""
+        n = self._shared.get(page, 1)
+        if n == 1:
+            self._free.append(page)
+        elif n == 2:
+            del self._shared[page]
+        else:
+            self._shared[page] = n - 1
+
     def release(self, request_id: Hashable) -> None:
-        self._free += [p for p in reversed(self._pages.pop(request_id)) if p >= 0]
+        for p in reversed(self._pages.pop(request_id)):
+            if p >= 0:
+                self._give(p)
         del self._length[request_id]
 
     def take_back(self, request_id: Hashable, n: int) -> None:
@@ -142,8 +170,83 @@ class PagePool:
         if any(p < 0 and (i * self.page < self.first or (i + 1) * self.page > reach) for i, p in enumerate(pages[:keep])):
             raise ValueError(f"page pool: pages that the window at {length} reaches were given back")
         self._length[request_id] = length
-        self._free += [p for p in reversed(pages[keep:]) if p >= 0]
+        for p in reversed(pages[keep:]):
+            if p >= 0:
+                self._give(p)
         del pages[keep:]
+
+    # ------------------------------------------------------------------ pages that sequences share
+    def _partial(self, request_id: Hashable) -> int:
+        """The page that the sequence's next token lies in, or -1 where that begins one (or the page was given back)."""
+        return self._pages[request_id][-1] if self._length[request_id] % self.page else -1
+
+    def fork(self, source: Hashable, request_id: Hashable) -> List[Tuple[int, int]]:
+        """A new sequence with the tokens of `source`, which stays.  They share the full pages; the one that both go on writing the new one gets a copy of: returns
+        the pages to be copied, (from, to), for `PagedLayers.copy` before either sequence's next step.  Raises PagesFull, with nothing changed."""
+        if request_id in self._pages:
+            raise ValueError(f"page pool: {request_id!r} is a sequence already")
+        return self.reorder({request_id: source})
+
+    def reorder(self, sources: Mapping[Hashable, Hashable]) -> List[Tuple[int, int]]:
+        """Every sequence of `sources` (new ones too) becomes one with the tokens that its source had before the call; others stay.  What a sequence had is given
+        back where no other goes on from it.  Returns the pages to be copied, (from, to), for `PagedLayers.copy` before the next step: none is copied that only one
+        sequence goes on writing.  Raises PagesFull, with nothing changed."""
+        for s in sources.values():
+            if s not in self._pages:
+                raise KeyError(f"page pool: no sequence {s!r}")
+        keeps: Dict[Hashable, Hashable] = {}                                # source -> the sequence that goes on with its last page
+        for s in sources.values():
+            if s not in sources or sources[s] == s:
+                keeps[s] = s
+        for rid, s in sources.items():
+            keeps.setdefault(s, rid)
+        pages = {rid: list(self._pages[s]) for rid, s in sources.items()}
+        copied = [rid for rid, s in sources.items() if keeps[s] != rid and self._partial(s) >= 0]
+        for rid in copied:
+            pages[rid][-1] = -2                                             # to come
+        count: Dict[int, int] = {}
+        for rid in set(self._pages) | set(pages):
+            for p in pages.get(rid, self._pages.get(rid, ())):
+                if p >= 0:
+                    count[p] = count.get(p, 0) + 1
+        had = [p for rid in sources if rid in self._pages for p in self._pages[rid] if p >= 0]
+        free = self._free + [p for p in dict.fromkeys(reversed(had)) if p not in count]
+        if len(copied) > len(free):
+            raise PagesFull(f"{len(copied)} pages are needed, {len(free)} of {self.n_pages} would be free")
+        pairs, lengths = [], {rid: self._length[s] for rid, s in sources.items()}
+        for rid in copied:
+            pages[rid][-1] = free.pop()
+            count[pages[rid][-1]] = 1
+            pairs.append((self._partial(sources[rid]), pages[rid][-1]))
+        self._free, self._shared = free, {p: n for p, n in count.items() if n > 1}
+        self._pages.update(pages)
+        self._length.update(lengths)
+        return pairs
+
+    def own(self, request_id: Hashable) -> List[Tuple[int, int]]:
+        """A copy of the page that the sequence goes on writing where others have it too (after `take_back` into a page that was full when it was shared): the pages
+        to be copied, (from, to)."""
+        page = self._partial(request_id)
+        if page not in self._shared:
+            return []
+        if not self._free:
+            raise PagesFull(f"a page is needed, none of {self.n_pages} is free")
+        to = self._free.pop()
+        self._pages[request_id][-1] = to
+        self._give(page)
+        return [(page, to)]
+
+    def compact(self) -> List[Tuple[int, int]]:
+        """All sequences' pages among the first ones, as many as there are: the pages to be copied, (from, to), for `PagedLayers.copy` before the next step.  Steps
+        that were booked before have the old places."""
+        used = {p for pages in self._pages.values() for p in pages if p >= 0}
+        to = [p for p in range(len(used)) if p not in used]
+        moved = dict(zip(sorted(p for p in used if p >= len(used)), to))
+        for pages in self._pages.values():
+            pages[:] = [moved.get(p, p) for p in pages]
+        self._shared = {moved.get(p, p): n for p, n in self._shared.items()}
+        self._free = list(range(self.n_pages - 1, len(used) - 1, -1))
+        return list(moved.items())
 
     def _behind(self, request_id: Hashable) -> List[int]:
         """Places in the sequence's table that no later token sees."""
@@ -154,19 +257,26 @@ class PagePool:
 
     def step(self, entries: Sequence[Tuple[Hashable, int]], *, width: int = 0) -> PagedStep:
         """Books `n` more tokens for every (request id, n); ids that are not known begin a sequence.  Raises PagesFull, with nothing booked, where the
-        pages do not suffice."""
+        pages do not suffice.  A sequence does not write into a page that others have too: `own` gives it a copy first."""
         if len({rid for rid, _ in entries}) < len(entries):
             raise ValueError("page pool: a request comes twice in one step")
         if any(n < 0 for _, n in entries):
             raise ValueError("page pool: a negative number of tokens")
         behind, new = {rid: self._behind(rid) for rid, _ in entries}, {rid for rid, _ in entries if rid not in self._pages}
         need = sum(max(0, -(-(self._length.get(rid, 0) + n) // self.page) - len(self._pages.get(rid, ()))) for rid, n in entries)
-        if need > len(self._free) + sum(len(b) for b in behind.values()):
+        for rid, n in entries:
+            if n and rid in self._pages and self._partial(rid) in self._shared:
+                raise ValueError(f"page pool: {rid!r} would write into a page that others have too: it needs one of its own first")
+        given: Dict[int, int] = {}
+        for rid, places in behind.items():
+            for i in places:
+                given[self._pages[rid][i]] = given.get(self._pages[rid][i], 0) + 1
+        if need > len(self._free) + sum(n == self._shared.get(p, 1) for p, n in given.items()):
             raise PagesFull(f"{need} pages are needed, {len(self._free)} of {self.n_pages} are free")
         sequences = []
         for rid, _ in entries:
             for i in behind[rid]:
-                self._free.append(self._pages[rid][i])
+                self._give(self._pages[rid][i])
                 self._pages[rid][i] = -1
         for rid, n in entries:
             pages = self._pages.setdefault(rid, [])
@@ -182,6 +292,96 @@ class PagePool:
                 if rid in new:
                     self.release(rid)
             raise
+
+
+def _launch(device: torch.device, name: str, *args) -> None:
+    """A kernel on the device, whichever is the current one."""
+    if device.type != "cuda":
+        raise RuntimeError(f"tensors on {device}: the sequence kernels run on CUDA only (no CPU fallback)")
+    function = getattr(S.lib(), name)
+    if torch._C._cuda_getDevice() == device.index:
+        rc = function(*args, S.stream_ptr())
+    else:
+        with torch.cuda.device(device):
+            rc = function(*args, S.stream_ptr())
+    if rc:
+        S.check(rc, name)
+
+
+def _whole(what: str, x: torch.Tensor, dtype: torch.dtype, device: torch.device, entries: int) -> torch.Tensor:
+    """x, of at least so many entries one behind the other."""
+    if x.dtype != dtype or x.dim() != 1 or x.shape[0] < entries or x.device != device or (x.shape[0] > 1 and x.stride(0) != 1):
+        raise ValueError(f"{what} {tuple(x.shape)} {x.dtype} on {x.device}: [{entries}] {dtype} on {device}, consecutive, is wanted")
+    return x
+
+
+class PagedTree:
+    """The new tokens of a step as trees: parents[r] (int32 [rows], on the device) is the place, among its sequence's new tokens, of the token that row r follows,
+    one before it, or -1 where it follows the sequence as it was.  A token is at the position of its parent and one more (`positions`, int32 [rows], for the rotation of
+    queries and keys); keys and values lie in the order of the rows all the same.
+
+    `attend(.., tree=tree)` lets a token see what was there before the step, its ancestors and itself: the bits of `masks` (int32 [rows, words], bit i of a row for new
+    token i), which may be written over to see others.  `window` and `first`, those of `attend`, hide ancestors out of reach.  `nodes`: the most new tokens that a
+    sequence of the step ever has (by default what the step says of it); tokens from 32 `words` on are not seen.
+
+    The step's tensors and `parents` may be overwritten between replays of a graph that was recorded with them; then `update` belongs into the graph too."""
+
+    def __init__(self, step: PagedStep, parents: torch.Tensor, *, nodes: int = 0, window: int = 0, first: int = 0) -> None:
+        self.step, self.device = step, step.device
+        self.parents = _whole("paged tree: parents", parents, torch.int32, step.device, step.rows)
+        if nodes < 0 or window < 0 or first < 0:
+            raise ValueError("paged tree: a negative number of tokens, window or number of first tokens")
+        self.words = max(1, -(-(int(nodes) or step.max_new or step.rows) // 32))
+        self.window, self.first = min(int(window), 2 ** 30), min(int(first), 2 ** 30)
+        make = step.starts.new_empty if step.seqs else step.starts.new_zeros
+        self.masks, self.depths, self.positions = make((step.rows, self.words)), make((step.rows,)), make((step.rows,))
+        self.update()
+
+    def update(self) -> None:
+        """masks, depths and positions from the parents and the step as they are now."""
+        s = self.step
+        _launch(self.device, "b2l_seq_tree_build", self.parents.data_ptr(), s.starts.data_ptr(), s.lengths.data_ptr(), self.masks.data_ptr(), self.words, self.depths.data_ptr(),
+                self.positions.data_ptr(), s.rows, s.seqs, self.window, self.first)
+
+    def accept(self, logits: torch.Tensor, tokens: torch.Tensor, *, temperature: float = 0.0,
+               noise: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Which of the step's tokens (int32 or int64 [rows]) the model would have chosen itself.  A row's target is the largest of its logits ([rows, vocab], bf16 or
+        f32), with a temperature one drawn from softmax(logits / temperature): the largest of logits / temperature - log noise, the noise (f32 [rows, vocab]) drawn from
+        Exp(1) unless given.  From a sequence's first new token (which is taken) the path goes to a child whose token is its parent's target as long as there is one; so
+        the tokens of the path and the last one's target are what step after step without drafts gives.
+
+        Returns int32 tensors: kept [rows], the places of the path's tokens among the sequence's new ones, -1 behind them; counts [sequences], how many; following
+        [sequences], the last one's target (-1 for a sequence without new tokens)."""
+        s = self.step
+        if logits.dim() != 2 or logits.shape[0] < s.rows or logits.shape[1] < 1 or logits.device != self.device or logits.dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError(f"paged tree: logits {tuple(logits.shape)} {logits.dtype} on {logits.device}, [{s.rows}, vocab] in bf16 or f32 on {self.device} are wanted")
+        if tokens.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"paged tree: tokens in {tokens.dtype}: int32 or int64")
+        tokens = _whole("paged tree: tokens", tokens, tokens.dtype, self.device, s.rows)
+        if not 0.0 <= temperature < float("inf"):
+            raise ValueError(f"paged tree: a temperature of {temperature}")
+        vocab = logits.shape[1]
+        if vocab > 1 and logits.stride(1) != 1 or logits.shape[0] > 1 and logits.stride(0) < vocab:
+            logits = logits.contiguous()
+        if temperature > 0.0:
+            if noise is None:
+                noise = torch.empty((s.rows, vocab), dtype=torch.float32, device=self.device).exponential_(1)
+            if noise.dtype != torch.float32 or noise.dim() != 2 or noise.shape[0] < s.rows or noise.shape[1] != vocab or noise.device != self.device:
+                raise ValueError(f"paged tree: noise {tuple(noise.shape)} {noise.dtype} on {noise.device}, [{s.rows}, {vocab}] in f32 on {self.device} is wanted")
+            if vocab > 1 and noise.stride(1) != 1 or noise.shape[0] > 1 and noise.stride(0) < vocab:
+                noise = noise.contiguous()
+        else:
+            noise = None
+        make = s.starts.new_empty if s.seqs else s.starts.new_full
+        more = () if s.seqs else (-1,)
+        kept, both = make((s.rows,), *more), s.starts.new_empty((2, s.seqs))
+        size = S.lib().b2l_seq_tree_accept_work(s.rows, vocab)
+        work = torch.empty((size,), dtype=torch.uint8, device=self.device) if size else None
+        _launch(self.device, "b2l_seq_tree_accept", logits.data_ptr(), logits.stride(0) if logits.shape[0] > 1 else vocab, noise.data_ptr() if noise is not None else None,
+                noise.stride(0) if noise is not None and noise.shape[0] > 1 else vocab, float(temperature), self.parents.data_ptr(), s.starts.data_ptr(), tokens.data_ptr(),
+                int(tokens.dtype == torch.int64), kept.data_ptr(), both[0].data_ptr(), both[1].data_ptr(), work.data_ptr() if size else None, size, s.rows, s.seqs, vocab,
+                S.act_code(logits.dtype))
+        return kept, both[0], both[1]
 
 
 class PagedCache:
@@ -291,16 +491,20 @@ class PagedCache:
         return k, v
 
     def attend(self, q: torch.Tensor, step: PagedStep, *, scale: Optional[float] = None, window: int = 0, first: int = 0,
-               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+               out: Optional[torch.Tensor] = None, tree: Optional[PagedTree] = None) -> torch.Tensor:
         """Causal softmax attention of the step's tokens (already written) over their sequences:
 
             out[r, h] = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale q[r, h] . k_j), j <= p and (window == 0 or j > p - window or j < first)
 
         q [rows, heads, dim] with heads a multiple of kv_heads (head h reads key/value head h // (heads / kv_heads)), p the position of row r; scale
         dim^-1/2 unless given.  Returns [rows, heads, vdim] (`out`, contiguous, where given); rows of no sequence, behind the step's last one or before its first,
-        are zeros, or as they were in `out`."""
+        are zeros, or as they were in `out`.
+
+        With a `tree` of the step, p is the token's position in it, and of the step's new tokens a row sees those that the tree says, whatever the window."""
         q, s0, s1 = self._rows(q, 0, self.dim, step, "queries")
         rows, heads, _ = q.shape
+        if tree is not None:
+            return self._attend_tree(q, s0, s1, step, tree, scale, window, first, out)
         plan = step._plans.get((rows, heads, scale, window, first, self._sizes))
         if plan is None:
             plan = self._plan(rows, heads, scale, window, first, step)
@@ -312,6 +516,28 @@ class PagedCache:
             raise ValueError(f"paged cache: out must be {(rows, heads, self.vdim)} {self.dtype} on {self.device}, contiguous and 16-byte aligned")
         work = step._tensors[1].new_empty((floats,)) if floats else None          # four bytes an entry
         self._call(name, step, q.data_ptr(), s0, s1, *(self._at or ()), *(step._at or ()), out.data_ptr(), work.data_ptr() if floats else None, floats, *sizes)
+        return out
+
+    def _attend_tree(self, q: torch.Tensor, s0: int, s1: int, step: PagedStep, tree: PagedTree, scale: Optional[float], window: int, first: int,
+                     out: Optional[torch.Tensor]) -> torch.Tensor:
+        if tree.step is not step:
+            raise ValueError("paged cache: the tree of another step")
+        rows, heads = step.rows, q.shape[1]                                 # masks are of these
+        shape = (q.shape[0], heads, self.vdim)
+        plan = step._plans.get((rows, heads, scale, window, first, self._sizes))
+        if plan is None:
+            plan = self._plan(rows, heads, scale, window, first, step)
+        floats, sizes = plan
+        zeros = out is None
+        if zeros:
+            out = (q.new_empty if step.seqs else q.new_zeros)(shape)
+            if shape[0] > rows:
+                out[rows:].zero_()
+        elif out.shape != shape or out.dtype != self.dtype or out.device != self.device or not out.is_contiguous() or out.data_ptr() % 16:
+            raise ValueError(f"paged cache: out must be {shape} {self.dtype} on {self.device}, contiguous and 16-byte aligned")
+        work = step._tensors[1].new_empty((floats,)) if floats else None
+        self._call("b2l_seq_paged_attention_tree", step, q.data_ptr(), s0, s1, *(self._at or ()), *(step._at or ()), tree.masks.data_ptr(), tree.words, tree.depths.data_ptr(), int(zeros),
+                   out.data_ptr(), work.data_ptr() if floats else None, floats, *sizes)
         return out
 
     def _plan(self, rows: int, heads: int, scale: Optional[float], window: int, first: int, step: PagedStep) -> tuple:
@@ -331,3 +557,49 @@ class PagedCache:
         plan = (floats, (rows, step.seqs, self.n_pages, self.page) + sizes + (float(self.dim ** -0.5 if scale is None else scale),) + hints)
         step._plans[(rows, heads, scale, window, first, self._sizes)] = plan
         return plan
+
+
+class PagedLayers:
+    """The pools of all of a model's layers, alike in sizes and types, whose pages are moved together."""
+
+    def __init__(self, caches: Sequence[PagedCache]) -> None:
+        self.caches = list(caches)
+        if not self.caches:
+            raise ValueError("paged layers: no pool")
+        one = self.caches[0]
+        if any(c._sizes != one._sizes or c.device != one.device for c in self.caches):
+            raise ValueError("paged layers: pools of different sizes or types, or on different devices")
+        self.device = one.device
+        self._sizes = one._sizes
+        flat = [a or 0 for c in self.caches for a in (c._at or (0, 0, 0, 0))]
+        self._at = (C.c_void_p * len(flat))(*flat)
+
+    def copy(self, pages: Union[torch.Tensor, Sequence[Tuple[int, int]]]) -> None:
+        """Pages of every layer: (from, to) of each, from the host or as int32 [n, 2] on the device.  No page comes twice as `to`, and none as both.  Pairs with a page
+        outside the pool are left out."""
+        if not isinstance(pages, torch.Tensor):
+            pages = list(pages)
+            if any(not 0 <= p < self._sizes[0] for pair in pages for p in pair):
+                raise ValueError(f"paged layers: pages outside the pool of {self._sizes[0]}")
+            targets = {b for _, b in pages}
+            if len(targets) < len(pages) or targets & {a for a, _ in pages}:
+                raise ValueError("paged layers: a page that is written twice, or copied and written")
+            if not pages:
+                return
+            pages = torch.tensor(pages, dtype=torch.int32).to(self.device)
+        if pages.dtype != torch.int32 or pages.dim() != 2 or pages.shape[1] != 2 or pages.device != self.device or not pages.is_contiguous():
+            raise ValueError(f"paged layers: pages {tuple(pages.shape)} {pages.dtype} on {pages.device}: [n, 2] int32 on {self.device}, contiguous, is wanted")
+        if pages.data_ptr() % 8:
+            pages = pages.clone()
+        _launch(self.device, "b2l_seq_paged_copy", C.addressof(self._at), len(self.caches), pages.data_ptr(), pages.shape[0], *self._sizes)
+
+    def keep(self, step: PagedStep, kept: torch.Tensor, counts: torch.Tensor) -> None:
+        """Of a step's new tokens those of a path (as `PagedTree.accept` returns them: kept int32 [rows], ascending for every sequence, counts int32 [sequences]) moved
+        together in every layer: behind the tokens that the sequence had before the step.  `PagePool.take_back` gives the other tokens' places back."""
+        kept = _whole("paged layers: kept", kept, torch.int32, self.device, step.rows)
+        counts = _whole("paged layers: counts", counts, torch.int32, self.device, step.seqs)
+        if step.device != self.device:
+            raise ValueError(f"paged layers: a step on {step.device} for pools on {self.device}")
+        pages, page, *sizes = self._sizes
+        _launch(self.device, "b2l_seq_paged_keep", C.addressof(self._at), len(self.caches), *(step._at or (None, None, None, 1, 1)), kept.data_ptr(), counts.data_ptr(), step.rows,
+                step.seqs, pages, page, *sizes)
