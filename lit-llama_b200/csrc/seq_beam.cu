@@ -3,10 +3,11 @@
 //   value[w, v] = score[w] + x[w, v] - log sum_u exp x[w, u],    ties to the lowest w V + v
 //
 // Within a beam the order is that of its logits, so one pass over them gives the sum and each part's `count` largest, as keys of 64 bits: the logit as an integer of
-// the same order, and what is left to the lowest index.  A block holds its part in registers.  Its groups of threads have a largest key each; the count-th largest of
-// these is a bound that at least `count` entries reach, all of them in `count` groups, so the few that do are found without a sort and ranked by counting.  A
-// second launch, a block for a group of beams, does the same with the beams' parts, by values in 64 bits (scores and logits of different beams may be
-// neighbours: what f32 keeps of a sum of 32000 terms would change their order).
+// the same order, and what is left to the lowest index.  A block holds its part in registers, bf16 as it lies.  Its threads, by fours where few are wanted, have a largest
+// value each; the count-th largest of these is a bound that at least `count` entries reach and few more (18 for 16 of 8192 at random), so these are found without a
+// sort, and ranked by counting.  Where more than a list holds reach it, entries alike, keys take the place of values in the same steps: then they are all in `count`
+// threads' entries.  A second launch, a block for a group of beams, does the same with the beams' parts, by values in 64 bits (scores and logits of different beams
+// may be neighbours: what f32 keeps of a sum of 32000 terms would change their order).
 //
 // A beam whose score or log-probabilities are no numbers (a score of -inf, a logit that is NaN or +inf, none above -inf) is out: its values are -inf.
 //
@@ -42,142 +43,248 @@ struct Select {
   int groups, beams, vocab, count, splits;
   unsigned long long* keys;                                  // [rows][splits][count]
   double* sums;                                              // [rows][splits], of exp(x - largest)
-  float* tops;                                               // [rows][splits]; +inf: a logit that is no number or +inf
+  float* tops;                                               // [rows][splits]; +inf: a logit is NaN or +inf
   float* values;
   int *from, *tokens;
 };
 
+// A block's entries as they lie: 16 bytes of a row at a time, -inf where there is none
+template <typename act_t, int VECS> struct Entries;
+template <int VECS> struct Entries<float, VECS> {
+  float x[4 * VECS];
+  __device__ __forceinline__ void load(const float* row, int at, int n) { rows::load<float, VECS>(row, at, n, -INFINITY, x); }
+  __device__ __forceinline__ float operator[](int i) const { return x[i]; }
+  __device__ __forceinline__ float top() const {             // NaN if one is
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < 4 * VECS; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(x[i]));
+    return m;
+  }
+};
+template <int VECS> struct Entries<__nv_bfloat16, VECS> {
+  uint32_t w[4 * VECS];
+  __device__ __forceinline__ void load(const __nv_bfloat16* row, int at, int n) {
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) {
+      const int i = at + (v * (int)blockDim.x + (int)threadIdx.x) * 8;
+      if (i >= 0 && i + 8 <= n) {
+        const uint4 u = __ldcs(reinterpret_cast<const uint4*>(row + i));
+        w[4 * v] = u.x; w[4 * v + 1] = u.y; w[4 * v + 2] = u.z; w[4 * v + 3] = u.w;
+      } else {
+        const uint16_t* bits = reinterpret_cast<const uint16_t*>(row);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int k = i + 2 * e;
+          w[4 * v + e] = (k >= 0 && k < n ? bits[k] : 0xff80u) | (uint32_t)(k + 1 >= 0 && k + 1 < n ? bits[k + 1] : 0xff80u) << 16;
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ float operator[](int i) const { return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16); }
+  __device__ __forceinline__ float top() const {             // two at a time
+    uint32_t m = w[0];
+#pragma unroll
+    for (int i = 1; i < 4 * VECS; ++i) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i]));
+    float lo = __uint_as_float(m << 16);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(__uint_as_float(m & 0xffff0000u)));
+    return lo;
+  }
+};
+__device__ __forceinline__ float larger(float x, float y) {  // NaN if one is
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(y));
+  return x;
+}
+__device__ __forceinline__ float exp2_f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float2 add2(float2 x, float2 y) {
+  float2 z;
+  asm("{\n\t.reg .b64 u, v;\n\tmov.b64 u, {%2, %3};\n\tmov.b64 v, {%4, %5};\n\tadd.rn.f32x2 u, u, v;\n\tmov.b64 {%0, %1}, u;\n\t}" : "=f"(z.x), "=f"(z.y) : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
+  return z;
+}
+// e^(x + c) and e^(y + c) by powers of two
+__device__ __forceinline__ float2 powers2(float x, float y, float c) {
+  const float2 d = add2(make_float2(x, y), make_float2(c, c));
+  float2 e;
+  asm("{\n\t.reg .b64 u, v;\n\tmov.b64 u, {%2, %3};\n\tmov.b64 v, {%4, %4};\n\tmul.rn.f32x2 u, u, v;\n\tmov.b64 {%0, %1}, u;\n\t}"
+      : "=f"(e.x), "=f"(e.y) : "f"(d.x), "f"(d.y), "f"(1.44269502162933349609375f));      // log2(e)
+  return make_float2(exp2_f(e.x), exp2_f(e.y));
+}
+
 template <typename act_t, int ENTRIES>
-__global__ void __launch_bounds__(THREADS) beam_parts_kernel(const __grid_constant__ Select a) {
+__global__ void __launch_bounds__(THREADS, ENTRIES == 32 ? (sizeof(act_t) == 2 ? 5 : 4) : 8) beam_parts_kernel(const __grid_constant__ Select a) {
   __shared__ float tops[THREADS / 32];
   __shared__ double sums[THREADS / 32];
-  __shared__ __align__(16) unsigned long long bests[THREADS];
-  __shared__ unsigned long long bound, list[LIST];
+  __shared__ __align__(16) unsigned long long bests[THREADS], list[LIST];
+  __shared__ unsigned long long bound;
+  __shared__ uint32_t least_bits;
   __shared__ int found;
+  pdl_launch_dependents();                                   // the second launch waits for the end of this one
   const int row = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const act_t* logits = reinterpret_cast<const act_t*>(a.logits) + row * a.ld;
   constexpr int PER = rows::PER<act_t>;
   const int at = rows::border(logits) + blockIdx.x * THREADS * ENTRIES;
-  float x[ENTRIES];
-  rows::load<act_t, ENTRIES / PER>(logits, at, a.vocab, -INFINITY, x);
+  Entries<act_t, ENTRIES / PER> x;
+  x.load(logits, at, a.vocab);
   auto index = [&](int i) { return at + (i / PER * THREADS + (int)threadIdx.x) * PER + i % PER; };
-  auto key = [&](int i) {
+  auto key = [&](int i) -> unsigned long long {
     const int v = index(i);
-    return v >= 0 && v < a.vocab ? (unsigned long long)ordered(x[i]) << 32 | (uint32_t)~v : 0ull;
+    return v >= 0 && v < a.vocab ? (unsigned long long)ordered(ld_act(logits, v)) << 32 | (uint32_t)~v : 0ull;
   };
-  float top = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < ENTRIES; ++i) {
-    if (!(x[i] < INFINITY)) x[i] = INFINITY;
-    top = fmaxf(top, x[i]);
+  const float mine = x.top();
+  const int lanes = lanes_of(a.count), groups = THREADS / lanes;
+  float group = mine;
+  if (lanes == 4) {
+    group = larger(group, __shfl_xor_sync(0xffffffffu, group, 1));
+    group = larger(group, __shfl_xor_sync(0xffffffffu, group, 2));
   }
-  const float mine = top;
+  uint32_t* firsts = reinterpret_cast<uint32_t*>(bests);     // the groups' largest as integers
+  if (threadIdx.x % lanes == 0) firsts[threadIdx.x / lanes] = ordered(group);
+  float top = group;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  for (int o = 16; o > 0; o >>= 1) top = larger(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (lane == 0) tops[warp] = top;
   if (threadIdx.x == 0) {
     found = 0;
     bound = 0ull;
+    least_bits = 0xffffffffu;
   }
-  // this thread's largest entry, the first of equal ones (they ascend)
-  unsigned long long best = 0ull;
-#pragma unroll
-  for (int i = ENTRIES - 1; i >= 0; --i)
-    if (x[i] == mine) {
-      const unsigned long long k = key(i);
-      if (k) best = k;
-    }
-  const int lanes = lanes_of(a.count), keys = THREADS / lanes;
-  if (lanes == 4) {
-    for (int o = 1; o < 4; o <<= 1) {
-      const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
-      best = max(best, other);
-    }
-  }
-  if (threadIdx.x % lanes == 0) bests[threadIdx.x / lanes] = best;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) top = fmaxf(top, tops[w]);
-  // in pairs: five roundings at most, where one behind the other would be 32 (the rest of the sum is in 64 bits)
-  float sum[ENTRIES / 4];
-  if (top > -INFINITY && top < INFINITY) {
-#pragma unroll
-    for (int i = 0; i < ENTRIES; i += 4) sum[i / 4] = (expf(x[i] - top) + expf(x[i + 1] - top)) + (expf(x[i + 2] - top) + expf(x[i + 3] - top));
-#pragma unroll
-    for (int n = ENTRIES / 8; n > 0; n /= 2)
-#pragma unroll
-      for (int i = 0; i < n; ++i) sum[i] += sum[i + n];
-  } else {
-    sum[0] = 0.f;
+  for (int w = 0; w < THREADS / 32; ++w) top = larger(top, tops[w]);
+  const bool out = !(top > -INFINITY && top < INFINITY);     // no sum, no order: the second launch does not look at its keys unless the others' parts have numbers
+  // the count-th largest of the groups' values, by counting how many are larger
+  if ((int)threadIdx.x < groups) {
+    const uint32_t own = firsts[threadIdx.x];
+    int above = 0;
+    for (int i = 0; i < groups; i += 4) {
+      const uint4 y = *reinterpret_cast<const uint4*>(&firsts[i]);
+      above += (y.x > own) + (y.y > own) + (y.z > own) + (y.w > own);
+    }
+    if (above < a.count) atomicMin(&least_bits, own);
   }
-  double all = sum[0];
+  // the sum in pairs: five roundings at most, where one behind the other would be 32 (the rest of it is in 64 bits)
+  float2 sum[ENTRIES / 4];
+  const float ref = out ? 0.f : -top;
+#pragma unroll
+  for (int i = 0; i < ENTRIES; i += 4) {                     // the differences are exact, or rounded once
+    const float2 u = powers2(x[i], x[i + 1], ref), v = powers2(x[i + 2], x[i + 3], ref);
+    sum[i / 4] = add2(u, v);
+  }
+#pragma unroll
+  for (int n = ENTRIES / 8; n > 0; n /= 2)
+#pragma unroll
+    for (int i = 0; i < n; ++i) sum[i] = add2(sum[i], sum[i + n]);
+  double all = sum[0].x + sum[0].y;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
   if (lane == 0) sums[warp] = all;
-  // the count-th largest of the groups' keys, by counting how many are larger; with fewer groups that have entries than that, all there are
-  if ((int)threadIdx.x < keys) {
-    const unsigned long long own = bests[threadIdx.x];
-    int rank = 0;
-    for (int i = 0; i < keys; i += 2) {
-      const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(&bests[i]);
-      rank += (y.x > own) + (y.y > own);
-    }
-    if (rank == a.count - 1 && own) bound = own;
-  }
   __syncthreads();
-  const unsigned long long least = max(bound, 1ull);
   if (threadIdx.x == 0) {
     double s = 0.0;
     for (int w = 0; w < THREADS / 32; ++w) s += sums[w];
-    a.sums[(size_t)row * a.splits + blockIdx.x] = s;
-    a.tops[(size_t)row * a.splits + blockIdx.x] = top;
+    a.sums[(size_t)row * a.splits + blockIdx.x] = out ? 0.0 : s;
+    a.tops[(size_t)row * a.splits + blockIdx.x] = top != top ? INFINITY : top;
   }
-  if (best >= least)
+  // Entries that reach the bound, found again where they come from: what to do with each is written once, not ENTRIES times
+  const float least = unordered(least_bits);
+  if (mine >= least) {
+    uint32_t hits = 0u;
 #pragma unroll
-    for (int i = 0; i < ENTRIES; ++i) {
-      const unsigned long long k = key(i);
-      if (k >= least) {
-        const int to = atomicAdd(&found, 1);
-        if (to < LIST) list[to] = k;
-      }
+    for (int i = 0; i < ENTRIES; ++i) hits |= x[i] >= least ? 1u << i : 0u;
+    if (__popc(hits) + found > LIST) atomicMax(&found, LIST + 1);      // many alike: not one after the other
+    for (; hits && found <= LIST; hits &= hits - 1) {
+      const unsigned long long k = key(__ffs(hits) - 1);
+      const int to = k ? atomicAdd(&found, 1) : LIST;
+      if (to < LIST) list[to] = k;
     }
+  }
   __syncthreads();
+  if (found > LIST) {                                        // by keys, which are all different
+    unsigned long long best = 0ull;
+#pragma unroll 4
+    for (int i = 0; i < ENTRIES; ++i) best = max(best, key(i));
+    if (lanes == 4) {
+      best = max(best, __shfl_xor_sync(0xffffffffu, best, 1));
+      best = max(best, __shfl_xor_sync(0xffffffffu, best, 2));
+    }
+    if (threadIdx.x % lanes == 0) bests[threadIdx.x / lanes] = best;
+    __syncthreads();
+    if (threadIdx.x == 0) found = 0;
+    if ((int)threadIdx.x < groups) {
+      const unsigned long long own = bests[threadIdx.x];
+      int above = 0;
+      for (int i = 0; i < groups; ++i) above += bests[i] > own;
+      if (above == a.count - 1 && own) bound = own;          // with fewer groups that have entries than that, all there are
+    }
+    __syncthreads();
+    const unsigned long long from = max(bound, 1ull);
+    if (best >= from)
+#pragma unroll 4
+      for (int i = 0; i < ENTRIES; ++i) {
+        const unsigned long long k = key(i);
+        if (k >= from) {
+          const int to = atomicAdd(&found, 1);
+          if (to < LIST) list[to] = k;
+        }
+      }
+    __syncthreads();
+  }
   const int n = min(found, LIST);
-  unsigned long long* out = a.keys + ((size_t)row * a.splits + blockIdx.x) * a.count;
+  unsigned long long* keys = a.keys + ((size_t)row * a.splits + blockIdx.x) * a.count;
   for (int i = threadIdx.x; i < n; i += THREADS) {
     const unsigned long long own = list[i];
     int rank = 0;
     for (int j = 0; j < n; ++j) rank += list[j] > own;
-    if (rank < a.count) out[rank] = own;
+    if (rank < a.count) keys[rank] = own;
   }
-  for (int i = n + (int)threadIdx.x; i < a.count; i += THREADS) out[i] = 0ull;
+  for (int i = n + (int)threadIdx.x; i < a.count; i += THREADS) keys[i] = 0ull;
 }
 
+constexpr int HELD = 8;              // entries of a thread that stay in registers
 __global__ void __launch_bounds__(THREADS) beam_select_kernel(const __grid_constant__ Select a) {
   __shared__ double offset[MOST_BEAMS];                      // score less the logarithm of the sum of exp(x - largest); NaN: the beam is out
   __shared__ float largest[MOST_BEAMS];
-  __shared__ Key bests[THREADS], list[LIST], bound;
+  __shared__ __align__(16) unsigned long long firsts[THREADS];
+  __shared__ Key list[LIST / 2];
+  __shared__ unsigned long long least_bits;
   __shared__ int found;
   const int group = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = a.splits * a.count, all = a.beams * per;
-  pdl_wait();
+  const unsigned long long* keys = a.keys + (size_t)group * all;
   if (threadIdx.x == 0) {
     found = 0;
-    bound = Key{0ull, 0u};
+    least_bits = ~0ull;
+  }
+  pdl_wait();
+  unsigned long long held[HELD];
+#pragma unroll
+  for (int k = 0; k < HELD; ++k) {
+    const int i = threadIdx.x + THREADS * k;
+    held[k] = i < all ? keys[i] : 0ull;
   }
   for (int w = warp; w < a.beams; w += THREADS / 32) {       // a warp for a beam
     const size_t at = ((size_t)group * a.beams + w) * a.splits;
-    float top = -INFINITY;
-    for (int s = lane; s < a.splits; s += 32) top = fmaxf(top, a.tops[at + s]);
+    const float score = a.scores[(size_t)group * a.beams + w];
+    float top = -INFINITY, t = -INFINITY;
+    double s = 0.0;
+    if (lane < a.splits) {
+      t = a.tops[at + lane];
+      s = a.sums[at + lane];
+    }
+    top = t;
+    for (int i = lane + 32; i < a.splits; i += 32) top = fmaxf(top, a.tops[at + i]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    double sum = 0.0;
-    for (int s = lane; s < a.splits; s += 32) {
-      const float t = a.tops[at + s];
-      if (t > -INFINITY) sum += a.sums[at + s] * exp((double)t - (double)top);
+    double sum = t > -INFINITY ? s * exp((double)t - (double)top) : 0.0;
+    for (int i = lane + 32; i < a.splits; i += 32) {
+      const float u = a.tops[at + i];
+      if (u > -INFINITY) sum += a.sums[at + i] * exp((double)u - (double)top);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const float score = a.scores[(size_t)group * a.beams + w];
     const bool out = !(top > -INFINITY && top < INFINITY && fabsf(score) < INFINITY);
     if (lane == 0) {
       offset[w] = out ? NAN : (double)score - log(sum);
@@ -185,12 +292,13 @@ __global__ void __launch_bounds__(THREADS) beam_select_kernel(const __grid_const
     }
   }
   __syncthreads();
-  const unsigned long long* keys = a.keys + (size_t)group * all;
-  auto entry = [&](int i) -> Key {                           // of a beam's and a part's largest the next
-    const int w = i / per, r = i - w * per;
+  auto entry = [&](int i, unsigned long long k) -> Key {     // of a beam's and a part's largest the next
+    const int w = i / per;
     const double c = offset[w];
-    if (c != c) return r < a.count && r < a.vocab ? Key{ordered(-(double)INFINITY), (uint32_t)w * a.vocab + r} : Key{0ull, 0u};
-    const unsigned long long k = keys[i];
+    if (c != c) {
+      const int r = i - w * per;
+      return r < a.count && r < a.vocab ? Key{ordered(-(double)INFINITY), (uint32_t)w * a.vocab + r} : Key{0ull, 0u};
+    }
     return k ? Key{ordered(c + ((double)unordered((uint32_t)(k >> 32)) - (double)largest[w])), (uint32_t)w * a.vocab + (uint32_t)~k} : Key{0ull, 0u};
   };
   auto put = [&](const Key& k, int rank) {
@@ -199,58 +307,75 @@ __global__ void __launch_bounds__(THREADS) beam_select_kernel(const __grid_const
     a.from[to] = (int)(k.lo / (uint32_t)a.vocab);
     a.tokens[to] = (int)(k.lo % (uint32_t)a.vocab);
   };
-  if (a.count * ((all + THREADS - 1) / THREADS) > LIST) {    // more than the list is sure to hold: one after the other
-    Key last{~0ull, 0u};
-    for (int r = 0; r < a.count; ++r) {
-      Key best{0ull, 0u};
-      for (int i = threadIdx.x; i < all; i += THREADS) {
-        const Key k = entry(i);
-        if (k.hi && before(last, k) && (best.hi == 0ull || before(k, best))) best = k;
-      }
+  unsigned long long mine = 0ull, values[HELD];
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const Key other{__shfl_xor_sync(0xffffffffu, best.hi, o), __shfl_xor_sync(0xffffffffu, best.lo, o)};
-        if (other.hi && (best.hi == 0ull || before(other, best))) best = other;
-      }
-      if (lane == 0) bests[warp] = best;
-      __syncthreads();
-      for (int w = 0; w < THREADS / 32; ++w)
-        if (bests[w].hi && (best.hi == 0ull || before(bests[w], best))) best = bests[w];
-      if (threadIdx.x == 0) put(best, r);
-      last = best;
-      __syncthreads();
+  for (int k = 0; k < HELD; ++k) {
+    const int i = threadIdx.x + THREADS * k;
+    values[k] = i < all ? entry(i, held[k]).hi : 0ull;
+    mine = max(mine, values[k]);
+  }
+  for (int i = threadIdx.x + THREADS * HELD; i < all; i += THREADS) mine = max(mine, entry(i, keys[i]).hi);
+  const int lanes = lanes_of(a.count), groups = THREADS / lanes;
+  unsigned long long best = mine;
+  if (lanes == 4) {
+    best = max(best, __shfl_xor_sync(0xffffffffu, best, 1));
+    best = max(best, __shfl_xor_sync(0xffffffffu, best, 2));
+  }
+  if (threadIdx.x % lanes == 0) firsts[threadIdx.x / lanes] = best;
+  __syncthreads();
+  if ((int)threadIdx.x < groups) {
+    const unsigned long long own = firsts[threadIdx.x];
+    int above = 0;
+    for (int i = 0; i < groups; i += 2) {
+      const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(&firsts[i]);
+      above += (y.x > own) + (y.y > own);
+    }
+    if (above < a.count) atomicMin(&least_bits, own);
+  }
+  __syncthreads();
+  const unsigned long long least = max(least_bits, 1ull);
+  if (mine >= least) {
+    auto take = [&](int i, unsigned long long k) {
+      const int to = atomicAdd(&found, 1);
+      if (to < LIST / 2) list[to] = entry(i, k);
+    };
+#pragma unroll
+    for (int k = 0; k < HELD; ++k)
+      if (values[k] >= least) take(threadIdx.x + THREADS * k, held[k]);
+    for (int i = threadIdx.x + THREADS * HELD; i < all; i += THREADS)
+      if (entry(i, keys[i]).hi >= least) take(i, keys[i]);
+  }
+  __syncthreads();
+  const int n = found;
+  if (n <= LIST / 2) {
+    for (int i = threadIdx.x; i < n; i += THREADS) {
+      const Key own = list[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += before(list[j], own);
+      if (rank < a.count) put(own, rank);
     }
     return;
   }
-  Key best{0ull, 0u};
-  for (int i = threadIdx.x; i < all; i += THREADS) {
-    const Key k = entry(i);
-    if (k.hi && (best.hi == 0ull || before(k, best))) best = k;
-  }
-  bests[threadIdx.x] = best;
-  __syncthreads();
-  if (best.hi) {
-    int rank = 0;
-    for (int i = 0; i < THREADS; ++i) rank += bests[i].hi && before(bests[i], best);
-    if (rank == a.count - 1) bound = best;
-  }
-  __syncthreads();
-  const Key least = bound;                                   // none: fewer threads than that have entries
-  if (best.hi && (least.hi == 0ull || !before(least, best)))
+  // more values alike than the list holds: one after the other
+  Key last{~0ull, 0u};
+  for (int r = 0; r < a.count; ++r) {
+    Key next{0ull, 0u};
     for (int i = threadIdx.x; i < all; i += THREADS) {
-      const Key k = entry(i);
-      if (k.hi && (least.hi == 0ull || !before(least, k))) {
-        const int to = atomicAdd(&found, 1);
-        if (to < LIST) list[to] = k;
-      }
+      const Key k = entry(i, keys[i]);
+      if (k.hi && before(last, k) && (next.hi == 0ull || before(k, next))) next = k;
     }
-  __syncthreads();
-  const int n = min(found, LIST);
-  for (int i = threadIdx.x; i < n; i += THREADS) {
-    const Key own = list[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += before(list[j], own);
-    if (rank < a.count) put(own, rank);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const Key other{__shfl_xor_sync(0xffffffffu, next.hi, o), __shfl_xor_sync(0xffffffffu, next.lo, o)};
+      if (other.hi && (next.hi == 0ull || before(other, next))) next = other;
+    }
+    if (lane == 0) list[warp] = next;
+    __syncthreads();
+    for (int w = 0; w < THREADS / 32; ++w)
+      if (list[w].hi && (next.hi == 0ull || before(list[w], next))) next = list[w];
+    if (threadIdx.x == 0) put(next, r);
+    last = next;
+    __syncthreads();
   }
 }
 

@@ -6,7 +6,7 @@
 // The second launch joins the parts of the rows and goes down the trees, a block for each sequence.
 //
 // What bounds acceptance: logits (and noise) read once.  Values are compared in 64 bits, as two logits may be neighbours: a block finds its largest in f32 and
-// computes those close to it (a margin of 16 times what f32 loses) again.
+// computes those that f32 cannot tell from it again.
 #include "seq_paged.cuh"
 #include "seq_rows.cuh"
 
@@ -76,6 +76,8 @@ template <typename act_t, bool DRAWN>
 __global__ void __launch_bounds__(THREADS) tree_targets_kernel(const __grid_constant__ Targets a) {
   __shared__ float tops[THREADS / 32];
   __shared__ Best bests[THREADS / 32];
+  __shared__ int list[DRAWN ? CHUNK : 1], found;
+  pdl_launch_dependents();                                   // the second launch waits for the end of this one
   const int row = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const act_t* logits = reinterpret_cast<const act_t*>(a.logits) + row * a.ld;
   constexpr int VECS = ENTRIES / rows::PER<act_t>;
@@ -92,16 +94,24 @@ __global__ void __launch_bounds__(THREADS) tree_targets_kernel(const __grid_cons
     const float* noise = a.noise + row * a.ldn;
     const float over = 1.f / a.temperature;
     float y[ENTRIES], top = -INFINITY;
+    const bool even = ((uintptr_t)(noise + at) & 15) == 0;
 #pragma unroll
-    for (int i = 0; i < ENTRIES; ++i) {
+    for (int i = 0; i < ENTRIES; i += 4) {
       const int v = index(i);
-      y[i] = v >= 0 && v < a.vocab ? __ldcs(noise + v) : 1.f;
-    }
+      if (even && v >= 0 && v + 4 <= a.vocab) {
+        const float4 u = __ldcs(reinterpret_cast<const float4*>(noise + v));
+        y[i] = u.x; y[i + 1] = u.y; y[i + 2] = u.z; y[i + 3] = u.w;
+      } else {
 #pragma unroll
-    for (int i = 0; i < ENTRIES; ++i) {
-      // off by less than 2^-20 of its two terms; NaN nowhere (then -inf)
-      const float z = x[i] * over - __logf(y[i]);
-      top = fmaxf(top, z);
+        for (int e = 0; e < 4; ++e) y[i + e] = v + e >= 0 && v + e < a.vocab ? __ldcs(noise + v + e) : 1.f;
+      }
+    }
+    if (threadIdx.x == 0) found = 0;
+    constexpr float LN2 = 0.693147182464599609375f, SLACK = 1.9073486328125e-6f;      // 2^-19
+#pragma unroll
+    for (int i = 0; i < ENTRIES; ++i) {                      // x / T - log q, off by less than 2^-21 of its two terms together
+      asm("lg2.approx.f32 %0, %1;" : "=f"(y[i]) : "f"(y[i]));
+      top = fmaxf(top, fmaf(y[i], -LN2, x[i] * over));       // NaN: not the largest
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -109,14 +119,22 @@ __global__ void __launch_bounds__(THREADS) tree_targets_kernel(const __grid_cons
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) top = fmaxf(top, tops[w]);
+    // Those near the largest, one or two, again in 64 bits: x / T is no larger than its difference and the logarithm together, and a logarithm at most 104, so the largest
+    // is off by 2^-21 (208 + |top|) at most and one near it by 2^-21 (|top| + 2 |log q|)
+    const float least = top - SLACK * (64.f + 2.f * fabsf(top));
+    uint32_t hits = 0u;
 #pragma unroll
     for (int i = 0; i < ENTRIES; ++i) {
-      const float u = x[i] * over, l = __logf(y[i]), z = u - l;
-      if (z == top || z >= top - 1.52587890625e-5f * (1.f + fabsf(u) + fabsf(l) + fabsf(top))) {      // 2^-16
-        const double value = (double)x[i] / (double)a.temperature - log((double)y[i]);
-        const Best here{value, index(i)};
-        if (value > -INFINITY && better(here, best)) best = here;
-      }
+      const float z = fmaf(y[i], -LN2, x[i] * over);
+      hits |= fmaf(fabsf(y[i]), SLACK, z) >= least || z == top ? 1u << i : 0u;
+    }
+    for (; hits; hits &= hits - 1) list[atomicAdd(&found, 1)] = index(__ffs(hits) - 1);
+    __syncthreads();
+    for (int i = threadIdx.x; i < found; i += THREADS) {
+      const int v = list[i];
+      if (v < 0 || v >= a.vocab) continue;
+      const Best here{(double)ld_act(logits, v) / (double)a.temperature - log((double)noise[v]), v};
+      if (here.value > -INFINITY && better(here, best)) best = here;
     }
   }
 #pragma unroll
