@@ -542,7 +542,7 @@ long long b2l_seq_paged_attention_work(int rows, int seqs, int width, int page, 
  *                                 `first`.  Tokens from 32 words on have no bit.  A row of no sequence: zeros.
  *   b2l_seq_paged_attention_tree  b2l_seq_paged_attention over the context (keys before the new tokens; the window counts from the row's position, depths
  *                                 clipped to 0 .. rows of b - 1) and, of the new tokens, those of the row's mask (any mask).  zeros: whether the outputs of rows of no
- *                                 sequence become zeros (else they stay).  Its work space is b2l_seq_paged_attention_work's.
+ *                                 sequence become zeros (else they stay).  `work` has b2l_seq_paged_attention_tree_work floats.
  *   b2l_seq_tree_accept           target[r] = argmax_v x[r, v], or with noise (f32 [rows, ldn]) argmax_v x[r, v] / temperature - log noise[r, v], which draws v with
  *                                 probability softmax(x / temperature)[v] where the noise is Exp(1); ties to the lowest v, a NaN is nowhere the largest, 0 where
  *                                 nothing is above -inf.  x act [rows, ld].  Then from each sequence's first new token on: its first child (of the lowest place)
@@ -566,6 +566,8 @@ int b2l_seq_paged_attention_tree(const void* q, long long ldq, long long hsq, co
                                  const int* lengths, const int* table, int ldt, int width, const unsigned* masks, int words, const int* depths, int zeros, void* out,
                                  float* work, long long work_floats, int rows, int seqs, int pages, int page, int heads, int kv_heads, int K, int V, int window, int first,
                                  float scale, int max_new, int max_length, int store, int act_dtype, b2l_stream_t stream);
+long long b2l_seq_paged_attention_tree_work(int rows, int seqs, int width, int page, int heads, int kv_heads, int K, int V, int window, int first, int max_new,
+                                            int max_length, int store, int act_dtype);
 int b2l_seq_tree_accept(const void* logits, long long ld, const float* noise, long long ldn, float temperature, const int* parents, const int* starts, const void* tokens,
                         int tokens64, int* kept, int* counts, int* next, void* work, long long work_bytes, int rows, int seqs, int vocab, int act_dtype,
                         b2l_stream_t stream);

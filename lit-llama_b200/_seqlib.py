@@ -225,6 +225,7 @@ _SIGS = {
     "b2l_seq_tree_build": (c_int, [c_void_p] * 4 + [c_int] + [c_void_p] * 2 + [c_int] * 4 + [c_void_p]),
     "b2l_seq_paged_attention_tree": (c_int, [c_void_p, C.c_longlong, C.c_longlong] + [c_void_p] * 7 + [c_int] * 2 + [c_void_p, c_int, c_void_p, c_int] + [c_void_p] * 2 + [C.c_longlong]
                                      + [c_int] * 10 + [c_float] + [c_int] * 4 + [c_void_p]),
+    "b2l_seq_paged_attention_tree_work": (C.c_longlong, [c_int] * 14),
     "b2l_seq_tree_accept": (c_int, [c_void_p, C.c_longlong] * 2 + [c_float] + [c_void_p] * 3 + [c_int] + [c_void_p] * 4 + [C.c_longlong] + [c_int] * 4 + [c_void_p]),
     "b2l_seq_tree_accept_work": (C.c_longlong, [c_int] * 2),
     "b2l_seq_paged_keep": (c_int, [c_void_p, c_int] + [c_void_p] * 3 + [c_int] * 2 + [c_void_p] * 2 + [c_int] * 9 + [c_void_p]),

@@ -710,6 +710,7 @@ template <bool TREE> __global__ void __launch_bounds__(32 * MERGE_WARPS) paged_m
 struct Plan {
   int few_max, few_rows, few_tiles, few_splits, many_ctas;   // few_tiles: of the few-row kernel, 0 where the chunk kernel takes the step; many_ctas: the other way round
   long long few_count, floats;
+  bool pair;                                                 // form of the chunk kernel
 };
 constexpr long long MOST_WORK = 1ll << 27;                   // floats of partial results
 
@@ -718,7 +719,8 @@ static long long few_floats(int splits, long long count, int V) { return splits 
 // A window, or a number of first tokens, as long as all that a table holds.  (A position below zero less a longer window need not fit 32 bits.)
 static bool hides_nothing(int window, int first, int width, int page) { return std::max(window, first) >= (long long)width * page; }
 
-static Plan plan_of(int rows, int seqs, int width, int page, int heads, int kv_heads, int K, int V, int window, int first, int max_new, int max_length, int store, int act_dtype) {
+static Plan plan_of(bool tree, int rows, int seqs, int width, int page, int heads, int kv_heads, int K, int V, int window, int first, int max_new, int max_length, int store,
+                    int act_dtype) {
   Plan p{};
   if (hides_nothing(window, first, width, page)) window = first = 0;
   const int G = heads / kv_heads, sms = sm_count(), most = std::min(seqs, rows);
@@ -734,11 +736,16 @@ static Plan plan_of(int rows, int seqs, int width, int page, int heads, int kv_h
   long long singles = seqs;
   p.few_max = INT32_MAX;
   if (act_dtype == B2L_BF16 && longest > 16 && many_takes(K, V, store)) {
-    p.many_ctas = many_ctas((packed / 256 + most) * kv_heads, keys + (window > 0 ? 256 / G : 0), sms);
-    p.floats = many_floats(p.many_ctas, V);
+    // Trees of at most 128 packed rows: row tiles of 128, which both halves of a CTA compute
+    p.pair = tree && longest <= 128 && pair_takes(K, V, store);
+    p.many_ctas = many_ctas(p.pair, packed, most, kv_heads, keys + (window > 0 ? 256 / G : 0), sms);
+    p.floats = many_floats(p.pair, p.many_ctas, V);
     const long long more = longest / G - 1;                  // rows of the longest beside its first
     singles -= (std::max(rows - seqs, 0) + more - 1) / std::max(more, 1ll);
-    const bool both = G <= 16 && singles > 0 && singles * kv_heads * 0.5 * keys * (store == ACT ? 0.015e-3 : 0.119e-3) > 12;
+    // Trees: no more of them than there must be, as steps whose sequences all have drafts are what is common (32 trees of up to 32 tokens, e4m3, one of a single
+    // token: 27 us of 231 were the other kernel's)
+    const long long sure = tree ? std::max(0ll, 2ll * seqs - rows) : singles;
+    const bool both = G <= 16 && sure > 0 && sure * kv_heads * 0.5 * keys * (store == ACT ? 0.015e-3 : 0.119e-3) > 12;
     p.few_max = both ? (G <= 8 ? 8 : 16) : 0;
     if (!both) return p;
     p.few_rows = p.few_max;
@@ -799,7 +806,12 @@ using namespace b2l;
 extern "C" long long b2l_seq_paged_attention_work(int rows, int seqs, int width, int page, int heads, int kv_heads, int K, int V, int window, int first, int max_new,
                                                   int max_length, int store, int act_dtype) {
   if (rows <= 0 || seqs <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0) return 0;
-  return paged::plan_of(rows, seqs, width, page, heads, kv_heads, K, V, window, first, max_new, max_length, store, act_dtype).floats;
+  return paged::plan_of(false, rows, seqs, width, page, heads, kv_heads, K, V, window, first, max_new, max_length, store, act_dtype).floats;
+}
+extern "C" long long b2l_seq_paged_attention_tree_work(int rows, int seqs, int width, int page, int heads, int kv_heads, int K, int V, int window, int first, int max_new,
+                                                       int max_length, int store, int act_dtype) {
+  if (rows <= 0 || seqs <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0) return 0;
+  return paged::plan_of(true, rows, seqs, width, page, heads, kv_heads, K, V, window, first, max_new, max_length, store, act_dtype).floats;
 }
 
 template <bool TREE> static int attention(const char* who, bool zeros, const paged::Tree& nodes, const void* q, long long ldq, long long hsq, const void* k, const void* v, const float* k_scale, const float* v_scale,
@@ -818,7 +830,7 @@ template <bool TREE> static int attention(const char* who, bool zeros, const pag
                       "%s: sizes beyond the grid's or a copy's coordinates", who);
   if (rows == 0 || seqs == 0) return 0;
   if (paged::hides_nothing(window, first, width, page)) window = first = 0;
-  const Plan p = plan_of(rows, seqs, width, page, heads, kv_heads, K, V, window, first, max_new, max_length, store, act_dtype);
+  const Plan p = plan_of(TREE, rows, seqs, width, page, heads, kv_heads, K, V, window, first, max_new, max_length, store, act_dtype);
   B2L_CHECK_ARG(p.floats == 0 || (work && work_floats >= p.floats), "%s: a work space of %lld floats is needed", who, p.floats);
   Attn<TREE> a{};
   a.s = step_of(starts, lengths, table, ldt, width, rows, seqs, pages, page);
@@ -834,10 +846,10 @@ template <bool TREE> static int attention(const char* who, bool zeros, const pag
   a.nodes = nodes;
   a.both = p.few_tiles > 0 && p.many_ctas > 0;
   if (p.many_ctas) {
-    const int rc = many_launch(a, p.many_ctas, work, st);
+    const int rc = many_launch(a, p.pair, p.many_ctas, work, st);
     if (rc || !a.both) return rc;
     a.zeros = 0;                                             // they are there
-    work += many_floats(p.many_ctas, V);
+    work += many_floats(p.pair, p.many_ctas, V);
   }
   a.few.splits = p.few_splits;
   a.few.count = p.few_count;

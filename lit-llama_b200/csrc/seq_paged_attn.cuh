@@ -328,11 +328,13 @@ __device__ __forceinline__ bool finite4(const float (&x)[4], float inv) {
   return fabsf(x[0] * inv) < INFINITY && fabsf(x[1] * inv) < INFINITY && fabsf(x[2] * inv) < INFINITY && fabsf(x[3] * inv) < INFINITY;
 }
 
-// the tensor-core kernel of longer chunks (seq_paged_tc.cu): heads that it takes, the CTAs for at most so many row tiles and keys, its work space, its launch
+// the tensor-core kernel of longer chunks (seq_paged_tc.cu): heads that it takes; the CTAs for at most so many packed rows of `tiles` sequences, and keys; its work space;
+// its launch.  pair: row tiles of 128 rows that both halves of a CTA compute
 bool many_takes(int K, int V, int store);
-int many_ctas(long long row_tiles, long long keys, int sms);
-long long many_floats(int ctas, int V);
-template <bool TREE> int many_launch(Attn<TREE>& a, int ctas, float* work, cudaStream_t stream);
+bool pair_takes(int K, int V, int store);
+int many_ctas(bool pair, long long packed, long long tiles, int kv_heads, long long keys, int sms);
+long long many_floats(bool pair, int ctas, int V);
+template <bool TREE> int many_launch(const Attn<TREE>& a, bool pair, int ctas, float* work, cudaStream_t stream);
 
 }  // namespace paged
 }  // namespace b2l

@@ -47,44 +47,57 @@ using atc::desc_mn;
 using atc::fma2;
 using atc::mma_ss;
 
-constexpr int KEYS = 128, TILE = 128, ROWS = 2 * TILE, MOST_K = 192, MOST_V = 128;
+constexpr int KEYS = 128, TILE = 128, MOST_K = 192, MOST_V = 128;
 constexpr int TC_ATOM = 128 * 128;                           // bytes of 64 columns of 128 rows
 constexpr int INFOS = 4;
 
-struct alignas(16) Info {                                    // of a tile of keys
-  uint2 k_by[KEYS], v_by[KEYS];                              // 8-bit pools: what a key's and a value's codes are multiplied with
+// TREE: trees of drafted tokens.  PAIR: a row tile has one half only, 128 rows, and both halves' warps compute it: they take its tiles of keys in turn, each with a
+// maximum, a sum and outputs of its own, which are joined at the end.  So one's products and softmax fill the time of the other's as they do in a whole row tile, and the room
+// of the second half's queries is free for more stages.  For steps of few rows, whose time is that of the keys on their way.
+template <bool TREE_, bool PAIR_> struct Tiles : Attn<TREE_> {
+  static constexpr bool TREE = TREE_, PAIR = PAIR_;
+  static constexpr int ROWS = PAIR ? TILE : 2 * TILE;
+};
+
+struct alignas(16) Info { uint2 k_by[KEYS], v_by[KEYS]; };   // 8-bit pools, of a tile of keys: what a key's and a value's codes are multiplied with
+struct alignas(16) Note {                                    // of a tile of keys
   uint32_t there;                                            // 16 keys each: whether their page is there; bits 8 and 9: whether a scale of a key, a value is below 2^-12 of the largest
   float k_up, v_up;                                          // 8-bit pools: powers of two that the scales were multiplied with
 };
-// A row tile: 256 packed rows of a head, the tiles of its sequence's rows one after the other, then the next head's, then the next sequence's
+// PAIR: twice as many as tiles that are prepared at a time, as the one half's next tile may be multiplied while the other still has to look at the one before
+template <bool PAIR> constexpr int NOTES = PAIR ? 2 * INFOS : INFOS;
+constexpr int MOST_NOTES = NOTES<true>, MOST_STAGES = 3;
+// A row tile: 256 (or 128) packed rows of a head, the tiles of its sequence's rows one after the other, then the next head's, then the next sequence's
 struct Walk {
   Place pl;
   int h;
   long long at;                                              // cost of all before it
 };
 struct Control {
-  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_half[2][2], o_done[2], info_full[INFOS], tail, gave_up;
-  uint64_t ref_full, rk_full, rk_empty, rv_full, rv_empty;   // 8-bit pools: the first tile's largest scales, codes of keys and values
+  uint64_t q_full, k_full[MOST_STAGES], k_empty[MOST_STAGES], v_full[MOST_STAGES], v_empty[MOST_STAGES], s_full[2], p_half[2][2], o_done[2], info_full[MOST_NOTES], tail, gave_up;
+  uint64_t ref_full, rk_full[2], rk_empty[2], rv_full[2], rv_empty[2];   // 8-bit pools: the first tile's largest scales, codes of keys and values
   uint32_t tmem, k_ref[3], v_ref[3];                         // largest scales of the first tile's keys and values, as bits, of a row tile, the next and the one before
   long long x0, x1;                                          // the CTA's part
   Walk at[20];                                               // each warp's row tile
 };
 struct Scales { float k[KEYS], v[KEYS]; };                   // 8-bit pools: what lies beside a tile's codes
 constexpr size_t CONTROL_BYTES = 1024;
-template <int STORE> constexpr size_t INFO_BYTES = STORE == ACT ? 1024 : (INFOS * sizeof(Info) + sizeof(Scales) + 1023) / 1024 * 1024;
-static_assert(sizeof(Control) <= CONTROL_BYTES && sizeof(Info) % 16 == 0);
+template <int STORE> constexpr size_t INFO_BYTES = STORE == ACT ? 1024 : (MOST_NOTES * sizeof(Note) + INFOS * sizeof(Info) + 1023) / 1024 * 1024;
+static_assert(sizeof(Control) <= CONTROL_BYTES && sizeof(Info) % 16 == 0 && sizeof(Scales) == 1024);
 template <int STORE> constexpr int THREADS = STORE == ACT ? 384 : 640;
 
-struct Layout { int ks, vs; size_t smem; };                  // stages of keys and values; none: the sizes do not fit
-template <int STORE> static Layout layout(int K, int V) {
-  const size_t base = CONTROL_BYTES + INFO_BYTES<STORE> + (STORE == ACT ? 0 : KEYS * (K + V)), ka = atoms_of(K, 2), va = atoms_of(V, 2), q = 2 * ka * TC_ATOM, room = 227 * 1024;
-  Layout l{0, 0, 0};
-  const std::pair<int, int> stages[3] = {{2, 2}, {2, 1}, {1, 1}};
-  for (const auto& [ks, vs] : stages)
-    if (base + q + (ks * ka + vs * va) * TC_ATOM <= room) {
-      l = {ks, vs, base + q + (ks * ka + vs * va) * TC_ATOM};
-      break;
-    }
+// Stages of keys and values, and of 8-bit pools' codes (with both's scales beside the keys'); none: the sizes do not fit.  What comes first is what measured best
+struct Layout { int ks, vs, raw_ks, raw_vs; size_t smem; };
+template <int STORE, bool PAIR> static Layout layout(int K, int V) {
+  const size_t ka = atoms_of(K, 2), va = atoms_of(V, 2), q = (PAIR ? 1 : 2) * ka * TC_ATOM + (PAIR ? 2048 : 0), room = 227 * 1024;
+  constexpr int N = 5;
+  const Layout whole[N] = {{2, 2, 1, 1}, {2, 1, 1, 1}, {1, 1, 1, 1}}, pair8[N] = {{2, 2, 2, 2}, {2, 1, 2, 2}, {1, 1, 2, 2}, {2, 1, 1, 1}, {1, 1, 1, 1}}, pair16[N] = {{3, 3, 1, 1}, {3, 2, 1, 1}, {2, 2, 1, 1}, {2, 1, 1, 1}, {1, 1, 1, 1}};
+  Layout l{};
+  for (int i = 0; i < N && !l.ks; ++i) {
+    Layout s = !PAIR ? whole[i] : STORE == ACT ? pair16[i] : pair8[i];
+    s.smem = CONTROL_BYTES + INFO_BYTES<STORE> + q + (s.ks * ka + s.vs * va) * TC_ATOM + (STORE == ACT ? 0 : KEYS * (s.raw_ks * K + s.raw_vs * V) + s.raw_ks * sizeof(Scales));
+    if (s.ks && s.smem <= room) l = s;
+  }
   if (l.ks && l.smem < 120 * 1024) l.smem = 120 * 1024;      // one CTA per SM: each takes all of tensor memory
   return l;
 }
@@ -206,7 +219,9 @@ __device__ __forceinline__ uint32_t piece_at(int r, int c) { return (uint32_t)((
 
 // This thread's 16-byte pieces of a tile's codes (rows of D bytes) as f16 into its rows, code times its row's factor (in two parts) rounded once: every `threads`-th
 // piece.  HIDE: a factor of 0 hides whatever the codes are
-template <int STORE, bool HIDE> __device__ __forceinline__ void codes_to_f16(uint32_t raw, int D, const uint2* factors, uint32_t base, int me, int threads) {
+// UNROLL: 2; PAIR 1, with one place in the code for keys and values (37 trees of 32 tokens over 4096 keys, e4m3: 153 us so, 173 with 2 and two places, 167 with 4 pieces'
+// loads ahead)
+template <int STORE, bool HIDE, int UNROLL> __device__ __forceinline__ void codes_to_f16(uint32_t raw, int D, const uint2* factors, uint32_t base, int me, int threads) {
   const int pieces = D / 16;
   auto one = [&](uint32_t from, uint2 f, uint32_t first, uint32_t second, bool odd) {
     uint4 w = ld128(from);
@@ -226,7 +241,7 @@ template <int STORE, bool HIDE> __device__ __forceinline__ void codes_to_f16(uin
     const int c = me & (pieces - 1), key = me / pieces, step = threads / pieces;
     const bool odd = (c >> 2) & 1;
     uint32_t from = raw + 16 * me, first = base + piece_at(key, 2 * c + odd), second = base + piece_at(key, 2 * c + 1 - odd);
-#pragma unroll 2
+#pragma unroll UNROLL
     for (int k = key; k < KEYS; k += step, from += 16 * threads, first += 128 * step, second += 128 * step) one(from, factors[k], first, second, odd);
   } else {
     const int by = 65536 / pieces + 1;                       // x / pieces = x by >> 16 for x < 128 pieces, pieces <= 12
@@ -256,17 +271,17 @@ struct Cost {
     return y < LEAST ? 0 : units - y < LEAST ? units : y;
   }
 };
-template <bool TREE> __device__ __forceinline__ Cost cost_of(const Attn<TREE>& a, const Place& pl) {
+template <class A> __device__ __forceinline__ Cost cost_of(const A& a, const Place& pl) {
   Cost c;
-  c.all = a.keys(pl, ROWS).units(7);
+  c.all = a.keys(pl, A::ROWS).units(7);
   c.units = max(c.all, 1);
-  c.each = pl.n * (a.heads / a.kv_heads) - pl.first > TILE ? 4 : 3;
+  c.each = !A::PAIR && pl.n * (a.heads / a.kv_heads) - pl.first > TILE ? 4 : A::PAIR ? 2 : 3;
   return c;
 }
 // of one head of a sequence, by a whole warp
-template <bool TREE> __device__ __forceinline__ long long sequence_cost(const Attn<TREE>& a, Place pl, int lane) {
+template <class A> __device__ __forceinline__ long long sequence_cost(const A& a, Place pl, int lane) {
   long long sum = 0;
-  for (pl.first = lane * ROWS; pl.first < pl.n * (a.heads / a.kv_heads); pl.first += 32 * ROWS) sum += cost_of(a, pl).total();
+  for (pl.first = lane * A::ROWS; pl.first < pl.n * (a.heads / a.kv_heads); pl.first += 32 * A::ROWS) sum += cost_of(a, pl).total();
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   return sum;
@@ -283,10 +298,10 @@ template <bool TREE, typename F> __device__ __forceinline__ void each_sequence(c
   }
 }
 // the row tile after this one; pl.n is 0 behind the last
-template <bool TREE> __device__ __forceinline__ void advance(const Attn<TREE>& a, Walk& w, const Cost& c, int lane) {
+template <class A> __device__ __forceinline__ void advance(const A& a, Walk& w, const Cost& c, int lane) {
   w.at += c.total();
-  if (w.pl.n * (a.heads / a.kv_heads) - w.pl.first > ROWS) {
-    w.pl.first += ROWS;
+  if (w.pl.n * (a.heads / a.kv_heads) - w.pl.first > A::ROWS) {
+    w.pl.first += A::ROWS;
     return;
   }
   w.pl.first = 0;
@@ -304,7 +319,7 @@ struct Item {
   int h, t0, t1, n;                                          // n: tiles of keys that its rows see
   bool whole;
 };
-template <bool TREE> __device__ __forceinline__ bool next(const Attn<TREE>& a, Control& ct, int warp, int lane, Item& x) {
+template <class A> __device__ __forceinline__ bool next(const A& a, Control& ct, int warp, int lane, Item& x) {
   Walk w = ct.at[warp];
   const long long x0 = ct.x0, x1 = ct.x1;
   bool found = false;
@@ -327,17 +342,22 @@ template <bool TREE> __device__ __forceinline__ bool next(const Attn<TREE>& a, C
   return found;
 }
 
-__device__ __forceinline__ int pl_groups(const Place& pl, int G) { return pl.n * G - pl.first > TILE ? 2 : 1; }
+// Warps 4 .. 11 among themselves
+__device__ __forceinline__ void both_halves() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-template <int STORE, bool TREE>
-__global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __grid_constant__ Attn<TREE> a, const __grid_constant__ CUtensorMap map_k,
-                                                                                  const __grid_constant__ CUtensorMap map_v, int k_stages, int v_stages) {
-  constexpr bool HALF = STORE != ACT;
+template <class A> __device__ __forceinline__ int pl_groups(const Place& pl, int G) { return !A::PAIR && pl.n * G - pl.first > TILE ? 2 : 1; }
+
+template <int STORE, class A>
+__global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __grid_constant__ A a, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                                       int k_stages, int v_stages, int k_codes, int v_codes) {
+  constexpr bool HALF = STORE != ACT, TREE = A::TREE, PAIR = A::PAIR;
+  constexpr int ROWS = A::ROWS, NOTES = paged::NOTES<PAIR>;
+  const int raw_ks = PAIR ? k_codes : 1, raw_vs = PAIR ? v_codes : 1;
   constexpr float LIFT = HALF ? 6.f : 0.f;                   // weights up to 2^14 in f16
   extern __shared__ __align__(1024) uint8_t smem[];
   Control& ct = *reinterpret_cast<Control*>(smem);
-  Info* infos = reinterpret_cast<Info*>(smem + CONTROL_BYTES);      // ACT: only `there`, at uint32_t steps
-  uint32_t* there_of = reinterpret_cast<uint32_t*>(smem + CONTROL_BYTES);
+  Note* notes_of = reinterpret_cast<Note*>(smem + CONTROL_BYTES);
+  Info* infos = reinterpret_cast<Info*>(smem + CONTROL_BYTES + MOST_NOTES * sizeof(Note));      // 8-bit pools
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.heads / a.kv_heads;
   // this CTA's part, x0 .. x1
   {
@@ -402,31 +422,35 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
       });
   }
   const int ka = atoms_of(a.K, 2), va = atoms_of(a.V, 2);
-  const uint32_t sq = smem_u32(smem) + CONTROL_BYTES + INFO_BYTES<STORE>, sk = sq + 2 * ka * TC_ATOM, sv = sk + k_stages * ka * TC_ATOM;
-  const uint32_t raw_k = sv + v_stages * va * TC_ATOM, raw_v = raw_k + KEYS * a.K;      // 8-bit pools
-  Scales& scales = *reinterpret_cast<Scales*>(smem + CONTROL_BYTES + INFOS * sizeof(Info));
+  const uint32_t sq = smem_u32(smem) + CONTROL_BYTES + INFO_BYTES<STORE>, sk = sq + (PAIR ? 1 : 2) * ka * TC_ATOM, sv = sk + k_stages * ka * TC_ATOM;
+  const uint32_t raw_k = sv + v_stages * va * TC_ATOM, raw_v = raw_k + raw_ks * KEYS * a.K, raw_s = raw_v + raw_vs * KEYS * a.V;      // 8-bit pools: codes, scales
+  const Scales* scales_of = reinterpret_cast<const Scales*>(smem + (raw_s - smem_u32(smem)));
+  const uint32_t telling = HALF ? raw_s + raw_ks * (uint32_t)sizeof(Scales) : sv + v_stages * va * TC_ATOM;      // PAIR: what the halves tell one another, 2 KB
   auto bar = [&](const uint64_t& b) { return smem_u32(&b); };
   uint32_t dead = (sq & 1023u) ? 1u : 0u;
   if (tid == 0) {
     mbar_init(bar(ct.q_full), 256);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(bar(ct.k_full[i]), HALF ? 128 : 1);
-      mbar_init(bar(ct.v_full[i]), HALF ? 128 : 1);
-      mbar_init(bar(ct.k_empty[i]), 1);
-      mbar_init(bar(ct.v_empty[i]), 1);
       mbar_init(bar(ct.s_full[i]), 1);
       mbar_init(bar(ct.p_half[i][0]), 4);
       mbar_init(bar(ct.p_half[i][1]), 4);
       mbar_init(bar(ct.o_done[i]), 1);
     }
     mbar_init(bar(ct.gave_up), 1);
-    for (int i = 0; i < INFOS; ++i) mbar_init(bar(ct.info_full[i]), HALF ? 129 : 1);
+    for (int i = 0; i < NOTES; ++i) mbar_init(bar(ct.info_full[i]), HALF ? 129 : 1);
     mbar_init(bar(ct.tail), 1);
     mbar_init(bar(ct.ref_full), 128);
-    mbar_init(bar(ct.rk_full), 1);
-    mbar_init(bar(ct.rv_full), 1);
-    mbar_init(bar(ct.rk_empty), 128);
-    mbar_init(bar(ct.rv_empty), 128);
+    for (int i = 0; i < MOST_STAGES; ++i) {
+      mbar_init(bar(ct.k_full[i]), HALF ? 128 : 1);
+      mbar_init(bar(ct.v_full[i]), HALF ? 128 : 1);
+      mbar_init(bar(ct.k_empty[i]), 1);
+      mbar_init(bar(ct.v_empty[i]), 1);
+      if (i >= 2) break;
+      mbar_init(bar(ct.rk_full[i]), 1);
+      mbar_init(bar(ct.rv_full[i]), 1);
+      mbar_init(bar(ct.rk_empty[i]), 128);
+      mbar_init(bar(ct.rv_empty[i]), 128);
+    }
     for (int i = 0; i < 3; ++i) ct.k_ref[i] = ct.v_ref[i] = 0u;
     mbar_init_fence();
   }
@@ -451,13 +475,13 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
     auto scores = [&](int g) {
 #pragma unroll 1
       for (int x = 0; 4 * x < steps; ++x) {
-        const uint64_t qd = desc_sw128(sq + (g * ka + x) * TC_ATOM), kd = desc_sw128(sk + (kst * ka + x) * TC_ATOM);
+        const uint64_t qd = desc_sw128(sq + ((PAIR ? 0 : g) * ka + x) * TC_ATOM), kd = desc_sw128(sk + (kst * ka + x) * TC_ATOM);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           if (4 * x + k < steps) mma_ss(tmem + 128 * g, qd + 2 * k, kd + 2 * k, id_s, x + k > 0 ? 1u : 0u, lead);
       }
       commit_by(lead, bar(ct.s_full[g]));
-      if (g == groups - 1) {
+      if (PAIR || g == groups - 1) {
         commit_by(lead, bar(ct.k_empty[kst]));
         if (++kst == k_stages) { kst = 0; kph ^= 1u; }
       }
@@ -465,8 +489,43 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
     while (!dead && next(a, ct, warp, lane, x)) {
      const int n = x.n;
      if (n == 0) continue;                                   // rows that see nothing
-     groups = pl_groups(x.pl, G);
+     groups = pl_groups<A>(x.pl, G);
      wait_lead(bar(ct.q_full), item++ & 1u, lead, dead);
+     if constexpr (PAIR) {
+       for (int g = 0; g < min(n, 2) && !dead; ++g) {
+         wait_lead(bar(ct.k_full[kst]), kph, lead, dead);
+         fence_after();
+         if (!dead) scores(g);
+       }
+#pragma unroll 1
+       for (int t = 0; t < n && !dead; ++t) {
+         const int g = t & 1;
+         wait_lead(bar(ct.v_full[vst]), vph, lead, dead);
+#pragma unroll
+         for (int half = 1; half >= 0; --half) {
+           wait_lead(bar(ct.p_half[g][half]), (done[g] + (t >> 1)) & 1u, lead, dead);
+           if (dead) break;
+           fence_after();
+           const uint64_t vd = desc_mn(sv + vst * va * TC_ATOM + half * (TC_ATOM / 2), TC_ATOM);
+#pragma unroll
+           for (int k = 0; k < 4; ++k) mma_ts(tmem + 256 + 128 * g, tmem + 128 * g + 64 * half + 8 * k, vd + k * (16 * 128 / 16), id_o, t < 2 && half == 1 && k == 0 ? 0u : 1u, lead);
+         }
+         if (dead) break;
+         commit_by(lead, bar(ct.v_empty[vst]));
+         if (t + 2 < n) {
+           wait_lead(bar(ct.k_full[kst]), kph, lead, dead);
+           if (dead) break;
+           fence_after();
+           scores(g);
+         } else {
+           commit_by(lead, bar(ct.o_done[g]));
+         }
+         if (++vst == v_stages) { vst = 0; vph ^= 1u; }
+       }
+       done[0] += (n + 1) >> 1;
+       done[1] += n >> 1;
+       continue;
+     }
      wait_lead(bar(ct.k_full[kst]), kph, lead, dead);
      fence_after();
      for (int g = 0; g < groups && !dead; ++g) scores(g);
@@ -505,11 +564,14 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
       wait_for(bar(ct.gave_up), 0, late);
     }
     __syncwarp();
-   } else if (warp == 1) {
+   } else if (warp == 1 || (TREE && warp == 3)) {
     // ===================== tiled copies =====================
+    // TREE: keys by warp 1, values by warp 3.  One warp for both asks for the keys of a tile when the place of values before it is free, which is late where nearly all of
+    // the time is that of copies: 37 trees of 32 tokens, bf16, took 125 us so
+    const bool keys_here = warp == 1, values_here = !TREE || warp == 3;
     const int box = min(1 << a.s.shift, KEYS), boxes = KEYS / box, gone = (a.s.pages * a.kv_heads) << a.s.shift;      // a row beyond the pool: zeros
     int kst = 0, vst = 0;
-    uint32_t kph = 1, vph = 1, tail_waits = 0, tile = 0;     // a stage is free at first
+    uint32_t kph = 1, vph = 1, tail_waits = 0, tile = 0;     // a stage is free at first; 8-bit pools: stages of codes
     while (!dead && next(a, ct, warp, lane, x)) {
      const Keys keys = a.keys(x.pl, ROWS);
      const int h = x.h, sequence = x.pl.b;
@@ -521,39 +583,41 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
       const int row = page >= 0 ? ((page * a.kv_heads + h) << a.s.shift) + ((key0 + lane * box) & ((1 << a.s.shift) - 1)) : gone;
       uint32_t there = 0;                                    // by 16 keys
       for (int i = 0; i < 8; ++i) there |= (seen >> (i * 16 / box) & 1u) << i;
-      const uint32_t k_to = bar(HALF ? ct.rk_full : ct.k_full[kst]);
-      wait_warp(bar(HALF ? ct.rk_empty : ct.k_empty[kst]), kph, dead);
-      if (dead) break;
-      if (lane == 0) {
-        if (HALF) infos[tile % INFOS].there = there;
-        else there_of[tile % INFOS] = there;
-        mbar_arrive(bar(ct.info_full[tile % INFOS]));
-        mbar_expect_tx(k_to, HALF ? KEYS * (a.K + 8) : ka * TC_ATOM);
-      }
-      __syncwarp();                                          // the bytes are expected before they come
-      // a lane per box: one lane after the other took 100 ns for each, with pages of 16 tokens 3.1 us for a tile
-      const int b = lane & (boxes - 1), x = lane / boxes, r = __shfl_sync(0xffffffffu, row, b);      // 24 boxes at most
-      if (x < (HALF ? 3 : ka)) {
-        if (HALF) {
-          const int at = r < gone ? r : 0;                   // of a page that is not there: any scales, which nobody takes
-          if (x == 0) tma_load_2d(raw_k + b * box * a.K, &map_k, 0, r, k_to);
-          else bulk(smem_u32((x == 1 ? scales.k : scales.v) + b * box), (x == 1 ? a.ks : a.vs) + at, 4 * box, k_to);
-        } else {
-          tma_load_2d(sk + (kst * ka + x) * TC_ATOM + b * box * 128, &map_k, 64 * x, r, k_to);
+      const int b = lane & (boxes - 1), x = lane / boxes, r = __shfl_sync(0xffffffffu, row, b);      // a lane per box, 24 at most
+      if (keys_here) {
+        const uint32_t k_to = bar(HALF ? ct.rk_full[kst] : ct.k_full[kst]);
+        wait_warp(bar(HALF ? ct.rk_empty[kst] : ct.k_empty[kst]), kph, dead);
+        if (dead) break;
+        if (lane == 0) {
+          notes_of[tile % NOTES].there = there;
+          mbar_arrive(bar(ct.info_full[tile % NOTES]));
+          mbar_expect_tx(k_to, HALF ? KEYS * (a.K + 8) : ka * TC_ATOM);
         }
+        __syncwarp();                                        // the bytes are expected before they come
+        // one lane after the other took 100 ns for each box, with pages of 16 tokens 3.1 us for a tile
+        if (x < (HALF ? 3 : ka)) {
+          if (HALF) {
+            const int at = r < gone ? r : 0;                 // of a page that is not there: any scales, which nobody takes
+            if (x == 0) tma_load_2d(raw_k + kst * KEYS * a.K + b * box * a.K, &map_k, 0, r, k_to);
+            else bulk(smem_u32((x == 1 ? scales_of[kst].k : scales_of[kst].v) + b * box), (x == 1 ? a.ks : a.vs) + at, 4 * box, k_to);
+          } else {
+            tma_load_2d(sk + (kst * ka + x) * TC_ATOM + b * box * 128, &map_k, 64 * x, r, k_to);
+          }
+        }
+        __syncwarp();
+        if (++kst == (HALF ? raw_ks : k_stages)) { kst = 0; kph ^= 1u; }
       }
-      __syncwarp();
-      if (HALF || ++kst == k_stages) { kst = 0; kph ^= 1u; }
-      wait_warp(bar(HALF ? ct.rv_empty : ct.v_empty[vst]), vph, dead);
+      if (!values_here) continue;
+      wait_warp(bar(HALF ? ct.rv_empty[vst] : ct.v_empty[vst]), vph, dead);
       if (dead) break;
       const int valid = keys.end - key0;
       // bf16: behind the last key that is seen the page may hold anything, and a weight of zero does not hide an infinity: zeros there
       const bool cut = !HALF && valid < KEYS;
-      const uint32_t v_to = bar(HALF ? ct.rv_full : cut ? ct.tail : ct.v_full[vst]);
+      const uint32_t v_to = bar(HALF ? ct.rv_full[vst] : cut ? ct.tail : ct.v_full[vst]);
       if (lane == 0) mbar_expect_tx(v_to, HALF ? KEYS * a.V : va * TC_ATOM);
       __syncwarp();
       if (x < (HALF ? 1 : va)) {
-        if (HALF) tma_load_2d(raw_v + b * box * a.V, &map_v, 0, r, v_to);
+        if (HALF) tma_load_2d(raw_v + vst * KEYS * a.V + b * box * a.V, &map_v, 0, r, v_to);
         else tma_load_2d(sv + (vst * va + x) * TC_ATOM + b * box * 128, &map_v, 64 * x, r, v_to);
       }
       __syncwarp();
@@ -565,15 +629,15 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(ct.v_full[vst]));
       }
-      if (HALF || ++vst == v_stages) { vst = 0; vph ^= 1u; }
+      if (++vst == (HALF ? raw_vs : v_stages)) { vst = 0; vph ^= 1u; }
      }
     }
     // every copy has landed before the CTA ends: what reads them comes after, unless a wait ran out
     if (dead) {
       uint32_t late = 0;
-      for (int i = 0; i < (HALF ? 1 : k_stages); ++i) wait_for(bar(HALF ? ct.rk_full : ct.k_full[i]), i < kst ? kph ^ 1u : kph, late);
+      for (int i = 0; i < (HALF ? raw_ks : k_stages) && keys_here; ++i) wait_for(bar(HALF ? ct.rk_full[i] : ct.k_full[i]), i < kst ? kph ^ 1u : kph, late);
       late = 0;
-      for (int i = 0; i < (HALF ? 1 : v_stages); ++i) wait_for(bar(HALF ? ct.rv_full : ct.v_full[i]), i < vst ? vph ^ 1u : vph, late);
+      for (int i = 0; i < (HALF ? raw_vs : v_stages) && values_here; ++i) wait_for(bar(HALF ? ct.rv_full[i] : ct.v_full[i]), i < vst ? vph ^ 1u : vph, late);
     }
     __syncwarp();
    } else if (warp == 2) {
@@ -598,8 +662,8 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
       asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
       const bool keys_too = warp < 16;                       // warps 12 .. 15: the factors of keys and values, and the keys; 16 .. 19: the values
       const int me = tid & 127;
-      int st = 0, ref = 0;
-      uint32_t ph = 1, tile = 0, item = 0;
+      int st = 0, ref = 0, raw = 0;
+      uint32_t ph = 1, tile = 0, item = 0, raw_ph = 0;
       float k_up = 1.f, v_up = 1.f;
       // the factor in two f16, twice each: as precise as 22 bits, or steps of 2^-25 (2^-13 of a factor of 2^-12); NaN where the scale is out of range; 0 for a row of
       // zeros (2^-126) or one never written (0)
@@ -618,14 +682,15 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
        const Keys keys = a.keys(x.pl, ROWS);
        for (int t = x.t0; t < x.t1; ++t, ++tile) {
         Info& info = infos[tile % INFOS];
+        Note& note = notes_of[tile % NOTES];
         if (keys_too) {
-          wait_warp(bar(ct.rk_full), tile & 1u, dead);
+          wait_warp(bar(ct.rk_full[raw]), raw_ph, dead);
           if (dead) break;
-          const float ks = scales.k[me], vs = scales.v[me];
+          const float ks = scales_of[raw].k[me], vs = scales_of[raw].v[me];
           // A key that some row sees: behind the last one and before the windows there may be anything, and of a page that is not there the scales are those of
           // another place (`there` was written before the copies were asked for)
           const int j = keys.key0(t, 7) + me;
-          const bool valid = j < keys.end && (j >= keys.lo || j < keys.early) && (*reinterpret_cast<volatile uint32_t*>(&info.there) >> (me / 16) & 1u);
+          const bool valid = j < keys.end && (j >= keys.lo || j < keys.early) && (*reinterpret_cast<volatile uint32_t*>(&note.there) >> (me / 16) & 1u);
           if (t == x.t0) {
             if (valid && ks >= SMALLEST_SCALE && ks <= 1.f / SMALLEST_SCALE) atomicMax(&ct.k_ref[ref], __float_as_uint(ks));
             if (valid && vs >= SMALLEST_SCALE && vs <= 1.f / SMALLEST_SCALE) atomicMax(&ct.v_ref[ref], __float_as_uint(vs));
@@ -637,7 +702,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
             if (me == 0) ct.k_ref[ref == 0 ? 2 : ref - 1] = ct.v_ref[ref == 0 ? 2 : ref - 1] = 0u;      // the ones before, which all have read: for the ones after the next
             ref = ref == 2 ? 0 : ref + 1;
           }
-          uint2 k_by = valid ? factor(ks, k_up, 256u, &info.there) : make_uint2(0u, 0u), v_by = valid ? factor(vs, v_up, 512u, &info.there) : make_uint2(0u, 0u);
+          uint2 k_by = valid ? factor(ks, k_up, 256u, &note.there) : make_uint2(0u, 0u), v_by = valid ? factor(vs, v_up, 512u, &note.there) : make_uint2(0u, 0u);
           if (v_by.x == NO) {                                // a row that sees this key is computed again: its scores say so
             k_by = v_by;
             v_by = make_uint2(0u, 0u);
@@ -647,20 +712,26 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
           info.k_by[me] = k_by;
           info.v_by[me] = v_by;
           if (me == 0) {
-            info.k_up = k_up;
-            info.v_up = v_up;
+            note.k_up = k_up;
+            note.v_up = v_up;
           }
-          mbar_arrive(bar(ct.info_full[tile % INFOS]));
+          mbar_arrive(bar(ct.info_full[tile % NOTES]));
         } else {
-          wait_warp(bar(ct.rv_full), tile & 1u, dead);
+          wait_warp(bar(ct.rv_full[raw]), raw_ph, dead);
           wait_warp(bar(ct.v_empty[st]), ph, dead);
         }
-        wait_warp(bar(ct.info_full[tile % INFOS]), tile / INFOS & 1u, dead);      // all keys' factors
+        wait_warp(bar(ct.info_full[tile % NOTES]), tile / NOTES & 1u, dead);      // all keys' factors
         if (dead) break;
-        if (keys_too) codes_to_f16<STORE, false>(raw_k, a.K, info.k_by, sk + st * ka * TC_ATOM, me, 128);
-        else codes_to_f16<STORE, true>(raw_v, a.V, info.v_by, sv + st * va * TC_ATOM, me, 128);
+        if constexpr (PAIR) {
+          codes_to_f16<STORE, true, 1>(keys_too ? raw_k + raw * KEYS * a.K : raw_v + raw * KEYS * a.V, keys_too ? a.K : a.V, keys_too ? info.k_by : info.v_by,
+                                       keys_too ? sk + st * ka * TC_ATOM : sv + st * va * TC_ATOM, me, 128);
+        } else {
+          if (keys_too) codes_to_f16<STORE, false, 2>(raw_k + raw * KEYS * a.K, a.K, info.k_by, sk + st * ka * TC_ATOM, me, 128);
+          else codes_to_f16<STORE, true, 2>(raw_v + raw * KEYS * a.V, a.V, info.v_by, sv + st * va * TC_ATOM, me, 128);
+        }
         mbar_arrive(bar(keys_too ? ct.k_full[st] : ct.v_full[st]));
-        mbar_arrive(bar(keys_too ? ct.rk_empty : ct.rv_empty));
+        mbar_arrive(bar(keys_too ? ct.rk_empty[raw] : ct.rv_empty[raw]));
+        if (++raw == (keys_too ? raw_ks : raw_vs)) { raw = 0; raw_ph ^= 1u; }
         if (++st == (keys_too ? k_stages : v_stages)) { st = 0; ph ^= 1u; }
        }
       }
@@ -673,11 +744,13 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
     uint32_t tile = 0, mine = 0, item = 0, own_items = 0;    // tiles of keys, those of this half; row tiles with keys, those of this half
     while (next(a, ct, warp, lane, x)) {
     const Place pl = x.pl;
-    const int n = x.n, t0 = x.t0, rows = min(ROWS, pl.n * G - pl.first), groups = pl_groups(pl, G), at = pl.first + TILE * g + r;
-    const bool part = !x.whole, live = TILE * g + r < rows;
+    const int n = x.n, t0 = x.t0, rows = min(ROWS, pl.n * G - pl.first), groups = pl_groups<A>(pl, G);
+    const int in_tile = (PAIR ? 0 : TILE * g) + r, at = pl.first + in_tile;
+    const bool part = !x.whole, live = in_tile < rows;
     const int token = live ? at / G : 0, head = x.h * G + (live ? at % G : 0), row = pl.start + token, base = pl.length - pl.n, pos = live ? a.position(pl.start, base, pl.n, token) : -1;
     const Keys keys = a.keys(pl, ROWS);
     float cr = a.scale_log2;
+    const uint32_t told = telling + 4 * r;                   // PAIR: the second half's maxima, sums and notes; factors of the scores
     if (n > 0) {
      if (g < groups) {
       // The warp's 32 rows, neighbouring lanes along a row: with a row per lane the load unit was busy with 32 lines for every instruction, 5400 cycles.  A
@@ -711,6 +784,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
           }
           st128(own + piece_at(r, c), make_uint4(u[0], u[1], u[2], u[3]));
         }
+        if (PAIR) asm volatile("st.shared.f32 [%0+1536], %1;" ::"r"(told), "f"(cr) : "memory");
       }
       fence_proxy_async();
      }
@@ -722,23 +796,25 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
     uint32_t notes = 0;                                      // those of its tiles; bit 31: a score that is NaN or an infinity
     // positions of this group's rows: where all of them see a tile no mask is needed
     const int p_min = TREE ? keys.p_min : pl.length - pl.n + (pl.first + TILE * g) / G, p_max = TREE ? keys.p_max : pl.length - pl.n + (pl.first + min(TILE * (g + 1), rows) - 1) / G;
-    if (g < groups) {
+    int taken = 0;                                           // tiles of keys of this half
+    if (PAIR || g < groups) {
       const bool idle = !__any_sync(0xffffffffu, live);
-      for (int t = 0; t < n; ++t) {
+      for (int t = PAIR ? g : 0; t < n; t += PAIR ? 2 : 1, ++taken) {
         const int key0 = keys.key0(t0 + t, 7);
-        wait_for(bar(ct.info_full[(tile + t) % INFOS]), (tile + t) / INFOS & 1u, dead);
-        wait_warp(bar(ct.s_full[g]), (mine + t) & 1u, dead);
+        wait_for(bar(ct.info_full[(tile + t) % NOTES]), (tile + t) / NOTES & 1u, dead);
+        wait_warp(bar(ct.s_full[g]), (mine + taken) & 1u, dead);
         if (dead) break;
         if (idle) {                                          // no row: whatever the weights are
           if (lane < 2) mbar_arrive(bar(ct.p_half[g][lane]));
           continue;
         }
         fence_after();
-        const Info& info = infos[(tile + t) % INFOS];
-        const uint32_t there = HALF ? info.there : there_of[(tile + t) % INFOS];
-        if (HALF && t == 0) {
-          cr *= 1.f / info.k_up;
-          down = 1.f / info.v_up;
+        const Note& note = notes_of[(tile + t) % NOTES];
+        const uint32_t there = note.there;
+        if (HALF && taken == 0) {
+          if (PAIR && g > 0) asm volatile("ld.shared.f32 %0, [%1+1536];" : "=f"(cr) : "r"(told) : "memory");      // there since these scores are
+          cr *= 1.f / note.k_up;
+          down = 1.f / note.v_up;
         }
         if (HALF) notes |= there;
         const bool whole = (there & 0xffu) == 0xffu && key0 + KEYS - 1 <= p_min && (a.window == 0 || key0 > p_max - a.window || key0 + KEYS <= a.first);
@@ -777,7 +853,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
           const float f = grows ? exp2_f(m - top) : 1.f;     // 0 where nothing was added yet
           if (grows) m = top;
           l *= f;
-          if (t > 0) {                                       // these scores came after the product of tile t - 1
+          if (taken > 0) {                                   // these scores came after the product of this half's tile before
 #pragma unroll 1
             for (int c = 0; 16 * c < a.V; ++c) {
               uint32_t o[16];
@@ -828,12 +904,33 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
         }
         l += sum[0] + sum[1];
       }
-      if (n > 0) wait_warp(bar(ct.o_done[g]), own_items & 1u, dead);
+      const int tiles = PAIR ? (n + 1 - g) >> 1 : n;         // (taken, if no wait ran out)
+      if (tiles > 0) wait_warp(bar(ct.o_done[g]), own_items & 1u, dead);
       fence_after();
       if (dead || notes >> 31) l = NAN;
+      float f0 = 1.f, f1 = 0.f;                              // of the halves' outputs
+      if (PAIR && n > 0) {
+        if (g > 0) asm volatile("st.shared.f32 [%0], %1;\n\tst.shared.f32 [%0+512], %2;\n\tst.shared.b32 [%0+1024], %3;" ::"r"(told), "f"(m), "f"(l), "r"(notes) : "memory");
+        fence_before();
+        both_halves();
+        fence_after();
+        if (g == 0) {
+          float m1, l1;
+          uint32_t notes1;
+          asm volatile("ld.shared.f32 %0, [%3];\n\tld.shared.f32 %1, [%3+512];\n\tld.shared.b32 %2, [%3+1024];" : "=f"(m1), "=f"(l1), "=r"(notes1) : "r"(told) : "memory");
+          const float M = fmaxf(m, m1);
+          f0 = m == M ? 1.f : exp2_f(m - M);
+          f1 = n < 2 ? 0.f : m1 == M ? 1.f : exp2_f(m1 - M);
+          l = l * f0 + (n < 2 ? 0.f : l1 * f1);
+          m = M;
+          notes |= notes1;
+        }
+        both_halves();                                       // read before what comes next there
+      }
+      if (!PAIR || g == 0) {
       const float inv = part ? down : l == 0.f ? 0.f : down / l;
       float peak = 0.f;                                      // the row's largest output, NaN if one is
-      const int slot = 2 * (int)blockIdx.x + (t0 == 0 ? 1 : 0), place = !live ? -1 : part ? slot * ROWS + TILE * g + r : row * a.heads + head;      // of the row's outputs
+      const int slot = 2 * (int)blockIdx.x + (t0 == 0 ? 1 : 0), place = !live ? -1 : part ? slot * ROWS + in_tile : row * a.heads + head;      // of the row's outputs
       // Outputs through the warp's rows of the queries (every score of this row tile is done), 128 bytes of each row at a time; then eight lanes along a row (a
       // row per lane took 9500 cycles)
       const int per = part ? 32 : 64;                        // columns
@@ -844,6 +941,12 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
           uint32_t o[16];
           if (n > 0 && !dead) tmem_ld16(O + c, o);
           float x[16];
+          if (PAIR && n > 1 && !dead) {
+            uint32_t o1[16];
+            tmem_ld16(O + 128 + c, o1);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(fmaf(__uint_as_float(o1[i]), f1, __uint_as_float(o[i]) * f0));
+          }
 #pragma unroll
           for (int i = 0; i < 16; ++i) x[i] = dead ? NAN : n > 0 ? __uint_as_float(o[i]) * inv : 0.f;
 #pragma unroll
@@ -882,11 +985,12 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
         constexpr float LARGEST = STORE == E4M3 ? 448.f : 127.f;
         if (notes > 255u && l > 0.f && (((notes & 256u) && cr * (float)a.K * LARGEST > 1.f) || ((notes & 512u) && !(peak >= LARGEST * 1.220703125e-4f * down * (part ? l : 1.f))))) l = NAN;
       }
-      if (part) *reinterpret_cast<float2*>(a.many.ml + 2 * (slot * ROWS + TILE * g + r)) = make_float2(m, l);
+      if (part) *reinterpret_cast<float2*>(a.many.ml + 2 * (slot * ROWS + in_tile)) = make_float2(m, l);
       if (!part) {
         __syncwarp();
         const uint32_t bad = __ballot_sync(0xffffffffu, live && !(peak < INFINITY && fabsf(l) < INFINITY));
         if (bad) mend_rows<2>(a, pl.b, pl.start, pl.length - pl.n, x.h, pl.first + TILE * g + (warp & 3) * 32, bad, lane);
+      }
       }
     }
     if (n > 0) {
@@ -894,10 +998,9 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
       if (g > 0) wait_warp(bar(ct.o_done[0]), item & 1u, dead);
       ++item;
       tile += n;
-      if (g < groups) {
-        mine += n;
-        ++own_items;
-      }
+      const int tiles = PAIR ? (n + 1 - g) >> 1 : g < groups ? n : 0;
+      mine += tiles;
+      own_items += tiles > 0;
     }
     }
   }
@@ -906,9 +1009,12 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
   if (warp == 0) tmem_dealloc(tmem, 512);
 }
 
-// The row tiles that go on from CTA blockIdx.x to others; a warp has four rows, a lane four columns of each
-template <bool TREE> __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ Attn<TREE> a) {
-  const int lane = threadIdx.x & 31, G = a.heads / a.kv_heads, r0 = blockIdx.y * 32 + threadIdx.x / 32 * 4;
+// The row tiles that go on from CTA blockIdx.x to others; a warp has JOINED rows, a lane four columns of each.  Parts are read four at a time: one after the other ten of
+// a tile took 18.7 us for 16 tiles.
+constexpr int JOINED = 2, JOIN_AHEAD = 4;
+template <class A> __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ A a) {
+  constexpr int ROWS = A::ROWS;
+  const int lane = threadIdx.x & 31, G = a.heads / a.kv_heads, r0 = blockIdx.y * 8 * JOINED + threadIdx.x / 32 * JOINED;
   pdl_wait();                                                // launched as the last CTAs that compute parts end: they let nothing in earlier
   const int4 last = a.many.last[blockIdx.x];
   if (last.w < 2) return;
@@ -916,39 +1022,44 @@ template <bool TREE> __global__ void __launch_bounds__(256) paged_join_kernel(co
   sequence(a.s, last.x, start, n, length);
   const int rows = min(ROWS, n * G - last.y);
   if (r0 >= rows) return;
-  float M[4], L[4];
-  float4 x[4];
+  float M[JOINED], L[JOINED];
+  float4 x[JOINED];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < JOINED; ++k) {
     M[k] = -INFINITY;
     L[k] = 0.f;
     x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  for (int i = 0; i < last.w; ++i) {
-    const int at = (i == 0 ? 2 * (int)blockIdx.x + 1 : 2 * ((int)blockIdx.x + i)) * ROWS + r0;
-    float2 ml[4];
-    float4 z[4];
+  for (int i0 = 0; i0 < last.w; i0 += JOIN_AHEAD) {
+    float2 ml[JOIN_AHEAD][JOINED];
+    float4 z[JOIN_AHEAD][JOINED];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      ml[k] = make_float2(-INFINITY, 0.f);
-      z[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (r0 + k < rows) {
-        ml[k] = *reinterpret_cast<const float2*>(a.many.ml + 2 * (at + k));
-        if (4 * lane < a.V) z[k] = *reinterpret_cast<const float4*>(a.many.o + (size_t)(at + k) * a.V + 4 * lane);
+    for (int e = 0; e < JOIN_AHEAD; ++e) {
+      const int i = i0 + e, at = (i == 0 ? 2 * (int)blockIdx.x + 1 : 2 * ((int)blockIdx.x + i)) * ROWS + r0;
+#pragma unroll
+      for (int k = 0; k < JOINED; ++k) {
+        ml[e][k] = make_float2(-INFINITY, 0.f);
+        z[e][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < last.w && r0 + k < rows) {
+          ml[e][k] = *reinterpret_cast<const float2*>(a.many.ml + 2 * (at + k));
+          if (4 * lane < a.V) z[e][k] = *reinterpret_cast<const float4*>(a.many.o + (size_t)(at + k) * a.V + 4 * lane);
+        }
       }
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (ml[k].x == -INFINITY && ml[k].y == 0.f) continue;  // saw nothing
-      const float now = fmaxf(M[k], ml[k].x), f = M[k] == now ? 1.f : exp2_f(M[k] - now), w = ml[k].x == now ? 1.f : exp2_f(ml[k].x - now);
-      M[k] = now;
-      L[k] = L[k] * f + w * ml[k].y;
-      x[k] = make_float4(x[k].x * f + w * z[k].x, x[k].y * f + w * z[k].y, x[k].z * f + w * z[k].z, x[k].w * f + w * z[k].w);
-    }
+    for (int e = 0; e < JOIN_AHEAD; ++e)
+#pragma unroll
+      for (int k = 0; k < JOINED; ++k) {
+        if (ml[e][k].x == -INFINITY && ml[e][k].y == 0.f) continue;      // saw nothing
+        const float now = fmaxf(M[k], ml[e][k].x), f = M[k] == now ? 1.f : exp2_f(M[k] - now), w = ml[e][k].x == now ? 1.f : exp2_f(ml[e][k].x - now);
+        M[k] = now;
+        L[k] = L[k] * f + w * ml[e][k].y;
+        x[k] = make_float4(x[k].x * f + w * z[e][k].x, x[k].y * f + w * z[e][k].y, x[k].z * f + w * z[e][k].z, x[k].w * f + w * z[e][k].w);
+      }
   }
   uint32_t bad = 0u;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < JOINED; ++k) {
     if (r0 + k >= rows) break;
     const int at = last.y + r0 + k, row = start + at / G, head = last.z * G + at % G;
     const float inv = L[k] == 0.f ? 0.f : 1.f / L[k], y[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
@@ -959,16 +1070,17 @@ template <bool TREE> __global__ void __launch_bounds__(256) paged_join_kernel(co
   if (bad) mend_rows<2>(a, last.x, start, length - n, last.z, last.y + r0, bad, lane);
 }
 
-int many_ctas(long long row_tiles, long long keys, int sms) {
-  const long long cost = row_tiles * (EXTRA + 4 * ((keys + KEYS - 1) / KEYS + 2));
+int many_ctas(bool pair, long long packed, long long tiles, int kv_heads, long long keys, int sms) {
+  const long long row_tiles = (packed / (pair ? TILE : 2 * TILE) + tiles) * kv_heads, cost = row_tiles * (EXTRA + (pair ? 2 : 4) * ((keys + KEYS - 1) / KEYS + 2));
   return (int)std::max<long long>(1, std::min<long long>(sms, cost / SMALLEST_SHARE));
 }
-long long many_floats(int ctas, int V) { return 4ll * ctas + 2ll * ctas * ROWS * (2 + V); }
+long long many_floats(bool pair, int ctas, int V) { return 4ll * ctas + 2ll * ctas * (pair ? TILE : 2 * TILE) * (2 + V); }
 
 bool many_takes(int K, int V, int store) {
   if (K > MOST_K || V > MOST_V) return false;
-  return (store == ACT ? layout<ACT>(K, V) : layout<INT8>(K, V)).ks > 0;
+  return (store == ACT ? layout<ACT, false>(K, V) : layout<INT8, false>(K, V)).ks > 0;
 }
+bool pair_takes(int K, int V, int store) { return (store == ACT ? layout<ACT, true>(K, V) : layout<INT8, true>(K, V)).ks > 0; }
 
 // Rows of `cols` bytes (a multiple of 16, up to 256), whole ones, as they lie
 static int map_rows(CUtensorMap* m, const void* base, long long rows, int cols, int box_rows) {
@@ -988,8 +1100,8 @@ static int map_rows(CUtensorMap* m, const void* base, long long rows, int cols, 
   return 0;
 }
 
-template <int STORE, bool TREE> static int go(const Attn<TREE>& a, int ctas, cudaStream_t stream) {
-  const Layout l = layout<STORE>(a.K, a.V);
+template <int STORE, class A> static int go(const A& a, int ctas, cudaStream_t stream) {
+  const Layout l = layout<STORE, A::PAIR>(a.K, a.V);
   CUtensorMap mk, mv;
   const long long rows = ((long long)a.s.pages * a.kv_heads) << a.s.shift;
   const int box = 1 << a.s.shift < KEYS ? 1 << a.s.shift : KEYS;
@@ -1001,24 +1113,34 @@ template <int STORE, bool TREE> static int go(const Attn<TREE>& a, int ctas, cud
     if (int rc = map_rows(&mv, a.v, rows, a.V, box)) return rc;
   }
   static DynSmemCache cache;
-  if (int rc = ensure_dyn_smem(paged_many_kernel<STORE, TREE>, l.smem, cache)) return rc;
-  paged_many_kernel<STORE, TREE><<<(unsigned)ctas, THREADS<STORE>, l.smem, stream>>>(a, mk, mv, l.ks, l.vs);
+  if (int rc = ensure_dyn_smem(paged_many_kernel<STORE, A>, l.smem, cache)) return rc;
+  paged_many_kernel<STORE, A><<<(unsigned)ctas, THREADS<STORE>, l.smem, stream>>>(a, mk, mv, l.ks, l.vs, l.raw_ks, l.raw_vs);
   B2L_LAUNCH_CHECK("paged_many_kernel");
   return 0;
 }
-template <bool TREE> int many_launch(Attn<TREE>& a, int ctas, float* work, cudaStream_t stream) {
+template <class A> static int launch(A& a, int ctas, float* work, cudaStream_t stream) {
   a.many.last = reinterpret_cast<int4*>(work);
   a.many.ml = work + 4 * ctas;
-  a.many.o = a.many.ml + 4ll * ctas * ROWS;
+  a.many.o = a.many.ml + 4ll * ctas * A::ROWS;
   const int rc = a.store_kind == ACT ? go<ACT>(a, ctas, stream) : a.store_kind == E4M3 ? go<E4M3>(a, ctas, stream) : go<INT8>(a, ctas, stream);
   if (rc || ctas == 1) return rc;
-  LaunchCfg launch(dim3((unsigned)ctas, ROWS / 32), dim3(256), 0, stream, true);
-  B2L_CUDA(cudaLaunchKernelEx(&launch.cfg, paged_join_kernel<TREE>, a));
+  LaunchCfg cfg(dim3((unsigned)ctas, A::ROWS / (8 * JOINED)), dim3(256), 0, stream, true);
+  B2L_CUDA(cudaLaunchKernelEx(&cfg.cfg, paged_join_kernel<A>, a));
   B2L_LAUNCH_CHECK("paged_join_kernel");
   return 0;
 }
-template int many_launch<false>(Attn<false>&, int, float*, cudaStream_t);
-template int many_launch<true>(Attn<true>&, int, float*, cudaStream_t);
+template <bool TREE> int many_launch(const Attn<TREE>& a, bool pair, int ctas, float* work, cudaStream_t stream) {
+  if constexpr (TREE) {
+    if (pair) {
+      Tiles<true, true> x{a};
+      return launch(x, ctas, work, stream);
+    }
+  }
+  Tiles<TREE, false> x{a};
+  return launch(x, ctas, work, stream);
+}
+template int many_launch<false>(const Attn<false>&, bool, int, float*, cudaStream_t);
+template int many_launch<true>(const Attn<true>&, bool, int, float*, cudaStream_t);
 
 }  // namespace paged
 }  // namespace b2l

@@ -40,6 +40,7 @@ from .state import PagesFull
 
 STORES = {"act": S.STORE_ACT, "fp8": S.STORE_E4M3, "int8": S.STORE_INT8}
 PAGES = (16, 32, 64, 128, 256)
+ACTS = (torch.bfloat16, torch.float32)
 
 
 class PagedStep:
@@ -315,6 +316,16 @@ def _whole(what: str, x: torch.Tensor, dtype: torch.dtype, device: torch.device,
     return x
 
 
+def _matrix(x: torch.Tensor, columns: int) -> Tuple[torch.Tensor, int]:
+    """x [rows, columns] with its rows' entries consecutive (else a copy), and the entries between its rows."""
+    s0, s1 = x.stride()
+    if x.shape[0] <= 1:
+        s0 = columns
+    if (s1 != 1 and columns > 1) or s0 < columns:
+        return x.contiguous(), columns
+    return x, s0
+
+
 class PagedTree:
     """The new tokens of a step as trees: parents[r] (int32 [rows], on the device) is the place, among its sequence's new tokens, of the token that row r follows,
     one before it, or -1 where it follows the sequence as it was.  A token is at the position of its parent and one more (`positions`, int32 [rows], for the rotation of
@@ -335,6 +346,7 @@ class PagedTree:
         self.window, self.first = min(int(window), 2 ** 30), min(int(first), 2 ** 30)
         make = step.starts.new_empty if step.seqs else step.starts.new_zeros
         self.masks, self.depths, self.positions = make((step.rows, self.words)), make((step.rows,)), make((step.rows,))
+        self._works: Dict[int, int] = {}                                    # bytes of work space of `accept`, by the vocabulary
         self.update()
 
     def update(self) -> None:
@@ -352,36 +364,32 @@ class PagedTree:
 
         Returns int32 tensors: kept [rows], the places of the path's tokens among the sequence's new ones, -1 behind them; counts [sequences], how many; following
         [sequences], the last one's target (-1 for a sequence without new tokens)."""
-        s = self.step
-        if logits.dim() != 2 or logits.shape[0] < s.rows or logits.shape[1] < 1 or logits.device != self.device or logits.dtype not in (torch.bfloat16, torch.float32):
-            raise ValueError(f"paged tree: logits {tuple(logits.shape)} {logits.dtype} on {logits.device}, [{s.rows}, vocab] in bf16 or f32 on {self.device} are wanted")
-        if tokens.dtype not in (torch.int32, torch.int64):
-            raise ValueError(f"paged tree: tokens in {tokens.dtype}: int32 or int64")
-        tokens = _whole("paged tree: tokens", tokens, tokens.dtype, self.device, s.rows)
+        s, rows, shape = self.step, self.step.rows, logits.shape
+        if len(shape) != 2 or shape[0] < rows or shape[1] < 1 or logits.device != self.device or logits.dtype not in ACTS:
+            raise ValueError(f"paged tree: logits {tuple(shape)} {logits.dtype} on {logits.device}, [{rows}, vocab] in bf16 or f32 on {self.device} are wanted")
+        wide = tokens.dtype == torch.int64
+        tokens = _whole("paged tree: tokens", tokens, torch.int64 if wide else torch.int32, self.device, rows)
         if not 0.0 <= temperature < float("inf"):
             raise ValueError(f"paged tree: a temperature of {temperature}")
-        vocab = logits.shape[1]
-        if vocab > 1 and logits.stride(1) != 1 or logits.shape[0] > 1 and logits.stride(0) < vocab:
-            logits = logits.contiguous()
+        vocab = shape[1]
+        logits, ld = _matrix(logits, vocab)
+        ldn, at = vocab, None
         if temperature > 0.0:
             if noise is None:
-                noise = torch.empty((s.rows, vocab), dtype=torch.float32, device=self.device).exponential_(1)
-            if noise.dtype != torch.float32 or noise.dim() != 2 or noise.shape[0] < s.rows or noise.shape[1] != vocab or noise.device != self.device:
-                raise ValueError(f"paged tree: noise {tuple(noise.shape)} {noise.dtype} on {noise.device}, [{s.rows}, {vocab}] in f32 on {self.device} is wanted")
-            if vocab > 1 and noise.stride(1) != 1 or noise.shape[0] > 1 and noise.stride(0) < vocab:
-                noise = noise.contiguous()
-        else:
-            noise = None
-        make = s.starts.new_empty if s.seqs else s.starts.new_full
-        more = () if s.seqs else (-1,)
-        kept, both = make((s.rows,), *more), s.starts.new_empty((2, s.seqs))
-        size = S.lib().b2l_seq_tree_accept_work(s.rows, vocab)
-        work = torch.empty((size,), dtype=torch.uint8, device=self.device) if size else None
-        _launch(self.device, "b2l_seq_tree_accept", logits.data_ptr(), logits.stride(0) if logits.shape[0] > 1 else vocab, noise.data_ptr() if noise is not None else None,
-                noise.stride(0) if noise is not None and noise.shape[0] > 1 else vocab, float(temperature), self.parents.data_ptr(), s.starts.data_ptr(), tokens.data_ptr(),
-                int(tokens.dtype == torch.int64), kept.data_ptr(), both[0].data_ptr(), both[1].data_ptr(), work.data_ptr() if size else None, size, s.rows, s.seqs, vocab,
-                S.act_code(logits.dtype))
-        return kept, both[0], both[1]
+                noise = torch.empty((rows, vocab), dtype=torch.float32, device=self.device).exponential_(1)
+            if noise.dtype != torch.float32 or noise.dim() != 2 or noise.shape[0] < rows or noise.shape[1] != vocab or noise.device != self.device:
+                raise ValueError(f"paged tree: noise {tuple(noise.shape)} {noise.dtype} on {noise.device}, [{rows}, {vocab}] in f32 on {self.device} is wanted")
+            noise, ldn = _matrix(noise, vocab)
+            at = noise.data_ptr()
+        size = self._works.get(vocab)
+        if size is None:
+            size = self._works[vocab] = S.lib().b2l_seq_tree_accept_work(rows, vocab)
+        starts = s._tensors[0]
+        kept, counts, following = starts.new_empty(rows) if s.seqs else starts.new_full((rows,), -1), starts.new_empty(s.seqs), starts.new_empty(s.seqs)
+        work = starts.new_empty(-(-size // 4))
+        _launch(self.device, "b2l_seq_tree_accept", logits.data_ptr(), ld, at, ldn, float(temperature), self.parents.data_ptr(), starts.data_ptr(), tokens.data_ptr(), int(wide),
+                kept.data_ptr(), counts.data_ptr(), following.data_ptr(), work.data_ptr(), size, rows, s.seqs, vocab, S.act_code(logits.dtype))
+        return kept, counts, following
 
 
 class PagedCache:
@@ -524,9 +532,9 @@ class PagedCache:
             raise ValueError("paged cache: the tree of another step")
         rows, heads = step.rows, q.shape[1]                                 # masks are of these
         shape = (q.shape[0], heads, self.vdim)
-        plan = step._plans.get((rows, heads, scale, window, first, self._sizes))
+        plan = step._plans.get((rows, heads, scale, window, first, self._sizes, True))
         if plan is None:
-            plan = self._plan(rows, heads, scale, window, first, step)
+            plan = self._plan(rows, heads, scale, window, first, step, True)
         floats, sizes = plan
         zeros = out is None
         if zeros:
@@ -540,7 +548,7 @@ class PagedCache:
                    out.data_ptr(), work.data_ptr() if floats else None, floats, *sizes)
         return out
 
-    def _plan(self, rows: int, heads: int, scale: Optional[float], window: int, first: int, step: PagedStep) -> tuple:
+    def _plan(self, rows: int, heads: int, scale: Optional[float], window: int, first: int, step: PagedStep, tree: bool = False) -> tuple:
         """(floats of work space, arguments that are the same in every layer of the step); kept with the step."""
         if heads < 1 or heads % self.kv_heads:
             raise ValueError(f"paged cache: {heads} query heads over {self.kv_heads} key/value heads")
@@ -553,9 +561,10 @@ class PagedCache:
             first = 0
         sizes = (heads, self.kv_heads, self.dim, self.vdim, window, first)
         hints = (step.max_new, step.max_length) + self._codes
-        floats = S.lib().b2l_seq_paged_attention_work(rows, step.seqs, step.table.shape[1], self.page, *sizes, *hints)
+        work = S.lib().b2l_seq_paged_attention_tree_work if tree else S.lib().b2l_seq_paged_attention_work
+        floats = work(rows, step.seqs, step.table.shape[1], self.page, *sizes, *hints)
         plan = (floats, (rows, step.seqs, self.n_pages, self.page) + sizes + (float(self.dim ** -0.5 if scale is None else scale),) + hints)
-        step._plans[(rows, heads, scale, window, first, self._sizes)] = plan
+        step._plans[(rows, heads, scale, window, first, self._sizes) + ((True,) if tree else ())] = plan
         return plan
 
 
