@@ -12,6 +12,8 @@
 // A beam whose score or log-probabilities are no numbers (a score of -inf, a logit that is NaN or +inf, none above -inf) is out: its values are -inf.
 //
 // What bounds it: the logits read once; few beams: two launches.
+#include <algorithm>
+
 #include "seq_rows.cuh"
 
 namespace b2l {
@@ -64,6 +66,14 @@ template <int VECS> struct Entries<float, VECS> {
 template <int VECS> struct Entries<__nv_bfloat16, VECS> {
   uint32_t w[4 * VECS];
   __device__ __forceinline__ void load(const __nv_bfloat16* row, int at, int n) {
+    if (rows::inside<__nv_bfloat16, VECS>(at, n)) {
+#pragma unroll
+      for (int v = 0; v < VECS; ++v) {
+        const uint4 u = __ldcs(reinterpret_cast<const uint4*>(row + at + (v * (int)blockDim.x + (int)threadIdx.x) * 8));
+        w[4 * v] = u.x; w[4 * v + 1] = u.y; w[4 * v + 2] = u.z; w[4 * v + 3] = u.w;
+      }
+      return;
+    }
 #pragma unroll
     for (int v = 0; v < VECS; ++v) {
       const int i = at + (v * (int)blockDim.x + (int)threadIdx.x) * 8;
@@ -114,34 +124,52 @@ __device__ __forceinline__ float2 powers2(float x, float y, float c) {
   return make_float2(exp2_f(e.x), exp2_f(e.y));
 }
 
+// Entries that are at least `least`, as bits; bit i: entry `of(i)` of the thread
+template <int VECS> __device__ __forceinline__ unsigned long long reach(const Entries<float, VECS>& x, float least) {
+  unsigned long long hits = 0ull;
+#pragma unroll
+  for (int i = 0; i < 4 * VECS; ++i) hits |= x[i] >= least ? 1ull << i : 0ull;
+  return hits;
+}
+template <int VECS> __device__ __forceinline__ unsigned long long reach(const Entries<__nv_bfloat16, VECS>& x, float least) {      // two at a time
+  const uint32_t bound = (__float_as_uint(least) >> 16) * 0x10001u;
+  uint32_t hits[2] = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 4 * VECS; ++i) {
+    uint32_t m;
+    asm("set.ge.u32.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(x.w[i]), "r"(bound));
+    hits[i >> 4] |= m & (0x10001u << (i & 15));
+  }
+  return hits[0] | (unsigned long long)hits[1] << 32;
+}
+template <typename act_t> __device__ __forceinline__ int of(int bit) { return sizeof(act_t) == 4 ? bit : 2 * (bit & 15) + (bit >> 4 & 1) + 32 * (bit >> 5); }
+
 template <typename act_t, int ENTRIES>
-__global__ void __launch_bounds__(THREADS, ENTRIES == 32 ? (sizeof(act_t) == 2 ? 5 : 4) : 8) beam_parts_kernel(const __grid_constant__ Select a) {
+__global__ void __launch_bounds__(THREADS, ENTRIES == 8 ? 8 : sizeof(act_t) == 2 ? (ENTRIES == 64 ? 3 : 5) : 4) beam_parts_kernel(const __grid_constant__ Select a) {
   __shared__ float tops[THREADS / 32];
   __shared__ double sums[THREADS / 32];
   __shared__ __align__(16) unsigned long long bests[THREADS], list[LIST];
   __shared__ unsigned long long bound;
-  __shared__ uint32_t least_bits;
+  __shared__ float least_of;
   __shared__ int found;
   pdl_launch_dependents();                                   // the second launch waits for the end of this one
-  const int row = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const act_t* logits = reinterpret_cast<const act_t*>(a.logits) + row * a.ld;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lanes = lanes_of(a.count), groups = THREADS / lanes, unit = blockIdx.y * a.splits + blockIdx.x;
   constexpr int PER = rows::PER<act_t>;
+  const act_t* logits = reinterpret_cast<const act_t*>(a.logits) + blockIdx.y * a.ld;
   const int at = rows::border(logits) + blockIdx.x * THREADS * ENTRIES;
   Entries<act_t, ENTRIES / PER> x;
   x.load(logits, at, a.vocab);
-  auto index = [&](int i) { return at + (i / PER * THREADS + (int)threadIdx.x) * PER + i % PER; };
   auto key = [&](int i) -> unsigned long long {
-    const int v = index(i);
+    const int v = at + (i / PER * THREADS + (int)threadIdx.x) * PER + i % PER;
     return v >= 0 && v < a.vocab ? (unsigned long long)ordered(ld_act(logits, v)) << 32 | (uint32_t)~v : 0ull;
   };
   const float mine = x.top();
-  const int lanes = lanes_of(a.count), groups = THREADS / lanes;
   float group = mine;
   if (lanes == 4) {
     group = larger(group, __shfl_xor_sync(0xffffffffu, group, 1));
     group = larger(group, __shfl_xor_sync(0xffffffffu, group, 2));
   }
-  uint32_t* firsts = reinterpret_cast<uint32_t*>(bests);     // the groups' largest as integers
+  uint32_t* firsts = reinterpret_cast<uint32_t*>(bests);   // the groups' largest as integers
   if (threadIdx.x % lanes == 0) firsts[threadIdx.x / lanes] = ordered(group);
   float top = group;
 #pragma unroll
@@ -150,27 +178,26 @@ __global__ void __launch_bounds__(THREADS, ENTRIES == 32 ? (sizeof(act_t) == 2 ?
   if (threadIdx.x == 0) {
     found = 0;
     bound = 0ull;
-    least_bits = 0xffffffffu;
   }
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) top = larger(top, tops[w]);
-  const bool out = !(top > -INFINITY && top < INFINITY);     // no sum, no order: the second launch does not look at its keys unless the others' parts have numbers
   // the count-th largest of the groups' values, by counting how many are larger
   if ((int)threadIdx.x < groups) {
     const uint32_t own = firsts[threadIdx.x];
-    int above = 0;
+    int above = 0, reached = 0;
     for (int i = 0; i < groups; i += 4) {
       const uint4 y = *reinterpret_cast<const uint4*>(&firsts[i]);
       above += (y.x > own) + (y.y > own) + (y.z > own) + (y.w > own);
+      reached += (y.x >= own) + (y.y >= own) + (y.z >= own) + (y.w >= own);
     }
-    if (above < a.count) atomicMin(&least_bits, own);
+    if (above < a.count && reached >= a.count) least_of = unordered(own);      // the same from all who say it
   }
+  top = larger(larger(larger(tops[0], tops[1]), larger(tops[2], tops[3])), larger(larger(tops[4], tops[5]), larger(tops[6], tops[7])));
+  const bool out = !(top > -INFINITY && top < INFINITY);   // no sum; the second launch does not look at the keys of a beam that is out
   // the sum in pairs: five roundings at most, where one behind the other would be 32 (the rest of it is in 64 bits)
   float2 sum[ENTRIES / 4];
   const float ref = out ? 0.f : -top;
 #pragma unroll
-  for (int i = 0; i < ENTRIES; i += 4) {                     // the differences are exact, or rounded once
+  for (int i = 0; i < ENTRIES; i += 4) {                   // the differences are exact, or rounded once
     const float2 u = powers2(x[i], x[i + 1], ref), v = powers2(x[i + 2], x[i + 3], ref);
     sum[i / 4] = add2(u, v);
   }
@@ -186,24 +213,22 @@ __global__ void __launch_bounds__(THREADS, ENTRIES == 32 ? (sizeof(act_t) == 2 ?
   if (threadIdx.x == 0) {
     double s = 0.0;
     for (int w = 0; w < THREADS / 32; ++w) s += sums[w];
-    a.sums[(size_t)row * a.splits + blockIdx.x] = out ? 0.0 : s;
-    a.tops[(size_t)row * a.splits + blockIdx.x] = top != top ? INFINITY : top;
+    a.sums[unit] = out ? 0.0 : s;
+    a.tops[unit] = top != top ? INFINITY : top;
   }
   // Entries that reach the bound, found again where they come from: what to do with each is written once, not ENTRIES times
-  const float least = unordered(least_bits);
+  const float least = least_of;
   if (mine >= least) {
-    uint32_t hits = 0u;
-#pragma unroll
-    for (int i = 0; i < ENTRIES; ++i) hits |= x[i] >= least ? 1u << i : 0u;
-    if (__popc(hits) + found > LIST) atomicMax(&found, LIST + 1);      // many alike: not one after the other
+    unsigned long long hits = reach(x, least);
+    if (__popcll(hits) + found > LIST) atomicMax(&found, LIST + 1);      // many alike: not one after the other
     for (; hits && found <= LIST; hits &= hits - 1) {
-      const unsigned long long k = key(__ffs(hits) - 1);
+      const unsigned long long k = key(of<act_t>(__ffsll((long long)hits) - 1));
       const int to = k ? atomicAdd(&found, 1) : LIST;
       if (to < LIST) list[to] = k;
     }
   }
   __syncthreads();
-  if (found > LIST) {                                        // by keys, which are all different
+  if (found > LIST) {                                      // by keys, which are all different
     unsigned long long best = 0ull;
 #pragma unroll 4
     for (int i = 0; i < ENTRIES; ++i) best = max(best, key(i));
@@ -218,7 +243,7 @@ __global__ void __launch_bounds__(THREADS, ENTRIES == 32 ? (sizeof(act_t) == 2 ?
       const unsigned long long own = bests[threadIdx.x];
       int above = 0;
       for (int i = 0; i < groups; ++i) above += bests[i] > own;
-      if (above == a.count - 1 && own) bound = own;          // with fewer groups that have entries than that, all there are
+      if (above == a.count - 1 && own) bound = own;        // with fewer groups that have entries than that, all there are
     }
     __syncthreads();
     const unsigned long long from = max(bound, 1ull);
@@ -234,7 +259,7 @@ __global__ void __launch_bounds__(THREADS, ENTRIES == 32 ? (sizeof(act_t) == 2 ?
     __syncthreads();
   }
   const int n = min(found, LIST);
-  unsigned long long* keys = a.keys + ((size_t)row * a.splits + blockIdx.x) * a.count;
+  unsigned long long* keys = a.keys + (size_t)unit * a.count;
   for (int i = threadIdx.x; i < n; i += THREADS) {
     const unsigned long long own = list[i];
     int rank = 0;
@@ -250,14 +275,11 @@ __global__ void __launch_bounds__(THREADS) beam_select_kernel(const __grid_const
   __shared__ float largest[MOST_BEAMS];
   __shared__ __align__(16) unsigned long long firsts[THREADS];
   __shared__ Key list[LIST / 2];
-  __shared__ unsigned long long least_bits;
+  __shared__ unsigned long long least_of;
   __shared__ int found;
   const int group = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = a.splits * a.count, all = a.beams * per;
   const unsigned long long* keys = a.keys + (size_t)group * all;
-  if (threadIdx.x == 0) {
-    found = 0;
-    least_bits = ~0ull;
-  }
+  if (threadIdx.x == 0) found = 0;
   pdl_wait();
   unsigned long long held[HELD];
 #pragma unroll
@@ -325,15 +347,16 @@ __global__ void __launch_bounds__(THREADS) beam_select_kernel(const __grid_const
   __syncthreads();
   if ((int)threadIdx.x < groups) {
     const unsigned long long own = firsts[threadIdx.x];
-    int above = 0;
+    int above = 0, reached = 0;
     for (int i = 0; i < groups; i += 2) {
       const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(&firsts[i]);
       above += (y.x > own) + (y.y > own);
+      reached += (y.x >= own) + (y.y >= own);
     }
-    if (above < a.count) atomicMin(&least_bits, own);
+    if (above < a.count && reached >= a.count) least_of = own;      // the same from all who say it
   }
   __syncthreads();
-  const unsigned long long least = max(least_bits, 1ull);
+  const unsigned long long least = max(least_of, 1ull);
   if (mine >= least) {
     auto take = [&](int i, unsigned long long k) {
       const int to = atomicAdd(&found, 1);
@@ -410,6 +433,7 @@ extern "C" int b2l_seq_beam_select(const void* logits, long long ld, const float
   const long long need = b2l_seq_beam_work(groups, beams, vocab, count);
   B2L_CHECK_ARG(work && work_bytes >= need && ((uintptr_t)work & 15) == 0, "%s: a work space of %lld bytes is needed", who, need);
   const int rows = groups * beams, splits = splits_of(rows, vocab);
+  B2L_CHECK_SUPPORTED((long long)rows * splits < (1ll << 31), "%s: %d rows over %d tokens", who, rows, vocab);
   Select a{logits, scores, ld, groups, beams, vocab, count, splits};
   a.keys = (unsigned long long*)work;
   a.sums = (double*)(a.keys + (size_t)rows * splits * count);

@@ -70,72 +70,91 @@ struct Targets {
   int rows, vocab, splits;
   Best* parts;                                               // [rows][splits]
 };
-constexpr int THREADS = 256, ENTRIES = 16, CHUNK = THREADS * ENTRIES;
+// A warp goes through its part of a row by itself, 512 entries at a time: what is near the largest so far it notes, and with barriers between the steps (a block's
+// largest first, then what is near it) 32 trees with noise took 49 us in place of 36.
+constexpr int THREADS = 256, ENTRIES = 16, ROUNDS = 2, CHUNK = THREADS * ENTRIES * ROUNDS, LIST = 1024;
 
 template <typename act_t, bool DRAWN>
-__global__ void __launch_bounds__(THREADS) tree_targets_kernel(const __grid_constant__ Targets a) {
-  __shared__ float tops[THREADS / 32];
+__global__ void __launch_bounds__(THREADS, 5) tree_targets_kernel(const __grid_constant__ Targets a) {
   __shared__ Best bests[THREADS / 32];
-  __shared__ int list[DRAWN ? CHUNK : 1], found;
+  __shared__ int list[DRAWN ? LIST : 1], found;
   pdl_launch_dependents();                                   // the second launch waits for the end of this one
   const int row = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const act_t* logits = reinterpret_cast<const act_t*>(a.logits) + row * a.ld;
-  constexpr int VECS = ENTRIES / rows::PER<act_t>;
+  const float* noise = DRAWN ? a.noise + row * a.ldn : nullptr;
+  constexpr int PER = rows::PER<act_t>;
   const int at = rows::border(logits) + blockIdx.x * CHUNK;
-  float x[ENTRIES];
-  rows::load<act_t, VECS>(logits, at, a.vocab, -INFINITY, x);
-  auto index = [&](int i) { return at + (i / rows::PER<act_t> * THREADS + (int)threadIdx.x) * rows::PER<act_t> + i % rows::PER<act_t>; };
+  const bool even = DRAWN && ((uintptr_t)(noise + at) & 15) == 0;
+  const float over = DRAWN ? 1.f / a.temperature : 1.f;
+  constexpr float LN2 = 0.693147182464599609375f, SLACK = 1.9073486328125e-6f;      // 2^-19
   Best best{-INFINITY, INT32_MAX};
-  if constexpr (!DRAWN) {
+  auto exactly = [&](int v) {
+    if (v < 0 || v >= a.vocab) return;
+    const Best here{(double)ld_act(logits, v) / (double)a.temperature - log((double)noise[v]), v};
+    if (here.value > -INFINITY && better(here, best)) best = here;
+  };
+  if (DRAWN) {
+    if (threadIdx.x == 0) found = 0;
+    __syncthreads();
+  }
+  float top = -INFINITY;                                     // of the warp so far
+#pragma unroll 1
+  for (int round = 0; round < ROUNDS; ++round) {
+    const int from = at + round * THREADS * ENTRIES;
+    if (from >= a.vocab) break;
+    float x[ENTRIES];
+    rows::load<act_t, ENTRIES / PER>(logits, from, a.vocab, -INFINITY, x);
+    auto index = [&](int i) { return from + (i / PER * THREADS + (int)threadIdx.x) * PER + i % PER; };
+    if constexpr (!DRAWN) {
 #pragma unroll
-    for (int i = 0; i < ENTRIES; ++i)
-      if (x[i] > best.value) best = {x[i], index(i)};        // no NaN; a thread's entries ascend
-  } else {
-    const float* noise = a.noise + row * a.ldn;
-    const float over = 1.f / a.temperature;
-    float y[ENTRIES], top = -INFINITY;
-    const bool even = ((uintptr_t)(noise + at) & 15) == 0;
+      for (int i = 0; i < ENTRIES; ++i)
+        if (x[i] > best.value) best = {x[i], index(i)};      // no NaN; a thread's entries ascend
+    } else {
+      float y[ENTRIES];
+      if (even && rows::inside<act_t, ENTRIES / PER>(from, a.vocab)) {
+        float4 u[ENTRIES / 4];
 #pragma unroll
-    for (int i = 0; i < ENTRIES; i += 4) {
-      const int v = index(i);
-      if (even && v >= 0 && v + 4 <= a.vocab) {
-        const float4 u = __ldcs(reinterpret_cast<const float4*>(noise + v));
-        y[i] = u.x; y[i + 1] = u.y; y[i + 2] = u.z; y[i + 3] = u.w;
-      } else {
+        for (int i = 0; i < ENTRIES / 4; ++i) u[i] = __ldcs(reinterpret_cast<const float4*>(noise + index(4 * i)));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[i + e] = v + e >= 0 && v + e < a.vocab ? __ldcs(noise + v + e) : 1.f;
+        for (int i = 0; i < ENTRIES / 4; ++i) {
+          y[4 * i] = u[i].x; y[4 * i + 1] = u[i].y; y[4 * i + 2] = u[i].z; y[4 * i + 3] = u[i].w;
+        }
+      } else
+#pragma unroll
+      for (int i = 0; i < ENTRIES; i += 4) {
+        const int v = index(i);
+        if (even && v >= 0 && v + 4 <= a.vocab) {
+          const float4 u = __ldcs(reinterpret_cast<const float4*>(noise + v));
+          y[i] = u.x; y[i + 1] = u.y; y[i + 2] = u.z; y[i + 3] = u.w;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[i + e] = v + e >= 0 && v + e < a.vocab ? __ldcs(noise + v + e) : 1.f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < ENTRIES; ++i) {                    // x / T - log q, off by less than 2^-21 of its two terms together
+        asm("lg2.approx.f32 %0, %1;" : "=f"(y[i]) : "f"(y[i]));
+        x[i] = fmaf(y[i], -LN2, x[i] * over);
+        top = fmaxf(top, x[i]);                              // NaN: not the largest
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      // Those near the largest, one or two, again in 64 bits: x / T is no larger than its difference and the logarithm together, and a logarithm at most 104, so the
+      // largest is off by 2^-21 (208 + |top|) at most and one near it by 2^-21 (|top| + 2 |log q|)
+      const float least = top - SLACK * (64.f + 2.f * fabsf(top));
+      uint32_t hits = 0u;
+#pragma unroll
+      for (int i = 0; i < ENTRIES; ++i) hits |= fmaf(fabsf(y[i]), SLACK, x[i]) >= least || x[i] == top ? 1u << i : 0u;
+      for (; hits; hits &= hits - 1) {
+        const int to = atomicAdd(&found, 1), v = index(__ffs(hits) - 1);
+        if (to < LIST) list[to] = v;
+        else exactly(v);                                     // many alike
       }
     }
-    if (threadIdx.x == 0) found = 0;
-    constexpr float LN2 = 0.693147182464599609375f, SLACK = 1.9073486328125e-6f;      // 2^-19
-#pragma unroll
-    for (int i = 0; i < ENTRIES; ++i) {                      // x / T - log q, off by less than 2^-21 of its two terms together
-      asm("lg2.approx.f32 %0, %1;" : "=f"(y[i]) : "f"(y[i]));
-      top = fmaxf(top, fmaf(y[i], -LN2, x[i] * over));       // NaN: not the largest
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) tops[warp] = top;
+  }
+  if constexpr (DRAWN) {
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) top = fmaxf(top, tops[w]);
-    // Those near the largest, one or two, again in 64 bits: x / T is no larger than its difference and the logarithm together, and a logarithm at most 104, so the largest
-    // is off by 2^-21 (208 + |top|) at most and one near it by 2^-21 (|top| + 2 |log q|)
-    const float least = top - SLACK * (64.f + 2.f * fabsf(top));
-    uint32_t hits = 0u;
-#pragma unroll
-    for (int i = 0; i < ENTRIES; ++i) {
-      const float z = fmaf(y[i], -LN2, x[i] * over);
-      hits |= fmaf(fabsf(y[i]), SLACK, z) >= least || z == top ? 1u << i : 0u;
-    }
-    for (; hits; hits &= hits - 1) list[atomicAdd(&found, 1)] = index(__ffs(hits) - 1);
-    __syncthreads();
-    for (int i = threadIdx.x; i < found; i += THREADS) {
-      const int v = list[i];
-      if (v < 0 || v >= a.vocab) continue;
-      const Best here{(double)ld_act(logits, v) / (double)a.temperature - log((double)noise[v]), v};
-      if (here.value > -INFINITY && better(here, best)) best = here;
-    }
+    for (int i = threadIdx.x; i < min(found, LIST); i += THREADS) exactly(list[i]);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
