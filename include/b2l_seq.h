@@ -578,7 +578,7 @@ int b2l_seq_paged_copy(const void* const* pools, int layers, const int* pairs, i
                        b2l_stream_t stream);
 int b2l_seq_beam_select(const void* logits, long long ld, const float* scores, float* values, int* from, int* tokens, void* work, long long work_bytes, int groups, int beams,
                         int vocab, int count, int act_dtype, b2l_stream_t stream);
-long long b2l_seq_beam_work(int groups, int beams, int vocab, int count);
+long long b2l_seq_beam_work(int groups, int beams, int vocab, int count, int act_dtype);
 
 #ifdef __cplusplus
 }

@@ -231,7 +231,7 @@ _SIGS = {
     "b2l_seq_paged_keep": (c_int, [c_void_p, c_int] + [c_void_p] * 3 + [c_int] * 2 + [c_void_p] * 2 + [c_int] * 9 + [c_void_p]),
     "b2l_seq_paged_copy": (c_int, [c_void_p, c_int, c_void_p] + [c_int] * 8 + [c_void_p]),
     "b2l_seq_beam_select": (c_int, [c_void_p, C.c_longlong] + [c_void_p] * 5 + [C.c_longlong] + [c_int] * 5 + [c_void_p]),
-    "b2l_seq_beam_work": (C.c_longlong, [c_int] * 4),
+    "b2l_seq_beam_work": (C.c_longlong, [c_int] * 5),
 }
 
 EXPORTS = tuple(_SIGS)

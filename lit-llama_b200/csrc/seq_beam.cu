@@ -19,7 +19,7 @@
 namespace b2l {
 namespace beam {
 
-constexpr int THREADS = 256, MOST_COUNT = 64, MOST_BEAMS = 64, LIST = 2048;
+constexpr int THREADS = 256, MOST_COUNT = 64, MOST_BEAMS = 64, LIST = 4096;
 
 struct Key { unsigned long long hi; uint32_t lo; };          // larger first, then the lowest `lo`
 __device__ __forceinline__ bool before(const Key& x, const Key& y) { return x.hi > y.hi || (x.hi == y.hi && x.lo < y.lo); }
@@ -124,6 +124,24 @@ __device__ __forceinline__ float2 powers2(float x, float y, float c) {
   return make_float2(exp2_f(e.x), exp2_f(e.y));
 }
 
+// The sum of entries I .. I + N - 1's e^(x + c), in pairs: six roundings at most for 64, where one behind the other would be as many (the rest of the sum is in 64 bits).
+// Halves one after the other, so that few of them are in registers
+template <int I, int N, typename E> __device__ __forceinline__ float2 powers(const E& x, float c) {
+  if constexpr (N == 2) return powers2(x[I], x[I + 1], c);
+  else return add2(powers<I, N / 2>(x, c), powers<I + N / 2, N / 2>(x, c));
+}
+// Of threads that have one of GROUPS values each: those whose value is the count-th largest say so
+template <int GROUPS> __device__ __forceinline__ bool is_nth(const uint32_t* all, uint32_t own, int count) {
+  int above = 0, reached = 0;
+#pragma unroll(GROUPS == 64 ? 16 : 8)
+  for (int i = 0; i < GROUPS; i += 4) {
+    const uint4 y = *reinterpret_cast<const uint4*>(all + i);
+    above += (y.x > own) + (y.y > own) + (y.z > own) + (y.w > own);
+    reached += (y.x >= own) + (y.y >= own) + (y.z >= own) + (y.w >= own);
+  }
+  return above < count && reached >= count;
+}
+
 // Entries that are at least `least`, as bits; bit i: entry `of(i)` of the thread
 template <int VECS> __device__ __forceinline__ unsigned long long reach(const Entries<float, VECS>& x, float least) {
   unsigned long long hits = 0ull;
@@ -145,7 +163,7 @@ template <int VECS> __device__ __forceinline__ unsigned long long reach(const En
 template <typename act_t> __device__ __forceinline__ int of(int bit) { return sizeof(act_t) == 4 ? bit : 2 * (bit & 15) + (bit >> 4 & 1) + 32 * (bit >> 5); }
 
 template <typename act_t, int ENTRIES>
-__global__ void __launch_bounds__(THREADS, ENTRIES == 8 ? 8 : sizeof(act_t) == 2 ? (ENTRIES == 64 ? 3 : 5) : 4) beam_parts_kernel(const __grid_constant__ Select a) {
+__global__ void __launch_bounds__(THREADS, ENTRIES == 8 ? 8 : sizeof(act_t) == 2 ? (ENTRIES == 64 ? 4 : 5) : 4) beam_parts_kernel(const __grid_constant__ Select a) {
   __shared__ float tops[THREADS / 32];
   __shared__ double sums[THREADS / 32];
   __shared__ __align__(16) unsigned long long bests[THREADS], list[LIST];
@@ -183,29 +201,12 @@ __global__ void __launch_bounds__(THREADS, ENTRIES == 8 ? 8 : sizeof(act_t) == 2
   // the count-th largest of the groups' values, by counting how many are larger
   if ((int)threadIdx.x < groups) {
     const uint32_t own = firsts[threadIdx.x];
-    int above = 0, reached = 0;
-    for (int i = 0; i < groups; i += 4) {
-      const uint4 y = *reinterpret_cast<const uint4*>(&firsts[i]);
-      above += (y.x > own) + (y.y > own) + (y.z > own) + (y.w > own);
-      reached += (y.x >= own) + (y.y >= own) + (y.z >= own) + (y.w >= own);
-    }
-    if (above < a.count && reached >= a.count) least_of = unordered(own);      // the same from all who say it
+    if (lanes == 4 ? is_nth<64>(firsts, own, a.count) : is_nth<THREADS>(firsts, own, a.count)) least_of = unordered(own);      // the same from all who say it
   }
   top = larger(larger(larger(tops[0], tops[1]), larger(tops[2], tops[3])), larger(larger(tops[4], tops[5]), larger(tops[6], tops[7])));
   const bool out = !(top > -INFINITY && top < INFINITY);   // no sum; the second launch does not look at the keys of a beam that is out
-  // the sum in pairs: five roundings at most, where one behind the other would be 32 (the rest of it is in 64 bits)
-  float2 sum[ENTRIES / 4];
-  const float ref = out ? 0.f : -top;
-#pragma unroll
-  for (int i = 0; i < ENTRIES; i += 4) {                   // the differences are exact, or rounded once
-    const float2 u = powers2(x[i], x[i + 1], ref), v = powers2(x[i + 2], x[i + 3], ref);
-    sum[i / 4] = add2(u, v);
-  }
-#pragma unroll
-  for (int n = ENTRIES / 8; n > 0; n /= 2)
-#pragma unroll
-    for (int i = 0; i < n; ++i) sum[i] = add2(sum[i], sum[i + n]);
-  double all = sum[0].x + sum[0].y;
+  const float2 sum = powers<0, ENTRIES>(x, out ? 0.f : -top);
+  double all = sum.x + sum.y;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
   if (lane == 0) sums[warp] = all;
@@ -263,29 +264,31 @@ __global__ void __launch_bounds__(THREADS, ENTRIES == 8 ? 8 : sizeof(act_t) == 2
   for (int i = threadIdx.x; i < n; i += THREADS) {
     const unsigned long long own = list[i];
     int rank = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) rank += list[j] > own;
     if (rank < a.count) keys[rank] = own;
   }
   for (int i = n + (int)threadIdx.x; i < a.count; i += THREADS) keys[i] = 0ull;
 }
 
-constexpr int HELD = 8;              // entries of a thread that stay in registers
+// What bounds it: a chain of loads, logarithms in 64 bits, and code that runs once.  One group of 512 entries 6.9 us, 48 of 896 11.2 us.
+constexpr int HELD = 2048, TIES = 1024;      // entries in shared memory; of those that reach the bound
 __global__ void __launch_bounds__(THREADS) beam_select_kernel(const __grid_constant__ Select a) {
   __shared__ double offset[MOST_BEAMS];                      // score less the logarithm of the sum of exp(x - largest); NaN: the beam is out
   __shared__ float largest[MOST_BEAMS];
   __shared__ __align__(16) unsigned long long firsts[THREADS];
-  __shared__ Key list[LIST / 2];
+  __shared__ Key list[TIES];
+  __shared__ unsigned long long held[HELD];
   __shared__ unsigned long long least_of;
   __shared__ int found;
   const int group = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = a.splits * a.count, all = a.beams * per;
   const unsigned long long* keys = a.keys + (size_t)group * all;
   if (threadIdx.x == 0) found = 0;
   pdl_wait();
-  unsigned long long held[HELD];
-#pragma unroll
-  for (int k = 0; k < HELD; ++k) {
-    const int i = threadIdx.x + THREADS * k;
-    held[k] = i < all ? keys[i] : 0ull;
+  if (all <= HELD) {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < all; i += THREADS) held[i] = keys[i];
+    keys = held;
   }
   for (int w = warp; w < a.beams; w += THREADS / 32) {       // a warp for a beam
     const size_t at = ((size_t)group * a.beams + w) * a.splits;
@@ -314,8 +317,11 @@ __global__ void __launch_bounds__(THREADS) beam_select_kernel(const __grid_const
     }
   }
   __syncthreads();
+  const float over = 1.f / (float)per;
   auto entry = [&](int i, unsigned long long k) -> Key {     // of a beam's and a part's largest the next
-    const int w = i / per;
+    int w = (int)((float)i * over);                          // i / per, or one off: fewer than 2^24 entries
+    w += (w + 1) * per <= i;
+    w -= w * per > i;
     const double c = offset[w];
     if (c != c) {
       const int r = i - w * per;
@@ -329,51 +335,50 @@ __global__ void __launch_bounds__(THREADS) beam_select_kernel(const __grid_const
     a.from[to] = (int)(k.lo / (uint32_t)a.vocab);
     a.tokens[to] = (int)(k.lo % (uint32_t)a.vocab);
   };
-  unsigned long long mine = 0ull, values[HELD];
-#pragma unroll
-  for (int k = 0; k < HELD; ++k) {
-    const int i = threadIdx.x + THREADS * k;
-    values[k] = i < all ? entry(i, held[k]).hi : 0ull;
-    mine = max(mine, values[k]);
-  }
-  for (int i = threadIdx.x + THREADS * HELD; i < all; i += THREADS) mine = max(mine, entry(i, keys[i]).hi);
   const int lanes = lanes_of(a.count), groups = THREADS / lanes;
-  unsigned long long best = mine;
-  if (lanes == 4) {
-    best = max(best, __shfl_xor_sync(0xffffffffu, best, 1));
-    best = max(best, __shfl_xor_sync(0xffffffffu, best, 2));
-  }
-  if (threadIdx.x % lanes == 0) firsts[threadIdx.x / lanes] = best;
-  __syncthreads();
-  if ((int)threadIdx.x < groups) {
-    const unsigned long long own = firsts[threadIdx.x];
-    int above = 0, reached = 0;
-    for (int i = 0; i < groups; i += 2) {
-      const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(&firsts[i]);
-      above += (y.x > own) + (y.y > own);
-      reached += (y.x >= own) + (y.y >= own);
+  unsigned long long mine = 0ull, least = 0ull;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {                     // the largest value of each thread; then what reaches the bound
+    if (pass == 0 || mine >= least)
+#pragma unroll 1
+      for (int i = threadIdx.x; i < all; i += THREADS) {
+        const Key k = entry(i, keys[i]);
+        if (pass == 0) {
+          mine = max(mine, k.hi);
+        } else if (k.hi >= least) {
+          const int to = atomicAdd(&found, 1);
+          if (to < TIES) list[to] = k;
+        }
+      }
+    if (pass == 1) break;
+    unsigned long long best = mine;
+    if (lanes == 4) {
+      best = max(best, __shfl_xor_sync(0xffffffffu, best, 1));
+      best = max(best, __shfl_xor_sync(0xffffffffu, best, 2));
     }
-    if (above < a.count && reached >= a.count) least_of = own;      // the same from all who say it
-  }
-  __syncthreads();
-  const unsigned long long least = max(least_of, 1ull);
-  if (mine >= least) {
-    auto take = [&](int i, unsigned long long k) {
-      const int to = atomicAdd(&found, 1);
-      if (to < LIST / 2) list[to] = entry(i, k);
-    };
-#pragma unroll
-    for (int k = 0; k < HELD; ++k)
-      if (values[k] >= least) take(threadIdx.x + THREADS * k, held[k]);
-    for (int i = threadIdx.x + THREADS * HELD; i < all; i += THREADS)
-      if (entry(i, keys[i]).hi >= least) take(i, keys[i]);
+    if (threadIdx.x % lanes == 0) firsts[threadIdx.x / lanes] = best;
+    __syncthreads();
+    if ((int)threadIdx.x < groups) {
+      const unsigned long long own = firsts[threadIdx.x];
+      int above = 0, reached = 0;
+#pragma unroll 4
+      for (int i = 0; i < groups; i += 2) {
+        const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(&firsts[i]);
+        above += (y.x > own) + (y.y > own);
+        reached += (y.x >= own) + (y.y >= own);
+      }
+      if (above < a.count && reached >= a.count) least_of = own;      // the same from all who say it
+    }
+    __syncthreads();
+    least = max(least_of, 1ull);
   }
   __syncthreads();
   const int n = found;
-  if (n <= LIST / 2) {
+  if (n <= TIES) {
     for (int i = threadIdx.x; i < n; i += THREADS) {
       const Key own = list[i];
       int rank = 0;
+#pragma unroll 4
       for (int j = 0; j < n; ++j) rank += before(list[j], own);
       if (rank < a.count) put(own, rank);
     }
@@ -402,10 +407,13 @@ __global__ void __launch_bounds__(THREADS) beam_select_kernel(const __grid_const
   }
 }
 
-// Entries of a thread: 32 where the parts fill the GPU, else 8, so that more SMs have one
-static int entries_of(long long rows, int vocab) { return rows * ((vocab + 8191) / 8192) >= 2ll * sm_count() ? 32 : 8; }
-static int splits_of(long long rows, int vocab) {
-  const int per = THREADS * entries_of(rows, vocab);
+// Entries of a thread: 32 (bf16: 64) where the parts fill the GPU, else 8, so that more SMs have one
+static int entries_of(long long rows, int vocab, int act_dtype) {
+  const int large = act_dtype == B2L_BF16 ? 64 : 32;
+  return rows * ((vocab + THREADS * large - 1) / (THREADS * large)) >= 2ll * sm_count() ? large : 8;
+}
+static int splits_of(long long rows, int vocab, int act_dtype) {
+  const int per = THREADS * entries_of(rows, vocab, act_dtype);
   return (vocab + 7 + per - 1) / per;                        // 7: a row that does not begin on a border
 }
 
@@ -414,9 +422,9 @@ static int splits_of(long long rows, int vocab) {
 
 using namespace b2l;
 
-extern "C" long long b2l_seq_beam_work(int groups, int beams, int vocab, int count) {
+extern "C" long long b2l_seq_beam_work(int groups, int beams, int vocab, int count, int act_dtype) {
   if (groups <= 0 || beams <= 0 || vocab <= 0 || count <= 0) return 0;
-  const long long rows = (long long)groups * beams, parts = rows * beam::splits_of(rows, vocab);
+  const long long rows = (long long)groups * beams, parts = rows * beam::splits_of(rows, vocab, act_dtype);
   return parts * (8ll * count + 8 + 4);
 }
 
@@ -430,10 +438,10 @@ extern "C" int b2l_seq_beam_select(const void* logits, long long ld, const float
                       "%s: %d groups of %d beams over %d tokens, %d of them: at most 65535 rows, %d beams, %d of them", who, groups, beams, vocab, count, MOST_BEAMS, MOST_COUNT);
   B2L_CHECK_ARG(count <= (long long)beams * vocab, "%s: %d of %lld", who, count, (long long)beams * vocab);
   if (groups == 0) return 0;
-  const long long need = b2l_seq_beam_work(groups, beams, vocab, count);
+  const long long need = b2l_seq_beam_work(groups, beams, vocab, count, act_dtype);
   B2L_CHECK_ARG(work && work_bytes >= need && ((uintptr_t)work & 15) == 0, "%s: a work space of %lld bytes is needed", who, need);
-  const int rows = groups * beams, splits = splits_of(rows, vocab);
-  B2L_CHECK_SUPPORTED((long long)rows * splits < (1ll << 31), "%s: %d rows over %d tokens", who, rows, vocab);
+  const int rows = groups * beams, splits = splits_of(rows, vocab, act_dtype);
+  B2L_CHECK_SUPPORTED((long long)rows * splits < (1ll << 31) && (long long)beams * splits * count < (1ll << 24), "%s: %d rows over %d tokens, %d of them", who, rows, vocab, count);
   Select a{logits, scores, ld, groups, beams, vocab, count, splits};
   a.keys = (unsigned long long*)work;
   a.sums = (double*)(a.keys + (size_t)rows * splits * count);
@@ -442,9 +450,9 @@ extern "C" int b2l_seq_beam_select(const void* logits, long long ld, const float
   a.from = from;
   a.tokens = tokens;
   const cudaStream_t st = (cudaStream_t)stream;
-  const bool large = entries_of(rows, vocab) == 32;
+  const bool large = entries_of(rows, vocab, act_dtype) > 8;
   B2L_SEQ_DISPATCH(act_dtype, {
-    if (large) beam_parts_kernel<act_t, 32><<<dim3(splits, rows), THREADS, 0, st>>>(a);
+    if (large) beam_parts_kernel<act_t, sizeof(act_t) == 2 ? 64 : 32><<<dim3(splits, rows), THREADS, 0, st>>>(a);
     else beam_parts_kernel<act_t, 8><<<dim3(splits, rows), THREADS, 0, st>>>(a);
   });
   B2L_LAUNCH_CHECK("beam_parts_kernel");

@@ -35,7 +35,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int) -> Tuple
         logits, ld = logits.contiguous(), vocab
     if not scores.is_contiguous():
         scores = scores.contiguous()
-    size = _work(groups, beams, vocab, count, device.index)
+    size = _work(groups, beams, vocab, count, logits.dtype, device.index)
     values = scores.new_empty((groups, count))
     of, tokens = scores.new_empty((groups, count), dtype=torch.int32), scores.new_empty((groups, count), dtype=torch.int32)
     work = scores.new_empty(-(-size // 4))
@@ -45,9 +45,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int) -> Tuple
 
 
 @lru_cache(maxsize=256)
-def _work(groups: int, beams: int, vocab: int, count: int, device) -> int:
+def _work(groups: int, beams: int, vocab: int, count: int, dtype: torch.dtype, device) -> int:
     """Bytes of work space: by the device too, whose SMs decide how rows are split."""
     if device is None:
         return 0                                                            # refused by the launch
     with torch.cuda.device(device):
-        return S.lib().b2l_seq_beam_work(groups, beams, vocab, count)
+        return S.lib().b2l_seq_beam_work(groups, beams, vocab, count, S.act_code(dtype))
