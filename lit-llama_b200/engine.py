@@ -5,7 +5,8 @@ A model plugs in through three members: `state_specs()` (what a sequence carries
 return f32 logits at the wanted places); one that books memory of its own for a slot (pages of a cache) is told by
 `release_slot(slot)` when its request is gone, and may be asked `has_room(live, tokens, portion)` (slot -> the tokens that its sequence grows to)
 before a request of `tokens` tokens is let in beside the live ones; where several engines may have it, `for_engine()` gives each the object that it calls, with
-slots of its own.  The engine owns the `SequenceStatePool`, maps request ids to slots,
+slots of its own.  Beam search asks for `reorder_slots(sources)` and `forward_together(slots, positions, tokens)`, drafted tokens for `forward_tree(..)` and `keep(..)`
+(the LLaMA with pages has them, registry.py).  The engine owns the `SequenceStatePool`, maps request ids to slots,
 and offers two ways in:
 
   * `step(entries, end)`: the caller decides which tokens each request gets in this step (a replayed trace,
@@ -19,7 +20,7 @@ keeps coming (a long prompt's chunks) for models whose launches depend on the le
 width 1024 is 64 launches, 490 us on the device and 920 from Python."""
 from collections import OrderedDict, deque
 from dataclasses import dataclass, field
-from typing import Dict, Hashable, List, Optional, Sequence
+from typing import Callable, Dict, Hashable, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -273,3 +274,143 @@ class Engine:
         rid = ("generate", self.steps, len(self.finished))
         self.add_request(rid, prompt, max_new_tokens, **kw)
         return list(prompt) + self.run()[rid]
+
+    # ------------------------------------------------------------------ several continuations of a prompt
+    def _begin(self, rid: Hashable, prompt: Sequence[int]) -> torch.Tensor:
+        """The prompt through a slot of its own, in portions; logits of its last token."""
+        if not prompt:
+            raise ValueError("empty prompt")
+        self.pool.acquire(rid)
+        for at in range(0, len(prompt), self.prefill_chunk):
+            part = prompt[at:at + self.prefill_chunk]
+            out = self._run(rid, part, [len(part) - 1] if at + len(part) == len(prompt) else [])
+        return out
+
+    def beam_search(self, prompt: Sequence[int], max_new_tokens: int, beams: int, *, eos_id: Optional[int] = None,
+                    length_penalty: float = 1.0) -> List[Tuple[List[int], float]]:
+        """The most likely continuations found by a search that keeps the `beams` (at most 32) best by sums of log-probabilities, token by token: (generated tokens, the EOS
+        token included, sum / length ** length_penalty), the best first, at most `beams`.  One that ends in EOS is finished; the search ends when `beams` are and none
+        that goes on scores higher at its present length, or after max_new_tokens.  Takes a slot for every beam, beside those of live requests; the beams share the pages
+        of what they have in common."""
+        m, ids = self.model, []
+        if not hasattr(m, "reorder_slots"):
+            raise RuntimeError(f"{type(m).__name__}: beams need a model whose sequences can be forked")
+        if not 1 <= beams <= 32 or max_new_tokens < 1:
+            raise ValueError(f"beam search: {beams} beams of {max_new_tokens} tokens: 1 to 32, at least one")
+        if self.pool.free_slots() < beams:
+            raise PoolFull(f"{beams} beams, {self.pool.free_slots()} free slots")
+        from .search import beam_select
+
+        def score(total: float, n: int) -> float:
+            return total / n ** length_penalty
+
+        done: List[Tuple[List[int], float]] = []
+        try:
+            ids.append(("beam", self.steps, 0))
+            logits = self._begin(ids[0], list(prompt))
+            live: List[Tuple[List[int], float]] = [([], 0.0)]
+            for n in range(1, max_new_tokens + 1):
+                scores = torch.tensor([[s for _, s in live]], dtype=torch.float32).to(self.device)
+                found = beam_select(logits[None], scores, min(2 * beams, logits.numel()))
+                values, of, tokens = (x[0].tolist() for x in found)
+                after, sources = [], []
+                for rank, (value, w, token) in enumerate(zip(values, of, tokens)):
+                    if value == float("-inf"):
+                        break
+                    if eos_id is not None and token == eos_id:
+                        if rank < beams:
+                            done.append((live[w][0] + [token], score(value, n)))
+                    elif len(after) < beams:
+                        after.append((live[w][0] + [token], value))
+                        sources.append(w)
+                done.sort(key=lambda x: -x[1])
+                del done[beams:]
+                if not after or n == max_new_tokens or (len(done) == beams and score(after[0][1], n) <= done[-1][1]):
+                    done += [(x, score(s, n)) for x, s in after]
+                    break
+                self._reorder(ids, sources)
+                live = after
+                logits = self._together(ids[:len(live)], [x[-1] for x, _ in live])
+        finally:
+            for rid in ids:
+                if self.pool.has(rid):
+                    self.pool.release(rid)
+        return sorted(done, key=lambda x: -x[1])[:beams]
+
+    def _reorder(self, ids: List[Hashable], sources: List[int]) -> None:
+        """Sequence i goes on from what sequence sources[i] had; more or fewer of them than there were."""
+        position = self.pool.position(ids[0])
+        while len(ids) < len(sources):
+            ids.append(ids[0][:-1] + (len(ids),))
+            self.pool.acquire(ids[-1])
+            self.pool.reserve(ids[-1], position)
+            self.pool.advance(ids[-1], position)
+        slots = [self.pool.slot(rid) for rid in ids]
+        self.model.reorder_slots({slots[i]: slots[w] for i, w in enumerate(sources)})
+        while len(ids) > len(sources):
+            self.pool.release(ids.pop())
+
+    def _together(self, ids: Sequence[Hashable], tokens: Sequence[int]) -> torch.Tensor:
+        """One more token of each sequence; f32 logits [sequences, vocab]."""
+        at = [self.pool.position(rid) for rid in ids]
+        cap = getattr(self.model, "max_positions", 0)
+        if cap and max(at) + 1 > cap:
+            raise PoolFull(f"beams would reach position {max(at) + 1}, a slot holds {cap}")
+        if self.pool.max_tokens and self.pool.live_tokens() + len(ids) > self.pool.max_tokens:
+            raise PoolFull(f"{self.pool.live_tokens()} live tokens + {len(ids)} exceed the budget of {self.pool.max_tokens}")
+        out = self.model.forward_together([self.pool.slot(rid) for rid in ids], at, torch.tensor(list(tokens), dtype=torch.int64).to(self.device))
+        for rid in ids:
+            self.pool.advance(rid, 1)
+        self.steps += 1
+        return out
+
+    def generate_drafted(self, prompt: Sequence[int], max_new_tokens: int, draft: Callable[[List[int]], Tuple[Sequence[int], Sequence[int]]], *, temperature: float = 0.0,
+                         eos_id: Optional[int] = None) -> List[int]:
+        """As `generate` (prompt + generated tokens; no top_k), several tokens a step where `draft` guesses well.  draft(tokens so far) returns the guessed tokens and their
+        parents: the place in the guess of the token that each follows, before it, or -1 for what follows the last token so far; both may be empty.  What comes out is what the
+        model chooses itself, token by token: the guesses only save steps."""
+        m, rid = self.model, ("drafted", self.steps)
+        if not hasattr(m, "forward_tree"):
+            raise RuntimeError(f"{type(m).__name__}: drafts need a model that takes trees of tokens")
+        if max_new_tokens < 1:
+            return list(prompt)
+        tokens = list(prompt)
+        end = len(tokens) + max_new_tokens
+        try:
+            logits = self._begin(rid, tokens)
+            tokens.append(self._sample(logits[0], Request(rid, [], 1, temperature)))
+            while len(tokens) < end and (eos_id is None or tokens[-1] != eos_id):
+                guess, parents = (list(x) for x in draft(list(tokens)))
+                if len(guess) != len(parents) or any(not -1 <= p < i for i, p in enumerate(parents)):
+                    raise ValueError("draft: as many parents as tokens, each before its token or -1")
+                pos0, slot = self.pool.position(rid), self.pool.slot(rid)
+                room = [end - len(tokens) - 1] + [cap - pos0 - 1 for cap in (getattr(m, "max_positions", 0),) if cap]
+                if self.pool.max_tokens:
+                    room.append(self.pool.max_tokens - self.pool.live_tokens() - 1)
+                if min(room[1:], default=0) < 0:
+                    raise PoolFull(f"request {rid!r} would reach position {pos0 + 1}")
+                del guess[max(min(room), 0):]                # what comes first; parents come before their children
+                while True:
+                    nodes = [tokens[-1]] + guess
+                    both = torch.tensor([nodes, [-1] + [p + 1 for p in parents[:len(guess)]]], dtype=torch.int32).to(self.device)
+                    try:
+                        logits, tree = m.forward_tree(slot, pos0, both[0], both[1])
+                        break
+                    except PagesFull:
+                        if not guess:
+                            raise
+                        guess = []                           # no page for guesses: the last token alone
+                kept, counts, following = tree.accept(logits, both[0], temperature=temperature)
+                told = torch.cat([counts, following, kept]).tolist()
+                n, path = told[0], told[2:2 + told[0]]
+                m.keep(slot, tree, kept, counts, n)
+                self.pool.advance(rid, n)
+                self.steps += 1
+                new = [nodes[i] for i in path[1:]] + [told[1]]
+                if eos_id is not None and eos_id in new:
+                    del new[new.index(eos_id) + 1:]
+                tokens += new[:end - len(tokens)]
+        finally:
+            if self.pool.has(rid):
+                self.pool.release(rid)
+        return tokens

@@ -128,7 +128,7 @@ class PagedLLaMAModel:
     graph_safe = False     # pages are booked on the host
 
     def __init__(self, model, *, pages: int, page: int = 64, store: str = "act", window: int = 0, first: int = 0, max_positions: int = 0) -> None:
-        from .paged import PagedCache, PagePool
+        from .paged import PagedCache, PagedLayers, PagePool
 
         cfg = model.config
         if model.transformer.wte.weight.dtype != torch.bfloat16:
@@ -140,6 +140,7 @@ class PagedLLaMAModel:
         self.max_positions = int(max_positions) or (0 if window else cfg.block_size)
         self.pages = PagePool(pages, page, self.device, window=self.window, first=self.first)
         self.caches = [PagedCache.empty(pages, page, self.heads, self.size, dtype=self.dtype, store=store, device=self.device) for _ in range(cfg.n_layer)]
+        self.layers = PagedLayers(self.caches)
         self.freq = (1.0 / 10000 ** (torch.arange(0, self.size, 2, dtype=torch.float32) / self.size)).to(self.device)
         self._owner = object()                              # whose slots these are: the model's own, or an engine's
 
@@ -185,23 +186,63 @@ class PagedLLaMAModel:
 
         return self.pages.has_room({(self._owner, slot): most(n) for slot, n in live.items()}, most(tokens), portion)
 
-    def _rotated(self, x: torch.Tensor, ctx) -> torch.Tensor:
-        """Every head of x [T, heads * size] (rows of a wider product) turned by position, pairs of neighbouring entries (lit_llama/model.py:306-323)."""
+    def _rotated(self, x: torch.Tensor, ctx, positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Every head of x [T, heads * size] (rows of a wider product) turned by position, pairs of neighbouring entries (lit_llama/model.py:306-323): the portion's, or
+        those of `positions` (int32 [T])."""
         from . import _seqlib as S
 
         T, n = x.shape
         out = torch.empty((T, self.heads, self.size), dtype=x.dtype, device=x.device)
-        S.check(S.lib().b2l_seq_rope(S.ptr(x), x.stride(0), 0, S.ptr(self.freq), self.size, 1, 0, 1.0, 1.0, S.ptr(ctx.meta), S.ptr(out), n, 0, T, self.heads, self.size, self.size,
-                                     self.size, ctx.act, ctx.stream), "b2l_seq_rope")
+        args = (S.ptr(x), x.stride(0), 0, S.ptr(self.freq), self.size, 1, 0, 1.0, 1.0)
+        rest = (S.ptr(out), n, 0, T, self.heads, self.size, self.size, self.size, S.act_code(self.dtype), S.stream_ptr())
+        if positions is None:
+            S.check(S.lib().b2l_seq_rope(*args, S.ptr(ctx.meta), *rest), "b2l_seq_rope")
+        else:
+            S.check(S.lib().b2l_seq_rope_at(*args, S.ptr(positions), *rest), "b2l_seq_rope_at")
         return out
+
+    # ------------------------------------------------------------------ several continuations of a sequence
+    @torch.no_grad()
+    def forward_tree(self, slot: int, pos0: int, tokens: torch.Tensor, parents: torch.Tensor):
+        """A slot's next tokens, at position pos0 of its sequence on, as a tree: parents (int32, on the device) as `PagedTree` takes them.  Logits of all of them (in
+        bf16) and the tree; `keep` says afterwards which of them the sequence goes on with."""
+        from .paged import PagedTree
+
+        with self.booked(slot, pos0, tokens.numel()) as step:
+            tree = PagedTree(step, parents, window=self.window, first=self.first)
+            return self._portion(tokens, None, None, step, tree.positions, tree), tree
+
+    def keep(self, slot: int, tree, kept: torch.Tensor, counts: torch.Tensor, n: int) -> None:
+        """Of `forward_tree`'s tokens the n of a path (as `PagedTree.accept` returns it) are the sequence's, in every layer; the others never were."""
+        self.layers.keep(tree.step, kept, counts)
+        self.pages.take_back((self._owner, slot), tree.step.rows - n)
+
+    def reorder_slots(self, sources) -> None:
+        """Every slot of `sources` (slot -> slot) goes on from what its source had before the call: full pages are shared, the others copied in all layers."""
+        self.layers.copy(self.pages.reorder({(self._owner, s): (self._owner, t) for s, t in sources.items()}))
+
+    @torch.no_grad()
+    def forward_together(self, slots, positions, tokens: torch.Tensor) -> torch.Tensor:
+        """One token of each of several slots, at the position that its sequence is at, in one step; f32 logits [slots, vocab]."""
+        ids = [(self._owner, s) for s in slots]
+        for rid, p in zip(ids, positions):
+            if not self.pages.has(rid) or self.pages.position(rid) != p:
+                raise RuntimeError(f"paged LLaMA: slot {rid[1]} is not at position {p}")
+        step = self.pages.step([(rid, 1) for rid in ids])
+        try:
+            return self._portion(tokens, None, None, step, torch.tensor(list(positions), dtype=torch.int32).to(self.device)).float()
+        except BaseException:
+            for rid in ids:
+                self.pages.take_back(rid, 1)
+            raise
 
     @torch.no_grad()
     def forward_portion(self, tokens: torch.Tensor, ctx, want: Optional[torch.Tensor] = None) -> torch.Tensor:
         slot, pos0 = (ctx.slot_hint, ctx.pos_hint) if ctx.slot_hint is not None else ctx.meta.tolist()
         with self.booked(slot, pos0, tokens.numel()) as step:
-            return self._portion(tokens, ctx, want, step)
+            return self._portion(tokens, ctx, want, step).float()
 
-    def _portion(self, tokens: torch.Tensor, ctx, want: Optional[torch.Tensor], step) -> torch.Tensor:
+    def _portion(self, tokens: torch.Tensor, ctx, want: Optional[torch.Tensor], step, positions: Optional[torch.Tensor] = None, tree=None) -> torch.Tensor:
         from . import _lib as L
         from .model import _add
 
@@ -212,15 +253,15 @@ class PagedLLaMAModel:
         L.check(L.lib().b2l_embedding(tokens.data_ptr(), 1, wte.data_ptr(), x.data_ptr(), T, C, wte.shape[0], L.stream_ptr()), "b2l_embedding")
         for block, cache in zip(self.model.transformer.h, self.caches):
             qkv = block.attn.c_attn(block.rms_1(x))[0]
-            cache.write(self._rotated(qkv[:, C:2 * C], ctx), qkv[:, 2 * C:].unflatten(1, (self.heads, self.size)), step)
-            att = cache.attend(self._rotated(qkv[:, :C], ctx), step, window=self.window, first=self.first)
+            cache.write(self._rotated(qkv[:, C:2 * C], ctx, positions), qkv[:, 2 * C:].unflatten(1, (self.heads, self.size)), step)
+            att = cache.attend(self._rotated(qkv[:, :C], ctx, positions), step, window=self.window, first=self.first, tree=tree)
             x = _add(x, block.attn.c_proj(att.view(1, T, C)))
             x = _add(x, block.mlp(block.rms_2(x)))
         if want is not None:
             x = x.index_select(1, want.to(torch.int64))
         if x.shape[1] == 0:
             return torch.empty((0, self.vocab), dtype=torch.float32, device=self.device)
-        return self.model.lm_head(self.model.transformer.ln_f(x))[0].float()
+        return self.model.lm_head(self.model.transformer.ln_f(x))[0]
 
 
 def read_config(model_dir: str) -> dict:
