@@ -214,6 +214,41 @@ def test_pages_that_are_not_there_and_rows_behind_the_last_sequence(new, store):
     assert bool((out[0] == 7.0).all()) and bool((out[new:] == 7.0).all()) and torch.equal(out[1:new], got[1:new])
 
 
+@pytest.mark.parametrize("store", ["fp8", "int8"])
+@pytest.mark.parametrize("new", [6, 70])
+def test_a_tree_among_many_single_tokens(new, store):
+    """Enough of them that the step runs the kernels of few and of many rows side by side (from 8-bit pools)."""
+    from lit_llama_b200 import PagedTree
+
+    sequences = [(1, 2000 + 10 * b) for b in range(60)]
+    sequences[7] = (new, 1200)
+    cache, q, step, seqs = setup(sequences, 64, 8, 32, 32, 32, store, BF)
+    trees = trees_of(seqs, random.Random(6))
+    tree = PagedTree(step, flat(trees))
+    got = cache.attend(q, step, tree=tree)
+    some = [0, 7, 30, 59]                                                   # of the oracle's, some sequences
+    at = [sum(n for n, _ in sequences[:b]) for b in range(61)]
+    rows = [r for b in some for r in range(at[b], at[b + 1])]
+    sets, depths = sights([seqs[b] for b in some], [trees[b] for b in some])
+    want = T.attend(q[rows], cache, [seqs[b] for b in some], sets, depths, 32 ** -0.5)
+    check(got[rows], want, 32, 3000, False, store)
+
+
+def test_rows_of_logits_far_apart():
+    """Rows whose distance passes 32 bits."""
+    from lit_llama_b200 import PagedStep, PagedTree, beam_select
+
+    far = 3 * 2 ** 29
+    big = torch.empty(2 * far + 5000, dtype=BF, device=DEV)
+    x = big.as_strided((3, 5000), (far, 1))
+    x.copy_(torch.randn(3, 5000, device=DEV))
+    tree = PagedTree(PagedStep.of([(1, 1, [0])] * 3, DEV), torch.full((3,), -1, dtype=torch.int32, device=DEV))
+    assert tree.accept(x, torch.zeros(3, dtype=torch.int64, device=DEV))[2].tolist() == T.targets(x)
+    scores = torch.zeros(1, 3, device=DEV)
+    got, want = beam_select(x[None], scores, 12), beam_select(x.contiguous()[None], scores, 12)
+    assert all(torch.equal(a, b) for a, b in zip(got[1:], want[1:]))
+
+
 def test_queries_of_any_stride():
     from lit_llama_b200 import PagedTree
 
