@@ -88,13 +88,13 @@ template <int STORE> constexpr int THREADS = STORE == ACT ? 384 : 640;
 
 // Stages of keys and values, and of 8-bit pools' codes (with both's scales beside the keys'); none: the sizes do not fit.  What comes first is what measured best
 struct Layout { int ks, vs, raw_ks, raw_vs; size_t smem; };
-template <int STORE, bool PAIR> static Layout layout(int K, int V) {
+template <int STORE, bool PAIR, bool TREE = PAIR> static Layout layout(int K, int V) {
   const size_t ka = atoms_of(K, 2), va = atoms_of(V, 2), q = (PAIR ? 1 : 2) * ka * TC_ATOM + (PAIR ? 2048 : 0), room = 227 * 1024;
   constexpr int N = 5;
   const Layout whole[N] = {{2, 2, 1, 1}, {2, 1, 1, 1}, {1, 1, 1, 1}}, pair8[N] = {{2, 2, 2, 2}, {2, 1, 2, 2}, {1, 1, 2, 2}, {2, 1, 1, 1}, {1, 1, 1, 1}}, pair16[N] = {{3, 3, 1, 1}, {3, 2, 1, 1}, {2, 2, 1, 1}, {2, 1, 1, 1}, {1, 1, 1, 1}};
   Layout l{};
   for (int i = 0; i < N && !l.ks; ++i) {
-    Layout s = !PAIR ? whole[i] : STORE == ACT ? pair16[i] : pair8[i];
+    Layout s = STORE != ACT ? (PAIR ? pair8[i] : whole[i]) : TREE ? pair16[i] : whole[i];
     s.smem = CONTROL_BYTES + INFO_BYTES<STORE> + q + (s.ks * ka + s.vs * va) * TC_ATOM + (STORE == ACT ? 0 : KEYS * (s.raw_ks * K + s.raw_vs * V) + s.raw_ks * sizeof(Scales));
     if (s.ks && s.smem <= room) l = s;
   }
@@ -1101,7 +1101,7 @@ static int map_rows(CUtensorMap* m, const void* base, long long rows, int cols, 
 }
 
 template <int STORE, class A> static int go(const A& a, int ctas, cudaStream_t stream) {
-  const Layout l = layout<STORE, A::PAIR>(a.K, a.V);
+  const Layout l = layout<STORE, A::PAIR, A::TREE>(a.K, a.V);
   CUtensorMap mk, mv;
   const long long rows = ((long long)a.s.pages * a.kv_heads) << a.s.shift;
   const int box = 1 << a.s.shift < KEYS ? 1 << a.s.shift : KEYS;
