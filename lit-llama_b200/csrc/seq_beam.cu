@@ -11,7 +11,9 @@
 //
 // A beam whose score or log-probabilities are no numbers (a score of -inf, a logit that is NaN or +inf, none above -inf) is out: its values are -inf.
 //
-// What bounds it: the logits read once; few beams: two launches.
+// What bounds it: for many rows the latency of a block's steps (bound, sums, what reaches the bound, ranks) with four blocks on an SM, and an exponential for every logit: 48 x 8
+// beams of 100003 bf16, 16 of each group: 27 us for the parts, 2.8 TB/s, and 11 us for the second launch.  Few beams: the two launches, 4 of 32000 in 4.5 and 6.9 us.
+// (Parts of 8192 entries 32 us; keys of 64 bits compared throughout 94; blocks that stay and load the next part ahead 40, as fewer have room.)
 #include <algorithm>
 
 #include "seq_rows.cuh"

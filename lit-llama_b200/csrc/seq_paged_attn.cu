@@ -24,6 +24,9 @@
 // sequences over up to 8192 keys of 8 heads, e4m3: 123 us, 4.3 TB/s, where the issue of instructions is busy for half of the cycles and their latency is the
 // other half (12 warps on an SM, as many as the copies in flight leave room for).  One token over 1031 keys: 12 us, two launches of a chain of loads each.
 // 16 rows of f32 are bound by their six products: 461 tokens over a window of 512, 8 / 2 heads of 128, 73 us.
+//
+// Trees of drafted tokens (TREE): what a row sees of the step's new tokens are the bits of its mask, 32 keys at a time; the context's units need none.  Eight tokens over 1031 keys
+// of 32 heads: 14.4 us; five trees of up to 21 tokens, f32, a window of 512, 8 / 2 heads: 21 us.
 #include <algorithm>
 #include <cmath>
 

@@ -32,6 +32,12 @@
 // which its next product waits for.  8-bit 645 us (e4m3; int8 690): a row tile waits for its values' codes as well (f16 twice in shared memory do not fit), and queries, keys,
 // values and codes keep shared memory's 128 bytes a cycle busy for some 2700 of a tile's 5600 cycles.  (8 warps for keys and values together: 731; with keys a
 // tile ahead 787.)
+//
+// Trees of drafted tokens (TREE) read all of the context for few rows, so what bounds them is the keys on their way: a warp each copies keys and values, three stages of keys
+// where they fit, and up to 128 packed rows take row tiles of one half that both halves' warps compute (PAIR, below).  64 tokens each of two sequences of 65536, 32 / 8 heads of
+// 128, bf16: 144 us, 950 TFLOP/s and 3.7 TB/s (171 with one warp for both, two stages and parts joined one after the other).  37 trees of 32 tokens over 4096 keys: bf16
+// 118 us, 5.4 TB/s (131 in whole row tiles), e4m3 149 us, 2.2 TB/s (206): there each tile's values are turned into f16 in 2200 cycles and multiplied in 1100 before the next
+// one's can be, as two stages of f16 values do not fit beside two stages of codes.
 #include <algorithm>
 #include <utility>
 
@@ -86,7 +92,8 @@ template <int STORE> constexpr size_t INFO_BYTES = STORE == ACT ? 1024 : (MOST_N
 static_assert(sizeof(Control) <= CONTROL_BYTES && sizeof(Info) % 16 == 0 && sizeof(Scales) == 1024);
 template <int STORE> constexpr int THREADS = STORE == ACT ? 384 : 640;
 
-// Stages of keys and values, and of 8-bit pools' codes (with both's scales beside the keys'); none: the sizes do not fit.  What comes first is what measured best
+// Stages of keys and values, and of 8-bit pools' codes (with both's scales beside the keys'); none: the sizes do not fit.  The first that fits is taken: PAIR with codes in two
+// stages before values in two, as a tile of codes comes some 1200 cycles after it is asked for
 struct Layout { int ks, vs, raw_ks, raw_vs; size_t smem; };
 template <int STORE, bool PAIR, bool TREE = PAIR> static Layout layout(int K, int V) {
   const size_t ka = atoms_of(K, 2), va = atoms_of(V, 2), q = (PAIR ? 1 : 2) * ka * TC_ATOM + (PAIR ? 2048 : 0), room = 227 * 1024;
@@ -219,8 +226,8 @@ __device__ __forceinline__ uint32_t piece_at(int r, int c) { return (uint32_t)((
 
 // This thread's 16-byte pieces of a tile's codes (rows of D bytes) as f16 into its rows, code times its row's factor (in two parts) rounded once: every `threads`-th
 // piece.  HIDE: a factor of 0 hides whatever the codes are
-// UNROLL: 2; PAIR 1, with one place in the code for keys and values (37 trees of 32 tokens over 4096 keys, e4m3: 153 us so, 173 with 2 and two places, 167 with 4 pieces'
-// loads ahead)
+// UNROLL: 2; PAIR 1, with one place in the code for keys and values (37 trees of 32 tokens over 4096 keys, e4m3: 153 us so, 173 with 2 and two places, 167 with the loads of
+// four pieces together; values in two halves of 64 keys 160, twice as many warps of half the registers 170)
 template <int STORE, bool HIDE, int UNROLL> __device__ __forceinline__ void codes_to_f16(uint32_t raw, int D, const uint2* factors, uint32_t base, int me, int threads) {
   const int pieces = D / 16;
   auto one = [&](uint32_t from, uint2 f, uint32_t first, uint32_t second, bool odd) {
@@ -567,7 +574,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
    } else if (warp == 1 || (TREE && warp == 3)) {
     // ===================== tiled copies =====================
     // TREE: keys by warp 1, values by warp 3.  One warp for both asks for the keys of a tile when the place of values before it is free, which is late where nearly all of
-    // the time is that of copies: 37 trees of 32 tokens, bf16, took 125 us so
+    // the time is that of copies: 37 trees of 32 tokens over 4096 keys, bf16, 125 us so, 120 apart
     const bool keys_here = warp == 1, values_here = !TREE || warp == 3;
     const int box = min(1 << a.s.shift, KEYS), boxes = KEYS / box, gone = (a.s.pages * a.kv_heads) << a.s.shift;      // a row beyond the pool: zeros
     int kst = 0, vst = 0;

