@@ -275,10 +275,12 @@ __global__ void __launch_bounds__(THREADS, ENTRIES == 8 ? 8 : sizeof(act_t) == 2
 
 // What bounds it: a chain of loads, logarithms in 64 bits, and code that runs once.  One group of 512 entries 6.9 us, 48 of 896 11.2 us.
 constexpr int HELD = 2048, TIES = 1024;      // entries in shared memory; of those that reach the bound
-__global__ void __launch_bounds__(THREADS) beam_select_kernel(const __grid_constant__ Select a) {
+constexpr int SELECTORS = 512, OCTETS = SELECTORS / 8;      // threads; groups of eight, at least as many as are chosen
+static_assert(OCTETS >= MOST_COUNT);
+__global__ void __launch_bounds__(SELECTORS) beam_select_kernel(const __grid_constant__ Select a) {
   __shared__ double offset[MOST_BEAMS];                      // score less the logarithm of the sum of exp(x - largest); NaN: the beam is out
   __shared__ float largest[MOST_BEAMS];
-  __shared__ __align__(16) unsigned long long firsts[THREADS];
+  __shared__ __align__(16) unsigned long long firsts[OCTETS];
   __shared__ Key list[TIES];
   __shared__ unsigned long long held[HELD];
   __shared__ unsigned long long least_of;
@@ -289,10 +291,10 @@ __global__ void __launch_bounds__(THREADS) beam_select_kernel(const __grid_const
   pdl_wait();
   if (all <= HELD) {
 #pragma unroll 4
-    for (int i = threadIdx.x; i < all; i += THREADS) held[i] = keys[i];
+    for (int i = threadIdx.x; i < all; i += SELECTORS) held[i] = keys[i];
     keys = held;
   }
-  for (int w = warp; w < a.beams; w += THREADS / 32) {       // a warp for a beam
+  for (int w = warp; w < a.beams; w += SELECTORS / 32) {       // a warp for a beam
     const size_t at = ((size_t)group * a.beams + w) * a.splits;
     const float score = a.scores[(size_t)group * a.beams + w];
     float top = -INFINITY, t = -INFINITY;
@@ -337,13 +339,12 @@ __global__ void __launch_bounds__(THREADS) beam_select_kernel(const __grid_const
     a.from[to] = (int)(k.lo / (uint32_t)a.vocab);
     a.tokens[to] = (int)(k.lo % (uint32_t)a.vocab);
   };
-  const int lanes = lanes_of(a.count), groups = THREADS / lanes;
   unsigned long long mine = 0ull, least = 0ull;
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {                     // the largest value of each thread; then what reaches the bound
     if (pass == 0 || mine >= least)
 #pragma unroll 1
-      for (int i = threadIdx.x; i < all; i += THREADS) {
+      for (int i = threadIdx.x; i < all; i += SELECTORS) {
         const Key k = entry(i, keys[i]);
         if (pass == 0) {
           mine = max(mine, k.hi);
@@ -354,17 +355,15 @@ __global__ void __launch_bounds__(THREADS) beam_select_kernel(const __grid_const
       }
     if (pass == 1) break;
     unsigned long long best = mine;
-    if (lanes == 4) {
-      best = max(best, __shfl_xor_sync(0xffffffffu, best, 1));
-      best = max(best, __shfl_xor_sync(0xffffffffu, best, 2));
-    }
-    if (threadIdx.x % lanes == 0) firsts[threadIdx.x / lanes] = best;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+    if (threadIdx.x % 8 == 0) firsts[threadIdx.x / 8] = best;
     __syncthreads();
-    if ((int)threadIdx.x < groups) {
+    if (threadIdx.x < OCTETS) {
       const unsigned long long own = firsts[threadIdx.x];
       int above = 0, reached = 0;
-#pragma unroll 4
-      for (int i = 0; i < groups; i += 2) {
+#pragma unroll 8
+      for (int i = 0; i < OCTETS; i += 2) {
         const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(&firsts[i]);
         above += (y.x > own) + (y.y > own);
         reached += (y.x >= own) + (y.y >= own);
@@ -377,7 +376,7 @@ __global__ void __launch_bounds__(THREADS) beam_select_kernel(const __grid_const
   __syncthreads();
   const int n = found;
   if (n <= TIES) {
-    for (int i = threadIdx.x; i < n; i += THREADS) {
+    for (int i = threadIdx.x; i < n; i += SELECTORS) {
       const Key own = list[i];
       int rank = 0;
 #pragma unroll 4
@@ -390,7 +389,7 @@ __global__ void __launch_bounds__(THREADS) beam_select_kernel(const __grid_const
   Key last{~0ull, 0u};
   for (int r = 0; r < a.count; ++r) {
     Key next{0ull, 0u};
-    for (int i = threadIdx.x; i < all; i += THREADS) {
+    for (int i = threadIdx.x; i < all; i += SELECTORS) {
       const Key k = entry(i, keys[i]);
       if (k.hi && before(last, k) && (next.hi == 0ull || before(k, next))) next = k;
     }
@@ -401,7 +400,7 @@ __global__ void __launch_bounds__(THREADS) beam_select_kernel(const __grid_const
     }
     if (lane == 0) list[warp] = next;
     __syncthreads();
-    for (int w = 0; w < THREADS / 32; ++w)
+    for (int w = 0; w < SELECTORS / 32; ++w)
       if (list[w].hi && (next.hi == 0ull || before(list[w], next))) next = list[w];
     if (threadIdx.x == 0) put(next, r);
     last = next;
@@ -458,7 +457,7 @@ extern "C" int b2l_seq_beam_select(const void* logits, long long ld, const float
     else beam_parts_kernel<act_t, 8><<<dim3(splits, rows), THREADS, 0, st>>>(a);
   });
   B2L_LAUNCH_CHECK("beam_parts_kernel");
-  LaunchCfg launch(dim3((unsigned)groups), dim3(THREADS), 0, st, true);
+  LaunchCfg launch(dim3((unsigned)groups), dim3(SELECTORS), 0, st, true);
   B2L_CUDA(cudaLaunchKernelEx(&launch.cfg, beam_select_kernel, a));
   B2L_LAUNCH_CHECK("beam_select_kernel");
   return 0;

@@ -722,6 +722,14 @@ static long long few_floats(int splits, long long count, int V) { return splits 
 // A window, or a number of first tokens, as long as all that a table holds.  (A position below zero less a longer window need not fit 32 bits.)
 static bool hides_nothing(int window, int first, int width, int page) { return std::max(window, first) >= (long long)width * page; }
 
+// Whether the few-row kernel takes trees whose longest has more than 16 packed rows: as a step's time in both, microseconds measured with heads of 128 and fitted to the tiles of
+// 128 keys of all sequences and heads.  The chunk kernel begins later (its shares, its join) and takes the same for 17 rows as for 128; the few-row one takes every 16 rows by
+// themselves.  8 tokens of 32 / 8 heads over 4096 keys, e4m3: one sequence 23 and 31, four 34 and 40, 37 198 and 147; bf16 22 and 25, 40 and 30, 234 and 113.
+static bool few_for_trees(long long longest, double tiles, int store) {
+  const double few = tiles * (double)((longest + 15) / 16), many = tiles * (double)((longest + 127) / 128);
+  return store == ACT ? 14 + 0.0158 * few < 21 + 0.0098 * many : 19 + 0.0085 * few < 28 + 0.0125 * many;
+}
+
 static Plan plan_of(bool tree, int rows, int seqs, int width, int page, int heads, int kv_heads, int K, int V, int window, int first, int max_new, int max_length, int store,
                     int act_dtype) {
   Plan p{};
@@ -738,7 +746,8 @@ static Plan plan_of(bool tree, int rows, int seqs, int width, int page, int head
   // and 670.  There are at most `singles` of them.  (Heads of 128 in groups of four; other sizes were not measured.)
   long long singles = seqs;
   p.few_max = INT32_MAX;
-  if (act_dtype == B2L_BF16 && longest > 16 && many_takes(K, V, store)) {
+  const bool few_trees = tree && few_for_trees(longest, (double)most * kv_heads * ((keys + 127) / 128), store);
+  if (act_dtype == B2L_BF16 && longest > 16 && many_takes(K, V, store) && !few_trees) {
     // Trees of at most 128 packed rows: row tiles of 128, which both halves of a CTA compute
     p.pair = tree && longest <= 128 && pair_takes(K, V, store);
     p.many_ctas = many_ctas(p.pair, packed, most, kv_heads, keys + (window > 0 ? 256 / G : 0), sms);
@@ -759,7 +768,8 @@ static Plan plan_of(bool tree, int rows, int seqs, int width, int page, int head
     p.few_rows = (max_new > 0 ? (long long)max_new * G <= 8 : G <= 8 && packed <= 8ll * most) ? 8 : 16;
     p.few_tiles = seqs + (int)std::min<long long>(packed / p.few_rows, INT32_MAX - seqs);
     p.few_count = (long long)rows * heads;
-    singles = std::max<long long>(seqs, packed / p.few_rows);
+    // (trees: a tile that is not full is one too; 24 rows over 1000 keys of 32 heads, bf16: 31 us in parts that do not all have room, 21 so)
+    singles = std::max<long long>(seqs, (packed + (tree ? p.few_rows - 1 : 0)) / p.few_rows);
   }
   // An SM has three CTAs at a time (with f32 rows, or heads beyond 128, two or one: then this takes up to three times the parts that fill it, or finds room for parts
   // where there is none; chosen and measured for three).  Few CTAs: as many parts as fill them once, of 128 keys at least (one token over 1031 keys of 32 heads: 15.1 us in 4 parts,

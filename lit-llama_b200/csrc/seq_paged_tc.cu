@@ -267,6 +267,8 @@ template <int STORE, bool HIDE, int UNROLL> __device__ __forceinline__ void code
 // 6000 keys of an e4m3 pool take 209 us so, 217 with 12 or 8, 224 with 24 (and 250 in row tiles that were all cut into as many parts).  No share is below 16: 64
 // tokens over 4096 keys, 41 us, take 55 in shares of 48.
 constexpr int EXTRA = 16, LEAST = 2, SMALLEST_SHARE = 16;      // LEAST: tiles of keys that a cut leaves on either side
+// PAIR, where a tile costs 2: 8 (a tree of 32 tokens over 4096 keys of 8 heads, e4m3: 31 us so, 36 with 16; EXTRA of 8 takes 162 us for 32 uneven sequences, 157 with 16)
+template <bool PAIR> constexpr int LEAST_SHARE = PAIR ? SMALLEST_SHARE / 2 : SMALLEST_SHARE;
 
 struct Cost {
   int all, units, each;                                      // tiles of keys, the same but one at least, cost of each
@@ -390,7 +392,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
       if (r0 > 0) clear_rows(a, 0, r0, 0, a.heads, blockIdx.x * 32 + lane, gridDim.x * 32);
       if (r1 < a.s.rows) clear_rows(a, r1, a.s.rows, 0, a.heads, blockIdx.x * 32 + lane, gridDim.x * 32);
     }
-    const long long share = max((all + gridDim.x - 1) / gridDim.x, (long long)SMALLEST_SHARE);
+    const long long share = max((all + gridDim.x - 1) / gridDim.x, (long long)LEAST_SHARE<PAIR>);
     const long long x0 = blockIdx.x * share;
     if (x0 >= all) {                                         // nothing is left
       if (tid == 0) a.many.last[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -1079,7 +1081,7 @@ template <class A> __global__ void __launch_bounds__(256) paged_join_kernel(cons
 
 int many_ctas(bool pair, long long packed, long long tiles, int kv_heads, long long keys, int sms) {
   const long long row_tiles = (packed / (pair ? TILE : 2 * TILE) + tiles) * kv_heads, cost = row_tiles * (EXTRA + (pair ? 2 : 4) * ((keys + KEYS - 1) / KEYS + 2));
-  return (int)std::max<long long>(1, std::min<long long>(sms, cost / SMALLEST_SHARE));
+  return (int)std::max<long long>(1, std::min<long long>(sms, cost / (pair ? LEAST_SHARE<true> : LEAST_SHARE<false>)));
 }
 long long many_floats(bool pair, int ctas, int V) { return 4ll * ctas + 2ll * ctas * (pair ? TILE : 2 * TILE) * (2 + V); }
 
