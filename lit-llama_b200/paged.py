@@ -384,11 +384,13 @@ class PagedTree:
         size = self._works.get(vocab)
         if size is None:
             size = self._works[vocab] = S.lib().b2l_seq_tree_accept_work(rows, vocab)
-        starts = s._tensors[0]
-        kept, counts, following = starts.new_empty(rows) if s.seqs else starts.new_full((rows,), -1), starts.new_empty(s.seqs), starts.new_empty(s.seqs)
-        work = starts.new_empty(-(-size // 4))
+        starts, seqs = s._tensors[0], s.seqs
+        whole = -(-size // 4)                                               # one allocation for all, the work space first: it is aligned
+        work, kept, counts, following = starts.new_empty(whole + rows + 2 * seqs).split_with_sizes([whole, rows, seqs, seqs])
+        if not seqs:
+            kept.fill_(-1)
         _launch(self.device, "b2l_seq_tree_accept", logits.data_ptr(), ld, at, ldn, float(temperature), self.parents.data_ptr(), starts.data_ptr(), tokens.data_ptr(), int(wide),
-                kept.data_ptr(), counts.data_ptr(), following.data_ptr(), work.data_ptr(), size, rows, s.seqs, vocab, S.act_code(logits.dtype))
+                kept.data_ptr(), counts.data_ptr(), following.data_ptr(), work.data_ptr(), size, rows, seqs, vocab, S.act_code(logits.dtype))
         return kept, counts, following
 
 

@@ -36,9 +36,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int) -> Tuple
     if not scores.is_contiguous():
         scores = scores.contiguous()
     size = _work(groups, beams, vocab, count, logits.dtype, device.index)
-    values = scores.new_empty((groups, count))
-    of, tokens = scores.new_empty((groups, count), dtype=torch.int32), scores.new_empty((groups, count), dtype=torch.int32)
-    work = scores.new_empty(-(-size // 4))
+    values, of, tokens = scores.new_empty((3, groups, count), dtype=torch.int32).unbind(0)
+    values, work = values.view(torch.float32), scores.new_empty(-(-size // 4))
     _launch(device, "b2l_seq_beam_select", logits.data_ptr(), ld, scores.data_ptr(), values.data_ptr(), of.data_ptr(), tokens.data_ptr(), work.data_ptr(), size, groups, beams, vocab, count,
             S.act_code(logits.dtype))
     return values, of, tokens

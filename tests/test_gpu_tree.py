@@ -105,6 +105,107 @@ def test_attention_over_context_and_ancestors(case, store, dtype):
     check(cache.attend(q, step, tree=tree), want, dim, max(m for _, m in sequences), dtype == F32, store)
 
 
+def steered(seqs, group, form):
+    """The same step with hints that make the call take one of its forms: few rows at a time, row tiles of 128 rows, of 256.  (A wide table: many keys, as far as the host knows.)"""
+    from lit_llama_b200 import PagedStep
+
+    step = PagedStep.of(seqs, DEV, width=8192)
+    new = {"few": max(16 // group, 1), "pair": max(128 // group, 1), "many": 4096}[form]
+    return PagedStep(step.starts, step.lengths, step.table, rows=step.rows, max_new=new)
+
+
+@pytest.mark.parametrize("store", ["act", "fp8", "int8"])
+@pytest.mark.parametrize("form", ["few", "pair", "many"])
+@pytest.mark.parametrize("case", range(len(CASES) - 1))
+def test_every_form_is_right(case, form, store):
+    """Whatever the hints say: trees of more rows than a form is chosen for, and of fewer."""
+    from lit_llama_b200 import PagedTree
+
+    sequences, page, kv, heads, dim, vdim = CASES[case]
+    cache, q, _, seqs = setup(sequences, page, kv, heads, dim, vdim, store, BF, seed=case)
+    step = steered(seqs, heads // kv, form)
+    trees = trees_of(seqs, random.Random(case))
+    tree = PagedTree(step, flat(trees), nodes=max(n for n, _ in sequences))
+    sets, depths = sights(seqs, trees)
+    check(cache.attend(q, step, tree=tree), T.attend(q, cache, seqs, sets, depths, dim ** -0.5), dim, max(m for _, m in sequences), False, store)
+
+
+@pytest.mark.parametrize("store", ["act", "fp8", "int8"])
+@pytest.mark.parametrize("form", ["pair", "many"])
+@pytest.mark.parametrize("dim,vdim,page", [(16, 16, 16), (192, 128, 64), (176, 112, 32), (48, 128, 128), (96, 16, 256), (32, 80, 16)])
+def test_sizes_of_heads_in_row_tiles(dim, vdim, page, form, store):
+    from lit_llama_b200 import PagedTree
+
+    sequences = [(20, 700), (9, 128), (32, 290), (1, 129), (3, 3)]
+    cache, q, _, seqs = setup(sequences, page, 2, 8, dim, vdim, store, BF, seed=dim)
+    step = steered(seqs, 4, form)
+    trees = trees_of(seqs, random.Random(dim))
+    tree = PagedTree(step, flat(trees), nodes=32)
+    sets, depths = sights(seqs, trees)
+    check(cache.attend(q, step, tree=tree), T.attend(q, cache, seqs, sets, depths, dim ** -0.5), dim, 700, False, store)
+
+
+@pytest.mark.parametrize("store", ["act", "fp8"])
+@pytest.mark.parametrize("form", ["pair", "many"])
+@pytest.mark.parametrize("keys", [1, 100, 128, 129, 256, 257, 384, 640])
+def test_one_tile_of_keys_two_and_more(keys, form, store):
+    """Row tiles whose halves have none, one or several tiles of keys."""
+    from lit_llama_b200 import PagedTree
+
+    sequences = [(min(keys, 12), keys), (min(keys, 30), keys), (1, keys)]
+    cache, q, _, seqs = setup(sequences, 64, 1, 4, 64, 64, store, BF, seed=keys)
+    step = steered(seqs, 4, form)
+    trees = trees_of(seqs, random.Random(keys))
+    tree = PagedTree(step, flat(trees), nodes=30)
+    sets, depths = sights(seqs, trees)
+    check(cache.attend(q, step, tree=tree), T.attend(q, cache, seqs, sets, depths, 64 ** -0.5), 64, keys, False, store)
+
+
+@pytest.mark.parametrize("store", ["act", "int8"])
+@pytest.mark.parametrize("form", ["pair", "many"])
+@pytest.mark.parametrize("window,first", [(1, 0), (40, 0), (64, 5), (130, 300), (300, 16)])
+def test_windows_in_row_tiles(window, first, form, store):
+    from lit_llama_b200 import PagedTree
+
+    sequences = [(21, 900), (6, 40), (1, 600), (12, 12), (30, 1000)]
+    cache, q, _, seqs = setup(sequences, 16, 1, 4, 64, 64, store, BF)
+    step = steered(seqs, 4, form)
+    trees = trees_of(seqs, random.Random(window))
+    tree = PagedTree(step, flat(trees), nodes=30, window=window, first=first)
+    sets, depths = sights(seqs, trees, window, first)
+    check(cache.attend(q, step, tree=tree, window=window, first=first), T.attend(q, cache, seqs, sets, depths, 64 ** -0.5, window, first), 64, 1000, False, store)
+
+
+@pytest.mark.parametrize("store", ["act", "fp8", "int8"])
+@pytest.mark.parametrize("form", ["pair", "many"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_bad_rows_and_odd_masks_in_row_tiles(bad, form, store):
+    """Tokens that see nothing or later ones, depths out of range, pages that are not there, and a value that is no number: only rows that see it have it."""
+    from lit_llama_b200 import PagedStep, PagedTree
+
+    sequences = [(25, 25), (28, 400), (5, 80)]
+    cache, q, _, seqs = setup(sequences, 16, 2, 8, 64, 64, store, BF)
+    k, v = cache.read(PagedStep.of([(400, 400, seqs[1][2])], DEV))
+    k[380], v[380] = bad, bad                                              # new token 8 of the second
+    cache.write(k, v, PagedStep.of([(400, 400, seqs[1][2])], DEV))
+    seqs[1] = (28, 400, [-1 if i in (2, 3, 4, 5, 6, 7, 8, 9, 20) else p for i, p in enumerate(seqs[1][2])])
+    step = steered(seqs, 4, form)
+    tree = PagedTree(step, flat(trees_of(seqs, random.Random(1))), nodes=28)
+    rng = random.Random(2)
+    sets = [{i for i in range(32) if rng.random() < 0.3} for _ in range(step.rows)]
+    for r in (0, 3, 24):
+        sets[r] = set()
+    hit = [r for r in range(25, 53) if 8 in sets[r]]
+    spared = [r for r in range(58) if r not in hit]
+    tree.masks.copy_(T.bits(sets, 1))
+    depths = [rng.choice([-3, 0, 1, 4, 1000]) for _ in range(step.rows)]
+    tree.depths.copy_(torch.tensor(depths, dtype=torch.int32))
+    got = cache.attend(q, step, tree=tree, window=300, first=40)
+    assert hit and not torch.isfinite(got[hit]).any() and not got[[0, 3, 24]].any()
+    want = T.attend(q, cache, seqs, [s - {8} if 25 <= r < 53 else s for r, s in enumerate(sets)], depths, 64 ** -0.5, 300, 40)
+    check(got[spared], tuple(x[spared] for x in want), 64, 400, False, store)
+
+
 @pytest.mark.parametrize("store,dtype", [("act", BF), ("int8", BF), ("act", F32)], ids=str)
 @pytest.mark.parametrize("window,first", [(1, 0), (40, 0), (64, 5), (33, 70), (500, 16)])
 @pytest.mark.parametrize("group", [1, 4, 16])
