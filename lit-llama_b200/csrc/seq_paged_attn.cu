@@ -26,7 +26,7 @@
 // 16 rows of f32 are bound by their six products: 461 tokens over a window of 512, 8 / 2 heads of 128, 73 us.
 //
 // Trees of drafted tokens (TREE): what a row sees of the step's new tokens are the bits of its mask, 32 keys at a time; the context's units need none.  Eight tokens over 1031 keys
-// of 32 heads: 14.4 us; five trees of up to 21 tokens, f32, a window of 512, 8 / 2 heads: 21 us.
+// of 32 heads: 14.4 us; five trees of up to 21 tokens, f32, a window of 512, 8 / 2 heads: 22 us.
 #include <algorithm>
 #include <cmath>
 
@@ -80,6 +80,20 @@ template <int PARTS> __device__ __forceinline__ void parts2(float x, float y, ui
   }
   const __nv_bfloat162 r = __floats2bfloat162_rn(x, y);
   p[PARTS - 1] = *reinterpret_cast<const uint32_t*>(&r);
+}
+// the same with every part rounded (truncated where that would make an infinity): the parts of one operand then have either sign, and the three products that are left out
+// and what the tensor core truncates no longer all lower the sum.  A tree's queries, once a CTA: five trees of up to 21 tokens, f32, are off by 6.6e-7 of their norm in 22 us,
+// 8.8e-7 in 21.5 with truncated parts (with the keys', values' and weights' rounded too 5.3e-7 in 23)
+template <int PARTS> __device__ __forceinline__ void rounded2(float x, float y, uint32_t (&p)[PARTS]) {
+  constexpr float MOST = 3.38953138925153547590470800371487866880e38f;      // the largest bf16
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(fabsf(x) <= MOST ? x : hi_of(x), fabsf(y) <= MOST ? y : hi_of(y));
+    const float2 f = __bfloat1622float2(h);
+    p[i] = *reinterpret_cast<const uint32_t*>(&h);
+    x -= f.x;
+    y -= f.y;
+  }
 }
 // the same in f16, each part rounded
 template <int PARTS> __device__ __forceinline__ void halves2(float x, float y, uint32_t (&p)[PARTS]) {
@@ -269,8 +283,13 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
     float up = 1.f, down;
     if (HALF) lift_of(__uint_as_float(largest[r]), a.scale_log2, up, down);
     uint32_t p[2][QP];
-    operand2<HALF, QP>(x[0] * up, x[1] * up, p[0]);
-    operand2<HALF, QP>(x[2] * up, x[3] * up, p[1]);
+    if constexpr (TREE && F32 && !HALF) {
+      rounded2<QP>(x[0], x[1], p[0]);
+      rounded2<QP>(x[2], x[3], p[1]);
+    } else {
+      operand2<HALF, QP>(x[0] * up, x[1] * up, p[0]);
+      operand2<HALF, QP>(x[2] * up, x[3] * up, p[1]);
+    }
 #pragma unroll
     for (int q = 0; q < QP; ++q) *reinterpret_cast<uint2*>(queries + q * steps * NR * 256 + (threadIdx.x + i * blockDim.x) * 8) = make_uint2(p[0][q], p[1][q]);
   });

@@ -245,7 +245,7 @@ template <int STORE, bool HIDE, int UNROLL> __device__ __forceinline__ void code
     st128(second, make_uint4(y[4], y[5], y[6], y[7]));
   };
   if ((pieces & (pieces - 1)) == 0) {                        // a thread's pieces lie at the same place of every 128th, 64th .. key
-    const int c = me & (pieces - 1), key = me / pieces, step = threads / pieces;
+    const int by = 31 - __clz(pieces), c = me & (pieces - 1), key = me >> by, step = threads >> by;
     const bool odd = (c >> 2) & 1;
     uint32_t from = raw + 16 * me, first = base + piece_at(key, 2 * c + odd), second = base + piece_at(key, 2 * c + 1 - odd);
 #pragma unroll UNROLL

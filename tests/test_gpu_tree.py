@@ -350,6 +350,24 @@ def test_rows_of_logits_far_apart():
     assert all(torch.equal(a, b) for a, b in zip(got[1:], want[1:]))
 
 
+@pytest.mark.parametrize("heads", [2, 8])
+def test_queries_as_large_as_f32_goes(heads):
+    """Rounded to bf16 the largest f32 are infinities: the parts a query is computed in are not.  The keys have few bits and are as small as their products ask for."""
+    from lit_llama_b200 import PagedStep, PagedTree
+
+    cache, q, step, seqs = setup([(9, 150)], 16, 2, heads, 16, 32, "act", F32)
+    g = torch.Generator().manual_seed(3)
+    k = (torch.randint(2, 8, (150, 2, 16), generator=g) * (torch.randint(0, 2, (150, 2, 16), generator=g) * 2 - 1)).to(F32) * 2.0 ** -128
+    cache.write(k.to(DEV), torch.randn(150, 2, 32, generator=g).to(DEV), PagedStep.of([(150, 150, seqs[0][2])], DEV))
+    most = torch.finfo(F32).max
+    q = ((torch.rand(9, heads, 16, generator=g) * 0.01 + 0.99).clamp(max=1.0) * most * (torch.randint(0, 2, (9, heads, 16), generator=g) * 2 - 1)).to(DEV)
+    q[::2, :, 3] = most
+    trees = trees_of(seqs, random.Random(heads))
+    sets, depths = sights(seqs, trees)
+    want = T.attend(q, cache, seqs, sets, depths, 16 ** -0.5)
+    check(cache.attend(q, step, tree=PagedTree(step, flat(trees))), want, 16, 150, True, "act")
+
+
 def test_queries_of_any_stride():
     from lit_llama_b200 import PagedTree
 
