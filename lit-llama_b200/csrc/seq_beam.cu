@@ -12,7 +12,7 @@
 // A beam whose score or log-probabilities are no numbers (a score of -inf, a logit that is NaN or +inf, none above -inf) is out: its values are -inf.
 //
 // What bounds it: for many rows the latency of a block's steps (bound, sums, what reaches the bound, ranks) with four blocks on an SM, and an exponential for every logit: 48 x 8
-// beams of 100003 bf16, 16 of each group: 27 us for the parts, 2.8 TB/s, and 11 us for the second launch.  Few beams: the two launches, 4 of 32000 in 4.5 and 6.9 us.
+// beams of 100003 bf16, 16 of each group: 27 us for the parts, 2.8 TB/s, and 10 us for the second launch, 32 together.  Few beams: the two launches, 4 of 32000 in 4.5 and 5.9 us.
 // (Parts of 8192 entries 32 us; keys of 64 bits compared throughout 94; blocks that stay and load the next part ahead 40, as fewer have room.)
 #include <algorithm>
 
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(THREADS, ENTRIES == 8 ? 8 : sizeof(act_t) == 2
   for (int i = n + (int)threadIdx.x; i < a.count; i += THREADS) keys[i] = 0ull;
 }
 
-// What bounds it: a chain of loads, logarithms in 64 bits, and code that runs once.  One group of 512 entries 6.9 us, 48 of 896 11.2 us.
+// What bounds it: a chain of loads, logarithms in 64 bits, and code that runs once.  One group of 512 entries 5.9 us, 48 of 896 10.3 us (with 256 threads 6.9 and 11.2).
 constexpr int HELD = 2048, TIES = 1024;      // entries in shared memory; of those that reach the bound
 constexpr int SELECTORS = 512, OCTETS = SELECTORS / 8;      // threads; groups of eight, at least as many as are chosen
 static_assert(OCTETS >= MOST_COUNT);
