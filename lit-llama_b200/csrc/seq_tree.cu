@@ -139,6 +139,25 @@ __global__ void __launch_bounds__(THREADS, 5) tree_targets_kernel(const __grid_c
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (top <= -1e25f) {
+        // Nothing but masks: a logarithm does not reach quotients like these in 64 bits either, so the lowest of the largest logits is the one to look at (of a vocabulary
+        // that is hidden but for a few tokens all would be near the largest: 758 rows of 32000 190 us, 69 so)
+        float most = -INFINITY;
+        int first = -1;
+#pragma unroll 1
+        for (int i = 0; i < ENTRIES; ++i) {
+          const int v = index(i);
+          if (v < 0 || v >= a.vocab) continue;
+          const float q = noise[v], here = ld_act(logits, v);
+          if (!(q > 0.f) || over == INFINITY) exactly(v);
+          else if (q < INFINITY && here > most) {
+            most = here;
+            first = v;
+          }
+        }
+        exactly(first);
+        continue;
+      }
       // Those near the largest, one or two, again in 64 bits: x / T is no larger than its difference and the logarithm together, and a logarithm at most 104, so the
       // largest is off by 2^-21 (208 + |top|) at most and one near it by 2^-21 (|top| + 2 |log q|)
       const float least = top - SLACK * (64.f + 2.f * fabsf(top));

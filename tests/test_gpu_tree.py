@@ -450,6 +450,28 @@ def test_acceptance_of_logits_that_are_no_numbers_and_of_ties():
 
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=str)
+@pytest.mark.parametrize("mask", [float("-inf"), None])
+@pytest.mark.parametrize("temperature", [1.0, 0.5, 1e-39])
+def test_acceptance_of_a_vocabulary_that_is_hidden_but_for_a_few(temperature, mask, dtype):
+    from lit_llama_b200 import PagedStep, PagedTree
+
+    rows, vocab = 9, 20011
+    tree = PagedTree(PagedStep.of([(1, 1, [0])] * rows, DEV), torch.full((rows,), -1, dtype=torch.int32, device=DEV))
+    g = torch.Generator().manual_seed(8)
+    mask = torch.finfo(dtype).min if mask is None else mask
+    x = torch.full((rows, vocab), mask, dtype=dtype)
+    noise = torch.empty(rows, vocab).exponential_(1, generator=g)
+    for r in range(5):                                                     # some few left, the next four rows have none or a curious one
+        at = torch.randint(0, vocab, (r + 1,), generator=g)
+        x[r, at] = torch.randn(r + 1, generator=g).to(dtype)
+    noise[6, :9000], noise[7, 12345] = float("inf"), 0.0
+    x[8] = torch.where(torch.arange(vocab) % 3 == 0, -0.0, x[8].float()).to(dtype)
+    x[8, 3000:] = mask
+    tokens = torch.zeros(rows, dtype=torch.int64, device=DEV)
+    assert tree.accept(x.to(DEV), tokens, temperature=temperature, noise=noise.to(DEV))[2].tolist() == T.targets(x, temperature, noise)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=str)
 def test_logits_and_noise_of_any_stride(dtype):
     from lit_llama_b200 import PagedStep, PagedTree
 
