@@ -144,6 +144,7 @@ class PagePool:
         """Whether one more sequence, of `tokens` tokens, finds its pages whatever the sequences of `live` (request id -> the tokens that it grows to) still
         take.  Other sequences are counted with the pages that they have."""
         held = len({p for rid in live for p in self._pages.get(rid, ()) if p >= 0})
+        held -= sum(rid in self._pages and self._partial(rid) in self._shared for rid in live)      # another takes that page's place
         return len(self._free) + held >= sum(self.most_pages(n, portion) for n in live.values()) + self.most_pages(tokens, portion)
 
     def _give(self, page: int) -> None:
@@ -606,7 +607,8 @@ class PagedLayers:
 
     def keep(self, step: PagedStep, kept: torch.Tensor, counts: torch.Tensor) -> None:
         """Of a step's new tokens those of a path (as `PagedTree.accept` returns them: kept int32 [rows], ascending for every sequence, counts int32 [sequences]) moved
-        together in every layer: behind the tokens that the sequence had before the step.  `PagePool.take_back` gives the other tokens' places back."""
+        together in every layer: behind the tokens that the sequence had before the step.  `PagePool.take_back` gives the other tokens' places back.
+        Between the step and this none of its sequences is forked: their pages are written."""
         kept = _whole("paged layers: kept", kept, torch.int32, self.device, step.rows)
         counts = _whole("paged layers: counts", counts, torch.int32, self.device, step.seqs)
         if step.device != self.device:

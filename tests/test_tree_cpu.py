@@ -123,6 +123,18 @@ def test_only_what_goes_on_being_written_is_copied():
     assert p.free_pages() == 8 and not p._shared
 
 
+def test_room_counts_the_copy_of_a_page_that_others_have_too():
+    p = PagePool(4, 16, CPU)
+    p.step([("a", 32)])
+    p.fork("a", "b")
+    p.take_back("b", 5)                                      # goes on in a page that a keeps
+    assert p.has_room({"b": 32}, 16) and not p.has_room({"b": 32}, 17)
+    p.own("b")
+    assert p.has_room({"b": 32}, 16) and not p.has_room({"b": 32}, 17)
+    p.step([("b", 5), ("new", 16)])
+    assert p.free_pages() == 0
+
+
 def test_a_shared_page_is_not_written():
     p = PagePool(8, 16, CPU)
     p.step([("a", 32)])
