@@ -25,8 +25,8 @@
 // other half (12 warps on an SM, as many as the copies in flight leave room for).  One token over 1031 keys: 12 us, two launches of a chain of loads each.
 // 16 rows of f32 are bound by their six products: 461 tokens over a window of 512, 8 / 2 heads of 128, 73 us.
 //
-// Trees of drafted tokens (TREE): what a row sees of the step's new tokens are the bits of its mask, 32 keys at a time; the context's units need none.  Eight tokens over 1031 keys
-// of 32 heads: 14.4 us; five trees of up to 21 tokens, f32, a window of 512, 8 / 2 heads: 22 us.
+// Trees of drafted tokens (TREE): what a row sees of the step's new tokens are the bits of its mask, 32 keys at a time; the context's units need none.  Parts of the keys whose CTAs have room at once are a cluster, which joins them itself.  Eight tokens over 1031 keys
+// of 32 heads: 12.4 us, one launch; five trees of up to 21 tokens, f32, a window of 512, 8 / 2 heads: 22 us.
 #include <algorithm>
 #include <cmath>
 
@@ -609,6 +609,7 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
   }
   __syncthreads();
   const int quads = a.V / 4;
+  float* mine = so + R * W * ov;                             // a.joined: this CTA's [R] maxima and sums, [R][ov] outputs
   for (int i = threadIdx.x; i < R * quads; i += blockDim.x) {
     const int r = i / quads, d = 4 * (i - r * quads), at = pl.first + r;
     if (at >= pl.n * G) break;
@@ -626,7 +627,10 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
       x[3] = fmaf(f, y.w, x[3]);
     }
     const int row = pl.start + at / G, head = h * G + at % G;
-    if (a.few.splits > 1) {
+    if (TREE && a.joined) {
+      if (d == 0) *reinterpret_cast<float2*>(mine + 2 * r) = make_float2(M, L);
+      *reinterpret_cast<float4*>(mine + 2 * R + r * ov + d) = make_float4(x[0], x[1], x[2], x[3]);
+    } else if (a.few.splits > 1) {
       const long long to = (long long)split * a.few.count + (a.both ? (long long)(pl.b * a.kv_heads + h) * a.few_max + at : (long long)row * a.heads + head);
       if (d == 0) *reinterpret_cast<float2*>(a.few.ml + 2 * to) = make_float2(M, L);
       *reinterpret_cast<float4*>(a.few.o + to * a.V + d) = make_float4(x[0], x[1], x[2], x[3]);
@@ -636,7 +640,34 @@ __global__ void __launch_bounds__(128, NV <= 8 ? (NR == 1 && STORE != ACT ? 4 : 
       if (!finite4(x, inv)) atomicOr(&bad, 1u << r);
     }
   }
-  if (a.few.splits == 1) {
+  if (TREE && a.joined) {                                    // the parts are the CTAs of a cluster: each joins every splits-th row, all of it, as a row is computed again as a whole
+    const uint32_t parts = tc::smem_u32(mine);
+    const int splits = a.few.splits;
+    tc::cluster_sync_all();
+    for (int i = threadIdx.x;; i += blockDim.x) {
+      const int r = split + splits * (i / quads), d = 4 * (i % quads), at = pl.first + r;
+      if (r >= R || at >= pl.n * G) break;
+      float M = -INFINITY, L = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int s = 0; s < splits; ++s) M = fmaxf(M, __uint_as_float(tc::ld_dsmem_u32(parts + 8 * r, s)));
+#pragma unroll 4
+      for (int s = 0; s < splits; ++s) {
+        const float ms = __uint_as_float(tc::ld_dsmem_u32(parts + 8 * r, s)), ls = __uint_as_float(tc::ld_dsmem_u32(parts + 8 * r + 4, s));
+        const uint4 y = tc::ld_dsmem(parts + 8 * R + (r * ov + d) * 4, s);
+        if (ms == -INFINITY && ls == 0.f) continue;          // saw nothing
+        const float f = ms == M ? 1.f : exp2_f(ms - M);
+        L += f * ls;
+        x[0] = fmaf(f, __uint_as_float(y.x), x[0]);
+        x[1] = fmaf(f, __uint_as_float(y.y), x[1]);
+        x[2] = fmaf(f, __uint_as_float(y.z), x[2]);
+        x[3] = fmaf(f, __uint_as_float(y.w), x[3]);
+      }
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      a.store(((size_t)(pl.start + at / G) * a.heads + h * G + at % G) * a.V + d, x, inv);
+      if (!finite4(x, inv)) atomicOr(&bad, 1u << r);
+    }
+    tc::cluster_sync_all();                                  // nobody ends while others read what it has
+  }
+  if (a.few.splits == 1 || (TREE && a.joined)) {
     __syncthreads();
     const uint32_t own = (W == 4 ? 0x11111111u : W == 2 ? 0x55555555u : 0xffffffffu) << warp;      // every W-th row
     if (bad & own) mend_rows<4>(a, pl.b, pl.start, pl.length - pl.n, h, pl.first, bad & own, lane);
@@ -732,8 +763,10 @@ template <bool TREE> __global__ void __launch_bounds__(32 * MERGE_WARPS) paged_m
 struct Plan {
   int few_max, few_rows, few_tiles, few_splits, many_ctas;   // few_tiles: of the few-row kernel, 0 where the chunk kernel takes the step; many_ctas: the other way round
   long long few_count, floats;
+  bool joined;                                               // the few-row kernel's parts by a cluster
   bool pair;                                                 // form of the chunk kernel
 };
+constexpr int MOST_JOINED = 8;                               // CTAs of a cluster that every device has room for
 constexpr long long MOST_WORK = 1ll << 27;                   // floats of partial results
 
 static long long few_floats(int splits, long long count, int V) { return splits > 1 ? (2 * splits * count + 3) / 4 * 4 + splits * count * V : 0; }
@@ -785,7 +818,7 @@ static Plan plan_of(bool tree, int rows, int seqs, int width, int page, int head
   } else {
     // rows of a tile: 8 where a token's heads, or all that the longest of the sequences has, fit
     p.few_rows = (max_new > 0 ? (long long)max_new * G <= 8 : G <= 8 && packed <= 8ll * most) ? 8 : 16;
-    p.few_tiles = seqs + (int)std::min<long long>(packed / p.few_rows, INT32_MAX - seqs);
+    p.few_tiles = seqs + (int)std::min<long long>((packed - 1) / p.few_rows, INT32_MAX - seqs);
     p.few_count = (long long)rows * heads;
     // (trees: a tile that is not full is one too; 24 rows over 1000 keys of 32 heads, bf16: 31 us in parts that do not all have room, 21 so)
     singles = std::max<long long>(seqs, (packed + (tree ? p.few_rows - 1 : 0)) / p.few_rows);
@@ -798,7 +831,11 @@ static Plan plan_of(bool tree, int rows, int seqs, int width, int page, int head
   const bool room = 2 * ctas <= slots;
   const long long want = room ? slots / ctas : (4 * slots + ctas - 1) / ctas;
   p.few_splits = (int)std::max<long long>(1, std::min({want, keys / (room ? 128 : 512), 128ll, MOST_WORK / (p.few_count * (V + 2) + 1)}));
-  p.floats += few_floats(p.few_splits, p.few_count, V);
+  // Trees: by a cluster of the parts' CTAs, where all find room at once (8 tokens of 32 heads over 1000 keys, e4m3: 13.2 us so, 14.9 by a second launch, which is the host's too;
+  // 32 trees of 2 tokens of 32 / 8 heads over 4096 keys, in four parts each: 103 and 84)
+  const long long at_once = (act_dtype == B2L_F32 || K > 128 || V > 128 ? 1 : 3) * (long long)sms;
+  p.joined = tree && room && !p.many_ctas && p.few_splits > 1 && p.few_splits <= MOST_JOINED && ctas * p.few_splits <= at_once;
+  if (!p.joined) p.floats += few_floats(p.few_splits, p.few_count, V);
   return p;
 }
 
@@ -815,7 +852,7 @@ template <typename act_t, int STORE, int NV, int NR, bool TREE> static int few_l
       if (stages >= 2) break;
     }
   B2L_CHECK_SUPPORTED(stages >= 2, "b2l_seq_paged_attention: heads of %d and %d entries do not fit", a.K, a.V);
-  const size_t smem = std::max(queries + W * stages * unit, (size_t)W * 8 * NR * (a.V + 6) * 4);
+  const size_t smem = std::max(queries + W * stages * unit, (size_t)(W + 1) * 8 * NR * (a.V + 6) * 4);
   const CUtensorMapDataType type = ES == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : ES == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   const long long rows = ((long long)a.s.pages * a.kv_heads) << a.s.shift;
   FewMaps maps;
@@ -825,7 +862,14 @@ template <typename act_t, int STORE, int NV, int NR, bool TREE> static int few_l
   static DynSmemCache cache;
   auto kernel = paged_few_kernel<act_t, STORE, NV, NR, TREE>;
   if (int rc = ensure_dyn_smem(kernel, smem, cache)) return rc;
-  kernel<<<dim3((unsigned)tiles, (unsigned)a.kv_heads, (unsigned)a.few.splits), 32 * W, smem, stream>>>(a, maps, stages);
+  const dim3 grid((unsigned)tiles, (unsigned)a.kv_heads, (unsigned)a.few.splits);
+  if (a.joined) {
+    LaunchCfg launch(grid, dim3(32 * W), smem, stream, false, a.few.splits);
+    std::swap(launch.attrs[0].val.clusterDim.x, launch.attrs[0].val.clusterDim.z);
+    B2L_CUDA(cudaLaunchKernelEx(&launch.cfg, kernel, a, maps, stages));
+  } else {
+    kernel<<<grid, 32 * W, smem, stream>>>(a, maps, stages);
+  }
   B2L_LAUNCH_CHECK("paged_few_kernel");
   return 0;
 }
@@ -884,6 +928,7 @@ template <bool TREE> static int attention(const char* who, bool zeros, const pag
     work += many_floats(p.pair, p.many_ctas, V);
   }
   a.few.splits = p.few_splits;
+  a.joined = p.joined;
   a.few.count = p.few_count;
   a.few.ml = work;
   a.few.o = work + (2 * p.few_splits * a.few.count + 3) / 4 * 4;
@@ -894,7 +939,7 @@ template <bool TREE> static int attention(const char* who, bool zeros, const pag
                    : (small ? few_launch<act_t, ST, 8, 2, TREE>(a, p.few_tiles, st) : few_launch<act_t, ST, 16, 2, TREE>(a, p.few_tiles, st)))
   B2L_SEQ_DISPATCH(act_dtype, rc = store == ACT ? GO(ACT) : store == E4M3 ? GO(E4M3) : GO(INT8));
 #undef GO
-  if (rc || p.few_splits == 1) return rc;
+  if (rc || p.few_splits == 1 || p.joined) return rc;
   const int warps = p.few_splits >= 32 ? 8 : p.few_splits >= 16 ? 4 : p.few_splits >= 8 ? 2 : 1, here = MERGE_WARPS / warps;
   LaunchCfg launch(dim3((unsigned)((a.few.count + here - 1) / here)), dim3(32 * MERGE_WARPS), 0, st, true);
   B2L_CUDA(cudaLaunchKernelEx(&launch.cfg, paged_merge_kernel<TREE>, a, warps));

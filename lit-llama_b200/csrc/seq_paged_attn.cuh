@@ -85,6 +85,7 @@ template <bool TREE> struct Attn {
   Parts few;
   Shared many;
   Tree nodes;
+  bool joined;                                               // the few-row kernel's parts are joined by a cluster of CTAs
 
   // position of new token i of a sequence whose n new ones begin at position `base` and row `start`
   __device__ __forceinline__ int position(int start, int base, int n, int i) const {
