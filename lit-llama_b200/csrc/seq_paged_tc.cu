@@ -207,6 +207,26 @@ __device__ __forceinline__ void wait_lead(uint32_t a, uint32_t parity, uint32_t 
   }
   dead = 1u;
 }
+// Three barriers at once, each by a lane of its own; for all lanes
+__device__ __forceinline__ void wait_three(uint32_t a, uint32_t parity, int lane, uint32_t& dead) {
+  if (dead) return;
+  for (long long begin = 0;;) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.lt.s32 q, %3, 3;\n\tsetp.eq.b32 p, 0, 0;\n\t@q mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(a), "r"(parity), "r"(lane)
+        : "memory");
+    if (__all_sync(0xffffffffu, ok)) break;
+    const long long now = clock64();
+    if (begin == 0) begin = now;
+    if (__any_sync(0xffffffffu, now - begin > PATIENCE)) {
+      dead = 1u;
+      break;
+    }
+  }
+  __syncwarp();
+}
 __device__ __forceinline__ void commit_by(uint32_t lead, uint32_t mbar) {
   asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(mbar), "r"(lead) : "memory");
 }
@@ -361,6 +381,7 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
                                                                        int k_stages, int v_stages, int k_codes, int v_codes) {
   constexpr bool HALF = STORE != ACT, TREE = A::TREE, PAIR = A::PAIR;
   constexpr int ROWS = A::ROWS, NOTES = paged::NOTES<PAIR>;
+  constexpr int CONVERTERS = PAIR ? 4 : 128;                 // arrivals of those that convert keys, or values
   const int raw_ks = PAIR ? k_codes : 1, raw_vs = PAIR ? v_codes : 1;
   constexpr float LIFT = HALF ? 6.f : 0.f;                   // weights up to 2^14 in f16
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -446,19 +467,19 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
       mbar_init(bar(ct.o_done[i]), 1);
     }
     mbar_init(bar(ct.gave_up), 1);
-    for (int i = 0; i < NOTES; ++i) mbar_init(bar(ct.info_full[i]), HALF ? 129 : 1);
+    for (int i = 0; i < NOTES; ++i) mbar_init(bar(ct.info_full[i]), HALF ? CONVERTERS + 1 : 1);
     mbar_init(bar(ct.tail), 1);
     mbar_init(bar(ct.ref_full), 128);
     for (int i = 0; i < MOST_STAGES; ++i) {
-      mbar_init(bar(ct.k_full[i]), HALF ? 128 : 1);
-      mbar_init(bar(ct.v_full[i]), HALF ? 128 : 1);
+      mbar_init(bar(ct.k_full[i]), HALF ? CONVERTERS : 1);
+      mbar_init(bar(ct.v_full[i]), HALF ? CONVERTERS : 1);
       mbar_init(bar(ct.k_empty[i]), 1);
       mbar_init(bar(ct.v_empty[i]), 1);
       if (i >= 2) break;
       mbar_init(bar(ct.rk_full[i]), 1);
       mbar_init(bar(ct.rv_full[i]), 1);
-      mbar_init(bar(ct.rk_empty[i]), 128);
-      mbar_init(bar(ct.rv_empty[i]), 128);
+      mbar_init(bar(ct.rk_empty[i]), CONVERTERS);
+      mbar_init(bar(ct.rv_empty[i]), CONVERTERS);
     }
     for (int i = 0; i < 3; ++i) ct.k_ref[i] = ct.v_ref[i] = 0u;
     mbar_init_fence();
@@ -677,15 +698,16 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
       // the factor in two f16, twice each: as precise as 22 bits, or steps of 2^-25 (2^-13 of a factor of 2^-12); NaN where the scale is out of range; 0 for a row of
       // zeros (2^-126) or one never written (0)
       constexpr uint32_t NO = 0x7e007e00u;
-      auto factor = [](float scale, float up, uint32_t which, uint32_t* notes) {
+      auto factor = [](bool valid, float scale, float up, uint32_t which, uint32_t& low) {
         const float s = scale * up;
-        if (scale >= 0.f && scale <= 1.17549435e-38f) return make_uint2(0u, 0u);
-        if (!(s >= 2.44140625e-4f && s <= 128.f)) {
-          if (!(s >= 0.f && s <= 128.f)) return make_uint2(NO, NO);
-          atomicOr(notes, which);
-        }
+        const bool zero = !valid || (scale >= 0.f && scale <= 1.17549435e-38f), good = s >= 0.f && s <= 128.f;
+        if (!zero && good && s < 2.44140625e-4f) low |= which;
         const __half hi = __float2half_rn(s), lo = __float2half_rn(s - __half2float(hi));
-        return make_uint2(__half_as_ushort(hi) * 0x10001u, __half_as_ushort(lo) * 0x10001u);
+        return make_uint2(zero ? 0u : good ? __half_as_ushort(hi) * 0x10001u : NO, zero ? 0u : good ? __half_as_ushort(lo) * 0x10001u : NO);
+      };
+      // PAIR: by a lane of each warp, and waits for three barriers at once (37 trees of 32 tokens over 4096 keys, int8: 154 us so, 157 by all threads and one after the other)
+      auto arrive = [&](uint64_t& b) {
+        if (!PAIR || lane == 0) mbar_arrive(bar(b));
       };
       while (!dead && next(a, ct, warp, lane, x)) {
        const Keys keys = a.keys(x.pl, ROWS);
@@ -711,7 +733,9 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
             if (me == 0) ct.k_ref[ref == 0 ? 2 : ref - 1] = ct.v_ref[ref == 0 ? 2 : ref - 1] = 0u;      // the ones before, which all have read: for the ones after the next
             ref = ref == 2 ? 0 : ref + 1;
           }
-          uint2 k_by = valid ? factor(ks, k_up, 256u, &note.there) : make_uint2(0u, 0u), v_by = valid ? factor(vs, v_up, 512u, &note.there) : make_uint2(0u, 0u);
+          uint32_t low = 0u;
+          uint2 k_by = factor(valid, ks, k_up, 256u, low), v_by = factor(valid, vs, v_up, 512u, low);
+          if (low) atomicOr(&note.there, low);
           if (v_by.x == NO) {                                // a row that sees this key is computed again: its scores say so
             k_by = v_by;
             v_by = make_uint2(0u, 0u);
@@ -724,12 +748,16 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
             note.k_up = k_up;
             note.v_up = v_up;
           }
-          mbar_arrive(bar(ct.info_full[tile % NOTES]));
-        } else {
+          if (PAIR) __syncwarp();
+          arrive(ct.info_full[tile % NOTES]);
+        } else if (!PAIR) {
           wait_warp(bar(ct.rv_full[raw]), raw_ph, dead);
           wait_warp(bar(ct.v_empty[st]), ph, dead);
         }
-        wait_warp(bar(ct.info_full[tile % NOTES]), tile / NOTES & 1u, dead);      // all keys' factors
+        // all keys' factors
+        const uint32_t info_full = bar(ct.info_full[tile % NOTES]), info_ph = tile / NOTES & 1u;
+        if (!PAIR || keys_too) wait_warp(info_full, info_ph, dead);
+        else wait_three(lane == 0 ? info_full : lane == 1 ? bar(ct.rv_full[raw]) : bar(ct.v_empty[st]), lane == 0 ? info_ph : lane == 1 ? raw_ph : ph, lane, dead);
         if (dead) break;
         if constexpr (PAIR) {
           codes_to_f16<STORE, true, 1>(keys_too ? raw_k + raw * KEYS * a.K : raw_v + raw * KEYS * a.V, keys_too ? a.K : a.V, keys_too ? info.k_by : info.v_by,
@@ -738,8 +766,9 @@ __global__ void __launch_bounds__(THREADS<STORE>, 1) paged_many_kernel(const __g
           if (keys_too) codes_to_f16<STORE, false, 2>(raw_k + raw * KEYS * a.K, a.K, info.k_by, sk + st * ka * TC_ATOM, me, 128);
           else codes_to_f16<STORE, true, 2>(raw_v + raw * KEYS * a.V, a.V, info.v_by, sv + st * va * TC_ATOM, me, 128);
         }
-        mbar_arrive(bar(keys_too ? ct.k_full[st] : ct.v_full[st]));
-        mbar_arrive(bar(keys_too ? ct.rk_empty[raw] : ct.rv_empty[raw]));
+        if (PAIR) __syncwarp();
+        arrive(keys_too ? ct.k_full[st] : ct.v_full[st]);
+        arrive(keys_too ? ct.rk_empty[raw] : ct.rv_empty[raw]);
         if (++raw == (keys_too ? raw_ks : raw_vs)) { raw = 0; raw_ph ^= 1u; }
         if (++st == (keys_too ? k_stages : v_stages)) { st = 0; ph ^= 1u; }
        }
