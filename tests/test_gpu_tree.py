@@ -286,18 +286,18 @@ def test_what_a_token_does_not_see_does_not_reach_it(bad, heads, store, dtype):
 
 
 @pytest.mark.parametrize("store,dtype", [("act", BF), ("int8", BF), ("act", F32)], ids=str)
-@pytest.mark.parametrize("parts", [2, 3, 5, 6, 7, 8, 9, 12])
-def test_keys_in_any_number_of_parts(parts, store, dtype):
+@pytest.mark.parametrize("parts,dim,vdim", [(2, 64, 80), (3, 64, 80), (4, 256, 256), (5, 64, 80), (6, 64, 80), (7, 64, 80), (8, 64, 80), (8, 256, 192), (9, 64, 80), (12, 64, 80)])
+def test_keys_in_any_number_of_parts(parts, dim, vdim, store, dtype):
     """Two sequences that have so many parts of 128 keys, and a last part of another size; then a token that some rows see and others do not is NaN."""
     from lit_llama_b200 import PagedStep, PagedTree
 
     sequences = [(5, 128 * parts + 40), (3, 60)]
-    cache, q, step, seqs = setup(sequences, 16, 2, 4, 64, 80, store, dtype)
+    cache, q, step, seqs = setup(sequences, 16, 2, 4, dim, vdim, store, dtype)
     parents = [-1, 0, 0, 1, 2, -1, 0, 1]
     tree = PagedTree(step, torch.tensor(parents, dtype=torch.int32, device=DEV))
     sets, depths = sights(seqs, [parents[:5], parents[5:]])
-    want = T.attend(q, cache, seqs, sets, depths, 64 ** -0.5)
-    check(cache.attend(q, step, tree=tree), want, 64, 128 * parts + 40, dtype == F32, store)
+    want = T.attend(q, cache, seqs, sets, depths, dim ** -0.5)
+    check(cache.attend(q, step, tree=tree), want, dim, 128 * parts + 40, dtype == F32, store)
     again = PagedStep.of([(length, length, pages) for _, length, pages in seqs], DEV)
     k, v = cache.read(again)
     k[sequences[0][1] - 4], v[sequences[0][1] - 4] = float("nan"), float("inf")      # the first tree's token 1
@@ -306,8 +306,8 @@ def test_keys_in_any_number_of_parts(parts, store, dtype):
     hit = [1, 3]
     spared = [r for r in range(8) if r not in hit]
     assert not torch.isfinite(got[hit]).any()
-    hidden = T.attend(q, cache, seqs, [s - {1} if r < 5 else s for r, s in enumerate(sets)], depths, 64 ** -0.5)
-    check(got[spared], tuple(x[spared] for x in hidden), 64, 128 * parts + 40, dtype == F32, store)
+    hidden = T.attend(q, cache, seqs, [s - {1} if r < 5 else s for r, s in enumerate(sets)], depths, dim ** -0.5)
+    check(got[spared], tuple(x[spared] for x in hidden), dim, 128 * parts + 40, dtype == F32, store)
 
 
 @pytest.mark.parametrize("store", ["act", "fp8"])
