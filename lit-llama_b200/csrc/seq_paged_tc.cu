@@ -246,7 +246,7 @@ __device__ __forceinline__ uint32_t piece_at(int r, int c) { return (uint32_t)((
 
 // This thread's 16-byte pieces of a tile's codes (rows of D bytes) as f16 into its rows, code times its row's factor (in two parts) rounded once: every `threads`-th
 // piece.  HIDE: a factor of 0 hides whatever the codes are
-// UNROLL: 2; PAIR 1, with one place in the code for keys and values (37 trees of 32 tokens over 4096 keys, e4m3: 153 us so, 173 with 2 and two places, 167 with the loads of
+// UNROLL: 2; PAIR 1, with one place in the code for keys and values (37 trees of 32 tokens over 4096 keys, e4m3: 153 us so when it was chosen, 142 by now, 173 with 2 and two places, 167 with the loads of
 // four pieces together; values in two halves of 64 keys 160, twice as many warps of half the registers 170)
 template <int STORE, bool HIDE, int UNROLL> __device__ __forceinline__ void codes_to_f16(uint32_t raw, int D, const uint2* factors, uint32_t base, int me, int threads) {
   const int pieces = D / 16;
