@@ -226,9 +226,11 @@ template <int MENDED, bool TREE> __device__ __forceinline__ void mend_few(const 
     for (int e = 0; e < 8; ++e) o[r][e] = 0.f;
   }
   if constexpr (TREE) p_max = base + n_new - 1;
+  int from = p_min - a.window + 1;                           // the first window; of a tree's new tokens the masks decide
+  if constexpr (TREE) from = min(from, base);
   for (int j0 = 0; j0 <= p_max; j0 += 32) {
-    if (a.window && j0 >= a.first && j0 + 31 <= p_min - a.window) {      // on to the first window
-      j0 = ((p_min - a.window + 1) & ~31) - 32;
+    if (a.window && j0 >= a.first && j0 + 31 < from) {       // on to it
+      j0 = (from & ~31) - 32;
       continue;
     }
     const int j = j0 + lane;

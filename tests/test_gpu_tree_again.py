@@ -1,0 +1,44 @@
+"""GPU: rows of trees that are computed again, as a value that they do not see is infinite: what they see is what their masks say, whatever the window."""
+import pytest
+import torch
+
+import tree_oracle as T
+from test_gpu_tree import BF, DEV, F32, check, flat, setup, sights, steered
+
+pytestmark = pytest.mark.gpu
+
+FORMS = [("joined", "act", BF), ("joined", "act", F32), ("joined", "int8", BF), ("few", "act", BF), ("few", "fp8", BF), ("few", "act", F32), ("pair", "act", BF), ("pair", "fp8", BF),
+         ("many", "act", BF), ("many", "int8", BF)]
+
+
+def again(parents, base, form, store, dtype, window, first, own):
+    """The tree `parents` over `base` tokens; its last token, which follows the sequence and nobody else sees, is infinite.  `own`: whether the masks have the window too."""
+    from lit_llama_b200 import PagedStep, PagedTree
+
+    n = len(parents)
+    cache, q, step, seqs = setup([(n, base + n)], 16, 2, 2, 64, 64, store, dtype)
+    whole = PagedStep.of([(base + n, base + n, seqs[0][2])], DEV)
+    k, v = cache.read(whole)
+    v[-1] = float("inf")
+    cache.write(k, v, whole)                                               # 8-bit rows are quantised again: the oracle reads what is there now
+    if form != "joined":
+        step = steered(seqs, 1, form)
+    tree = PagedTree(step, flat([parents]), nodes=n, window=window if own else 0, first=first if own else 0)
+    sets, depths = sights(seqs, [parents], window if own else 0, first if own else 0)
+    got = cache.attend(q, step, tree=tree, window=window, first=first)
+    assert n - 1 in sets[-1] and not any(n - 1 in s for s in sets[:-1]) and not torch.isfinite(got[-1]).any()
+    want = T.attend(q, cache, seqs, sets[:-1] + [set()], depths, 64 ** -0.5, window, first)
+    check(got[:-1], tuple(x[:-1] for x in want), 64, base + n, dtype == F32, store)
+
+
+@pytest.mark.parametrize("form,store,dtype", FORMS, ids=str)
+@pytest.mark.parametrize("window,first", [(16, 0), (1, 0), (40, 70)])
+def test_masks_without_a_window_under_a_window(window, first, form, store, dtype):
+    """A chain of 96: the last of them see 96 new tokens, more than the window has."""
+    again([i - 1 for i in range(96)] + [-1], 200, form, store, dtype, window, first, False)
+
+
+@pytest.mark.parametrize("form,store,dtype", FORMS, ids=str)
+def test_a_first_position_at_a_later_place(form, store, dtype):
+    """A branch of 71 tokens behind a chain of 40: its first ones are at positions below `first`, their keys at places above it."""
+    again([i - 1 for i in range(40)] + [5] + list(range(40, 110)) + [-1], 200, form, store, dtype, 4, 220, True)
