@@ -32,6 +32,7 @@ A token's key and value rows are quantised by themselves, per head: scale = max(
 is a kernel of libb200seq (include/b2l_seq.h); CUDA only, no CPU fallback, no derivatives."""
 import ctypes as C
 from typing import Dict, Hashable, List, Mapping, Optional, Sequence, Tuple, Union
+from weakref import WeakSet
 
 import torch
 
@@ -66,6 +67,8 @@ class PagedStep:
         self.max_new, self.max_length = max(int(max_new), 0), max(int(max_length), 0)
         self._at = (S.ptr(starts), S.ptr(lengths), S.ptr(table), table.stride(0), table.shape[1]) if lengths.is_cuda else None
         self._plans: Dict[tuple, tuple] = {}                                # of attend: what does not change from layer to layer
+        self._known: Optional[Tuple[int, Optional[int]]] = None             # the most new tokens of a sequence, and the version of `starts` that has them
+        self._trees: Optional[WeakSet] = None                               # of `PagedTree`, whose masks are as wide as was needed when they were made
 
     # the kernels have the tensors' addresses: their contents may change, they stay
     starts = property(lambda self: self._tensors[0])
@@ -87,18 +90,36 @@ class PagedStep:
             flat += list(pages) + [-1] * (width - len(pages))
         n = len(lengths)
         both = torch.tensor(starts + lengths + flat, dtype=torch.int32).to(device)
-        return cls(both[:n + 1], both[n + 1:2 * n + 1], both[2 * n + 1:].view(n, width), rows=rows,
+        step = cls(both[:n + 1], both[n + 1:2 * n + 1], both[2 * n + 1:].view(n, width), rows=rows,
                    max_new=max((new for new, _, _ in sequences), default=0), max_length=max(lengths, default=0))
+        step._know(step.max_new)
+        return step
+
+    def _know(self, nodes: int) -> None:
+        starts = self._tensors[0]
+        self._known = (nodes, None if starts.is_inference() else starts._version)
+
+    def _nodes(self) -> int:
+        """No sequence has more new tokens than this, whatever the hints: all rows, unless the step was made from the host and not written over since."""
+        starts = self._tensors[0]
+        if self._known is not None and (starts.is_inference() or starts._version == self._known[1]):
+            return self._known[0]
+        return self.rows
 
     def refill(self, other: "PagedStep") -> None:
         """The other step's sequences in this one's tensors (of the same number of sequences and rows, and at least its width), for a graph that was
         recorded with this one."""
         if other.seqs != self.seqs or other.rows != self.rows or other.table.shape[1] > self.table.shape[1]:
             raise ValueError(f"paged step: {other.seqs} sequences with {other.rows} rows and {other.table.shape[1]} pages do not fit {self.seqs} with {self.rows} and {self.table.shape[1]}")
+        nodes = other._nodes()
+        for tree in self._trees or ():
+            if nodes > 32 * tree.words:
+                raise ValueError(f"paged step: sequences of up to {nodes} new tokens, the masks of a tree have {32 * tree.words}: it needs `nodes` when it is made")
         self.starts.copy_(other.starts, non_blocking=True)
         self.lengths.copy_(other.lengths, non_blocking=True)
         self.table[:, :other.table.shape[1]].copy_(other.table, non_blocking=True)
         self.table[:, other.table.shape[1]:].fill_(-1)
+        self._know(nodes)
 
 
 class PagePool:
@@ -334,20 +355,24 @@ class PagedTree:
 
     `attend(.., tree=tree)` lets a token see what was there before the step, its ancestors and itself: the bits of `masks` (int32 [rows, words], bit i of a row for new
     token i), which may be written over to see others.  `window` and `first`, those of `attend`, hide ancestors out of reach.  `nodes`: the most new tokens that a
-    sequence of the step ever has (by default what the step says of it); tokens from 32 `words` on are not seen.
+    sequence of the step ever has, by default the most that one has now (of a step that was made from tensors, all of its rows, as `max_new` is a hint).
 
-    The step's tensors and `parents` may be overwritten between replays of a graph that was recorded with them; then `update` belongs into the graph too."""
+    The step's tensors and `parents` may be overwritten between replays of a graph that was recorded with them; then `update` belongs into the graph too.  Where a
+    sequence may get more new tokens by that than one has now, `nodes` has to say so: tokens from 32 `words` on are not seen (`PagedStep.refill` refuses them)."""
 
     def __init__(self, step: PagedStep, parents: torch.Tensor, *, nodes: int = 0, window: int = 0, first: int = 0) -> None:
         self.step, self.device = step, step.device
         self.parents = _whole("paged tree: parents", parents, torch.int32, step.device, step.rows)
         if nodes < 0 or window < 0 or first < 0:
             raise ValueError("paged tree: a negative number of tokens, window or number of first tokens")
-        self.words = max(1, -(-(int(nodes) or step.max_new or step.rows) // 32))
+        self.words = max(1, -(-(int(nodes) or step._nodes()) // 32))
         self.window, self.first = min(int(window), 2 ** 30), min(int(first), 2 ** 30)
         make = step.starts.new_empty if step.seqs else step.starts.new_zeros
         self.masks, self.depths, self.positions = make((step.rows, self.words)), make((step.rows,)), make((step.rows,))
         self._works: Dict[int, int] = {}                                    # bytes of work space of `accept`, by the vocabulary
+        if step._trees is None:
+            step._trees = WeakSet()
+        step._trees.add(self)
         self.update()
 
     def update(self) -> None:

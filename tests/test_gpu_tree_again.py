@@ -42,3 +42,16 @@ def test_masks_without_a_window_under_a_window(window, first, form, store, dtype
 def test_a_first_position_at_a_later_place(form, store, dtype):
     """A branch of 71 tokens behind a chain of 40: its first ones are at positions below `first`, their keys at places above it."""
     again([i - 1 for i in range(40)] + [5] + list(range(40, 110)) + [-1], 200, form, store, dtype, 4, 220, True)
+
+
+@pytest.mark.parametrize("hint", [0, 1, 16, 70])
+@pytest.mark.parametrize("store", ["act", "fp8"])
+def test_hints_do_not_hide_tokens(store, hint):
+    """A step of tensors whose longest sequence is not what the host says."""
+    from lit_llama_b200 import PagedStep, PagedTree
+
+    cache, q, step, seqs = setup([(70, 170), (3, 20)], 16, 1, 4, 64, 64, store, BF)
+    step = PagedStep(step.starts, step.lengths, step.table, rows=step.rows, max_new=hint)
+    trees = [[i - 1 for i in range(70)], [-1, 0, 0]]
+    sets, depths = sights(seqs, trees)
+    check(cache.attend(q, step, tree=PagedTree(step, flat(trees))), T.attend(q, cache, seqs, sets, depths, 64 ** -0.5), 64, 170, False, store)
