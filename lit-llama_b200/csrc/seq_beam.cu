@@ -6,8 +6,8 @@
 // the same order, and what is left to the lowest index.  A block holds its part in registers, bf16 as it lies.  Its threads, by fours where few are wanted, have a largest
 // value each; the count-th largest of these is a bound that at least `count` entries reach and few more (18 for 16 of 8192 at random), so these are found without a
 // sort, and ranked by counting.  Where more than a list holds reach it, entries alike, keys take the place of values in the same steps: then they are all in `count`
-// threads' entries.  A second launch, a block for a group of beams, does the same with the beams' parts, by values in 64 bits (scores and logits of different beams
-// may be neighbours: what f32 keeps of a sum of 32000 terms would change their order).
+// threads' entries.  A second launch, a block for a group of beams, does the same with the beams' parts, by values in 64 bits.  Scores and logits of different beams
+// may be neighbours, or alike: where values are closer than what f32 has lost of their sums, these are formed again as whole numbers, which no order of the terms changes.
 //
 // A beam whose score or log-probabilities are no numbers (a score of -inf, a logit that is NaN or +inf, none above -inf) is out: its values are -inf.
 //
@@ -23,7 +23,7 @@ namespace beam {
 
 constexpr int THREADS = 256, MOST_COUNT = 64, MOST_BEAMS = 64, LIST = 4096;
 
-struct Key { unsigned long long hi; uint32_t lo; };          // larger first, then the lowest `lo`
+struct Key { unsigned long long hi; uint32_t lo, beam; };    // larger first, then the lowest `lo`
 __device__ __forceinline__ bool before(const Key& x, const Key& y) { return x.hi > y.hi || (x.hi == y.hi && x.lo < y.lo); }
 // a float or double as an unsigned integer of the same order, never 0 for a number
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -50,6 +50,7 @@ struct Select {
   float* tops;                                               // [rows][splits]; +inf: a logit is NaN or +inf
   float* values;
   int *from, *tokens;
+  int bf16;
 };
 
 // A block's entries as they lie: 16 bytes of a row at a time, -inf where there is none
@@ -126,7 +127,7 @@ __device__ __forceinline__ float2 powers2(float x, float y, float c) {
   return make_float2(exp2_f(e.x), exp2_f(e.y));
 }
 
-// The sum of entries I .. I + N - 1's e^(x + c), in pairs: six roundings at most for 64, where one behind the other would be as many (the rest of the sum is in 64 bits).
+// The sum of entries I .. I + N - 1's e^(x + c), in pairs: five roundings at most for 64, where one behind the other would be as many (the rest of the sum is in 64 bits).
 // Halves one after the other, so that few of them are in registers
 template <int I, int N, typename E> __device__ __forceinline__ float2 powers(const E& x, float c) {
   if constexpr (N == 2) return powers2(x[I], x[I + 1], c);
@@ -208,7 +209,7 @@ __global__ void __launch_bounds__(THREADS, ENTRIES == 8 ? 8 : sizeof(act_t) == 2
   top = larger(larger(larger(tops[0], tops[1]), larger(tops[2], tops[3])), larger(larger(tops[4], tops[5]), larger(tops[6], tops[7])));
   const bool out = !(top > -INFINITY && top < INFINITY);   // no sum; the second launch does not look at the keys of a beam that is out
   const float2 sum = powers<0, ENTRIES>(x, out ? 0.f : -top);
-  double all = sum.x + sum.y;
+  double all = (double)sum.x + (double)sum.y;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
   if (lane == 0) sums[warp] = all;
@@ -277,17 +278,67 @@ __global__ void __launch_bounds__(THREADS, ENTRIES == 8 ? 8 : sizeof(act_t) == 2
 constexpr int HELD = 2048, TIES = 1024;      // entries in shared memory; of those that reach the bound
 constexpr int SELECTORS = 512, OCTETS = SELECTORS / 8;      // threads; groups of eight, at least as many as are chosen
 static_assert(OCTETS >= MOST_COUNT);
+
+// How far a beam's sum may be off in the first launch: a term 2^(d log2 e), d = x - largest, by 3 |d| 2^-24 of itself (the difference, the product and the constant rounded) and
+// 2^-22 for the power of two; weighted with the terms |d| is at most ln 16384 < 9.8 in a part of 16384 entries (an entropy); five roundings of 2^-24 in a thread: less than
+// 39 x 2^-24, and the logarithm by as much, which depends on where in 16 bytes the row begins, too.  So values of different beams that are closer than twice that (and two roundings
+// of either in 64 bits) have no order yet: those beams' sums are formed again, and the selection is repeated.  What was farther apart stays in order when one of two values is
+// put right.
+__device__ __forceinline__ double nearly(double value) { return 80.0 / 16777216.0 + fabs(value) * 0x1p-50; }
+
+// 2^62 e^d as a whole number, d <= 0: d = n ln 2 + r with ln 2 in two parts (W. J. Cody and W. Waite), of which the first times n is exact, and the Taylor series of e^r, |r| < 0.35:
+// its terms from r^14 / 14! on are below 2^-57
+__device__ __forceinline__ unsigned long long whole_exp(double d) {
+  d = fmax(d, -50.0);                                        // e^-44 is half of 2^-62
+  const double y = fma(d, 1.4426950408889634, 0x1.8p52), n = y - 0x1.8p52, r = fma(n, -0x1.9ef35793c7673p-41, fma(n, -0x1.62e42fefa2000p-1, d));
+  constexpr double OVER[14] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320, 1.0 / 362880, 1.0 / 3628800, 1.0 / 39916800, 1.0 / 479001600, 1.0 / 6227020800.0};
+  double p = OVER[13];
+#pragma unroll
+  for (int k = 12; k >= 0; --k) p = fma(p, r, OVER[k]);
+  return __double2ull_rn(p * __hiloint2double((__double2loint(y) + 62 + 1023) << 20, 0));
+}
+// sum_u exp(x_u - top) of a row by the whole block, in whole numbers: the same for the same logits in whatever order; a term is off by 2^-51 of itself and 2^-63.  A row of 100003
+// takes 30 us, one of 32000 10: 48 groups of 8 beams that are all alike 275 us, where the selection takes 36 otherwise (with CUDA's exp, whose branches keep the terms apart, 730)
+template <typename act_t> __device__ __forceinline__ void add_up(const act_t* row, int vocab, float top, unsigned long long (&sum)[2]) {
+  constexpr int ENTRIES = 16;
+  unsigned long long lo = 0ull, hi = 0ull;
+#pragma unroll 1
+  for (int at = rows::border(row); at < vocab; at += SELECTORS * ENTRIES) {
+    float x[ENTRIES];
+    rows::load<act_t, ENTRIES / rows::PER<act_t>>(row, at, vocab, -INFINITY, x);
+#pragma unroll
+    for (int i = 0; i < ENTRIES; ++i) {
+      const unsigned long long t = whole_exp((double)x[i] - (double)top);
+      lo += t & 0xffffffffull;
+      hi += t >> 32;                                         // at most 2^30 for each of 2^30 tokens
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    lo += __shfl_xor_sync(0xffffffffu, lo, o);
+    hi += __shfl_xor_sync(0xffffffffu, hi, o);
+  }
+  if (threadIdx.x % 32 == 0) {
+    atomicAdd(&sum[0], lo);
+    atomicAdd(&sum[1], hi);
+  }
+}
+
 __global__ void __launch_bounds__(SELECTORS) beam_select_kernel(const __grid_constant__ Select a) {
   __shared__ double offset[MOST_BEAMS];                      // score less the logarithm of the sum of exp(x - largest); NaN: the beam is out
   __shared__ float largest[MOST_BEAMS];
   __shared__ __align__(16) unsigned long long firsts[OCTETS];
   __shared__ Key list[TIES];
-  __shared__ unsigned long long held[HELD];
-  __shared__ unsigned long long least_of;
+  __shared__ __align__(16) unsigned long long held[HELD];    // and then what reaches the bound, in order
+  static_assert(HELD * sizeof(unsigned long long) >= TIES * sizeof(Key));
+  __shared__ unsigned long long least_of, doubt, last_place, sum[2];      // beams whose sums are formed again; those with a value near the last that is chosen
   __shared__ int found;
   const int group = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = a.splits * a.count, all = a.beams * per;
   const unsigned long long* keys = a.keys + (size_t)group * all;
-  if (threadIdx.x == 0) found = 0;
+  if (threadIdx.x == 0) {
+    found = 0;
+    doubt = last_place = 0ull;
+  }
   pdl_wait();
   if (all <= HELD) {
 #pragma unroll 4
@@ -329,81 +380,126 @@ __global__ void __launch_bounds__(SELECTORS) beam_select_kernel(const __grid_con
     const double c = offset[w];
     if (c != c) {
       const int r = i - w * per;
-      return r < a.count && r < a.vocab ? Key{ordered(-(double)INFINITY), (uint32_t)w * a.vocab + r} : Key{0ull, 0u};
+      return r < a.count && r < a.vocab ? Key{ordered(-(double)INFINITY), (uint32_t)w * a.vocab + r, (uint32_t)w} : Key{0ull, 0u, 0u};
     }
-    return k ? Key{ordered(c + ((double)unordered((uint32_t)(k >> 32)) - (double)largest[w])), (uint32_t)w * a.vocab + (uint32_t)~k} : Key{0ull, 0u};
+    return k ? Key{ordered(c + ((double)unordered((uint32_t)(k >> 32)) - (double)largest[w])), (uint32_t)w * a.vocab + (uint32_t)~k, (uint32_t)w} : Key{0ull, 0u, 0u};
   };
+  // the lowest and the highest of values (as integers) that are close to one; none to -inf
+  auto below = [](unsigned long long hi) { return unordered(hi) > -(double)INFINITY ? ordered(unordered(hi) - nearly(unordered(hi))) : ~0ull; };
+  auto above = [](unsigned long long hi) { return ordered(unordered(hi) + nearly(unordered(hi))); };
   auto put = [&](const Key& k, int rank) {
     const size_t to = (size_t)group * a.count + rank;
     a.values[to] = (float)unordered(k.hi);
     a.from[to] = (int)(k.lo / (uint32_t)a.vocab);
     a.tokens[to] = (int)(k.lo % (uint32_t)a.vocab);
   };
-  unsigned long long mine = 0ull, least = 0ull;
 #pragma unroll 1
-  for (int pass = 0; pass < 2; ++pass) {                     // the largest value of each thread; then what reaches the bound
-    if (pass == 0 || mine >= least)
+  for (int round = 0;; ++round) {
+    const bool look = round == 0 && a.beams > 1;             // whether values of different beams are too close
+    unsigned long long mine = 0ull, least = 0ull;
 #pragma unroll 1
-      for (int i = threadIdx.x; i < all; i += SELECTORS) {
-        const Key k = entry(i, keys[i]);
-        if (pass == 0) {
-          mine = max(mine, k.hi);
-        } else if (k.hi >= least) {
-          const int to = atomicAdd(&found, 1);
-          if (to < TIES) list[to] = k;
+    for (int pass = 0; pass < 2; ++pass) {                   // the largest value of each thread; then what reaches the bound, or nearly does
+      if (pass == 0 || mine >= least)
+#pragma unroll 1
+        for (int i = threadIdx.x; i < all; i += SELECTORS) {
+          const Key k = entry(i, keys[i]);
+          if (pass == 0) {
+            mine = max(mine, k.hi);
+          } else if (k.hi >= least) {
+            const int to = atomicAdd(&found, 1);
+            if (to < TIES) list[to] = k;
+          }
         }
-      }
-    if (pass == 1) break;
-    unsigned long long best = mine;
+      if (pass == 1) break;
+      unsigned long long best = mine;
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if (threadIdx.x % 8 == 0) firsts[threadIdx.x / 8] = best;
-    __syncthreads();
-    if (threadIdx.x < OCTETS) {
-      const unsigned long long own = firsts[threadIdx.x];
-      int above = 0, reached = 0;
+      for (int o = 1; o < 8; o <<= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+      if (threadIdx.x % 8 == 0) firsts[threadIdx.x / 8] = best;
+      __syncthreads();
+      if (threadIdx.x < OCTETS) {
+        const unsigned long long own = firsts[threadIdx.x];
+        int larger = 0, reached = 0;
 #pragma unroll 8
-      for (int i = 0; i < OCTETS; i += 2) {
-        const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(&firsts[i]);
-        above += (y.x > own) + (y.y > own);
-        reached += (y.x >= own) + (y.y >= own);
+        for (int i = 0; i < OCTETS; i += 2) {
+          const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(&firsts[i]);
+          larger += (y.x > own) + (y.y > own);
+          reached += (y.x >= own) + (y.y >= own);
+        }
+        if (larger < a.count && reached >= a.count) least_of = own;      // the same from all who say it
       }
-      if (above < a.count && reached >= a.count) least_of = own;      // the same from all who say it
+      __syncthreads();
+      least = least_of;                                      // of a number, or 0
+      least = least ? ordered(unordered(least) - nearly(unordered(least))) : 1ull;
     }
     __syncthreads();
-    least = max(least_of, 1ull);
-  }
-  __syncthreads();
-  const int n = found;
-  if (n <= TIES) {
-    for (int i = threadIdx.x; i < n; i += SELECTORS) {
-      const Key own = list[i];
-      int rank = 0;
+    const int n = found;
+    if (n <= TIES) {
+      for (int i = threadIdx.x; i < n; i += SELECTORS) {
+        const Key own = list[i];
+        int rank = 0;
 #pragma unroll 4
-      for (int j = 0; j < n; ++j) rank += before(list[j], own);
-      if (rank < a.count) put(own, rank);
-    }
-    return;
-  }
-  // more values alike than the list holds: one after the other
-  Key last{~0ull, 0u};
-  for (int r = 0; r < a.count; ++r) {
-    Key next{0ull, 0u};
-    for (int i = threadIdx.x; i < all; i += SELECTORS) {
-      const Key k = entry(i, keys[i]);
-      if (k.hi && before(last, k) && (next.hi == 0ull || before(k, next))) next = k;
-    }
+        for (int j = 0; j < n; ++j) rank += before(list[j], own);
+        if (rank < a.count) put(own, rank);
+        if (look) reinterpret_cast<Key*>(held)[rank] = own;
+      }
+      if (!look) return;
+      __syncthreads();
+      const Key* sorted = reinterpret_cast<const Key*>(held);
+      for (int r = threadIdx.x; r < n - 1; r += SELECTORS) {      // of a run of close values each has a neighbour of another beam, or one of its own that has
+        const Key x = sorted[r], y = sorted[r + 1];
+        if (x.beam != y.beam && y.hi >= below(x.hi) && (r + 1 < a.count || y.hi >= below(sorted[a.count - 1].hi))) atomicOr(&doubt, 1ull << x.beam | 1ull << y.beam);
+      }
+      keys = a.keys + (size_t)group * all;
+    } else {
+      // more values alike than the list holds: one after the other
+      Key last{~0ull, 0u, 0u};
+      for (int r = 0; r < a.count; ++r) {
+        Key next{0ull, 0u, 0u};
+        for (int i = threadIdx.x; i < all; i += SELECTORS) {
+          const Key k = entry(i, keys[i]);
+          if (k.hi && before(last, k) && (next.hi == 0ull || before(k, next))) next = k;
+        }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const Key other{__shfl_xor_sync(0xffffffffu, next.hi, o), __shfl_xor_sync(0xffffffffu, next.lo, o)};
-      if (other.hi && (next.hi == 0ull || before(other, next))) next = other;
+        for (int o = 16; o > 0; o >>= 1) {
+          const Key other{__shfl_xor_sync(0xffffffffu, next.hi, o), __shfl_xor_sync(0xffffffffu, next.lo, o), __shfl_xor_sync(0xffffffffu, next.beam, o)};
+          if (other.hi && (next.hi == 0ull || before(other, next))) next = other;
+        }
+        if (lane == 0) list[warp] = next;
+        __syncthreads();
+        for (int w = 0; w < SELECTORS / 32; ++w)
+          if (list[w].hi && (next.hi == 0ull || before(list[w], next))) next = list[w];
+        if (threadIdx.x == 0) {
+          put(next, r);
+          if (look && r > 0 && next.beam != last.beam && next.hi >= below(last.hi)) doubt |= 1ull << next.beam | 1ull << last.beam;
+        }
+        last = next;
+        __syncthreads();
+      }
+      if (look) {                                            // those that are not chosen: near the last one that is
+        const unsigned long long lo = below(last.hi), hi = above(last.hi);
+        unsigned long long beams = 0ull;
+        for (int i = threadIdx.x; i < all; i += SELECTORS) {
+          const Key k = entry(i, keys[i]);
+          if (k.hi >= lo && k.hi <= hi) beams |= 1ull << k.beam;
+        }
+        if (beams) atomicOr(&last_place, beams);
+      }
     }
-    if (lane == 0) list[warp] = next;
+    if (!look) return;
     __syncthreads();
-    for (int w = 0; w < SELECTORS / 32; ++w)
-      if (list[w].hi && (next.hi == 0ull || before(list[w], next))) next = list[w];
-    if (threadIdx.x == 0) put(next, r);
-    last = next;
+    const unsigned long long again = doubt | (last_place & (last_place - 1ull) ? last_place : 0ull);
+    if (!again) return;
+    for (int w = 0; w < a.beams; ++w) {
+      if (!(again >> w & 1ull)) continue;
+      const size_t row = (size_t)group * a.beams + w;
+      if (threadIdx.x == 0) sum[0] = sum[1] = 0ull;
+      __syncthreads();
+      if (a.bf16) add_up(reinterpret_cast<const __nv_bfloat16*>(a.logits) + row * (size_t)a.ld, a.vocab, largest[w], sum);
+      else add_up(reinterpret_cast<const float*>(a.logits) + row * (size_t)a.ld, a.vocab, largest[w], sum);
+      __syncthreads();
+      if (threadIdx.x == 0) offset[w] = (double)a.scores[row] - log((double)sum[1] * 0x1p-30 + (double)sum[0] * 0x1p-62);
+    }
+    if (threadIdx.x == 0) found = 0;
     __syncthreads();
   }
 }
@@ -450,6 +546,7 @@ extern "C" int b2l_seq_beam_select(const void* logits, long long ld, const float
   a.values = values;
   a.from = from;
   a.tokens = tokens;
+  a.bf16 = act_dtype == B2L_BF16;
   const cudaStream_t st = (cudaStream_t)stream;
   const bool large = entries_of(rows, vocab, act_dtype) > 8;
   B2L_SEQ_DISPATCH(act_dtype, {
