@@ -559,7 +559,7 @@ long long b2l_seq_paged_attention_work(int rows, int seqs, int width, int page, 
  *                                 largest of scores[g, w] + x[w, v] - log sum_u exp x[w, u], falling, ties to the lowest w vocab + v: values (f32), from (the beam w)
  *                                 and tokens (v), [groups, count] each.  The order is that before values are rounded to f32.  A beam is out (all its values
  *                                 are -inf) where its score is no finite number, a logit is NaN or +inf, or none is above -inf.  `work` has
- *                                 b2l_seq_beam_work bytes.  At most 64 beams. */
+ *                                 b2l_seq_beam_work bytes.  At most 64 beams, fewer than 2^30 tokens. */
 int b2l_seq_tree_build(const int* parents, const int* starts, const int* lengths, unsigned* masks, int words, int* depths, int* positions, int rows, int seqs, int window,
                        int first, b2l_stream_t stream);
 int b2l_seq_paged_attention_tree(const void* q, long long ldq, long long hsq, const void* k, const void* v, const float* k_scale, const float* v_scale, const int* starts,

@@ -22,6 +22,7 @@ namespace b2l {
 namespace beam {
 
 constexpr int THREADS = 256, MOST_COUNT = 64, MOST_BEAMS = 64, LIST = 4096;
+constexpr int MOST_VOCAB = 1 << 30;                          // places in a row, and behind it as far as a part goes, are 32-bit integers
 
 struct Key { unsigned long long hi; uint32_t lo, beam; };    // larger first, then the lowest `lo`
 __device__ __forceinline__ bool before(const Key& x, const Key& y) { return x.hi > y.hi || (x.hi == y.hi && x.lo < y.lo); }
@@ -520,7 +521,7 @@ static int splits_of(long long rows, int vocab, int act_dtype) {
 using namespace b2l;
 
 extern "C" long long b2l_seq_beam_work(int groups, int beams, int vocab, int count, int act_dtype) {
-  if (groups <= 0 || beams <= 0 || vocab <= 0 || count <= 0) return 0;
+  if (groups <= 0 || beams <= 0 || vocab <= 0 || vocab >= beam::MOST_VOCAB || count <= 0) return 0;
   const long long rows = (long long)groups * beams, parts = rows * beam::splits_of(rows, vocab, act_dtype);
   return parts * (8ll * count + 8 + 4);
 }
@@ -531,8 +532,9 @@ extern "C" int b2l_seq_beam_select(const void* logits, long long ld, const float
   const char* who = "b2l_seq_beam_select";
   B2L_CHECK_ARG(groups >= 0 && beams > 0 && vocab > 0 && count > 0 && ld >= vocab, "%s: bad sizes", who);
   B2L_CHECK_ARG(groups == 0 || (logits && scores && values && from && tokens), "%s: null pointer", who);
-  B2L_CHECK_SUPPORTED(beams <= MOST_BEAMS && count <= MOST_COUNT && (long long)groups * beams < 65536 && (long long)beams * vocab < (1ll << 31),
-                      "%s: %d groups of %d beams over %d tokens, %d of them: at most 65535 rows, %d beams, %d of them", who, groups, beams, vocab, count, MOST_BEAMS, MOST_COUNT);
+  B2L_CHECK_SUPPORTED(beams <= MOST_BEAMS && count <= MOST_COUNT && (long long)groups * beams < 65536 && vocab < MOST_VOCAB && (long long)beams * vocab < (1ll << 31),
+                      "%s: %d groups of %d beams over %d tokens, %d of them: at most 65535 rows, %d beams, %d of them, fewer than %d tokens", who, groups, beams, vocab, count, MOST_BEAMS,
+                      MOST_COUNT, MOST_VOCAB);
   B2L_CHECK_ARG(count <= (long long)beams * vocab, "%s: %d of %lld", who, count, (long long)beams * vocab);
   if (groups == 0) return 0;
   const long long need = b2l_seq_beam_work(groups, beams, vocab, count, act_dtype);

@@ -7,7 +7,7 @@ import torch
 from . import _seqlib as S
 from .paged import ACTS, _launch
 
-MOST = 64
+MOST, MOST_VOCAB = 64, 1 << 30
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -27,8 +27,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int) -> Tuple
     if scores.shape != shape[:2] or scores.dtype != torch.float32 or scores.device != device:
         raise ValueError(f"beam selection: scores {tuple(scores.shape)} {scores.dtype} on {scores.device}: {(groups, beams)} f32 on {device}")
     count = int(count)
-    if not 0 < count <= min(MOST, beams * vocab) or beams > MOST:
-        raise ValueError(f"beam selection: {count} of {beams} beams and {vocab} tokens: at most {MOST} beams and {MOST} of them")
+    if not 0 < count <= min(MOST, beams * vocab) or beams > MOST or vocab >= MOST_VOCAB:
+        raise ValueError(f"beam selection: {count} of {beams} beams and {vocab} tokens: at most {MOST} beams and {MOST} of them, fewer than {MOST_VOCAB} tokens")
     # rows at equal distances, their entries consecutive; strides of a single row, beam or group are whatever torch says
     s0, s1, s2 = logits.stride()
     ld = s1 if beams > 1 else s0 if groups > 1 else vocab
