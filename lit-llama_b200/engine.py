@@ -338,17 +338,27 @@ class Engine:
         return sorted(done, key=lambda x: -x[1])[:beams]
 
     def _reorder(self, ids: List[Hashable], sources: List[int]) -> None:
-        """Sequence i goes on from what sequence sources[i] had; more or fewer of them than there were."""
-        position = self.pool.position(ids[0])
-        while len(ids) < len(sources):
-            ids.append(ids[0][:-1] + (len(ids),))
-            self.pool.acquire(ids[-1])
-            self.pool.reserve(ids[-1], position)
-            self.pool.advance(ids[-1], position)
-        slots = [self.pool.slot(rid) for rid in ids]
-        self.model.reorder_slots({slots[i]: slots[w] for i, w in enumerate(sources)})
-        while len(ids) > len(sources):
-            self.pool.release(ids.pop())
+        """Sequence i of `ids` becomes one that goes on from what sequence sources[i] had; more or fewer of them than there were.  What somebody goes on from stays with the
+        first who does, and what nobody does is given up before anything is copied."""
+        had, position = list(ids), self.pool.position(ids[0])
+        first = {w: i for i, w in reversed(list(enumerate(sources)))}
+        order = {i: had[w] for w, i in first.items()}
+        unused = [rid for w, rid in enumerate(had) if w not in first]
+        others = [i for i in range(len(sources)) if i not in order]
+        for i in others[:len(unused)]:
+            order[i] = unused.pop()
+        for rid in unused[:max(len(had) - len(sources), 0)]:
+            self.pool.release(rid)
+            ids.remove(rid)
+        for i in others:
+            if i not in order:
+                order[i] = next(rid for rid in (had[0][:-1] + (n,) for n in range(len(ids) + 1)) if rid not in ids)
+                ids.append(order[i])
+                self.pool.acquire(order[i])
+                self.pool.reserve(order[i], position)
+                self.pool.advance(order[i], position)
+        ids[:] = [order[i] for i in range(len(sources))]
+        self.model.reorder_slots({self.pool.slot(order[i]): self.pool.slot(had[w]) for i, w in enumerate(sources)})
 
     def _together(self, ids: Sequence[Hashable], tokens: Sequence[int]) -> torch.Tensor:
         """One more token of each sequence; f32 logits [sequences, vocab]."""
