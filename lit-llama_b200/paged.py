@@ -590,7 +590,8 @@ class PagedCache:
         sizes = (heads, self.kv_heads, self.dim, self.vdim, window, first)
         hints = (step.max_new, step.max_length) + self._codes
         work = S.lib().b2l_seq_paged_attention_tree_work if tree else S.lib().b2l_seq_paged_attention_work
-        floats = work(rows, step.seqs, step.table.shape[1], self.page, *sizes, *hints)
+        with torch.cuda.device(self.device if self.device.type == "cuda" else -1):      # its SMs decide how keys are split
+            floats = work(rows, step.seqs, step.table.shape[1], self.page, *sizes, *hints)
         plan = (floats, (rows, step.seqs, self.n_pages, self.page) + sizes + (float(self.dim ** -0.5 if scale is None else scale),) + hints)
         step._plans[(rows, heads, scale, window, first, self._sizes) + ((True,) if tree else ())] = plan
         return plan
