@@ -326,8 +326,8 @@ template <typename act_t> __device__ __forceinline__ void add_up(const act_t* ro
 }
 
 __global__ void __launch_bounds__(SELECTORS) beam_select_kernel(const __grid_constant__ Select a) {
-  __shared__ double offset[MOST_BEAMS];                      // score less the logarithm of the sum of exp(x - largest); NaN: the beam is out
-  __shared__ float largest[MOST_BEAMS];
+  __shared__ double logs[MOST_BEAMS];                        // of the sum of exp(x - largest); NaN: the beam is out
+  __shared__ float largest[MOST_BEAMS], scores[MOST_BEAMS];
   __shared__ __align__(16) unsigned long long firsts[OCTETS];
   __shared__ Key list[TIES];
   __shared__ __align__(16) unsigned long long held[HELD];    // and then what reaches the bound, in order
@@ -368,8 +368,9 @@ __global__ void __launch_bounds__(SELECTORS) beam_select_kernel(const __grid_con
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const bool out = !(top > -INFINITY && top < INFINITY && fabsf(score) < INFINITY);
     if (lane == 0) {
-      offset[w] = out ? NAN : (double)score - log(sum);
+      logs[w] = out ? NAN : log(sum);
       largest[w] = top;
+      scores[w] = score;
     }
   }
   __syncthreads();
@@ -378,12 +379,13 @@ __global__ void __launch_bounds__(SELECTORS) beam_select_kernel(const __grid_con
     int w = (int)((float)i * over);                          // i / per, or one off: fewer than 2^24 entries
     w += (w + 1) * per <= i;
     w -= w * per > i;
-    const double c = offset[w];
+    const double c = logs[w];
     if (c != c) {
       const int r = i - w * per;
       return r < a.count && r < a.vocab ? Key{ordered(-(double)INFINITY), (uint32_t)w * a.vocab + r, (uint32_t)w} : Key{0ull, 0u, 0u};
     }
-    return k ? Key{ordered(c + ((double)unordered((uint32_t)(k >> 32)) - (double)largest[w])), (uint32_t)w * a.vocab + (uint32_t)~k, (uint32_t)w} : Key{0ull, 0u, 0u};
+    // the logarithm last: beams of equal sums whose scores make up for the difference of their logits are alike
+    return k ? Key{ordered((double)scores[w] + ((double)unordered((uint32_t)(k >> 32)) - (double)largest[w]) - c), (uint32_t)w * a.vocab + (uint32_t)~k, (uint32_t)w} : Key{0ull, 0u, 0u};
   };
   // the lowest and the highest of values (as integers) that are close to one; none to -inf
   auto below = [](unsigned long long hi) { return unordered(hi) > -(double)INFINITY ? ordered(unordered(hi) - nearly(unordered(hi))) : ~0ull; };
@@ -498,7 +500,7 @@ __global__ void __launch_bounds__(SELECTORS) beam_select_kernel(const __grid_con
       if (a.bf16) add_up(reinterpret_cast<const __nv_bfloat16*>(a.logits) + row * (size_t)a.ld, a.vocab, largest[w], sum);
       else add_up(reinterpret_cast<const float*>(a.logits) + row * (size_t)a.ld, a.vocab, largest[w], sum);
       __syncthreads();
-      if (threadIdx.x == 0) offset[w] = (double)a.scores[row] - log((double)sum[1] * 0x1p-30 + (double)sum[0] * 0x1p-62);
+      if (threadIdx.x == 0) logs[w] = log((double)sum[1] * 0x1p-30 + (double)sum[0] * 0x1p-62);
     }
     if (threadIdx.x == 0) found = 0;
     __syncthreads();

@@ -74,3 +74,19 @@ def test_what_is_given_repeats_itself():
     assert [int(b) for b in once[1][3]] == T.select(x[3], s[3], 16)[1].tolist()
     for _ in range(20):
         assert all(torch.equal(a, b) for a, b in zip(beam_select(x, s, 16), once))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=str)
+@pytest.mark.parametrize("vocab", [7, 500, 4097, 32000])
+def test_scores_that_make_up_for_logits(vocab, dtype):
+    """The same logits, in eighths, with scores that are eighths too: many tokens of different beams have the same value, which is that of sums without a rounding."""
+    from lit_llama_b200 import beam_select
+
+    g = torch.Generator().manual_seed(vocab)
+    x = (torch.randint(-40, 40, (8, 1, vocab), generator=g) / 8).to(dtype)
+    for _ in range(8):
+        s = -torch.randint(0, 40, (8, 6), generator=g) / 8
+        sums = (s[..., None] + x.float()).flatten(1)                       # exact; a group's beams have one logarithm
+        at = torch.sort(sums, dim=-1, descending=True, stable=True).indices[:, :32]
+        values, beams, tokens = beam_select(x.expand(8, 6, vocab).contiguous().to(DEV), s.to(DEV), min(32, 6 * vocab))
+        assert torch.equal(beams.cpu().long() * vocab + tokens.cpu(), at)
