@@ -160,10 +160,10 @@ __global__ void __launch_bounds__(THREADS, 5) tree_targets_kernel(const __grid_c
       }
       // Those near the largest, one or two, again in 64 bits: x / T is no larger than its difference and the logarithm together, and a logarithm at most 104, so the
       // largest is off by 2^-21 (208 + |top|) at most and one near it by 2^-21 (|top| + 2 |log q|)
-      const float least = top - SLACK * (64.f + 2.f * fabsf(top));
+      const float least = top < INFINITY ? top - SLACK * (64.f + 2.f * fabsf(top)) : INFINITY;
       uint32_t hits = 0u;
 #pragma unroll
-      for (int i = 0; i < ENTRIES; ++i) hits |= fmaf(fabsf(y[i]), SLACK, x[i]) >= least || x[i] == top ? 1u << i : 0u;
+      for (int i = 0; i < ENTRIES; ++i) hits |= fmaf(fabsf(y[i]), SLACK, x[i]) < least ? 0u : 1u << i;      // NaN too: infinities of f32 that 64 bits may not have
       for (; hits; hits &= hits - 1) {
         const int to = atomicAdd(&found, 1), v = index(__ffs(hits) - 1);
         if (to < LIST) list[to] = v;

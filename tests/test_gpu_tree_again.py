@@ -55,3 +55,24 @@ def test_hints_do_not_hide_tokens(store, hint):
     trees = [[i - 1 for i in range(70)], [-1, 0, 0]]
     sets, depths = sights(seqs, trees)
     check(cache.attend(q, step, tree=PagedTree(step, flat(trees))), T.attend(q, cache, seqs, sets, depths, 64 ** -0.5), 64, 170, False, store)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=str)
+@pytest.mark.parametrize("temperature", [1e-39, 2e-38, 1.0])
+def test_drawn_targets_where_quotients_and_noise_are_infinite(temperature, dtype):
+    """Noise of 0 (its token wins, whatever its logit) and of infinity (it never does), at temperatures whose reciprocal f32 does not have."""
+    from lit_llama_b200 import PagedStep, PagedTree
+
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(12, 9000, generator=g).to(dtype)
+    noise = torch.empty(12, 9000).exponential_(generator=g)
+    noise[0, 700], noise[1, 8999], noise[2, 5], noise[2, 8500], noise[3, :] = 0.0, 0.0, 0.0, 0.0, float("inf")
+    x[0, 700], x[1, 8999], x[2, 5], x[2, 8500] = -9.0, 9.0, -1.0, 2.0
+    x[4, :], x[5, ::2], x[6, 77] = 0.0, -0.0, float("-inf")
+    noise[6, 77] = 0.0                                                     # no number: nowhere the largest
+    noise[7, x[7].argmax()] = float("inf")
+    step = PagedStep.of([(1, 1, [0])] * 12, DEV)
+    tree = PagedTree(step, torch.full((12,), -1, dtype=torch.int32, device=DEV))
+    _, _, following = tree.accept(x.to(DEV), torch.zeros(12, dtype=torch.int32, device=DEV), temperature=temperature, noise=noise.to(DEV))
+    want = T.targets(x, temperature, noise)
+    assert following.tolist() == want and want[0] == 700 and want[2] == 5
