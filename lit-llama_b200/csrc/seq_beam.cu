@@ -11,8 +11,9 @@
 //
 // A beam whose score or log-probabilities are no numbers (a score of -inf, a logit that is NaN or +inf, none above -inf) is out: its values are -inf.
 //
-// What bounds it: for many rows the latency of a block's steps (bound, sums, what reaches the bound, ranks) with four blocks on an SM, and an exponential for every logit: 48 x 8
-// beams of 100003 bf16, 16 of each group: 27 us for the parts, 2.8 TB/s, and 10 us for the second launch, 32 together.  Few beams: the two launches, 4 of 32000 in 4.5 and 5.9 us.
+// What bounds it: for many rows the latency of a block's steps (its loads, bound, sums, what reaches the bound, ranks) with four blocks on an SM, and an exponential for every
+// logit: 48 x 8 beams of 100003 bf16, 16 of each group: 29 us for the parts, 2.7 TB/s, and 13 for the second launch by themselves; a call 36 where L2 has the logits, as it has
+// those that a model's last product has just written, 56 where it has not.  Few beams: the two launches, 4 of 32000 in 4.5 and 5.9 us.
 // (Parts of 8192 entries 32 us; keys of 64 bits compared throughout 94; blocks that stay and load the next part ahead 40, as fewer have room.)
 #include <algorithm>
 

@@ -776,7 +776,8 @@ static bool hides_nothing(int window, int first, int width, int page) { return s
 
 // Whether the few-row kernel takes trees whose longest has more than 16 packed rows: as a step's time in both, microseconds measured with heads of 128 and fitted to the tiles of
 // 128 keys of all sequences and heads.  The chunk kernel begins later (its shares, its join) and takes the same for 17 rows as for 128; the few-row one takes every 16 rows by
-// themselves.  8 tokens of 32 / 8 heads over 4096 keys, e4m3: one sequence 23 and 31, four 34 and 40, 37 198 and 147; bf16 22 and 25, 40 and 30, 234 and 113.
+// themselves.  8 tokens of 32 / 8 heads over 4096 keys, e4m3: one sequence 23 and 31, four 34 and 40, 37 198 and 147; bf16 22 and 25, 40 and 30, 234 and 113.  Heads of other
+// sizes, and steps of which one sequence is much longer than the others (all are counted as the longest), were not measured: what is chosen is right there, but may be the slower.
 static bool few_for_trees(long long longest, double tiles, int store) {
   const double few = tiles * (double)((longest + 15) / 16), many = tiles * (double)((longest + 127) / 128);
   return store == ACT ? 14 + 0.0158 * few < 21 + 0.0098 * many : 19 + 0.0085 * few < 28 + 0.0125 * many;

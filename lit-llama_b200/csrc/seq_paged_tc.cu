@@ -35,9 +35,13 @@
 //
 // Trees of drafted tokens (TREE) read all of the context for few rows, so what bounds them is the keys on their way: a warp each copies keys and values, three stages of keys
 // where they fit, and up to 128 packed rows take row tiles of one half that both halves' warps compute (PAIR, below).  64 tokens each of two sequences of 65536, 32 / 8 heads of
-// 128, bf16: 144 us, 950 TFLOP/s and 3.7 TB/s (171 with one warp for both, two stages and parts joined one after the other).  37 trees of 32 tokens over 4096 keys: bf16
-// 118 us, 5.4 TB/s (131 in whole row tiles), e4m3 149 us, 2.2 TB/s (206): there each tile's values are turned into f16 in 2200 cycles and multiplied in 1100 before the next
-// one's can be, as two stages of f16 values do not fit beside two stages of codes.
+// 128, bf16: 144 us at 1965 MHz, 950 TFLOP/s and 3.7 TB/s (171 with one warp for both, two stages and parts joined one after the other); where they follow one another for more
+// than 0.2 s, at the 1450 MHz that 1000 W allow, 173.  37 trees of 32 tokens over 4096 keys: bf16 117 us, 5.3 TB/s (131 in whole row tiles), e4m3 142 us, 2.2 TB/s (206): there
+// each tile's values are turned into f16 in 1850 cycles and multiplied in 1100 before the next one's can be, as two stages of f16 values do not fit beside two stages of codes.
+//
+// Weights meet the values as one bf16 (with codes one f16), as the tensor core takes two operands of one type and a second product for a second part would cost as much as the
+// first.  Trees' outputs in bf16 are off by 1.66e-3 of their norm by their own rounding; so they are by 1.67e-3 to 1.77e-3 (few keys and large weights), 5e-4 to 1.6e-3 from what
+// f32 weights give.  (Few rows have weights of two bf16 parts, seq_paged_attn.cu: 8e-5.)
 #include <algorithm>
 #include <utility>
 
@@ -246,7 +250,7 @@ __device__ __forceinline__ uint32_t piece_at(int r, int c) { return (uint32_t)((
 
 // This thread's 16-byte pieces of a tile's codes (rows of D bytes) as f16 into its rows, code times its row's factor (in two parts) rounded once: every `threads`-th
 // piece.  HIDE: a factor of 0 hides whatever the codes are
-// UNROLL: 2; PAIR 1, with one place in the code for keys and values (37 trees of 32 tokens over 4096 keys, e4m3: 153 us so when it was chosen, 142 by now, 173 with 2 and two places, 167 with the loads of
+// UNROLL: 2; PAIR 1, with one place in the code for keys and values (37 trees of 32 tokens over 4096 keys, e4m3: 153 us so when it was chosen, 142 with what came later, 173 with 2 and two places, 167 with the loads of
 // four pieces together; values in two halves of 64 keys 160, twice as many warps of half the registers 170)
 template <int STORE, bool HIDE, int UNROLL> __device__ __forceinline__ void codes_to_f16(uint32_t raw, int D, const uint2* factors, uint32_t base, int me, int threads) {
   const int pieces = D / 16;

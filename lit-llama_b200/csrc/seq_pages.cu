@@ -4,8 +4,9 @@
 //   keep   row base + kept[i] -> base + i, base the position of a sequence's first new token: the accepted tokens of a tree one behind the other
 //
 // Both move bytes and compute nothing.  What bounds them: HBM, every byte read once and written once: 48 pages of 32 layers of 8 heads of 128, bf16, 805 MB, in 125 us,
-// 6.4 TB/s; a page or two: the launch.  Kept rows lie apart, 128 bytes (and a scale of 4) of a head each: 64 sequences of some five rows in 32 layers of 8 heads of int8, 28 MB,
-// 15 us (as long with blocks that take several layers), one sequence 4.4 us.
+// 6.4 TB/s; a page or two: the launch.  Kept rows lie apart, 128 bytes (and a scale of 4) of a head each: 64 sequences of some five rows in 32 layers of 8 heads of int8, 34 MB,
+// 16 us from HBM, 11 where L2 has them (as long with blocks that take several layers).  A sequence's rows in a layer are 144 pieces there, two blocks of 128 threads, each with the
+// whole chain of lookups.  One sequence 4.4 us by itself.
 #include <algorithm>
 
 #include "seq_paged.cuh"

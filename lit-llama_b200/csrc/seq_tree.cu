@@ -5,8 +5,8 @@
 //   path: the first new token; then, as long as there is one, the first child whose token is its parent's target
 // The second launch joins the parts of the rows and goes down the trees, a block for each sequence.
 //
-// What bounds acceptance: logits (and noise) read once: 758 rows of 32000 f32 logits with noise 37 us, 5.3 TB/s; one tree of 8 tokens: two launches, 4.4 and 5.7 us.  Values are compared in 64 bits, as two logits may be neighbours: a block finds its largest in f32 and
-// computes those that f32 cannot tell from it again.
+// What bounds acceptance: logits (and noise) read once: 758 rows of 32000 f32 logits with noise 38 us for the targets, 5.2 TB/s, a call 40; one tree of 8 tokens: two launches, 4.4
+// and 5.7 us by themselves.  Values are compared in 64 bits, as two logits may be neighbours: a block finds its largest in f32 and computes those that f32 cannot tell from it again.
 #include "seq_paged.cuh"
 #include "seq_rows.cuh"
 

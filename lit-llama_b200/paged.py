@@ -536,7 +536,8 @@ class PagedCache:
         dim^-1/2 unless given.  Returns [rows, heads, vdim] (`out`, contiguous, where given); rows of no sequence, behind the step's last one or before its first,
         are zeros, or as they were in `out`.
 
-        With a `tree` of the step, p is the token's position in it, and of the step's new tokens a row sees those that the tree says, whatever the window."""
+        With a `tree` of the step, p is the token's position in it, and of the step's new tokens a row sees those that the tree says, whatever the window: `window` and
+        `first` hide what was there before the step, and the tree hides ancestors by those that it was made with."""
         q, s0, s1 = self._rows(q, 0, self.dim, step, "queries")
         rows, heads, _ = q.shape
         if tree is not None:
