@@ -90,7 +90,8 @@ class PagedStep:
             flat += list(pages) + [-1] * (width - len(pages))
         n = len(lengths)
         both = torch.tensor(starts + lengths + flat, dtype=torch.int32).to(device)
-        step = cls(both[:n + 1], both[n + 1:2 * n + 1], both[2 * n + 1:].view(n, width), rows=rows,
+        # (.data: `starts` has a version of its own, which tells when it is written over)
+        step = cls(both.data[:n + 1], both[n + 1:2 * n + 1], both[2 * n + 1:].view(n, width), rows=rows,
                    max_new=max((new for new, _, _ in sequences), default=0), max_length=max(lengths, default=0))
         step._know(step.max_new)
         return step

@@ -52,7 +52,14 @@ def test_a_step_that_is_refilled():
 
 
 def test_a_step_that_is_written_over():
-    step = of(32, 32)
+    step, other = of(32, 32), of(32, 32)
+    tree = PagedTree(step, chain(64))
+    for s in (step, other):                                                # longer sequences, other pages: as many new tokens
+        s.lengths.add_(1)
+        s.table.fill_(1)
+        assert PagedTree(s, chain(64)).words == 1
+    step.refill(other)
+    assert step.lengths.tolist() == [38, 38] and tree.words == 1
     step.starts.copy_(torch.tensor([0, 63, 64], dtype=torch.int32))
     assert PagedTree(step, chain(64)).words == 2
     with torch.inference_mode():
